@@ -358,6 +358,62 @@ int im_sample_rows(const uint16_t* logits, int64_t rows, int64_t V, int64_t ld, 
                    int32_t* out, int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream);
 int im_philox4x32_10(uint64_t seed, uint64_t offset, uint32_t stream_id, uint32_t n, uint32_t* out, void* stream);
 
+/* ---- mixture-of-experts blocks over 4-bit experts ----------------------------------------------------------
+ *
+ * No counterpart in the reference, whose models are dense. A row m has top_k places j; pair p = m * top_k + j.
+ *
+ * im_moe_route: logits [M, E] (bf16, or float32 with logits_f32; row stride ld elements) -> per row the top_k experts
+ * with the largest keys float32(logit) + bias[e] (bias float32 [E] or NULL; -0 counts as +0, ties to the lower expert),
+ * in that order: ids [M, top_k] and weights [M, top_k]. A logit of -inf or NaN closes the expert to the row; places
+ * beyond the open experts get id -1 and weight 0. Weights come from the unbiased logits, times `scale`:
+ *   IM_MOE_SOFTMAX: exp(v - max) / sum, over the chosen experts (normalise) or over all open ones;
+ *   IM_MOE_SIGMOID: 1 / (1 + exp(-v)), divided by the chosen experts' sum (normalise) or as it is.
+ * pairs [M * top_k] holds the pairs sorted by expert (ascending within one; places without an expert last),
+ * offsets [E + 2] where each expert's begin (offsets[E]: the places without one, offsets[E + 1] = M * top_k). `plan`
+ * (16-byte aligned, im_moe_plan_bytes(M, E, top_k) bytes, nothing to initialise) holds the work items of the products.
+ * E <= 512, top_k <= min(E, 32).
+ *
+ * im_moe_pack_w4g64: E matrices w [E, N, K/8], scales and biases [E, N, K/64] -> packed units, expert after expert
+ * (im_moe_packed_bytes(E, N, K) bytes, 16-byte aligned): im_qgemm_pack_w4g64 of each.
+ *
+ * im_moe_grouped_qgemm: y[p] = W[id(p)] x[p / top_k] (x [M, K]), or x[p] with x_by_pair (x [M, top_k, K]); y bf16
+ * [M, top_k, N], zero for places without an expert. pairs and plan come from im_moe_route with the same M, E, top_k.
+ *
+ * im_moe_mlp: y[p] = D[e] (act(G[e] x) * (U[e] x)), e = id(p), x = x[p / top_k]; act IM_EPI_SWIGLU or IM_EPI_GEGLU.
+ * gate_up is packed from [E, 2 I, H] with gate and up rows interleaved in 16-row blocks, down from [E, H, I]; y
+ * [M, top_k, H]. The gated activations are rounded to bf16 once, in the workspace (256-byte aligned, nothing to
+ * initialise, im_moe_mlp_workspace_bytes bytes).
+ *
+ * Sums are float32. A pair's result does not depend on the other rows.
+ *
+ * im_block_residual: joins the places of a block, and the block to the residual stream, and takes the next norm:
+ *   b = sum_j weights[m, j] y[m, j] (places of weight 0 are not read; weights NULL: the one place as it is)
+ *   b = b / sqrt(mean(b^2) + eps) * w'            with post_norm (w' = w, or 1 + w with gemma)
+ *   h_out = bf16(residual_scale * h + gate * b)   (gate bf16: gate[m * gate_row_stride + i * gate_col_stride], or NULL)
+ *   z = bf16(v / sqrt(mean(v^2) + eps) * w')      with next_norm; v = h_out before its rounding
+ * y bf16 [M, places, H], h, h_out (may be h), z bf16 [M, H]; out_sq [M] (or NULL) = sums of squares of the rounded
+ * h_out rows, what im_qgemm_packed's RMSNorm prologue takes. H <= 16384, places <= 32.
+ */
+enum { IM_MOE_SOFTMAX = 0, IM_MOE_SIGMOID = 1 };
+size_t im_moe_plan_bytes(int64_t M, int64_t E, int64_t top_k);
+int im_moe_route(const void* logits, int logits_f32, int64_t M, int64_t E, int64_t ld, const float* bias,
+                 int64_t top_k, int scoring, int normalise, float scale, int32_t* ids, float* weights,
+                 int32_t* offsets, int32_t* pairs, void* plan, size_t plan_bytes, void* stream);
+size_t im_moe_packed_bytes(int64_t E, int64_t N, int64_t K);
+int im_moe_pack_w4g64(const uint32_t* w, const uint16_t* scales, const uint16_t* biases, int64_t E, int64_t N,
+                      int64_t K, void* packed, void* stream);
+int im_moe_grouped_qgemm(const void* packed, const uint16_t* x, uint16_t* y, int64_t M, int64_t E, int64_t top_k,
+                         int64_t N, int64_t K, int x_by_pair, const int32_t* pairs, const void* plan,
+                         size_t plan_bytes, void* stream);
+size_t im_moe_mlp_workspace_bytes(int64_t M, int64_t E, int64_t top_k, int64_t H, int64_t I);
+int im_moe_mlp(const void* gate_up, const void* down, const uint16_t* x, uint16_t* y, int64_t M, int64_t E,
+               int64_t top_k, int64_t H, int64_t I, int activation, const int32_t* pairs, const void* plan,
+               size_t plan_bytes, void* workspace, size_t workspace_bytes, void* stream);
+int im_block_residual(const uint16_t* y, const float* weights, int64_t places, const uint16_t* h,
+                      const uint16_t* post_norm, const uint16_t* gate, int64_t gate_row_stride,
+                      int64_t gate_col_stride, float residual_scale, const uint16_t* next_norm, float eps, int gemma,
+                      int64_t M, int64_t H, uint16_t* h_out, uint16_t* z, float* out_sq, void* stream);
+
 /* ---- GGUF k-quant matmul (the ggml path) ------------------------------------------------------------------
  *
  * y[B][N] = x[B][K] . W^T for W in llama.cpp's GGUF blocks of 256 weights: type 12 = Q4_K (144-byte blocks, W 16-byte

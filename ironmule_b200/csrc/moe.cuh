@@ -1,0 +1,53 @@
+// Shared by the mixture-of-experts kernels: the routing plan that im_moe_route writes and the products read.
+#pragma once
+
+#include <cstddef>
+#include <cstdint>
+
+#include <cuda_runtime.h>
+
+namespace im {
+
+constexpr int MOE_MAX_EXPERTS = 512;
+constexpr int MOE_MAX_TOP_K = 32;
+constexpr int64_t MOE_MAX_ROWS = 1 << 22;
+constexpr int MOE_ROUTE_BLOCKS = 148;   // blocks of the routing kernels at most (one per SM)
+constexpr int MOE_ROUTE_ROWS = 64;      // rows that one block alone routes
+constexpr int MOE_PLAN_HEADER = 8;      // ints: [0] work items, [1] error word of the bounded waits
+
+// One work item: `rows` consecutive entries of the sorted pair list, all of one expert (or, with expert == E, of the
+// places that chose no expert, whose outputs are zero).
+struct MoeItem {
+  int expert, first, rows, pad;
+};
+
+// Plan layout in ints: header | items | per-block expert counts (the routing's own scratch).
+struct MoePlan {
+  int64_t item_rows;   // most rows of an item; 8, 16, 32: the warp-MMA kernel
+  int64_t max_items;   // bound on the items of any routing of these sizes
+  int64_t blocks, rows_per_block;
+  int64_t counts;      // int offset of the counts
+  size_t bytes;
+};
+
+MoePlan moe_plan(int64_t M, int64_t E, int64_t top_k);
+
+// Where a product's input and output rows are: by token (pair / top_k), by pair, or by position in the sorted list.
+enum MoeRows { MOE_BY_TOKEN = 0, MOE_BY_PAIR = 1, MOE_SORTED = 2 };
+
+struct MoeProduct {
+  const unsigned char* wp;  // [E] matrices in packed units
+  const uint16_t* x;
+  uint16_t* y;
+  const int* plan;
+  const int* pairs;
+  int M, E, top_k, N, K;
+  int src, dst;   // MoeRows
+  int epilogue;   // IM_EPI_STORE, IM_EPI_SWIGLU, IM_EPI_GEGLU
+  int early;      // the plan was finished before the preceding launch began: items and weights may be read before
+                  // the dependency wait
+};
+
+int moe_mma_launch(const MoePlan& p, const MoeProduct& a, cudaStream_t st);
+
+}  // namespace im

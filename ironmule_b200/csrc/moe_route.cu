@@ -1,0 +1,365 @@
+// The router of a mixture-of-experts block: per row the k experts with the largest keys and their weights, then the
+// (row, place) pairs sorted by expert and cut into the work items of the grouped products.
+//
+// Selection is exact: the key of expert e is float32(logit) + bias[e] (one rounding; -0 counts as +0), the k largest
+// keys are taken in order, ties to the lower expert. A logit of -inf or NaN closes the expert to the row; a row with
+// fewer than k open experts has id -1 and weight 0 in its remaining places.
+//   softmax: p_e = exp(v_e - max v) / sum over the chosen (normalise) or over every open expert
+//   sigmoid: p_e = 1 / (1 + exp(-v_e)), over the chosen's sum when normalised. There the sums run over
+//            exp(ls - max ls), ls = log sigmoid(v), so that far-negative logits do not underflow to 0 / 0.
+// Weights are float32 and unbiased by `bias`.
+//
+// One warp per row: lane l holds experts l, l + 32, ...; each of the k rounds takes the warp's largest 32-bit sortable
+// key with one reduction and the lowest expert holding it with a second. Up to 64 rows one block does all of it in one
+// launch. More rows are cut over up to 148 blocks: the first launch selects and counts, the second sums the blocks'
+// counts (every block for itself), scans them and places its pairs. The order is stable: within an expert, pairs ascend.
+// Bytes are few (a row's logits once, 12 bytes a place); what bounds it is launch and barrier latency.
+#include <math.h>
+
+#include "common.cuh"
+#include "moe.cuh"
+#include "../../include/imspec.h"
+
+namespace im {
+
+constexpr int MR_WARPS = 16;
+constexpr int MR_THREADS = MR_WARPS * 32;
+
+struct RouteArgs {
+  const void* logits;
+  const float* bias;
+  int* ids;
+  float* weights;
+  int* offsets;
+  int* pairs;
+  int* plan;
+  int* counts;
+  int f32, scoring, normalise;
+  float scale;
+  int M, E, top_k, item_rows, rows_per_block, blocks;
+  long long ld;
+};
+
+MoePlan moe_plan(int64_t M, int64_t E, int64_t top_k) {
+  MoePlan p;
+  const int64_t pairs = M * top_k;
+  // rows per item by the average number of rows an expert gets; an expert never gets more than M
+  const int64_t avg = (pairs + E - 1) / E;
+  p.item_rows = M <= 8 || avg <= 4 ? 8 : (M <= 16 || avg <= 12 ? 16 : 32);
+  const int64_t buckets = pairs < E + 1 ? pairs : E + 1;
+  p.max_items = buckets + pairs / p.item_rows;
+  const int64_t per = (M + MOE_ROUTE_BLOCKS - 1) / MOE_ROUTE_BLOCKS;
+  p.rows_per_block = M <= MOE_ROUTE_ROWS ? MOE_ROUTE_ROWS : (per < 16 ? 16 : per);
+  p.blocks = M <= MOE_ROUTE_ROWS ? 1 : (M + p.rows_per_block - 1) / p.rows_per_block;
+  p.counts = MOE_PLAN_HEADER + 4 * p.max_items;
+  p.bytes = (size_t)(p.counts + (p.blocks > 1 ? p.blocks * (E + 1) : 0)) * 4;
+  return p;
+}
+
+__device__ __forceinline__ unsigned mr_key(float f) {
+  const unsigned u = __float_as_uint(f + 0.f);  // -0 -> +0
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+__device__ __forceinline__ float mr_warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+// The chosen experts of one row: lane j < top_k returns place j's expert (-1: none) and writes its weight.
+template <int EL>
+__device__ __forceinline__ int mr_row(const RouteArgs& a, int row, int lane) {
+  float v[EL];
+  unsigned key[EL];
+  const float neg = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < EL; i++) {
+    const int e = i * 32 + lane;
+    v[i] = neg;
+    key[i] = 0u;
+    if (e < a.E) {
+      const size_t at = (size_t)row * a.ld + e;
+      const float l = a.f32 ? reinterpret_cast<const float*>(a.logits)[at]
+                            : bf(reinterpret_cast<const uint16_t*>(a.logits)[at]);
+      const float k = a.bias ? l + a.bias[e] : l;
+      if (l > neg && k > neg) {  // false for NaN too
+        v[i] = l;
+        key[i] = mr_key(k);
+      }
+    }
+  }
+  int mine = -1;
+  float value = neg;
+  for (int j = 0; j < a.top_k; j++) {
+    unsigned best = 0u;
+    int at = 0;
+    float bv = neg;
+#pragma unroll
+    for (int i = 0; i < EL; i++)
+      if (key[i] > best) {
+        best = key[i];
+        at = i;
+        bv = v[i];
+      }
+    const unsigned top = __reduce_max_sync(0xffffffffu, best);
+    if (top == 0u) break;  // no open expert is left (the same in every lane)
+    const unsigned cand = best == top ? (unsigned)(at * 32 + lane) : 0xffffffffu;
+    const unsigned e = __reduce_min_sync(0xffffffffu, cand);
+    const float ev = __shfl_sync(0xffffffffu, bv, (int)(e & 31u));
+    if (cand == e) {
+#pragma unroll
+      for (int i = 0; i < EL; i++)
+        if (i == at) key[i] = 0u;
+    }
+    if (lane == j) {
+      mine = (int)e;
+      value = ev;
+    }
+  }
+  // the weights
+  const bool live = mine >= 0;
+  float w = 0.f;
+  if (a.scoring == IM_MOE_SOFTMAX) {
+    float top = neg;
+#pragma unroll
+    for (int i = 0; i < EL; i++) top = fmaxf(top, v[i]);
+    top = mr_warp_max(top);
+    const float p = live ? (value == top ? 1.f : expf(value - top)) : 0.f;  // (inf - inf counts as 0)
+    float total = p;
+    if (!a.normalise) {
+      total = 0.f;
+#pragma unroll
+      for (int i = 0; i < EL; i++) total += v[i] > neg ? (v[i] == top ? 1.f : expf(v[i] - top)) : 0.f;
+    }
+    total = warp_sum(total);
+    w = live ? p / total : 0.f;
+  } else if (a.normalise) {
+    const float ls = live ? fminf(value, 0.f) - log1pf(expf(-fabsf(value))) : neg;
+    const float top = mr_warp_max(ls);
+    const float p = live ? expf(ls - top) : 0.f;
+    const float total = warp_sum(p);
+    w = live ? p / total : 0.f;
+  } else {
+    w = live ? 1.f / (1.f + expf(-value)) : 0.f;
+  }
+  if (lane < a.top_k) {
+    a.ids[(size_t)row * a.top_k + lane] = mine;
+    a.weights[(size_t)row * a.top_k + lane] = w * a.scale;
+  }
+  return mine;
+}
+
+// Exclusive scan of v[0..n) in shared memory into out[0..n) (out may be v); returns the total. All threads call it.
+__device__ __forceinline__ int mr_scan(const int* v, int* out, int n, int* sh) {
+  const int per = (n + MR_THREADS - 1) / MR_THREADS, lo = threadIdx.x * per;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int sum = 0;
+  for (int i = lo; i < min(lo + per, n); i++) sum += v[i];
+  int incl = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int t = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += t;
+  }
+  if (lane == 31) sh[warp] = incl;
+  __syncthreads();
+  int before = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < MR_WARPS; w++) {
+    if (w < warp) before += sh[w];
+    total += sh[w];
+  }
+  int run = before + incl - sum;
+  for (int i = lo; i < min(lo + per, n); i++) {
+    const int t = v[i];
+    out[i] = run;
+    run += t;
+  }
+  __syncthreads();
+  return total;
+}
+
+struct RouteSmem {
+  int total[MOE_MAX_EXPERTS + 1];   // pairs of each bucket over all blocks
+  int base[MOE_MAX_EXPERTS + 1];    // pairs of each bucket in earlier blocks, then where the next one goes
+  int scan[MOE_MAX_EXPERTS + 1];
+  int cnt[MR_WARPS][MOE_MAX_EXPERTS + 1];
+  int sh[MR_WARPS];
+};
+
+// Offsets, work items (block 0) and this block's pairs, from s.total and s.base.
+__device__ __forceinline__ void mr_place(const RouteArgs& a, RouteSmem& s) {
+  const int nb = a.E + 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (blockIdx.x == 0) {
+    for (int e = threadIdx.x; e < nb; e += MR_THREADS) s.scan[e] = (s.total[e] + a.item_rows - 1) / a.item_rows;
+    __syncthreads();
+    const int items = mr_scan(s.scan, s.scan, nb, s.sh);
+    if (threadIdx.x == 0) {
+      a.plan[0] = items;
+      a.plan[1] = 0;
+    }
+  }
+  // s.cnt[0] holds the bucket offsets until the pairs are counted
+  const int all = mr_scan(s.total, s.cnt[0], nb, s.sh);
+  if (blockIdx.x == 0) {
+    int4* items = reinterpret_cast<int4*>(a.plan + MOE_PLAN_HEADER);
+    for (int e = threadIdx.x; e < nb; e += MR_THREADS) {
+      const int c = s.total[e], first = s.cnt[0][e];
+      a.offsets[e] = first;
+      // an expert's rows in as few items as they fit, evenly, in multiples of 8
+      const int n = (c + a.item_rows - 1) / a.item_rows;
+      const int each = n ? ((c + n - 1) / n + 7) / 8 * 8 : 0;
+      for (int i = 0; i < n; i++)
+        items[s.scan[e] + i] = make_int4(e, first + i * each, max(0, min(each, c - i * each)), 0);
+    }
+    if (threadIdx.x == 0) a.offsets[nb] = all;
+  }
+  for (int e = threadIdx.x; e < nb; e += MR_THREADS) s.base[e] += s.cnt[0][e];
+  __syncthreads();
+  const int row0 = blockIdx.x * a.rows_per_block;
+  const int p0 = row0 * a.top_k, p1 = min(a.M, row0 + a.rows_per_block) * a.top_k;
+  for (int c0 = p0; c0 < p1; c0 += MR_THREADS) {
+    for (int i = threadIdx.x; i < MR_WARPS * nb; i += MR_THREADS) s.cnt[i / nb][i % nb] = 0;
+    __syncthreads();
+    const int pair = c0 + threadIdx.x;
+    int bucket = -1, rank = 0;
+    if (pair < p1) {
+      const int id = a.ids[pair];
+      bucket = id < 0 ? a.E : id;
+    }
+    const unsigned same = __match_any_sync(0xffffffffu, bucket);
+    rank = __popc(same & ((1u << lane) - 1u));
+    if (bucket >= 0 && rank == 0) s.cnt[warp][bucket] = __popc(same);
+    __syncthreads();
+    for (int e = threadIdx.x; e < nb; e += MR_THREADS) {
+      int run = s.base[e];
+#pragma unroll
+      for (int w = 0; w < MR_WARPS; w++) {
+        const int t = s.cnt[w][e];
+        s.cnt[w][e] = run;
+        run += t;
+      }
+      s.base[e] = run;
+    }
+    __syncthreads();
+    if (bucket >= 0) a.pairs[s.cnt[warp][bucket] + rank] = pair;
+    __syncthreads();
+  }
+}
+
+// Selection and counting; with ONE the block holds every row and places the pairs too.
+template <int EL, bool ONE>
+__global__ void __launch_bounds__(MR_THREADS) moe_select_kernel(RouteArgs a) {
+  __shared__ RouteSmem s;
+  const int nb = a.E + 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int e = threadIdx.x; e < nb; e += MR_THREADS) {
+    s.total[e] = 0;
+    s.base[e] = 0;
+  }
+  pdl_wait();
+  pdl_trigger();
+  __syncthreads();
+  const int r0 = blockIdx.x * a.rows_per_block, r1 = min(a.M, r0 + a.rows_per_block);
+  for (int row = r0 + warp; row < r1; row += MR_WARPS) {
+    const int id = mr_row<EL>(a, row, lane);
+    if (lane < a.top_k) atomicAdd(&s.total[id < 0 ? a.E : id], 1);
+  }
+  __syncthreads();
+  if constexpr (ONE) {
+    mr_place(a, s);
+  } else {
+    for (int e = threadIdx.x; e < nb; e += MR_THREADS) a.counts[(size_t)blockIdx.x * nb + e] = s.total[e];
+  }
+}
+
+__global__ void __launch_bounds__(MR_THREADS) moe_place_kernel(RouteArgs a) {
+  __shared__ RouteSmem s;
+  const int nb = a.E + 1;
+  for (int e = threadIdx.x; e < nb; e += MR_THREADS) {
+    s.total[e] = 0;
+    s.base[e] = 0;
+  }
+  pdl_wait();
+  pdl_trigger();
+  __syncthreads();
+  const int n = a.blocks * nb, mine = blockIdx.x * nb;
+  for (int i = threadIdx.x; i < n; i += MR_THREADS) {
+    const int c = a.counts[i];
+    if (c) {
+      const int e = i % nb;
+      atomicAdd(&s.total[e], c);
+      if (i < mine) atomicAdd(&s.base[e], c);
+    }
+  }
+  __syncthreads();
+  mr_place(a, s);
+}
+
+template <int EL>
+static int mr_launch(const RouteArgs& a, cudaStream_t st) {
+  if (a.blocks <= 1)
+    return launch("moe_select_kernel", moe_select_kernel<EL, true>, dim3(1), dim3(MR_THREADS), 0, st, a);
+  const int rc = launch("moe_select_kernel", moe_select_kernel<EL, false>, dim3(a.blocks), dim3(MR_THREADS), 0, st, a);
+  if (rc) return rc;
+  return launch("moe_place_kernel", moe_place_kernel, dim3(a.blocks), dim3(MR_THREADS), 0, st, a);
+}
+
+}  // namespace im
+
+using namespace im;
+
+static bool moe_sizes_ok(int64_t M, int64_t E, int64_t top_k) {
+  return M >= 0 && M <= MOE_MAX_ROWS && E >= 1 && E <= MOE_MAX_EXPERTS && top_k >= 1 && top_k <= MOE_MAX_TOP_K &&
+         top_k <= E;
+}
+
+extern "C" size_t im_moe_plan_bytes(int64_t M, int64_t E, int64_t top_k) {
+  return moe_sizes_ok(M, E, top_k) ? moe_plan(M, E, top_k).bytes : 0;
+}
+
+extern "C" int im_moe_route(const void* logits, int logits_f32, int64_t M, int64_t E, int64_t ld, const float* bias,
+                            int64_t top_k, int scoring, int normalise, float scale, int32_t* ids, float* weights,
+                            int32_t* offsets, int32_t* pairs, void* plan, size_t plan_bytes, void* stream) {
+  clear_error();
+  IM_REQUIRE(M >= 0 && E >= 1 && top_k >= 1 && top_k <= E, IM_INVALID,
+             "im_moe_route: bad sizes M=%lld E=%lld top_k=%lld", (long long)M, (long long)E, (long long)top_k);
+  IM_REQUIRE(moe_sizes_ok(M, E, top_k), IM_UNSUPPORTED,
+             "im_moe_route: at most %lld rows, %d experts and %d places a row (M=%lld E=%lld top_k=%lld)",
+             (long long)MOE_MAX_ROWS, MOE_MAX_EXPERTS, MOE_MAX_TOP_K, (long long)M, (long long)E, (long long)top_k);
+  IM_REQUIRE(scoring == IM_MOE_SOFTMAX || scoring == IM_MOE_SIGMOID, IM_INVALID, "im_moe_route: bad scoring");
+  IM_REQUIRE(offsets && plan, IM_INVALID, "im_moe_route: null pointer");
+  IM_REQUIRE(M == 0 || (logits && ids && weights && pairs), IM_INVALID, "im_moe_route: null pointer");
+  IM_REQUIRE(ld >= E, IM_INVALID, "im_moe_route: row stride %lld below %lld experts", (long long)ld, (long long)E);
+  IM_REQUIRE(aligned(logits, logits_f32 ? 4 : 2) && aligned(plan, 16), IM_INVALID,
+             "im_moe_route: misaligned logits or plan");
+  const MoePlan p = moe_plan(M, E, top_k);
+  IM_REQUIRE(plan_bytes >= p.bytes, IM_INVALID, "im_moe_route: plan of %zu bytes needed, %zu given", p.bytes,
+             plan_bytes);
+  RouteArgs a = {};
+  a.logits = logits;
+  a.bias = bias;
+  a.ids = ids;
+  a.weights = weights;
+  a.offsets = offsets;
+  a.pairs = pairs;
+  a.plan = reinterpret_cast<int*>(plan);
+  a.counts = a.plan + p.counts;
+  a.f32 = logits_f32;
+  a.scoring = scoring;
+  a.normalise = normalise;
+  a.scale = scale;
+  a.M = (int)M;
+  a.E = (int)E;
+  a.top_k = (int)top_k;
+  a.item_rows = (int)p.item_rows;
+  a.rows_per_block = (int)p.rows_per_block;
+  a.blocks = (int)p.blocks;
+  a.ld = ld;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (E <= 32) return mr_launch<1>(a, st);
+  if (E <= 64) return mr_launch<2>(a, st);
+  if (E <= 128) return mr_launch<4>(a, st);
+  if (E <= 256) return mr_launch<8>(a, st);
+  return mr_launch<16>(a, st);
+}

@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import threading
+from dataclasses import dataclass
 
 import torch
 
@@ -498,6 +499,192 @@ def qgemm_packed_attn(attn_ws: torch.Tensor, p: Packed, seq_rows: torch.Tensor, 
               b, max_rows_per_seq, hq, hkv, d, max_kv_len, keys_per_split, out.data_ptr(), residual.data_ptr(), rows,
               p.n, p.k, _ptr_or_none(out_sq), sq_ld, ws_ptr, ws_bytes, _stream(device))
     return out
+
+
+# ---- mixture-of-experts blocks ------------------------------------------------------------------------------
+_SCORING = {"softmax": _lib.MOE_SOFTMAX, "sigmoid": _lib.MOE_SIGMOID}
+
+
+class Experts:
+    """E 4-bit matrices [N, K] of one shape, repacked once into MMA-fragment order: w int32 [E, N, K/8], scales and
+    biases bf16 [E, N, K/64] (MLX's layout of stacked experts)."""
+
+    def __init__(self, w: torch.Tensor, scales: torch.Tensor, biases: torch.Tensor):
+        _check(w, "w", (torch.int32, torch.uint32))
+        _check(scales, "scales", (torch.bfloat16,), w.device)
+        _check(biases, "biases", (torch.bfloat16,), w.device)
+        if w.dim() != 3:
+            raise ValueError(f"w must be [E, N, K/8], got {tuple(w.shape)}")
+        self.e, self.n, self.k = int(w.shape[0]), int(w.shape[1]), int(w.shape[2]) * 8
+        if scales.shape != (self.e, self.n, self.k // 64) or biases.shape != scales.shape:
+            raise ValueError(f"shape mismatch: w {tuple(w.shape)}, scales {tuple(scales.shape)}, "
+                             f"biases {tuple(biases.shape)}")
+        nbytes = int(_lib.load().im_moe_packed_bytes(self.e, self.n, self.k))
+        self.data = torch.empty(nbytes, dtype=torch.uint8, device=w.device)
+        _lib.call("im_moe_pack_w4g64", w.data_ptr(), scales.data_ptr(), biases.data_ptr(), self.e, self.n, self.k,
+                  self.data.data_ptr(), _stream(w.device))
+
+    @classmethod
+    def gate_up(cls, gate: tuple, up: tuple) -> "Experts":
+        """The first product of a gated MLP: gate and up as (w, scales, biases) of [E, I, K], interleaved in 16-row
+        blocks so that one tile holds both halves of its outputs."""
+        def weave(g: torch.Tensor, u: torch.Tensor) -> torch.Tensor:
+            e, i, c = g.shape
+            if u.shape != g.shape or i % 16:
+                raise ValueError("gate and up must have one shape, the intermediate size a multiple of 16")
+            return torch.stack([g.view(e, i // 16, 16, c), u.view(e, i // 16, 16, c)], dim=2).reshape(e, 2 * i, c)
+
+        return cls(*(weave(g.contiguous(), u.contiguous()) for g, u in zip(gate, up)))
+
+
+@dataclass
+class Routing:
+    """What moe_route found: per row and place the expert (int32 [M, k], -1: none) and its weight (float32 [M, k]); the
+    pairs m * k + j sorted by expert (int32 [M * k]), where each expert's begin (int32 [E + 2]; the last bucket holds
+    the places without an expert), and the products' work items."""
+    ids: torch.Tensor
+    weights: torch.Tensor
+    offsets: torch.Tensor
+    pairs: torch.Tensor
+    plan: torch.Tensor
+    rows: int
+    experts: int
+    top_k: int
+
+
+def moe_route(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax", normalise: bool = True,
+              scale: float = 1.0, bias: torch.Tensor | None = None, rows: int | None = None) -> Routing:
+    """Choose top_k experts for each of the first `rows` rows of logits [M, E] (bf16 or float32): the largest
+    logit + bias, ties to the lower expert; -inf or NaN closes an expert to a row."""
+    _check(logits, "logits", (torch.bfloat16, torch.float32))
+    if logits.dim() != 2:
+        raise ValueError(f"logits must be [M, E], got {tuple(logits.shape)}")
+    if scoring not in _SCORING:
+        raise ValueError(f"scoring {scoring!r}: softmax or sigmoid")
+    device, e = logits.device, logits.shape[1]
+    m = logits.shape[0] if rows is None else rows
+    if not 0 <= m <= logits.shape[0]:
+        raise ValueError(f"{m} rows of {logits.shape[0]}")
+    if bias is not None:
+        _check(bias, "bias", (torch.float32,), device)
+        if bias.shape != (e,):
+            raise ValueError(f"bias must be [{e}], got {tuple(bias.shape)}")
+    if not 1 <= top_k <= e:
+        raise ValueError(f"top_k {top_k} of {e} experts")
+    ids = torch.empty((m, top_k), dtype=torch.int32, device=device)
+    weights = torch.empty((m, top_k), dtype=torch.float32, device=device)
+    offsets = torch.empty(e + 2, dtype=torch.int32, device=device)
+    pairs = torch.empty(m * top_k, dtype=torch.int32, device=device)
+    nbytes = int(_lib.load().im_moe_plan_bytes(m, e, top_k))
+    plan = torch.empty((nbytes + 3) // 4, dtype=torch.int32, device=device)
+    _lib.call("im_moe_route", logits.data_ptr(), int(logits.dtype == torch.float32), m, e, e, _ptr_or_none(bias), top_k,
+              _SCORING[scoring], int(normalise), float(scale), ids.data_ptr(), weights.data_ptr(), offsets.data_ptr(),
+              pairs.data_ptr(), plan.data_ptr(), nbytes, _stream(device))
+    return Routing(ids, weights, offsets, pairs, plan, m, e, top_k)
+
+
+def _moe_rows(x: torch.Tensor, experts: Experts, routing: Routing) -> bool:
+    """Check x against the routing and the weights; whether x holds a row per pair ([M, k, K]) or per row ([M, K])."""
+    _check(x, "x", (torch.bfloat16,), experts.data.device)
+    if routing.ids.device != x.device:
+        raise ValueError(f"the routing is on {routing.ids.device}, x on {x.device}")
+    if x.shape[-1] != experts.k:
+        raise ValueError(f"x has K={x.shape[-1]}, the experts {experts.k}")
+    if experts.e != routing.experts:
+        raise ValueError(f"{experts.e} experts, the routing is over {routing.experts}")
+    by_pair = x.dim() == 3
+    lead = (routing.rows, routing.top_k) if by_pair else (routing.rows,)
+    if tuple(x.shape[:-1]) != lead:
+        raise ValueError(f"x {tuple(x.shape)} does not match a routing of {routing.rows} rows, {routing.top_k} places")
+    return by_pair
+
+
+def _moe_out(out: torch.Tensor | None, shape: tuple, device: torch.device) -> torch.Tensor:
+    if out is None:
+        return torch.empty(shape, dtype=torch.bfloat16, device=device)
+    _check(out, "out", (torch.bfloat16,), device)
+    if tuple(out.shape) != shape:
+        raise ValueError(f"out must be {shape}, got {tuple(out.shape)}")
+    return out
+
+
+def grouped_qgemm(x: torch.Tensor, experts: Experts, routing: Routing, *,
+                  out: torch.Tensor | None = None) -> torch.Tensor:
+    """y[m, j] = W[ids[m, j]] x[m] for x [M, K], or W[ids[m, j]] x[m, j] for x [M, k, K]; bf16 [M, k, N], zero for
+    places without an expert."""
+    by_pair = _moe_rows(x, experts, routing)
+    out = _moe_out(out, (routing.rows, routing.top_k, experts.n), x.device)
+    _lib.call("im_moe_grouped_qgemm", experts.data.data_ptr(), x.data_ptr(), out.data_ptr(), routing.rows, experts.e,
+              routing.top_k, experts.n, experts.k, int(by_pair), routing.pairs.data_ptr(), routing.plan.data_ptr(),
+              routing.plan.numel() * 4, _stream(x.device))
+    return out
+
+
+def moe_mlp(x: torch.Tensor, gate_up: Experts, down: Experts, routing: Routing, *, activation: str = "swiglu",
+            out: torch.Tensor | None = None) -> torch.Tensor:
+    """y[m, j] = D (act(G x[m]) * (U x[m])) with the matrices of expert ids[m, j]; act "swiglu" or "geglu"; bf16
+    [M, k, H], zero for places without an expert. `gate_up` is Experts.gate_up's."""
+    if _moe_rows(x, gate_up, routing):
+        raise ValueError("x must be [M, H]")
+    if activation not in ("swiglu", "geglu"):
+        raise ValueError(f"activation {activation!r}: swiglu or geglu")
+    h, inter = gate_up.k, gate_up.n // 2
+    if (down.e, down.n, down.k) != (gate_up.e, h, inter) or down.data.device != x.device:
+        raise ValueError(f"down is {down.e} x [{down.n}, {down.k}], expected {gate_up.e} x [{h}, {inter}]")
+    out = _moe_out(out, (routing.rows, routing.top_k, h), x.device)
+    need = int(_lib.load().im_moe_mlp_workspace_bytes(routing.rows, gate_up.e, routing.top_k, h, inter))
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+    _lib.call("im_moe_mlp", gate_up.data.data_ptr(), down.data.data_ptr(), x.data_ptr(), out.data_ptr(), routing.rows,
+              gate_up.e, routing.top_k, h, inter, _EPILOGUES[activation], routing.pairs.data_ptr(),
+              routing.plan.data_ptr(), routing.plan.numel() * 4, ws.data_ptr(), need, _stream(x.device))
+    return out
+
+
+def block_residual(y: torch.Tensor, h: torch.Tensor, eps: float, *, weights: torch.Tensor | None = None,
+                   post_norm: torch.Tensor | None = None, gate: torch.Tensor | None = None,
+                   residual_scale: float = 1.0, next_norm: torch.Tensor | None = None, gemma: bool = False,
+                   out: torch.Tensor | None = None, out_sq: torch.Tensor | None = None):
+    """(h', z): a block's output joins the residual stream and the next block's input is normalised, in one pass.
+    b = sum_j weights[m, j] y[m, j] (y [M, k, H] with weights float32 [M, k]; or y [M, H]); with post_norm its RMSNorm;
+    h' = residual_scale * h + gate * b (gate bf16 [H], [M, 1] or [M, H]); z = RMSNorm(h') with next_norm, else None.
+    `out` may be h. out_sq (float32 [M]) gets the sums of squares of the rounded h' rows."""
+    _check(h, "h", (torch.bfloat16,))
+    device = h.device
+    _check(y, "y", (torch.bfloat16,), device)
+    if h.dim() != 2:
+        raise ValueError(f"h must be [M, H], got {tuple(h.shape)}")
+    m, hsz = h.shape
+    if weights is None:
+        places = 1
+        if tuple(y.shape) not in ((m, hsz), (m, 1, hsz)):
+            raise ValueError(f"y must be [{m}, {hsz}] without weights, got {tuple(y.shape)}")
+    else:
+        _check(weights, "weights", (torch.float32,), device)
+        places = weights.shape[-1]
+        if tuple(weights.shape) != (m, places) or tuple(y.shape) != (m, places, hsz):
+            raise ValueError(f"weights {tuple(weights.shape)} and y {tuple(y.shape)} do not match h {tuple(h.shape)}")
+    for name, t in (("post_norm", post_norm), ("next_norm", next_norm)):
+        if t is not None:
+            _check(t, name, (torch.bfloat16,), device)
+            if t.shape != (hsz,):
+                raise ValueError(f"{name} must be [{hsz}], got {tuple(t.shape)}")
+    row = col = 0
+    if gate is not None:
+        _check(gate, "gate", (torch.bfloat16,), device)
+        strides = {(hsz,): (0, 1), (m, 1): (1, 0), (m, hsz): (hsz, 1)}.get(tuple(gate.shape))
+        if strides is None:
+            raise ValueError(f"gate must be [{hsz}], [{m}, 1] or [{m}, {hsz}], got {tuple(gate.shape)}")
+        row, col = strides
+    if out_sq is not None:
+        _check(out_sq, "out_sq", (torch.float32,), device)
+        if out_sq.numel() < m:
+            raise ValueError(f"out_sq needs {m} elements")
+    out = _moe_out(out, (m, hsz), device)
+    z = torch.empty((m, hsz), dtype=torch.bfloat16, device=device) if next_norm is not None else None
+    _lib.call("im_block_residual", y.data_ptr(), _ptr_or_none(weights), places, h.data_ptr(), _ptr_or_none(post_norm),
+              _ptr_or_none(gate), row, col, float(residual_scale), _ptr_or_none(next_norm), float(eps), int(gemma), m, hsz,
+              out.data_ptr(), _ptr_or_none(z), _ptr_or_none(out_sq), _stream(device))
+    return out, z
 
 
 # ---- GGUF k-quants (the ggml path) ----------------------------------------------------------------------------
