@@ -1,4 +1,6 @@
 // Entry points of the products by expert: one grouped 4-bit product, and the gated MLP of two of them.
+#include <math.h>
+
 #include "common.cuh"
 #include "moe.cuh"
 #include "../../include/imspec.h"
@@ -6,16 +8,17 @@
 namespace im {
 
 // The checks that both entry points share; IM_OK when the sizes and the plan are usable.
-static int moe_check(const char* who, int64_t M, int64_t E, int64_t top_k, const int32_t* pairs, const void* plan,
-                     size_t plan_bytes) {
+static int moe_check(const char* who, int64_t M, int64_t E, int64_t top_k, const int32_t* pairs, int path,
+                     const void* plan, size_t plan_bytes) {
   IM_REQUIRE(M >= 0 && E >= 1 && top_k >= 1 && top_k <= E, IM_INVALID, "%s: bad sizes M=%lld E=%lld top_k=%lld", who,
              (long long)M, (long long)E, (long long)top_k);
   IM_REQUIRE(M <= MOE_MAX_ROWS && E <= MOE_MAX_EXPERTS && top_k <= MOE_MAX_TOP_K, IM_UNSUPPORTED,
              "%s: at most %lld rows, %d experts and %d places a row", who, (long long)MOE_MAX_ROWS, MOE_MAX_EXPERTS,
              MOE_MAX_TOP_K);
+  IM_REQUIRE(path >= IM_MOE_AUTO && path <= IM_MOE_TENSOR, IM_INVALID, "%s: bad path", who);
   if (M == 0) return IM_OK;
   IM_REQUIRE(pairs && plan && aligned(plan, 16), IM_INVALID, "%s: null or misaligned plan", who);
-  const size_t need = moe_plan(M, E, top_k).bytes;
+  const size_t need = moe_plan(M, E, top_k, path).bytes;
   IM_REQUIRE(plan_bytes >= need, IM_INVALID, "%s: plan of %zu bytes needed, %zu given", who, need, plan_bytes);
   return IM_OK;
 }
@@ -24,7 +27,41 @@ static bool moe_nk_ok(int64_t N, int64_t K) {
   return N >= 1 && N <= (1 << 24) && K >= 64 && K % 64 == 0 && K <= (1 << 20);
 }
 
-static int moe_product(const MoePlan& p, const MoeProduct& a, cudaStream_t st) { return moe_mma_launch(p, a, st); }
+// One thread per row of a block's group: its codes into the packed order, the largest |w| of the expert into wmax (all
+// values non-negative, so their bit patterns order as integers and the maximum does not depend on the order).
+__global__ void __launch_bounds__(128)
+moe_pack_kernel(const uint32_t* __restrict__ w, const uint16_t* __restrict__ sc, const uint16_t* __restrict__ bi, int N,
+                int K, int blocks, unsigned char* __restrict__ out, unsigned* __restrict__ wmax) {
+  const int G = K >> 6;
+  const long long unit = blockIdx.x;  // (expert * blocks + block) * G + group
+  const int grp = (int)(unit % G), block = (int)(unit / G % blocks);
+  const long long expert = unit / G / blocks;
+  const int r = block * 128 + threadIdx.x, tile = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint32_t words[8] = {};
+  uint16_t s = 0, b = 0;
+  float top = 0.f;
+  if (r < N) {
+    const size_t row = (size_t)expert * N + r;
+#pragma unroll
+    for (int i = 0; i < 8; i++) words[i] = w[row * (K >> 3) + grp * 8 + i];
+    s = sc[row * G + grp];
+    b = bi[row * G + grp];
+    top = fmaxf(fabsf(bf(b)), fabsf(fmaf(15.f, bf(s), bf(b))));
+    if (!(top < INFINITY)) top = 0.f;  // (a broken group does not hide the scale of the others)
+  }
+  unsigned char* dst = out + unit * MOE_BLOCK_BYTES;
+  uint4* d = reinterpret_cast<uint4*>(dst + tile * 1024 + lane * 16);
+  d[0] = make_uint4(words[0], words[1], words[2], words[3]);
+  d[32] = make_uint4(words[4], words[5], words[6], words[7]);
+  uint16_t* sb = reinterpret_cast<uint16_t*>(dst + 4096 + tile * 128 + (lane & 7) * 16);
+  sb[lane >> 3] = s;
+  sb[4 + (lane >> 3)] = b;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (lane == 0 && top > 0.f) atomicMax(wmax + expert, __float_as_uint(top));
+}
+
+static size_t moe_expert_bytes(int64_t N, int64_t K) { return (size_t)((N + 127) / 128) * (K / 64) * MOE_BLOCK_BYTES; }
 
 }  // namespace im
 
@@ -32,7 +69,7 @@ using namespace im;
 
 extern "C" size_t im_moe_packed_bytes(int64_t E, int64_t N, int64_t K) {
   if (E < 1 || E > MOE_MAX_EXPERTS || !moe_nk_ok(N, K)) return 0;
-  return (size_t)E * im_qgemm_packed_bytes(N, K);
+  return (size_t)E * (moe_expert_bytes(N, K) + 4);
 }
 
 extern "C" int im_moe_pack_w4g64(const uint32_t* w, const uint16_t* scales, const uint16_t* biases, int64_t E,
@@ -41,20 +78,48 @@ extern "C" int im_moe_pack_w4g64(const uint32_t* w, const uint16_t* scales, cons
   IM_REQUIRE(E >= 1 && E <= MOE_MAX_EXPERTS && moe_nk_ok(N, K), IM_INVALID,
              "im_moe_pack_w4g64: bad sizes E=%lld N=%lld K=%lld", (long long)E, (long long)N, (long long)K);
   IM_REQUIRE(w && scales && biases && packed, IM_INVALID, "im_moe_pack_w4g64: null pointer");
-  const size_t bytes = im_qgemm_packed_bytes(N, K);
-  for (int64_t e = 0; e < E; e++) {  // once per model load; rows of an expert are padded to whole tiles
-    const int rc = im_qgemm_pack_w4g64(w + e * N * (K / 8), scales + e * N * (K / 64), biases + e * N * (K / 64), N, K,
-                                       reinterpret_cast<char*>(packed) + e * bytes, stream);
-    if (rc) return rc;
+  IM_REQUIRE(aligned(packed, 16) && aligned(w, 4) && aligned(scales, 2) && aligned(biases, 2), IM_INVALID,
+             "im_moe_pack_w4g64: misaligned buffer");
+  const int64_t blocks = (N + 127) / 128, units = E * blocks * (K / 64);
+  IM_REQUIRE(units < (1ll << 31), IM_UNSUPPORTED, "im_moe_pack_w4g64: too many units");
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  unsigned char* out = reinterpret_cast<unsigned char*>(packed);
+  unsigned* wmax = reinterpret_cast<unsigned*>(out + (size_t)E * moe_expert_bytes(N, K));
+  const cudaError_t e = cudaMemsetAsync(wmax, 0, (size_t)E * 4, st);
+  if (e != cudaSuccess) {
+    set_error("im_moe_pack_w4g64: %s", cudaGetErrorString(e));
+    return IM_CUDA_ERROR;
   }
-  return IM_OK;
+  moe_pack_kernel<<<(unsigned)units, 128, 0, st>>>(w, scales, biases, (int)N, (int)K, (int)blocks, out, wmax);
+  return check_launch("moe_pack_kernel");
+}
+
+extern "C" int im_moe_status(const void* plan) {
+  clear_error();
+  IM_REQUIRE(plan, IM_INVALID, "im_moe_status: null plan");
+  int word = 0;
+  const cudaError_t e = cudaMemcpy(&word, reinterpret_cast<const int*>(plan) + 1, 4, cudaMemcpyDeviceToHost);
+  if (e != cudaSuccess) {
+    set_error("im_moe_status: %s", cudaGetErrorString(e));
+    return IM_CUDA_ERROR;
+  }
+  return word;
+}
+
+extern "C" size_t im_moe_grouped_workspace_bytes(int64_t M, int64_t E, int64_t top_k, int64_t K, int x_by_pair,
+                                                 int path) {
+  if (M < 1 || M > MOE_MAX_ROWS || E < 1 || E > MOE_MAX_EXPERTS || top_k < 1 || top_k > MOE_MAX_TOP_K || top_k > E ||
+      !moe_nk_ok(1, K) || moe_plan(M, E, top_k, path).item_rows != MOE_TC_ROWS)
+    return 0;
+  return moe_tc_space(x_by_pair ? M * top_k : M, K, 0, 0).total;
 }
 
 extern "C" int im_moe_grouped_qgemm(const void* packed, const uint16_t* x, uint16_t* y, int64_t M, int64_t E,
-                                    int64_t top_k, int64_t N, int64_t K, int x_by_pair, const int32_t* pairs,
-                                    const void* plan, size_t plan_bytes, void* stream) {
+                                    int64_t top_k, int64_t N, int64_t K, int x_by_pair, const int32_t* pairs, int path,
+                                    void* plan, size_t plan_bytes, void* workspace, size_t workspace_bytes,
+                                    void* stream) {
   clear_error();
-  const int rc = moe_check("im_moe_grouped_qgemm", M, E, top_k, pairs, plan, plan_bytes);
+  const int rc = moe_check("im_moe_grouped_qgemm", M, E, top_k, pairs, path, plan, plan_bytes);
   if (rc) return rc;
   IM_REQUIRE(moe_nk_ok(N, K), IM_INVALID, "im_moe_grouped_qgemm: bad sizes N=%lld K=%lld", (long long)N,
              (long long)K);
@@ -62,6 +127,9 @@ extern "C" int im_moe_grouped_qgemm(const void* packed, const uint16_t* x, uint1
   IM_REQUIRE(packed && x && y, IM_INVALID, "im_moe_grouped_qgemm: null pointer");
   IM_REQUIRE(aligned(packed, 16) && aligned(x, 16) && aligned(y, 2), IM_INVALID,
              "im_moe_grouped_qgemm: packed and x must be 16-byte aligned");
+  const size_t need = im_moe_grouped_workspace_bytes(M, E, top_k, K, x_by_pair, path);
+  IM_REQUIRE(!need || (workspace && aligned(workspace, 256) && workspace_bytes >= need), IM_INVALID,
+             "im_moe_grouped_qgemm: workspace of %zu bytes (256-aligned) needed, %zu given", need, workspace_bytes);
   MoeProduct a = {};
   a.wp = reinterpret_cast<const unsigned char*>(packed);
   a.x = x;
@@ -76,21 +144,28 @@ extern "C" int im_moe_grouped_qgemm(const void* packed, const uint16_t* x, uint1
   a.src = x_by_pair ? MOE_BY_PAIR : MOE_BY_TOKEN;
   a.dst = MOE_BY_PAIR;
   a.epilogue = IM_EPI_STORE;
-  return moe_product(moe_plan(M, E, top_k), a, reinterpret_cast<cudaStream_t>(stream));
+  const MoePlan p = moe_plan(M, E, top_k, path);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (p.item_rows != MOE_TC_ROWS) return moe_mma_launch(p, a, st);
+  const int64_t rows = x_by_pair ? M * top_k : M;
+  const MoeTcSpace space = moe_tc_space(rows, K, 0, 0);
+  const int prep = moe_prep_launch(x, rows, K, space, workspace, st);
+  return prep ? prep : moe_tc_launch(p, a, space, workspace, st);
 }
 
-extern "C" size_t im_moe_mlp_workspace_bytes(int64_t M, int64_t E, int64_t top_k, int64_t H, int64_t I) {
-  if (M < 0 || M > MOE_MAX_ROWS || E < 1 || E > MOE_MAX_EXPERTS || top_k < 1 || top_k > MOE_MAX_TOP_K || top_k > E ||
+extern "C" size_t im_moe_mlp_workspace_bytes(int64_t M, int64_t E, int64_t top_k, int64_t H, int64_t I, int path) {
+  if (M < 1 || M > MOE_MAX_ROWS || E < 1 || E > MOE_MAX_EXPERTS || top_k < 1 || top_k > MOE_MAX_TOP_K || top_k > E ||
       H < 64 || H % 64 || I < 64 || I % 64)
     return 0;
+  if (moe_plan(M, E, top_k, path).item_rows == MOE_TC_ROWS) return moe_tc_space(M, H, M * top_k, I).total;
   return (size_t)M * top_k * I * 2;
 }
 
 extern "C" int im_moe_mlp(const void* gate_up, const void* down, const uint16_t* x, uint16_t* y, int64_t M, int64_t E,
-                          int64_t top_k, int64_t H, int64_t I, int activation, const int32_t* pairs, const void* plan,
-                          size_t plan_bytes, void* workspace, size_t workspace_bytes, void* stream) {
+                          int64_t top_k, int64_t H, int64_t I, int activation, const int32_t* pairs, int path,
+                          void* plan, size_t plan_bytes, void* workspace, size_t workspace_bytes, void* stream) {
   clear_error();
-  const int rc = moe_check("im_moe_mlp", M, E, top_k, pairs, plan, plan_bytes);
+  const int rc = moe_check("im_moe_mlp", M, E, top_k, pairs, path, plan, plan_bytes);
   if (rc) return rc;
   IM_REQUIRE(moe_nk_ok(H, H) && moe_nk_ok(2 * I, I), IM_INVALID,
              "im_moe_mlp: hidden and intermediate sizes are multiples of 64 (H=%lld I=%lld)", (long long)H,
@@ -100,16 +175,19 @@ extern "C" int im_moe_mlp(const void* gate_up, const void* down, const uint16_t*
   IM_REQUIRE(gate_up && down && x && y, IM_INVALID, "im_moe_mlp: null pointer");
   IM_REQUIRE(aligned(gate_up, 16) && aligned(down, 16) && aligned(x, 16) && aligned(y, 2), IM_INVALID,
              "im_moe_mlp: weights and x must be 16-byte aligned");
-  const size_t need = im_moe_mlp_workspace_bytes(M, E, top_k, H, I);
+  const size_t need = im_moe_mlp_workspace_bytes(M, E, top_k, H, I, path);
   IM_REQUIRE(workspace && aligned(workspace, 256) && workspace_bytes >= need, IM_INVALID,
              "im_moe_mlp: workspace of %zu bytes (256-aligned) needed, %zu given", need, workspace_bytes);
-  const MoePlan p = moe_plan(M, E, top_k);
+  const MoePlan p = moe_plan(M, E, top_k, path);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const bool tc = p.item_rows == MOE_TC_ROWS;
+  const MoeTcSpace space = tc ? moe_tc_space(M, H, M * top_k, I) : MoeTcSpace{};
   // the gated activations lie in the order of the sorted pairs, so that an item's rows are contiguous
+  uint16_t* hidden = reinterpret_cast<uint16_t*>(reinterpret_cast<char*>(workspace) + space.h16);
   MoeProduct a = {};
   a.wp = reinterpret_cast<const unsigned char*>(gate_up);
   a.x = x;
-  a.y = reinterpret_cast<uint16_t*>(workspace);
+  a.y = hidden;
   a.plan = reinterpret_cast<const int*>(plan);
   a.pairs = pairs;
   a.M = (int)M;
@@ -120,10 +198,12 @@ extern "C" int im_moe_mlp(const void* gate_up, const void* down, const uint16_t*
   a.src = MOE_BY_TOKEN;
   a.dst = MOE_SORTED;
   a.epilogue = activation;
-  const int first = moe_product(p, a, st);
-  if (first) return first;
+  int status = IM_OK;
+  if (tc) status = moe_prep_launch(x, M, H, space, workspace, st);
+  if (!status) status = tc ? moe_tc_launch(p, a, space, workspace, st) : moe_mma_launch(p, a, st);
+  if (status) return status;
   a.wp = reinterpret_cast<const unsigned char*>(down);
-  a.x = reinterpret_cast<const uint16_t*>(workspace);
+  a.x = hidden;
   a.y = y;
   a.N = (int)H;
   a.K = (int)I;
@@ -132,5 +212,5 @@ extern "C" int im_moe_mlp(const void* gate_up, const void* down, const uint16_t*
   a.epilogue = IM_EPI_STORE;
   // the first product waited for the routing before its CTAs let this launch begin
   a.early = 1;
-  return moe_product(p, a, st);
+  return tc ? moe_tc_launch(p, a, space, workspace, st) : moe_mma_launch(p, a, st);
 }

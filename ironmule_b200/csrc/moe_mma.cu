@@ -1,8 +1,7 @@
-// Products by expert for few rows an expert: y[p] = W[e(p)] x[.] over 4-bit weights in packed units (32-row tiles x
-// 64-wide groups, the layout of the packed qGEMM), on warp-level tensor-core MMA.
+// Products by expert for few rows an expert: y[p] = W[e(p)] x[.] over packed 4-bit weights, on warp-level tensor-core MMA.
 //
-// An item is up to 8 NT rows of one expert. A CTA is 4 warps = 4 consecutive tiles (128 outputs) of an item; each warp
-// streams its tile's contiguous 1152-byte units through a register ring, expands the codes to exact bf16 (128 + q) and
+// An item is up to 8 NT rows of one expert. A CTA is 4 warps = the 4 tiles (128 outputs) of a packed block; each warp
+// streams its tile's part of the block's groups through a register ring, expands the codes to exact bf16 (128 + q) and
 // folds each group's affine in float32: tot += s acc + (b - 128 s) sum(x). The item's input rows are gathered by index
 // into shared memory as MMA fragments, one K segment at a time.
 //
@@ -15,7 +14,6 @@
 // before the routing is known; the second product of a gated MLP knows it and fetches before its dependency wait.
 #include "common.cuh"
 #include "moe.cuh"
-#include "qgemm_packed.cuh"
 #include "../../include/imspec.h"
 
 namespace im {
@@ -117,22 +115,27 @@ __global__ void __launch_bounds__(MM_THREADS, NT == 1 ? 4 : 2) moe_mma_kernel(Mm
   }
 
   const int seg0 = SPLIT ? blockIdx.y : 0, seg1 = SPLIT ? seg0 + 1 : a.segs;
-  const unsigned char* wtile = a.p.wp + (size_t)item.x * a.expert_bytes + (size_t)(live ? tile : 0) * G * Q4_UNIT;
-  uint4 rc0[MM_DEPTH], rc1[MM_DEPTH], rsb[MM_DEPTH];
+  const unsigned char* wblock =
+      a.p.wp + (size_t)item.x * a.expert_bytes + (size_t)blockIdx.x * G * MOE_BLOCK_BYTES;
+  // this lane's 8 bytes (words 2t, 2t + 1 of the group) of rows g + 8 j: + 128 j; its scales and biases
+  const int code_off = warp * 1024 + (t >> 1) * 512 + g * 16 + (t & 1) * 8, sb_off = 4096 + warp * 128 + g * 16;
+  uint2 rc[MM_DEPTH][4];
+  uint4 rsb[MM_DEPTH];
+  auto fetch = [&](const unsigned char* p, uint2 (&c)[4], uint4& sb) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) c[j] = ldg_stream_u2(p + code_off + 128 * j);
+    sb = __ldg(reinterpret_cast<const uint4*>(p + sb_off));
+  };
   // the first units of a segment into the register ring, the rest of it towards L2
   auto begin = [&](int seg) {
     const int cg0 = (int)((long long)G * seg / a.segs), ng = (int)((long long)G * (seg + 1) / a.segs) - cg0;
-    const unsigned char* up = wtile + (size_t)cg0 * Q4_UNIT;
+    const unsigned char* up = wblock + (size_t)cg0 * MOE_BLOCK_BYTES;
+    if (threadIdx.x == 0 && ng > MM_DEPTH)
+      mm_prefetch_l2(up + MM_DEPTH * MOE_BLOCK_BYTES, (uint32_t)(ng - MM_DEPTH) * MOE_BLOCK_BYTES);
     if (!live) return;
-    if (lane == 0 && ng > MM_DEPTH) mm_prefetch_l2(up + MM_DEPTH * Q4_UNIT, (uint32_t)(ng - MM_DEPTH) * Q4_UNIT);
 #pragma unroll
-    for (int d = 0; d < MM_DEPTH; d++) {
-      if (d < ng) {
-        rc0[d] = ldg_stream_u4(up + d * Q4_UNIT + lane * 32);
-        rc1[d] = ldg_stream_u4(up + d * Q4_UNIT + lane * 32 + 16);
-        rsb[d] = __ldg(reinterpret_cast<const uint4*>(up + d * Q4_UNIT + 1024 + g * 16));
-      }
-    }
+    for (int d = 0; d < MM_DEPTH; d++)
+      if (d < ng) fetch(up + (size_t)d * MOE_BLOCK_BYTES, rc[d], rsb[d]);
   };
   begin(seg0);
   if (threadIdx.x < 8 * NT && (int)threadIdx.x < rows) {
@@ -200,15 +203,11 @@ __global__ void __launch_bounds__(MM_THREADS, NT == 1 ? 4 : 2) moe_mma_kernel(Mm
       for (int nt = 0; nt < NT; nt++)
 #pragma unroll
         for (int e = 0; e < 4; e++) tot[tt][nt][e] = 0.f;
-    const unsigned char* up = wtile + (size_t)cg0 * Q4_UNIT;
-    auto unit = [&](const int gl, uint4& r0, uint4& r1, uint4& rb) {
-      const uint4 c0 = r0, c1 = r1, sb = rb;
-      if (gl + MM_DEPTH < ng) {
-        const unsigned char* nu = up + (size_t)(gl + MM_DEPTH) * Q4_UNIT;
-        r0 = ldg_stream_u4(nu + lane * 32);
-        r1 = ldg_stream_u4(nu + lane * 32 + 16);
-        rb = __ldg(reinterpret_cast<const uint4*>(nu + 1024 + g * 16));
-      }
+    const unsigned char* up = wblock + (size_t)cg0 * MOE_BLOCK_BYTES;
+    auto unit = [&](const int gl, uint2 (&r)[4], uint4& rb) {
+      const uint2 c[4] = {r[0], r[1], r[2], r[3]};
+      const uint4 sb = rb;
+      if (gl + MM_DEPTH < ng) fetch(up + (size_t)(gl + MM_DEPTH) * MOE_BLOCK_BYTES, r, rb);
       uint32_t px[NT][8];
       float sx[NT][2];
 #pragma unroll
@@ -222,7 +221,7 @@ __global__ void __launch_bounds__(MM_THREADS, NT == 1 ? 4 : 2) moe_mma_kernel(Mm
       }
       const float sv[4] = {bf_lo(sb.x), bf_hi(sb.x), bf_lo(sb.y), bf_hi(sb.y)};
       const float bv[4] = {bf_lo(sb.z), bf_hi(sb.z), bf_lo(sb.w), bf_hi(sb.w)};
-      const uint32_t wd[2][4] = {{c0.x, c0.y, c0.z, c0.w}, {c1.x, c1.y, c1.z, c1.w}};
+      const uint32_t wd[2][4] = {{c[0].x, c[0].y, c[1].x, c[1].y}, {c[2].x, c[2].y, c[3].x, c[3].y}};
 #pragma unroll
       for (int tt = 0; tt < 2; tt++) {
         uint32_t pa[8], pb[8];
@@ -257,7 +256,7 @@ __global__ void __launch_bounds__(MM_THREADS, NT == 1 ? 4 : 2) moe_mma_kernel(Mm
 #pragma unroll
         for (int d = 0; d < MM_DEPTH; d++) {
           if (gl0 + d >= ng) break;
-          unit(gl0 + d, rc0[d], rc1[d], rsb[d]);
+          unit(gl0 + d, rc[d], rsb[d]);
         }
       }
     }
@@ -386,8 +385,8 @@ int moe_mma_launch(const MoePlan& p, const MoeProduct& prod, cudaStream_t st) {
   a.items = reinterpret_cast<const int4*>(prod.plan + MOE_PLAN_HEADER);
   const int G = prod.K / 64;
   a.tiles = (prod.N + 31) / 32;
-  a.expert_bytes = (size_t)a.tiles * G * Q4_UNIT;
   const int ctas_x = (a.tiles + MM_WARPS - 1) / MM_WARPS;
+  a.expert_bytes = (size_t)ctas_x * G * MOE_BLOCK_BYTES;
   a.segs = mm_segments(ctas_x, G);
   a.rg = (G + a.segs - 1) / a.segs;
   // one segment per CTA while the grid still fits one wave of CTAs; beyond, a CTA walks its item's segments

@@ -40,12 +40,15 @@ struct RouteArgs {
   long long ld;
 };
 
-MoePlan moe_plan(int64_t M, int64_t E, int64_t top_k) {
+MoePlan moe_plan(int64_t M, int64_t E, int64_t top_k, int path) {
   MoePlan p;
   const int64_t pairs = M * top_k;
   // rows per item by the average number of rows an expert gets; an expert never gets more than M
   const int64_t avg = (pairs + E - 1) / E;
-  p.item_rows = M <= 8 || avg <= 4 ? 8 : (M <= 16 || avg <= 12 ? 16 : 32);
+  if (path == IM_MOE_TENSOR || (path == IM_MOE_AUTO && M > 8 && avg > 4))
+    p.item_rows = MOE_TC_ROWS;
+  else
+    p.item_rows = M <= 8 || avg <= 4 ? 8 : (M <= 16 || avg <= 12 ? 16 : 32);
   const int64_t buckets = pairs < E + 1 ? pairs : E + 1;
   p.max_items = buckets + pairs / p.item_rows;
   const int64_t per = (M + MOE_ROUTE_BLOCKS - 1) / MOE_ROUTE_BLOCKS;
@@ -314,13 +317,14 @@ static bool moe_sizes_ok(int64_t M, int64_t E, int64_t top_k) {
          top_k <= E;
 }
 
-extern "C" size_t im_moe_plan_bytes(int64_t M, int64_t E, int64_t top_k) {
-  return moe_sizes_ok(M, E, top_k) ? moe_plan(M, E, top_k).bytes : 0;
+extern "C" size_t im_moe_plan_bytes(int64_t M, int64_t E, int64_t top_k, int path) {
+  return moe_sizes_ok(M, E, top_k) && path >= IM_MOE_AUTO && path <= IM_MOE_TENSOR ? moe_plan(M, E, top_k, path).bytes
+                                                                                   : 0;
 }
 
 extern "C" int im_moe_route(const void* logits, int logits_f32, int64_t M, int64_t E, int64_t ld, const float* bias,
                             int64_t top_k, int scoring, int normalise, float scale, int32_t* ids, float* weights,
-                            int32_t* offsets, int32_t* pairs, void* plan, size_t plan_bytes, void* stream) {
+                            int32_t* offsets, int32_t* pairs, int path, void* plan, size_t plan_bytes, void* stream) {
   clear_error();
   IM_REQUIRE(M >= 0 && E >= 1 && top_k >= 1 && top_k <= E, IM_INVALID,
              "im_moe_route: bad sizes M=%lld E=%lld top_k=%lld", (long long)M, (long long)E, (long long)top_k);
@@ -328,12 +332,13 @@ extern "C" int im_moe_route(const void* logits, int logits_f32, int64_t M, int64
              "im_moe_route: at most %lld rows, %d experts and %d places a row (M=%lld E=%lld top_k=%lld)",
              (long long)MOE_MAX_ROWS, MOE_MAX_EXPERTS, MOE_MAX_TOP_K, (long long)M, (long long)E, (long long)top_k);
   IM_REQUIRE(scoring == IM_MOE_SOFTMAX || scoring == IM_MOE_SIGMOID, IM_INVALID, "im_moe_route: bad scoring");
+  IM_REQUIRE(path >= IM_MOE_AUTO && path <= IM_MOE_TENSOR, IM_INVALID, "im_moe_route: bad path");
   IM_REQUIRE(offsets && plan, IM_INVALID, "im_moe_route: null pointer");
   IM_REQUIRE(M == 0 || (logits && ids && weights && pairs), IM_INVALID, "im_moe_route: null pointer");
   IM_REQUIRE(ld >= E, IM_INVALID, "im_moe_route: row stride %lld below %lld experts", (long long)ld, (long long)E);
   IM_REQUIRE(aligned(logits, logits_f32 ? 4 : 2) && aligned(plan, 16), IM_INVALID,
              "im_moe_route: misaligned logits or plan");
-  const MoePlan p = moe_plan(M, E, top_k);
+  const MoePlan p = moe_plan(M, E, top_k, path);
   IM_REQUIRE(plan_bytes >= p.bytes, IM_INVALID, "im_moe_route: plan of %zu bytes needed, %zu given", p.bytes,
              plan_bytes);
   RouteArgs a = {};

@@ -32,6 +32,7 @@
 // then waits (bounded) for its own bulk copies and MMAs in flight before it frees its tensor memory and exits.
 #include "common.cuh"
 #include "qgemm_packed.cuh"
+#include "tc.cuh"
 #include "../../include/imspec.h"
 
 namespace im {
@@ -58,7 +59,6 @@ constexpr int QT_SBB = 4 * 128;           // a group's scales and biases of the 
 constexpr size_t QT_OFF_SB = QT_OFF_SX + (size_t)QT_SR * QT_N * 4;
 constexpr size_t QT_OFF_BAR = QT_OFF_SB + (size_t)QT_SR * QT_SBB;
 constexpr size_t QT_SMEM = 1024 + QT_OFF_BAR + (size_t)QT_BARS * 8 + 16;
-constexpr unsigned long long QT_WAIT_NS = 1000000000ull;
 constexpr uint32_t QT_128 = 0x43004300u;
 
 struct QtArgs {
@@ -101,80 +101,12 @@ __device__ __forceinline__ bool qt_next(const QtArgs& a, QtCursor& c) {
   return true;
 }
 
-__device__ __forceinline__ uint32_t qt_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-__device__ __forceinline__ bool qt_try_wait(uint32_t bar, uint32_t parity) {
-  uint32_t done;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
-      : "=r"(done)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return done != 0;
-}
-
-// The same with a suspend-time hint: the thread sleeps (up to 20 us) instead of spinning until the phase completes.
-__device__ __forceinline__ bool qt_try_wait_sleep(uint32_t bar, uint32_t parity) {
-  uint32_t done;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
-      : "=r"(done)
-      : "r"(bar), "r"(parity), "r"(20000u)
-      : "memory");
-  return done != 0;
-}
-
 // d = a * b + d on two fp32 lanes at once, each rounded once to nearest (the same bits as two fmaf).
 __device__ __forceinline__ void qt_fma2(float& d0, float& d1, float a0, float a1, float b0, float b1) {
   asm("{\n\t.reg .b64 ra, rb, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tmov.b64 rd, {%0, %1};\n\t"
       "fma.rn.f32x2 rd, ra, rb, rd;\n\tmov.b64 {%0, %1}, rd;\n\t}"
       : "+f"(d0), "+f"(d1)
       : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
-}
-
-__device__ __forceinline__ unsigned long long qt_clock() {
-  unsigned long long t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-  return t;
-}
-
-// Bounded wait for the phase of `parity`; false when this CTA has given up (now or earlier).
-__device__ __forceinline__ bool qt_wait(unsigned long long* bar, uint32_t parity, volatile int* abort_flag,
-                                        unsigned* error) {
-  const uint32_t b = qt_smem(bar);
-  if (*abort_flag) return false;
-  if (qt_try_wait(b, parity)) return true;
-  const unsigned long long t0 = qt_clock();
-  while (true) {
-    if (qt_try_wait_sleep(b, parity)) return true;
-    if (*abort_flag) return false;
-    if (qt_clock() - t0 > QT_WAIT_NS) {
-      *abort_flag = 1;
-      atomicExch(error, 1u);
-      return false;
-    }
-  }
-}
-
-// Bounded wait that ignores the abort flag (draining copies and MMAs already in flight).
-__device__ __forceinline__ void qt_drain(unsigned long long* bar, uint32_t parity) {
-  const uint32_t b = qt_smem(bar);
-  const unsigned long long t0 = qt_clock();
-  while (!qt_try_wait(b, parity) && qt_clock() - t0 < QT_WAIT_NS) {
-  }
-}
-
-__device__ __forceinline__ void qt_arrive(unsigned long long* bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(qt_smem(bar)) : "memory");
-}
-
-__device__ __forceinline__ void qt_init(unsigned long long* bar, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(qt_smem(bar)), "r"(count));
-}
-
-__device__ __forceinline__ uint64_t qt_desc(uint32_t saddr) {
-  // K-major, 128-byte swizzle: 8-row groups 1024 bytes apart (SBO), leading offset 1 (unused), version 1
-  return (uint64_t)((saddr >> 4) & 0x3FFFu) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
 }
 
 // instruction descriptor: f32 accumulate, bf16 A and B, both K-major, N = n, M = 128

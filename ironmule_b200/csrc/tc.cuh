@@ -1,0 +1,78 @@
+// Bounded mbarrier waits and the shared-memory descriptor of the tcgen05 kernels.
+#pragma once
+
+#include <cstdint>
+
+namespace im {
+
+constexpr unsigned long long QT_WAIT_NS = 1000000000ull;
+
+__device__ __forceinline__ uint32_t qt_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ bool qt_try_wait(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+
+// The same with a suspend-time hint: the thread sleeps (up to 20 us) instead of spinning until the phase completes.
+__device__ __forceinline__ bool qt_try_wait_sleep(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(done)
+      : "r"(bar), "r"(parity), "r"(20000u)
+      : "memory");
+  return done != 0;
+}
+
+__device__ __forceinline__ unsigned long long qt_clock() {
+  unsigned long long t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  return t;
+}
+
+// Bounded wait for the phase of `parity`; false when this CTA has given up (now or earlier).
+__device__ __forceinline__ bool qt_wait(unsigned long long* bar, uint32_t parity, volatile int* abort_flag,
+                                        unsigned* error) {
+  const uint32_t b = qt_smem(bar);
+  if (*abort_flag) return false;
+  if (qt_try_wait(b, parity)) return true;
+  const unsigned long long t0 = qt_clock();
+  while (true) {
+    if (qt_try_wait_sleep(b, parity)) return true;
+    if (*abort_flag) return false;
+    if (qt_clock() - t0 > QT_WAIT_NS) {
+      *abort_flag = 1;
+      atomicExch(error, 1u);
+      return false;
+    }
+  }
+}
+
+// Bounded wait that ignores the abort flag (draining copies and MMAs already in flight).
+__device__ __forceinline__ void qt_drain(unsigned long long* bar, uint32_t parity) {
+  const uint32_t b = qt_smem(bar);
+  const unsigned long long t0 = qt_clock();
+  while (!qt_try_wait(b, parity) && qt_clock() - t0 < QT_WAIT_NS) {
+  }
+}
+
+__device__ __forceinline__ void qt_arrive(unsigned long long* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(qt_smem(bar)) : "memory");
+}
+
+__device__ __forceinline__ void qt_init(unsigned long long* bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(qt_smem(bar)), "r"(count));
+}
+
+__device__ __forceinline__ uint64_t qt_desc(uint32_t saddr) {
+  // K-major, 128-byte swizzle: 8-row groups 1024 bytes apart (SBO), leading offset 1 (unused), version 1
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+
+}  // namespace im

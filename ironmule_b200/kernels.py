@@ -503,10 +503,11 @@ def qgemm_packed_attn(attn_ws: torch.Tensor, p: Packed, seq_rows: torch.Tensor, 
 
 # ---- mixture-of-experts blocks ------------------------------------------------------------------------------
 _SCORING = {"softmax": _lib.MOE_SOFTMAX, "sigmoid": _lib.MOE_SIGMOID}
+_PATHS = {"auto": _lib.MOE_AUTO, "warp": _lib.MOE_WARP, "tensor": _lib.MOE_TENSOR}
 
 
 class Experts:
-    """E 4-bit matrices [N, K] of one shape, repacked once into MMA-fragment order: w int32 [E, N, K/8], scales and
+    """E 4-bit matrices [N, K] of one shape, repacked once for the products by expert: w int32 [E, N, K/8], scales and
     biases bf16 [E, N, K/64] (MLX's layout of stacked experts)."""
 
     def __init__(self, w: torch.Tensor, scales: torch.Tensor, biases: torch.Tensor):
@@ -550,17 +551,27 @@ class Routing:
     rows: int
     experts: int
     top_k: int
+    path: str
+
+    def status(self) -> int:
+        """The error word of the products that used this routing (0: every bounded wait completed); synchronises."""
+        return int(_lib.load().im_moe_status(self.plan.data_ptr()))
 
 
 def moe_route(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax", normalise: bool = True,
-              scale: float = 1.0, bias: torch.Tensor | None = None, rows: int | None = None) -> Routing:
+              scale: float = 1.0, bias: torch.Tensor | None = None, rows: int | None = None,
+              path: str = "auto") -> Routing:
     """Choose top_k experts for each of the first `rows` rows of logits [M, E] (bf16 or float32): the largest
-    logit + bias, ties to the lower expert; -inf or NaN closes an expert to a row."""
+    logit + bias, ties to the lower expert; -inf or NaN closes an expert to a row. `path`: the kernel of the products
+    that use the routing, "warp" or "tensor"; "auto" chooses by the sizes. Within one kernel a row's results do not
+    depend on the other rows."""
     _check(logits, "logits", (torch.bfloat16, torch.float32))
     if logits.dim() != 2:
         raise ValueError(f"logits must be [M, E], got {tuple(logits.shape)}")
     if scoring not in _SCORING:
         raise ValueError(f"scoring {scoring!r}: softmax or sigmoid")
+    if path not in _PATHS:
+        raise ValueError(f"path {path!r}: auto, warp or tensor")
     device, e = logits.device, logits.shape[1]
     m = logits.shape[0] if rows is None else rows
     if not 0 <= m <= logits.shape[0]:
@@ -575,12 +586,12 @@ def moe_route(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax", nor
     weights = torch.empty((m, top_k), dtype=torch.float32, device=device)
     offsets = torch.empty(e + 2, dtype=torch.int32, device=device)
     pairs = torch.empty(m * top_k, dtype=torch.int32, device=device)
-    nbytes = int(_lib.load().im_moe_plan_bytes(m, e, top_k))
+    nbytes = int(_lib.load().im_moe_plan_bytes(m, e, top_k, _PATHS[path]))
     plan = torch.empty((nbytes + 3) // 4, dtype=torch.int32, device=device)
     _lib.call("im_moe_route", logits.data_ptr(), int(logits.dtype == torch.float32), m, e, e, _ptr_or_none(bias), top_k,
               _SCORING[scoring], int(normalise), float(scale), ids.data_ptr(), weights.data_ptr(), offsets.data_ptr(),
-              pairs.data_ptr(), plan.data_ptr(), nbytes, _stream(device))
-    return Routing(ids, weights, offsets, pairs, plan, m, e, top_k)
+              pairs.data_ptr(), _PATHS[path], plan.data_ptr(), nbytes, _stream(device))
+    return Routing(ids, weights, offsets, pairs, plan, m, e, top_k, path)
 
 
 def _moe_rows(x: torch.Tensor, experts: Experts, routing: Routing) -> bool:
@@ -614,9 +625,13 @@ def grouped_qgemm(x: torch.Tensor, experts: Experts, routing: Routing, *,
     places without an expert."""
     by_pair = _moe_rows(x, experts, routing)
     out = _moe_out(out, (routing.rows, routing.top_k, experts.n), x.device)
+    path = _PATHS[routing.path]
+    need = int(_lib.load().im_moe_grouped_workspace_bytes(routing.rows, experts.e, routing.top_k, experts.k,
+                                                          int(by_pair), path))
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device)
     _lib.call("im_moe_grouped_qgemm", experts.data.data_ptr(), x.data_ptr(), out.data_ptr(), routing.rows, experts.e,
-              routing.top_k, experts.n, experts.k, int(by_pair), routing.pairs.data_ptr(), routing.plan.data_ptr(),
-              routing.plan.numel() * 4, _stream(x.device))
+              routing.top_k, experts.n, experts.k, int(by_pair), routing.pairs.data_ptr(), path,
+              routing.plan.data_ptr(), routing.plan.numel() * 4, ws.data_ptr(), need, _stream(x.device))
     return out
 
 
@@ -632,11 +647,12 @@ def moe_mlp(x: torch.Tensor, gate_up: Experts, down: Experts, routing: Routing, 
     if (down.e, down.n, down.k) != (gate_up.e, h, inter) or down.data.device != x.device:
         raise ValueError(f"down is {down.e} x [{down.n}, {down.k}], expected {gate_up.e} x [{h}, {inter}]")
     out = _moe_out(out, (routing.rows, routing.top_k, h), x.device)
-    need = int(_lib.load().im_moe_mlp_workspace_bytes(routing.rows, gate_up.e, routing.top_k, h, inter))
+    need = int(_lib.load().im_moe_mlp_workspace_bytes(routing.rows, gate_up.e, routing.top_k, h, inter,
+                                                      _PATHS[routing.path]))
     ws = torch.empty(need, dtype=torch.uint8, device=x.device)
     _lib.call("im_moe_mlp", gate_up.data.data_ptr(), down.data.data_ptr(), x.data_ptr(), out.data_ptr(), routing.rows,
               gate_up.e, routing.top_k, h, inter, _EPILOGUES[activation], routing.pairs.data_ptr(),
-              routing.plan.data_ptr(), routing.plan.numel() * 4, ws.data_ptr(), need, _stream(x.device))
+              _PATHS[routing.path], routing.plan.data_ptr(), routing.plan.numel() * 4, ws.data_ptr(), need, _stream(x.device))
     return out
 
 
