@@ -39,7 +39,6 @@ namespace im {
 constexpr int MT_N = MOE_TC_ROWS;       // rows of an item at most (MMA N)
 constexpr int MT_S = 8;                 // A and B stages
 constexpr int MT_W = 12;                // weight ring
-constexpr int MT_LAG = 5;               // B stages whose copies are in flight
 constexpr int MT_B = MT_N * 128;        // bytes of a B stage
 constexpr int MT_W_LOAD = 6, MT_W_TRANS = 10;  // first gather and expansion warps
 constexpr int MT_THREADS = 18 * 32;
@@ -47,7 +46,9 @@ constexpr uint32_t MT_TMEM = 512;       // 2 accumulators of 128 columns, 8 A st
 constexpr int MT_A0 = 256;
 constexpr size_t MT_OFF_W = (size_t)MT_S * MT_B;
 constexpr size_t MT_OFF_BAR = MT_OFF_W + (size_t)MT_W * MOE_BLOCK_BYTES;
-constexpr int MT_BARS = 3 * MT_S + 2 * MT_W + 4;
+// barriers: a stage's MMAs completed; a stage's A and B in place; weight ring; accumulators
+constexpr int MT_DONE = 0, MT_FULL = MT_DONE + MT_S, MT_W_FULL = MT_FULL + MT_S, MT_W_EMPTY = MT_W_FULL + MT_W,
+              MT_D_FULL = MT_W_EMPTY + MT_W, MT_D_EMPTY = MT_D_FULL + 2, MT_BARS = MT_D_EMPTY + 2;
 constexpr size_t MT_SMEM = 1024 + MT_OFF_BAR + MT_BARS * 8 + 16;
 
 struct TcArgs {
@@ -159,23 +160,25 @@ __device__ __forceinline__ float mt_gated(bool geglu, float g, float u) {
   return 0.5f * g * (1.0f + tanhf(inner)) * u;
 }
 
+__device__ __forceinline__ void mt_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+__device__ __forceinline__ void mt_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+
 template <bool GLU>
 __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
   extern __shared__ unsigned char mt_raw[];
   const uint32_t raw = qt_smem(mt_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   unsigned char* sbase = mt_raw + (base - raw);
-  unsigned long long* done = reinterpret_cast<unsigned long long*>(sbase + MT_OFF_BAR);  // a stage's MMAs completed
-  unsigned long long* a_full = done + MT_S;
-  unsigned long long* b_full = a_full + MT_S;
-  unsigned long long* w_full = b_full + MT_S;
-  unsigned long long* w_empty = w_full + MT_W;
-  unsigned long long* d_full = w_empty + MT_W;
-  unsigned long long* d_empty = d_full + 2;
-  uint32_t* holder = reinterpret_cast<uint32_t*>(d_empty + 2);
+  const uint32_t bars = base + (uint32_t)MT_OFF_BAR;
+  uint32_t* holder = reinterpret_cast<uint32_t*>(sbase + MT_OFF_BAR + MT_BARS * 8);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(holder + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int G = a.p.K >> 6;
   const int nout = GLU ? a.p.N >> 1 : a.p.N;
 
@@ -185,18 +188,18 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   if (threadIdx.x == 0) {
+    unsigned long long* b = reinterpret_cast<unsigned long long*>(sbase + MT_OFF_BAR);
     for (int s = 0; s < MT_S; s++) {
-      qt_init(&done[s], 1u);
-      qt_init(&a_full[s], 4u);
-      qt_init(&b_full[s], 4u);
+      qt_init(&b[MT_DONE + s], 1u);
+      qt_init(&b[MT_FULL + s], 4u + 128u);  // four expansion warps, every gather thread
     }
     for (int s = 0; s < MT_W; s++) {
-      qt_init(&w_full[s], 1u);
-      qt_init(&w_empty[s], 4u);
+      qt_init(&b[MT_W_FULL + s], 1u);
+      qt_init(&b[MT_W_EMPTY + s], 4u);
     }
     for (int s = 0; s < 2; s++) {
-      qt_init(&d_full[s], 1u);
-      qt_init(&d_empty[s], 4u);
+      qt_init(&b[MT_D_FULL + s], 1u);
+      qt_init(&b[MT_D_EMPTY + s], 4u);
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -212,73 +215,76 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
   if (warp == 0) {
     // ---- weights -------------------------------------------------------------------------------------------
     if (lane == 0) {
+      uint32_t s = 0, phase = 0;
       int k = 0;
-      bool ok = true;
-      for (int tile = blockIdx.x; ok && tile < ntiles; tile += gridDim.x) {
+      for (int tile = blockIdx.x; tile < ntiles; tile += gridDim.x) {
         const int expert = a.items[tile / a.cols].x;
         if (expert == a.p.E) continue;
         const unsigned char* src =
             a.p.wp + (size_t)expert * a.expert_bytes + (size_t)(tile % a.cols) * G * MOE_BLOCK_BYTES;
         for (int g = 0; g < G; g++, k++) {
-          const int s = k % MT_W;
-          if (k >= MT_W && !qt_wait(&w_empty[s], (uint32_t)((k / MT_W - 1) & 1), abort_flag, a.error)) {
-            ok = false;
-            break;
-          }
-          asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(qt_smem(&w_full[s])),
+          const uint32_t full = bars + 8 * (MT_W_FULL + s);
+          if (!qt_wait_short(bars + 8 * (MT_W_EMPTY + s), phase ^ 1u, abort_flag, a.error)) goto weights_done;
+          asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full),
                        "r"((uint32_t)MOE_BLOCK_BYTES)
                        : "memory");
           asm volatile(
               "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                  base + (uint32_t)(MT_OFF_W + (size_t)s * MOE_BLOCK_BYTES)),
-              "l"(src + (size_t)g * MOE_BLOCK_BYTES), "r"((uint32_t)MOE_BLOCK_BYTES), "r"(qt_smem(&w_full[s]))
+                  base + (uint32_t)MT_OFF_W + s * MOE_BLOCK_BYTES),
+              "l"(src), "r"((uint32_t)MOE_BLOCK_BYTES), "r"(full)
               : "memory");
+          src += MOE_BLOCK_BYTES;
+          if (++s == MT_W) s = 0, phase ^= 1u;
         }
       }
+    weights_done:
       if (*abort_flag)  // copies still landing in this CTA's shared memory finish before it exits
-        for (int j = k > MT_W ? k - MT_W : 0; j < k; j++) qt_drain(&w_full[j % MT_W], (uint32_t)((j / MT_W) & 1));
+        for (int j = k > MT_W ? k - MT_W : 0; j < k; j++)
+          qt_drain(reinterpret_cast<unsigned long long*>(sbase + MT_OFF_BAR) + MT_W_FULL + j % MT_W,
+                   (uint32_t)((j / MT_W) & 1));
     }
   } else if (warp == 1) {
     // ---- MMA issue -----------------------------------------------------------------------------------------
-    if (lane == 0) {
-      int k = 0, t = 0;
-      bool ok = true;
-      for (int tile = blockIdx.x; ok && tile < ntiles; tile += gridDim.x) {
-        const int4 item = a.items[tile / a.cols];
-        if (item.x == a.p.E) continue;
-        // f32 accumulate, f16 A and B, K-major, N = the item's rows in sixteens, M = 128
-        const uint32_t idesc = (1u << 4) | ((uint32_t)((item.z + 15) / 16 * 2) << 17) | ((128u >> 4) << 24);
-        const int buf = t & 1;
-        if (t >= 2 && !qt_wait(&d_empty[buf], (uint32_t)((t / 2 - 1) & 1), abort_flag, a.error)) break;
-        const uint32_t d = tmem + (uint32_t)(buf * MT_N);
-        for (int g = 0; g < G; g++, k++) {
-          const int s = k % MT_S;
-          const uint32_t parity = (uint32_t)((k / MT_S) & 1);
-          if (!qt_wait(&b_full[s], parity, abort_flag, a.error) || !qt_wait(&a_full[s], parity, abort_flag, a.error)) {
-            ok = false;
-            break;
-          }
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    // (the whole warp walks the loop, so that its addresses stay in uniform registers; one lane issues)
+    const bool leader = qt_elect();
+    uint32_t s = 0, phase = 0;
+    int k = 0, t = 0;
+    for (int tile = blockIdx.x; tile < ntiles; tile += gridDim.x) {
+      const int4 item = a.items[tile / a.cols];
+      if (item.x == a.p.E) continue;
+      // f32 accumulate, f16 A and B, K-major, N = the item's rows in sixteens, M = 128
+      const uint32_t idesc = (1u << 4) | ((uint32_t)((item.z + 15) / 16 * 2) << 17) | ((128u >> 4) << 24);
+      const int buf = t & 1;
+      if (!qt_wait_short(bars + 8 * (MT_D_EMPTY + buf), (uint32_t)((t / 2 + 1) & 1), abort_flag, a.error)) break;
+      const uint32_t d = tmem + (uint32_t)(buf * MT_N);
+      int g = 0;
+      for (; g < G; g++, k++) {
+        if (!qt_wait_short(bars + 8 * (MT_FULL + s), phase, abort_flag, a.error)) break;
+        // the gathered rows were written through the generic proxy; the MMA reads them through the async one
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (leader) {
+          const uint64_t bd = qt_desc(base + s * MT_B);
+          const uint32_t ta = tmem + MT_A0 + 32 * s;
 #pragma unroll
-          for (int q = 0; q < 4; q++) {
-            const uint64_t bd = qt_desc(base + (uint32_t)(s * MT_B + 32 * q));
+          for (int q = 0; q < 4; q++)
             asm volatile(
                 "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
-                "r"(tmem + (uint32_t)(MT_A0 + 32 * s + 8 * q)), "l"(bd), "r"(idesc), "r"((uint32_t)(g + q > 0)));
-          }
-          asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                           qt_smem(&done[s]))
-                       : "memory");
+                "r"(ta + 8 * q), "l"(bd + 2 * q), "r"(idesc), "r"((uint32_t)(g + q > 0)));
+          mt_commit(bars + 8 * (MT_DONE + s));
         }
-        if (ok)
-          asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                           qt_smem(&d_full[buf]))
-                       : "memory");
-        t++;
+        __syncwarp();
+        if (++s == MT_S) s = 0, phase ^= 1u;
       }
-      if (*abort_flag && k > 0) qt_drain(&done[(k - 1) % MT_S], (uint32_t)(((k - 1) / MT_S) & 1));
+      if (g < G) break;
+      if (leader) mt_commit(bars + 8 * (MT_D_FULL + buf));
+      __syncwarp();
+      t++;
     }
+    if (*abort_flag && k > 0)
+      qt_drain(reinterpret_cast<unsigned long long*>(sbase + MT_OFF_BAR) + MT_DONE + (k - 1) % MT_S,
+               (uint32_t)(((k - 1) / MT_S) & 1));
   } else if (warp < MT_W_LOAD) {
     // ---- epilogue: thread = output row of the block, columns = the item's rows ---------------------------------
     const int q = warp & 3;
@@ -299,7 +305,7 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
       const int buf = t & 1;
       const float wmax = a.wmax[item.x];
       const float wscale = mt_pow2(mt_exp(wmax, 8));
-      if (!qt_wait(&d_full[buf], (uint32_t)((t / 2) & 1), abort_flag, a.error)) break;
+      if (!qt_wait_short(bars + 8 * (MT_D_FULL + buf), (uint32_t)((t / 2) & 1), abort_flag, a.error)) break;
       t++;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       for (int c0 = 0; c0 < rows; c0 += 32) {
@@ -333,7 +339,7 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
         if (c0 + 32 >= rows) {
           asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
           __syncwarp();
-          if (lane == 0) qt_arrive(&d_empty[buf]);
+          if (lane == 0) mt_arrive(bars + 8 * (MT_D_EMPTY + buf));
         }
         if constexpr (GLU) {
           // lanes 0-15 hold gate features, 16-31 the matching up features: of two columns each half takes one
@@ -368,94 +374,75 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
   } else if (warp < MT_W_TRANS) {
     // ---- gather of B -------------------------------------------------------------------------------------------
     const int th = threadIdx.x - MT_W_LOAD * 32, c = th & 7, r0 = th >> 3;  // 16-byte chunk c of rows r0 + 16 i
-    const uint32_t soff = (uint32_t)(r0 * 128 + ((c ^ (r0 & 7)) << 4));
+    const uint32_t dst0 = base + (uint32_t)(r0 * 128 + ((c ^ (r0 & 7)) << 4));
     pdl_wait();
-    int k = 0;
-    bool ok = true;
-    auto arrive = [&](int step) {
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) qt_arrive(&b_full[step % MT_S]);
-    };
-    for (int tile = blockIdx.x; ok && tile < ntiles; tile += gridDim.x) {
+    uint32_t s = 0, phase = 1;
+    for (int tile = blockIdx.x; tile < ntiles; tile += gridDim.x) {
       const int4 item = a.items[tile / a.cols];
       if (item.x == a.p.E) continue;
       const __half* src[MT_N / 16];
 #pragma unroll
       for (int i = 0; i < MT_N / 16; i++) {
-        const int r = r0 + 16 * i;
-        src[i] = nullptr;
-        if (r < item.z) {
-          const int pos = item.y + r;
-          int row = pos;
-          if (a.p.src != MOE_SORTED) {
-            row = a.p.pairs[pos];
-            if (a.p.src == MOE_BY_TOKEN) row /= a.p.top_k;
-          }
-          src[i] = a.x16 + (size_t)row * a.p.K + 8 * c;
+        const int r = min(r0 + 16 * i, item.z - 1);  // (rows past the item's repeat its last one: columns nobody reads)
+        const int pos = item.y + r;
+        int row = pos;
+        if (a.p.src != MOE_SORTED) {
+          row = a.p.pairs[pos];
+          if (a.p.src == MOE_BY_TOKEN) row /= a.p.top_k;
         }
+        src[i] = a.x16 + (size_t)row * a.p.K + 8 * c;
       }
-      for (int g = 0; g < G; g++, k++) {
-        const int s = k % MT_S;
-        if (k >= MT_S && !qt_wait(&done[s], (uint32_t)((k / MT_S - 1) & 1), abort_flag, a.error)) {
-          ok = false;
-          break;
-        }
-        const uint32_t dst = base + (uint32_t)(s * MT_B) + soff;
+      const int n16 = (item.z + 15) / 16;
+      for (int g = 0; g < G; g++) {
+        if (!qt_wait_short(bars + 8 * (MT_DONE + s), phase, abort_flag, a.error)) goto gather_done;
+        const uint32_t dst = dst0 + s * MT_B;
 #pragma unroll
-        for (int i = 0; i < MT_N / 16; i++)
-          if (src[i])
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + (uint32_t)(i * 2048)),
-                         "l"(src[i] + (size_t)g * 64)
+        for (int i = 0; i < MT_N / 16; i++) {
+          if (i < n16)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + (uint32_t)(i * 2048)), "l"(src[i])
                          : "memory");
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        if (k >= MT_LAG) {
-          asm volatile("cp.async.wait_group %0;" ::"n"(MT_LAG) : "memory");
-          arrive(k - MT_LAG);
+          src[i] += 64;
         }
+        // arrives once this thread's copies have landed
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bars + 8 * (MT_FULL + s)) : "memory");
+        if (++s == MT_S) s = 0, phase ^= 1u;
       }
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-    if (ok)
-      for (int j = k > MT_LAG ? k - MT_LAG : 0; j < k; j++) arrive(j);
+  gather_done:
+    asm volatile("cp.async.wait_all;" ::: "memory");
   } else {
-    // ---- code expansion ------------------------------------------------------------------------------------------
+    // ---- code expansion: set 0 takes the even steps of the CTA's sequence, set 1 the odd ones ---------------------
     const int set = (warp - MT_W_TRANS) >> 2, q = warp & 3;
-    const int g8 = lane & 7, j8 = lane >> 3;
-    int k = 0;
-    bool ok = true;
-    for (int tile = blockIdx.x; ok && tile < ntiles; tile += gridDim.x) {
+    const uint32_t code_off = (uint32_t)(q * 1024 + lane * 16);
+    const uint32_t sb_off = (uint32_t)(4096 + q * 128 + (lane & 7) * 16 + (lane >> 3) * 2);
+    uint32_t s = set, phase = 1, sw = set, wphase = 0;
+    int skip = set;  // steps of the next tile that lie before this set's next one
+    for (int tile = blockIdx.x; tile < ntiles; tile += gridDim.x) {
       const int expert = a.items[tile / a.cols].x;
       if (expert == a.p.E) continue;
       const float inv = mt_pow2(-mt_exp(a.wmax[expert], 8));
-      for (int g = 0; g < G; g++, k++) {
-        if ((k & 1) != set) continue;
-        const int s = k % MT_S, sw = k % MT_W;
-        if (!qt_wait(&w_full[sw], (uint32_t)((k / MT_W) & 1), abort_flag, a.error)) {
-          ok = false;
-          break;
-        }
-        const unsigned char* w = sbase + MT_OFF_W + (size_t)sw * MOE_BLOCK_BYTES;
-        const uint4 c0 = *reinterpret_cast<const uint4*>(w + q * 1024 + lane * 16);
-        const uint4 c1 = *reinterpret_cast<const uint4*>(w + q * 1024 + 512 + lane * 16);
-        const uint16_t* sb = reinterpret_cast<const uint16_t*>(w + 4096 + q * 128 + g8 * 16);
-        const float sf = bf(sb[j8]) * inv, bfv = bf(sb[4 + j8]) * inv;
-        __syncwarp();
-        if (lane == 0) qt_arrive(&w_empty[sw]);
-        const __half2 s2 = __float2half2_rn(sf), b2 = __float2half2_rn(bfv);
+      int g = skip;
+      for (; g < G; g += 2) {
+        if (!qt_wait_short(bars + 8 * (MT_W_FULL + sw), wphase, abort_flag, a.error)) goto expand_done;
+        const unsigned char* w = sbase + MT_OFF_W + sw * MOE_BLOCK_BYTES;
+        const uint4 c0 = *reinterpret_cast<const uint4*>(w + code_off);
+        const uint4 c1 = *reinterpret_cast<const uint4*>(w + code_off + 512);
+        const float sf = bf(*reinterpret_cast<const uint16_t*>(w + sb_off)) * inv;
+        const float of = bf(*reinterpret_cast<const uint16_t*>(w + sb_off + 8)) * inv;
+        const __half2 s2 = __float2half2_rn(sf), b2 = __float2half2_rn(of);
         uint32_t p[32];
         const uint32_t words[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
 #pragma unroll
         for (int i = 0; i < 8; i++) mt_expand(words[i], s2, b2, p + 4 * i);
-        if (k >= MT_S && !qt_wait(&done[s], (uint32_t)((k / MT_S - 1) & 1), abort_flag, a.error)) {
-          ok = false;
-          break;
-        }
+        __syncwarp();
+        if (lane == 0) mt_arrive(bars + 8 * (MT_W_EMPTY + sw));
+        if ((sw += 2) >= MT_W) sw -= MT_W, wphase ^= 1u;
+        if (!qt_wait_short(bars + 8 * (MT_DONE + s), phase, abort_flag, a.error)) goto expand_done;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile(
             "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
             "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(
-                tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(MT_A0 + 32 * s)),
+                tmem + ((uint32_t)(32 * q) << 16) + MT_A0 + 32 * s),
             "r"(p[0]), "r"(p[1]), "r"(p[2]), "r"(p[3]), "r"(p[4]), "r"(p[5]), "r"(p[6]), "r"(p[7]), "r"(p[8]),
             "r"(p[9]), "r"(p[10]), "r"(p[11]), "r"(p[12]), "r"(p[13]), "r"(p[14]), "r"(p[15]), "r"(p[16]),
             "r"(p[17]), "r"(p[18]), "r"(p[19]), "r"(p[20]), "r"(p[21]), "r"(p[22]), "r"(p[23]), "r"(p[24]),
@@ -464,9 +451,12 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncwarp();
-        if (lane == 0) qt_arrive(&a_full[s]);
+        if (lane == 0) mt_arrive(bars + 8 * (MT_FULL + s));
+        if ((s += 2) >= MT_S) s -= MT_S, phase ^= 1u;
       }
+      skip = g - G;
     }
+  expand_done:;
   }
   __syncwarp();
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");

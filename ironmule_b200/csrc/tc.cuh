@@ -54,6 +54,49 @@ __device__ __forceinline__ bool qt_wait(unsigned long long* bar, uint32_t parity
   }
 }
 
+// Up to 64 attempts (each suspends the thread for a microsecond or two at most) in a loop of three instructions.
+__device__ __forceinline__ bool qt_try_wait_64(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\tmov.u32 n, 64;\n"
+      "AGAIN:\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t@p bra OUT;\n\t"
+      "sub.u32 n, n, 1;\n\tsetp.ne.u32 q, n, 0;\n\t@q bra AGAIN;\n"
+      "OUT:\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+
+// The rest of a long wait: false when it gave up (now or earlier).
+static __device__ __noinline__ bool qt_wait_long(uint32_t bar, uint32_t parity, volatile int* abort_flag,
+                                                 unsigned* error) {
+  const unsigned long long t0 = qt_clock();
+  while (true) {
+    if (qt_try_wait(bar, parity)) return true;
+    if (*abort_flag) return false;
+    if (qt_clock() - t0 > QT_WAIT_NS) {
+      *abort_flag = 1;
+      atomicExch(error, 1u);
+      return false;
+    }
+  }
+}
+
+// Bounded wait for pipelines whose stages last a few hundred cycles: few instructions while it is short, the abort flag
+// and the timer (whose reads cost more than such a wait) only once it is long.
+__device__ __forceinline__ bool qt_wait_short(uint32_t bar, uint32_t parity, volatile int* abort_flag,
+                                              unsigned* error) {
+  return qt_try_wait_64(bar, parity) || qt_wait_long(bar, parity, abort_flag, error);
+}
+
+// One lane of a converged warp (the same one every time).
+__device__ __forceinline__ bool qt_elect() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(p));
+  return p != 0;
+}
+
 // Bounded wait that ignores the abort flag (draining copies and MMAs already in flight).
 __device__ __forceinline__ void qt_drain(unsigned long long* bar, uint32_t parity) {
   const uint32_t b = qt_smem(bar);
