@@ -14,14 +14,15 @@
 //
 // A persistent grid (one CTA per SM) walks tiles; its warps are coupled by mbarriers only:
 //  * warp 0 copies each 64-wide group of packed weights (4608 contiguous bytes) into a ring of 12;
-//  * warps 10-17, two sets of 4, expand a group each: thread = output row, 64 codes -> 32 registers of fp16 pairs
+//  * warps 14-21, two sets of 4, expand a group each: thread = output row, 64 codes -> 32 registers of fp16 pairs
 //    (q exact, then one fused multiply-add) -> tensor memory, where the MMA reads A directly. Neither shared memory
 //    nor its bandwidth carries expanded weights;
-//  * warps 6-9 gather the item's rows, 16 bytes at a time (cp.async), into K-major 128-byte-swizzled B stages. The
+//  * warps 10-13 gather the item's rows, 16 bytes at a time (cp.async), into K-major 128-byte-swizzled B stages. The
 //    k order within 8 follows the code expansion (k, k + 4 adjacent): the prep kernel and the gated epilogue write
 //    their fp16 rows in that order;
 //  * warp 1 issues 4 MMAs of K = 16 a group into one of two 128-column accumulators;
-//  * warps 2-5 read a finished accumulator (lane = output), scale it, apply the gate, and store.
+//  * warps 2-9, two sets of 4 for alternate 32 columns, read a finished accumulator (lane = output), scale it, apply
+//    the gate, and store.
 // Every column (row of x) is its own sum in K order, so a row's bits do not depend on the other rows.
 //
 // Every mbarrier wait is bounded (1 s): one that runs out sets the plan's error word and the CTA's abort flag, which
@@ -40,8 +41,9 @@ constexpr int MT_N = MOE_TC_ROWS;       // rows of an item at most (MMA N)
 constexpr int MT_S = 8;                 // A and B stages
 constexpr int MT_W = 12;                // weight ring
 constexpr int MT_B = MT_N * 128;        // bytes of a B stage
-constexpr int MT_W_LOAD = 6, MT_W_TRANS = 10;  // first gather and expansion warps
-constexpr int MT_THREADS = 18 * 32;
+constexpr int MT_EPI = 8;               // epilogue warps
+constexpr int MT_W_EPI = 2, MT_W_LOAD = MT_W_EPI + MT_EPI, MT_W_TRANS = MT_W_LOAD + 4;  // first warps of the roles
+constexpr int MT_THREADS = (MT_W_TRANS + 8) * 32;
 constexpr uint32_t MT_TMEM = 512;       // 2 accumulators of 128 columns, 8 A stages of 32
 constexpr int MT_A0 = 256;
 constexpr size_t MT_OFF_W = (size_t)MT_S * MT_B;
@@ -49,7 +51,8 @@ constexpr size_t MT_OFF_BAR = MT_OFF_W + (size_t)MT_W * MOE_BLOCK_BYTES;
 // barriers: a stage's MMAs completed; a stage's A and B in place; weight ring; accumulators
 constexpr int MT_DONE = 0, MT_FULL = MT_DONE + MT_S, MT_W_FULL = MT_FULL + MT_S, MT_W_EMPTY = MT_W_FULL + MT_W,
               MT_D_FULL = MT_W_EMPTY + MT_W, MT_D_EMPTY = MT_D_FULL + 2, MT_BARS = MT_D_EMPTY + 2;
-constexpr size_t MT_SMEM = 1024 + MT_OFF_BAR + MT_BARS * 8 + 16;
+constexpr size_t MT_OFF_META = (MT_OFF_BAR + MT_BARS * 8 + 16 + 15) / 16 * 16;  // an epilogue warp's columns
+constexpr size_t MT_SMEM = 1024 + MT_OFF_META + (size_t)MT_EPI * 64 * 16;
 
 struct TcArgs {
   MoeProduct p;
@@ -199,7 +202,7 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
     }
     for (int s = 0; s < 2; s++) {
       qt_init(&b[MT_D_FULL + s], 1u);
-      qt_init(&b[MT_D_EMPTY + s], 4u);
+      qt_init(&b[MT_D_EMPTY + s], MT_EPI);
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -286,8 +289,10 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
       qt_drain(reinterpret_cast<unsigned long long*>(sbase + MT_OFF_BAR) + MT_DONE + (k - 1) % MT_S,
                (uint32_t)(((k - 1) / MT_S) & 1));
   } else if (warp < MT_W_LOAD) {
-    // ---- epilogue: thread = output row of the block, columns = the item's rows ---------------------------------
-    const int q = warp & 3;
+    // ---- epilogue: lane = output of the block, columns = the item's rows ---------------------------------------
+    const int q = warp & 3, set = (warp - MT_W_EPI) >> 2;
+    float4* meta = reinterpret_cast<float4*>(sbase + MT_OFF_META) + (warp - MT_W_EPI) * 64;
+    const bool paired = (nout & 1) == 0 && (reinterpret_cast<uintptr_t>(a.p.y) & 3) == 0;
     pdl_wait();
     pdl_trigger();
     int t = 0;
@@ -297,18 +302,40 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
       if (item.x == a.p.E) {  // places without an expert: zeros (a sorted output holds none of them)
         if (a.p.dst != MOE_SORTED) {
           const int f = col * 128 + q * 32 + lane;
-          for (int j = 0; j < rows; j++)
+          for (int j = set; j < rows; j += 2)
             if (f < nout) a.p.y[(size_t)a.p.pairs[item.y + j] * nout + f] = 0;
         }
         continue;
       }
-      const int buf = t & 1;
+      // this warp's columns 64 i + 32 set + lane: the factors of the accumulator and of h, the output row
       const float wmax = a.wmax[item.x];
       const float wscale = mt_pow2(mt_exp(wmax, 8));
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        const int c = 64 * i + 32 * set + lane;
+        if (c < rows) {
+          const int pos = item.y + c, pair = a.p.pairs[pos];
+          const int src = a.p.src == MOE_SORTED ? pos : (a.p.src == MOE_BY_PAIR ? pair : pair / a.p.top_k);
+          float hs = 0.f;
+          if constexpr (GLU) {
+            const float bound = 2.f * a.xlog[src] + log2f((float)a.p.K) + 2.f * log2f(wmax);
+            const int e = bound > -100.f ? (int)ceilf(fminf(bound, 135.f)) - 15 : -110;
+            hs = mt_pow2(-e);
+            if (col == 0 && q == 0) a.hscale[pos] = mt_pow2(e);
+          }
+          meta[32 * i + lane] =
+              make_float4(a.xscale[src], hs, __int_as_float(a.p.dst == MOE_SORTED ? pos : pair), 0.f);
+        }
+      }
+      __syncwarp();
+      const int buf = t & 1;
       if (!qt_wait_short(bars + 8 * (MT_D_FULL + buf), (uint32_t)((t / 2) & 1), abort_flag, a.error)) break;
       t++;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      for (int c0 = 0; c0 < rows; c0 += 32) {
+#pragma unroll 1
+      for (int i = 0; 64 * i + 32 * set < rows; i++) {
+        const int c0 = 64 * i + 32 * set, n = min(32, rows - c0);
         uint32_t v[32];
         const uint32_t ta = tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(buf * MT_N + c0);
         asm volatile(
@@ -319,57 +346,54 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
               "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
               "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
             : "r"(ta));
-        // lane j: column c0 + j's output row and factors
-        const int pos = item.y + c0 + lane;
-        int dst = 0;
-        float xs = 0.f, hs = 0.f;
-        if (c0 + lane < rows) {
-          const int pair = a.p.pairs[pos];
-          const int src = a.p.src == MOE_SORTED ? pos : (a.p.src == MOE_BY_PAIR ? pair : pair / a.p.top_k);
-          dst = a.p.dst == MOE_SORTED ? pos : pair;
-          xs = a.xscale[src];
-          if constexpr (GLU) {
-            const float bound = 2.f * a.xlog[src] + log2f((float)a.p.K) + 2.f * log2f(wmax);
-            const int e = bound > -100.f ? (int)ceilf(fminf(bound, 135.f)) - 15 : -110;
-            hs = mt_pow2(-e);
-            if (col == 0 && q == 0) a.hscale[pos] = mt_pow2(e);
-          }
-        }
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-        if (c0 + 32 >= rows) {
-          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-          __syncwarp();
-          if (lane == 0) mt_arrive(bars + 8 * (MT_D_EMPTY + buf));
-        }
+        const float4* m = meta + 32 * i;
+        // Of two columns j, j + 1 each lane finishes one, with its partner lane's value of it (the partner: the other
+        // half of a gated output, or the neighbouring output, so that two outputs leave in one store).
+        const int other = GLU ? 16 : 1;
+        const bool second = lane & other;
+        const int f = GLU ? (col * 4 + q) * 16 + (lane & 15) : col * 128 + q * 32 + lane;
         if constexpr (GLU) {
-          // lanes 0-15 hold gate features, 16-31 the matching up features: of two columns each half takes one
-          const bool up = lane >= 16;
-          const int f = (col * 4 + q) * 16 + (lane & 15);
-          __half* h = reinterpret_cast<__half*>(a.p.y);
+          __half* h = reinterpret_cast<__half*>(a.p.y) + (f & ~7) + mt_perm(f & 7);
 #pragma unroll
           for (int j = 0; j < 32; j += 2) {
-            const float give = __uint_as_float(up ? v[j] : v[j + 1]), keep = __uint_as_float(up ? v[j + 1] : v[j]);
+            const float give = __uint_as_float(second ? v[j] : v[j + 1]);
+            const float keep = __uint_as_float(second ? v[j + 1] : v[j]);
             const float got = __shfl_xor_sync(0xffffffffu, give, 16);
-            const int jj = up ? j + 1 : j;
-            const float x1 = __shfl_sync(0xffffffffu, xs, jj), h1 = __shfl_sync(0xffffffffu, hs, jj);
-            const int o = __shfl_sync(0xffffffffu, dst, jj);
-            if (c0 + jj < rows && f < nout) {
-              const float g = (up ? got : keep) * wscale * x1, u = (up ? keep : got) * wscale * x1;
-              h[(size_t)o * nout + (f & ~7) + mt_perm(f & 7)] =
-                  __float2half_rn(mt_gated(a.p.epilogue == IM_EPI_GEGLU, g, u) * h1);
-            }
+            const float4 mj = m[second ? j + 1 : j];
+            const float x1 = mj.x * wscale;
+            // lanes 0-15 hold gate features, 16-31 the matching up features
+            const float g = (second ? got : keep) * x1, u = (second ? keep : got) * x1;
+            const float o = mt_gated(a.p.epilogue == IM_EPI_GEGLU, g, u) * mj.y;
+            if (j + (second ? 1 : 0) < n && f < nout)
+              h[(size_t)__float_as_int(mj.z) * nout] = __float2half_rn(o);
+          }
+        } else if (paired) {
+          uint16_t* y = a.p.y + (f & ~1);
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            const float give = __uint_as_float(second ? v[j] : v[j + 1]);
+            const float keep = __uint_as_float(second ? v[j + 1] : v[j]);
+            const float got = __shfl_xor_sync(0xffffffffu, give, 1);
+            const float4 mj = m[second ? j + 1 : j];
+            const float k1 = keep * wscale * mj.x, g1 = got * wscale * mj.x;
+            uint32_t o;
+            asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(o) : "f"(second ? k1 : g1), "f"(second ? g1 : k1));
+            if (j + (second ? 1 : 0) < n && f < nout)
+              *reinterpret_cast<uint32_t*>(y + (size_t)__float_as_int(mj.z) * nout) = o;
           }
         } else {
-          const int f = col * 128 + q * 32 + lane;
 #pragma unroll
           for (int j = 0; j < 32; j++) {
-            const float x1 = __shfl_sync(0xffffffffu, xs, j);
-            const int o = __shfl_sync(0xffffffffu, dst, j);
-            if (c0 + j < rows && f < nout)
-              a.p.y[(size_t)o * nout + f] = to_bf(__uint_as_float(v[j]) * wscale * x1);
+            const float4 mj = m[j];
+            if (j < n && f < nout)
+              a.p.y[(size_t)__float_as_int(mj.z) * nout + f] = to_bf(__uint_as_float(v[j]) * wscale * mj.x);
           }
         }
       }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mt_arrive(bars + 8 * (MT_D_EMPTY + buf));
     }
   } else if (warp < MT_W_TRANS) {
     // ---- gather of B -------------------------------------------------------------------------------------------
