@@ -408,7 +408,7 @@ int im_moe_status(const void* plan);
 size_t im_moe_packed_bytes(int64_t E, int64_t N, int64_t K);
 int im_moe_pack_w4g64(const uint32_t* w, const uint16_t* scales, const uint16_t* biases, int64_t E, int64_t N,
                       int64_t K, void* packed, void* stream);
-size_t im_moe_grouped_workspace_bytes(int64_t M, int64_t E, int64_t top_k, int64_t K, int x_by_pair, int path);
+size_t im_moe_grouped_workspace_bytes(int64_t M, int64_t E, int64_t top_k, int64_t K, int path);
 int im_moe_grouped_qgemm(const void* packed, const uint16_t* x, uint16_t* y, int64_t M, int64_t E, int64_t top_k,
                          int64_t N, int64_t K, int x_by_pair, const int32_t* pairs, int path, void* plan,
                          size_t plan_bytes, void* workspace, size_t workspace_bytes, void* stream);

@@ -85,7 +85,7 @@ SIGNATURES: dict[str, tuple] = {
     "im_moe_status": (_INT, [_P]),
     "im_moe_packed_bytes": (_SZ, [_I64, _I64, _I64]),
     "im_moe_pack_w4g64": (_INT, [_P, _P, _P, _I64, _I64, _I64, _P, _P]),
-    "im_moe_grouped_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64, _INT, _INT]),
+    "im_moe_grouped_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64, _INT]),
     "im_moe_grouped_qgemm": (_INT, [_P, _P, _P, _I64, _I64, _I64, _I64, _I64, _INT, _P, _INT, _P, _SZ, _P, _SZ, _P]),
     "im_moe_mlp_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64, _I64, _INT]),
     "im_moe_mlp": (_INT, [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _INT, _P, _INT, _P, _SZ, _P, _SZ, _P]),

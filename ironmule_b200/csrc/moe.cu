@@ -27,11 +27,12 @@ static bool moe_nk_ok(int64_t N, int64_t K) {
   return N >= 1 && N <= (1 << 24) && K >= 64 && K % 64 == 0 && K <= (1 << 20);
 }
 
-// One thread per row of a block's group: its codes into the packed order, the largest |w| of the expert into wmax (all
-// values non-negative, so their bit patterns order as integers and the maximum does not depend on the order).
+// One thread per row of a block's group: its codes into the packed order, the largest |w| of the row and of the expert's
+// halves (all values non-negative, so their bit patterns order as integers; a maximum does not depend on the order).
 __global__ void __launch_bounds__(128)
 moe_pack_kernel(const uint32_t* __restrict__ w, const uint16_t* __restrict__ sc, const uint16_t* __restrict__ bi, int N,
-                int K, int blocks, unsigned char* __restrict__ out, unsigned* __restrict__ wmax) {
+                int K, int blocks, unsigned char* __restrict__ out, unsigned* __restrict__ row_max,
+                unsigned* __restrict__ half_max) {
   const int G = K >> 6;
   const long long unit = blockIdx.x;  // (expert * blocks + block) * G + group
   const int grp = (int)(unit % G), block = (int)(unit / G % blocks);
@@ -56,12 +57,14 @@ moe_pack_kernel(const uint32_t* __restrict__ w, const uint16_t* __restrict__ sc,
   uint16_t* sb = reinterpret_cast<uint16_t*>(dst + 4096 + tile * 128 + (lane & 7) * 16);
   sb[lane >> 3] = s;
   sb[4 + (lane >> 3)] = b;
+  if (top > 0.f) atomicMax(row_max + (expert * blocks + block) * 128 + threadIdx.x, __float_as_uint(top));
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (lane == 0 && top > 0.f) atomicMax(wmax + expert, __float_as_uint(top));
+  for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if ((lane & 15) == 0 && top > 0.f) atomicMax(half_max + 2 * expert + (lane >> 4), __float_as_uint(top));
 }
 
 static size_t moe_expert_bytes(int64_t N, int64_t K) { return (size_t)((N + 127) / 128) * (K / 64) * MOE_BLOCK_BYTES; }
+static size_t moe_max_bytes(int64_t N) { return (size_t)((N + 127) / 128) * 512 + 8; }  // of an expert
 
 }  // namespace im
 
@@ -69,7 +72,7 @@ using namespace im;
 
 extern "C" size_t im_moe_packed_bytes(int64_t E, int64_t N, int64_t K) {
   if (E < 1 || E > MOE_MAX_EXPERTS || !moe_nk_ok(N, K)) return 0;
-  return (size_t)E * (moe_expert_bytes(N, K) + 4);
+  return (size_t)E * (moe_expert_bytes(N, K) + moe_max_bytes(N));
 }
 
 extern "C" int im_moe_pack_w4g64(const uint32_t* w, const uint16_t* scales, const uint16_t* biases, int64_t E,
@@ -84,13 +87,14 @@ extern "C" int im_moe_pack_w4g64(const uint32_t* w, const uint16_t* scales, cons
   IM_REQUIRE(units < (1ll << 31), IM_UNSUPPORTED, "im_moe_pack_w4g64: too many units");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   unsigned char* out = reinterpret_cast<unsigned char*>(packed);
-  unsigned* wmax = reinterpret_cast<unsigned*>(out + (size_t)E * moe_expert_bytes(N, K));
-  const cudaError_t e = cudaMemsetAsync(wmax, 0, (size_t)E * 4, st);
+  unsigned* row_max = reinterpret_cast<unsigned*>(out + (size_t)E * moe_expert_bytes(N, K));
+  const cudaError_t e = cudaMemsetAsync(row_max, 0, (size_t)E * moe_max_bytes(N), st);
   if (e != cudaSuccess) {
     set_error("im_moe_pack_w4g64: %s", cudaGetErrorString(e));
     return IM_CUDA_ERROR;
   }
-  moe_pack_kernel<<<(unsigned)units, 128, 0, st>>>(w, scales, biases, (int)N, (int)K, (int)blocks, out, wmax);
+  moe_pack_kernel<<<(unsigned)units, 128, 0, st>>>(w, scales, biases, (int)N, (int)K, (int)blocks, out, row_max,
+                                                row_max + (size_t)E * blocks * 128);
   return check_launch("moe_pack_kernel");
 }
 
@@ -106,12 +110,11 @@ extern "C" int im_moe_status(const void* plan) {
   return word;
 }
 
-extern "C" size_t im_moe_grouped_workspace_bytes(int64_t M, int64_t E, int64_t top_k, int64_t K, int x_by_pair,
-                                                 int path) {
+extern "C" size_t im_moe_grouped_workspace_bytes(int64_t M, int64_t E, int64_t top_k, int64_t K, int path) {
   if (M < 1 || M > MOE_MAX_ROWS || E < 1 || E > MOE_MAX_EXPERTS || top_k < 1 || top_k > MOE_MAX_TOP_K || top_k > E ||
       !moe_nk_ok(1, K) || moe_plan(M, E, top_k, path).item_rows != MOE_TC_ROWS)
     return 0;
-  return moe_tc_space(x_by_pair ? M * top_k : M, K, 0, 0).total;
+  return moe_tc_space(moe_plan(M, E, top_k, path), M * top_k, K, 0).total;
 }
 
 extern "C" int im_moe_grouped_qgemm(const void* packed, const uint16_t* x, uint16_t* y, int64_t M, int64_t E,
@@ -127,7 +130,7 @@ extern "C" int im_moe_grouped_qgemm(const void* packed, const uint16_t* x, uint1
   IM_REQUIRE(packed && x && y, IM_INVALID, "im_moe_grouped_qgemm: null pointer");
   IM_REQUIRE(aligned(packed, 16) && aligned(x, 16) && aligned(y, 2), IM_INVALID,
              "im_moe_grouped_qgemm: packed and x must be 16-byte aligned");
-  const size_t need = im_moe_grouped_workspace_bytes(M, E, top_k, K, x_by_pair, path);
+  const size_t need = im_moe_grouped_workspace_bytes(M, E, top_k, K, path);
   IM_REQUIRE(!need || (workspace && aligned(workspace, 256) && workspace_bytes >= need), IM_INVALID,
              "im_moe_grouped_qgemm: workspace of %zu bytes (256-aligned) needed, %zu given", need, workspace_bytes);
   MoeProduct a = {};
@@ -147,9 +150,8 @@ extern "C" int im_moe_grouped_qgemm(const void* packed, const uint16_t* x, uint1
   const MoePlan p = moe_plan(M, E, top_k, path);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (p.item_rows != MOE_TC_ROWS) return moe_mma_launch(p, a, st);
-  const int64_t rows = x_by_pair ? M * top_k : M;
-  const MoeTcSpace space = moe_tc_space(rows, K, 0, 0);
-  const int prep = moe_prep_launch(x, rows, K, space, workspace, st);
+  const MoeTcSpace space = moe_tc_space(p, M * top_k, K, 0);
+  const int prep = moe_prep_launch(p, a, space, workspace, st);
   return prep ? prep : moe_tc_launch(p, a, space, workspace, st);
 }
 
@@ -157,7 +159,8 @@ extern "C" size_t im_moe_mlp_workspace_bytes(int64_t M, int64_t E, int64_t top_k
   if (M < 1 || M > MOE_MAX_ROWS || E < 1 || E > MOE_MAX_EXPERTS || top_k < 1 || top_k > MOE_MAX_TOP_K || top_k > E ||
       H < 64 || H % 64 || I < 64 || I % 64)
     return 0;
-  if (moe_plan(M, E, top_k, path).item_rows == MOE_TC_ROWS) return moe_tc_space(M, H, M * top_k, I).total;
+  const MoePlan p = moe_plan(M, E, top_k, path);
+  if (p.item_rows == MOE_TC_ROWS) return moe_tc_space(p, M * top_k, H, I).total;
   return (size_t)M * top_k * I * 2;
 }
 
@@ -181,9 +184,9 @@ extern "C" int im_moe_mlp(const void* gate_up, const void* down, const uint16_t*
   const MoePlan p = moe_plan(M, E, top_k, path);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const bool tc = p.item_rows == MOE_TC_ROWS;
-  const MoeTcSpace space = tc ? moe_tc_space(M, H, M * top_k, I) : MoeTcSpace{};
+  const MoeTcSpace space = tc ? moe_tc_space(p, M * top_k, H, I) : MoeTcSpace{};
   // the gated activations lie in the order of the sorted pairs, so that an item's rows are contiguous
-  uint16_t* hidden = reinterpret_cast<uint16_t*>(reinterpret_cast<char*>(workspace) + space.h16);
+  uint16_t* hidden = reinterpret_cast<uint16_t*>(workspace);  // (the tensor-core path lays its own out)
   MoeProduct a = {};
   a.wp = reinterpret_cast<const unsigned char*>(gate_up);
   a.x = x;
@@ -199,7 +202,7 @@ extern "C" int im_moe_mlp(const void* gate_up, const void* down, const uint16_t*
   a.dst = MOE_SORTED;
   a.epilogue = activation;
   int status = IM_OK;
-  if (tc) status = moe_prep_launch(x, M, H, space, workspace, st);
+  if (tc) status = moe_prep_launch(p, a, space, workspace, st);
   if (!status) status = tc ? moe_tc_launch(p, a, space, workspace, st) : moe_mma_launch(p, a, st);
   if (status) return status;
   a.wp = reinterpret_cast<const unsigned char*>(down);

@@ -20,13 +20,15 @@ constexpr int MOE_PLAN_HEADER = 8;      // ints: [0] work items, [1] error word 
 // MOE_BLOCK_BYTES = 4 tiles of 32 rows x (two 16-byte halves a row, [half][row]) of codes, then per tile 128 bytes of
 // scales and biases: for g = 0..7 the bf16 scales of rows g, g + 8, g + 16, g + 24, then their biases. One copy brings
 // a block's group; a thread reads its row's codes in two 16-byte loads without bank conflicts, and a warp-MMA lane the
-// 8 bytes of each of its four rows. After the E experts: float32 [E], the largest |scale * q + bias| of each.
+// 8 bytes of each of its four rows. After the E experts: float32 [E][padded rows], the
+// largest |scale * q + bias| that a row's scales and biases allow; float32 [E][2], the largest over an expert's rows
+// with r & 16 == 0 (the gate rows of a gated product) and over the others (the up rows).
 constexpr int MOE_BLOCK_BYTES = 4608;
 
 // One work item: `rows` consecutive entries of the sorted pair list, all of one expert (or, with expert == E, of the
 // places that chose no expert, whose outputs are zero).
 struct MoeItem {
-  int expert, first, rows, pad;
+  int expert, first, rows, padded;  // padded: the rows before it when every item is rounded up to 16
 };
 
 // Plan layout in ints: header | items | per-block expert counts (the routing's own scratch).
@@ -59,10 +61,10 @@ struct MoeProduct {
 
 // Byte offsets in the workspace of the tensor-core path.
 struct MoeTcSpace {
-  size_t x16, xscale, xlog, h16, hscale, total;
+  size_t tiles, scale, xlog, next, hscale, total;
 };
-MoeTcSpace moe_tc_space(int64_t rows, int64_t K, int64_t pairs, int64_t I);
-int moe_prep_launch(const uint16_t* x, int64_t rows, int64_t K, const MoeTcSpace& s, void* workspace, cudaStream_t st);
+MoeTcSpace moe_tc_space(const MoePlan& p, int64_t pairs, int64_t K, int64_t I);
+int moe_prep_launch(const MoePlan& p, const MoeProduct& a, const MoeTcSpace& s, void* workspace, cudaStream_t st);
 int moe_tc_launch(const MoePlan& p, const MoeProduct& a, const MoeTcSpace& s, void* workspace, cudaStream_t st);
 int moe_mma_launch(const MoePlan& p, const MoeProduct& a, cudaStream_t st);
 

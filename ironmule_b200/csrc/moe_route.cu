@@ -186,18 +186,30 @@ __device__ __forceinline__ int mr_scan(const int* v, int* out, int n, int* sh) {
 struct RouteSmem {
   int total[MOE_MAX_EXPERTS + 1];   // pairs of each bucket over all blocks
   int base[MOE_MAX_EXPERTS + 1];    // pairs of each bucket in earlier blocks, then where the next one goes
-  int scan[MOE_MAX_EXPERTS + 1];
+  int scan[MOE_MAX_EXPERTS + 1];    // work items before each bucket's
+  int pad[MOE_MAX_EXPERTS + 1];     // rows before each bucket's when every item is rounded up to 16
   int cnt[MR_WARPS][MOE_MAX_EXPERTS + 1];
   int sh[MR_WARPS];
 };
+
+// A bucket of c pairs is cut into as few items as it fits, evenly, in multiples of 8 rows.
+__device__ __forceinline__ int mr_item_rows(int c, int most) {
+  const int n = (c + most - 1) / most;
+  return n ? ((c + n - 1) / n + 7) / 8 * 8 : 0;
+}
 
 // Offsets, work items (block 0) and this block's pairs, from s.total and s.base.
 __device__ __forceinline__ void mr_place(const RouteArgs& a, RouteSmem& s) {
   const int nb = a.E + 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (blockIdx.x == 0) {
-    for (int e = threadIdx.x; e < nb; e += MR_THREADS) s.scan[e] = (s.total[e] + a.item_rows - 1) / a.item_rows;
+    for (int e = threadIdx.x; e < nb; e += MR_THREADS) {
+      const int c = s.total[e], each = mr_item_rows(c, a.item_rows), n = (c + a.item_rows - 1) / a.item_rows;
+      s.scan[e] = n;
+      s.pad[e] = n ? (n - 1) * ((each + 15) & ~15) + ((c - (n - 1) * each + 15) & ~15) : 0;
+    }
     __syncthreads();
     const int items = mr_scan(s.scan, s.scan, nb, s.sh);
+    mr_scan(s.pad, s.pad, nb, s.sh);
     if (threadIdx.x == 0) {
       a.plan[0] = items;
       a.plan[1] = 0;
@@ -210,11 +222,9 @@ __device__ __forceinline__ void mr_place(const RouteArgs& a, RouteSmem& s) {
     for (int e = threadIdx.x; e < nb; e += MR_THREADS) {
       const int c = s.total[e], first = s.cnt[0][e];
       a.offsets[e] = first;
-      // an expert's rows in as few items as they fit, evenly, in multiples of 8
-      const int n = (c + a.item_rows - 1) / a.item_rows;
-      const int each = n ? ((c + n - 1) / n + 7) / 8 * 8 : 0;
+      const int n = (c + a.item_rows - 1) / a.item_rows, each = mr_item_rows(c, a.item_rows);
       for (int i = 0; i < n; i++)
-        items[s.scan[e] + i] = make_int4(e, first + i * each, max(0, min(each, c - i * each)), 0);
+        items[s.scan[e] + i] = make_int4(e, first + i * each, min(each, c - i * each), s.pad[e] + i * ((each + 15) & ~15));
     }
     if (threadIdx.x == 0) a.offsets[nb] = all;
   }

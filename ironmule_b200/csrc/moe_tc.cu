@@ -5,21 +5,24 @@
 //
 // Why fp16: w = scale * q + bias needs one rounding to become an operand. In bf16 (8 bits) that costs as much as the
 // output's own rounding; in fp16 (11 bits) it is an eighth of it. The range is met by powers of two, which are exact:
-//  * weights are scaled by the expert's largest |w| (found when they are packed), which lands in [2^7, 2^8);
+//  * a weight row is scaled by its largest |w| (found when it is packed), which lands in [2^-7, 2^-6): then a code in
+//    the low bits of a half IS the subnormal q 2^-24 (or 16 q 2^-24), and one fused multiply-add with scale * 2^24
+//    (2^20) makes the weight. What this range costs is below 2^-18 of the row's largest weight;
 //  * a row of x by its largest finite element, which lands in [2^9, 2^10) (moe_prep_kernel; bf16 values fit fp16);
-//  * the gated activations h = act(g) u by a bound on the row: |g|, |u| <= |x|_2 sqrt(K) max |w|, so
-//    |h| <= |x|_2^2 K max|w|^2, which lands below 2^15. No row can overflow, and typical rows stay well above
+//  * the gated activations h = act(g) u by a bound on the row: |g| <= |x|_2 sqrt(K) max |G|, |u| likewise, so
+//    |h| <= |x|_2^2 K max|G| max|U|, which lands below 2^15. No row can overflow, and typical rows stay well above
 //    fp16's subnormals (the bound is loose by K or so, of 2^29).
 // The factors return in float32 after the sum. A row with infinities or NaN gives those.
 //
 // A persistent grid (one CTA per SM) walks tiles; its warps are coupled by mbarriers only:
 //  * warp 0 copies each 64-wide group of packed weights (4608 contiguous bytes) into a ring of 12;
-//  * warps 14-21, two sets of 4, expand a group each: thread = output row, 64 codes -> 32 registers of fp16 pairs
-//    (q exact, then one fused multiply-add) -> tensor memory, where the MMA reads A directly. Neither shared memory
-//    nor its bandwidth carries expanded weights;
-//  * warps 10-13 gather the item's rows, 16 bytes at a time (cp.async), into K-major 128-byte-swizzled B stages. The
-//    k order within 8 follows the code expansion (k, k + 4 adjacent): the prep kernel and the gated epilogue write
-//    their fp16 rows in that order;
+//  * warps 12-27, four sets of 4, expand a group each: thread = output row, 64 codes -> 32 registers of fp16 pairs ->
+//    tensor memory, where the MMA reads A directly. Neither shared memory nor its bandwidth carries expanded weights;
+//  * warp 10 copies the item's rows of the group, one contiguous copy: moe_prep_kernel lays each item's rows out as the
+//    K-major 128-byte-swizzled tiles that the MMA reads, and the gated epilogue writes its outputs as the next
+//    product's tiles. (Gathering here was measured: TMA gather4 of 128-byte rows takes 64 cycles a row quadruple, and
+//    16-byte asynchronous copies occupied four warps and the load pipe; a prefill took 1407 and 527 us.) The k order
+//    within 8 follows the code expansion (k, k + 4 adjacent);
 //  * warp 1 issues 4 MMAs of K = 16 a group into one of two 128-column accumulators;
 //  * warps 2-9, two sets of 4 for alternate 32 columns, read a finished accumulator (lane = output), scale it, apply
 //    the gate, and store.
@@ -42,8 +45,11 @@ constexpr int MT_S = 8;                 // A and B stages
 constexpr int MT_W = 12;                // weight ring
 constexpr int MT_B = MT_N * 128;        // bytes of a B stage
 constexpr int MT_EPI = 8;               // epilogue warps
-constexpr int MT_W_EPI = 2, MT_W_LOAD = MT_W_EPI + MT_EPI, MT_W_TRANS = MT_W_LOAD + 4;  // first warps of the roles
-constexpr int MT_THREADS = (MT_W_TRANS + 8) * 32;
+constexpr int MT_SETS = 4;              // expansion sets of four warps
+constexpr int MT_W_EPI = 2, MT_W_LOAD = MT_W_EPI + MT_EPI, MT_W_TRANS = MT_W_LOAD + 2;  // first warps of the roles
+constexpr int MT_THREADS = (MT_W_TRANS + 4 * MT_SETS) * 32;
+static_assert(MT_S % MT_SETS == 0 && MT_W % MT_SETS == 0, "a set keeps its stages");
+constexpr int MT_WBITS = -6;            // an expert's largest weight lands in [2^-7, 2^-6)
 constexpr uint32_t MT_TMEM = 512;       // 2 accumulators of 128 columns, 8 A stages of 32
 constexpr int MT_A0 = 256;
 constexpr size_t MT_OFF_W = (size_t)MT_S * MT_B;
@@ -58,11 +64,13 @@ struct TcArgs {
   MoeProduct p;
   const int4* items;
   unsigned* error;
-  const __half* x16;     // rows of K, scaled
-  const float* xscale;   // per row of x16: the factor it was divided by
-  const float* xlog;     // per row: log2 |x|_2 (first product of a gated MLP)
-  float* hscale;         // per sorted position: the factor h was divided by (written by the first product)
-  const float* wmax;     // per expert: largest |w|
+  const unsigned char* tiles;  // the items' rows as tiles
+  const float* scale;    // per sorted position: the factor its row was divided by
+  const float* xlog;     // per sorted position: log2 |x|_2 (first product of a gated MLP)
+  unsigned char* next;   // the next product's tiles, and its rows' factors (written by the first product)
+  float* hscale;
+  const float* row_max;  // [E][128 cols]: a weight row's largest |w|
+  const float* half_max; // [E][2]: an expert's largest over the gate rows (r & 16 == 0) and over the up rows
   size_t expert_bytes;
   int cols;              // 128-output blocks
 };
@@ -81,19 +89,32 @@ __device__ __forceinline__ int mt_exp(float max, int bits) {
 // Position of element k (0..7) of 8 in the operands' order.
 __device__ __forceinline__ int mt_perm(int k) { return k < 4 ? 2 * k : 2 * (k - 4) + 1; }
 
-// ---- rows of x -> scaled fp16 in operand order, one CTA per row --------------------------------------------
-__global__ void __launch_bounds__(256)
-moe_prep_kernel(const uint16_t* __restrict__ x, int K, __half* __restrict__ x16, float* __restrict__ xscale,
+// An item's rows as tiles: per 64-wide group, its rows (rounded up to 16) of 128 bytes; 16-byte chunk c of row r at
+// c ^ r % 8. Items lie one after another from their padded first row on.
+__device__ __forceinline__ size_t mt_tile(int padded, int n16, int K, int group) {
+  return (size_t)padded * K * 2 + (size_t)group * n16 * 128;
+}
+__device__ __forceinline__ uint32_t mt_chunk(int r, int c) { return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4)); }
+
+// ---- the items' rows of x -> scaled fp16 tiles; a warp per row, grid (items, 128 / 16) -------------------------
+constexpr int MP_ROWS = 16;
+__global__ void __launch_bounds__(MP_ROWS * 32)
+moe_prep_kernel(const uint16_t* __restrict__ x, const int* __restrict__ plan, const int* __restrict__ pairs, int E,
+                int top_k, int by_pair, int K, unsigned char* __restrict__ tiles, float* __restrict__ scale,
                 float* __restrict__ xlog) {
-  __shared__ float sh[2][8];
   pdl_wait();
   pdl_trigger();
-  const size_t row = blockIdx.x;
-  const uint4* src = reinterpret_cast<const uint4*>(x + row * K);
+  if ((int)blockIdx.x >= plan[0]) return;
+  const int4 item = reinterpret_cast<const int4*>(plan + MOE_PLAN_HEADER)[blockIdx.x];
+  const int r = blockIdx.y * MP_ROWS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (item.x == E || r >= item.z) return;
+  const int pos = item.y + r, pair = pairs[pos];
+  const uint4* src = reinterpret_cast<const uint4*>(x + (size_t)(by_pair ? pair : pair / top_k) * K);
   const int n = K / 8;
   float top = 0.f;
-  for (int i = threadIdx.x; i < n; i += 256) {
-    const uint4 u = src[i];
+#pragma unroll 4
+  for (int i = lane; i < n; i += 32) {
+    const uint4 u = __ldg(src + i);
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
     for (int j = 0; j < 4; j++) {
@@ -104,54 +125,48 @@ moe_prep_kernel(const uint16_t* __restrict__ x, int K, __half* __restrict__ x16,
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if ((threadIdx.x & 31) == 0) sh[0][threadIdx.x >> 5] = top;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < 8; w++) top = fmaxf(top, sh[0][w]);
   const int e = mt_exp(top, 10);
   const float inv = mt_pow2(-e);
+  const int n16 = (item.z + 15) & ~15;
   float ss = 0.f;
-  for (int i = threadIdx.x; i < n; i += 256) {
-    const uint4 u = src[i];
+#pragma unroll 4
+  for (int i = lane; i < n; i += 32) {
+    const uint4 u = __ldg(src + i);
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
     float f[8];
-    alignas(16) __half h[8];
 #pragma unroll
     for (int j = 0; j < 4; j++) {
       f[2 * j] = bf_lo(w[j]) * inv;
       f[2 * j + 1] = bf_hi(w[j]) * inv;
     }
+    uint32_t h[4];
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
+    for (int j = 0; j < 4; j++) {
       if (fabsf(f[j]) < INFINITY) ss = fmaf(f[j], f[j], ss);
-      h[mt_perm(j)] = __float2half_rn(f[j]);
+      if (fabsf(f[j + 4]) < INFINITY) ss = fmaf(f[j + 4], f[j + 4], ss);
+      const __half2 v = __floats2half2_rn(f[j], f[j + 4]);
+      h[j] = *reinterpret_cast<const uint32_t*>(&v);
     }
-    *reinterpret_cast<uint4*>(x16 + row * K + 8 * i) = *reinterpret_cast<const uint4*>(h);
+    *reinterpret_cast<uint4*>(tiles + mt_tile(item.w, n16, K, i >> 3) + mt_chunk(r, i & 7)) =
+        make_uint4(h[0], h[1], h[2], h[3]);
   }
   ss = warp_sum(ss);
-  if ((threadIdx.x & 31) == 0) sh[1][threadIdx.x >> 5] = ss;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    float t = 0.f;
-#pragma unroll
-    for (int w = 0; w < 8; w++) t += sh[1][w];
-    xscale[row] = mt_pow2(e);
-    xlog[row] = 0.5f * log2f(t) + (float)e;  // -inf for a zero row
+  if (lane == 0) {
+    scale[pos] = mt_pow2(e);
+    xlog[pos] = 0.5f * log2f(ss) + (float)e;  // -inf for a zero row
   }
 }
 
 // ---- the products ----------------------------------------------------------------------------------------------
-// fp16 pairs (k, k + 4) of a word's eight codes: scale * q + bias, one rounding.
-__device__ __forceinline__ void mt_expand(uint32_t u, __half2 s, __half2 b, uint32_t* out) {
-  const __half2 m1024 = __half2half2(__ushort_as_half(0xE400)), m64 = __half2half2(__ushort_as_half(0xD400)),
-                r16 = __half2half2(__ushort_as_half(0x2C00));  // -1024, -64, 1/16
+// fp16 pairs (k, k + 4) of a word's eight codes: the code as a subnormal, times scale * 2^24 (low nibble of a byte) or
+// scale * 2^20 (high nibble), plus the bias, one rounding.
+__device__ __forceinline__ void mt_expand(uint32_t u, __half2 s24, __half2 s20, __half2 b, uint32_t* out) {
 #pragma unroll
   for (int i = 0; i < 2; i++) {
     const uint32_t v = u >> (8 * i);
-    uint32_t lo = (v & 0x000F000Fu) | 0x64006400u, hi = (v & 0x00F000F0u) | 0x64006400u;  // 1024 + q, 1024 + 16 q
-    const __half2 ql = __hadd2(*reinterpret_cast<__half2*>(&lo), m1024);
-    const __half2 qh = __hfma2(*reinterpret_cast<__half2*>(&hi), r16, m64);
-    const __half2 wl = __hfma2(ql, s, b), wh = __hfma2(qh, s, b);
+    const uint32_t lo = v & 0x000F000Fu, hi = v & 0x00F000F0u;
+    const __half2 wl = __hfma2(*reinterpret_cast<const __half2*>(&lo), s24, b);
+    const __half2 wh = __hfma2(*reinterpret_cast<const __half2*>(&hi), s20, b);
     out[2 * i] = *reinterpret_cast<const uint32_t*>(&wl);
     out[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&wh);
   }
@@ -165,6 +180,14 @@ __device__ __forceinline__ float mt_gated(bool geglu, float g, float u) {
 
 __device__ __forceinline__ void mt_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// `bytes` from src into shared memory, counted on (and arriving once at) the barrier.
+__device__ __forceinline__ void mt_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
 }
 
 __device__ __forceinline__ void mt_commit(uint32_t bar) {
@@ -194,7 +217,7 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
     unsigned long long* b = reinterpret_cast<unsigned long long*>(sbase + MT_OFF_BAR);
     for (int s = 0; s < MT_S; s++) {
       qt_init(&b[MT_DONE + s], 1u);
-      qt_init(&b[MT_FULL + s], 4u + 128u);  // four expansion warps, every gather thread
+      qt_init(&b[MT_FULL + s], 4u + 1u);  // four expansion warps, the rows' bytes
     }
     for (int s = 0; s < MT_W; s++) {
       qt_init(&b[MT_W_FULL + s], 1u);
@@ -226,16 +249,8 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
         const unsigned char* src =
             a.p.wp + (size_t)expert * a.expert_bytes + (size_t)(tile % a.cols) * G * MOE_BLOCK_BYTES;
         for (int g = 0; g < G; g++, k++) {
-          const uint32_t full = bars + 8 * (MT_W_FULL + s);
           if (!qt_wait_short(bars + 8 * (MT_W_EMPTY + s), phase ^ 1u, abort_flag, a.error)) goto weights_done;
-          asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full),
-                       "r"((uint32_t)MOE_BLOCK_BYTES)
-                       : "memory");
-          asm volatile(
-              "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                  base + (uint32_t)MT_OFF_W + s * MOE_BLOCK_BYTES),
-              "l"(src), "r"((uint32_t)MOE_BLOCK_BYTES), "r"(full)
-              : "memory");
+          mt_copy(base + (uint32_t)MT_OFF_W + s * MOE_BLOCK_BYTES, src, MOE_BLOCK_BYTES, bars + 8 * (MT_W_FULL + s));
           src += MOE_BLOCK_BYTES;
           if (++s == MT_W) s = 0, phase ^= 1u;
         }
@@ -263,8 +278,6 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
       int g = 0;
       for (; g < G; g++, k++) {
         if (!qt_wait_short(bars + 8 * (MT_FULL + s), phase, abort_flag, a.error)) break;
-        // the gathered rows were written through the generic proxy; the MMA reads them through the async one
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         if (leader) {
           const uint64_t bd = qt_desc(base + s * MT_B);
@@ -300,32 +313,31 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
       const int4 item = a.items[tile / a.cols];
       const int col = tile % a.cols, rows = item.z;
       if (item.x == a.p.E) {  // places without an expert: zeros (a sorted output holds none of them)
-        if (a.p.dst != MOE_SORTED) {
+        if (!GLU) {
           const int f = col * 128 + q * 32 + lane;
           for (int j = set; j < rows; j += 2)
             if (f < nout) a.p.y[(size_t)a.p.pairs[item.y + j] * nout + f] = 0;
         }
         continue;
       }
-      // this warp's columns 64 i + 32 set + lane: the factors of the accumulator and of h, the output row
-      const float wmax = a.wmax[item.x];
-      const float wscale = mt_pow2(mt_exp(wmax, 8));
+      // this lane's weight row's factor; this warp's columns 64 i + 32 set + lane: the rows' factors, the output row
+      const float wscale =
+          mt_pow2(mt_exp(a.row_max[((size_t)item.x * a.cols + col) * 128 + q * 32 + lane], MT_WBITS));
       __syncwarp();
 #pragma unroll
       for (int i = 0; i < 2; i++) {
         const int c = 64 * i + 32 * set + lane;
         if (c < rows) {
-          const int pos = item.y + c, pair = a.p.pairs[pos];
-          const int src = a.p.src == MOE_SORTED ? pos : (a.p.src == MOE_BY_PAIR ? pair : pair / a.p.top_k);
+          const int pos = item.y + c;
           float hs = 0.f;
           if constexpr (GLU) {
-            const float bound = 2.f * a.xlog[src] + log2f((float)a.p.K) + 2.f * log2f(wmax);
+            const float bound = 2.f * a.xlog[pos] + log2f((float)a.p.K) + log2f(a.half_max[2 * item.x]) +
+                                log2f(a.half_max[2 * item.x + 1]);
             const int e = bound > -100.f ? (int)ceilf(fminf(bound, 135.f)) - 15 : -110;
             hs = mt_pow2(-e);
             if (col == 0 && q == 0) a.hscale[pos] = mt_pow2(e);
           }
-          meta[32 * i + lane] =
-              make_float4(a.xscale[src], hs, __int_as_float(a.p.dst == MOE_SORTED ? pos : pair), 0.f);
+          meta[32 * i + lane] = make_float4(a.scale[pos], hs, __int_as_float(GLU ? 0 : a.p.pairs[pos]), 0.f);
         }
       }
       __syncwarp();
@@ -354,29 +366,30 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
         const bool second = lane & other;
         const int f = GLU ? (col * 4 + q) * 16 + (lane & 15) : col * 128 + q * 32 + lane;
         if constexpr (GLU) {
-          __half* h = reinterpret_cast<__half*>(a.p.y) + (f & ~7) + mt_perm(f & 7);
+          // the next product's tiles: group f / 64, chunk f % 64 / 8, the element's place in the operand order
+          const int n16 = (rows + 15) & ~15, chunk = (f & 63) >> 3;
+          unsigned char* h = a.next + mt_tile(item.w, n16, nout, f >> 6) + 2 * mt_perm(f & 7);
 #pragma unroll
           for (int j = 0; j < 32; j += 2) {
-            const float give = __uint_as_float(second ? v[j] : v[j + 1]);
-            const float keep = __uint_as_float(second ? v[j + 1] : v[j]);
+            const float give = __uint_as_float(second ? v[j] : v[j + 1]) * wscale;
+            const float keep = __uint_as_float(second ? v[j + 1] : v[j]) * wscale;
             const float got = __shfl_xor_sync(0xffffffffu, give, 16);
             const float4 mj = m[second ? j + 1 : j];
-            const float x1 = mj.x * wscale;
             // lanes 0-15 hold gate features, 16-31 the matching up features
-            const float g = (second ? got : keep) * x1, u = (second ? keep : got) * x1;
+            const float g = (second ? got : keep) * mj.x, u = (second ? keep : got) * mj.x;
             const float o = mt_gated(a.p.epilogue == IM_EPI_GEGLU, g, u) * mj.y;
-            if (j + (second ? 1 : 0) < n && f < nout)
-              h[(size_t)__float_as_int(mj.z) * nout] = __float2half_rn(o);
+            const int jj = j + (second ? 1 : 0);
+            if (jj < n && f < nout) *reinterpret_cast<__half*>(h + mt_chunk(c0 + jj, chunk)) = __float2half_rn(o);
           }
         } else if (paired) {
           uint16_t* y = a.p.y + (f & ~1);
 #pragma unroll
           for (int j = 0; j < 32; j += 2) {
-            const float give = __uint_as_float(second ? v[j] : v[j + 1]);
-            const float keep = __uint_as_float(second ? v[j + 1] : v[j]);
+            const float give = __uint_as_float(second ? v[j] : v[j + 1]) * wscale;
+            const float keep = __uint_as_float(second ? v[j + 1] : v[j]) * wscale;
             const float got = __shfl_xor_sync(0xffffffffu, give, 1);
             const float4 mj = m[second ? j + 1 : j];
-            const float k1 = keep * wscale * mj.x, g1 = got * wscale * mj.x;
+            const float k1 = keep * mj.x, g1 = got * mj.x;
             uint32_t o;
             asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(o) : "f"(second ? k1 : g1), "f"(second ? g1 : k1));
             if (j + (second ? 1 : 0) < n && f < nout)
@@ -396,46 +409,32 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
       if (lane == 0) mt_arrive(bars + 8 * (MT_D_EMPTY + buf));
     }
   } else if (warp < MT_W_TRANS) {
-    // ---- gather of B -------------------------------------------------------------------------------------------
-    const int th = threadIdx.x - MT_W_LOAD * 32, c = th & 7, r0 = th >> 3;  // 16-byte chunk c of rows r0 + 16 i
-    const uint32_t dst0 = base + (uint32_t)(r0 * 128 + ((c ^ (r0 & 7)) << 4));
-    pdl_wait();
-    uint32_t s = 0, phase = 1;
-    for (int tile = blockIdx.x; tile < ntiles; tile += gridDim.x) {
-      const int4 item = a.items[tile / a.cols];
-      if (item.x == a.p.E) continue;
-      const __half* src[MT_N / 16];
-#pragma unroll
-      for (int i = 0; i < MT_N / 16; i++) {
-        const int r = min(r0 + 16 * i, item.z - 1);  // (rows past the item's repeat its last one: columns nobody reads)
-        const int pos = item.y + r;
-        int row = pos;
-        if (a.p.src != MOE_SORTED) {
-          row = a.p.pairs[pos];
-          if (a.p.src == MOE_BY_TOKEN) row /= a.p.top_k;
+    // ---- rows ----------------------------------------------------------------------------------------------------
+    if (warp == MT_W_LOAD && lane == 0) {
+      pdl_wait();
+      uint32_t s = 0, phase = 1;
+      int k = 0;
+      for (int tile = blockIdx.x; tile < ntiles; tile += gridDim.x) {
+        const int4 item = a.items[tile / a.cols];
+        if (item.x == a.p.E) continue;
+        const uint32_t bytes = (uint32_t)((item.z + 15) & ~15) * 128u;
+        const unsigned char* src = a.tiles + (size_t)item.w * a.p.K * 2;
+        for (int g = 0; g < G; g++, k++) {
+          if (!qt_wait_short(bars + 8 * (MT_DONE + s), phase, abort_flag, a.error)) goto rows_done;
+          mt_copy(base + s * MT_B, src, bytes, bars + 8 * (MT_FULL + s));
+          src += bytes;
+          if (++s == MT_S) s = 0, phase ^= 1u;
         }
-        src[i] = a.x16 + (size_t)row * a.p.K + 8 * c;
       }
-      const int n16 = (item.z + 15) / 16;
-      for (int g = 0; g < G; g++) {
-        if (!qt_wait_short(bars + 8 * (MT_DONE + s), phase, abort_flag, a.error)) goto gather_done;
-        const uint32_t dst = dst0 + s * MT_B;
-#pragma unroll
-        for (int i = 0; i < MT_N / 16; i++) {
-          if (i < n16)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + (uint32_t)(i * 2048)), "l"(src[i])
-                         : "memory");
-          src[i] += 64;
-        }
-        // arrives once this thread's copies have landed
-        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bars + 8 * (MT_FULL + s)) : "memory");
-        if (++s == MT_S) s = 0, phase ^= 1u;
-      }
+    rows_done:
+      if (*abort_flag)  // copies still landing finish before the CTA exits (a second a stage is ample, and the limit
+                        // where the expansion's arrivals never come)
+        for (int j = k > MT_S ? k - MT_S : 0; j < k; j++)
+          qt_drain(reinterpret_cast<unsigned long long*>(sbase + MT_OFF_BAR) + MT_FULL + j % MT_S,
+                   (uint32_t)((j / MT_S) & 1));
     }
-  gather_done:
-    asm volatile("cp.async.wait_all;" ::: "memory");
   } else {
-    // ---- code expansion: set 0 takes the even steps of the CTA's sequence, set 1 the odd ones ---------------------
+    // ---- code expansion: set i takes every fourth step of the CTA's sequence, from step i on ------------------------
     const int set = (warp - MT_W_TRANS) >> 2, q = warp & 3;
     const uint32_t code_off = (uint32_t)(q * 1024 + lane * 16);
     const uint32_t sb_off = (uint32_t)(4096 + q * 128 + (lane & 7) * 16 + (lane >> 3) * 2);
@@ -444,23 +443,24 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
     for (int tile = blockIdx.x; tile < ntiles; tile += gridDim.x) {
       const int expert = a.items[tile / a.cols].x;
       if (expert == a.p.E) continue;
-      const float inv = mt_pow2(-mt_exp(a.wmax[expert], 8));
+      const float inv = mt_pow2(
+          -mt_exp(a.row_max[((size_t)expert * a.cols + tile % a.cols) * 128 + q * 32 + lane], MT_WBITS));
       int g = skip;
-      for (; g < G; g += 2) {
+      for (; g < G; g += MT_SETS) {
         if (!qt_wait_short(bars + 8 * (MT_W_FULL + sw), wphase, abort_flag, a.error)) goto expand_done;
         const unsigned char* w = sbase + MT_OFF_W + sw * MOE_BLOCK_BYTES;
         const uint4 c0 = *reinterpret_cast<const uint4*>(w + code_off);
         const uint4 c1 = *reinterpret_cast<const uint4*>(w + code_off + 512);
         const float sf = bf(*reinterpret_cast<const uint16_t*>(w + sb_off)) * inv;
-        const float of = bf(*reinterpret_cast<const uint16_t*>(w + sb_off + 8)) * inv;
-        const __half2 s2 = __float2half2_rn(sf), b2 = __float2half2_rn(of);
+        const __half2 s24 = __float2half2_rn(sf * 16777216.f), s20 = __float2half2_rn(sf * 1048576.f);
+        const __half2 b2 = __float2half2_rn(bf(*reinterpret_cast<const uint16_t*>(w + sb_off + 8)) * inv);
         uint32_t p[32];
         const uint32_t words[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
 #pragma unroll
-        for (int i = 0; i < 8; i++) mt_expand(words[i], s2, b2, p + 4 * i);
+        for (int i = 0; i < 8; i++) mt_expand(words[i], s24, s20, b2, p + 4 * i);
         __syncwarp();
         if (lane == 0) mt_arrive(bars + 8 * (MT_W_EMPTY + sw));
-        if ((sw += 2) >= MT_W) sw -= MT_W, wphase ^= 1u;
+        if ((sw += MT_SETS) >= MT_W) sw -= MT_W, wphase ^= 1u;
         if (!qt_wait_short(bars + 8 * (MT_DONE + s), phase, abort_flag, a.error)) goto expand_done;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile(
@@ -476,7 +476,7 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncwarp();
         if (lane == 0) mt_arrive(bars + 8 * (MT_FULL + s));
-        if ((s += 2) >= MT_S) s -= MT_S, phase ^= 1u;
+        if ((s += MT_SETS) >= MT_S) s -= MT_S, phase ^= 1u;
       }
       skip = g - G;
     }
@@ -491,29 +491,33 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
   }
 }
 
-// Workspace of the tensor-core path: the scaled rows and their factors.
-MoeTcSpace moe_tc_space(int64_t rows, int64_t K, int64_t pairs, int64_t I) {
+// Workspace of the tensor-core path: the items' rows as tiles (each item rounded up to 16 rows), their factors, the
+// same of the gated activations (I > 0).
+MoeTcSpace moe_tc_space(const MoePlan& p, int64_t pairs, int64_t K, int64_t I) {
   MoeTcSpace s;
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t r = at;
-    at += (bytes + 255) / 256 * 256;
+    at += (bytes + 1023) / 1024 * 1024;
     return r;
   };
-  s.x16 = take((size_t)rows * K * 2);
-  s.xscale = take((size_t)rows * 4);
-  s.xlog = take((size_t)rows * 4);
-  s.h16 = take((size_t)pairs * I * 2);
+  const size_t padded = (size_t)(pairs + 15 * p.max_items);
+  s.tiles = take(padded * K * 2);
+  s.scale = take((size_t)pairs * 4);
+  s.xlog = take((size_t)pairs * 4);
+  s.next = take(padded * I * 2);
   s.hscale = take(I ? (size_t)pairs * 4 : 0);
   s.total = at;
   return s;
 }
 
-int moe_prep_launch(const uint16_t* x, int64_t rows, int64_t K, const MoeTcSpace& s, void* workspace,
-                    cudaStream_t st) {
+int moe_prep_launch(const MoePlan& p, const MoeProduct& a, const MoeTcSpace& s, void* workspace, cudaStream_t st) {
   char* ws = reinterpret_cast<char*>(workspace);
-  return launch("moe_prep_kernel", moe_prep_kernel, dim3((unsigned)rows), dim3(256), 0, st, x, (int)K,
-                reinterpret_cast<__half*>(ws + s.x16), reinterpret_cast<float*>(ws + s.xscale),
+  const int64_t most = a.M < MOE_TC_ROWS ? a.M : MOE_TC_ROWS;  // rows of an item
+  return launch("moe_prep_kernel", moe_prep_kernel,
+                dim3((unsigned)p.max_items, (unsigned)((most + MP_ROWS - 1) / MP_ROWS)), dim3(MP_ROWS * 32), 0, st, a.x,
+                a.plan, a.pairs, a.E, a.top_k, (int)(a.src == MOE_BY_PAIR), a.K,
+                reinterpret_cast<unsigned char*>(ws + s.tiles), reinterpret_cast<float*>(ws + s.scale),
                 reinterpret_cast<float*>(ws + s.xlog));
 }
 
@@ -542,14 +546,16 @@ int moe_tc_launch(const MoePlan& p, const MoeProduct& prod, const MoeTcSpace& s,
   a.p = prod;
   a.items = reinterpret_cast<const int4*>(prod.plan + MOE_PLAN_HEADER);
   a.error = reinterpret_cast<unsigned*>(const_cast<int*>(prod.plan)) + 1;
-  a.x16 = reinterpret_cast<const __half*>(ws + (second ? s.h16 : s.x16));
-  a.xscale = reinterpret_cast<const float*>(ws + (second ? s.hscale : s.xscale));
+  a.tiles = reinterpret_cast<const unsigned char*>(ws + (second ? s.next : s.tiles));
+  a.scale = reinterpret_cast<const float*>(ws + (second ? s.hscale : s.scale));
   a.xlog = reinterpret_cast<const float*>(ws + s.xlog);
+  a.next = reinterpret_cast<unsigned char*>(ws + s.next);
   a.hscale = reinterpret_cast<float*>(ws + s.hscale);
   const int G = prod.K / 64;
   a.cols = (prod.N + 127) / 128;
   a.expert_bytes = (size_t)a.cols * G * MOE_BLOCK_BYTES;
-  a.wmax = reinterpret_cast<const float*>(prod.wp + (size_t)prod.E * a.expert_bytes);
+  a.row_max = reinterpret_cast<const float*>(prod.wp + (size_t)prod.E * a.expert_bytes);
+  a.half_max = a.row_max + (size_t)prod.E * a.cols * 128;
   const int64_t tiles = p.max_items * a.cols;
   IM_REQUIRE(tiles < (1ll << 31), IM_UNSUPPORTED, "grouped product: too many tiles");
   if (prod.epilogue == IM_EPI_STORE) return mt_launch<false>(a, tiles, st);

@@ -627,7 +627,7 @@ def grouped_qgemm(x: torch.Tensor, experts: Experts, routing: Routing, *,
     out = _moe_out(out, (routing.rows, routing.top_k, experts.n), x.device)
     path = _PATHS[routing.path]
     need = int(_lib.load().im_moe_grouped_workspace_bytes(routing.rows, experts.e, routing.top_k, experts.k,
-                                                          int(by_pair), path))
+                                                          path))
     ws = torch.empty(need, dtype=torch.uint8, device=x.device)
     _lib.call("im_moe_grouped_qgemm", experts.data.data_ptr(), x.data_ptr(), out.data_ptr(), routing.rows, experts.e,
               routing.top_k, experts.n, experts.k, int(by_pair), routing.pairs.data_ptr(), path,

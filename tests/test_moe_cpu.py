@@ -48,12 +48,12 @@ def test_plan_sizes():
         for path in range(3):
             assert lib.im_moe_plan_bytes(m, e, k, path) >= 32 + 16 * min(pairs, e + 1)
             assert lib.im_moe_plan_bytes(m, e, k, path) <= 32 + 16 * (min(pairs, e + 1) + pairs / 8) + 4 * 148 * (e + 1)
-    assert lib.im_moe_packed_bytes(3, 33, 128) == 3 * (2 * 4608 + 4)  # 128-output blocks of 64-wide groups
+    assert lib.im_moe_packed_bytes(3, 33, 128) == 3 * (2 * 4608 + 512 + 8)  # 128-output blocks of 64-wide groups, maxima
     assert lib.im_moe_packed_bytes(3, 33, 100) == 0
     assert lib.im_moe_mlp_workspace_bytes(4, 8, 2, 128, 64, _lib.MOE_WARP) == 4 * 2 * 64 * 2
     assert lib.im_moe_mlp_workspace_bytes(4, 8, 2, 100, 64, _lib.MOE_WARP) == 0
-    assert lib.im_moe_grouped_workspace_bytes(4, 8, 2, 128, 0, _lib.MOE_WARP) == 0
-    assert lib.im_moe_grouped_workspace_bytes(4, 8, 2, 128, 0, _lib.MOE_TENSOR) >= 4 * 128 * 2
+    assert lib.im_moe_grouped_workspace_bytes(4, 8, 2, 128, _lib.MOE_WARP) == 0
+    assert lib.im_moe_grouped_workspace_bytes(4, 8, 2, 128, _lib.MOE_TENSOR) >= 4 * 128 * 2
 
 
 def test_product_refusals():
