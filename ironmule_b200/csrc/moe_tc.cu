@@ -15,15 +15,16 @@
 // The factors return in float32 after the sum. A row with infinities or NaN gives those.
 //
 // A persistent grid (one CTA per SM) walks tiles; its warps are coupled by mbarriers only:
-//  * warp 0 copies each 64-wide group of packed weights (4608 contiguous bytes) into a ring of 12;
-//  * warps 12-27, four sets of 4, expand a group each: thread = output row, 64 codes -> 32 registers of fp16 pairs ->
+//  * warp 0 copies the packed weights, two 64-wide groups (9216 contiguous bytes) at a time, into a ring of 8 (one
+//    thread starts a copy every 280 cycles or so, whatever its size: hence two groups a stage everywhere);
+//  * warps 12-27, four sets of 4, expand a group each (two sets a stage): thread = output row, 64 codes -> 32 registers of fp16 pairs ->
 //    tensor memory, where the MMA reads A directly. Neither shared memory nor its bandwidth carries expanded weights;
-//  * warp 10 copies the item's rows of the group, one contiguous copy: moe_prep_kernel lays each item's rows out as the
+//  * warp 10 copies the item's rows of a stage, one contiguous copy: moe_prep_kernel lays each item's rows out as the
 //    K-major 128-byte-swizzled tiles that the MMA reads, and the gated epilogue writes its outputs as the next
 //    product's tiles. (Gathering here was measured: TMA gather4 of 128-byte rows takes 64 cycles a row quadruple, and
 //    16-byte asynchronous copies occupied four warps and the load pipe; a prefill took 1407 and 527 us.) The k order
 //    within 8 follows the code expansion (k, k + 4 adjacent);
-//  * warp 1 issues 4 MMAs of K = 16 a group into one of two 128-column accumulators;
+//  * warp 1 issues 8 MMAs of K = 16 a stage into one of two 128-column accumulators;
 //  * warps 2-9, two sets of 4 for alternate 32 columns, read a finished accumulator (lane = output), scale it, apply
 //    the gate, and store.
 // Every column (row of x) is its own sum in K order, so a row's bits do not depend on the other rows.
@@ -41,19 +42,19 @@
 namespace im {
 
 constexpr int MT_N = MOE_TC_ROWS;       // rows of an item at most (MMA N)
-constexpr int MT_S = 8;                 // A and B stages
-constexpr int MT_W = 12;                // weight ring
-constexpr int MT_B = MT_N * 128;        // bytes of a B stage
+constexpr int MT_S = 4;                 // A and B stages of two groups (128 of K)
+constexpr int MT_W = 8;                 // weight ring, two groups each
+constexpr int MT_B = 2 * MT_N * 128;    // bytes of a B stage
 constexpr int MT_EPI = 8;               // epilogue warps
 constexpr int MT_SETS = 4;              // expansion sets of four warps
 constexpr int MT_W_EPI = 2, MT_W_LOAD = MT_W_EPI + MT_EPI, MT_W_TRANS = MT_W_LOAD + 2;  // first warps of the roles
 constexpr int MT_THREADS = (MT_W_TRANS + 4 * MT_SETS) * 32;
-static_assert(MT_S % MT_SETS == 0 && MT_W % MT_SETS == 0, "a set keeps its stages");
+static_assert(MT_S % 2 == 0 && MT_W % 2 == 0 && MT_SETS == 4, "sets 0, 1 take the even stages, 2, 3 the odd ones");
 constexpr int MT_WBITS = -6;            // an expert's largest weight lands in [2^-7, 2^-6)
-constexpr uint32_t MT_TMEM = 512;       // 2 accumulators of 128 columns, 8 A stages of 32
+constexpr uint32_t MT_TMEM = 512;       // 2 accumulators of 128 columns, 4 A stages of 64
 constexpr int MT_A0 = 256;
 constexpr size_t MT_OFF_W = (size_t)MT_S * MT_B;
-constexpr size_t MT_OFF_BAR = MT_OFF_W + (size_t)MT_W * MOE_BLOCK_BYTES;
+constexpr size_t MT_OFF_BAR = MT_OFF_W + (size_t)MT_W * 2 * MOE_BLOCK_BYTES;
 // barriers: a stage's MMAs completed; a stage's A and B in place; weight ring; accumulators
 constexpr int MT_DONE = 0, MT_FULL = MT_DONE + MT_S, MT_W_FULL = MT_FULL + MT_S, MT_W_EMPTY = MT_W_FULL + MT_W,
               MT_D_FULL = MT_W_EMPTY + MT_W, MT_D_EMPTY = MT_D_FULL + 2, MT_BARS = MT_D_EMPTY + 2;
@@ -190,6 +191,13 @@ __device__ __forceinline__ void mt_copy(uint32_t dst, const void* src, uint32_t 
                : "memory");
 }
 
+__device__ __forceinline__ void mt_mma(uint32_t d, uint32_t ta, uint64_t bd, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+      "r"(ta), "l"(bd), "r"(idesc), "r"((uint32_t)add));
+}
+
 __device__ __forceinline__ void mt_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
@@ -217,11 +225,11 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
     unsigned long long* b = reinterpret_cast<unsigned long long*>(sbase + MT_OFF_BAR);
     for (int s = 0; s < MT_S; s++) {
       qt_init(&b[MT_DONE + s], 1u);
-      qt_init(&b[MT_FULL + s], 4u + 1u);  // four expansion warps, the rows' bytes
+      qt_init(&b[MT_FULL + s], 8u + 1u);  // eight expansion warps, the rows' bytes
     }
     for (int s = 0; s < MT_W; s++) {
       qt_init(&b[MT_W_FULL + s], 1u);
-      qt_init(&b[MT_W_EMPTY + s], 4u);
+      qt_init(&b[MT_W_EMPTY + s], 8u);
     }
     for (int s = 0; s < 2; s++) {
       qt_init(&b[MT_D_FULL + s], 1u);
@@ -248,10 +256,11 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
         if (expert == a.p.E) continue;
         const unsigned char* src =
             a.p.wp + (size_t)expert * a.expert_bytes + (size_t)(tile % a.cols) * G * MOE_BLOCK_BYTES;
-        for (int g = 0; g < G; g++, k++) {
+        for (int g = 0; g < G; g += 2, k++) {
           if (!qt_wait_short(bars + 8 * (MT_W_EMPTY + s), phase ^ 1u, abort_flag, a.error)) goto weights_done;
-          mt_copy(base + (uint32_t)MT_OFF_W + s * MOE_BLOCK_BYTES, src, MOE_BLOCK_BYTES, bars + 8 * (MT_W_FULL + s));
-          src += MOE_BLOCK_BYTES;
+          mt_copy(base + (uint32_t)MT_OFF_W + s * 2 * MOE_BLOCK_BYTES, src, g + 1 < G ? 2 * MOE_BLOCK_BYTES : MOE_BLOCK_BYTES,
+                  bars + 8 * (MT_W_FULL + s));
+          src += 2 * MOE_BLOCK_BYTES;
           if (++s == MT_W) s = 0, phase ^= 1u;
         }
       }
@@ -272,22 +281,23 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
       if (item.x == a.p.E) continue;
       // f32 accumulate, f16 A and B, K-major, N = the item's rows in sixteens, M = 128
       const uint32_t idesc = (1u << 4) | ((uint32_t)((item.z + 15) / 16 * 2) << 17) | ((128u >> 4) << 24);
+      const uint32_t tile_step = (uint32_t)((item.z + 15) / 16 * 128);  // (16 bytes units) to the second group's rows
       const int buf = t & 1;
       if (!qt_wait_short(bars + 8 * (MT_D_EMPTY + buf), (uint32_t)((t / 2 + 1) & 1), abort_flag, a.error)) break;
       const uint32_t d = tmem + (uint32_t)(buf * MT_N);
       int g = 0;
-      for (; g < G; g++, k++) {
+      for (; g < G; g += 2, k++) {
         if (!qt_wait_short(bars + 8 * (MT_FULL + s), phase, abort_flag, a.error)) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         if (leader) {
-          const uint64_t bd = qt_desc(base + s * MT_B);
-          const uint32_t ta = tmem + MT_A0 + 32 * s;
+          const uint64_t bd = qt_desc(base + s * MT_B), bd1 = bd + tile_step;
+          const uint32_t ta = tmem + MT_A0 + 64 * s;
 #pragma unroll
-          for (int q = 0; q < 4; q++)
-            asm volatile(
-                "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
-                "r"(ta + 8 * q), "l"(bd + 2 * q), "r"(idesc), "r"((uint32_t)(g + q > 0)));
+          for (int q = 0; q < 4; q++) mt_mma(d, ta + 8 * q, bd + 2 * q, idesc, g + q > 0);
+          if (g + 1 < G) {
+#pragma unroll
+            for (int q = 0; q < 4; q++) mt_mma(d, ta + 32 + 8 * q, bd1 + 2 * q, idesc, true);
+          }
           mt_commit(bars + 8 * (MT_DONE + s));
         }
         __syncwarp();
@@ -419,10 +429,10 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
         if (item.x == a.p.E) continue;
         const uint32_t bytes = (uint32_t)((item.z + 15) & ~15) * 128u;
         const unsigned char* src = a.tiles + (size_t)item.w * a.p.K * 2;
-        for (int g = 0; g < G; g++, k++) {
+        for (int g = 0; g < G; g += 2, k++) {
           if (!qt_wait_short(bars + 8 * (MT_DONE + s), phase, abort_flag, a.error)) goto rows_done;
-          mt_copy(base + s * MT_B, src, bytes, bars + 8 * (MT_FULL + s));
-          src += bytes;
+          mt_copy(base + s * MT_B, src, g + 1 < G ? 2 * bytes : bytes, bars + 8 * (MT_FULL + s));
+          src += 2 * bytes;
           if (++s == MT_S) s = 0, phase ^= 1u;
         }
       }
@@ -434,21 +444,23 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
                    (uint32_t)((j / MT_S) & 1));
     }
   } else {
-    // ---- code expansion: set i takes every fourth step of the CTA's sequence, from step i on ------------------------
-    const int set = (warp - MT_W_TRANS) >> 2, q = warp & 3;
-    const uint32_t code_off = (uint32_t)(q * 1024 + lane * 16);
-    const uint32_t sb_off = (uint32_t)(4096 + q * 128 + (lane & 7) * 16 + (lane >> 3) * 2);
-    uint32_t s = set, phase = 1, sw = set, wphase = 0;
-    int skip = set;  // steps of the next tile that lie before this set's next one
+    // ---- code expansion: sets 0 and 1 take the two groups of the even stages of the CTA's sequence, 2 and 3 of the
+    // odd ones -------------------------------------------------------------------------------------------------------
+    const int set = (warp - MT_W_TRANS) >> 2, q = warp & 3, half = set & 1;
+    const uint32_t code_off = (uint32_t)(half * MOE_BLOCK_BYTES + q * 1024 + lane * 16);
+    const uint32_t sb_off = (uint32_t)(half * MOE_BLOCK_BYTES + 4096 + q * 128 + (lane & 7) * 16 + (lane >> 3) * 2);
+    uint32_t s = set >> 1, phase = 1, sw = set >> 1, wphase = 0;
+    int skip = 2 * (set >> 1);  // groups of the next tile that lie before this set's next stage
+    const int even = G + (G & 1);
     for (int tile = blockIdx.x; tile < ntiles; tile += gridDim.x) {
       const int expert = a.items[tile / a.cols].x;
       if (expert == a.p.E) continue;
       const float inv = mt_pow2(
           -mt_exp(a.row_max[((size_t)expert * a.cols + tile % a.cols) * 128 + q * 32 + lane], MT_WBITS));
       int g = skip;
-      for (; g < G; g += MT_SETS) {
+      for (; g < G; g += 4) {
         if (!qt_wait_short(bars + 8 * (MT_W_FULL + sw), wphase, abort_flag, a.error)) goto expand_done;
-        const unsigned char* w = sbase + MT_OFF_W + sw * MOE_BLOCK_BYTES;
+        const unsigned char* w = sbase + MT_OFF_W + sw * 2 * MOE_BLOCK_BYTES;  // (a last odd group: stale, not used)
         const uint4 c0 = *reinterpret_cast<const uint4*>(w + code_off);
         const uint4 c1 = *reinterpret_cast<const uint4*>(w + code_off + 512);
         const float sf = bf(*reinterpret_cast<const uint16_t*>(w + sb_off)) * inv;
@@ -460,13 +472,13 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
         for (int i = 0; i < 8; i++) mt_expand(words[i], s24, s20, b2, p + 4 * i);
         __syncwarp();
         if (lane == 0) mt_arrive(bars + 8 * (MT_W_EMPTY + sw));
-        if ((sw += MT_SETS) >= MT_W) sw -= MT_W, wphase ^= 1u;
+        if ((sw += 2) >= MT_W) sw -= MT_W, wphase ^= 1u;
         if (!qt_wait_short(bars + 8 * (MT_DONE + s), phase, abort_flag, a.error)) goto expand_done;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile(
             "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
             "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(
-                tmem + ((uint32_t)(32 * q) << 16) + MT_A0 + 32 * s),
+                tmem + ((uint32_t)(32 * q) << 16) + MT_A0 + 64 * s + 32 * half),
             "r"(p[0]), "r"(p[1]), "r"(p[2]), "r"(p[3]), "r"(p[4]), "r"(p[5]), "r"(p[6]), "r"(p[7]), "r"(p[8]),
             "r"(p[9]), "r"(p[10]), "r"(p[11]), "r"(p[12]), "r"(p[13]), "r"(p[14]), "r"(p[15]), "r"(p[16]),
             "r"(p[17]), "r"(p[18]), "r"(p[19]), "r"(p[20]), "r"(p[21]), "r"(p[22]), "r"(p[23]), "r"(p[24]),
@@ -476,9 +488,9 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncwarp();
         if (lane == 0) mt_arrive(bars + 8 * (MT_FULL + s));
-        if ((s += MT_SETS) >= MT_S) s -= MT_S, phase ^= 1u;
+        if ((s += 2) >= MT_S) s -= MT_S, phase ^= 1u;
       }
-      skip = g - G;
+      skip = g - even;
     }
   expand_done:;
   }
