@@ -370,25 +370,23 @@ int im_philox4x32_10(uint64_t seed, uint64_t offset, uint32_t stream_id, uint32_
  *   IM_MOE_SIGMOID: 1 / (1 + exp(-v)), divided by the chosen experts' sum (normalise) or as it is.
  * pairs [M * top_k] holds the pairs sorted by expert (ascending within one; places without an expert last),
  * offsets [E + 2] where each expert's begin (offsets[E]: the places without one, offsets[E + 1] = M * top_k). `plan`
- * (16-byte aligned, im_moe_plan_bytes(M, E, top_k, path) bytes, nothing to initialise) holds the work items of the
- * products; `path` chooses their kernel (IM_MOE_*) and must be the same in every call that uses the plan. E <= 512,
- * top_k <= min(E, 32).
+ * (16-byte aligned, im_moe_plan_bytes(M, E, top_k) bytes, nothing to initialise) holds the work items of the products.
+ * E <= 512, top_k <= min(E, 32).
  *
  * im_moe_pack_w4g64: E matrices w [E, N, K/8], scales and biases [E, N, K/64] -> packed units, expert after expert
  * (im_moe_packed_bytes(E, N, K) bytes, 16-byte aligned).
  *
  * im_moe_grouped_qgemm: y[p] = W[id(p)] x[p / top_k] (x [M, K]), or x[p] with x_by_pair (x [M, top_k, K]); y bf16
- * [M, top_k, N], zero for places without an expert. pairs and plan come from im_moe_route with the same M, E, top_k,
- * path. Its workspace, like im_moe_mlp's, is 256-byte aligned with nothing to initialise.
+ * [M, top_k, N], zero for places without an expert. pairs and plan come from im_moe_route with the same M, E,
+ * top_k. Its workspace, like im_moe_mlp's, is 256-byte aligned with nothing to initialise.
  *
  * im_moe_mlp: y[p] = D[e] (act(G[e] x) * (U[e] x)), e = id(p), x = x[p / top_k]; act IM_EPI_SWIGLU or IM_EPI_GEGLU.
  * gate_up is packed from [E, 2 I, H] with gate and up rows interleaved in 16-row blocks, down from [E, H, I]; y
  * [M, top_k, H].
  *
- * The products' kernels: the warp-MMA kernel (IM_MOE_WARP: exact codes in bf16, hidden activations rounded to bf16) for
- * few rows an expert, the tcgen05 kernel (IM_MOE_TENSOR: operands in fp16 scaled by powers of two) for more; IM_MOE_AUTO
- * picks by M, E and top_k. Sums are float32; within one kernel a pair's result does not depend on the other rows.
- * im_moe_status: the plan's error word (0: every bounded wait of the tcgen05 kernel completed); synchronises.
+ * The products run on tcgen05 with operands in fp16 scaled by powers of two and float32 sums; a pair's result does not
+ * depend on the other rows, whatever the batch. im_moe_status: the plan's error word (0: every bounded wait of the
+ * products completed); synchronises.
  *
  * im_block_residual: joins the places of a block, and the block to the residual stream, and takes the next norm:
  *   b = sum_j weights[m, j] y[m, j] (places of weight 0 are not read; weights NULL: the one place as it is)
@@ -399,22 +397,21 @@ int im_philox4x32_10(uint64_t seed, uint64_t offset, uint32_t stream_id, uint32_
  * h_out rows, what im_qgemm_packed's RMSNorm prologue takes. H <= 16384, places <= 32.
  */
 enum { IM_MOE_SOFTMAX = 0, IM_MOE_SIGMOID = 1 };
-enum { IM_MOE_AUTO = 0, IM_MOE_WARP = 1, IM_MOE_TENSOR = 2 };
-size_t im_moe_plan_bytes(int64_t M, int64_t E, int64_t top_k, int path);
+size_t im_moe_plan_bytes(int64_t M, int64_t E, int64_t top_k);
 int im_moe_route(const void* logits, int logits_f32, int64_t M, int64_t E, int64_t ld, const float* bias,
                  int64_t top_k, int scoring, int normalise, float scale, int32_t* ids, float* weights,
-                 int32_t* offsets, int32_t* pairs, int path, void* plan, size_t plan_bytes, void* stream);
+                 int32_t* offsets, int32_t* pairs, void* plan, size_t plan_bytes, void* stream);
 int im_moe_status(const void* plan);
 size_t im_moe_packed_bytes(int64_t E, int64_t N, int64_t K);
 int im_moe_pack_w4g64(const uint32_t* w, const uint16_t* scales, const uint16_t* biases, int64_t E, int64_t N,
                       int64_t K, void* packed, void* stream);
-size_t im_moe_grouped_workspace_bytes(int64_t M, int64_t E, int64_t top_k, int64_t K, int path);
+size_t im_moe_grouped_workspace_bytes(int64_t M, int64_t E, int64_t top_k, int64_t K);
 int im_moe_grouped_qgemm(const void* packed, const uint16_t* x, uint16_t* y, int64_t M, int64_t E, int64_t top_k,
-                         int64_t N, int64_t K, int x_by_pair, const int32_t* pairs, int path, void* plan,
-                         size_t plan_bytes, void* workspace, size_t workspace_bytes, void* stream);
-size_t im_moe_mlp_workspace_bytes(int64_t M, int64_t E, int64_t top_k, int64_t H, int64_t I, int path);
+                         int64_t N, int64_t K, int x_by_pair, const int32_t* pairs, void* plan, size_t plan_bytes,
+                         void* workspace, size_t workspace_bytes, void* stream);
+size_t im_moe_mlp_workspace_bytes(int64_t M, int64_t E, int64_t top_k, int64_t H, int64_t I);
 int im_moe_mlp(const void* gate_up, const void* down, const uint16_t* x, uint16_t* y, int64_t M, int64_t E,
-               int64_t top_k, int64_t H, int64_t I, int activation, const int32_t* pairs, int path, void* plan,
+               int64_t top_k, int64_t H, int64_t I, int activation, const int32_t* pairs, void* plan,
                size_t plan_bytes, void* workspace, size_t workspace_bytes, void* stream);
 int im_block_residual(const uint16_t* y, const float* weights, int64_t places, const uint16_t* h,
                       const uint16_t* post_norm, const uint16_t* gate, int64_t gate_row_stride,

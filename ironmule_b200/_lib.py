@@ -15,7 +15,6 @@ LIB_PATH = HERE / "libimspec.so"
 IM_OK, IM_UNSUPPORTED, IM_INVALID, IM_CUDA_ERROR = 0, 1, 2, 3
 EPI_STORE, EPI_RESIDUAL, EPI_SWIGLU, EPI_GEGLU = 0, 1, 2, 3
 MOE_SOFTMAX, MOE_SIGMOID = 0, 1
-MOE_AUTO, MOE_WARP, MOE_TENSOR = 0, 1, 2
 QGEMM_AUTO, QGEMM_MMA, QGEMM_FMA = 0, 1, 2
 ABI_VERSION = 1
 
@@ -79,16 +78,16 @@ SIGNATURES: dict[str, tuple] = {
                                     ctypes.c_uint64, ctypes.c_uint64, _P, _P, _P, _P, _P, _SZ, _P]),
     "im_sample_rows": (_INT, [_P, _I64, _I64, _I64, ctypes.c_float, ctypes.c_float, ctypes.c_uint64,
                               ctypes.c_uint64, _P, _P, ctypes.c_uint32, _P, _I64, _P, _SZ, _P]),
-    "im_moe_plan_bytes": (_SZ, [_I64, _I64, _I64, _INT]),
-    "im_moe_route": (_INT, [_P, _INT, _I64, _I64, _I64, _P, _I64, _INT, _INT, ctypes.c_float, _P, _P, _P, _P, _INT, _P,
-                            _SZ, _P]),
+    "im_moe_plan_bytes": (_SZ, [_I64, _I64, _I64]),
+    "im_moe_route": (_INT, [_P, _INT, _I64, _I64, _I64, _P, _I64, _INT, _INT, ctypes.c_float, _P, _P, _P, _P, _P, _SZ,
+                            _P]),
     "im_moe_status": (_INT, [_P]),
     "im_moe_packed_bytes": (_SZ, [_I64, _I64, _I64]),
     "im_moe_pack_w4g64": (_INT, [_P, _P, _P, _I64, _I64, _I64, _P, _P]),
-    "im_moe_grouped_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64, _INT]),
-    "im_moe_grouped_qgemm": (_INT, [_P, _P, _P, _I64, _I64, _I64, _I64, _I64, _INT, _P, _INT, _P, _SZ, _P, _SZ, _P]),
-    "im_moe_mlp_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64, _I64, _INT]),
-    "im_moe_mlp": (_INT, [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _INT, _P, _INT, _P, _SZ, _P, _SZ, _P]),
+    "im_moe_grouped_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64]),
+    "im_moe_grouped_qgemm": (_INT, [_P, _P, _P, _I64, _I64, _I64, _I64, _I64, _INT, _P, _P, _SZ, _P, _SZ, _P]),
+    "im_moe_mlp_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64, _I64]),
+    "im_moe_mlp": (_INT, [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _INT, _P, _P, _SZ, _P, _SZ, _P]),
     "im_block_residual": (_INT, [_P, _P, _I64, _P, _P, _P, _I64, _I64, ctypes.c_float, _P, ctypes.c_float, _INT, _I64,
                                  _I64, _P, _P, _P, _P]),
     "im_philox4x32_10": (_INT, [ctypes.c_uint64, ctypes.c_uint64, ctypes.c_uint32, ctypes.c_uint32, _P, _P]),

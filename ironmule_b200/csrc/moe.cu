@@ -8,17 +8,16 @@
 namespace im {
 
 // The checks that both entry points share; IM_OK when the sizes and the plan are usable.
-static int moe_check(const char* who, int64_t M, int64_t E, int64_t top_k, const int32_t* pairs, int path,
-                     const void* plan, size_t plan_bytes) {
+static int moe_check(const char* who, int64_t M, int64_t E, int64_t top_k, const int32_t* pairs, const void* plan,
+                     size_t plan_bytes) {
   IM_REQUIRE(M >= 0 && E >= 1 && top_k >= 1 && top_k <= E, IM_INVALID, "%s: bad sizes M=%lld E=%lld top_k=%lld", who,
              (long long)M, (long long)E, (long long)top_k);
   IM_REQUIRE(M <= MOE_MAX_ROWS && E <= MOE_MAX_EXPERTS && top_k <= MOE_MAX_TOP_K, IM_UNSUPPORTED,
              "%s: at most %lld rows, %d experts and %d places a row", who, (long long)MOE_MAX_ROWS, MOE_MAX_EXPERTS,
              MOE_MAX_TOP_K);
-  IM_REQUIRE(path >= IM_MOE_AUTO && path <= IM_MOE_TENSOR, IM_INVALID, "%s: bad path", who);
   if (M == 0) return IM_OK;
   IM_REQUIRE(pairs && plan && aligned(plan, 16), IM_INVALID, "%s: null or misaligned plan", who);
-  const size_t need = moe_plan(M, E, top_k, path).bytes;
+  const size_t need = moe_plan(M, E, top_k).bytes;
   IM_REQUIRE(plan_bytes >= need, IM_INVALID, "%s: plan of %zu bytes needed, %zu given", who, need, plan_bytes);
   return IM_OK;
 }
@@ -110,19 +109,19 @@ extern "C" int im_moe_status(const void* plan) {
   return word;
 }
 
-extern "C" size_t im_moe_grouped_workspace_bytes(int64_t M, int64_t E, int64_t top_k, int64_t K, int path) {
+extern "C" size_t im_moe_grouped_workspace_bytes(int64_t M, int64_t E, int64_t top_k, int64_t K) {
   if (M < 1 || M > MOE_MAX_ROWS || E < 1 || E > MOE_MAX_EXPERTS || top_k < 1 || top_k > MOE_MAX_TOP_K || top_k > E ||
-      !moe_nk_ok(1, K) || moe_plan(M, E, top_k, path).item_rows != MOE_TC_ROWS)
+      !moe_nk_ok(1, K))
     return 0;
-  return moe_tc_space(moe_plan(M, E, top_k, path), M * top_k, K, 0).total;
+  return moe_space(moe_plan(M, E, top_k), M * top_k, K, 0).total;
 }
 
 extern "C" int im_moe_grouped_qgemm(const void* packed, const uint16_t* x, uint16_t* y, int64_t M, int64_t E,
-                                    int64_t top_k, int64_t N, int64_t K, int x_by_pair, const int32_t* pairs, int path,
+                                    int64_t top_k, int64_t N, int64_t K, int x_by_pair, const int32_t* pairs,
                                     void* plan, size_t plan_bytes, void* workspace, size_t workspace_bytes,
                                     void* stream) {
   clear_error();
-  const int rc = moe_check("im_moe_grouped_qgemm", M, E, top_k, pairs, path, plan, plan_bytes);
+  const int rc = moe_check("im_moe_grouped_qgemm", M, E, top_k, pairs, plan, plan_bytes);
   if (rc) return rc;
   IM_REQUIRE(moe_nk_ok(N, K), IM_INVALID, "im_moe_grouped_qgemm: bad sizes N=%lld K=%lld", (long long)N,
              (long long)K);
@@ -130,12 +129,11 @@ extern "C" int im_moe_grouped_qgemm(const void* packed, const uint16_t* x, uint1
   IM_REQUIRE(packed && x && y, IM_INVALID, "im_moe_grouped_qgemm: null pointer");
   IM_REQUIRE(aligned(packed, 16) && aligned(x, 16) && aligned(y, 2), IM_INVALID,
              "im_moe_grouped_qgemm: packed and x must be 16-byte aligned");
-  const size_t need = im_moe_grouped_workspace_bytes(M, E, top_k, K, path);
-  IM_REQUIRE(!need || (workspace && aligned(workspace, 256) && workspace_bytes >= need), IM_INVALID,
+  const size_t need = im_moe_grouped_workspace_bytes(M, E, top_k, K);
+  IM_REQUIRE(workspace && aligned(workspace, 256) && workspace_bytes >= need, IM_INVALID,
              "im_moe_grouped_qgemm: workspace of %zu bytes (256-aligned) needed, %zu given", need, workspace_bytes);
   MoeProduct a = {};
   a.wp = reinterpret_cast<const unsigned char*>(packed);
-  a.x = x;
   a.y = y;
   a.plan = reinterpret_cast<const int*>(plan);
   a.pairs = pairs;
@@ -144,31 +142,26 @@ extern "C" int im_moe_grouped_qgemm(const void* packed, const uint16_t* x, uint1
   a.top_k = (int)top_k;
   a.N = (int)N;
   a.K = (int)K;
-  a.src = x_by_pair ? MOE_BY_PAIR : MOE_BY_TOKEN;
-  a.dst = MOE_BY_PAIR;
   a.epilogue = IM_EPI_STORE;
-  const MoePlan p = moe_plan(M, E, top_k, path);
+  const MoePlan p = moe_plan(M, E, top_k);
+  const MoeSpace space = moe_space(p, M * top_k, K, 0);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (p.item_rows != MOE_TC_ROWS) return moe_mma_launch(p, a, st);
-  const MoeTcSpace space = moe_tc_space(p, M * top_k, K, 0);
-  const int prep = moe_prep_launch(p, a, space, workspace, st);
-  return prep ? prep : moe_tc_launch(p, a, space, workspace, st);
+  const int prep = moe_prep_launch(p, a, x, x_by_pair != 0, space, workspace, st);
+  return prep ? prep : moe_product_launch(p, a, space, workspace, st);
 }
 
-extern "C" size_t im_moe_mlp_workspace_bytes(int64_t M, int64_t E, int64_t top_k, int64_t H, int64_t I, int path) {
+extern "C" size_t im_moe_mlp_workspace_bytes(int64_t M, int64_t E, int64_t top_k, int64_t H, int64_t I) {
   if (M < 1 || M > MOE_MAX_ROWS || E < 1 || E > MOE_MAX_EXPERTS || top_k < 1 || top_k > MOE_MAX_TOP_K || top_k > E ||
-      H < 64 || H % 64 || I < 64 || I % 64)
+      !moe_nk_ok(H, H) || !moe_nk_ok(2 * I, I))
     return 0;
-  const MoePlan p = moe_plan(M, E, top_k, path);
-  if (p.item_rows == MOE_TC_ROWS) return moe_tc_space(p, M * top_k, H, I).total;
-  return (size_t)M * top_k * I * 2;
+  return moe_space(moe_plan(M, E, top_k), M * top_k, H, I).total;
 }
 
 extern "C" int im_moe_mlp(const void* gate_up, const void* down, const uint16_t* x, uint16_t* y, int64_t M, int64_t E,
-                          int64_t top_k, int64_t H, int64_t I, int activation, const int32_t* pairs, int path,
-                          void* plan, size_t plan_bytes, void* workspace, size_t workspace_bytes, void* stream) {
+                          int64_t top_k, int64_t H, int64_t I, int activation, const int32_t* pairs, void* plan,
+                          size_t plan_bytes, void* workspace, size_t workspace_bytes, void* stream) {
   clear_error();
-  const int rc = moe_check("im_moe_mlp", M, E, top_k, pairs, path, plan, plan_bytes);
+  const int rc = moe_check("im_moe_mlp", M, E, top_k, pairs, plan, plan_bytes);
   if (rc) return rc;
   IM_REQUIRE(moe_nk_ok(H, H) && moe_nk_ok(2 * I, I), IM_INVALID,
              "im_moe_mlp: hidden and intermediate sizes are multiples of 64 (H=%lld I=%lld)", (long long)H,
@@ -178,19 +171,14 @@ extern "C" int im_moe_mlp(const void* gate_up, const void* down, const uint16_t*
   IM_REQUIRE(gate_up && down && x && y, IM_INVALID, "im_moe_mlp: null pointer");
   IM_REQUIRE(aligned(gate_up, 16) && aligned(down, 16) && aligned(x, 16) && aligned(y, 2), IM_INVALID,
              "im_moe_mlp: weights and x must be 16-byte aligned");
-  const size_t need = im_moe_mlp_workspace_bytes(M, E, top_k, H, I, path);
+  const size_t need = im_moe_mlp_workspace_bytes(M, E, top_k, H, I);
   IM_REQUIRE(workspace && aligned(workspace, 256) && workspace_bytes >= need, IM_INVALID,
              "im_moe_mlp: workspace of %zu bytes (256-aligned) needed, %zu given", need, workspace_bytes);
-  const MoePlan p = moe_plan(M, E, top_k, path);
+  const MoePlan p = moe_plan(M, E, top_k);
+  const MoeSpace space = moe_space(p, M * top_k, H, I);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const bool tc = p.item_rows == MOE_TC_ROWS;
-  const MoeTcSpace space = tc ? moe_tc_space(p, M * top_k, H, I) : MoeTcSpace{};
-  // the gated activations lie in the order of the sorted pairs, so that an item's rows are contiguous
-  uint16_t* hidden = reinterpret_cast<uint16_t*>(workspace);  // (the tensor-core path lays its own out)
   MoeProduct a = {};
   a.wp = reinterpret_cast<const unsigned char*>(gate_up);
-  a.x = x;
-  a.y = hidden;
   a.plan = reinterpret_cast<const int*>(plan);
   a.pairs = pairs;
   a.M = (int)M;
@@ -198,22 +186,15 @@ extern "C" int im_moe_mlp(const void* gate_up, const void* down, const uint16_t*
   a.top_k = (int)top_k;
   a.N = (int)(2 * I);
   a.K = (int)H;
-  a.src = MOE_BY_TOKEN;
-  a.dst = MOE_SORTED;
   a.epilogue = activation;
-  int status = IM_OK;
-  if (tc) status = moe_prep_launch(p, a, space, workspace, st);
-  if (!status) status = tc ? moe_tc_launch(p, a, space, workspace, st) : moe_mma_launch(p, a, st);
+  int status = moe_prep_launch(p, a, x, 0, space, workspace, st);
+  if (!status) status = moe_product_launch(p, a, space, workspace, st);
   if (status) return status;
   a.wp = reinterpret_cast<const unsigned char*>(down);
-  a.x = hidden;
   a.y = y;
   a.N = (int)H;
   a.K = (int)I;
-  a.src = MOE_SORTED;
-  a.dst = MOE_BY_PAIR;
   a.epilogue = IM_EPI_STORE;
-  // the first product waited for the routing before its CTAs let this launch begin
-  a.early = 1;
-  return tc ? moe_tc_launch(p, a, space, workspace, st) : moe_mma_launch(p, a, st);
+  a.second = true;
+  return moe_product_launch(p, a, space, workspace, st);
 }

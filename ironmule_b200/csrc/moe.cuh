@@ -13,7 +13,7 @@ constexpr int MOE_MAX_TOP_K = 32;
 constexpr int64_t MOE_MAX_ROWS = 1 << 22;
 constexpr int MOE_ROUTE_BLOCKS = 148;   // blocks of the routing kernels at most (one per SM)
 constexpr int MOE_ROUTE_ROWS = 64;      // rows that one block alone routes
-constexpr int MOE_TC_ROWS = 128;        // rows of a work item on the tensor-core kernel
+constexpr int MOE_ITEM_ROWS = 128;      // rows of a work item at most (MMA N)
 constexpr int MOE_PLAN_HEADER = 8;      // ints: [0] work items, [1] error word of the bounded waits
 
 // Packed weights of an expert: 128-output blocks (rows past N are zero), each a run of 64-wide groups of
@@ -33,39 +33,32 @@ struct MoeItem {
 
 // Plan layout in ints: header | items | per-block expert counts (the routing's own scratch).
 struct MoePlan {
-  int64_t item_rows;   // most rows of an item; 8, 16, 32: the warp-MMA kernel, MOE_TC_ROWS: the tensor-core kernel
   int64_t max_items;   // bound on the items of any routing of these sizes
   int64_t blocks, rows_per_block;
   int64_t counts;      // int offset of the counts
   size_t bytes;
 };
 
-// path: IM_MOE_AUTO, IM_MOE_WARP, IM_MOE_TENSOR
-MoePlan moe_plan(int64_t M, int64_t E, int64_t top_k, int path);
-
-// Where a product's input and output rows are: by token (pair / top_k), by pair, or by position in the sorted list.
-enum MoeRows { MOE_BY_TOKEN = 0, MOE_BY_PAIR = 1, MOE_SORTED = 2 };
+MoePlan moe_plan(int64_t M, int64_t E, int64_t top_k);
 
 struct MoeProduct {
-  const unsigned char* wp;  // [E] matrices in packed units
-  const uint16_t* x;
-  uint16_t* y;
+  const unsigned char* wp;  // [E] packed matrices
+  uint16_t* y;              // [M, top_k, N], or unused by the first product of a gated MLP
   const int* plan;
   const int* pairs;
   int M, E, top_k, N, K;
-  int src, dst;   // MoeRows
-  int epilogue;   // IM_EPI_STORE, IM_EPI_SWIGLU, IM_EPI_GEGLU
-  int early;      // the plan was finished before the preceding launch began: items and weights may be read before
-                  // the dependency wait
+  int epilogue;             // IM_EPI_STORE, IM_EPI_SWIGLU, IM_EPI_GEGLU
+  bool second;              // its rows are the gated activations that the first product left in the workspace
 };
 
-// Byte offsets in the workspace of the tensor-core path.
-struct MoeTcSpace {
+// Byte offsets in the products' workspace.
+struct MoeSpace {
   size_t tiles, scale, xlog, next, hscale, total;
 };
-MoeTcSpace moe_tc_space(const MoePlan& p, int64_t pairs, int64_t K, int64_t I);
-int moe_prep_launch(const MoePlan& p, const MoeProduct& a, const MoeTcSpace& s, void* workspace, cudaStream_t st);
-int moe_tc_launch(const MoePlan& p, const MoeProduct& a, const MoeTcSpace& s, void* workspace, cudaStream_t st);
-int moe_mma_launch(const MoePlan& p, const MoeProduct& a, cudaStream_t st);
+MoeSpace moe_space(const MoePlan& p, int64_t pairs, int64_t K, int64_t I);
+// x [M, K], or [M, top_k, K] with by_pair, into the workspace's operand tiles.
+int moe_prep_launch(const MoePlan& p, const MoeProduct& a, const uint16_t* x, int by_pair, const MoeSpace& s,
+                    void* workspace, cudaStream_t st);
+int moe_product_launch(const MoePlan& p, const MoeProduct& a, const MoeSpace& s, void* workspace, cudaStream_t st);
 
 }  // namespace im

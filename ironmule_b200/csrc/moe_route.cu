@@ -36,21 +36,14 @@ struct RouteArgs {
   int* counts;
   int f32, scoring, normalise;
   float scale;
-  int M, E, top_k, item_rows, rows_per_block, blocks;
+  int M, E, top_k, rows_per_block, blocks;
   long long ld;
 };
 
-MoePlan moe_plan(int64_t M, int64_t E, int64_t top_k, int path) {
+MoePlan moe_plan(int64_t M, int64_t E, int64_t top_k) {
   MoePlan p;
-  const int64_t pairs = M * top_k;
-  // rows per item by the average number of rows an expert gets; an expert never gets more than M
-  const int64_t avg = (pairs + E - 1) / E;
-  if (path == IM_MOE_TENSOR || (path == IM_MOE_AUTO && M > 8 && avg > 4))
-    p.item_rows = MOE_TC_ROWS;
-  else
-    p.item_rows = M <= 8 || avg <= 4 ? 8 : (M <= 16 || avg <= 12 ? 16 : 32);
-  const int64_t buckets = pairs < E + 1 ? pairs : E + 1;
-  p.max_items = buckets + pairs / p.item_rows;
+  const int64_t pairs = M * top_k, buckets = pairs < E + 1 ? pairs : E + 1;
+  p.max_items = buckets + pairs / MOE_ITEM_ROWS;
   const int64_t per = (M + MOE_ROUTE_BLOCKS - 1) / MOE_ROUTE_BLOCKS;
   p.rows_per_block = M <= MOE_ROUTE_ROWS ? MOE_ROUTE_ROWS : (per < 16 ? 16 : per);
   p.blocks = M <= MOE_ROUTE_ROWS ? 1 : (M + p.rows_per_block - 1) / p.rows_per_block;
@@ -193,8 +186,9 @@ struct RouteSmem {
 };
 
 // A bucket of c pairs is cut into as few items as it fits, evenly, in multiples of 8 rows.
-__device__ __forceinline__ int mr_item_rows(int c, int most) {
-  const int n = (c + most - 1) / most;
+__device__ __forceinline__ int mr_items(int c) { return (c + MOE_ITEM_ROWS - 1) / MOE_ITEM_ROWS; }
+__device__ __forceinline__ int mr_item_rows(int c) {
+  const int n = mr_items(c);
   return n ? ((c + n - 1) / n + 7) / 8 * 8 : 0;
 }
 
@@ -203,7 +197,7 @@ __device__ __forceinline__ void mr_place(const RouteArgs& a, RouteSmem& s) {
   const int nb = a.E + 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (blockIdx.x == 0) {
     for (int e = threadIdx.x; e < nb; e += MR_THREADS) {
-      const int c = s.total[e], each = mr_item_rows(c, a.item_rows), n = (c + a.item_rows - 1) / a.item_rows;
+      const int c = s.total[e], each = mr_item_rows(c), n = mr_items(c);
       s.scan[e] = n;
       s.pad[e] = n ? (n - 1) * ((each + 15) & ~15) + ((c - (n - 1) * each + 15) & ~15) : 0;
     }
@@ -222,7 +216,7 @@ __device__ __forceinline__ void mr_place(const RouteArgs& a, RouteSmem& s) {
     for (int e = threadIdx.x; e < nb; e += MR_THREADS) {
       const int c = s.total[e], first = s.cnt[0][e];
       a.offsets[e] = first;
-      const int n = (c + a.item_rows - 1) / a.item_rows, each = mr_item_rows(c, a.item_rows);
+      const int n = mr_items(c), each = mr_item_rows(c);
       for (int i = 0; i < n; i++)
         items[s.scan[e] + i] = make_int4(e, first + i * each, min(each, c - i * each), s.pad[e] + i * ((each + 15) & ~15));
     }
@@ -327,14 +321,13 @@ static bool moe_sizes_ok(int64_t M, int64_t E, int64_t top_k) {
          top_k <= E;
 }
 
-extern "C" size_t im_moe_plan_bytes(int64_t M, int64_t E, int64_t top_k, int path) {
-  return moe_sizes_ok(M, E, top_k) && path >= IM_MOE_AUTO && path <= IM_MOE_TENSOR ? moe_plan(M, E, top_k, path).bytes
-                                                                                   : 0;
+extern "C" size_t im_moe_plan_bytes(int64_t M, int64_t E, int64_t top_k) {
+  return moe_sizes_ok(M, E, top_k) ? moe_plan(M, E, top_k).bytes : 0;
 }
 
 extern "C" int im_moe_route(const void* logits, int logits_f32, int64_t M, int64_t E, int64_t ld, const float* bias,
                             int64_t top_k, int scoring, int normalise, float scale, int32_t* ids, float* weights,
-                            int32_t* offsets, int32_t* pairs, int path, void* plan, size_t plan_bytes, void* stream) {
+                            int32_t* offsets, int32_t* pairs, void* plan, size_t plan_bytes, void* stream) {
   clear_error();
   IM_REQUIRE(M >= 0 && E >= 1 && top_k >= 1 && top_k <= E, IM_INVALID,
              "im_moe_route: bad sizes M=%lld E=%lld top_k=%lld", (long long)M, (long long)E, (long long)top_k);
@@ -342,13 +335,12 @@ extern "C" int im_moe_route(const void* logits, int logits_f32, int64_t M, int64
              "im_moe_route: at most %lld rows, %d experts and %d places a row (M=%lld E=%lld top_k=%lld)",
              (long long)MOE_MAX_ROWS, MOE_MAX_EXPERTS, MOE_MAX_TOP_K, (long long)M, (long long)E, (long long)top_k);
   IM_REQUIRE(scoring == IM_MOE_SOFTMAX || scoring == IM_MOE_SIGMOID, IM_INVALID, "im_moe_route: bad scoring");
-  IM_REQUIRE(path >= IM_MOE_AUTO && path <= IM_MOE_TENSOR, IM_INVALID, "im_moe_route: bad path");
   IM_REQUIRE(offsets && plan, IM_INVALID, "im_moe_route: null pointer");
   IM_REQUIRE(M == 0 || (logits && ids && weights && pairs), IM_INVALID, "im_moe_route: null pointer");
   IM_REQUIRE(ld >= E, IM_INVALID, "im_moe_route: row stride %lld below %lld experts", (long long)ld, (long long)E);
   IM_REQUIRE(aligned(logits, logits_f32 ? 4 : 2) && aligned(plan, 16), IM_INVALID,
              "im_moe_route: misaligned logits or plan");
-  const MoePlan p = moe_plan(M, E, top_k, path);
+  const MoePlan p = moe_plan(M, E, top_k);
   IM_REQUIRE(plan_bytes >= p.bytes, IM_INVALID, "im_moe_route: plan of %zu bytes needed, %zu given", p.bytes,
              plan_bytes);
   RouteArgs a = {};
@@ -367,7 +359,6 @@ extern "C" int im_moe_route(const void* logits, int logits_f32, int64_t M, int64
   a.M = (int)M;
   a.E = (int)E;
   a.top_k = (int)top_k;
-  a.item_rows = (int)p.item_rows;
   a.rows_per_block = (int)p.rows_per_block;
   a.blocks = (int)p.blocks;
   a.ld = ld;

@@ -41,7 +41,7 @@
 
 namespace im {
 
-constexpr int MT_N = MOE_TC_ROWS;       // rows of an item at most (MMA N)
+constexpr int MT_N = MOE_ITEM_ROWS;       // rows of an item at most (MMA N)
 constexpr int MT_S = 4;                 // A and B stages of two groups (128 of K)
 constexpr int MT_W = 8;                 // weight ring, two groups each
 constexpr int MT_B = 2 * MT_N * 128;    // bytes of a B stage
@@ -503,10 +503,10 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
   }
 }
 
-// Workspace of the tensor-core path: the items' rows as tiles (each item rounded up to 16 rows), their factors, the
+// The products' workspace: the items' rows as tiles (each item rounded up to 16 rows), their factors, the
 // same of the gated activations (I > 0).
-MoeTcSpace moe_tc_space(const MoePlan& p, int64_t pairs, int64_t K, int64_t I) {
-  MoeTcSpace s;
+MoeSpace moe_space(const MoePlan& p, int64_t pairs, int64_t K, int64_t I) {
+  MoeSpace s;
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t r = at;
@@ -523,12 +523,13 @@ MoeTcSpace moe_tc_space(const MoePlan& p, int64_t pairs, int64_t K, int64_t I) {
   return s;
 }
 
-int moe_prep_launch(const MoePlan& p, const MoeProduct& a, const MoeTcSpace& s, void* workspace, cudaStream_t st) {
+int moe_prep_launch(const MoePlan& p, const MoeProduct& a, const uint16_t* x, int by_pair, const MoeSpace& s,
+                    void* workspace, cudaStream_t st) {
   char* ws = reinterpret_cast<char*>(workspace);
-  const int64_t most = a.M < MOE_TC_ROWS ? a.M : MOE_TC_ROWS;  // rows of an item
+  const int64_t most = a.M < MOE_ITEM_ROWS ? a.M : MOE_ITEM_ROWS;  // rows of an item
   return launch("moe_prep_kernel", moe_prep_kernel,
-                dim3((unsigned)p.max_items, (unsigned)((most + MP_ROWS - 1) / MP_ROWS)), dim3(MP_ROWS * 32), 0, st, a.x,
-                a.plan, a.pairs, a.E, a.top_k, (int)(a.src == MOE_BY_PAIR), a.K,
+                dim3((unsigned)p.max_items, (unsigned)((most + MP_ROWS - 1) / MP_ROWS)), dim3(MP_ROWS * 32), 0, st, x,
+                a.plan, a.pairs, a.E, a.top_k, by_pair, a.K,
                 reinterpret_cast<unsigned char*>(ws + s.tiles), reinterpret_cast<float*>(ws + s.scale),
                 reinterpret_cast<float*>(ws + s.xlog));
 }
@@ -551,15 +552,14 @@ static int mt_launch(const TcArgs& a, int64_t tiles, cudaStream_t st) {
                 MT_SMEM, st, a);
 }
 
-int moe_tc_launch(const MoePlan& p, const MoeProduct& prod, const MoeTcSpace& s, void* workspace, cudaStream_t st) {
+int moe_product_launch(const MoePlan& p, const MoeProduct& prod, const MoeSpace& s, void* workspace, cudaStream_t st) {
   char* ws = reinterpret_cast<char*>(workspace);
-  const bool second = prod.src == MOE_SORTED;
   TcArgs a = {};
   a.p = prod;
   a.items = reinterpret_cast<const int4*>(prod.plan + MOE_PLAN_HEADER);
   a.error = reinterpret_cast<unsigned*>(const_cast<int*>(prod.plan)) + 1;
-  a.tiles = reinterpret_cast<const unsigned char*>(ws + (second ? s.next : s.tiles));
-  a.scale = reinterpret_cast<const float*>(ws + (second ? s.hscale : s.scale));
+  a.tiles = reinterpret_cast<const unsigned char*>(ws + (prod.second ? s.next : s.tiles));
+  a.scale = reinterpret_cast<const float*>(ws + (prod.second ? s.hscale : s.scale));
   a.xlog = reinterpret_cast<const float*>(ws + s.xlog);
   a.next = reinterpret_cast<unsigned char*>(ws + s.next);
   a.hscale = reinterpret_cast<float*>(ws + s.hscale);

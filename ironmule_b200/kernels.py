@@ -11,8 +11,8 @@ otherwise a shared per-device buffer is used.
 from __future__ import annotations
 
 import ctypes
+import functools
 import threading
-from dataclasses import dataclass
 
 import torch
 
@@ -24,7 +24,8 @@ _VARIANTS = {"auto": _lib.QGEMM_AUTO, "mma": _lib.QGEMM_MMA, "fma": _lib.QGEMM_F
 
 
 def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    """The handle of torch's current stream on the device (without building a Stream object for it)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _check(t: torch.Tensor, name: str, dtypes: tuple, device: torch.device | None = None) -> None:
@@ -503,7 +504,6 @@ def qgemm_packed_attn(attn_ws: torch.Tensor, p: Packed, seq_rows: torch.Tensor, 
 
 # ---- mixture-of-experts blocks ------------------------------------------------------------------------------
 _SCORING = {"softmax": _lib.MOE_SOFTMAX, "sigmoid": _lib.MOE_SIGMOID}
-_PATHS = {"auto": _lib.MOE_AUTO, "warp": _lib.MOE_WARP, "tensor": _lib.MOE_TENSOR}
 
 
 class Experts:
@@ -538,40 +538,79 @@ class Experts:
         return cls(*(weave(g.contiguous(), u.contiguous()) for g, u in zip(gate, up)))
 
 
-@dataclass
 class Routing:
-    """What moe_route found: per row and place the expert (int32 [M, k], -1: none) and its weight (float32 [M, k]); the
-    pairs m * k + j sorted by expert (int32 [M * k]), where each expert's begin (int32 [E + 2]; the last bucket holds
-    the places without an expert), and the products' work items."""
-    ids: torch.Tensor
-    weights: torch.Tensor
-    offsets: torch.Tensor
-    pairs: torch.Tensor
-    plan: torch.Tensor
-    rows: int
-    experts: int
-    top_k: int
-    path: str
+    """What moe_route found, in one int32 buffer: per row and place the expert (`ids` int32 [M, k], -1: none) and its
+    weight (`weights` float32 [M, k]); the pairs m * k + j sorted by expert (`pairs` int32 [M * k]), where each expert's
+    begin (`offsets` int32 [E + 2]; the last bucket holds the places without an expert), and the products' work items.
+    The tensors are views made when they are asked for."""
+
+    __slots__ = ("buf", "rows", "experts", "top_k", "plan_bytes")
+
+    def __init__(self, rows: int, experts: int, top_k: int, device: torch.device):
+        self.rows, self.experts, self.top_k = rows, experts, top_k
+        self.plan_bytes = _plan_bytes(rows, experts, top_k)
+        self.buf = torch.empty(self._plan_at + self.plan_bytes // 4, dtype=torch.int32, device=device)
+
+    @property
+    def _plan_at(self) -> int:  # 16-byte aligned, after ids, weights, pairs and offsets
+        return (3 * self.rows * self.top_k + self.experts + 2 + 3) // 4 * 4
+
+    @property
+    def ids(self) -> torch.Tensor:
+        return self.buf[:self.rows * self.top_k].view(self.rows, self.top_k)
+
+    @property
+    def weights(self) -> torch.Tensor:
+        n = self.rows * self.top_k
+        return self.buf[n:2 * n].view(torch.float32).view(self.rows, self.top_k)
+
+    @property
+    def pairs(self) -> torch.Tensor:
+        n = self.rows * self.top_k
+        return self.buf[2 * n:3 * n]
+
+    @property
+    def offsets(self) -> torch.Tensor:
+        n = 3 * self.rows * self.top_k
+        return self.buf[n:n + self.experts + 2]
+
+    @property
+    def _pairs_ptr(self) -> int:
+        return self.buf.data_ptr() + 8 * self.rows * self.top_k
+
+    @property
+    def _plan_ptr(self) -> int:
+        return self.buf.data_ptr() + 4 * self._plan_at
 
     def status(self) -> int:
         """The error word of the products that used this routing (0: every bounded wait completed); synchronises."""
-        return int(_lib.load().im_moe_status(self.plan.data_ptr()))
+        return int(_lib.load().im_moe_status(self._plan_ptr))
+
+
+@functools.lru_cache(maxsize=4096)
+def _plan_bytes(m: int, e: int, k: int) -> int:
+    return int(_lib.load().im_moe_plan_bytes(m, e, k))
+
+
+@functools.lru_cache(maxsize=4096)
+def _grouped_workspace(m: int, e: int, k: int, kdim: int) -> int:
+    return int(_lib.load().im_moe_grouped_workspace_bytes(m, e, k, kdim))
+
+
+@functools.lru_cache(maxsize=4096)
+def _mlp_workspace(m: int, e: int, k: int, h: int, inter: int) -> int:
+    return int(_lib.load().im_moe_mlp_workspace_bytes(m, e, k, h, inter))
 
 
 def moe_route(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax", normalise: bool = True,
-              scale: float = 1.0, bias: torch.Tensor | None = None, rows: int | None = None,
-              path: str = "auto") -> Routing:
+              scale: float = 1.0, bias: torch.Tensor | None = None, rows: int | None = None) -> Routing:
     """Choose top_k experts for each of the first `rows` rows of logits [M, E] (bf16 or float32): the largest
-    logit + bias, ties to the lower expert; -inf or NaN closes an expert to a row. `path`: the kernel of the products
-    that use the routing, "warp" or "tensor"; "auto" chooses by the sizes. Within one kernel a row's results do not
-    depend on the other rows."""
+    logit + bias, ties to the lower expert; -inf or NaN closes an expert to a row."""
     _check(logits, "logits", (torch.bfloat16, torch.float32))
     if logits.dim() != 2:
         raise ValueError(f"logits must be [M, E], got {tuple(logits.shape)}")
     if scoring not in _SCORING:
         raise ValueError(f"scoring {scoring!r}: softmax or sigmoid")
-    if path not in _PATHS:
-        raise ValueError(f"path {path!r}: auto, warp or tensor")
     device, e = logits.device, logits.shape[1]
     m = logits.shape[0] if rows is None else rows
     if not 0 <= m <= logits.shape[0]:
@@ -582,23 +621,19 @@ def moe_route(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax", nor
             raise ValueError(f"bias must be [{e}], got {tuple(bias.shape)}")
     if not 1 <= top_k <= e:
         raise ValueError(f"top_k {top_k} of {e} experts")
-    ids = torch.empty((m, top_k), dtype=torch.int32, device=device)
-    weights = torch.empty((m, top_k), dtype=torch.float32, device=device)
-    offsets = torch.empty(e + 2, dtype=torch.int32, device=device)
-    pairs = torch.empty(m * top_k, dtype=torch.int32, device=device)
-    nbytes = int(_lib.load().im_moe_plan_bytes(m, e, top_k, _PATHS[path]))
-    plan = torch.empty((nbytes + 3) // 4, dtype=torch.int32, device=device)
+    r = Routing(m, e, top_k, device)
+    base, n = r.buf.data_ptr(), 4 * m * top_k
     _lib.call("im_moe_route", logits.data_ptr(), int(logits.dtype == torch.float32), m, e, e, _ptr_or_none(bias), top_k,
-              _SCORING[scoring], int(normalise), float(scale), ids.data_ptr(), weights.data_ptr(), offsets.data_ptr(),
-              pairs.data_ptr(), _PATHS[path], plan.data_ptr(), nbytes, _stream(device))
-    return Routing(ids, weights, offsets, pairs, plan, m, e, top_k, path)
+              _SCORING[scoring], int(normalise), float(scale), base, base + n, base + 3 * n, base + 2 * n,
+              r._plan_ptr, r.plan_bytes, _stream(device))
+    return r
 
 
 def _moe_rows(x: torch.Tensor, experts: Experts, routing: Routing) -> bool:
     """Check x against the routing and the weights; whether x holds a row per pair ([M, k, K]) or per row ([M, K])."""
     _check(x, "x", (torch.bfloat16,), experts.data.device)
-    if routing.ids.device != x.device:
-        raise ValueError(f"the routing is on {routing.ids.device}, x on {x.device}")
+    if routing.buf.device != x.device:
+        raise ValueError(f"the routing is on {routing.buf.device}, x on {x.device}")
     if x.shape[-1] != experts.k:
         raise ValueError(f"x has K={x.shape[-1]}, the experts {experts.k}")
     if experts.e != routing.experts:
@@ -625,13 +660,11 @@ def grouped_qgemm(x: torch.Tensor, experts: Experts, routing: Routing, *,
     places without an expert."""
     by_pair = _moe_rows(x, experts, routing)
     out = _moe_out(out, (routing.rows, routing.top_k, experts.n), x.device)
-    path = _PATHS[routing.path]
-    need = int(_lib.load().im_moe_grouped_workspace_bytes(routing.rows, experts.e, routing.top_k, experts.k,
-                                                          path))
+    need = _grouped_workspace(routing.rows, experts.e, routing.top_k, experts.k)
     ws = torch.empty(need, dtype=torch.uint8, device=x.device)
     _lib.call("im_moe_grouped_qgemm", experts.data.data_ptr(), x.data_ptr(), out.data_ptr(), routing.rows, experts.e,
-              routing.top_k, experts.n, experts.k, int(by_pair), routing.pairs.data_ptr(), path,
-              routing.plan.data_ptr(), routing.plan.numel() * 4, ws.data_ptr(), need, _stream(x.device))
+              routing.top_k, experts.n, experts.k, int(by_pair), routing._pairs_ptr, routing._plan_ptr,
+              routing.plan_bytes, ws.data_ptr(), need, _stream(x.device))
     return out
 
 
@@ -647,12 +680,11 @@ def moe_mlp(x: torch.Tensor, gate_up: Experts, down: Experts, routing: Routing, 
     if (down.e, down.n, down.k) != (gate_up.e, h, inter) or down.data.device != x.device:
         raise ValueError(f"down is {down.e} x [{down.n}, {down.k}], expected {gate_up.e} x [{h}, {inter}]")
     out = _moe_out(out, (routing.rows, routing.top_k, h), x.device)
-    need = int(_lib.load().im_moe_mlp_workspace_bytes(routing.rows, gate_up.e, routing.top_k, h, inter,
-                                                      _PATHS[routing.path]))
+    need = _mlp_workspace(routing.rows, gate_up.e, routing.top_k, h, inter)
     ws = torch.empty(need, dtype=torch.uint8, device=x.device)
     _lib.call("im_moe_mlp", gate_up.data.data_ptr(), down.data.data_ptr(), x.data_ptr(), out.data_ptr(), routing.rows,
-              gate_up.e, routing.top_k, h, inter, _EPILOGUES[activation], routing.pairs.data_ptr(),
-              _PATHS[routing.path], routing.plan.data_ptr(), routing.plan.numel() * 4, ws.data_ptr(), need, _stream(x.device))
+              gate_up.e, routing.top_k, h, inter, _EPILOGUES[activation], routing._pairs_ptr, routing._plan_ptr,
+              routing.plan_bytes, ws.data_ptr(), need, _stream(x.device))
     return out
 
 

@@ -10,9 +10,9 @@ def _status(name, *args):
     return getattr(lib, name)(*args), lib.im_last_error().decode()
 
 
-def route(m=4, e=8, ld=8, k=2, scoring=0, ptr=256, path=0, plan_bytes=1 << 20):
-    return _status("im_moe_route", ptr, 0, m, e, ld, None, k, scoring, 1, 1.0, ptr, ptr, ptr, ptr, path,
-                   ptr, plan_bytes, None)
+def route(m=4, e=8, ld=8, k=2, scoring=0, ptr=256, plan_bytes=1 << 20):
+    return _status("im_moe_route", ptr, 0, m, e, ld, None, k, scoring, 1, 1.0, ptr, ptr, ptr, ptr, ptr,
+                   plan_bytes, None)
 
 
 def test_route_refusals():
@@ -27,8 +27,6 @@ def test_route_refusals():
     assert rc == _lib.IM_UNSUPPORTED and "places" in msg
     rc, msg = route(scoring=2)
     assert rc == _lib.IM_INVALID and "scoring" in msg
-    rc, msg = route(path=3)
-    assert rc == _lib.IM_INVALID and "path" in msg
     rc, msg = route(ptr=None)
     assert rc == _lib.IM_INVALID and "null" in msg
     rc, msg = route(ptr=8)
@@ -39,26 +37,23 @@ def test_route_refusals():
 
 def test_plan_sizes():
     lib = _lib.load()
-    assert lib.im_moe_plan_bytes(0, 8, 2, 0) >= 32
-    assert lib.im_moe_plan_bytes(1, 600, 2, 0) == 0 and lib.im_moe_plan_bytes(1, 8, 9, 0) == 0
-    assert lib.im_moe_plan_bytes(1, 8, 2, 3) == 0
-    # every expert can end in a part-filled item: one item per non-empty bucket and one per full item
+    assert lib.im_moe_plan_bytes(0, 8, 2) >= 32
+    assert lib.im_moe_plan_bytes(1, 600, 2) == 0 and lib.im_moe_plan_bytes(1, 8, 9) == 0
+    # every expert can end in a part-filled item: one item per non-empty bucket and one per full item of 128
     for m, e, k in [(1, 128, 8), (5, 128, 8), (64, 8, 8), (65, 8, 2), (8192, 128, 8), (1 << 22, 512, 32)]:
         pairs = m * k
-        for path in range(3):
-            assert lib.im_moe_plan_bytes(m, e, k, path) >= 32 + 16 * min(pairs, e + 1)
-            assert lib.im_moe_plan_bytes(m, e, k, path) <= 32 + 16 * (min(pairs, e + 1) + pairs / 8) + 4 * 148 * (e + 1)
+        items = 16 * (min(pairs, e + 1) + pairs // 128)
+        assert 32 + items <= lib.im_moe_plan_bytes(m, e, k) <= 32 + items + 4 * 148 * (e + 1)
     assert lib.im_moe_packed_bytes(3, 33, 128) == 3 * (2 * 4608 + 512 + 8)  # 128-output blocks of 64-wide groups, maxima
     assert lib.im_moe_packed_bytes(3, 33, 100) == 0
-    assert lib.im_moe_mlp_workspace_bytes(4, 8, 2, 128, 64, _lib.MOE_WARP) == 4 * 2 * 64 * 2
-    assert lib.im_moe_mlp_workspace_bytes(4, 8, 2, 100, 64, _lib.MOE_WARP) == 0
-    assert lib.im_moe_grouped_workspace_bytes(4, 8, 2, 128, _lib.MOE_WARP) == 0
-    assert lib.im_moe_grouped_workspace_bytes(4, 8, 2, 128, _lib.MOE_TENSOR) >= 4 * 128 * 2
+    assert lib.im_moe_mlp_workspace_bytes(4, 8, 2, 128, 64) >= 8 * (128 + 64) * 2
+    assert lib.im_moe_mlp_workspace_bytes(4, 8, 2, 100, 64) == 0
+    assert lib.im_moe_grouped_workspace_bytes(4, 8, 2, 128) >= 8 * 128 * 2
 
 
 def test_product_refusals():
-    args = lambda m=4, n=32, k=64, x=256, plan=256, size=1 << 20, path=0, wsize=1 << 20: (  # noqa: E731
-        "im_moe_grouped_qgemm", 256, x, 256, m, 8, 2, n, k, 0, 256, path, plan, size, 256, wsize, None)
+    args = lambda m=4, n=32, k=64, x=256, plan=256, size=1 << 20, wsize=1 << 20: (  # noqa: E731
+        "im_moe_grouped_qgemm", 256, x, 256, m, 8, 2, n, k, 0, 256, plan, size, 256, wsize, None)
     rc, msg = _status(*args(k=100))
     assert rc == _lib.IM_INVALID and "K=100" in msg
     rc, msg = _status(*args(x=None))
@@ -69,13 +64,11 @@ def test_product_refusals():
     assert rc == _lib.IM_INVALID and "plan" in msg
     rc, msg = _status(*args(size=8))
     assert rc == _lib.IM_INVALID and "plan of" in msg
-    rc, msg = _status(*args(path=7))
-    assert rc == _lib.IM_INVALID and "path" in msg
-    rc, msg = _status(*args(path=2, wsize=8))
+    rc, msg = _status(*args(wsize=8))
     assert rc == _lib.IM_INVALID and "workspace of" in msg
     assert _status(*args(m=0, x=None, plan=None))[0] == _lib.IM_OK
     mlp = lambda h=128, i=64, act=2, ws=256, size=1 << 20: (  # noqa: E731
-        "im_moe_mlp", 256, 256, 256, 256, 4, 8, 2, h, i, act, 256, 0, 256, 1 << 20, ws, size, None)
+        "im_moe_mlp", 256, 256, 256, 256, 4, 8, 2, h, i, act, 256, 256, 1 << 20, ws, size, None)
     assert _status(*mlp(h=100))[0] == _lib.IM_INVALID
     assert _status(*mlp(i=100))[0] == _lib.IM_INVALID
     rc, msg = _status(*mlp(act=1))

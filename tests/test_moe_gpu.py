@@ -122,13 +122,13 @@ def test_route_empty_batch(cuda):
     assert kernels.grouped_qgemm(x, kernels.Experts(*quantised(gen, 16, 32, 64, cuda)), r).shape == (0, 2, 32)
 
 
-def check_grouped(cuda, m, e, k, n, kdim, path, by_pair=False, closed=0.0, skew=0.5, seed=0):
+def check_grouped(cuda, m, e, k, n, kdim, by_pair=False, closed=0.0, skew=0.5, seed=0):
     gen = torch.Generator(device=cuda).manual_seed(seed)
     q = quantised(gen, e, n, kdim, cuda)
     logits = torch.randn((m, e), generator=gen, device=cuda) + skew * torch.randn((e,), generator=gen, device=cuda)
     logits[torch.rand((m, e), generator=gen, device=cuda) < closed] = float("-inf")
     x = torch.randn((m, k, kdim) if by_pair else (m, kdim), generator=gen, device=cuda).to(torch.bfloat16)
-    r = kernels.moe_route(logits, k, path=path)
+    r = kernels.moe_route(logits, k)
     y = kernels.grouped_qgemm(x, kernels.Experts(*q), r, out=torch.full((m, k, n), float("nan"), device=cuda,
                                                                         dtype=torch.bfloat16))
     ids = r.ids.long()
@@ -146,17 +146,15 @@ def check_grouped(cuda, m, e, k, n, kdim, path, by_pair=False, closed=0.0, skew=
                                           (5, 128, 8, 256, 768), (3, 2, 2, 31, 128), (12, 5, 3, 100, 320),
                                           (77, 60, 4, 1000, 576), (160, 16, 4, 512, 1024), (700, 8, 2, 320, 704),
                                           (300, 3, 3, 129, 64), (2000, 32, 4, 160, 256)])
-@pytest.mark.parametrize("path", ["warp", "tensor"])
-def test_grouped_product(cuda, m, e, k, n, kdim, path):
-    check_grouped(cuda, m, e, k, n, kdim, path)
+def test_grouped_product(cuda, m, e, k, n, kdim):
+    check_grouped(cuda, m, e, k, n, kdim)
 
 
 @pytest.mark.parametrize("m,e,k", [(1, 8, 2), (30, 12, 4), (900, 6, 2)])
-@pytest.mark.parametrize("path", ["warp", "tensor"])
-def test_grouped_product_by_pair_and_closed(cuda, m, e, k, path):
-    check_grouped(cuda, m, e, k, 96, 448, path, by_pair=True, closed=0.3, skew=2.0, seed=m)
-    check_grouped(cuda, m, e, k, 96, 448, path, closed=0.9, seed=m + 1)
-    check_grouped(cuda, m, e, k, 40, 192, path, by_pair=True, closed=1.0, seed=m + 2)
+def test_grouped_product_by_pair_and_closed(cuda, m, e, k):
+    check_grouped(cuda, m, e, k, 96, 448, by_pair=True, closed=0.3, skew=2.0, seed=m)
+    check_grouped(cuda, m, e, k, 96, 448, closed=0.9, seed=m + 1)
+    check_grouped(cuda, m, e, k, 40, 192, by_pair=True, closed=1.0, seed=m + 2)
 
 
 def mlp_case(cuda, m, e, k, h, inter, seed, skew=0.5):
@@ -170,13 +168,12 @@ def mlp_case(cuda, m, e, k, h, inter, seed, skew=0.5):
 @pytest.mark.parametrize("m,e,k,h,inter", [(1, 128, 8, 2048, 768), (5, 16, 4, 512, 192), (2, 4, 2, 64, 64),
                                            (33, 9, 3, 320, 448), (160, 128, 8, 256, 128), (1200, 8, 2, 384, 320)])
 @pytest.mark.parametrize("act", ["swiglu", "geglu"])
-@pytest.mark.parametrize("path", ["warp", "tensor"])
-def test_gated_mlp(cuda, m, e, k, h, inter, act, path):
+def test_gated_mlp(cuda, m, e, k, h, inter, act):
     gate, up, down, x, logits = mlp_case(cuda, m, e, k, h, inter, m + h)
     logits[0] = float("-inf")
     if m > 1:
         logits[1, : e // 2] = float("-inf")
-    r = kernels.moe_route(logits, k, path=path)
+    r = kernels.moe_route(logits, k)
     y = kernels.moe_mlp(x, kernels.Experts.gate_up(gate, up), kernels.Experts(*down), r, activation=act)
     ids = r.ids.long()
     assert r.status() == 0
@@ -200,27 +197,25 @@ def test_gated_mlp(cuda, m, e, k, h, inter, act, path):
         assert bool((off <= tol).all()), (ex, float((off / tol).max()))
 
 
-@pytest.mark.parametrize("path", ["warp", "tensor"])
-def test_rows_do_not_depend_on_the_batch(cuda, path):
+def test_rows_do_not_depend_on_the_batch(cuda):
     """A verification pass must give every row the bits that it gets alone (speculative decoding returns the tokens of
     plain decoding): batches of 1 to 160 rows over the same rows."""
     gate, up, down, x, logits = mlp_case(cuda, 160, 24, 4, 512, 320, 3)
     gu, dn = kernels.Experts.gate_up(gate, up), kernels.Experts(*down)
-    whole = kernels.moe_mlp(x, gu, dn, kernels.moe_route(logits, 4, path=path))
+    whole = kernels.moe_mlp(x, gu, dn, kernels.moe_route(logits, 4))
     for r0, r1 in [(0, 1), (7, 8), (3, 8), (10, 26), (20, 90), (0, 159)]:
-        part = kernels.moe_mlp(x[r0:r1].contiguous(), gu, dn, kernels.moe_route(logits[r0:r1].contiguous(), 4, path=path))
+        part = kernels.moe_mlp(x[r0:r1].contiguous(), gu, dn, kernels.moe_route(logits[r0:r1].contiguous(), 4))
         assert torch.equal(part.view(torch.int16), whole[r0:r1].view(torch.int16)), (r0, r1)
 
 
-@pytest.mark.parametrize("path", ["warp", "tensor"])
-def test_overlap_off_and_graph_replay_give_the_same_bits(cuda, path):
+def test_overlap_off_and_graph_replay_give_the_same_bits(cuda):
     gate, up, down, x, logits = mlp_case(cuda, 5, 32, 4, 256, 192, 5)
     gu, dn = kernels.Experts.gate_up(gate, up), kernels.Experts(*down)
     h = torch.randn((5, 256), device=cuda).to(torch.bfloat16)
     norm = torch.ones(256, dtype=torch.bfloat16, device=cuda)
 
     def block():
-        r = kernels.moe_route(logits, 4, path=path)
+        r = kernels.moe_route(logits, 4)
         return kernels.block_residual(kernels.moe_mlp(x, gu, dn, r), h, 1e-6, weights=r.weights, next_norm=norm)
 
     want = [t.clone() for t in block()]
@@ -244,7 +239,7 @@ def test_overlap_off_and_graph_replay_give_the_same_bits(cuda, path):
     assert all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in zip(out, want))
 
 
-def test_tensor_path_holds_the_range_of_bf16(cuda):
+def test_products_hold_the_range_of_bf16(cuda):
     """Rows of 2^-90, 1 and 2^90 and experts of very different weights: the powers of two that bring the operands into
     fp16 must leave every row as exact as one of ordinary size. Infinities and NaN stay in their row."""
     gate, up, down, x, logits = mlp_case(cuda, 24, 4, 2, 256, 128, 11)
@@ -252,7 +247,7 @@ def test_tensor_path_holds_the_range_of_bf16(cuda):
         q[1][1:] *= f
         q[2][1:] *= f
     gu, dn = kernels.Experts.gate_up(gate, up), kernels.Experts(*down)
-    r = kernels.moe_route(logits, 2, path="tensor")
+    r = kernels.moe_route(logits, 2)
     y = kernels.grouped_qgemm(x, gu, r)
     for f in (2.0**-90, 2.0**90):
         # every value shifts by a power of two: the same bits apart from the exponent
