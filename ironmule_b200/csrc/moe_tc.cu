@@ -17,7 +17,7 @@
 // A persistent grid (one CTA per SM) walks tiles; its warps are coupled by mbarriers only:
 //  * warp 0 copies the packed weights, two 64-wide groups (9216 contiguous bytes) at a time, into a ring of 8 (one
 //    thread starts a copy every 280 cycles or so, whatever its size: hence two groups a stage everywhere);
-//  * warps 12-27, four sets of 4, expand a group each (two sets a stage): thread = output row, 64 codes -> 32 registers of fp16 pairs ->
+//  * warps 12-27, four sets of 4, expand a stage each: thread = output row, 64 codes -> 32 registers of fp16 pairs ->
 //    tensor memory, where the MMA reads A directly. Neither shared memory nor its bandwidth carries expanded weights;
 //  * warp 10 copies the item's rows of a stage, one contiguous copy: moe_prep_kernel lays each item's rows out as the
 //    K-major 128-byte-swizzled tiles that the MMA reads, and the gated epilogue writes its outputs as the next
@@ -49,7 +49,7 @@ constexpr int MT_EPI = 8;               // epilogue warps
 constexpr int MT_SETS = 4;              // expansion sets of four warps
 constexpr int MT_W_EPI = 2, MT_W_LOAD = MT_W_EPI + MT_EPI, MT_W_TRANS = MT_W_LOAD + 2;  // first warps of the roles
 constexpr int MT_THREADS = (MT_W_TRANS + 4 * MT_SETS) * 32;
-static_assert(MT_S % 2 == 0 && MT_W % 2 == 0 && MT_SETS == 4, "sets 0, 1 take the even stages, 2, 3 the odd ones");
+static_assert(MT_S == MT_SETS && MT_W % MT_SETS == 0, "a set has its own A stage and its own slots of the weight ring");
 constexpr int MT_WBITS = -6;            // an expert's largest weight lands in [2^-7, 2^-6)
 constexpr uint32_t MT_TMEM = 512;       // 2 accumulators of 128 columns, 4 A stages of 64
 constexpr int MT_A0 = 256;
@@ -202,6 +202,30 @@ __device__ __forceinline__ void mt_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
+// One row's 64 codes of a group -> 32 fp16 pairs -> columns [col, + 32) of tensor memory, once ready() says so.
+template <typename F>
+__device__ __forceinline__ void mt_group(const unsigned char* codes, const unsigned char* affine, float inv, int q,
+                                         uint32_t col, F ready) {
+  const uint4 c0 = *reinterpret_cast<const uint4*>(codes), c1 = *reinterpret_cast<const uint4*>(codes + 512);
+  const float sf = bf(*reinterpret_cast<const uint16_t*>(affine)) * inv;
+  const __half2 s24 = __float2half2_rn(sf * 16777216.f), s20 = __float2half2_rn(sf * 1048576.f);
+  const __half2 b2 = __float2half2_rn(bf(*reinterpret_cast<const uint16_t*>(affine + 8)) * inv);
+  uint32_t p[32];
+  const uint32_t words[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+#pragma unroll
+  for (int i = 0; i < 8; i++) mt_expand(words[i], s24, s20, b2, p + 4 * i);
+  if (!ready()) return;
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
+      "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(((uint32_t)(32 * q) << 16) + col),
+      "r"(p[0]), "r"(p[1]), "r"(p[2]), "r"(p[3]), "r"(p[4]), "r"(p[5]), "r"(p[6]), "r"(p[7]), "r"(p[8]), "r"(p[9]),
+      "r"(p[10]), "r"(p[11]), "r"(p[12]), "r"(p[13]), "r"(p[14]), "r"(p[15]), "r"(p[16]), "r"(p[17]), "r"(p[18]),
+      "r"(p[19]), "r"(p[20]), "r"(p[21]), "r"(p[22]), "r"(p[23]), "r"(p[24]), "r"(p[25]), "r"(p[26]), "r"(p[27]),
+      "r"(p[28]), "r"(p[29]), "r"(p[30]), "r"(p[31])
+      : "memory");
+}
+
 template <bool GLU>
 __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
   extern __shared__ unsigned char mt_raw[];
@@ -225,11 +249,11 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
     unsigned long long* b = reinterpret_cast<unsigned long long*>(sbase + MT_OFF_BAR);
     for (int s = 0; s < MT_S; s++) {
       qt_init(&b[MT_DONE + s], 1u);
-      qt_init(&b[MT_FULL + s], 8u + 1u);  // eight expansion warps, the rows' bytes
+      qt_init(&b[MT_FULL + s], 4u + 1u);  // four expansion warps, the rows' bytes
     }
     for (int s = 0; s < MT_W; s++) {
       qt_init(&b[MT_W_FULL + s], 1u);
-      qt_init(&b[MT_W_EMPTY + s], 8u);
+      qt_init(&b[MT_W_EMPTY + s], 4u);
     }
     for (int s = 0; s < 2; s++) {
       qt_init(&b[MT_D_FULL + s], 1u);
@@ -241,7 +265,7 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  const uint32_t tmem = *holder;
+  constexpr uint32_t tmem = 0;  // the whole tensor memory: its allocation can only start at column 0
   // The routing's plan was finished before the launch that precedes this one (the prep kernel, or the first product)
   // let this one begin: the plan and the weights are read without waiting, rows and outputs only after pdl_wait().
   const int ntiles = a.p.plan[0] * a.cols;
@@ -359,7 +383,7 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
       for (int i = 0; 64 * i + 32 * set < rows; i++) {
         const int c0 = 64 * i + 32 * set, n = min(32, rows - c0);
         uint32_t v[32];
-        const uint32_t ta = tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(buf * MT_N + c0);
+        const uint32_t ta = ((uint32_t)(32 * q) << 16) + (uint32_t)(buf * MT_N + c0);
         asm volatile(
             "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
             "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
@@ -444,13 +468,12 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
                    (uint32_t)((j / MT_S) & 1));
     }
   } else {
-    // ---- code expansion: sets 0 and 1 take the two groups of the even stages of the CTA's sequence, 2 and 3 of the
-    // odd ones -------------------------------------------------------------------------------------------------------
-    const int set = (warp - MT_W_TRANS) >> 2, q = warp & 3, half = set & 1;
-    const uint32_t code_off = (uint32_t)(half * MOE_BLOCK_BYTES + q * 1024 + lane * 16);
-    const uint32_t sb_off = (uint32_t)(half * MOE_BLOCK_BYTES + 4096 + q * 128 + (lane & 7) * 16 + (lane >> 3) * 2);
-    uint32_t s = set >> 1, phase = 1, sw = set >> 1, wphase = 0;
-    int skip = 2 * (set >> 1);  // groups of the next tile that lie before this set's next stage
+    // ---- code expansion: set i takes every fourth stage of the CTA's sequence, from stage i on -----------------------
+    const int set = (warp - MT_W_TRANS) >> 2, q = warp & 3;
+    const unsigned char* codes = sbase + MT_OFF_W + q * 1024 + lane * 16;
+    const unsigned char* affine = sbase + MT_OFF_W + 4096 + q * 128 + (lane & 7) * 16 + (lane >> 3) * 2;
+    uint32_t phase = 1, sw = set, wphase = 0;
+    int skip = 2 * set;  // groups of the next tile that lie before this set's next stage
     const int even = G + (G & 1);
     for (int tile = blockIdx.x; tile < ntiles; tile += gridDim.x) {
       const int expert = a.items[tile / a.cols].x;
@@ -458,37 +481,25 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
       const float inv = mt_pow2(
           -mt_exp(a.row_max[((size_t)expert * a.cols + tile % a.cols) * 128 + q * 32 + lane], MT_WBITS));
       int g = skip;
-      for (; g < G; g += 4) {
+      for (; g < G; g += 2 * MT_SETS) {
         if (!qt_wait_short(bars + 8 * (MT_W_FULL + sw), wphase, abort_flag, a.error)) goto expand_done;
-        const unsigned char* w = sbase + MT_OFF_W + sw * 2 * MOE_BLOCK_BYTES;  // (a last odd group: stale, not used)
-        const uint4 c0 = *reinterpret_cast<const uint4*>(w + code_off);
-        const uint4 c1 = *reinterpret_cast<const uint4*>(w + code_off + 512);
-        const float sf = bf(*reinterpret_cast<const uint16_t*>(w + sb_off)) * inv;
-        const __half2 s24 = __float2half2_rn(sf * 16777216.f), s20 = __float2half2_rn(sf * 1048576.f);
-        const __half2 b2 = __float2half2_rn(bf(*reinterpret_cast<const uint16_t*>(w + sb_off + 8)) * inv);
-        uint32_t p[32];
-        const uint32_t words[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
-#pragma unroll
-        for (int i = 0; i < 8; i++) mt_expand(words[i], s24, s20, b2, p + 4 * i);
-        __syncwarp();
-        if (lane == 0) mt_arrive(bars + 8 * (MT_W_EMPTY + sw));
-        if ((sw += 2) >= MT_W) sw -= MT_W, wphase ^= 1u;
-        if (!qt_wait_short(bars + 8 * (MT_DONE + s), phase, abort_flag, a.error)) goto expand_done;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        asm volatile(
-            "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
-            "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(
-                tmem + ((uint32_t)(32 * q) << 16) + MT_A0 + 64 * s + 32 * half),
-            "r"(p[0]), "r"(p[1]), "r"(p[2]), "r"(p[3]), "r"(p[4]), "r"(p[5]), "r"(p[6]), "r"(p[7]), "r"(p[8]),
-            "r"(p[9]), "r"(p[10]), "r"(p[11]), "r"(p[12]), "r"(p[13]), "r"(p[14]), "r"(p[15]), "r"(p[16]),
-            "r"(p[17]), "r"(p[18]), "r"(p[19]), "r"(p[20]), "r"(p[21]), "r"(p[22]), "r"(p[23]), "r"(p[24]),
-            "r"(p[25]), "r"(p[26]), "r"(p[27]), "r"(p[28]), "r"(p[29]), "r"(p[30]), "r"(p[31])
-            : "memory");
+        const uint32_t at = sw * 2 * MOE_BLOCK_BYTES;
+        mt_group(codes + at, affine + at, inv, q, MT_A0 + 64 * set, [&] {
+          return qt_wait_short(bars + 8 * (MT_DONE + set), phase, abort_flag, a.error);
+        });
+        if (g + 1 < G)
+          mt_group(codes + at + MOE_BLOCK_BYTES, affine + at + MOE_BLOCK_BYTES, inv, q, MT_A0 + 64 * set + 32,
+                   [] { return true; });
+        if (*abort_flag) goto expand_done;
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncwarp();
-        if (lane == 0) mt_arrive(bars + 8 * (MT_FULL + s));
-        if ((s += 2) >= MT_S) s -= MT_S, phase ^= 1u;
+        if (lane == 0) {
+          mt_arrive(bars + 8 * (MT_W_EMPTY + sw));
+          mt_arrive(bars + 8 * (MT_FULL + set));
+        }
+        if ((sw += MT_SETS) >= MT_W) sw -= MT_W, wphase ^= 1u;
+        phase ^= 1u;
       }
       skip = g - even;
     }
