@@ -16,7 +16,7 @@
 //
 // A persistent grid (one CTA per SM) walks tiles; its warps are coupled by mbarriers only:
 //  * warp 0 copies the packed weights, two 64-wide groups (9216 contiguous bytes) at a time, into a ring of 8 (one
-//    thread starts a copy every 280 cycles or so, whatever its size: hence two groups a stage everywhere);
+//    warp starts a copy every 200 to 300 cycles, whatever its size: hence two groups a stage everywhere);
 //  * warps 12-27, four sets of 4, expand a stage each: thread = output row, 64 codes -> 32 registers of fp16 pairs ->
 //    tensor memory, where the MMA reads A directly. Neither shared memory nor its bandwidth carries expanded weights;
 //  * warp 10 copies the item's rows of a stage, one contiguous copy: moe_prep_kernel lays each item's rows out as the
@@ -49,7 +49,9 @@ constexpr int MT_EPI = 8;               // epilogue warps
 constexpr int MT_SETS = 4;              // expansion sets of four warps
 constexpr int MT_W_EPI = 2, MT_W_LOAD = MT_W_EPI + MT_EPI, MT_W_TRANS = MT_W_LOAD + 2;  // first warps of the roles
 constexpr int MT_THREADS = (MT_W_TRANS + 4 * MT_SETS) * 32;
-static_assert(MT_S == MT_SETS && MT_W % MT_SETS == 0, "a set has its own A stage and its own slots of the weight ring");
+// A set has its own A stage and its own slots of the weight ring: a slot that two sets take in turn would let one of
+// them take the completion of its last use for that of the next (a wait knows only a phase's parity).
+static_assert(MT_S == MT_SETS && MT_W % MT_SETS == 0, "ring lengths");
 constexpr int MT_WBITS = -6;            // an expert's largest weight lands in [2^-7, 2^-6)
 constexpr uint32_t MT_TMEM = 512;       // 2 accumulators of 128 columns, 4 A stages of 64
 constexpr int MT_A0 = 256;
@@ -272,28 +274,30 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
 
   if (warp == 0) {
     // ---- weights -------------------------------------------------------------------------------------------
-    if (lane == 0) {
-      uint32_t s = 0, phase = 0;
-      int k = 0;
-      for (int tile = blockIdx.x; tile < ntiles; tile += gridDim.x) {
-        const int expert = a.items[tile / a.cols].x;
-        if (expert == a.p.E) continue;
-        const unsigned char* src =
-            a.p.wp + (size_t)expert * a.expert_bytes + (size_t)(tile % a.cols) * G * MOE_BLOCK_BYTES;
-        for (int g = 0; g < G; g += 2, k++) {
-          if (!qt_wait_short(bars + 8 * (MT_W_EMPTY + s), phase ^ 1u, abort_flag, a.error)) goto weights_done;
+    // (as for the MMAs, the whole warp walks the loop and one lane issues)
+    const bool leader = qt_elect();
+    uint32_t s = 0, phase = 1;
+    int k = 0;
+    for (int tile = blockIdx.x; tile < ntiles; tile += gridDim.x) {
+      const int expert = a.items[tile / a.cols].x;
+      if (expert == a.p.E) continue;
+      const unsigned char* src =
+          a.p.wp + (size_t)expert * a.expert_bytes + (size_t)(tile % a.cols) * G * MOE_BLOCK_BYTES;
+      for (int g = 0; g < G; g += 2, k++) {
+        if (!qt_wait_short(bars + 8 * (MT_W_EMPTY + s), phase, abort_flag, a.error)) goto weights_done;
+        if (leader)
           mt_copy(base + (uint32_t)MT_OFF_W + s * 2 * MOE_BLOCK_BYTES, src, g + 1 < G ? 2 * MOE_BLOCK_BYTES : MOE_BLOCK_BYTES,
                   bars + 8 * (MT_W_FULL + s));
-          src += 2 * MOE_BLOCK_BYTES;
-          if (++s == MT_W) s = 0, phase ^= 1u;
-        }
+        __syncwarp();
+        src += 2 * MOE_BLOCK_BYTES;
+        if (++s == MT_W) s = 0, phase ^= 1u;
       }
-    weights_done:
-      if (*abort_flag)  // copies still landing in this CTA's shared memory finish before it exits
-        for (int j = k > MT_W ? k - MT_W : 0; j < k; j++)
-          qt_drain(reinterpret_cast<unsigned long long*>(sbase + MT_OFF_BAR) + MT_W_FULL + j % MT_W,
-                   (uint32_t)((j / MT_W) & 1));
     }
+  weights_done:
+    if (*abort_flag)  // copies still landing in this CTA's shared memory finish before it exits
+      for (int j = k > MT_W ? k - MT_W : 0; j < k; j++)
+        qt_drain(reinterpret_cast<unsigned long long*>(sbase + MT_OFF_BAR) + MT_W_FULL + j % MT_W,
+                 (uint32_t)((j / MT_W) & 1));
   } else if (warp == 1) {
     // ---- MMA issue -----------------------------------------------------------------------------------------
     // (the whole warp walks the loop, so that its addresses stay in uniform registers; one lane issues)
@@ -444,7 +448,8 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
     }
   } else if (warp < MT_W_TRANS) {
     // ---- rows ----------------------------------------------------------------------------------------------------
-    if (warp == MT_W_LOAD && lane == 0) {
+    if (warp == MT_W_LOAD) {
+      const bool leader = qt_elect();
       pdl_wait();
       uint32_t s = 0, phase = 1;
       int k = 0;
@@ -455,7 +460,8 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
         const unsigned char* src = a.tiles + (size_t)item.w * a.p.K * 2;
         for (int g = 0; g < G; g += 2, k++) {
           if (!qt_wait_short(bars + 8 * (MT_DONE + s), phase, abort_flag, a.error)) goto rows_done;
-          mt_copy(base + s * MT_B, src, g + 1 < G ? 2 * bytes : bytes, bars + 8 * (MT_FULL + s));
+          if (leader) mt_copy(base + s * MT_B, src, g + 1 < G ? 2 * bytes : bytes, bars + 8 * (MT_FULL + s));
+          __syncwarp();
           src += 2 * bytes;
           if (++s == MT_S) s = 0, phase ^= 1u;
         }
