@@ -11,7 +11,7 @@ namespace im {
 constexpr int MOE_MAX_EXPERTS = 512;
 constexpr int MOE_MAX_TOP_K = 32;
 constexpr int64_t MOE_MAX_ROWS = 1 << 22;
-constexpr int MOE_ROUTE_BLOCKS = 148;   // blocks of the routing kernels at most (one per SM)
+constexpr int MOE_ROUTE_BLOCKS = 296;   // blocks of the routing kernels at most (two per SM)
 constexpr int MOE_ROUTE_ROWS = 64;      // rows that one block alone routes
 constexpr int MOE_ITEM_ROWS = 128;      // rows of a work item at most (MMA N)
 constexpr int MOE_PLAN_HEADER = 8;      // ints: [0] work items, [1] error word of the bounded waits
@@ -31,11 +31,14 @@ struct MoeItem {
   int expert, first, rows, padded;  // padded: the rows before it when every item is rounded up to 16
 };
 
-// Plan layout in ints: header | items | per-block expert counts (the routing's own scratch).
+// Plan layout in ints: header | items | where each pair's row lies | per-block expert counts (the routing's own scratch).
+// where[pair] = {the item's padded first row (-1: no expert), its row r in the item | the item's rows rounded up to 16
+// << 16}.
 struct MoePlan {
   int64_t max_items;   // bound on the items of any routing of these sizes
   int64_t blocks, rows_per_block;
-  int64_t counts;      // int offset of the counts
+  int64_t where;       // int offsets
+  int64_t counts;
   size_t bytes;
 };
 

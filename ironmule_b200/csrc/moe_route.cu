@@ -11,7 +11,7 @@
 //
 // One warp per row: lane l holds experts l, l + 32, ...; each of the k rounds takes the warp's largest 32-bit sortable
 // key with one reduction and the lowest expert holding it with a second. Up to 64 rows one block does all of it in one
-// launch. More rows are cut over up to 148 blocks: the first launch selects and counts, the second sums the blocks'
+// launch. More rows are cut over up to 296 blocks: the first launch selects and counts, the second sums the blocks'
 // counts (every block for itself), scans them and places its pairs. The order is stable: within an expert, pairs ascend.
 // Bytes are few (a row's logits once, 12 bytes a place); what bounds it is launch and barrier latency.
 #include <math.h>
@@ -33,7 +33,8 @@ struct RouteArgs {
   int* offsets;
   int* pairs;
   int* plan;
-  int* counts;
+  int2* where;
+  int* counts;   // [E + 1][blocks]
   int f32, scoring, normalise;
   float scale;
   int M, E, top_k, rows_per_block, blocks;
@@ -47,7 +48,8 @@ MoePlan moe_plan(int64_t M, int64_t E, int64_t top_k) {
   const int64_t per = (M + MOE_ROUTE_BLOCKS - 1) / MOE_ROUTE_BLOCKS;
   p.rows_per_block = M <= MOE_ROUTE_ROWS ? MOE_ROUTE_ROWS : (per < 16 ? 16 : per);
   p.blocks = M <= MOE_ROUTE_ROWS ? 1 : (M + p.rows_per_block - 1) / p.rows_per_block;
-  p.counts = MOE_PLAN_HEADER + 4 * p.max_items;
+  p.where = MOE_PLAN_HEADER + 4 * p.max_items;
+  p.counts = p.where + 2 * pairs;
   p.bytes = (size_t)(p.counts + (p.blocks > 1 ? p.blocks * (E + 1) : 0)) * 4;
   return p;
 }
@@ -179,6 +181,7 @@ __device__ __forceinline__ int mr_scan(const int* v, int* out, int n, int* sh) {
 struct RouteSmem {
   int total[MOE_MAX_EXPERTS + 1];   // pairs of each bucket over all blocks
   int base[MOE_MAX_EXPERTS + 1];    // pairs of each bucket in earlier blocks, then where the next one goes
+  int first[MOE_MAX_EXPERTS + 1];   // where each bucket begins
   int scan[MOE_MAX_EXPERTS + 1];    // work items before each bucket's
   int pad[MOE_MAX_EXPERTS + 1];     // rows before each bucket's when every item is rounded up to 16
   int cnt[MR_WARPS][MOE_MAX_EXPERTS + 1];
@@ -191,52 +194,48 @@ __device__ __forceinline__ int mr_item_rows(int c) {
   const int n = mr_items(c);
   return n ? ((c + n - 1) / n + 7) / 8 * 8 : 0;
 }
+__device__ __forceinline__ int mr_ceil16(int n) { return (n + 15) & ~15; }
 
 // Offsets, work items (block 0) and this block's pairs, from s.total and s.base.
 __device__ __forceinline__ void mr_place(const RouteArgs& a, RouteSmem& s) {
   const int nb = a.E + 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int e = threadIdx.x; e < nb; e += MR_THREADS) {
+    const int c = s.total[e], each = mr_item_rows(c), n = mr_items(c);
+    s.scan[e] = n;
+    s.pad[e] = n ? (n - 1) * mr_ceil16(each) + mr_ceil16(c - (n - 1) * each) : 0;
+  }
+  __syncthreads();
+  const int all = mr_scan(s.total, s.first, nb, s.sh);
+  mr_scan(s.pad, s.pad, nb, s.sh);
   if (blockIdx.x == 0) {
+    const int items_all = mr_scan(s.scan, s.scan, nb, s.sh);
+    int4* items = reinterpret_cast<int4*>(a.plan + MOE_PLAN_HEADER);
     for (int e = threadIdx.x; e < nb; e += MR_THREADS) {
-      const int c = s.total[e], each = mr_item_rows(c), n = mr_items(c);
-      s.scan[e] = n;
-      s.pad[e] = n ? (n - 1) * ((each + 15) & ~15) + ((c - (n - 1) * each + 15) & ~15) : 0;
+      const int c = s.total[e], first = s.first[e], n = mr_items(c), each = mr_item_rows(c);
+      a.offsets[e] = first;
+      for (int i = 0; i < n; i++)
+        items[s.scan[e] + i] = make_int4(e, first + i * each, min(each, c - i * each), s.pad[e] + i * mr_ceil16(each));
     }
-    __syncthreads();
-    const int items = mr_scan(s.scan, s.scan, nb, s.sh);
-    mr_scan(s.pad, s.pad, nb, s.sh);
     if (threadIdx.x == 0) {
-      a.plan[0] = items;
+      a.offsets[nb] = all;
+      a.plan[0] = items_all;
       a.plan[1] = 0;
     }
   }
-  // s.cnt[0] holds the bucket offsets until the pairs are counted
-  const int all = mr_scan(s.total, s.cnt[0], nb, s.sh);
-  if (blockIdx.x == 0) {
-    int4* items = reinterpret_cast<int4*>(a.plan + MOE_PLAN_HEADER);
-    for (int e = threadIdx.x; e < nb; e += MR_THREADS) {
-      const int c = s.total[e], first = s.cnt[0][e];
-      a.offsets[e] = first;
-      const int n = mr_items(c), each = mr_item_rows(c);
-      for (int i = 0; i < n; i++)
-        items[s.scan[e] + i] = make_int4(e, first + i * each, min(each, c - i * each), s.pad[e] + i * ((each + 15) & ~15));
-    }
-    if (threadIdx.x == 0) a.offsets[nb] = all;
-  }
-  for (int e = threadIdx.x; e < nb; e += MR_THREADS) s.base[e] += s.cnt[0][e];
-  __syncthreads();
+  for (int e = threadIdx.x; e < nb; e += MR_THREADS) s.base[e] += s.first[e];
   const int row0 = blockIdx.x * a.rows_per_block;
   const int p0 = row0 * a.top_k, p1 = min(a.M, row0 + a.rows_per_block) * a.top_k;
   for (int c0 = p0; c0 < p1; c0 += MR_THREADS) {
-    for (int i = threadIdx.x; i < MR_WARPS * nb; i += MR_THREADS) s.cnt[i / nb][i % nb] = 0;
+    for (int e = lane; e < nb; e += 32) s.cnt[warp][e] = 0;
     __syncthreads();
     const int pair = c0 + threadIdx.x;
-    int bucket = -1, rank = 0;
+    int bucket = -1;
     if (pair < p1) {
       const int id = a.ids[pair];
       bucket = id < 0 ? a.E : id;
     }
     const unsigned same = __match_any_sync(0xffffffffu, bucket);
-    rank = __popc(same & ((1u << lane) - 1u));
+    const int rank = __popc(same & ((1u << lane) - 1u));
     if (bucket >= 0 && rank == 0) s.cnt[warp][bucket] = __popc(same);
     __syncthreads();
     for (int e = threadIdx.x; e < nb; e += MR_THREADS) {
@@ -250,8 +249,63 @@ __device__ __forceinline__ void mr_place(const RouteArgs& a, RouteSmem& s) {
       s.base[e] = run;
     }
     __syncthreads();
-    if (bucket >= 0) a.pairs[s.cnt[warp][bucket] + rank] = pair;
+    if (bucket >= 0) {
+      const int pos = s.cnt[warp][bucket] + rank, in = pos - s.first[bucket];
+      const int c = s.total[bucket], each = mr_item_rows(c), i = in / each;
+      a.pairs[pos] = pair;
+      a.where[pair] = bucket == a.E ? make_int2(-1, 0)
+                                    : make_int2(s.pad[bucket] + i * mr_ceil16(each),
+                                                (in - i * each) | mr_ceil16(min(each, c - i * each)) << 16);
+    }
     __syncthreads();
+  }
+}
+
+// The same for at most 128 pairs in one block (every bucket is one item): each pair counts the ones that go before it.
+constexpr int MR_FEW = 128;
+__device__ __forceinline__ void mr_place_few(const RouteArgs& a, RouteSmem& s) {
+  const int n = a.M * a.top_k, p = threadIdx.x;
+  int* bucket = s.cnt[0];  // [MR_FEW], then the size of the bucket that begins with pair q (0: it does not begin one)
+  int* size = s.cnt[0] + MR_FEW;
+  if (p < n) {
+    const int id = a.ids[p];
+    bucket[p] = id < 0 ? a.E : id;
+  }
+  __syncthreads();
+  int less = 0, same = 0, before = 0, b = 0;
+  if (p < n) {
+    b = bucket[p];
+    for (int q = 0; q < n; q++) {
+      const int t = bucket[q];
+      less += t < b;
+      same += t == b;
+      before += t == b && q < p;
+    }
+    a.pairs[less + before] = p;
+    size[p] = before == 0 ? same : 0;
+  }
+  for (int e = threadIdx.x; e < a.E + 2; e += MR_THREADS) {
+    int c = 0;
+    for (int q = 0; q < n; q++) c += bucket[q] < e;
+    a.offsets[e] = c;
+  }
+  const int items = __syncthreads_count(p < n && before == 0);
+  if (p < n) {
+    int item = 0, pad = 0;
+    for (int q = 0; q < n; q++) {
+      const int t = size[q];
+      if (t && bucket[q] < b) {
+        item++;
+        pad += mr_ceil16(t);
+      }
+    }
+    if (before == 0)
+      reinterpret_cast<int4*>(a.plan + MOE_PLAN_HEADER)[item] = make_int4(b, less, same, pad);
+    a.where[p] = b == a.E ? make_int2(-1, 0) : make_int2(pad, before | mr_ceil16(same) << 16);
+  }
+  if (p == 0) {
+    a.plan[0] = items;
+    a.plan[1] = 0;
   }
 }
 
@@ -274,29 +328,35 @@ __global__ void __launch_bounds__(MR_THREADS) moe_select_kernel(RouteArgs a) {
   }
   __syncthreads();
   if constexpr (ONE) {
-    mr_place(a, s);
+    if (a.M * a.top_k <= MR_FEW)
+      mr_place_few(a, s);
+    else
+      mr_place(a, s);
   } else {
-    for (int e = threadIdx.x; e < nb; e += MR_THREADS) a.counts[(size_t)blockIdx.x * nb + e] = s.total[e];
+    for (int e = threadIdx.x; e < nb; e += MR_THREADS) a.counts[(size_t)e * a.blocks + blockIdx.x] = s.total[e];
   }
 }
 
 __global__ void __launch_bounds__(MR_THREADS) moe_place_kernel(RouteArgs a) {
   __shared__ RouteSmem s;
-  const int nb = a.E + 1;
-  for (int e = threadIdx.x; e < nb; e += MR_THREADS) {
-    s.total[e] = 0;
-    s.base[e] = 0;
-  }
+  const int nb = a.E + 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
   pdl_trigger();
-  __syncthreads();
-  const int n = a.blocks * nb, mine = blockIdx.x * nb;
-  for (int i = threadIdx.x; i < n; i += MR_THREADS) {
-    const int c = a.counts[i];
-    if (c) {
-      const int e = i % nb;
-      atomicAdd(&s.total[e], c);
-      if (i < mine) atomicAdd(&s.base[e], c);
+  // a warp per bucket: the blocks' counts, all and the earlier blocks'
+  for (int e = warp; e < nb; e += MR_WARPS) {
+    int all = 0, earlier = 0;
+#pragma unroll
+    for (int i = 0; i < (MOE_ROUTE_BLOCKS + 31) / 32; i++) {
+      const int b = i * 32 + lane;
+      const int c = b < a.blocks ? a.counts[(size_t)e * a.blocks + b] : 0;
+      all += c;
+      earlier += b < (int)blockIdx.x ? c : 0;
+    }
+    all = __reduce_add_sync(0xffffffffu, all);
+    earlier = __reduce_add_sync(0xffffffffu, earlier);
+    if (lane == 0) {
+      s.total[e] = all;
+      s.base[e] = earlier;
     }
   }
   __syncthreads();
@@ -351,6 +411,7 @@ extern "C" int im_moe_route(const void* logits, int logits_f32, int64_t M, int64
   a.offsets = offsets;
   a.pairs = pairs;
   a.plan = reinterpret_cast<int*>(plan);
+  a.where = reinterpret_cast<int2*>(a.plan + p.where);
   a.counts = a.plan + p.counts;
   a.f32 = logits_f32;
   a.scoring = scoring;

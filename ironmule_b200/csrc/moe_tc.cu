@@ -68,8 +68,8 @@ struct TcArgs {
   const int4* items;
   unsigned* error;
   const unsigned char* tiles;  // the items' rows as tiles
-  const float* scale;    // per sorted position: the factor its row was divided by
-  const float* xlog;     // per sorted position: log2 |x|_2 (first product of a gated MLP)
+  const float* scale;    // per padded row: the factor it was divided by
+  const float* xlog;     // per padded row: log2 |x|_2 (first product of a gated MLP)
   unsigned char* next;   // the next product's tiles, and its rows' factors (written by the first product)
   float* hscale;
   const float* row_max;  // [E][128 cols]: a weight row's largest |w|
@@ -99,24 +99,23 @@ __device__ __forceinline__ size_t mt_tile(int padded, int n16, int K, int group)
 }
 __device__ __forceinline__ uint32_t mt_chunk(int r, int c) { return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4)); }
 
-// ---- the items' rows of x -> scaled fp16 tiles; a warp per row, grid (items, 128 / 16) -------------------------
-constexpr int MP_ROWS = 16;
-__global__ void __launch_bounds__(MP_ROWS * 32)
-moe_prep_kernel(const uint16_t* __restrict__ x, const int* __restrict__ plan, const int* __restrict__ pairs, int E,
-                int top_k, int by_pair, int K, unsigned char* __restrict__ tiles, float* __restrict__ scale,
-                float* __restrict__ xlog) {
+// ---- rows of x -> scaled fp16 tiles: a CTA per row, which it reads once and writes to the tiles of every expert that
+// its token chose (per_row = top_k; 1 when x has a row per pair) ------------------------------------------------------
+constexpr int MP_THREADS = 128;
+__global__ void __launch_bounds__(MP_THREADS)
+moe_prep_kernel(const uint16_t* __restrict__ x, const int2* __restrict__ where, int per_row, int K,
+                unsigned char* __restrict__ tiles, float* __restrict__ scale, float* __restrict__ xlog) {
+  __shared__ float sh[2][MP_THREADS / 32];
+  __shared__ int2 to[MOE_MAX_TOP_K];
   pdl_wait();
   pdl_trigger();
-  if ((int)blockIdx.x >= plan[0]) return;
-  const int4 item = reinterpret_cast<const int4*>(plan + MOE_PLAN_HEADER)[blockIdx.x];
-  const int r = blockIdx.y * MP_ROWS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (item.x == E || r >= item.z) return;
-  const int pos = item.y + r, pair = pairs[pos];
-  const uint4* src = reinterpret_cast<const uint4*>(x + (size_t)(by_pair ? pair : pair / top_k) * K);
+  const size_t row = blockIdx.x;
+  if ((int)threadIdx.x < per_row) to[threadIdx.x] = where[row * per_row + threadIdx.x];
+  const uint4* src = reinterpret_cast<const uint4*>(x + row * K);
   const int n = K / 8;
   float top = 0.f;
-#pragma unroll 4
-  for (int i = lane; i < n; i += 32) {
+#pragma unroll 2
+  for (int i = threadIdx.x; i < n; i += MP_THREADS) {
     const uint4 u = __ldg(src + i);
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
@@ -128,12 +127,15 @@ moe_prep_kernel(const uint16_t* __restrict__ x, const int* __restrict__ plan, co
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if ((threadIdx.x & 31) == 0) sh[0][threadIdx.x >> 5] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < MP_THREADS / 32; w++) top = fmaxf(top, sh[0][w]);
   const int e = mt_exp(top, 10);
   const float inv = mt_pow2(-e);
-  const int n16 = (item.z + 15) & ~15;
   float ss = 0.f;
-#pragma unroll 4
-  for (int i = lane; i < n; i += 32) {
+#pragma unroll 2
+  for (int i = threadIdx.x; i < n; i += MP_THREADS) {
     const uint4 u = __ldg(src + i);
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
     float f[8];
@@ -150,13 +152,23 @@ moe_prep_kernel(const uint16_t* __restrict__ x, const int* __restrict__ plan, co
       const __half2 v = __floats2half2_rn(f[j], f[j + 4]);
       h[j] = *reinterpret_cast<const uint32_t*>(&v);
     }
-    *reinterpret_cast<uint4*>(tiles + mt_tile(item.w, n16, K, i >> 3) + mt_chunk(r, i & 7)) =
-        make_uint4(h[0], h[1], h[2], h[3]);
+    for (int j = 0; j < per_row; j++) {
+      const int2 t = to[j];
+      if (t.x >= 0)
+        *reinterpret_cast<uint4*>(tiles + mt_tile(t.x, t.y >> 16, K, i >> 3) + mt_chunk(t.y & 0xffff, i & 7)) =
+            make_uint4(h[0], h[1], h[2], h[3]);
+    }
   }
   ss = warp_sum(ss);
-  if (lane == 0) {
-    scale[pos] = mt_pow2(e);
-    xlog[pos] = 0.5f * log2f(ss) + (float)e;  // -inf for a zero row
+  if ((threadIdx.x & 31) == 0) sh[1][threadIdx.x >> 5] = ss;
+  __syncthreads();
+  if ((int)threadIdx.x < per_row && to[threadIdx.x].x >= 0) {
+    float t = 0.f;
+#pragma unroll
+    for (int w = 0; w < MP_THREADS / 32; w++) t += sh[1][w];
+    const int at = to[threadIdx.x].x + (to[threadIdx.x].y & 0xffff);
+    scale[at] = mt_pow2(e);
+    xlog[at] = 0.5f * log2f(t) + (float)e;  // -inf for a zero row
   }
 }
 
@@ -366,16 +378,16 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
       for (int i = 0; i < 2; i++) {
         const int c = 64 * i + 32 * set + lane;
         if (c < rows) {
-          const int pos = item.y + c;
+          const int row = item.w + c;
           float hs = 0.f;
           if constexpr (GLU) {
-            const float bound = 2.f * a.xlog[pos] + log2f((float)a.p.K) + log2f(a.half_max[2 * item.x]) +
+            const float bound = 2.f * a.xlog[row] + log2f((float)a.p.K) + log2f(a.half_max[2 * item.x]) +
                                 log2f(a.half_max[2 * item.x + 1]);
             const int e = bound > -100.f ? (int)ceilf(fminf(bound, 135.f)) - 15 : -110;
             hs = mt_pow2(-e);
-            if (col == 0 && q == 0) a.hscale[pos] = mt_pow2(e);
+            if (col == 0 && q == 0) a.hscale[row] = mt_pow2(e);
           }
-          meta[32 * i + lane] = make_float4(a.scale[pos], hs, __int_as_float(GLU ? 0 : a.p.pairs[pos]), 0.f);
+          meta[32 * i + lane] = make_float4(a.scale[row], hs, __int_as_float(GLU ? 0 : a.p.pairs[item.y + c]), 0.f);
         }
       }
       __syncwarp();
@@ -532,10 +544,10 @@ MoeSpace moe_space(const MoePlan& p, int64_t pairs, int64_t K, int64_t I) {
   };
   const size_t padded = (size_t)(pairs + 15 * p.max_items);
   s.tiles = take(padded * K * 2);
-  s.scale = take((size_t)pairs * 4);
-  s.xlog = take((size_t)pairs * 4);
+  s.scale = take(padded * 4);
+  s.xlog = take(padded * 4);
   s.next = take(padded * I * 2);
-  s.hscale = take(I ? (size_t)pairs * 4 : 0);
+  s.hscale = take(I ? padded * 4 : 0);
   s.total = at;
   return s;
 }
@@ -543,10 +555,9 @@ MoeSpace moe_space(const MoePlan& p, int64_t pairs, int64_t K, int64_t I) {
 int moe_prep_launch(const MoePlan& p, const MoeProduct& a, const uint16_t* x, int by_pair, const MoeSpace& s,
                     void* workspace, cudaStream_t st) {
   char* ws = reinterpret_cast<char*>(workspace);
-  const int64_t most = a.M < MOE_ITEM_ROWS ? a.M : MOE_ITEM_ROWS;  // rows of an item
-  return launch("moe_prep_kernel", moe_prep_kernel,
-                dim3((unsigned)p.max_items, (unsigned)((most + MP_ROWS - 1) / MP_ROWS)), dim3(MP_ROWS * 32), 0, st, x,
-                a.plan, a.pairs, a.E, a.top_k, by_pair, a.K,
+  const int64_t rows = by_pair ? (int64_t)a.M * a.top_k : a.M;
+  return launch("moe_prep_kernel", moe_prep_kernel, dim3((unsigned)rows), dim3(MP_THREADS), 0, st, x,
+                reinterpret_cast<const int2*>(a.plan + p.where), by_pair ? 1 : a.top_k, a.K,
                 reinterpret_cast<unsigned char*>(ws + s.tiles), reinterpret_cast<float*>(ws + s.scale),
                 reinterpret_cast<float*>(ws + s.xlog));
 }
