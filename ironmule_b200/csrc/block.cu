@@ -17,6 +17,7 @@ namespace im {
 
 constexpr int BR_THREADS = 256;
 constexpr int BR_MAX_PLACES = 32;
+constexpr int BR_BATCH = 8;
 
 struct BlockArgs {
   const uint16_t* y;
@@ -87,6 +88,12 @@ __global__ void __launch_bounds__(BR_THREADS) block_residual_kernel(BlockArgs a)
   __syncthreads();
   const uint16_t* y = a.y + row * a.places * a.H;
   float b[VPT][8];
+  uint4 res[VPT];  // the residual, on its way while the places are summed
+#pragma unroll
+  for (int v = 0; v < VPT; v++) {
+    const int i = (v * BR_THREADS + threadIdx.x) * 8;
+    if (i < a.H) res[v] = br_load<VEC>(a.h + row * a.H, i, a.H);
+  }
 #pragma unroll
   for (int v = 0; v < VPT; v++) {
 #pragma unroll
@@ -96,14 +103,21 @@ __global__ void __launch_bounds__(BR_THREADS) block_residual_kernel(BlockArgs a)
       if (!a.w) {
         br_floats(br_load<VEC>(y, i, a.H), b[v]);
       } else {
-#pragma unroll 4
-        for (int j = 0; j < a.places; j++) {
-          const float w = ws[j];
-          if (w == 0.f) continue;
-          float f[8];
-          br_floats(br_load<VEC>(y + (size_t)j * a.H, i, a.H), f);
+        for (int j0 = 0; j0 < a.places; j0 += BR_BATCH) {  // a batch's loads leave together
+          uint4 u[BR_BATCH];
+          float w[BR_BATCH];
 #pragma unroll
-          for (int e = 0; e < 8; e++) b[v][e] = fmaf(w, f[e], b[v][e]);
+          for (int j = 0; j < BR_BATCH; j++) {
+            w[j] = j0 + j < a.places ? ws[j0 + j] : 0.f;
+            u[j] = w[j] != 0.f ? br_load<VEC>(y + (size_t)(j0 + j) * a.H, i, a.H) : make_uint4(0, 0, 0, 0);
+          }
+#pragma unroll
+          for (int j = 0; j < BR_BATCH; j++) {
+            float f[8];
+            br_floats(u[j], f);
+#pragma unroll
+            for (int e = 0; e < 8; e++) b[v][e] = fmaf(w[j], f[e], b[v][e]);
+          }
         }
       }
     }
@@ -145,7 +159,7 @@ __global__ void __launch_bounds__(BR_THREADS) block_residual_kernel(BlockArgs a)
           for (int e = 0; e < 8; e++) b[v][e] *= g0;
         }
       }
-      br_floats(br_load<VEC>(a.h + row * a.H, i, a.H), f);
+      br_floats(res[v], f);
 #pragma unroll
       for (int e = 0; e < 8; e++) {
         b[v][e] = fmaf(a.scale, f[e], b[v][e]);

@@ -61,7 +61,7 @@ constexpr size_t MT_OFF_BAR = MT_OFF_W + (size_t)MT_W * 2 * MOE_BLOCK_BYTES;
 constexpr int MT_DONE = 0, MT_FULL = MT_DONE + MT_S, MT_W_FULL = MT_FULL + MT_S, MT_W_EMPTY = MT_W_FULL + MT_W,
               MT_D_FULL = MT_W_EMPTY + MT_W, MT_D_EMPTY = MT_D_FULL + 2, MT_BARS = MT_D_EMPTY + 2;
 constexpr size_t MT_OFF_META = (MT_OFF_BAR + MT_BARS * 8 + 16 + 15) / 16 * 16;  // an epilogue warp's columns
-constexpr size_t MT_SMEM = 1024 + MT_OFF_META + (size_t)MT_EPI * 64 * 16;
+constexpr size_t MT_SMEM = 1024 + MT_OFF_META + (size_t)MT_EPI * 64 * 8;
 
 struct TcArgs {
   MoeProduct p;
@@ -187,10 +187,11 @@ __device__ __forceinline__ void mt_expand(uint32_t u, __half2 s24, __half2 s20, 
   }
 }
 
-__device__ __forceinline__ float mt_gated(bool geglu, float g, float u) {
-  if (!geglu) return __fdividef(g, 1.0f + __expf(-g)) * u;
-  const float inner = 0.7978845608028654f * (g + 0.044715f * g * g * g);
-  return 0.5f * g * (1.0f + tanhf(inner)) * u;
+// act(g) * u. Both gates are g times a sigmoid: of g, or (gelu by tanh: 0.5 (1 + tanh t) = sigmoid(2 t)) of 2 t.
+template <int EPI>
+__device__ __forceinline__ float mt_gated(float g, float u) {
+  const float t = EPI == IM_EPI_GEGLU ? 1.5957691216057308f * (g + 0.044715f * g * g * g) : g;
+  return __fdividef(g, 1.0f + __expf(-t)) * u;
 }
 
 __device__ __forceinline__ void mt_arrive(uint32_t bar) {
@@ -240,8 +241,9 @@ __device__ __forceinline__ void mt_group(const unsigned char* codes, const unsig
       : "memory");
 }
 
-template <bool GLU>
+template <int EPI>
 __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
+  constexpr bool GLU = EPI != IM_EPI_STORE;
   extern __shared__ unsigned char mt_raw[];
   const uint32_t raw = qt_smem(mt_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
@@ -354,7 +356,7 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
   } else if (warp < MT_W_LOAD) {
     // ---- epilogue: lane = output of the block, columns = the item's rows ---------------------------------------
     const int q = warp & 3, set = (warp - MT_W_EPI) >> 2;
-    float4* meta = reinterpret_cast<float4*>(sbase + MT_OFF_META) + (warp - MT_W_EPI) * 64;
+    float2* meta = reinterpret_cast<float2*>(sbase + MT_OFF_META) + (warp - MT_W_EPI) * 64;
     const bool paired = (nout & 1) == 0 && (reinterpret_cast<uintptr_t>(a.p.y) & 3) == 0;
     pdl_wait();
     pdl_trigger();
@@ -370,24 +372,29 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
         }
         continue;
       }
-      // this lane's weight row's factor; this warp's columns 64 i + 32 set + lane: the rows' factors, the output row
+      // this lane's weight row's factor; this warp's columns 64 i + 32 set + lane: the rows' factors (of the gate input,
+      // and of the up input with the factor of h), or the factor and the output row
       const float wscale =
           mt_pow2(mt_exp(a.row_max[((size_t)item.x * a.cols + col) * 128 + q * 32 + lane], MT_WBITS));
+      float lg = 0.f;
+      if constexpr (GLU) lg = log2f((float)a.p.K) + log2f(a.half_max[2 * item.x]) + log2f(a.half_max[2 * item.x + 1]);
       __syncwarp();
 #pragma unroll
       for (int i = 0; i < 2; i++) {
         const int c = 64 * i + 32 * set + lane;
         if (c < rows) {
           const int row = item.w + c;
-          float hs = 0.f;
+          const float xs = a.scale[row];
+          float2 m = make_float2(xs, 0.f);
           if constexpr (GLU) {
-            const float bound = 2.f * a.xlog[row] + log2f((float)a.p.K) + log2f(a.half_max[2 * item.x]) +
-                                log2f(a.half_max[2 * item.x + 1]);
+            const float bound = 2.f * a.xlog[row] + lg;
             const int e = bound > -100.f ? (int)ceilf(fminf(bound, 135.f)) - 15 : -110;
-            hs = mt_pow2(-e);
+            m.y = xs * mt_pow2(-e);
             if (col == 0 && q == 0) a.hscale[row] = mt_pow2(e);
+          } else {
+            m.y = __int_as_float(a.p.pairs[item.y + c]);
           }
-          meta[32 * i + lane] = make_float4(a.scale[row], hs, __int_as_float(GLU ? 0 : a.p.pairs[item.y + c]), 0.f);
+          meta[32 * i + lane] = m;
         }
       }
       __syncwarp();
@@ -409,48 +416,54 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
               "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
             : "r"(ta));
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-        const float4* m = meta + 32 * i;
         // Of two columns j, j + 1 each lane finishes one, with its partner lane's value of it (the partner: the other
         // half of a gated output, or the neighbouring output, so that two outputs leave in one store).
-        const int other = GLU ? 16 : 1;
-        const bool second = lane & other;
-        const int f = GLU ? (col * 4 + q) * 16 + (lane & 15) : col * 128 + q * 32 + lane;
+        const int other = GLU ? 16 : 1, second = (lane & other) != 0;
+        const float2* m = meta + 32 * i + second;
         if constexpr (GLU) {
-          // the next product's tiles: group f / 64, chunk f % 64 / 8, the element's place in the operand order
-          const int n16 = (rows + 15) & ~15, chunk = (f & 63) >> 3;
-          unsigned char* h = a.next + mt_tile(item.w, n16, nout, f >> 6) + 2 * mt_perm(f & 7);
+          // The next product's tiles: group f / 64, chunk f % 64 / 8, the element's place in the operand order; rows up
+          // to the next sixteen exist there and are written too. Row c0 + j + second swizzles with (j + second) % 8,
+          // so four pointers serve every j.
+          const int f = (col * 4 + q) * 16 + (lane & 15), n16 = (rows + 15) & ~15, chunk = (f & 63) >> 3;
+          unsigned char* h = a.next + mt_tile(item.w, n16, nout, f >> 6) + 2 * mt_perm(f & 7) + (c0 + second) * 128;
+          unsigned char* at[4];
 #pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            const float give = __uint_as_float(second ? v[j] : v[j + 1]) * wscale;
-            const float keep = __uint_as_float(second ? v[j + 1] : v[j]) * wscale;
-            const float got = __shfl_xor_sync(0xffffffffu, give, 16);
-            const float4 mj = m[second ? j + 1 : j];
-            // lanes 0-15 hold gate features, 16-31 the matching up features
-            const float g = (second ? got : keep) * mj.x, u = (second ? keep : got) * mj.x;
-            const float o = mt_gated(a.p.epilogue == IM_EPI_GEGLU, g, u) * mj.y;
-            const int jj = j + (second ? 1 : 0);
-            if (jj < n && f < nout) *reinterpret_cast<__half*>(h + mt_chunk(c0 + jj, chunk)) = __float2half_rn(o);
+          for (int w = 0; w < 4; w++) at[w] = h + ((chunk ^ (2 * w + second)) << 4);
+#pragma unroll
+          for (int half = 0; half < 2; half++) {
+            if (c0 + 16 * half >= n16) break;
+#pragma unroll
+            for (int j = 16 * half; j < 16 * half + 16; j += 2) {
+              const float give = __uint_as_float(second ? v[j] : v[j + 1]) * wscale;
+              const float keep = __uint_as_float(second ? v[j + 1] : v[j]) * wscale;
+              const float got = __shfl_xor_sync(0xffffffffu, give, 16);
+              const float2 mj = m[j];
+              // lanes 0-15 hold gate features, 16-31 the matching up features
+              const float g = (second ? got : keep) * mj.x, u = (second ? keep : got) * mj.y;
+              *reinterpret_cast<__half*>(at[j / 2 % 4] + j * 128) = __float2half_rn(mt_gated<EPI>(g, u));
+            }
           }
-        } else if (paired) {
+        } else {
+          const int f = col * 128 + q * 32 + lane;
           uint16_t* y = a.p.y + (f & ~1);
 #pragma unroll
           for (int j = 0; j < 32; j += 2) {
             const float give = __uint_as_float(second ? v[j] : v[j + 1]) * wscale;
             const float keep = __uint_as_float(second ? v[j + 1] : v[j]) * wscale;
             const float got = __shfl_xor_sync(0xffffffffu, give, 1);
-            const float4 mj = m[second ? j + 1 : j];
+            const float2 mj = m[j];
             const float k1 = keep * mj.x, g1 = got * mj.x;
             uint32_t o;
             asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(o) : "f"(second ? k1 : g1), "f"(second ? g1 : k1));
-            if (j + (second ? 1 : 0) < n && f < nout)
-              *reinterpret_cast<uint32_t*>(y + (size_t)__float_as_int(mj.z) * nout) = o;
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 32; j++) {
-            const float4 mj = m[j];
-            if (j < n && f < nout)
-              a.p.y[(size_t)__float_as_int(mj.z) * nout + f] = to_bf(__uint_as_float(v[j]) * wscale * mj.x);
+            if (j + second < n && (f & ~1) < nout) {
+              uint16_t* to = y + (size_t)__float_as_int(mj.y) * nout;
+              if (paired) {
+                *reinterpret_cast<uint32_t*>(to) = o;
+              } else {
+                to[0] = (uint16_t)o;
+                if ((f | 1) < nout) to[1] = (uint16_t)(o >> 16);
+              }
+            }
           }
         }
       }
@@ -562,12 +575,12 @@ int moe_prep_launch(const MoePlan& p, const MoeProduct& a, const uint16_t* x, in
                 reinterpret_cast<float*>(ws + s.xlog));
 }
 
-template <bool GLU>
+template <int EPI>
 static int mt_launch(const TcArgs& a, int64_t tiles, cudaStream_t st) {
   static int sms = 0;
   if (!sms) {
     int dev = 0, n = 0;
-    cudaError_t e = cudaFuncSetAttribute(moe_tc_kernel<GLU>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)MT_SMEM);
+    cudaError_t e = cudaFuncSetAttribute(moe_tc_kernel<EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)MT_SMEM);
     if (e == cudaSuccess) e = cudaGetDevice(&dev);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
     if (e != cudaSuccess) {
@@ -576,7 +589,7 @@ static int mt_launch(const TcArgs& a, int64_t tiles, cudaStream_t st) {
     }
     sms = n;
   }
-  return launch("moe_tc_kernel", moe_tc_kernel<GLU>, dim3((unsigned)(tiles < sms ? tiles : sms)), dim3(MT_THREADS),
+  return launch("moe_tc_kernel", moe_tc_kernel<EPI>, dim3((unsigned)(tiles < sms ? tiles : sms)), dim3(MT_THREADS),
                 MT_SMEM, st, a);
 }
 
@@ -598,8 +611,11 @@ int moe_product_launch(const MoePlan& p, const MoeProduct& prod, const MoeSpace&
   a.half_max = a.row_max + (size_t)prod.E * a.cols * 128;
   const int64_t tiles = p.max_items * a.cols;
   IM_REQUIRE(tiles < (1ll << 31), IM_UNSUPPORTED, "grouped product: too many tiles");
-  if (prod.epilogue == IM_EPI_STORE) return mt_launch<false>(a, tiles, st);
-  return mt_launch<true>(a, tiles, st);
+  switch (prod.epilogue) {
+    case IM_EPI_STORE: return mt_launch<IM_EPI_STORE>(a, tiles, st);
+    case IM_EPI_SWIGLU: return mt_launch<IM_EPI_SWIGLU>(a, tiles, st);
+    default: return mt_launch<IM_EPI_GEGLU>(a, tiles, st);
+  }
 }
 
 }  // namespace im
