@@ -25,6 +25,9 @@
 //    16-byte asynchronous copies occupied four warps and the load pipe; a prefill took 1407 and 527 us.) The k order
 //    within 8 follows the code expansion (k, k + 4 adjacent);
 //  * warp 1 issues 8 MMAs of K = 16 a stage into one of two 128-column accumulators;
+//  * warp 11 looks a tile up ahead of the others: its item, its weight rows' factors, its columns' factors and output
+//    rows, into a ring of 3 in shared memory (looked up by every warp for itself, two dependent trips to L2 stood at
+//    the head of every tile: 132 us against __DOWN__ for a prefill's second product);
 //  * warps 2-9, two sets of 4 for alternate 32 columns, read a finished accumulator (lane = output), scale it, apply
 //    the gate, and store.
 // Every column (row of x) is its own sum in K order, so a row's bits do not depend on the other rows.
@@ -44,6 +47,7 @@ namespace im {
 constexpr int MT_N = MOE_ITEM_ROWS;       // rows of an item at most (MMA N)
 constexpr int MT_S = 4;                 // A and B stages of two groups (128 of K)
 constexpr int MT_W = 8;                 // weight ring, two groups each
+constexpr int MT_I = 3;                 // tiles looked up ahead
 constexpr int MT_B = 2 * MT_N * 128;    // bytes of a B stage
 constexpr int MT_EPI = 8;               // epilogue warps
 constexpr int MT_SETS = 4;              // expansion sets of four warps
@@ -59,9 +63,17 @@ constexpr size_t MT_OFF_W = (size_t)MT_S * MT_B;
 constexpr size_t MT_OFF_BAR = MT_OFF_W + (size_t)MT_W * 2 * MOE_BLOCK_BYTES;
 // barriers: a stage's MMAs completed; a stage's A and B in place; weight ring; accumulators
 constexpr int MT_DONE = 0, MT_FULL = MT_DONE + MT_S, MT_W_FULL = MT_FULL + MT_S, MT_W_EMPTY = MT_W_FULL + MT_W,
-              MT_D_FULL = MT_W_EMPTY + MT_W, MT_D_EMPTY = MT_D_FULL + 2, MT_BARS = MT_D_EMPTY + 2;
-constexpr size_t MT_OFF_META = (MT_OFF_BAR + MT_BARS * 8 + 16 + 15) / 16 * 16;  // an epilogue warp's columns
-constexpr size_t MT_SMEM = 1024 + MT_OFF_META + (size_t)MT_EPI * 64 * 8;
+              MT_D_FULL = MT_W_EMPTY + MT_W, MT_D_EMPTY = MT_D_FULL + 2, MT_I_FULL = MT_D_EMPTY + 2,
+              MT_C_FULL = MT_I_FULL + MT_I, MT_I_EMPTY = MT_C_FULL + MT_I, MT_BARS = MT_I_EMPTY + MT_I;
+// What the roles need to know of a tile.
+struct MtTile {
+  int4 item;
+  float inv[128], wscale[128];  // the weight rows' factors: to the operands' range, and back
+  float2 col[128];              // the columns' factors: of the gate and of the up input; or the factor and the output row
+};
+constexpr size_t MT_OFF_TILE = (MT_OFF_BAR + MT_BARS * 8 + 16 + 15) / 16 * 16;
+constexpr size_t MT_SMEM = 1024 + MT_OFF_TILE + MT_I * sizeof(MtTile);
+constexpr int MT_READERS = 3 + MT_EPI + 4 * MT_SETS;  // warps that read a tile's entry
 
 struct TcArgs {
   MoeProduct p;
@@ -275,6 +287,11 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
       qt_init(&b[MT_D_FULL + s], 1u);
       qt_init(&b[MT_D_EMPTY + s], MT_EPI);
     }
+    for (int s = 0; s < MT_I; s++) {
+      qt_init(&b[MT_I_FULL + s], 1u);
+      qt_init(&b[MT_C_FULL + s], 1u);
+      qt_init(&b[MT_I_EMPTY + s], MT_READERS);
+    }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -285,6 +302,14 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
   // The routing's plan was finished before the launch that precedes this one (the prep kernel, or the first product)
   // let this one begin: the plan and the weights are read without waiting, rows and outputs only after pdl_wait().
   const int ntiles = a.p.plan[0] * a.cols;
+  MtTile* const info = reinterpret_cast<MtTile*>(sbase + MT_OFF_TILE);
+  uint32_t islot = 0, iphase = 0;  // this warp's place in the ring of tiles
+  auto tile_wait = [&] { return qt_wait_short(bars + 8 * (MT_I_FULL + islot), iphase, abort_flag, a.error); };
+  auto tile_free = [&] {  // this warp has read what it needs
+    __syncwarp();
+    if (lane == 0) mt_arrive(bars + 8 * (MT_I_EMPTY + islot));
+    if (++islot == MT_I) islot = 0, iphase ^= 1u;
+  };
 
   if (warp == 0) {
     // ---- weights -------------------------------------------------------------------------------------------
@@ -293,7 +318,9 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
     uint32_t s = 0, phase = 1;
     int k = 0;
     for (int tile = blockIdx.x; tile < ntiles; tile += gridDim.x) {
-      const int expert = a.items[tile / a.cols].x;
+      if (!tile_wait()) goto weights_done;
+      const int expert = info[islot].item.x;
+      tile_free();
       if (expert == a.p.E) continue;
       const unsigned char* src =
           a.p.wp + (size_t)expert * a.expert_bytes + (size_t)(tile % a.cols) * G * MOE_BLOCK_BYTES;
@@ -319,7 +346,9 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
     uint32_t s = 0, phase = 0;
     int k = 0, t = 0;
     for (int tile = blockIdx.x; tile < ntiles; tile += gridDim.x) {
-      const int4 item = a.items[tile / a.cols];
+      if (!tile_wait()) break;
+      const int4 item = info[islot].item;
+      tile_free();
       if (item.x == a.p.E) continue;
       // f32 accumulate, f16 A and B, K-major, N = the item's rows in sixteens, M = 128
       const uint32_t idesc = (1u << 4) | ((uint32_t)((item.z + 15) / 16 * 2) << 17) | ((128u >> 4) << 24);
@@ -356,48 +385,25 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
   } else if (warp < MT_W_LOAD) {
     // ---- epilogue: lane = output of the block, columns = the item's rows ---------------------------------------
     const int q = warp & 3, set = (warp - MT_W_EPI) >> 2;
-    float2* meta = reinterpret_cast<float2*>(sbase + MT_OFF_META) + (warp - MT_W_EPI) * 64;
     const bool paired = (nout & 1) == 0 && (reinterpret_cast<uintptr_t>(a.p.y) & 3) == 0;
     pdl_wait();
     pdl_trigger();
     int t = 0;
     for (int tile = blockIdx.x; tile < ntiles; tile += gridDim.x) {
-      const int4 item = a.items[tile / a.cols];
+      if (!tile_wait() || !qt_wait_short(bars + 8 * (MT_C_FULL + islot), iphase, abort_flag, a.error)) break;
+      const int4 item = info[islot].item;
+      const float wscale = info[islot].wscale[q * 32 + lane];
+      const float2* meta = info[islot].col;
       const int col = tile % a.cols, rows = item.z;
-      if (item.x == a.p.E) {  // places without an expert: zeros (a sorted output holds none of them)
+      if (item.x == a.p.E) {  // places without an expert: zeros
         if (!GLU) {
           const int f = col * 128 + q * 32 + lane;
           for (int j = set; j < rows; j += 2)
             if (f < nout) a.p.y[(size_t)a.p.pairs[item.y + j] * nout + f] = 0;
         }
+        tile_free();
         continue;
       }
-      // this lane's weight row's factor; this warp's columns 64 i + 32 set + lane: the rows' factors (of the gate input,
-      // and of the up input with the factor of h), or the factor and the output row
-      const float wscale =
-          mt_pow2(mt_exp(a.row_max[((size_t)item.x * a.cols + col) * 128 + q * 32 + lane], MT_WBITS));
-      float lg = 0.f;
-      if constexpr (GLU) lg = log2f((float)a.p.K) + log2f(a.half_max[2 * item.x]) + log2f(a.half_max[2 * item.x + 1]);
-      __syncwarp();
-#pragma unroll
-      for (int i = 0; i < 2; i++) {
-        const int c = 64 * i + 32 * set + lane;
-        if (c < rows) {
-          const int row = item.w + c;
-          const float xs = a.scale[row];
-          float2 m = make_float2(xs, 0.f);
-          if constexpr (GLU) {
-            const float bound = 2.f * a.xlog[row] + lg;
-            const int e = bound > -100.f ? (int)ceilf(fminf(bound, 135.f)) - 15 : -110;
-            m.y = xs * mt_pow2(-e);
-            if (col == 0 && q == 0) a.hscale[row] = mt_pow2(e);
-          } else {
-            m.y = __int_as_float(a.p.pairs[item.y + c]);
-          }
-          meta[32 * i + lane] = m;
-        }
-      }
-      __syncwarp();
       const int buf = t & 1;
       if (!qt_wait_short(bars + 8 * (MT_D_FULL + buf), (uint32_t)((t / 2) & 1), abort_flag, a.error)) break;
       t++;
@@ -419,7 +425,7 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
         // Of two columns j, j + 1 each lane finishes one, with its partner lane's value of it (the partner: the other
         // half of a gated output, or the neighbouring output, so that two outputs leave in one store).
         const int other = GLU ? 16 : 1, second = (lane & other) != 0;
-        const float2* m = meta + 32 * i + second;
+        const float2* m = meta + c0 + second;
         if constexpr (GLU) {
           // The next product's tiles: group f / 64, chunk f % 64 / 8, the element's place in the operand order; rows up
           // to the next sixteen exist there and are written too. Row c0 + j + second swizzles with (j + second) % 8,
@@ -470,8 +476,65 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
       if (lane == 0) mt_arrive(bars + 8 * (MT_D_EMPTY + buf));
+      tile_free();
     }
   } else if (warp < MT_W_TRANS) {
+    if (warp == MT_W_LOAD + 1) {
+      // ---- the tiles, ahead of the other warps -----------------------------------------------------------------------
+      const int step = gridDim.x;
+      int4 item = (int)blockIdx.x < ntiles ? a.items[blockIdx.x / a.cols] : make_int4(0, 0, 0, 0);
+      bool waited = false;
+      for (int tile = blockIdx.x; tile < ntiles; tile += step) {
+        const int4 next = tile + step < ntiles ? a.items[(tile + step) / a.cols] : item;
+        const bool closed = item.x == a.p.E;
+        float top[4] = {};
+        if (!closed) {
+          const float* rm = a.row_max + ((size_t)item.x * a.cols + tile % a.cols) * 128 + lane;
+#pragma unroll
+          for (int i = 0; i < 4; i++) top[i] = rm[32 * i];
+        }
+        if (!qt_wait_short(bars + 8 * (MT_I_EMPTY + islot), iphase ^ 1u, abort_flag, a.error)) break;
+        MtTile& out = info[islot];
+        if (lane == 0) out.item = item;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const int e = mt_exp(top[i], MT_WBITS);
+          out.inv[32 * i + lane] = mt_pow2(-e);
+          out.wscale[32 * i + lane] = mt_pow2(e);
+        }
+        __syncwarp();
+        if (lane == 0) mt_arrive(bars + 8 * (MT_I_FULL + islot));
+        if (!waited) {
+          pdl_wait();
+          waited = true;
+        }
+        if (!closed) {
+          float lg = 0.f;
+          if constexpr (GLU)
+            lg = log2f((float)a.p.K) + log2f(a.half_max[2 * item.x]) + log2f(a.half_max[2 * item.x + 1]);
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const int c = 32 * i + lane, row = item.w + c;
+            if (c < item.z) {
+              float2 m = make_float2(a.scale[row], 0.f);
+              if constexpr (GLU) {
+                const float bound = 2.f * a.xlog[row] + lg;
+                const int e = bound > -100.f ? (int)ceilf(fminf(bound, 135.f)) - 15 : -110;
+                m.y = m.x * mt_pow2(-e);
+                if (tile % a.cols == 0) a.hscale[row] = mt_pow2(e);
+              } else {
+                m.y = __int_as_float(a.p.pairs[item.y + c]);
+              }
+              out.col[c] = m;
+            }
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mt_arrive(bars + 8 * (MT_C_FULL + islot));
+        if (++islot == MT_I) islot = 0, iphase ^= 1u;
+        item = next;
+      }
+    }
     // ---- rows ----------------------------------------------------------------------------------------------------
     if (warp == MT_W_LOAD) {
       const bool leader = qt_elect();
@@ -479,7 +542,9 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
       uint32_t s = 0, phase = 1;
       int k = 0;
       for (int tile = blockIdx.x; tile < ntiles; tile += gridDim.x) {
-        const int4 item = a.items[tile / a.cols];
+        if (!tile_wait()) goto rows_done;
+        const int4 item = info[islot].item;
+        tile_free();
         if (item.x == a.p.E) continue;
         const uint32_t bytes = (uint32_t)((item.z + 15) & ~15) * 128u;
         const unsigned char* src = a.tiles + (size_t)item.w * a.p.K * 2;
@@ -507,10 +572,11 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
     int skip = 2 * set;  // groups of the next tile that lie before this set's next stage
     const int even = G + (G & 1);
     for (int tile = blockIdx.x; tile < ntiles; tile += gridDim.x) {
-      const int expert = a.items[tile / a.cols].x;
+      if (!tile_wait()) goto expand_done;
+      const int expert = info[islot].item.x;
+      const float inv = info[islot].inv[q * 32 + lane];
+      tile_free();
       if (expert == a.p.E) continue;
-      const float inv = mt_pow2(
-          -mt_exp(a.row_max[((size_t)expert * a.cols + tile % a.cols) * 128 + q * 32 + lane], MT_WBITS));
       int g = skip;
       for (; g < G; g += 2 * MT_SETS) {
         if (!qt_wait_short(bars + 8 * (MT_W_FULL + sw), wphase, abort_flag, a.error)) goto expand_done;
