@@ -389,7 +389,7 @@ int im_philox4x32_10(uint64_t seed, uint64_t offset, uint32_t stream_id, uint32_
  * products completed); synchronises.
  *
  * im_block_residual: joins the places of a block, and the block to the residual stream, and takes the next norm:
- *   b = sum_j weights[m, j] y[m, j] (places of weight 0 are not read; weights NULL: the one place as it is)
+ *   b = sum_j weights[m, j] y[m, j] (places of weight 0 are left out; weights NULL: the one place as it is)
  *   b = b / sqrt(mean(b^2) + eps) * w'            with post_norm (w' = w, or 1 + w with gemma)
  *   h_out = bf16(residual_scale * h + gate * b)   (gate bf16: gate[m * gate_row_stride + i * gate_col_stride], or NULL)
  *   z = bf16(v / sqrt(mean(v^2) + eps) * w')      with next_norm; v = h_out before its rounding

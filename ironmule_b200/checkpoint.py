@@ -216,6 +216,8 @@ def save_mlx_4bit(model: QuantModel, root: str | Path) -> Path:
 
     if model.tp != 1:
         raise CheckpointError("save a tensor-parallel model from its tp = 1 counterpart")
+    if model.cfg.experts:
+        raise CheckpointError("a model with experts keeps its experts' weights packed: it cannot be written back")
     c = model.cfg
     root = Path(root)
     root.mkdir(parents=True, exist_ok=True)

@@ -7,7 +7,7 @@
 //
 // Everything is float32 in registers between one read of y and h and one write of h' and z; each output is rounded
 // once, z from the float32 h'. out_sq is the sum of squares of the ROUNDED h' row (what a qGEMM with a fused RMSNorm
-// prologue normalises). A place of weight 0 is not read, so what lies there (no expert chosen) does not matter.
+// prologue normalises). A place of weight 0 is left out, so what lies there (no expert chosen) does not matter.
 // One CTA per row, 8 consecutive elements per thread and step; sums in a fixed order (thread, warp tree, warps in
 // order), so a row's bits do not depend on the other rows. Bound by HBM for many rows, by two block reductions for few.
 #include "common.cuh"
@@ -17,7 +17,7 @@ namespace im {
 
 constexpr int BR_THREADS = 256;
 constexpr int BR_MAX_PLACES = 32;
-constexpr int BR_BATCH = 8;
+constexpr int BR_BATCH = 4;
 
 struct BlockArgs {
   const uint16_t* y;
@@ -59,16 +59,23 @@ __device__ __forceinline__ uint4 br_load(const uint16_t* p, int i, int H) {
   }
 }
 
+// Eight floats rounded to bf16 (nearest even) in pairs.
+__device__ __forceinline__ uint4 br_round(const float (&f)[8]) {
+  uint32_t u[4];
+#pragma unroll
+  for (int j = 0; j < 4; j++) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(u[j]) : "f"(f[2 * j + 1]), "f"(f[2 * j]));
+  return make_uint4(u[0], u[1], u[2], u[3]);
+}
+
 template <bool VEC>
-__device__ __forceinline__ void br_store(uint16_t* p, int i, int H, const uint16_t (&e)[8]) {
+__device__ __forceinline__ void br_store(uint16_t* p, int i, int H, const uint4& u) {
   if constexpr (VEC) {
-    *reinterpret_cast<uint4*>(p + i) =
-        make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16, e[4] | (uint32_t)e[5] << 16,
-                   e[6] | (uint32_t)e[7] << 16);
+    *reinterpret_cast<uint4*>(p + i) = u;
   } else {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
     for (int j = 0; j < 8; j++)
-      if (i + j < H) p[i + j] = e[j];
+      if (i + j < H) p[i + j] = (uint16_t)(w[j / 2] >> (16 * (j & 1)));
   }
 }
 
@@ -78,14 +85,13 @@ __device__ __forceinline__ void br_floats(const uint4& u, float (&f)[8]) {
 }
 
 template <int VPT, bool VEC>
-__global__ void __launch_bounds__(BR_THREADS) block_residual_kernel(BlockArgs a) {
+// Up to 2048 columns eight CTAs an SM: a prefill of 4096 rows x 8 places x 2048 takes 37 us, 42 at the four that the
+// compiler's own register count allows.
+__global__ void __launch_bounds__(BR_THREADS, VPT == 1 && VEC ? 8 : 1) block_residual_kernel(BlockArgs a) {
   __shared__ float sh[BR_THREADS / 32];
-  __shared__ float ws[BR_MAX_PLACES];
   pdl_wait();
   pdl_trigger();
   const size_t row = blockIdx.x;
-  if (a.w && (int)threadIdx.x < a.places) ws[threadIdx.x] = a.w[row * a.places + threadIdx.x];
-  __syncthreads();
   const uint16_t* y = a.y + row * a.places * a.H;
   float b[VPT][8];
   uint4 res[VPT];  // the residual, on its way while the places are summed
@@ -103,20 +109,20 @@ __global__ void __launch_bounds__(BR_THREADS) block_residual_kernel(BlockArgs a)
       if (!a.w) {
         br_floats(br_load<VEC>(y, i, a.H), b[v]);
       } else {
-        for (int j0 = 0; j0 < a.places; j0 += BR_BATCH) {  // a batch's loads leave together
+        const float* w = a.w + row * a.places;
+        for (int j0 = 0; j0 < a.places; j0 += BR_BATCH) {  // a batch's loads leave together, whatever the weights
           uint4 u[BR_BATCH];
-          float w[BR_BATCH];
+#pragma unroll
+          for (int j = 0; j < BR_BATCH; j++)
+            u[j] = j0 + j < a.places ? br_load<VEC>(y + (size_t)(j0 + j) * a.H, i, a.H) : make_uint4(0, 0, 0, 0);
 #pragma unroll
           for (int j = 0; j < BR_BATCH; j++) {
-            w[j] = j0 + j < a.places ? ws[j0 + j] : 0.f;
-            u[j] = w[j] != 0.f ? br_load<VEC>(y + (size_t)(j0 + j) * a.H, i, a.H) : make_uint4(0, 0, 0, 0);
-          }
-#pragma unroll
-          for (int j = 0; j < BR_BATCH; j++) {
+            const float wj = j0 + j < a.places ? __ldg(w + j0 + j) : 0.f;
+            if (wj == 0.f) continue;  // what lies there does not matter, NaN included
             float f[8];
             br_floats(u[j], f);
 #pragma unroll
-            for (int e = 0; e < 8; e++) b[v][e] = fmaf(w[j], f[e], b[v][e]);
+            for (int e = 0; e < 8; e++) b[v][e] = fmaf(wj, f[e], b[v][e]);
           }
         }
       }
@@ -146,7 +152,6 @@ __global__ void __launch_bounds__(BR_THREADS) block_residual_kernel(BlockArgs a)
     const int i = (v * BR_THREADS + threadIdx.x) * 8;
     if (i < a.H) {
       float f[8];
-      uint16_t o[8];
       if (a.gate) {
         const uint16_t* g = a.gate + row * a.gate_row;
         if (a.gate_col) {
@@ -163,13 +168,16 @@ __global__ void __launch_bounds__(BR_THREADS) block_residual_kernel(BlockArgs a)
 #pragma unroll
       for (int e = 0; e < 8; e++) {
         b[v][e] = fmaf(a.scale, f[e], b[v][e]);
-        o[e] = to_bf(b[v][e]);
-        if (VEC || i + e < a.H) {
-          ss = fmaf(b[v][e], b[v][e], ss);
-          sq = fmaf(bf(o[e]), bf(o[e]), sq);
-        }
+        if (VEC || i + e < a.H) ss = fmaf(b[v][e], b[v][e], ss);
       }
+      const uint4 o = br_round(b[v]);
       br_store<VEC>(a.h_out + row * a.H, i, a.H, o);
+      if (a.out_sq) {
+        br_floats(o, f);
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+          if (VEC || i + e < a.H) sq = fmaf(f[e], f[e], sq);
+      }
     }
   }
   if (a.out_sq) {
@@ -183,11 +191,10 @@ __global__ void __launch_bounds__(BR_THREADS) block_residual_kernel(BlockArgs a)
       const int i = (v * BR_THREADS + threadIdx.x) * 8;
       if (i < a.H) {
         float w[8];
-        uint16_t o[8];
         br_floats(br_load<VEC>(a.next, i, a.H), w);
 #pragma unroll
-        for (int e = 0; e < 8; e++) o[e] = to_bf(b[v][e] * inv * (a.gemma ? 1.0f + w[e] : w[e]));
-        br_store<VEC>(a.z + row * a.H, i, a.H, o);
+        for (int e = 0; e < 8; e++) b[v][e] = b[v][e] * inv * (a.gemma ? 1.0f + w[e] : w[e]);
+        br_store<VEC>(a.z + row * a.H, i, a.H, br_round(b[v]));
       }
     }
   }

@@ -27,7 +27,7 @@
 //  * warp 1 issues 8 MMAs of K = 16 a stage into one of two 128-column accumulators;
 //  * warp 11 looks a tile up ahead of the others: its item, its weight rows' factors, its columns' factors and output
 //    rows, into a ring of 3 in shared memory (looked up by every warp for itself, two dependent trips to L2 stood at
-//    the head of every tile: 132 us against __DOWN__ for a prefill's second product);
+//    the head of every tile: 132 us against 120 for a prefill's second product);
 //  * warps 2-9, two sets of 4 for alternate 32 columns, read a finished accumulator (lane = output), scale it, apply
 //    the gate, and store.
 // Every column (row of x) is its own sum in K order, so a row's bits do not depend on the other rows.

@@ -14,6 +14,11 @@ of the SwiGLU), down -- plus bf16 norm weights; the tied 4-bit embedding doubles
 Every projection is also held repacked for the packed qGEMM (`kernels.Packed`: 1152-byte units of 32 rows x 64
 inputs in MMA-fragment order), which is what the forward reads.
 
+A model with experts (`ModelConfig.experts`) has a mixture-of-experts block in the place of its MLP: the attention's
+projection joins the residual stream and is normalised in one kernel (kernels.block_residual), the 4-bit router scores
+the rows, kernels.moe_route picks each row's experts, kernels.moe_mlp runs their gated MLPs over 4-bit weights, and
+block_residual joins the weighted places. Every one of them is row-invariant too.
+
 Forward of M rows (any mix of sequences), five launches per layer (seven for Gemma-3, whose attention and MLP
 outputs get their own RMSNorm before the residual add: o / down store, then im_rmsnorm_residual): embed (+ each row's sum of squares) -> per
 layer [qkv qGEMM with the input RMSNorm fused into its prologue, paged attention with the q/k norm + RoPE +
@@ -59,6 +64,9 @@ class ModelConfig:
     rope_local_theta: float = 10_000.0
     query_scale: float = 0.0        # attention scale; 0 -> head_dim ** -0.5
     rope_scale: float = 1.0         # linear RoPE scaling of the global layers (positions / rope_scale)
+    experts: int = 0                # experts per layer, each of intermediate size `inter` (0: one dense MLP)
+    experts_per_token: int = 0
+    norm_topk: bool = True          # the chosen experts' weights sum to one
 
     @property
     def qkv_rows(self) -> int:
@@ -68,14 +76,16 @@ class ModelConfig:
     def scale(self) -> float:
         return self.query_scale or self.head_dim ** -0.5
 
-    def params(self) -> int:
+    def params(self, active: bool = False) -> int:
+        """4-bit weights; `active`: those that one row's forward reads (its own experts only)."""
+        mlps = (self.experts_per_token if active else self.experts) if self.experts else 1
         per_layer = (self.hidden * self.qkv_rows + self.heads * self.head_dim * self.hidden
-                     + 3 * self.hidden * self.inter)
+                     + mlps * 3 * self.hidden * self.inter + self.experts * self.hidden)
         return self.layers * per_layer + self.vocab * self.hidden
 
     def weight_bytes(self) -> int:
-        """Bytes of 4-bit weights (0.5 B per weight + 4 B of scale and bias per 64) read by one forward pass."""
-        return self.params() * 9 // 16
+        """Bytes of 4-bit weights (0.5 B per weight + 4 B of scale and bias per 64) read by one row's forward pass."""
+        return self.params(active=True) * 9 // 16
 
     def kv_bytes_per_token(self) -> int:
         return self.layers * 2 * self.kv_heads * self.head_dim * 2
@@ -101,6 +111,9 @@ PRESETS = {
     "tiny-draft": ModelConfig("tiny-draft", 128, 2, 2, 1, 128, 256, 1000),
     "tiny-gemma": ModelConfig("tiny-gemma", 256, 3, 4, 2, 128, 512, 1000, family="gemma3", sliding_window=16,
                               global_every=3, query_scale=128 ** -0.5),
+    "tiny-moe": ModelConfig("tiny-moe", 256, 2, 4, 2, 128, 192, 1000, experts=8, experts_per_token=2),
+    "tiny-gemma-moe": ModelConfig("tiny-gemma-moe", 256, 3, 4, 2, 128, 128, 1000, family="gemma3", sliding_window=16,
+                                  global_every=3, query_scale=128 ** -0.5, experts=12, experts_per_token=3),
 }
 
 
@@ -125,14 +138,15 @@ class Linear4:
 class Layer:
     qkv: Linear4
     o: Linear4
-    gate_up: Linear4
-    down: Linear4
+    gate_up: Linear4 | kernels.Experts
+    down: Linear4 | kernels.Experts
     in_norm: torch.Tensor
     post_norm: torch.Tensor      # the norm before the MLP (Gemma-3: pre_feedforward_layernorm)
     q_norm: torch.Tensor
     k_norm: torch.Tensor
     post_attn_norm: torch.Tensor | None = None  # Gemma-3: on the attention output before its residual add
     post_ff_norm: torch.Tensor | None = None    # Gemma-3: on the MLP output before its residual add
+    router: Linear4 | None = None               # models with experts
 
 
 def interleave_gate_up(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
@@ -192,6 +206,10 @@ class QuantModel:
                  max_logit_rows: int = 32, keys_per_split: int | None = None, tp: int = 1, rank: int = 0, group=None,
                  weights: dict | None = None):
         self.cfg = cfg
+        if cfg.experts and (tp > 1 or weights is not None):
+            raise ValueError(f"{cfg.name}: a model with experts runs on one GPU, with random weights")
+        if cfg.experts and not 1 <= cfg.experts_per_token <= cfg.experts:
+            raise ValueError(f"{cfg.name}: {cfg.experts_per_token} of {cfg.experts} experts a token")
         if tp > 1 and (cfg.heads % tp or cfg.kv_heads % tp or cfg.inter % (64 * tp) or (cfg.inter // tp) % 16
                        or cfg.vocab % tp or (cfg.heads * cfg.head_dim // tp) % 64):
             raise ValueError(f"{cfg.name} does not split {tp} ways (heads, kv heads, 64-groups of K, vocabulary)")
@@ -224,6 +242,11 @@ class QuantModel:
         wq, s, b = kernels.quantize(w.contiguous())
         return Linear4(wq, s, b, kernels.Packed(wq, s, b))
 
+    def _stack(self, gen, n, k, sigma) -> tuple:
+        """A quantised [n, k] matrix for each expert: (w, scales, biases) with a leading axis of experts."""
+        e = self.cfg.experts
+        return tuple(t.view(e, n, -1) for t in kernels.quantize(self._rand(gen, e * n, k, sigma)))
+
     def _norm(self, gen, n) -> torch.Tensor:
         base = 0.0 if self.cfg.family == "gemma3" else 1.0
         return (base + 0.02 * torch.randn((n,), generator=gen, device=self.device)).to(torch.bfloat16)
@@ -249,16 +272,24 @@ class QuantModel:
             qkv = self._lin(qkv_full)
             o_full = self._rand(gen, c.hidden, c.heads * c.head_dim, sigma)
             o = self._lin(o_full[:, slice(*sh["o_cols"])] if tp > 1 else o_full)
-            gate, up = self._rand(gen, c.inter, c.hidden, sigma), self._rand(gen, c.inter, c.hidden, sigma)
-            if tp > 1:
-                gate, up = cut(gate, "inter"), cut(up, "inter")
-            gate_up = self._lin(interleave_gate_up(gate.contiguous(), up.contiguous()))
-            del gate, up, qkv_full, o_full
-            down_full = self._rand(gen, c.hidden, c.inter, sigma)
-            down = self._lin(down_full[:, slice(*sh["inter"])] if tp > 1 else down_full)
-            del down_full
+            router = None
+            if c.experts:
+                router = self._lin(self._rand(gen, c.experts, c.hidden, sigma))
+                gate_up = kernels.Experts.gate_up(self._stack(gen, c.inter, c.hidden, sigma),
+                                                  self._stack(gen, c.inter, c.hidden, sigma))
+                down = kernels.Experts(*self._stack(gen, c.hidden, c.inter, sigma))
+                del qkv_full, o_full
+            else:
+                gate, up = self._rand(gen, c.inter, c.hidden, sigma), self._rand(gen, c.inter, c.hidden, sigma)
+                if tp > 1:
+                    gate, up = cut(gate, "inter"), cut(up, "inter")
+                gate_up = self._lin(interleave_gate_up(gate.contiguous(), up.contiguous()))
+                del gate, up, qkv_full, o_full
+                down_full = self._rand(gen, c.hidden, c.inter, sigma)
+                down = self._lin(down_full[:, slice(*sh["inter"])] if tp > 1 else down_full)
+                del down_full
             layer = Layer(qkv, o, gate_up, down, self._norm(gen, c.hidden), self._norm(gen, c.hidden),
-                          self._norm(gen, c.head_dim), self._norm(gen, c.head_dim))
+                          self._norm(gen, c.head_dim), self._norm(gen, c.head_dim), router=router)
             if c.family == "gemma3":
                 layer.post_attn_norm, layer.post_ff_norm = self._norm(gen, c.hidden), self._norm(gen, c.hidden)
             self.layers.append(layer)
@@ -294,6 +325,8 @@ class QuantModel:
         self.qkv = torch.zeros((r, c.qkv_rows), dtype=bf, device=dev)
         self.attn = torch.zeros((r, c.heads * c.head_dim), dtype=bf, device=dev)  # [M, Hq, D] packed
         self.act = torch.zeros((r, c.inter), dtype=bf, device=dev)
+        if c.experts:
+            self.router_logits = torch.zeros((r, c.experts), dtype=bf, device=dev)
         self.y = torch.zeros((r, c.hidden), dtype=bf, device=dev)  # Gemma-3: projection output before its norm
         self.logits = torch.zeros((self.max_logit_rows, c.vocab), dtype=bf, device=dev)
         if self.tp > 1:  # this rank's vocabulary slice, and the all-gather target [tp][rows][V/tp]
@@ -312,15 +345,15 @@ class QuantModel:
         # the roped queries of forwards with more rows per sequence than the fused attention takes (prefill)
         self.q_wide = torch.zeros((r, c.heads * c.head_dim), dtype=bf, device=dev) if r > MAX_SEQ_ROWS else None
         # forwards of at most this many rows merge the attention's splits in the o-projection's prologue (not with
-        # tensor parallelism or Gemma-3's post-attention norm, whose o-projections have no residual epilogue)
+        # tensor parallelism, Gemma-3's post-attention norm or experts, whose o-projections have no residual epilogue)
         self.o_merge_rows = (kernels.qgemm_packed_attn_rows(c.hidden, c.heads * c.head_dim)
-                             if self.tp == 1 and c.family != "gemma3" else 0)
+                             if self.tp == 1 and c.family != "gemma3" and not c.experts else 0)
         self.ws_argmax = kernels.workspace(kernels.argmax_workspace_bytes(self.max_logit_rows, c.vocab), dev)
 
     def _gemm_shapes(self):
         c = self.lc
-        return [(c.qkv_rows, c.hidden), (c.hidden, c.heads * c.head_dim), (2 * c.inter, c.hidden),
-                (c.hidden, c.inter)]
+        mlp = [(c.experts, c.hidden)] if c.experts else [(2 * c.inter, c.hidden), (c.hidden, c.inter)]
+        return [(c.qkv_rows, c.hidden), (c.hidden, c.heads * c.head_dim), *mlp]
 
     # ---- forward ------------------------------------------------------------------------------------------
     def forward(self, meta: RowMeta, max_kv_len: int, logit_rows: int = 0,
@@ -387,6 +420,19 @@ class QuantModel:
                                           d=c.head_dim, max_kv_len=max_kv_len, keys_per_split=self.keys_per_split,
                                           out_sq=self.sq_attn, sq_ld=self.sq_ld, ws=ws)
             tr("attn", self.attn)
+            if c.experts:
+                kernels.qgemm_packed(self.attn, layer.o.p, out=self.y, rows=m, sq_ld=self.sq_ld, ws=ws)
+                _, x = kernels.block_residual(self.y[:m], h[:m], c.eps, post_norm=layer.post_attn_norm,
+                                              next_norm=layer.post_norm, gemma=gemma, out=h[:m])
+                tr("h_mid", h)
+                kernels.qgemm_packed(x, layer.router.p, out=self.router_logits, rows=m, sq_ld=self.sq_ld, ws=ws)
+                routing = kernels.moe_route(self.router_logits, c.experts_per_token, normalise=c.norm_topk, rows=m)
+                places = kernels.moe_mlp(x, layer.gate_up, layer.down, routing,
+                                         activation="geglu" if gemma else "swiglu")
+                kernels.block_residual(places, h[:m], c.eps, weights=routing.weights, post_norm=layer.post_ff_norm,
+                                       gemma=gemma, out=h[:m], out_sq=self.sq_mlp[0])
+                sq, parts = self.sq_mlp, 1
+                continue
             if self.tp > 1:  # partial sums of the row-sharded o and down, all-reduced before the residual add
                 kernels.qgemm_packed(self.attn, layer.o.p, out=self.y, rows=m, sq_ld=self.sq_ld, ws=ws)
                 self._all_reduce(self.y[:m])
