@@ -557,22 +557,21 @@ class Routing:
 
     @property
     def ids(self) -> torch.Tensor:
-        return self.buf[:self.rows * self.top_k].view(self.rows, self.top_k)
+        return torch.as_strided(self.buf, (self.rows, self.top_k), (self.top_k, 1), 0)
 
     @property
     def weights(self) -> torch.Tensor:
-        n = self.rows * self.top_k
-        return self.buf[n:2 * n].view(torch.float32).view(self.rows, self.top_k)
+        return torch.as_strided(self.buf.view(torch.float32), (self.rows, self.top_k), (self.top_k, 1),
+                                self.rows * self.top_k)
 
     @property
     def pairs(self) -> torch.Tensor:
         n = self.rows * self.top_k
-        return self.buf[2 * n:3 * n]
+        return torch.as_strided(self.buf, (n,), (1,), 2 * n)
 
     @property
     def offsets(self) -> torch.Tensor:
-        n = 3 * self.rows * self.top_k
-        return self.buf[n:n + self.experts + 2]
+        return torch.as_strided(self.buf, (self.experts + 2,), (1,), 3 * self.rows * self.top_k)
 
     @property
     def _pairs_ptr(self) -> int:
@@ -639,17 +638,16 @@ def _moe_rows(x: torch.Tensor, experts: Experts, routing: Routing) -> bool:
     if experts.e != routing.experts:
         raise ValueError(f"{experts.e} experts, the routing is over {routing.experts}")
     by_pair = x.dim() == 3
-    lead = (routing.rows, routing.top_k) if by_pair else (routing.rows,)
-    if tuple(x.shape[:-1]) != lead:
+    if x.shape[:-1] != ((routing.rows, routing.top_k) if by_pair else (routing.rows,)):
         raise ValueError(f"x {tuple(x.shape)} does not match a routing of {routing.rows} rows, {routing.top_k} places")
     return by_pair
 
 
-def _moe_out(out: torch.Tensor | None, shape: tuple, device: torch.device) -> torch.Tensor:
+def _moe_out(out: torch.Tensor | None, shape: tuple, like: torch.Tensor) -> torch.Tensor:
     if out is None:
-        return torch.empty(shape, dtype=torch.bfloat16, device=device)
-    _check(out, "out", (torch.bfloat16,), device)
-    if tuple(out.shape) != shape:
+        return like.new_empty(shape)
+    _check(out, "out", (torch.bfloat16,), like.device)
+    if out.shape != shape:
         raise ValueError(f"out must be {shape}, got {tuple(out.shape)}")
     return out
 
@@ -659,7 +657,7 @@ def grouped_qgemm(x: torch.Tensor, experts: Experts, routing: Routing, *,
     """y[m, j] = W[ids[m, j]] x[m] for x [M, K], or W[ids[m, j]] x[m, j] for x [M, k, K]; bf16 [M, k, N], zero for
     places without an expert."""
     by_pair = _moe_rows(x, experts, routing)
-    out = _moe_out(out, (routing.rows, routing.top_k, experts.n), x.device)
+    out = _moe_out(out, (routing.rows, routing.top_k, experts.n), x)
     need = _grouped_workspace(routing.rows, experts.e, routing.top_k, experts.k)
     ws = torch.empty(need, dtype=torch.uint8, device=x.device)
     _lib.call("im_moe_grouped_qgemm", experts.data.data_ptr(), x.data_ptr(), out.data_ptr(), routing.rows, experts.e,
@@ -679,13 +677,19 @@ def moe_mlp(x: torch.Tensor, gate_up: Experts, down: Experts, routing: Routing, 
     h, inter = gate_up.k, gate_up.n // 2
     if (down.e, down.n, down.k) != (gate_up.e, h, inter) or down.data.device != x.device:
         raise ValueError(f"down is {down.e} x [{down.n}, {down.k}], expected {gate_up.e} x [{h}, {inter}]")
-    out = _moe_out(out, (routing.rows, routing.top_k, h), x.device)
+    out = _moe_out(out, (routing.rows, routing.top_k, h), x)
     need = _mlp_workspace(routing.rows, gate_up.e, routing.top_k, h, inter)
     ws = torch.empty(need, dtype=torch.uint8, device=x.device)
     _lib.call("im_moe_mlp", gate_up.data.data_ptr(), down.data.data_ptr(), x.data_ptr(), out.data_ptr(), routing.rows,
               gate_up.e, routing.top_k, h, inter, _EPILOGUES[activation], routing._pairs_ptr, routing._plan_ptr,
               routing.plan_bytes, ws.data_ptr(), need, _stream(x.device))
     return out
+
+
+def _check_vector(t: torch.Tensor, name: str, n: int, device: torch.device) -> None:
+    _check(t, name, (torch.bfloat16,), device)
+    if t.shape != (n,):
+        raise ValueError(f"{name} must be [{n}], got {tuple(t.shape)}")
 
 
 def block_residual(y: torch.Tensor, h: torch.Tensor, eps: float, *, weights: torch.Tensor | None = None,
@@ -704,18 +708,17 @@ def block_residual(y: torch.Tensor, h: torch.Tensor, eps: float, *, weights: tor
     m, hsz = h.shape
     if weights is None:
         places = 1
-        if tuple(y.shape) not in ((m, hsz), (m, 1, hsz)):
+        if y.shape != (m, hsz) and y.shape != (m, 1, hsz):
             raise ValueError(f"y must be [{m}, {hsz}] without weights, got {tuple(y.shape)}")
     else:
         _check(weights, "weights", (torch.float32,), device)
         places = weights.shape[-1]
-        if tuple(weights.shape) != (m, places) or tuple(y.shape) != (m, places, hsz):
+        if weights.shape != (m, places) or y.shape != (m, places, hsz):
             raise ValueError(f"weights {tuple(weights.shape)} and y {tuple(y.shape)} do not match h {tuple(h.shape)}")
-    for name, t in (("post_norm", post_norm), ("next_norm", next_norm)):
-        if t is not None:
-            _check(t, name, (torch.bfloat16,), device)
-            if t.shape != (hsz,):
-                raise ValueError(f"{name} must be [{hsz}], got {tuple(t.shape)}")
+    if post_norm is not None:
+        _check_vector(post_norm, "post_norm", hsz, device)
+    if next_norm is not None:
+        _check_vector(next_norm, "next_norm", hsz, device)
     row = col = 0
     if gate is not None:
         _check(gate, "gate", (torch.bfloat16,), device)
@@ -727,8 +730,8 @@ def block_residual(y: torch.Tensor, h: torch.Tensor, eps: float, *, weights: tor
         _check(out_sq, "out_sq", (torch.float32,), device)
         if out_sq.numel() < m:
             raise ValueError(f"out_sq needs {m} elements")
-    out = _moe_out(out, (m, hsz), device)
-    z = torch.empty((m, hsz), dtype=torch.bfloat16, device=device) if next_norm is not None else None
+    out = _moe_out(out, (m, hsz), h)
+    z = h.new_empty((m, hsz)) if next_norm is not None else None
     _lib.call("im_block_residual", y.data_ptr(), _ptr_or_none(weights), places, h.data_ptr(), _ptr_or_none(post_norm),
               _ptr_or_none(gate), row, col, float(residual_scale), _ptr_or_none(next_norm), float(eps), int(gemma), m, hsz,
               out.data_ptr(), _ptr_or_none(z), _ptr_or_none(out_sq), _stream(device))
