@@ -265,13 +265,8 @@ __device__ __forceinline__ void mr_place(const RouteArgs& a, RouteSmem& s) {
 constexpr int MR_FEW = 128;
 __device__ __forceinline__ void mr_place_few(const RouteArgs& a, RouteSmem& s) {
   const int n = a.M * a.top_k, p = threadIdx.x;
-  int* bucket = s.cnt[0];  // [MR_FEW], then the size of the bucket that begins with pair q (0: it does not begin one)
-  int* size = s.cnt[0] + MR_FEW;
-  if (p < n) {
-    const int id = a.ids[p];
-    bucket[p] = id < 0 ? a.E : id;
-  }
-  __syncthreads();
+  const int* bucket = s.cnt[0];   // [MR_FEW], every pair's
+  int* size = s.cnt[0] + MR_FEW;  // of the bucket that begins with pair q (0: it does not begin one)
   int less = 0, same = 0, before = 0, b = 0;
   if (p < n) {
     b = bucket[p];
@@ -314,21 +309,30 @@ template <int EL, bool ONE>
 __global__ void __launch_bounds__(MR_THREADS) moe_select_kernel(RouteArgs a) {
   __shared__ RouteSmem s;
   const int nb = a.E + 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int e = threadIdx.x; e < nb; e += MR_THREADS) {
-    s.total[e] = 0;
-    s.base[e] = 0;
+  const bool few = ONE && a.M * a.top_k <= MR_FEW;
+  if (!few) {
+    for (int e = threadIdx.x; e < nb; e += MR_THREADS) {
+      s.total[e] = 0;
+      s.base[e] = 0;
+    }
+    __syncthreads();
   }
   pdl_wait();
   pdl_trigger();
-  __syncthreads();
   const int r0 = blockIdx.x * a.rows_per_block, r1 = min(a.M, r0 + a.rows_per_block);
   for (int row = r0 + warp; row < r1; row += MR_WARPS) {
     const int id = mr_row<EL>(a, row, lane);
-    if (lane < a.top_k) atomicAdd(&s.total[id < 0 ? a.E : id], 1);
+    if (lane < a.top_k) {
+      const int bucket = id < 0 ? a.E : id;
+      if (few)
+        s.cnt[0][row * a.top_k + lane] = bucket;
+      else
+        atomicAdd(&s.total[bucket], 1);
+    }
   }
   __syncthreads();
   if constexpr (ONE) {
-    if (a.M * a.top_k <= MR_FEW)
+    if (few)
       mr_place_few(a, s);
     else
       mr_place(a, s);
@@ -342,21 +346,30 @@ __global__ void __launch_bounds__(MR_THREADS) moe_place_kernel(RouteArgs a) {
   const int nb = a.E + 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
   pdl_trigger();
-  // a warp per bucket: the blocks' counts, all and the earlier blocks'
-  for (int e = warp; e < nb; e += MR_WARPS) {
-    int all = 0, earlier = 0;
+  // a warp per bucket, four at a time: the blocks' counts, all and the earlier blocks', every load in flight at once
+  for (int e0 = warp; e0 < nb; e0 += 4 * MR_WARPS) {
+    int c[4][(MOE_ROUTE_BLOCKS + 31) / 32];
 #pragma unroll
-    for (int i = 0; i < (MOE_ROUTE_BLOCKS + 31) / 32; i++) {
-      const int b = i * 32 + lane;
-      const int c = b < a.blocks ? a.counts[(size_t)e * a.blocks + b] : 0;
-      all += c;
-      earlier += b < (int)blockIdx.x ? c : 0;
-    }
-    all = __reduce_add_sync(0xffffffffu, all);
-    earlier = __reduce_add_sync(0xffffffffu, earlier);
-    if (lane == 0) {
-      s.total[e] = all;
-      s.base[e] = earlier;
+    for (int u = 0; u < 4; u++)
+#pragma unroll
+      for (int i = 0; i < (MOE_ROUTE_BLOCKS + 31) / 32; i++) {
+        const int e = e0 + u * MR_WARPS, b = i * 32 + lane;
+        c[u][i] = e < nb && b < a.blocks ? a.counts[(size_t)e * a.blocks + b] : 0;
+      }
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      int all = 0, earlier = 0;
+#pragma unroll
+      for (int i = 0; i < (MOE_ROUTE_BLOCKS + 31) / 32; i++) {
+        all += c[u][i];
+        earlier += i * 32 + lane < (int)blockIdx.x ? c[u][i] : 0;
+      }
+      all = __reduce_add_sync(0xffffffffu, all);
+      earlier = __reduce_add_sync(0xffffffffu, earlier);
+      if (lane == 0 && e0 + u * MR_WARPS < nb) {
+        s.total[e0 + u * MR_WARPS] = all;
+        s.base[e0 + u * MR_WARPS] = earlier;
+      }
     }
   }
   __syncthreads();
