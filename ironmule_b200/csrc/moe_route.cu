@@ -10,7 +10,8 @@
 // Weights are float32 and unbiased by `bias`.
 //
 // One warp per row: lane l holds experts l, l + 32, ...; each of the k rounds takes the warp's largest 32-bit sortable
-// key with one reduction and the lowest expert holding it with a second. Up to 64 rows one block does all of it in one
+// key with one reduction and the lowest expert holding it with a second (bf16 logits without a bias: key and expert in
+// one word, one reduction; 8192 rows of 128 experts 18.6 us against 20.6). Up to 64 rows one block does all of it in one
 // launch. More rows are cut over up to 296 blocks: the first launch selects and counts, the second sums the blocks'
 // counts (every block for itself), scans them and places its pairs. The order is stable: within an expert, pairs ascend.
 // Bytes are few (a row's logits once, 12 bytes a place); what bounds it is launch and barrier latency.
@@ -66,7 +67,8 @@ __device__ __forceinline__ float mr_warp_max(float v) {
 }
 
 // The chosen experts of one row: lane j < top_k returns place j's expert (-1: none) and writes its weight.
-template <int EL>
+// PACK (bf16 logits without a bias): key and expert share one word, so that a round is one reduction.
+template <int EL, bool PACK>
 __device__ __forceinline__ int mr_row(const RouteArgs& a, int row, int lane) {
   float v[EL];
   unsigned key[EL];
@@ -80,16 +82,31 @@ __device__ __forceinline__ int mr_row(const RouteArgs& a, int row, int lane) {
       const size_t at = (size_t)row * a.ld + e;
       const float l = a.f32 ? reinterpret_cast<const float*>(a.logits)[at]
                             : bf(reinterpret_cast<const uint16_t*>(a.logits)[at]);
-      const float k = a.bias ? l + a.bias[e] : l;
+      const float k = !PACK && a.bias ? l + a.bias[e] : l;
       if (l > neg && k > neg) {  // false for NaN too
         v[i] = l;
-        key[i] = mr_key(k);
+        key[i] = PACK ? (mr_key(k) & 0xffff0000u) | (0xffffu - e) : mr_key(k);
       }
     }
   }
   int mine = -1;
   float value = neg;
-  for (int j = 0; j < a.top_k; j++) {
+  for (int j = 0; PACK && j < a.top_k; j++) {
+    unsigned best = key[0];
+#pragma unroll
+    for (int i = 1; i < EL; i++) best = max(best, key[i]);
+    const unsigned top = __reduce_max_sync(0xffffffffu, best);
+    if (top == 0u) break;  // no open expert is left (the same in every lane)
+#pragma unroll
+    for (int i = 0; i < EL; i++)
+      if (key[i] == top) key[i] = 0u;
+    if (lane == j) {
+      mine = (int)(0xffffu - (top & 0xffffu));
+      const unsigned hi = top >> 16;
+      value = bf((uint16_t)(hi & 0x8000u ? hi ^ 0x8000u : ~hi));
+    }
+  }
+  for (int j = 0; !PACK && j < a.top_k; j++) {
     unsigned best = 0u;
     int at = 0;
     float bv = neg;
@@ -305,7 +322,7 @@ __device__ __forceinline__ void mr_place_few(const RouteArgs& a, RouteSmem& s) {
 }
 
 // Selection and counting; with ONE the block holds every row and places the pairs too.
-template <int EL, bool ONE>
+template <int EL, bool PACK, bool ONE>
 __global__ void __launch_bounds__(MR_THREADS) moe_select_kernel(RouteArgs a) {
   __shared__ RouteSmem s;
   const int nb = a.E + 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -321,7 +338,7 @@ __global__ void __launch_bounds__(MR_THREADS) moe_select_kernel(RouteArgs a) {
   pdl_trigger();
   const int r0 = blockIdx.x * a.rows_per_block, r1 = min(a.M, r0 + a.rows_per_block);
   for (int row = r0 + warp; row < r1; row += MR_WARPS) {
-    const int id = mr_row<EL>(a, row, lane);
+    const int id = mr_row<EL, PACK>(a, row, lane);
     if (lane < a.top_k) {
       const int bucket = id < 0 ? a.E : id;
       if (few)
@@ -376,13 +393,19 @@ __global__ void __launch_bounds__(MR_THREADS) moe_place_kernel(RouteArgs a) {
   mr_place(a, s);
 }
 
-template <int EL>
-static int mr_launch(const RouteArgs& a, cudaStream_t st) {
+template <int EL, bool PACK>
+static int mr_launch_as(const RouteArgs& a, cudaStream_t st) {
   if (a.blocks <= 1)
-    return launch("moe_select_kernel", moe_select_kernel<EL, true>, dim3(1), dim3(MR_THREADS), 0, st, a);
-  const int rc = launch("moe_select_kernel", moe_select_kernel<EL, false>, dim3(a.blocks), dim3(MR_THREADS), 0, st, a);
+    return launch("moe_select_kernel", moe_select_kernel<EL, PACK, true>, dim3(1), dim3(MR_THREADS), 0, st, a);
+  const int rc =
+      launch("moe_select_kernel", moe_select_kernel<EL, PACK, false>, dim3(a.blocks), dim3(MR_THREADS), 0, st, a);
   if (rc) return rc;
   return launch("moe_place_kernel", moe_place_kernel, dim3(a.blocks), dim3(MR_THREADS), 0, st, a);
+}
+
+template <int EL>
+static int mr_launch(const RouteArgs& a, cudaStream_t st) {
+  return !a.f32 && !a.bias ? mr_launch_as<EL, true>(a, st) : mr_launch_as<EL, false>(a, st);
 }
 
 }  // namespace im
