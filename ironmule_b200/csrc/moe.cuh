@@ -19,10 +19,9 @@ constexpr int MOE_PLAN_HEADER = 8;      // ints: [0] work items, [1] error word 
 // Packed weights of an expert: 128-output blocks (rows past N are zero), each a run of 64-wide groups of
 // MOE_BLOCK_BYTES = 4 tiles of 32 rows x (two 16-byte halves a row, [half][row]) of codes, then per tile 128 bytes of
 // scales and biases: for g = 0..7 the bf16 scales of rows g, g + 8, g + 16, g + 24, then their biases. One copy brings
-// a block's group; a thread reads its row's codes in two 16-byte loads without bank conflicts, and a warp-MMA lane the
-// 8 bytes of each of its four rows. After the E experts: float32 [E][padded rows], the
-// largest |scale * q + bias| that a row's scales and biases allow; float32 [E][2], the largest over an expert's rows
-// with r & 16 == 0 (the gate rows of a gated product) and over the others (the up rows).
+// a block's group; a thread reads its row's codes in two 16-byte loads without bank conflicts. After the E experts:
+// float32 [E][padded rows], the largest |scale * q + bias| that a row's scales and biases allow; float32 [E][2], the
+// largest over an expert's rows with r & 16 == 0 (the gate rows of a gated product) and over the others (the up rows).
 constexpr int MOE_BLOCK_BYTES = 4608;
 
 // One work item: `rows` consecutive entries of the sorted pair list, all of one expert (or, with expert == E, of the

@@ -23,9 +23,12 @@ _EPILOGUES = {"store": _lib.EPI_STORE, "residual": _lib.EPI_RESIDUAL, "swiglu": 
 _VARIANTS = {"auto": _lib.QGEMM_AUTO, "mma": _lib.QGEMM_MMA, "fma": _lib.QGEMM_FMA}
 
 
-def _stream(device: torch.device) -> int:
-    """The handle of torch's current stream on the device (without building a Stream object for it)."""
-    return torch._C._cuda_getCurrentRawStream(device.index)
+def _stream(device) -> int:
+    """The handle of torch's current stream on the device (without building a Stream object where its index is known)."""
+    index = getattr(device, "index", None)
+    if not isinstance(index, int):  # "cuda", "cuda:0", torch.device("cuda")
+        return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _check(t: torch.Tensor, name: str, dtypes: tuple, device: torch.device | None = None) -> None:
