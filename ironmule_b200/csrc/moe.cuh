@@ -24,12 +24,9 @@ constexpr int MOE_PLAN_HEADER = 8;      // ints: [0] work items, [1] error word 
 // largest over an expert's rows with r & 16 == 0 (the gate rows of a gated product) and over the others (the up rows).
 constexpr int MOE_BLOCK_BYTES = 4608;
 
-// One work item: `rows` consecutive entries of the sorted pair list, all of one expert (or, with expert == E, of the
-// places that chose no expert, whose outputs are zero).
-struct MoeItem {
-  int expert, first, rows, padded;  // padded: the rows before it when every item is rounded up to 16
-};
-
+// One work item (four ints): the expert, the first of its entries in the sorted pair list, their number, and the rows
+// before it when every item is rounded up to 16. Items of expert E are places that chose none; their outputs are zero.
+//
 // Plan layout in ints: header | items | where each pair's row lies | per-block expert counts (the routing's own scratch).
 // where[pair] = {the item's padded first row (-1: no expert), its row r in the item | the item's rows rounded up to 16
 // << 16}.

@@ -307,8 +307,9 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   constexpr uint32_t tmem = 0;  // the whole tensor memory: its allocation can only start at column 0
   // The routing's plan was finished before the launch that precedes this one (the prep kernel, or the first product)
-  // let this one begin: the plan and the weights are read without waiting, rows and outputs only after pdl_wait().
-  const int ntiles = a.p.plan[0] * a.cols;
+  // let this one begin: the plan and the weights are read without waiting (from L2, whatever an SM's L1 may hold of
+  // them), rows and outputs only after pdl_wait().
+  const int ntiles = __ldcg(a.p.plan) * a.cols;
   MtTile* const info = reinterpret_cast<MtTile*>(sbase + MT_OFF_TILE);
   uint32_t islot = 0, iphase = 0;  // this warp's place in the ring of tiles
   auto tile_wait = [&] { return qt_wait_short(bars + 8 * (MT_I_FULL + islot), iphase, abort_flag, a.error); };
@@ -489,16 +490,16 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
     if (warp == MT_W_LOAD + 1) {
       // ---- the tiles, ahead of the other warps -----------------------------------------------------------------------
       const int step = gridDim.x;
-      int4 item = (int)blockIdx.x < ntiles ? a.items[blockIdx.x / a.cols] : make_int4(0, 0, 0, 0);
+      int4 item = (int)blockIdx.x < ntiles ? __ldcg(a.items + blockIdx.x / a.cols) : make_int4(0, 0, 0, 0);
       bool waited = false;
       for (int tile = blockIdx.x; tile < ntiles; tile += step) {
-        const int4 next = tile + step < ntiles ? a.items[(tile + step) / a.cols] : item;
+        const int4 next = tile + step < ntiles ? __ldcg(a.items + (tile + step) / a.cols) : item;
         const bool closed = item.x == a.p.E;
         float top[4] = {};
         if (!closed) {
           const float* rm = a.row_max + ((size_t)item.x * a.cols + tile % a.cols) * 128 + lane;
 #pragma unroll
-          for (int i = 0; i < 4; i++) top[i] = rm[32 * i];
+          for (int i = 0; i < 4; i++) top[i] = __ldcg(rm + 32 * i);
         }
         if (!qt_wait_short(bars + 8 * (MT_I_EMPTY + islot), iphase ^ 1u, abort_flag, a.error)) break;
         MtTile& out = info[islot];
@@ -594,7 +595,7 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
         if (g + 1 < G)
           mt_group(codes + at + MOE_BLOCK_BYTES, affine + at + MOE_BLOCK_BYTES, inv, q, MT_A0 + 64 * set + 32,
                    [] { return true; });
-        if (*abort_flag) goto expand_done;
+        if (__any_sync(0xffffffffu, *abort_flag)) goto expand_done;
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncwarp();

@@ -68,26 +68,26 @@ __device__ __forceinline__ bool qt_try_wait_64(uint32_t bar, uint32_t parity) {
   return done != 0;
 }
 
-// The rest of a long wait: false when it gave up (now or earlier).
-static __device__ __noinline__ bool qt_wait_long(uint32_t bar, uint32_t parity, volatile int* abort_flag,
-                                                 unsigned* error) {
-  const unsigned long long t0 = qt_clock();
-  while (true) {
-    if (qt_try_wait(bar, parity)) return true;
-    if (*abort_flag) return false;
-    if (qt_clock() - t0 > QT_WAIT_NS) {
-      *abort_flag = 1;
-      atomicExch(error, 1u);
-      return false;
-    }
-  }
-}
-
-// Bounded wait for pipelines whose stages last a few hundred cycles: few instructions while it is short, the abort flag
-// and the timer (whose reads cost more than such a wait) only once it is long.
+// Bounded wait of a whole warp, for pipelines whose stages last a few hundred cycles: few instructions while it is
+// short, the abort flag and the timer (whose reads cost more than such a wait) only once it is long. It ends in a vote:
+// the warp leaves it converged (tcgen05's .aligned instructions follow, and lanes may see a phase complete at different
+// attempts) and of one mind (a lane that gave up takes the others along).
 __device__ __forceinline__ bool qt_wait_short(uint32_t bar, uint32_t parity, volatile int* abort_flag,
                                               unsigned* error) {
-  return qt_try_wait_64(bar, parity) || qt_wait_long(bar, parity, abort_flag, error);
+  bool ok = qt_try_wait_64(bar, parity);
+  if (!ok) {
+    const unsigned long long t0 = qt_clock();
+    while (true) {
+      ok = qt_try_wait(bar, parity);
+      if (ok || *abort_flag) break;
+      if (qt_clock() - t0 > QT_WAIT_NS) {
+        *abort_flag = 1;
+        atomicExch(error, 1u);
+        break;
+      }
+    }
+  }
+  return __all_sync(0xffffffffu, ok);
 }
 
 // One lane of a converged warp (the same one every time).
