@@ -366,7 +366,7 @@ int im_philox4x32_10(uint64_t seed, uint64_t offset, uint32_t stream_id, uint32_
  * with the largest keys float32(logit) + bias[e] (bias float32 [E] or NULL; -0 counts as +0, ties to the lower expert),
  * in that order: ids [M, top_k] and weights [M, top_k]. A logit of -inf or NaN closes the expert to the row; places
  * beyond the open experts get id -1 and weight 0. Weights come from the unbiased logits, times `scale`:
- *   IM_MOE_SOFTMAX: exp(v - max) / sum, over the chosen experts (normalise) or over all open ones;
+ *   IM_MOE_SOFTMAX: exp(v - max) / sum, both over the chosen experts (normalise) or over all open ones;
  *   IM_MOE_SIGMOID: 1 / (1 + exp(-v)), divided by the chosen experts' sum (normalise) or as it is.
  * pairs [M * top_k] holds the pairs sorted by expert (ascending within one; places without an expert last),
  * offsets [E + 2] where each expert's begin (offsets[E]: the places without one, offsets[E + 1] = M * top_k). `plan`

@@ -136,9 +136,14 @@ __device__ __forceinline__ int mr_row(const RouteArgs& a, int row, int lane) {
   const bool live = mine >= 0;
   float w = 0.f;
   if (a.scoring == IM_MOE_SOFTMAX) {
+    // relative to the largest of the terms that are summed: a bias can choose experts far below the row's largest
     float top = neg;
+    if (a.normalise) {
+      top = value;
+    } else {
 #pragma unroll
-    for (int i = 0; i < EL; i++) top = fmaxf(top, v[i]);
+      for (int i = 0; i < EL; i++) top = fmaxf(top, v[i]);
+    }
     top = mr_warp_max(top);
     const float p = live ? (value == top ? 1.f : expf(value - top)) : 0.f;  // (inf - inf counts as 0)
     float total = p;
