@@ -137,7 +137,7 @@ int im_qgemm_packed_path(int path);
  * cluster), 0 = through the workspace and a global arrival counter. Process-wide; both give the same bits. */
 int im_qgemm_packed_cluster(int on);
 /* The error word of a workspace last used by a call of more than 32 rows (the tensor-core kernel): 0 when
- * every bounded wait of that kernel completed, 1 when one ran out. Synchronous (reads device memory). */
+ * every bounded wait of that kernel completed, 1 when one ran out. Waits for every stream of the current device. */
 int im_qgemm_packed_status(const void* workspace);
 int im_qgemm_packed(const void* packed, const uint16_t* x, uint16_t* y, const uint16_t* residual, int64_t M, int64_t N,
                     int64_t K, int epilogue, const float* norm_sq, int64_t norm_parts, const uint16_t* norm_weight,
@@ -386,7 +386,7 @@ int im_philox4x32_10(uint64_t seed, uint64_t offset, uint32_t stream_id, uint32_
  *
  * The products run on tcgen05 with operands in fp16 scaled by powers of two and float32 sums; a pair's result does not
  * depend on the other rows, whatever the batch. im_moe_status: the plan's error word (0: every bounded wait of the
- * products completed); synchronises.
+ * products completed); waits for every stream of the current device.
  *
  * im_block_residual: joins the places of a block, and the block to the residual stream, and takes the next norm:
  *   b = sum_j weights[m, j] y[m, j] (places of weight 0 are left out; weights NULL: the one place as it is)

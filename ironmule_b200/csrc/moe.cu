@@ -101,7 +101,9 @@ extern "C" int im_moe_status(const void* plan) {
   clear_error();
   IM_REQUIRE(plan, IM_INVALID, "im_moe_status: null plan");
   int word = 0;
-  const cudaError_t e = cudaMemcpy(&word, reinterpret_cast<const int*>(plan) + 1, 4, cudaMemcpyDeviceToHost);
+  // the products may run on a stream that the copy's own (the default) stream does not wait for
+  cudaError_t e = cudaDeviceSynchronize();
+  if (e == cudaSuccess) e = cudaMemcpy(&word, reinterpret_cast<const int*>(plan) + 1, 4, cudaMemcpyDeviceToHost);
   if (e != cudaSuccess) {
     set_error("im_moe_status: %s", cudaGetErrorString(e));
     return IM_CUDA_ERROR;

@@ -778,8 +778,10 @@ extern "C" int im_qgemm_packed_status(const void* workspace) {
   clear_error();
   IM_REQUIRE(workspace, IM_INVALID, "im_qgemm_packed_status: null workspace");
   unsigned word = 0;
-  const cudaError_t e = cudaMemcpy(&word, reinterpret_cast<const char*>(workspace) + Q4_COUNTER_BYTES - 4, 4,
-                                   cudaMemcpyDeviceToHost);
+  // the product may run on a stream that the copy's own (the default) stream does not wait for
+  cudaError_t e = cudaDeviceSynchronize();
+  if (e == cudaSuccess)
+    e = cudaMemcpy(&word, reinterpret_cast<const char*>(workspace) + Q4_COUNTER_BYTES - 4, 4, cudaMemcpyDeviceToHost);
   if (e != cudaSuccess) {
     set_error("im_qgemm_packed_status: %s", cudaGetErrorString(e));
     return IM_CUDA_ERROR;

@@ -438,9 +438,11 @@ def qgemm_packed_workspace_bytes(m: int, n: int, k: int) -> int:
 
 
 def qgemm_packed_status(ws: torch.Tensor) -> int:
-    """The error word of a workspace last used by a call of more than 32 rows (0: every wait completed)."""
+    """The error word of a workspace last used by a call of more than 32 rows (0: every wait completed); waits for the
+    device."""
     ptr, _ = _ws(ws, 1 << 16)
-    return int(_lib.load().im_qgemm_packed_status(ptr))
+    with torch.cuda.device(ws.device):
+        return int(_lib.load().im_qgemm_packed_status(ptr))
 
 
 def qgemm_packed_path(path: int) -> None:
@@ -585,8 +587,10 @@ class Routing:
         return self.buf.data_ptr() + 4 * self._plan_at
 
     def status(self) -> int:
-        """The error word of the products that used this routing (0: every bounded wait completed); synchronises."""
-        return int(_lib.load().im_moe_status(self._plan_ptr))
+        """The error word of the products that used this routing (0: every bounded wait completed); waits for the
+        device, so for products on any stream."""
+        with torch.cuda.device(self.buf.device):
+            return int(_lib.load().im_moe_status(self._plan_ptr))
 
 
 @functools.lru_cache(maxsize=4096)

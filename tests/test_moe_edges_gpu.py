@@ -37,3 +37,20 @@ def test_softmax_with_a_bias_that_passes_over_the_largest_logits(cuda, rows):
     one = kernels.moe_route(torch.tensor([[0.0, -200.0, -300.0]], device=cuda), 1,
                             bias=torch.tensor([-10000.0, 0.0, 0.0], device=cuda))
     assert one.ids.tolist() == [[1]] and one.weights.tolist() == [[1.0]]
+
+
+# ---- status ---------------------------------------------------------------------------------------------------
+def test_status_waits_for_the_products_stream(cuda):
+    """On a stream of torch's pool, which the legacy default stream does not wait for: the error words are read after
+    the work that is queued there (here a write of the word behind a delay)."""
+    r = kernels.moe_route(torch.randn((4, 8), device=cuda), 2)
+    ws = kernels.workspace(1 << 20, cuda)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream(cuda)
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100_000_000)  # tens of milliseconds
+        r.buf[r._plan_at + 1] = 1
+        assert r.status() == 1
+        torch.cuda._sleep(100_000_000)
+        ws.fill_(1)
+        assert kernels.qgemm_packed_status(ws) == 0x01010101
