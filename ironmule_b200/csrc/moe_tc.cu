@@ -10,8 +10,9 @@
 //    (2^20) makes the weight. What this range costs is below 2^-18 of the row's largest weight;
 //  * a row of x by its largest finite element, which lands in [2^9, 2^10) (moe_prep_kernel; bf16 values fit fp16);
 //  * the gated activations h = act(g) u by a bound on the row: |g| <= |x|_2 sqrt(K) max |G|, |u| likewise, so
-//    |h| <= |x|_2^2 K max|G| max|U|, which lands below 2^15. No row can overflow, and typical rows stay well above
-//    fp16's subnormals (the bound is loose by K or so, of 2^29).
+//    |h| <= |x|_2^2 K max|G| max|U|, which lands below 2^15. No finite row can overflow, and typical rows stay well
+//    above fp16's subnormals (the bound is loose by K or so, of 2^29). Where G or U is zero throughout, so is h, and u
+//    and g are left as they are.
 // The factors return in float32 after the sum. A row with infinities or NaN gives those.
 //
 // A persistent grid (one CTA per SM) walks tiles; its warps are coupled by mbarriers only:
@@ -106,6 +107,15 @@ __device__ __forceinline__ int mt_exp(float max, int bits) {
   frexpf(max, &e);
   e -= bits;
   return e < -120 ? -120 : (e > 120 ? 120 : e);
+}
+
+// The exponent that gated activations are divided by, from the logarithms of the bounds on |g| and |u| and the row's own
+// factor: their product lands below 2^15, and neither u nor the factor that u takes on overflows on the way (g may be
+// tiny where u is large). 0 where g or u is zero throughout.
+__device__ __forceinline__ int mt_hidden_exp(float g, float u, float factor) {
+  if (!(g > -INFINITY) || !(u > -INFINITY)) return 0;
+  const int least = max(max((int)ceilf(u), ilogbf(factor)) - 120, -110);
+  return min(max((int)ceilf(g + u) - 15, least), 120);
 }
 
 // Position of element k (0..7) of 8 in the operands' order.
@@ -517,17 +527,19 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
           waited = true;
         }
         if (!closed) {
-          float lg = 0.f;
-          if constexpr (GLU)
-            lg = log2f((float)a.p.K) + log2f(a.half_max[2 * item.x]) + log2f(a.half_max[2 * item.x + 1]);
+          float lg = 0.f, lu = 0.f;  // what bounds g and u of a row of |x|_2 = 1
+          if constexpr (GLU) {
+            const float root = 0.5f * log2f((float)a.p.K);
+            lg = root + log2f(a.half_max[2 * item.x]);
+            lu = root + log2f(a.half_max[2 * item.x + 1]);
+          }
 #pragma unroll
           for (int i = 0; i < 4; i++) {
             const int c = 32 * i + lane, row = item.w + c;
             if (c < item.z) {
               float2 m = make_float2(a.scale[row], 0.f);
               if constexpr (GLU) {
-                const float bound = 2.f * a.xlog[row] + lg;
-                const int e = bound > -100.f ? (int)ceilf(fminf(bound, 135.f)) - 15 : -110;
+                const int e = mt_hidden_exp(a.xlog[row] + lg, a.xlog[row] + lu, m.x);
                 m.y = m.x * mt_pow2(-e);
                 if (tile % a.cols == 0) a.hscale[row] = mt_pow2(e);
               } else {

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from ironmule_b200 import kernels
+from tests.test_moe_gpu import dense, mlp_case
 
 pytestmark = pytest.mark.gpu
 
@@ -54,3 +55,59 @@ def test_status_waits_for_the_products_stream(cuda):
         torch.cuda._sleep(100_000_000)
         ws.fill_(1)
         assert kernels.qgemm_packed_status(ws) == 0x01010101
+
+
+# ---- gated MLP -------------------------------------------------------------------------------------------------
+def mlp_reference(x, gate, up, down, ex, act):
+    """float64 outputs of one expert, and the bound on the kernel's error: weights as fp16 (2^-11 of each, and 2^-18 of
+    its row's largest where a group is far below it), products and activations rounded to fp16 (2^-11), the gate's
+    exponential, float32 sums, one rounding to bf16 (2^-8)."""
+    def bound(q, xa):
+        w, _ = dense(q, ex)
+        return 2**-11 * (xa @ w.abs().T) + 2**-18 * xa.sum(1, keepdim=True) * w.abs().amax(1)
+
+    xd = x.double()
+    g, u = xd @ dense(gate, ex)[0].T, xd @ dense(up, ex)[0].T
+    dg, du = bound(gate, xd.abs()), bound(up, xd.abs())
+    a = g * torch.sigmoid(g) if act == "swiglu" else \
+        0.5 * g * (1.0 + torch.tanh(0.7978845608028654 * (g + 0.044715 * g**3)))
+    hid = a * u
+    dh = 1.13 * dg * (u.abs() + du) + a.abs() * du + 2**-10 * hid.abs()
+    w = dense(down, ex)[0]
+    want = hid @ w.T
+    return want, 2**-8 * want.abs() + dh @ w.abs().T + bound(down, hid.abs())
+
+
+def check_mlp(x, gate, up, down, r, act="swiglu"):
+    y = kernels.moe_mlp(x, kernels.Experts.gate_up(gate, up), kernels.Experts(*down), r, activation=act)
+    ids = r.ids.long()
+    for ex in range(gate[0].shape[0]):
+        row, place = torch.nonzero(ids == ex, as_tuple=True)
+        if row.numel():
+            want, tol = mlp_reference(x[row], gate, up, down, ex, act)
+            off = (y[row, place].double() - want).abs()
+            assert bool((off <= tol).all()), (ex, float((off / tol).max()))
+    return y
+
+
+@pytest.mark.parametrize("act", ["swiglu", "geglu"])
+@pytest.mark.parametrize("which", ["gate", "up"])
+def test_an_expert_whose_gate_or_up_matrix_is_zero_gives_zeros(cuda, which, act):
+    gate, up, down, x, logits = mlp_case(cuda, 40, 3, 2, 256, 128, 21)
+    for t in (gate if which == "gate" else up)[1:]:
+        t[0] = 0
+    r = kernels.moe_route(logits, 2)
+    for f in (1.0, 2.0**30, 2.0**-60):
+        y = kernels.moe_mlp(x * f, kernels.Experts.gate_up(gate, up), kernels.Experts(*down), r, activation=act)
+        assert bool((y[r.ids == 0] == 0).all()), f
+        assert bool(torch.isfinite(y.float()).all())
+
+
+@pytest.mark.parametrize("act", ["swiglu", "geglu"])
+def test_tiny_gates_beside_large_up_projections(cuda, act):
+    """g of about 2^-127, u of 2^48: their product is an ordinary number, u times its inverse is not."""
+    gate, up, down, x, logits = mlp_case(cuda, 24, 4, 2, 256, 128, 22)
+    for q, f in ((gate, 2.0**-115), (up, 2.0**60)):
+        q[1].mul_(f)
+        q[2].mul_(f)
+    check_mlp(x * 2.0**-10, gate, up, down, kernels.moe_route(logits, 2), act)
