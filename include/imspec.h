@@ -364,8 +364,11 @@ int im_philox4x32_10(uint64_t seed, uint64_t offset, uint32_t stream_id, uint32_
  *
  * im_moe_route: logits [M, E] (bf16, or float32 with logits_f32; row stride ld elements) -> per row the top_k experts
  * with the largest keys float32(logit) + bias[e] (bias float32 [E] or NULL; -0 counts as +0, ties to the lower expert),
- * in that order: ids [M, top_k] and weights [M, top_k]. A logit of -inf or NaN closes the expert to the row; places
- * beyond the open experts get id -1 and weight 0. Weights come from the unbiased logits, times `scale`:
+ * in that order: ids [M, top_k] and weights [M, top_k]. With IM_MOE_BIAS_ON_SCORE added to `scoring` the key is the
+ * expert's float32 score plus bias[e] instead (the score: 1 / (1 + exp(-v)), or the softmax over all open experts): what
+ * a load-balanced router's correction bias is defined on; on the logits it would choose other experts. A logit or bias of
+ * -inf or NaN closes the expert to the row; places beyond the open experts get id -1 and weight 0. The bias only
+ * chooses: weights come from the unbiased logits, times `scale`:
  *   IM_MOE_SOFTMAX: exp(v - max) / sum, both over the chosen experts (normalise) or over all open ones;
  *   IM_MOE_SIGMOID: 1 / (1 + exp(-v)), divided by the chosen experts' sum (normalise) or as it is.
  * pairs [M * top_k] holds the pairs sorted by expert (ascending within one; places without an expert last),
@@ -396,7 +399,7 @@ int im_philox4x32_10(uint64_t seed, uint64_t offset, uint32_t stream_id, uint32_
  * y bf16 [M, places, H], h, h_out (may be h), z bf16 [M, H]; out_sq [M] (or NULL) = sums of squares of the rounded
  * h_out rows, what im_qgemm_packed's RMSNorm prologue takes. H <= 16384, places <= 32.
  */
-enum { IM_MOE_SOFTMAX = 0, IM_MOE_SIGMOID = 1 };
+enum { IM_MOE_SOFTMAX = 0, IM_MOE_SIGMOID = 1, IM_MOE_BIAS_ON_SCORE = 16 };
 size_t im_moe_plan_bytes(int64_t M, int64_t E, int64_t top_k);
 int im_moe_route(const void* logits, int logits_f32, int64_t M, int64_t E, int64_t ld, const float* bias,
                  int64_t top_k, int scoring, int normalise, float scale, int32_t* ids, float* weights,

@@ -14,7 +14,7 @@ LIB_PATH = HERE / "libimspec.so"
 
 IM_OK, IM_UNSUPPORTED, IM_INVALID, IM_CUDA_ERROR = 0, 1, 2, 3
 EPI_STORE, EPI_RESIDUAL, EPI_SWIGLU, EPI_GEGLU = 0, 1, 2, 3
-MOE_SOFTMAX, MOE_SIGMOID = 0, 1
+MOE_SOFTMAX, MOE_SIGMOID, MOE_BIAS_ON_SCORE = 0, 1, 16
 QGEMM_AUTO, QGEMM_MMA, QGEMM_FMA = 0, 1, 2
 ABI_VERSION = 1
 

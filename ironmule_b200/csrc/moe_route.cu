@@ -2,8 +2,10 @@
 // (row, place) pairs sorted by expert and cut into the work items of the grouped products.
 //
 // Selection is exact: the key of expert e is float32(logit) + bias[e] (one rounding; -0 counts as +0), the k largest
-// keys are taken in order, ties to the lower expert. A logit of -inf or NaN closes the expert to the row; a row with
-// fewer than k open experts has id -1 and weight 0 in its remaining places.
+// keys are taken in order, ties to the lower expert. A logit or bias of -inf or NaN closes the expert to the row; a row
+// with fewer than k open experts has id -1 and weight 0 in its remaining places. With IM_MOE_BIAS_ON_SCORE the key is
+// the expert's float32 score plus the bias (the correction of a load-balanced router is defined so): 1 / (1 + exp(-v)),
+// or the softmax over the open experts. The two orders differ, as the scores are not linear in the logits.
 //   softmax: p_e = exp(v_e - max v) / sum over the chosen (normalise) or over every open expert
 //   sigmoid: p_e = 1 / (1 + exp(-v_e)), over the chosen's sum when normalised. There the sums run over
 //            exp(ls - max ls), ls = log sigmoid(v), so that far-negative logits do not underflow to 0 / 0.
@@ -36,7 +38,7 @@ struct RouteArgs {
   int* plan;
   int2* where;
   int* counts;   // [E + 1][blocks]
-  int f32, scoring, normalise;
+  int f32, scoring, on_score, normalise;
   float scale;
   int M, E, top_k, rows_per_block, blocks;
   long long ld;
@@ -82,12 +84,30 @@ __device__ __forceinline__ int mr_row(const RouteArgs& a, int row, int lane) {
       const size_t at = (size_t)row * a.ld + e;
       const float l = a.f32 ? reinterpret_cast<const float*>(a.logits)[at]
                             : bf(reinterpret_cast<const uint16_t*>(a.logits)[at]);
-      const float k = !PACK && a.bias ? l + a.bias[e] : l;
+      const float k = PACK || !a.bias ? l : a.on_score ? a.bias[e] : l + a.bias[e];
       if (l > neg && k > neg) {  // false for NaN too
         v[i] = l;
         key[i] = PACK ? (mr_key(k) & 0xffff0000u) | (0xffffu - e) : mr_key(k);
       }
     }
+  }
+  if (!PACK && a.on_score) {  // keys from the scores (held in their place meanwhile)
+    float top = neg, total = 0.f;
+#pragma unroll
+    for (int i = 0; i < EL; i++) top = fmaxf(top, v[i]);
+    top = mr_warp_max(top);
+#pragma unroll
+    for (int i = 0; i < EL; i++) {
+      float score = 0.f;
+      if (v[i] > neg)
+        score = a.scoring == IM_MOE_SIGMOID ? 1.f / (1.f + expf(-v[i])) : v[i] == top ? 1.f : expf(v[i] - top);
+      total += score;
+      key[i] = __float_as_uint(score);
+    }
+    total = a.scoring == IM_MOE_SIGMOID ? 1.f : warp_sum(total);
+#pragma unroll
+    for (int i = 0; i < EL; i++)
+      key[i] = v[i] > neg ? mr_key(__uint_as_float(key[i]) / total + a.bias[i * 32 + lane]) : 0u;
   }
   int mine = -1;
   float value = neg;
@@ -435,7 +455,10 @@ extern "C" int im_moe_route(const void* logits, int logits_f32, int64_t M, int64
   IM_REQUIRE(moe_sizes_ok(M, E, top_k), IM_UNSUPPORTED,
              "im_moe_route: at most %lld rows, %d experts and %d places a row (M=%lld E=%lld top_k=%lld)",
              (long long)MOE_MAX_ROWS, MOE_MAX_EXPERTS, MOE_MAX_TOP_K, (long long)M, (long long)E, (long long)top_k);
+  const int on_score = scoring & IM_MOE_BIAS_ON_SCORE;
+  scoring &= ~IM_MOE_BIAS_ON_SCORE;
   IM_REQUIRE(scoring == IM_MOE_SOFTMAX || scoring == IM_MOE_SIGMOID, IM_INVALID, "im_moe_route: bad scoring");
+  IM_REQUIRE(!on_score || bias, IM_INVALID, "im_moe_route: a bias on the scores needs bias");
   IM_REQUIRE(offsets && plan, IM_INVALID, "im_moe_route: null pointer");
   IM_REQUIRE(M == 0 || (logits && ids && weights && pairs), IM_INVALID, "im_moe_route: null pointer");
   IM_REQUIRE(ld >= E, IM_INVALID, "im_moe_route: row stride %lld below %lld experts", (long long)ld, (long long)E);
@@ -456,6 +479,7 @@ extern "C" int im_moe_route(const void* logits, int logits_f32, int64_t M, int64
   a.counts = a.plan + p.counts;
   a.f32 = logits_f32;
   a.scoring = scoring;
+  a.on_score = on_score;
   a.normalise = normalise;
   a.scale = scale;
   a.M = (int)M;

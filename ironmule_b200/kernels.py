@@ -609,14 +609,20 @@ def _mlp_workspace(m: int, e: int, k: int, h: int, inter: int) -> int:
 
 
 def moe_route(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax", normalise: bool = True,
-              scale: float = 1.0, bias: torch.Tensor | None = None, rows: int | None = None) -> Routing:
+              scale: float = 1.0, bias: torch.Tensor | None = None, bias_on: str = "logit",
+              rows: int | None = None) -> Routing:
     """Choose top_k experts for each of the first `rows` rows of logits [M, E] (bf16 or float32): the largest
-    logit + bias, ties to the lower expert; -inf or NaN closes an expert to a row."""
+    logit + bias, ties to the lower expert; -inf or NaN closes an expert to a row. bias_on="score" chooses by
+    sigmoid(logit) + bias or softmax(logits) + bias instead, what the correction bias of a load-balanced router is
+    trained for. The bias only chooses: weights are the unbiased scores."""
     _check(logits, "logits", (torch.bfloat16, torch.float32))
     if logits.dim() != 2:
         raise ValueError(f"logits must be [M, E], got {tuple(logits.shape)}")
     if scoring not in _SCORING:
         raise ValueError(f"scoring {scoring!r}: softmax or sigmoid")
+    if bias_on not in ("logit", "score"):
+        raise ValueError(f"bias_on {bias_on!r}: logit or score")
+    how = _SCORING[scoring] + (_lib.MOE_BIAS_ON_SCORE if bias is not None and bias_on == "score" else 0)
     device, e = logits.device, logits.shape[1]
     m = logits.shape[0] if rows is None else rows
     if not 0 <= m <= logits.shape[0]:
@@ -630,7 +636,7 @@ def moe_route(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax", nor
     r = Routing(m, e, top_k, device)
     base, n = r.buf.data_ptr(), 4 * m * top_k
     _lib.call("im_moe_route", logits.data_ptr(), int(logits.dtype == torch.float32), m, e, e, _ptr_or_none(bias), top_k,
-              _SCORING[scoring], int(normalise), float(scale), base, base + n, base + 3 * n, base + 2 * n,
+              how, int(normalise), float(scale), base, base + n, base + 3 * n, base + 2 * n,
               r._plan_ptr, r.plan_bytes, _stream(device))
     return r
 

@@ -40,6 +40,48 @@ def test_softmax_with_a_bias_that_passes_over_the_largest_logits(cuda, rows):
     assert one.ids.tolist() == [[1]] and one.weights.tolist() == [[1.0]]
 
 
+@pytest.mark.parametrize("scoring", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("rows,experts,top_k", [(1, 8, 2), (40, 60, 4), (300, 256, 8), (70, 500, 32)])
+def test_a_bias_on_the_scores_chooses_by_score_plus_bias(cuda, scoring, rows, experts, top_k):
+    gen = torch.Generator(device=cuda).manual_seed(rows + experts)
+    logits = 2.0 * torch.randn((rows, experts), generator=gen, device=cuda)
+    logits[torch.rand((rows, experts), generator=gen, device=cuda) < 0.1] = float("-inf")
+    bias = (0.2 if scoring == "sigmoid" else 2.0 / experts) * torch.randn((experts,), generator=gen, device=cuda)
+    for dtype in (torch.float32, torch.bfloat16):
+        given = logits.to(dtype)
+        r = kernels.moe_route(given, top_k, scoring=scoring, normalise=True, scale=2.5, bias=bias, bias_on="score")
+        v = given.double()
+        score = torch.sigmoid(v) if scoring == "sigmoid" else torch.softmax(v, 1)
+        key = torch.where(v > float("-inf"), score + bias.double(), float("-inf"))
+        order = torch.sort(key, dim=1, descending=True, stable=True)
+        # float32 scores are off by some 2^-22 of themselves: rows with keys closer than that may go either way
+        gap = (order.values[:, :top_k] - order.values[:, 1:top_k + 1]).amin(1)
+        clear = gap > 2.0**-20
+        assert int(clear.sum()) * 2 >= rows
+        ids = order.indices[:, :top_k]
+        assert torch.equal(r.ids[clear].long(), ids[clear])
+        picked = torch.gather(score, 1, ids)
+        want = 2.5 * picked / picked.sum(1, keepdim=True)
+        assert bool(((r.weights.double() - want).abs()[clear] <= 4e-6 * want[clear]).all())
+        flat = r.ids.flatten()
+        assert torch.equal(r.pairs.long(), torch.sort(torch.where(flat < 0, experts, flat), stable=True).indices)
+
+
+def test_where_the_bias_goes_decides(cuda):
+    logits, bias = torch.tensor([[6.0, 5.0, 0.0]], device=cuda), torch.tensor([0.0, 0.1, 0.0], device=cuda)
+    for dtype in (torch.float32, torch.bfloat16):
+        on = lambda where: kernels.moe_route(logits.to(dtype), 1, scoring="sigmoid", normalise=False, bias=bias,  # noqa: E731
+                                             bias_on=where)
+        assert on("logit").ids.tolist() == [[0]] and on("score").ids.tolist() == [[1]]
+        assert on("score").weights[0, 0].item() == pytest.approx(0.9933071490757153, rel=4e-6)
+    closing = torch.tensor([0.0, float("-inf"), float("nan")], device=cuda)
+    for scoring in ("sigmoid", "softmax"):
+        r = kernels.moe_route(logits, 2, scoring=scoring, bias=closing, bias_on="score")
+        assert r.ids.tolist() == [[0, -1]] and r.weights.tolist() == [[1.0, 0.0]]
+    with pytest.raises(ValueError, match="bias_on"):
+        kernels.moe_route(logits, 1, bias=bias, bias_on="probability")
+
+
 # ---- status ---------------------------------------------------------------------------------------------------
 def test_status_waits_for_the_products_stream(cuda):
     """On a stream of torch's pool, which the legacy default stream does not wait for: the error words are read after
