@@ -687,6 +687,8 @@ def moe_mlp(x: torch.Tensor, gate_up: Experts, down: Experts, routing: Routing, 
         raise ValueError("x must be [M, H]")
     if activation not in ("swiglu", "geglu"):
         raise ValueError(f"activation {activation!r}: swiglu or geglu")
+    if gate_up.n % 2:
+        raise ValueError(f"gate_up has {gate_up.n} rows: gate and up rows come in pairs (Experts.gate_up)")
     h, inter = gate_up.k, gate_up.n // 2
     if (down.e, down.n, down.k) != (gate_up.e, h, inter) or down.data.device != x.device:
         raise ValueError(f"down is {down.e} x [{down.n}, {down.k}], expected {gate_up.e} x [{h}, {inter}]")

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from ironmule_b200 import kernels
-from tests.test_moe_gpu import dense, mlp_case
+from tests.test_moe_gpu import dense, mlp_case, quantised
 
 pytestmark = pytest.mark.gpu
 
@@ -153,3 +153,13 @@ def test_tiny_gates_beside_large_up_projections(cuda, act):
         q[1].mul_(f)
         q[2].mul_(f)
     check_mlp(x * 2.0**-10, gate, up, down, kernels.moe_route(logits, 2), act)
+
+
+def test_gate_up_of_an_odd_number_of_rows_is_refused(cuda):
+    """Half of 129 rows is 64 too, but the packed matrices of 129 lie two blocks apart, not one."""
+    gen = torch.Generator(device=cuda).manual_seed(0)
+    r = kernels.moe_route(torch.randn((4, 8), device=cuda), 2)
+    x = torch.zeros((4, 128), dtype=torch.bfloat16, device=cuda)
+    with pytest.raises(ValueError, match="129 rows"):
+        kernels.moe_mlp(x, kernels.Experts(*quantised(gen, 8, 129, 128, cuda)),
+                        kernels.Experts(*quantised(gen, 8, 128, 64, cuda)), r)
