@@ -53,6 +53,10 @@ int im_abi_version(void);
  * activations. Results are the same either way. on = 0 turns this off process-wide; returns the previous
  * setting. */
 int im_set_launch_overlap(int on);
+/* Nanoseconds after which a bounded wait of the products by expert gives up and sets their error word (a second by
+ * default; a few attempts are made in any case). Process-wide, for calls from now on; a negative value changes nothing.
+ * Returns the previous limit. */
+int64_t im_set_wait_limit(int64_t ns);
 
 /* The message of the last non-zero return on this thread ("" when the last call succeeded). */
 const char* im_last_error(void);

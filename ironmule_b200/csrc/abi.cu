@@ -28,4 +28,10 @@ extern "C" int im_set_launch_overlap(int on) {
   return was;
 }
 
+extern "C" int64_t im_set_wait_limit(int64_t ns) {
+  const int64_t was = (int64_t)im::wait_limit();
+  if (ns >= 0) im::wait_limit() = (unsigned long long)ns;
+  return was;
+}
+
 extern "C" const char* im_last_error(void) { return im::g_error; }

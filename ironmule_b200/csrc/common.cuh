@@ -49,6 +49,12 @@ inline bool& launch_overlap() {
   return on;
 }
 
+// Nanoseconds after which a bounded wait gives up (im_set_wait_limit).
+inline unsigned long long& wait_limit() {
+  static unsigned long long ns = 1000000000ull;
+  return ns;
+}
+
 template <typename... KArgs, typename... Args>
 inline int launch(const char* what, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
                   Args... args) {

@@ -40,8 +40,9 @@
 // hops a stage). Tried and left out, no faster: stages of four groups; an item's rows resident for the whole tile;
 // separate barriers for a stage's halves; five B stages against a weight ring of four.
 //
-// Every mbarrier wait is bounded (1 s): one that runs out sets the plan's error word and the CTA's abort flag, which
-// every later wait honours; copies and MMAs in flight are drained before tensor memory is freed.
+// Every mbarrier wait is bounded (1 s, or im_set_wait_limit): one that runs out sets the plan's error word and the CTA's
+// abort flag, which every later wait that is not over at once honours. A role that gives up leaves its loop without
+// touching tensor memory again; copies and MMAs in flight are drained before tensor memory is freed.
 #include <cuda_fp16.h>
 #include <math.h>
 
@@ -96,6 +97,7 @@ struct TcArgs {
   const float* half_max; // [E][2]: an expert's largest over the gate rows (r & 16 == 0) and over the up rows
   size_t expert_bytes;
   int cols;              // 128-output blocks
+  unsigned long long wait_ns;
 };
 
 __device__ __forceinline__ float mt_pow2(int e) { return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23); }
@@ -246,9 +248,10 @@ __device__ __forceinline__ void mt_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
-// One row's 64 codes of a group -> 32 fp16 pairs -> columns [col, + 32) of tensor memory, once ready() says so.
+// One row's 64 codes of a group -> 32 fp16 pairs -> columns [col, + 32) of tensor memory, once ready() says so (the
+// whole warp's answer, which is passed on).
 template <typename F>
-__device__ __forceinline__ void mt_group(const unsigned char* codes, const unsigned char* affine, float inv, int q,
+__device__ __forceinline__ bool mt_group(const unsigned char* codes, const unsigned char* affine, float inv, int q,
                                          uint32_t col, F ready) {
   const uint4 c0 = *reinterpret_cast<const uint4*>(codes), c1 = *reinterpret_cast<const uint4*>(codes + 512);
   const float sf = bf(*reinterpret_cast<const uint16_t*>(affine)) * inv;
@@ -258,7 +261,7 @@ __device__ __forceinline__ void mt_group(const unsigned char* codes, const unsig
   const uint32_t words[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
 #pragma unroll
   for (int i = 0; i < 8; i++) mt_expand(words[i], s24, s20, b2, p + 4 * i);
-  if (!ready()) return;
+  if (!ready()) return false;
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
@@ -268,6 +271,7 @@ __device__ __forceinline__ void mt_group(const unsigned char* codes, const unsig
       "r"(p[19]), "r"(p[20]), "r"(p[21]), "r"(p[22]), "r"(p[23]), "r"(p[24]), "r"(p[25]), "r"(p[26]), "r"(p[27]),
       "r"(p[28]), "r"(p[29]), "r"(p[30]), "r"(p[31])
       : "memory");
+  return true;
 }
 
 template <int EPI>
@@ -322,7 +326,7 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
   const int ntiles = __ldcg(a.p.plan) * a.cols;
   MtTile* const info = reinterpret_cast<MtTile*>(sbase + MT_OFF_TILE);
   uint32_t islot = 0, iphase = 0;  // this warp's place in the ring of tiles
-  auto tile_wait = [&] { return qt_wait_short(bars + 8 * (MT_I_FULL + islot), iphase, abort_flag, a.error); };
+  auto tile_wait = [&] { return qt_wait_short(bars + 8 * (MT_I_FULL + islot), iphase, abort_flag, a.error, a.wait_ns); };
   auto tile_free = [&] {  // this warp has read what it needs
     __syncwarp();
     if (lane == 0) mt_arrive(bars + 8 * (MT_I_EMPTY + islot));
@@ -343,7 +347,7 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
       const unsigned char* src =
           a.p.wp + (size_t)expert * a.expert_bytes + (size_t)(tile % a.cols) * G * MOE_BLOCK_BYTES;
       for (int g = 0; g < G; g += 2, k++) {
-        if (!qt_wait_short(bars + 8 * (MT_W_EMPTY + s), phase, abort_flag, a.error)) goto weights_done;
+        if (!qt_wait_short(bars + 8 * (MT_W_EMPTY + s), phase, abort_flag, a.error, a.wait_ns)) goto weights_done;
         if (leader)
           mt_copy(base + (uint32_t)MT_OFF_W + s * 2 * MOE_BLOCK_BYTES, src, g + 1 < G ? 2 * MOE_BLOCK_BYTES : MOE_BLOCK_BYTES,
                   bars + 8 * (MT_W_FULL + s));
@@ -353,10 +357,11 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
       }
     }
   weights_done:
-    if (*abort_flag)  // copies still landing in this CTA's shared memory finish before it exits
-      for (int j = k > MT_W ? k - MT_W : 0; j < k; j++)
-        qt_drain(reinterpret_cast<unsigned long long*>(sbase + MT_OFF_BAR) + MT_W_FULL + j % MT_W,
-                 (uint32_t)((j / MT_W) & 1));
+    // copies still landing in this CTA's shared memory finish before it exits (in every case: another role may give up
+    // after this one has issued its last)
+    for (int j = k > MT_W ? k - MT_W : 0; j < k; j++)
+      qt_drain(reinterpret_cast<unsigned long long*>(sbase + MT_OFF_BAR) + MT_W_FULL + j % MT_W,
+               (uint32_t)((j / MT_W) & 1));
   } else if (warp == 1) {
     // ---- MMA issue -----------------------------------------------------------------------------------------
     // (the whole warp walks the loop, so that its addresses stay in uniform registers; one lane issues)
@@ -372,11 +377,11 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
       const uint32_t idesc = (1u << 4) | ((uint32_t)((item.z + 15) / 16 * 2) << 17) | ((128u >> 4) << 24);
       const uint32_t tile_step = (uint32_t)((item.z + 15) / 16 * 128);  // (16 bytes units) to the second group's rows
       const int buf = t & 1;
-      if (!qt_wait_short(bars + 8 * (MT_D_EMPTY + buf), (uint32_t)((t / 2 + 1) & 1), abort_flag, a.error)) break;
+      if (!qt_wait_short(bars + 8 * (MT_D_EMPTY + buf), (uint32_t)((t / 2 + 1) & 1), abort_flag, a.error, a.wait_ns)) break;
       const uint32_t d = tmem + (uint32_t)(buf * MT_N);
       int g = 0;
       for (; g < G; g += 2, k++) {
-        if (!qt_wait_short(bars + 8 * (MT_FULL + s), phase, abort_flag, a.error)) break;
+        if (!qt_wait_short(bars + 8 * (MT_FULL + s), phase, abort_flag, a.error, a.wait_ns)) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         if (leader) {
           const uint64_t bd = qt_desc(base + s * MT_B), bd1 = bd + tile_step;
@@ -397,9 +402,10 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
       __syncwarp();
       t++;
     }
-    if (*abort_flag && k > 0)
-      qt_drain(reinterpret_cast<unsigned long long*>(sbase + MT_OFF_BAR) + MT_DONE + (k - 1) % MT_S,
-               (uint32_t)(((k - 1) / MT_S) & 1));
+    // so do the MMAs, before tensor memory is freed, and the arrivals that follow them
+    unsigned long long* const b = reinterpret_cast<unsigned long long*>(sbase + MT_OFF_BAR);
+    for (int j = k > MT_S ? k - MT_S : 0; j < k; j++) qt_drain(b + MT_DONE + j % MT_S, (uint32_t)((j / MT_S) & 1));
+    for (int j = t > 2 ? t - 2 : 0; j < t; j++) qt_drain(b + MT_D_FULL + (j & 1), (uint32_t)((j / 2) & 1));
   } else if (warp < MT_W_LOAD) {
     // ---- epilogue: lane = output of the block, columns = the item's rows ---------------------------------------
     const int q = warp & 3, set = (warp - MT_W_EPI) >> 2;
@@ -408,7 +414,7 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
     pdl_trigger();
     int t = 0;
     for (int tile = blockIdx.x; tile < ntiles; tile += gridDim.x) {
-      if (!tile_wait() || !qt_wait_short(bars + 8 * (MT_C_FULL + islot), iphase, abort_flag, a.error)) break;
+      if (!tile_wait() || !qt_wait_short(bars + 8 * (MT_C_FULL + islot), iphase, abort_flag, a.error, a.wait_ns)) break;
       const int4 item = info[islot].item;
       const float wscale = info[islot].wscale[q * 32 + lane];
       const float2* meta = info[islot].col;
@@ -423,7 +429,7 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
         continue;
       }
       const int buf = t & 1;
-      if (!qt_wait_short(bars + 8 * (MT_D_FULL + buf), (uint32_t)((t / 2) & 1), abort_flag, a.error)) break;
+      if (!qt_wait_short(bars + 8 * (MT_D_FULL + buf), (uint32_t)((t / 2) & 1), abort_flag, a.error, a.wait_ns)) break;
       t++;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
@@ -511,7 +517,7 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
 #pragma unroll
           for (int i = 0; i < 4; i++) top[i] = __ldcg(rm + 32 * i);
         }
-        if (!qt_wait_short(bars + 8 * (MT_I_EMPTY + islot), iphase ^ 1u, abort_flag, a.error)) break;
+        if (!qt_wait_short(bars + 8 * (MT_I_EMPTY + islot), iphase ^ 1u, abort_flag, a.error, a.wait_ns)) break;
         MtTile& out = info[islot];
         if (lane == 0) out.item = item;
 #pragma unroll
@@ -569,7 +575,7 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
         const uint32_t bytes = (uint32_t)((item.z + 15) & ~15) * 128u;
         const unsigned char* src = a.tiles + (size_t)item.w * a.p.K * 2;
         for (int g = 0; g < G; g += 2, k++) {
-          if (!qt_wait_short(bars + 8 * (MT_DONE + s), phase, abort_flag, a.error)) goto rows_done;
+          if (!qt_wait_short(bars + 8 * (MT_DONE + s), phase, abort_flag, a.error, a.wait_ns)) goto rows_done;
           if (leader) mt_copy(base + s * MT_B, src, g + 1 < G ? 2 * bytes : bytes, bars + 8 * (MT_FULL + s));
           __syncwarp();
           src += 2 * bytes;
@@ -577,11 +583,10 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
         }
       }
     rows_done:
-      if (*abort_flag)  // copies still landing finish before the CTA exits (a second a stage is ample, and the limit
-                        // where the expansion's arrivals never come)
-        for (int j = k > MT_S ? k - MT_S : 0; j < k; j++)
-          qt_drain(reinterpret_cast<unsigned long long*>(sbase + MT_OFF_BAR) + MT_FULL + j % MT_S,
-                   (uint32_t)((j / MT_S) & 1));
+      // as for the weights (a second a stage is ample, and the limit where the expansion's arrivals never come)
+      for (int j = k > MT_S ? k - MT_S : 0; j < k; j++)
+        qt_drain(reinterpret_cast<unsigned long long*>(sbase + MT_OFF_BAR) + MT_FULL + j % MT_S,
+                 (uint32_t)((j / MT_S) & 1));
     }
   } else {
     // ---- code expansion: set i takes every fourth stage of the CTA's sequence, from stage i on -----------------------
@@ -599,15 +604,15 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
       if (expert == a.p.E) continue;
       int g = skip;
       for (; g < G; g += 2 * MT_SETS) {
-        if (!qt_wait_short(bars + 8 * (MT_W_FULL + sw), wphase, abort_flag, a.error)) goto expand_done;
+        if (!qt_wait_short(bars + 8 * (MT_W_FULL + sw), wphase, abort_flag, a.error, a.wait_ns)) goto expand_done;
         const uint32_t at = sw * 2 * MOE_BLOCK_BYTES;
-        mt_group(codes + at, affine + at, inv, q, MT_A0 + 64 * set, [&] {
-          return qt_wait_short(bars + 8 * (MT_DONE + set), phase, abort_flag, a.error);
-        });
+        if (!mt_group(codes + at, affine + at, inv, q, MT_A0 + 64 * set, [&] {
+              return qt_wait_short(bars + 8 * (MT_DONE + set), phase, abort_flag, a.error, a.wait_ns);
+            }))
+          goto expand_done;
         if (g + 1 < G)
           mt_group(codes + at + MOE_BLOCK_BYTES, affine + at + MOE_BLOCK_BYTES, inv, q, MT_A0 + 64 * set + 32,
                    [] { return true; });
-        if (__any_sync(0xffffffffu, *abort_flag)) goto expand_done;
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncwarp();
@@ -697,6 +702,7 @@ int moe_product_launch(const MoePlan& p, const MoeProduct& prod, const MoeSpace&
   a.expert_bytes = (size_t)a.cols * G * MOE_BLOCK_BYTES;
   a.row_max = reinterpret_cast<const float*>(prod.wp + (size_t)prod.E * a.expert_bytes);
   a.half_max = a.row_max + (size_t)prod.E * a.cols * 128;
+  a.wait_ns = wait_limit();
   const int64_t tiles = p.max_items * a.cols;
   IM_REQUIRE(tiles < (1ll << 31), IM_UNSUPPORTED, "grouped product: too many tiles");
   switch (prod.epilogue) {

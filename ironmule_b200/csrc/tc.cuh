@@ -5,7 +5,7 @@
 
 namespace im {
 
-constexpr unsigned long long QT_WAIT_NS = 1000000000ull;
+constexpr unsigned long long QT_WAIT_NS = 1000000000ull;  // of the drains, and of every other wait unless it is set
 
 __device__ __forceinline__ uint32_t qt_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
@@ -73,14 +73,14 @@ __device__ __forceinline__ bool qt_try_wait_64(uint32_t bar, uint32_t parity) {
 // the warp leaves it converged (tcgen05's .aligned instructions follow, and lanes may see a phase complete at different
 // attempts) and of one mind (a lane that gave up takes the others along).
 __device__ __forceinline__ bool qt_wait_short(uint32_t bar, uint32_t parity, volatile int* abort_flag,
-                                              unsigned* error) {
+                                              unsigned* error, unsigned long long limit) {
   bool ok = qt_try_wait_64(bar, parity);
   if (!ok) {
     const unsigned long long t0 = qt_clock();
     while (true) {
       ok = qt_try_wait(bar, parity);
       if (ok || *abort_flag) break;
-      if (qt_clock() - t0 > QT_WAIT_NS) {
+      if (qt_clock() - t0 > limit) {
         *abort_flag = 1;
         atomicExch(error, 1u);
         break;
@@ -100,6 +100,7 @@ __device__ __forceinline__ bool qt_elect() {
 // Bounded wait that ignores the abort flag (draining copies and MMAs already in flight).
 __device__ __forceinline__ void qt_drain(unsigned long long* bar, uint32_t parity) {
   const uint32_t b = qt_smem(bar);
+  if (qt_try_wait(b, parity)) return;
   const unsigned long long t0 = qt_clock();
   while (!qt_try_wait(b, parity) && qt_clock() - t0 < QT_WAIT_NS) {
   }

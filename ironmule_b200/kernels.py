@@ -433,6 +433,12 @@ def set_launch_overlap(on: bool) -> bool:
     return bool(_lib.load().im_set_launch_overlap(int(bool(on))))
 
 
+def set_wait_limit(ns: int) -> int:
+    """Nanoseconds after which a bounded wait of the products by expert gives up (a second by default); returns the
+    previous limit. Calls made from now on, captured graphs not."""
+    return int(_lib.load().im_set_wait_limit(ns))
+
+
 def qgemm_packed_workspace_bytes(m: int, n: int, k: int) -> int:
     return int(_lib.load().im_qgemm_packed_workspace_bytes(m, n, k))
 

@@ -163,3 +163,28 @@ def test_gate_up_of_an_odd_number_of_rows_is_refused(cuda):
     with pytest.raises(ValueError, match="129 rows"):
         kernels.moe_mlp(x, kernels.Experts(*quantised(gen, 8, 129, 128, cuda)),
                         kernels.Experts(*quantised(gen, 8, 128, 64, cuda)), r)
+
+
+# ---- bounded waits ----------------------------------------------------------------------------------------------
+def test_a_wait_that_runs_out_sets_the_status_and_leaves_the_gpu_usable(cuda):
+    """With no time beyond the first attempts, the one tile of a product over 2^20 inputs (milliseconds) outlasts its
+    waits: the routing says so, the kernel ends, and the next product is right."""
+    gen = torch.Generator(device=cuda).manual_seed(5)
+    experts = kernels.Experts(*quantised(gen, 1, 64, 1 << 20, cuda))
+    x = torch.randn((3, 1 << 20), generator=gen, device=cuda).to(torch.bfloat16)
+    logits = torch.zeros((3, 1), device=cuda)
+    r = kernels.moe_route(logits, 1)
+    want = kernels.grouped_qgemm(x, experts, r)
+    assert r.status() == 0
+    was = kernels.set_wait_limit(0)
+    try:
+        assert was == 1_000_000_000 and kernels.set_wait_limit(-1) == 0
+        kernels.grouped_qgemm(x, experts, r)
+        assert r.status() == 1
+    finally:
+        kernels.set_wait_limit(was)
+    again = kernels.moe_route(logits, 1)
+    got = kernels.grouped_qgemm(x, experts, again)
+    assert again.status() == 0 and torch.equal(got.view(torch.int16), want.view(torch.int16))
+    gate, up, down, xs, scores = mlp_case(cuda, 160, 24, 4, 512, 320, 3)
+    check_mlp(xs, gate, up, down, kernels.moe_route(scores, 4))
