@@ -408,6 +408,11 @@ size_t im_moe_plan_bytes(int64_t M, int64_t E, int64_t top_k);
 int im_moe_route(const void* logits, int logits_f32, int64_t M, int64_t E, int64_t ld, const float* bias,
                  int64_t top_k, int scoring, int normalise, float scale, int32_t* ids, float* weights,
                  int32_t* offsets, int32_t* pairs, void* plan, size_t plan_bytes, void* stream);
+/* The same with the caller's own error word (int32 on the device, or NULL; routing does not clear it): products of this
+ * routing set it to 1 too when a wait runs out. It outlives the plan, so one word can stand for many calls. */
+int im_moe_route_ex(const void* logits, int logits_f32, int64_t M, int64_t E, int64_t ld, const float* bias,
+                    int64_t top_k, int scoring, int normalise, float scale, int32_t* ids, float* weights,
+                    int32_t* offsets, int32_t* pairs, void* plan, size_t plan_bytes, int32_t* error, void* stream);
 int im_moe_status(const void* plan);
 size_t im_moe_packed_bytes(int64_t E, int64_t N, int64_t K);
 int im_moe_pack_w4g64(const uint32_t* w, const uint16_t* scales, const uint16_t* biases, int64_t E, int64_t N,

@@ -82,6 +82,8 @@ SIGNATURES: dict[str, tuple] = {
     "im_moe_plan_bytes": (_SZ, [_I64, _I64, _I64]),
     "im_moe_route": (_INT, [_P, _INT, _I64, _I64, _I64, _P, _I64, _INT, _INT, ctypes.c_float, _P, _P, _P, _P, _P, _SZ,
                             _P]),
+    "im_moe_route_ex": (_INT, [_P, _INT, _I64, _I64, _I64, _P, _I64, _INT, _INT, ctypes.c_float, _P, _P, _P, _P, _P, _SZ,
+                               _P, _P]),
     "im_moe_status": (_INT, [_P]),
     "im_moe_packed_bytes": (_SZ, [_I64, _I64, _I64]),
     "im_moe_pack_w4g64": (_INT, [_P, _P, _P, _I64, _I64, _I64, _P, _P]),

@@ -14,7 +14,8 @@ constexpr int64_t MOE_MAX_ROWS = 1 << 22;
 constexpr int MOE_ROUTE_BLOCKS = 296;   // blocks of the routing kernels at most (two per SM)
 constexpr int MOE_ROUTE_ROWS = 64;      // rows that one block alone routes
 constexpr int MOE_ITEM_ROWS = 128;      // rows of a work item at most (MMA N)
-constexpr int MOE_PLAN_HEADER = 8;      // ints: [0] work items, [1] error word of the bounded waits
+constexpr int MOE_PLAN_HEADER = 8;      // ints: [0] work items, [1] error word of the bounded waits, [2..3] the address
+                                        // of the caller's own error word (0: none)
 
 // Packed weights of an expert: 128-output blocks (rows past N are zero), each a run of 64-wide groups of
 // MOE_BLOCK_BYTES = 4 tiles of 32 rows x (two 16-byte halves a row, [half][row]) of codes, then per tile 128 bytes of

@@ -38,6 +38,7 @@ struct RouteArgs {
   int* plan;
   int2* where;
   int* counts;   // [E + 1][blocks]
+  int* error;    // the caller's error word, or NULL
   int f32, scoring, on_score, normalise;
   float scale;
   int M, E, top_k, rows_per_block, blocks;
@@ -238,6 +239,12 @@ __device__ __forceinline__ int mr_item_rows(int c) {
 }
 __device__ __forceinline__ int mr_ceil16(int n) { return (n + 15) & ~15; }
 
+__device__ __forceinline__ void mr_header(const RouteArgs& a, int items) {
+  a.plan[0] = items;
+  a.plan[1] = 0;
+  *reinterpret_cast<int**>(a.plan + 2) = a.error;
+}
+
 // Offsets, work items (block 0) and this block's pairs, from s.total and s.base.
 __device__ __forceinline__ void mr_place(const RouteArgs& a, RouteSmem& s) {
   const int nb = a.E + 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -260,8 +267,7 @@ __device__ __forceinline__ void mr_place(const RouteArgs& a, RouteSmem& s) {
     }
     if (threadIdx.x == 0) {
       a.offsets[nb] = all;
-      a.plan[0] = items_all;
-      a.plan[1] = 0;
+      mr_header(a, items_all);
     }
   }
   for (int e = threadIdx.x; e < nb; e += MR_THREADS) s.base[e] += s.first[e];
@@ -341,8 +347,7 @@ __device__ __forceinline__ void mr_place_few(const RouteArgs& a, RouteSmem& s) {
     a.where[p] = b == a.E ? make_int2(-1, 0) : make_int2(pad, before | mr_ceil16(same) << 16);
   }
   if (p == 0) {
-    a.plan[0] = items;
-    a.plan[1] = 0;
+    mr_header(a, items);
   }
 }
 
@@ -449,6 +454,14 @@ extern "C" size_t im_moe_plan_bytes(int64_t M, int64_t E, int64_t top_k) {
 extern "C" int im_moe_route(const void* logits, int logits_f32, int64_t M, int64_t E, int64_t ld, const float* bias,
                             int64_t top_k, int scoring, int normalise, float scale, int32_t* ids, float* weights,
                             int32_t* offsets, int32_t* pairs, void* plan, size_t plan_bytes, void* stream) {
+  return im_moe_route_ex(logits, logits_f32, M, E, ld, bias, top_k, scoring, normalise, scale, ids, weights, offsets,
+                         pairs, plan, plan_bytes, nullptr, stream);
+}
+
+extern "C" int im_moe_route_ex(const void* logits, int logits_f32, int64_t M, int64_t E, int64_t ld, const float* bias,
+                               int64_t top_k, int scoring, int normalise, float scale, int32_t* ids, float* weights,
+                               int32_t* offsets, int32_t* pairs, void* plan, size_t plan_bytes, int32_t* error,
+                               void* stream) {
   clear_error();
   IM_REQUIRE(M >= 0 && E >= 1 && top_k >= 1 && top_k <= E, IM_INVALID,
              "im_moe_route: bad sizes M=%lld E=%lld top_k=%lld", (long long)M, (long long)E, (long long)top_k);
@@ -462,8 +475,8 @@ extern "C" int im_moe_route(const void* logits, int logits_f32, int64_t M, int64
   IM_REQUIRE(offsets && plan, IM_INVALID, "im_moe_route: null pointer");
   IM_REQUIRE(M == 0 || (logits && ids && weights && pairs), IM_INVALID, "im_moe_route: null pointer");
   IM_REQUIRE(ld >= E, IM_INVALID, "im_moe_route: row stride %lld below %lld experts", (long long)ld, (long long)E);
-  IM_REQUIRE(aligned(logits, logits_f32 ? 4 : 2) && aligned(plan, 16), IM_INVALID,
-             "im_moe_route: misaligned logits or plan");
+  IM_REQUIRE(aligned(logits, logits_f32 ? 4 : 2) && aligned(plan, 16) && aligned(error, 4), IM_INVALID,
+             "im_moe_route: misaligned logits, plan or error word");
   const MoePlan p = moe_plan(M, E, top_k);
   IM_REQUIRE(plan_bytes >= p.bytes, IM_INVALID, "im_moe_route: plan of %zu bytes needed, %zu given", p.bytes,
              plan_bytes);
@@ -477,6 +490,7 @@ extern "C" int im_moe_route(const void* logits, int logits_f32, int64_t M, int64
   a.plan = reinterpret_cast<int*>(plan);
   a.where = reinterpret_cast<int2*>(a.plan + p.where);
   a.counts = a.plan + p.counts;
+  a.error = error;
   a.f32 = logits_f32;
   a.scoring = scoring;
   a.on_score = on_score;

@@ -40,8 +40,8 @@
 // hops a stage). Tried and left out, no faster: stages of four groups; an item's rows resident for the whole tile;
 // separate barriers for a stage's halves; five B stages against a weight ring of four.
 //
-// Every mbarrier wait is bounded (1 s, or im_set_wait_limit): one that runs out sets the plan's error word and the CTA's
-// abort flag, which every later wait that is not over at once honours. A role that gives up leaves its loop without
+// Every mbarrier wait is bounded (1 s, or im_set_wait_limit): one that runs out sets the plan's error word (and the
+// caller's) and the CTA's abort flag, which every later wait that is not over at once honours. A role that gives up leaves its loop without
 // touching tensor memory again; copies and MMAs in flight are drained before tensor memory is freed.
 #include <cuda_fp16.h>
 #include <math.h>
@@ -630,6 +630,10 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
   __syncwarp();
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();  // every MMA of this CTA has completed (or been drained)
+  if (threadIdx.x == 0 && *abort_flag) {
+    int* const word = *reinterpret_cast<int* const*>(a.p.plan + 2);
+    if (word) atomicExch(word, 1);
+  }
   if (warp == 1) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(MT_TMEM));

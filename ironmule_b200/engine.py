@@ -36,7 +36,7 @@ from dataclasses import dataclass, field
 
 import torch
 
-from . import kernels
+from . import _lib, kernels
 from .kvpool import PAGE, PagePool  # PAGE: KV slots per cache page
 
 MAX_QGEMM_ROWS = 320   # rows of one forward (the packed qGEMM takes them in chunks of 32)
@@ -327,6 +327,8 @@ class QuantModel:
         self.act = torch.zeros((r, c.inter), dtype=bf, device=dev)
         if c.experts:
             self.router_logits = torch.zeros((r, c.experts), dtype=bf, device=dev)
+        # set by any expert product whose bounded wait ran out (its rows are wrong from there on): check_waits() reads it
+        self.moe_error = torch.zeros((1,), dtype=torch.int32, device=dev) if c.experts else None
         self.y = torch.zeros((r, c.hidden), dtype=bf, device=dev)  # Gemma-3: projection output before its norm
         self.logits = torch.zeros((self.max_logit_rows, c.vocab), dtype=bf, device=dev)
         if self.tp > 1:  # this rank's vocabulary slice, and the all-gather target [tp][rows][V/tp]
@@ -426,7 +428,8 @@ class QuantModel:
                                               next_norm=layer.post_norm, gemma=gemma, out=h[:m])
                 tr("h_mid", h)
                 kernels.qgemm_packed(x, layer.router.p, out=self.router_logits, rows=m, sq_ld=self.sq_ld, ws=ws)
-                routing = kernels.moe_route(self.router_logits, c.experts_per_token, normalise=c.norm_topk, rows=m)
+                routing = kernels.moe_route(self.router_logits, c.experts_per_token, normalise=c.norm_topk, rows=m,
+                                            error=self.moe_error)
                 places = kernels.moe_mlp(x, layer.gate_up, layer.down, routing,
                                          activation="geglu" if gemma else "swiglu")
                 kernels.block_residual(places, h[:m], c.eps, weights=routing.weights, post_norm=layer.post_ff_norm,
@@ -487,6 +490,15 @@ class QuantModel:
             dist.all_gather_into_tensor(gathered, self.logits_local[:lr], group=self.group)
         self.logits[:lr].view(lr, self.tp, vl).copy_(gathered.view(self.tp, lr, vl).permute(1, 0, 2))
         return self.logits[:lr]
+
+    def check_waits(self, word: int | None = None) -> None:
+        """Raise when a bounded wait of an expert product ran out in an earlier forward; its results, and the K/V it
+        wrote, are not to be used (moe_error stays set until it is cleared). `word`: its value where the caller has
+        read it back already, else it is read here (a synchronisation, for models with experts only)."""
+        if self.moe_error is None:
+            return
+        if self.moe_error.item() if word is None else word:
+            raise _lib.KernelError("im_moe_mlp", 1, f"{self.cfg.name}: a bounded wait of an expert product ran out")
 
     def _all_reduce(self, t: torch.Tensor) -> None:
         import torch.distributed as dist
@@ -686,7 +698,7 @@ class SpecDecoder:
         self.end = [0] * batch
         self.reused = [0] * batch
         self.prefill_tokens = 0
-        self._host_n = self._host_tok = None
+        self._host_n = self._host_tok = self._host_err = None
         for b in range(batch):
             self._park(b)
 
@@ -887,10 +899,16 @@ class SpecDecoder:
         if self._host_n is None:
             self._host_n = torch.zeros(self.batch, dtype=torch.int32).pin_memory()
             self._host_tok = torch.zeros((self.batch, self.k + 1), dtype=torch.int32).pin_memory()
+            self._host_err = torch.zeros(2, dtype=torch.int32).pin_memory()
         self.run_rounds(1)
         self._host_n.copy_(self.n, non_blocking=True)
         self._host_tok.copy_(self.out_tokens, non_blocking=True)
+        models = [m for m in (self.target, self.draft) if m.moe_error is not None]
+        for i, m in enumerate(models):
+            self._host_err[i:i + 1].copy_(m.moe_error, non_blocking=True)
         torch.cuda.current_stream(self.device).synchronize()
+        for i, m in enumerate(models):
+            m.check_waits(int(self._host_err[i]))
         out = {}
         for b in range(self.batch):
             if not self.running[b]:
@@ -932,14 +950,21 @@ class SpecDecoder:
             if all(self.upto[b] >= self.end[b] for b in range(self.batch)):
                 return out
 
+    def _check_waits(self) -> None:
+        self.target.check_waits()
+        self.draft.check_waits()
+
     def done(self) -> bool:
+        self._check_waits()
         return bool(torch.all(self.n >= self.target_len).item())
 
     def read_stats(self) -> SpecStats:
+        self._check_waits()
         s = self.stats.sum(dim=0).tolist()
         return SpecStats(rounds=int(s[0]), tokens=int(s[1]), accepted=int(s[2]))
 
     def generated(self, b: int, prompt_len: int) -> list[int]:
+        self._check_waits()
         n = int(self.n[b].item())
         end = min(n, int(self.target_len[b].item()))
         return self.hist[b, prompt_len:end].tolist()
@@ -1061,6 +1086,7 @@ def greedy_decode(model: QuantModel, prompt: torch.Tensor, max_new: int, seq: in
         idx, _ = kernels.argmax_rows(logits, ws=model.ws_argmax)
         last = idx.clone()
         out.append(int(idx.item()))
+        model.check_waits()
         pos += 1
     return out
 
@@ -1182,6 +1208,7 @@ class DeviceDraftEngine:
                 self.filled[seqs[g]] += n
         if not picks:
             return []
+        m.check_waits()
         idx = torch.cat([p[0] for p in picks]).cpu().tolist()
         conf = torch.cat([p[1] for p in picks]).cpu().tolist()
         base = [0]
@@ -1236,6 +1263,7 @@ def drafter_generate(target: QuantModel, drafter, prompt, max_new: int, *, max_d
         feed = torch.tensor([context[-1]] + drafts, dtype=torch.int32, device=dev)
         logits = target.logits_for(feed, len(context) - 1, seq=seq)
         argmax, _ = kernels.argmax_rows(logits, ws=target.ws_argmax)
+        target.check_waits()
         new = accept(drafts, argmax.cpu().tolist())
         if drafts:
             drafter.settle(key, len(drafts), len(new) - 1)

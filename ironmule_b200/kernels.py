@@ -555,10 +555,10 @@ class Routing:
     begin (`offsets` int32 [E + 2]; the last bucket holds the places without an expert), and the products' work items.
     The tensors are views made when they are asked for."""
 
-    __slots__ = ("buf", "rows", "experts", "top_k", "plan_bytes")
+    __slots__ = ("buf", "rows", "experts", "top_k", "plan_bytes", "error")
 
-    def __init__(self, rows: int, experts: int, top_k: int, device: torch.device):
-        self.rows, self.experts, self.top_k = rows, experts, top_k
+    def __init__(self, rows: int, experts: int, top_k: int, device: torch.device, error: torch.Tensor | None = None):
+        self.rows, self.experts, self.top_k, self.error = rows, experts, top_k, error
         self.plan_bytes = _plan_bytes(rows, experts, top_k)
         self.buf = torch.empty(self._plan_at + self.plan_bytes // 4, dtype=torch.int32, device=device)
 
@@ -616,11 +616,12 @@ def _mlp_workspace(m: int, e: int, k: int, h: int, inter: int) -> int:
 
 def moe_route(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax", normalise: bool = True,
               scale: float = 1.0, bias: torch.Tensor | None = None, bias_on: str = "logit",
-              rows: int | None = None) -> Routing:
+              rows: int | None = None, error: torch.Tensor | None = None) -> Routing:
     """Choose top_k experts for each of the first `rows` rows of logits [M, E] (bf16 or float32): the largest
     logit + bias, ties to the lower expert; -inf or NaN closes an expert to a row. bias_on="score" chooses by
     sigmoid(logit) + bias or softmax(logits) + bias instead, what the correction bias of a load-balanced router is
-    trained for. The bias only chooses: weights are the unbiased scores."""
+    trained for. The bias only chooses: weights are the unbiased scores. `error` (one int32) is set to 1 when a bounded
+    wait of a product of this routing runs out: a word that a program keeps for many calls."""
     _check(logits, "logits", (torch.bfloat16, torch.float32))
     if logits.dim() != 2:
         raise ValueError(f"logits must be [M, E], got {tuple(logits.shape)}")
@@ -639,11 +640,15 @@ def moe_route(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax", nor
             raise ValueError(f"bias must be [{e}], got {tuple(bias.shape)}")
     if not 1 <= top_k <= e:
         raise ValueError(f"top_k {top_k} of {e} experts")
-    r = Routing(m, e, top_k, device)
+    if error is not None:
+        _check(error, "error", (torch.int32,), device)
+        if error.numel() != 1:
+            raise ValueError(f"error must be one element, got {tuple(error.shape)}")
+    r = Routing(m, e, top_k, device, error)
     base, n = r.buf.data_ptr(), 4 * m * top_k
-    _lib.call("im_moe_route", logits.data_ptr(), int(logits.dtype == torch.float32), m, e, e, _ptr_or_none(bias), top_k,
+    _lib.call("im_moe_route_ex", logits.data_ptr(), int(logits.dtype == torch.float32), m, e, e, _ptr_or_none(bias), top_k,
               how, int(normalise), float(scale), base, base + n, base + 3 * n, base + 2 * n,
-              r._plan_ptr, r.plan_bytes, _stream(device))
+              r._plan_ptr, r.plan_bytes, _ptr_or_none(error), _stream(device))
     return r
 
 

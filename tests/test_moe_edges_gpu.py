@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 import torch
 
-from ironmule_b200 import kernels
+from ironmule_b200 import _lib, engine, kernels
 from tests.test_moe_gpu import dense, mlp_case, quantised
 
 pytestmark = pytest.mark.gpu
@@ -188,3 +188,52 @@ def test_a_wait_that_runs_out_sets_the_status_and_leaves_the_gpu_usable(cuda):
     assert again.status() == 0 and torch.equal(got.view(torch.int16), want.view(torch.int16))
     gate, up, down, xs, scores = mlp_case(cuda, 160, 24, 4, 512, 320, 3)
     check_mlp(xs, gate, up, down, kernels.moe_route(scores, 4))
+
+
+def test_a_callers_error_word_outlives_the_routing(cuda):
+    gen = torch.Generator(device=cuda).manual_seed(6)
+    experts = kernels.Experts(*quantised(gen, 1, 64, 1 << 20, cuda))
+    x = torch.randn((1, 1 << 20), generator=gen, device=cuda).to(torch.bfloat16)
+    logits, word = torch.zeros((1, 1), device=cuda), torch.zeros(1, dtype=torch.int32, device=cuda)
+    kernels.grouped_qgemm(x, experts, kernels.moe_route(logits, 1, error=word))
+    assert word.item() == 0
+    was = kernels.set_wait_limit(0)
+    try:
+        kernels.grouped_qgemm(x, experts, kernels.moe_route(logits, 1, error=word))
+    finally:
+        kernels.set_wait_limit(was)
+    r = kernels.moe_route(torch.zeros((100, 1), device=cuda), 1, error=word)
+    assert r.status() == 0 and word.item() == 1
+    with pytest.raises(ValueError, match="one element"):
+        kernels.moe_route(logits, 1, error=torch.zeros(2, dtype=torch.int32, device=cuda))
+    with pytest.raises(TypeError):
+        kernels.moe_route(logits, 1, error=torch.zeros(1, device=cuda))
+
+
+def test_the_engine_passes_its_error_word_and_raises_when_it_is_set(cuda, monkeypatch):
+    cfg = engine.PRESETS["tiny-moe"]
+    target = engine.QuantModel(cfg, cuda, seed=1, sigma=0.05, max_rows=32, max_logit_rows=32, max_ctx=128)
+    draft = engine.QuantModel(engine.PRESETS["tiny-draft"], cuda, seed=2, max_ctx=128)
+    words, mlp = [], kernels.moe_mlp
+
+    def watched(x, gate_up, down, routing, **kw):
+        words.append(routing.error)
+        return mlp(x, gate_up, down, routing, **kw)
+
+    monkeypatch.setattr(kernels, "moe_mlp", watched)
+    dec = engine.SpecDecoder(target, draft, k=4, batch=1)
+    prompt = [5, 9, 100, 7, 3]
+    first = dec.generate([prompt], 8)
+    assert len(words) >= cfg.layers and all(w is target.moe_error for w in words)
+    dec.capture()
+    assert dec.generate([prompt], 8) == first
+    target.moe_error.fill_(1)  # what a product does whose wait runs out
+    tokens = torch.tensor(prompt, dtype=torch.int32, device=cuda)
+    engine_rows = [(t, i, 0, True) for i, t in enumerate(prompt)]
+    for read in (lambda: dec.generate([prompt], 8), dec.done, dec.read_stats, lambda: dec.generated(0, 5),
+                 lambda: engine.greedy_decode(target, tokens, 4),
+                 lambda: engine.DeviceDraftEngine(target)._decode_conf(engine_rows)):
+        with pytest.raises(_lib.KernelError, match="wait"):
+            read()
+    target.moe_error.zero_()
+    assert dec.generate([prompt], 8) == first
