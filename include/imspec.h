@@ -53,8 +53,8 @@ int im_abi_version(void);
  * activations. Results are the same either way. on = 0 turns this off process-wide; returns the previous
  * setting. */
 int im_set_launch_overlap(int on);
-/* Nanoseconds after which a bounded wait of the products by expert gives up and sets their error word (a second by
- * default; a few attempts are made in any case). Process-wide, for calls from now on; a negative value changes nothing.
+/* Nanoseconds after which a bounded wait of the tensor-core products (im_qgemm_packed above 32 rows, the products by
+ * expert) gives up and sets their error word (a second by default; a few attempts are made in any case). Process-wide, for calls from now on; a negative value changes nothing.
  * Returns the previous limit. */
 int64_t im_set_wait_limit(int64_t ns);
 
@@ -141,7 +141,8 @@ int im_qgemm_packed_path(int path);
  * cluster), 0 = through the workspace and a global arrival counter. Process-wide; both give the same bits. */
 int im_qgemm_packed_cluster(int on);
 /* The error word of a workspace last used by a call of more than 32 rows (the tensor-core kernel): 0 when
- * every bounded wait of that kernel completed, 1 when one ran out. Waits for every stream of the current device. */
+ * every bounded wait of that kernel completed, 1 when one ran out (the workspace is then used up: its counters and
+ * this word are zeroed before it serves again). Waits for every stream of the current device. */
 int im_qgemm_packed_status(const void* workspace);
 int im_qgemm_packed(const void* packed, const uint16_t* x, uint16_t* y, const uint16_t* residual, int64_t M, int64_t N,
                     int64_t K, int epilogue, const float* norm_sq, int64_t norm_parts, const uint16_t* norm_weight,

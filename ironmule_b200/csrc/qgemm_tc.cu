@@ -27,9 +27,10 @@
 //    group sums into 32 fp32 totals per thread; at an item's last group the split-K partials (the last split to
 //    arrive sums them in split order) and the epilogue (store / residual (+ sums of squares) / SwiGLU / GeGLU) in
 //    the warp-MMA kernel's order.
-// Every mbarrier wait is bounded (1 s). A wait that runs out sets the error word (the last word of the counter
-// region, read by im_qgemm_packed_status) and the CTA's abort flag, which every later wait honours; the CTA
-// then waits (bounded) for its own bulk copies and MMAs in flight before it frees its tensor memory and exits.
+// Every mbarrier wait is bounded (1 s, or im_set_wait_limit). A wait that runs out sets the error word (the last word
+// of the counter region, read by im_qgemm_packed_status) and the CTA's abort flag, which every later wait honours; a
+// warp leaves a wait as a whole. The CTA waits (bounded) for its own bulk copies and MMAs in flight before it frees its
+// tensor memory and exits.
 #include "common.cuh"
 #include "qgemm_packed.cuh"
 #include "tc.cuh"
@@ -74,6 +75,7 @@ struct QtArgs {
   int M, N, K, tiles, ctas_x, splits, sq_ld;
   int nmma;   // MMA N: rows per chunk, a multiple of 16
   int items;  // ctas_x * splits * chunks
+  unsigned long long wait_ns;
 };
 
 // An item and the position of a group in the CTA's sequence of groups.
@@ -273,17 +275,17 @@ qtc_kernel(QtArgs a) {
         }
       }
       pdl_wait();
-      int k = 0;
+      int k = 0, sums = 0;  // groups whose weights and rows, and whose sums, are on their way
       for (;; k++) {
         const int ls = k % QT_LS, r = k % QT_SR;
         if (k >= pre) {
-          if (!qt_wait(&ld_empty[ls], (uint32_t)(((k / QT_LS) - 1) & 1), abort_flag, a.error)) break;
+          if (!qt_wait(&ld_empty[ls], (uint32_t)(((k / QT_LS) - 1) & 1), abort_flag, a.error, a.wait_ns)) break;
           expect(&ld_full[ls], (uint32_t)QT_WBYTES + bbytes);
           weights(ls, c);
         }
         const size_t t = (size_t)c.chunk * G + c.cg0 + c.gl;
         copy(base + (uint32_t)(ls * QT_B), a.xt + t * QT_B, bbytes, &ld_full[ls]);
-        if (k >= QT_SR && !qt_wait(&sx_empty[r], (uint32_t)(((k / QT_SR) - 1) & 1), abort_flag, a.error)) {
+        if (k >= QT_SR && !qt_wait(&sx_empty[r], (uint32_t)(((k / QT_SR) - 1) & 1), abort_flag, a.error, a.wait_ns)) {
           k++;
           break;
         }
@@ -295,16 +297,18 @@ qtc_kernel(QtArgs a) {
           copy(base + (uint32_t)(QT_OFF_SB + (size_t)r * QT_SBB + tt * 128),
                a.wp + ((size_t)tile * G + c.cg0 + c.gl) * Q4_UNIT + 1024, 128u, &sx_full[r]);
         }
+        sums = k + 1;
         if (!qt_next(a, c)) {
           k++;
           break;
         }
       }
-      if (*abort_flag) {  // copies still landing in this CTA's shared memory finish before it exits
-        const int kk = k > pre ? k : pre;
-        for (int j = (kk > QT_LS ? kk - QT_LS : 0); j < kk; j++) qt_drain(&ld_full[j % QT_LS], (uint32_t)((j / QT_LS) & 1));
-        for (int j = (k > QT_SR ? k - QT_SR : 0); j < k; j++) qt_drain(&sx_full[j % QT_SR], (uint32_t)((j / QT_SR) & 1));
-      }
+      // copies still landing in this CTA's shared memory finish before it exits (in every case: another role may give up
+      // after this one has issued its last)
+      const int kk = k > pre ? k : pre;
+      for (int j = (kk > QT_LS ? kk - QT_LS : 0); j < kk; j++) qt_drain(&ld_full[j % QT_LS], (uint32_t)((j / QT_LS) & 1));
+      for (int j = (sums > QT_SR ? sums - QT_SR : 0); j < sums; j++)
+        qt_drain(&sx_full[j % QT_SR], (uint32_t)((j / QT_SR) & 1));
     }
     __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -321,9 +325,10 @@ qtc_kernel(QtArgs a) {
       int issued = -1;
       for (int k = 0;; k++) {
         const int ls = k % QT_LS, as = k % QT_AS, tb = k % QT_TB;
-        if (!qt_wait(&a_full[as], (uint32_t)((k / QT_AS) & 1), abort_flag, a.error)) break;
-        if (!qt_wait(&ld_full[ls], (uint32_t)((k / QT_LS) & 1), abort_flag, a.error)) break;
-        if (k >= QT_TB && !qt_wait(&t_empty[tb], (uint32_t)(((k / QT_TB) - 1) & 1), abort_flag, a.error)) break;
+        if (!qt_wait(&a_full[as], (uint32_t)((k / QT_AS) & 1), abort_flag, a.error, a.wait_ns)) break;
+        if (!qt_wait(&ld_full[ls], (uint32_t)((k / QT_LS) & 1), abort_flag, a.error, a.wait_ns)) break;
+        if (k >= QT_TB && !qt_wait(&t_empty[tb], (uint32_t)(((k / QT_TB) - 1) & 1), abort_flag, a.error, a.wait_ns))
+          break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint32_t d = tmem + (uint32_t)(tb * QT_N);
         const uint32_t sa = base + (uint32_t)(QT_OFF_A + (size_t)as * QT_A), sb = base + (uint32_t)(ls * QT_B);
@@ -348,7 +353,7 @@ qtc_kernel(QtArgs a) {
         issued = k;
         if (!qt_next(a, c)) break;
       }
-      if (*abort_flag && issued >= 0) qt_drain(&t_full[issued % QT_TB], (uint32_t)((issued / QT_TB) & 1));
+      if (issued >= 0) qt_drain(&t_full[issued % QT_TB], (uint32_t)((issued / QT_TB) & 1));
     }
     __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -370,8 +375,9 @@ qtc_kernel(QtArgs a) {
     qt_item(a, blockIdx.x, c);
     for (int k = 0;; k++) {
       const int ls = k % QT_LS, as = k % QT_AS;
-      if (!qt_wait(&ld_full[ls], (uint32_t)((k / QT_LS) & 1), abort_flag, a.error)) break;
-      if (k >= QT_AS && !qt_wait(&a_empty[as], (uint32_t)(((k / QT_AS) - 1) & 1), abort_flag, a.error)) break;
+      if (!qt_wait_warp(&ld_full[ls], (uint32_t)((k / QT_LS) & 1), abort_flag, a.error, a.wait_ns)) break;
+      if (k >= QT_AS && !qt_wait_warp(&a_empty[as], (uint32_t)(((k / QT_AS) - 1) & 1), abort_flag, a.error, a.wait_ns))
+        break;
       unsigned char* st = sbase + QT_OFF_A + (size_t)as * QT_A;
 #pragma unroll
       for (int tt = 0; tt < 2; tt++) {
@@ -415,14 +421,12 @@ qtc_kernel(QtArgs a) {
   float tot[QT_CW];
 #pragma unroll
   for (int j = 0; j < QT_CW; j++) tot[j] = 0.f;
-  QtCursor ce, cn;
+  QtCursor ce;
   qt_item(a, blockIdx.x, ce);
-  cn = ce;
-  bool has_next = qt_next(a, cn);
   for (int k = 0;; k++) {
     const int tb = k % QT_TB, r = k % QT_SR;
-    if (!qt_wait(&t_full[tb], (uint32_t)((k / QT_TB) & 1), abort_flag, a.error)) break;
-    if (!qt_wait(&sx_full[r], (uint32_t)((k / QT_SR) & 1), abort_flag, a.error)) break;
+    if (!qt_wait_warp(&t_full[tb], (uint32_t)((k / QT_TB) & 1), abort_flag, a.error, a.wait_ns)) break;
+    if (!qt_wait_warp(&sx_full[r], (uint32_t)((k / QT_SR) & 1), abort_flag, a.error, a.wait_ns)) break;
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const unsigned char* sbp = sbase + QT_OFF_SB + (size_t)r * QT_SBB + sb_off;
     const float s0 = bf(*reinterpret_cast<const uint16_t*>(sbp));
@@ -547,9 +551,7 @@ qtc_kernel(QtArgs a) {
 #pragma unroll
       for (int j = 0; j < QT_CW; j++) tot[j] = 0.f;
     }
-    if (!has_next) break;
-    ce = cn;
-    has_next = qt_next(a, cn);
+    if (!qt_next(a, ce)) break;
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();  // every MMA of this CTA has completed (or been drained): the MMA warp frees tensor memory
@@ -628,6 +630,7 @@ int qtc_launch(const Q4Plan& p, const Q4Args& a4, int epilogue, void* workspace,
   a.sq_ld = a4.sq_ld;
   a.nmma = nmma;
   a.items = p.ctas_x * p.splits * chunks;
+  a.wait_ns = wait_limit();
   switch (epilogue) {
     case IM_EPI_STORE: return qtc_launch_gemm<IM_EPI_STORE>(a, st);
     case IM_EPI_RESIDUAL: return qtc_launch_gemm<IM_EPI_RESIDUAL>(a, st);

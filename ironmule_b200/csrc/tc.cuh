@@ -36,9 +36,9 @@ __device__ __forceinline__ unsigned long long qt_clock() {
   return t;
 }
 
-// Bounded wait for the phase of `parity`; false when this CTA has given up (now or earlier).
+// Bounded wait of one thread for the phase of `parity`; false when this CTA has given up (now or earlier).
 __device__ __forceinline__ bool qt_wait(unsigned long long* bar, uint32_t parity, volatile int* abort_flag,
-                                        unsigned* error) {
+                                        unsigned* error, unsigned long long limit) {
   const uint32_t b = qt_smem(bar);
   if (*abort_flag) return false;
   if (qt_try_wait(b, parity)) return true;
@@ -46,12 +46,19 @@ __device__ __forceinline__ bool qt_wait(unsigned long long* bar, uint32_t parity
   while (true) {
     if (qt_try_wait_sleep(b, parity)) return true;
     if (*abort_flag) return false;
-    if (qt_clock() - t0 > QT_WAIT_NS) {
+    if (qt_clock() - t0 > limit) {
       *abort_flag = 1;
       atomicExch(error, 1u);
       return false;
     }
   }
+}
+
+// The same of a whole warp. It ends in a vote: the warp leaves it converged and of one mind (a lane that gave up takes
+// the others along), as the warp-wide barriers and tcgen05's .aligned instructions that follow require.
+__device__ __forceinline__ bool qt_wait_warp(unsigned long long* bar, uint32_t parity, volatile int* abort_flag,
+                                             unsigned* error, unsigned long long limit) {
+  return __all_sync(0xffffffffu, qt_wait(bar, parity, abort_flag, error, limit));
 }
 
 // Up to 64 attempts (each suspends the thread for a microsecond or two at most) in a loop of three instructions.

@@ -434,8 +434,8 @@ def set_launch_overlap(on: bool) -> bool:
 
 
 def set_wait_limit(ns: int) -> int:
-    """Nanoseconds after which a bounded wait of the products by expert gives up (a second by default); returns the
-    previous limit. Calls made from now on, captured graphs not."""
+    """Nanoseconds after which a bounded wait of the tensor-core products (packed qGEMM, products by expert) gives up (a
+    second by default); returns the previous limit. Calls made from now on, captured graphs not."""
     return int(_lib.load().im_set_wait_limit(ns))
 
 
