@@ -26,12 +26,11 @@ static bool moe_nk_ok(int64_t N, int64_t K) {
   return N >= 1 && N <= (1 << 24) && K >= 64 && K % 64 == 0 && K <= (1 << 20);
 }
 
-// One thread per row of a block's group: its codes into the packed order, the largest |w| of the row and of the expert's
-// halves (all values non-negative, so their bit patterns order as integers; a maximum does not depend on the order).
+// One thread per row of a block's group: its codes into the packed order, the largest |w| of the row (all values
+// non-negative, so their bit patterns order as integers; a maximum does not depend on the order).
 __global__ void __launch_bounds__(128)
 moe_pack_kernel(const uint32_t* __restrict__ w, const uint16_t* __restrict__ sc, const uint16_t* __restrict__ bi, int N,
-                int K, int blocks, unsigned char* __restrict__ out, unsigned* __restrict__ row_max,
-                unsigned* __restrict__ half_max) {
+                int K, int blocks, unsigned char* __restrict__ out, unsigned* __restrict__ row_max) {
   const int G = K >> 6;
   const long long unit = blockIdx.x;  // (expert * blocks + block) * G + group
   const int grp = (int)(unit % G), block = (int)(unit / G % blocks);
@@ -57,9 +56,40 @@ moe_pack_kernel(const uint32_t* __restrict__ w, const uint16_t* __restrict__ sc,
   sb[lane >> 3] = s;
   sb[4 + (lane >> 3)] = b;
   if (top > 0.f) atomicMax(row_max + (expert * blocks + block) * 128 + threadIdx.x, __float_as_uint(top));
+}
+
+// A warp per row: the row's 2-norm into the largest of its expert's half (over its finite groups, relative to its largest;
+// a thousandth and 2^-16 of the largest per weight cover what rounding the weights to operands can add).
+__global__ void __launch_bounds__(256)
+moe_norm_kernel(const uint32_t* __restrict__ w, const uint16_t* __restrict__ sc, const uint16_t* __restrict__ bi,
+                long long rows, int N, int K, int blocks, const float* __restrict__ row_max,
+                unsigned* __restrict__ norm_max) {
+  const int G = K >> 6, lane = threadIdx.x & 31;
+  const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  const long long expert = row / N;
+  const int r = (int)(row % N);
+  const float top = row_max[(expert * blocks + r / 128) * 128 + r % 128];
+  if (!(top > 0.f)) return;
+  const int e = min(max(ilogbf(top), -120), 120);
+  const float inv = ldexpf(1.f, -e);
+  float ss = 0.f;
+  for (int g = lane; g < G; g += 32) {
+    const float s = bf(sc[row * G + g]) * inv, b = bf(bi[row * G + g]) * inv;
+    if (!(fmaxf(fabsf(b), fabsf(fmaf(15.f, s, b))) < INFINITY)) continue;
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if ((lane & 15) == 0 && top > 0.f) atomicMax(half_max + 2 * expert + (lane >> 4), __float_as_uint(top));
+    for (int i = 0; i < 8; i++) {
+      const uint32_t u = w[row * (K >> 3) + g * 8 + i];
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const float v = fmaf((float)(u >> (4 * j) & 15u), s, b);
+        ss = fmaf(v, v, ss);
+      }
+    }
+  }
+  ss = warp_sum(ss);
+  const float norm = ldexpf(1.001f * sqrtf(ss) + 0x1p-16f * sqrtf((float)K), e);
+  if (lane == 0) atomicMax(norm_max + 2 * expert + (r >> 4 & 1), __float_as_uint(norm));
 }
 
 static size_t moe_expert_bytes(int64_t N, int64_t K) { return (size_t)((N + 127) / 128) * (K / 64) * MOE_BLOCK_BYTES; }
@@ -92,9 +122,13 @@ extern "C" int im_moe_pack_w4g64(const uint32_t* w, const uint16_t* scales, cons
     set_error("im_moe_pack_w4g64: %s", cudaGetErrorString(e));
     return IM_CUDA_ERROR;
   }
-  moe_pack_kernel<<<(unsigned)units, 128, 0, st>>>(w, scales, biases, (int)N, (int)K, (int)blocks, out, row_max,
-                                                row_max + (size_t)E * blocks * 128);
-  return check_launch("moe_pack_kernel");
+  moe_pack_kernel<<<(unsigned)units, 128, 0, st>>>(w, scales, biases, (int)N, (int)K, (int)blocks, out, row_max);
+  const int rc = check_launch("moe_pack_kernel");
+  if (rc) return rc;
+  moe_norm_kernel<<<(unsigned)((E * N + 7) / 8), 256, 0, st>>>(w, scales, biases, E * N, (int)N, (int)K, (int)blocks,
+                                                              reinterpret_cast<const float*>(row_max),
+                                                              row_max + (size_t)E * blocks * 128);
+  return check_launch("moe_norm_kernel");
 }
 
 extern "C" int im_moe_status(const void* plan) {

@@ -22,7 +22,7 @@ constexpr int MOE_PLAN_HEADER = 8;      // ints: [0] work items, [1] error word 
 // scales and biases: for g = 0..7 the bf16 scales of rows g, g + 8, g + 16, g + 24, then their biases. One copy brings
 // a block's group; a thread reads its row's codes in two 16-byte loads without bank conflicts. After the E experts:
 // float32 [E][padded rows], the largest |scale * q + bias| that a row's scales and biases allow; float32 [E][2], the
-// largest over an expert's rows with r & 16 == 0 (the gate rows of a gated product) and over the others (the up rows).
+// largest 2-norm of an expert's rows with r & 16 == 0 (the gate rows of a gated product) and of the others (the up rows).
 constexpr int MOE_BLOCK_BYTES = 4608;
 
 // One work item (four ints): the expert, the first of its entries in the sorted pair list, their number, and the rows

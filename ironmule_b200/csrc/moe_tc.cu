@@ -9,10 +9,12 @@
 //    the low bits of a half IS the subnormal q 2^-24 (or 16 q 2^-24), and one fused multiply-add with scale * 2^24
 //    (2^20) makes the weight. What this range costs is below 2^-18 of the row's largest weight;
 //  * a row of x by its largest finite element, which lands in [2^9, 2^10) (moe_prep_kernel; bf16 values fit fp16);
-//  * the gated activations h = act(g) u by a bound on the row: |g| <= |x|_2 sqrt(K) max |G|, |u| likewise, so
-//    |h| <= |x|_2^2 K max|G| max|U|, which lands below 2^15. No finite row can overflow, and typical rows stay well
-//    above fp16's subnormals (the bound is loose by K or so, of 2^29). Where G or U is zero throughout, so is h, and u
-//    and g are left as they are.
+//  * the gated activations h = act(g) u by a bound on the row: |g| <= |x|_2 max |G_r|_2 over the rows of G (found when it
+//    is packed), |u| likewise, so |h| <= |x|_2^2 max|G_r| max|U_r|, which lands below 2^15. No finite row can overflow.
+//    The bound is loose by K or so (2^11 of fp16's normal range of 2^29 at K = 2048), by the square of what a few large
+//    elements of x add to |x|_2, and by what the largest rows of G and U exceed the others: activations that lie 2^-40
+//    below the bound are rounded as subnormals, and lost below that. Where G or U is zero throughout, so is h, and u and
+//    g are left as they are.
 // The factors return in float32 after the sum. A row with infinities or NaN gives those.
 //
 // A persistent grid (one CTA per SM) walks tiles; its warps are coupled by mbarriers only:
@@ -94,7 +96,7 @@ struct TcArgs {
   unsigned char* next;   // the next product's tiles, and its rows' factors (written by the first product)
   float* hscale;
   const float* row_max;  // [E][128 cols]: a weight row's largest |w|
-  const float* half_max; // [E][2]: an expert's largest over the gate rows (r & 16 == 0) and over the up rows
+  const float* norm_max; // [E][2]: the largest 2-norm of an expert's gate rows (r & 16 == 0) and of its up rows
   size_t expert_bytes;
   int cols;              // 128-output blocks
   unsigned long long wait_ns;
@@ -535,9 +537,8 @@ __global__ void __launch_bounds__(MT_THREADS, 1) moe_tc_kernel(TcArgs a) {
         if (!closed) {
           float lg = 0.f, lu = 0.f;  // what bounds g and u of a row of |x|_2 = 1
           if constexpr (GLU) {
-            const float root = 0.5f * log2f((float)a.p.K);
-            lg = root + log2f(a.half_max[2 * item.x]);
-            lu = root + log2f(a.half_max[2 * item.x + 1]);
+            lg = log2f(a.norm_max[2 * item.x]);
+            lu = log2f(a.norm_max[2 * item.x + 1]);
           }
 #pragma unroll
           for (int i = 0; i < 4; i++) {
@@ -705,7 +706,7 @@ int moe_product_launch(const MoePlan& p, const MoeProduct& prod, const MoeSpace&
   a.cols = (prod.N + 127) / 128;
   a.expert_bytes = (size_t)a.cols * G * MOE_BLOCK_BYTES;
   a.row_max = reinterpret_cast<const float*>(prod.wp + (size_t)prod.E * a.expert_bytes);
-  a.half_max = a.row_max + (size_t)prod.E * a.cols * 128;
+  a.norm_max = a.row_max + (size_t)prod.E * a.cols * 128;
   a.wait_ns = wait_limit();
   const int64_t tiles = p.max_items * a.cols;
   IM_REQUIRE(tiles < (1ll << 31), IM_UNSUPPORTED, "grouped product: too many tiles");

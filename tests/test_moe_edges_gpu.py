@@ -165,6 +165,51 @@ def test_gate_up_of_an_odd_number_of_rows_is_refused(cuda):
                         kernels.Experts(*quantised(gen, 8, 128, 64, cuda)), r)
 
 
+def test_activations_keep_their_precision_beside_outliers(cuda):
+    """A group of x a thousand times the others, which the weights leave out, and one large weight in the gate and the
+    up matrix: neither may push the other rows' activations below fp16's range."""
+    gate, up, down, x, logits = mlp_case(cuda, 40, 3, 2, 512, 128, 23)
+    x[:, :64] *= 2.0**10
+    for q in (gate, up):
+        w, s, b = q
+        s[:, :, 0], b[:, :, 0] = 0, 0
+        w[:, 7, 8:16] = 0x88888888 - 2**32  # row 7, group 1: code 8 everywhere, worth zero
+        w[:, 7, 8] = 0x8888888F - 2**32     # but 15 at one place, worth 7 scales
+        s[:, 7, 1], b[:, 7, 1] = 0.25, -2.0
+    check_mlp(x, gate, up, down, kernels.moe_route(logits, 2))
+
+
+@pytest.mark.parametrize("f", [2.0**-40, 2.0**-6, 2.0**20])
+def test_gated_mlp_of_small_and_large_rows(cuda, f):
+    gate, up, down, x, logits = mlp_case(cuda, 24, 4, 2, 256, 128, 25)
+    check_mlp(x * f, gate, up, down, kernels.moe_route(logits, 2))
+
+
+@pytest.mark.parametrize("spread", [4, 10, 16])
+def test_weight_rows_whose_groups_differ_widely(cuda, spread):
+    """Scales of a row's groups spread over 2^spread: what a group far below the row's largest loses stays within 2^-18
+    of that largest weight."""
+    gate, up, down, x, logits = mlp_case(cuda, 24, 4, 2, 256, 128, 27)
+    gen = torch.Generator(device=cuda).manual_seed(spread)
+    for q in (gate, up, down):
+        f = torch.exp2(-spread * torch.rand(q[1].shape, generator=gen, device=cuda)).to(torch.bfloat16)
+        q[1].mul_(f)
+        q[2].mul_(f)
+    check_mlp(x, gate, up, down, kernels.moe_route(logits, 2))
+
+
+@pytest.mark.parametrize("h,inter", [(64, 64), (2048, 192), (512, 1000 // 64 * 64)])
+def test_gated_mlp_at_the_edge_of_its_bound(cuda, h, inter):
+    """Every row of x, and every row of G and U, the same vector: g and u reach the bound that scales the activations,
+    and must not overflow fp16 (with the largest value at the top of a power of two)."""
+    v = 1.9375 * torch.ones((2, h), device=cuda).to(torch.bfloat16)
+    ones = lambda n, k: (torch.full((2, n, k // 8), -1, dtype=torch.int32, device=cuda),  # noqa: E731
+                         torch.full((2, n, k // 64), 0.125, dtype=torch.bfloat16, device=cuda),
+                         torch.zeros((2, n, k // 64), dtype=torch.bfloat16, device=cuda))
+    gate, up, down = ones(inter, h), ones(inter, h), ones(h, inter)
+    check_mlp(v, gate, up, down, kernels.moe_route(torch.zeros((2, 2), device=cuda), 2))
+
+
 # ---- bounded waits ----------------------------------------------------------------------------------------------
 def test_a_wait_that_runs_out_sets_the_status_and_leaves_the_gpu_usable(cuda):
     """With no time beyond the first attempts, the one tile of a product over 2^20 inputs (milliseconds) outlasts its
