@@ -577,6 +577,14 @@ class QuantModel:
         return self.forward(meta, max_kv_len=self.max_ctx, logit_rows=m)
 
 
+def layer_launches(cfg: ModelConfig, rows: int) -> int:
+    """libimspec kernel launches of one layer. With experts: qkv, attention, o, block residual, router, routing (two
+    launches beyond 64 rows), the rows' layout, two products by expert, block residual."""
+    if cfg.experts:
+        return 11 if rows > 64 else 10
+    return 7 if cfg.family == "gemma3" else 5
+
+
 def prefill_plan(lengths: list[int], step: int, budget: int) -> list[list[tuple[int, int, int]]]:
     """The forwards of a packed prefill: each a list of (prompt index, offset, count). Every prompt advances by
     chunks of `step` tokens (the chunks a one-by-one prefill cuts); a forward takes, in prompt order, the next
@@ -747,11 +755,12 @@ class SpecDecoder:
 
     def launches_per_round(self) -> int:
         """libimspec kernel launches in one round (counted from the round's structure)."""
-        def fwd(model, logits):
-            per_layer = 7 if model.cfg.family == "gemma3" else 5
-            return 1 + per_layer * model.cfg.layers + (1 if logits else 0)
+        def fwd(model, rows):
+            return 2 + layer_launches(model.cfg, rows) * model.cfg.layers
+        b, k = self.batch, self.k
         pick, accept = (1, 1) if self.sampling is None else (2, 3)  # argmax | row distributions + sample
-        return 1 + self.k * (fwd(self.draft, True) + pick) + fwd(self.target, True) + accept + 1
+        drafts = fwd(self.draft, 2 * b) + (k - 1) * fwd(self.draft, b) + k * pick
+        return 1 + drafts + fwd(self.target, b * (k + 1)) + accept + 1
 
     # ---- state ------------------------------------------------------------------------------------------
     def start(self, prompts: list[torch.Tensor], max_new: int) -> None:
@@ -1067,10 +1076,11 @@ class TreeDecoder(SpecDecoder):
                             self.stats)
 
     def launches_per_round(self) -> int:
-        def fwd(model):
-            return 2 + (7 if model.cfg.family == "gemma3" else 5) * model.cfg.layers
-        levels = len(self.branch)
-        return 1 + levels * (fwd(self.draft) + 1) + fwd(self.target) + 1 + 1 + 2 + 1
+        def fwd(model, rows):
+            return 2 + layer_launches(model.cfg, rows) * model.cfg.layers
+        b = self.batch
+        drafts = sum(fwd(self.draft, rows) + 1 for rows in [2 * b] + [b * n for n in self.counts[:-1]])
+        return 1 + drafts + fwd(self.target, b * self.rows) + 1 + 1 + 2 + 1
 
 
 def greedy_decode(model: QuantModel, prompt: torch.Tensor, max_new: int, seq: int = 0) -> list[int]:

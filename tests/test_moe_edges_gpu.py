@@ -282,3 +282,22 @@ def test_the_engine_passes_its_error_word_and_raises_when_it_is_set(cuda, monkey
             read()
     target.moe_error.zero_()
     assert dec.generate([prompt], 8) == first
+
+
+@pytest.mark.parametrize("target,draft", [("tiny-moe", "tiny-draft"), ("tiny-gemma-moe", "tiny-moe"),
+                                          ("tiny-target", "tiny-draft")])
+@pytest.mark.parametrize("batch", [1, 14])
+def test_launches_of_a_round_are_counted_with_experts(cuda, monkeypatch, target, draft, batch):
+    models = [engine.QuantModel(engine.PRESETS[name], cuda, seed=i, sigma=0.05, max_seqs=batch, max_rows=80,
+                                max_logit_rows=80, max_ctx=64) for i, name in enumerate((target, draft))]
+    dec = engine.SpecDecoder(*models, k=4, batch=batch)
+    seen, call = [], _lib.call
+
+    def counted(name, *args):
+        # products: the rows' layout and two products; a routing of more than 64 rows (argument 2): two launches
+        seen.append(3 if name == "im_moe_mlp" else 2 if name == "im_moe_route_ex" and args[2] > 64 else 1)
+        return call(name, *args)
+
+    monkeypatch.setattr(_lib, "call", counted)
+    dec.round()
+    assert sum(seen) == dec.launches_per_round()
