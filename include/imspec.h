@@ -454,6 +454,82 @@ int im_kq_gemv(int type, const void* w, const float* x, float* y, int64_t N, int
                size_t workspace_bytes, void* stream);
 size_t im_kq_workspace_bytes(int64_t K, int64_t B);
 
+/* ---- decoding over a bounded cache -------------------------------------------------------------------------
+ *
+ * No counterpart in the reference, whose caches keep every token and whose models turn whole heads. A bounded cache
+ * keeps for every kv head of every sequence the slots that matter: a token's slot is then not its position, and differs
+ * between heads. Value types: IM_BF16, IM_F16, IM_F32. Caches are [pages][Hkv][16][D], tables int32 [seqs][max_pages];
+ * weights and slot_pos are [seqs][Hkv][cap] (slot s of a head at s). Every index from device memory is checked: a row,
+ * page or slot outside its table or cache is neither read nor written.
+ *
+ * im_rope: out[m, h] = x[m, h] turned to position pos[m] (int32, or int64 with pos_64; of any size, also negative). Pair i
+ * of the first `rotary` values turns by pos * inv_freq[i] (float32, or float64 with freq_f64; rotary / 2 of them) and is
+ * multiplied by `factor`; pairs are (i, i + rotary / 2) (IM_ROPE_HALF) or (2 i, 2 i + 1) (IM_ROPE_INTERLEAVED), the other
+ * values are copied. The angle is a float64 product. inverse turns back, by the transpose: the gradient of x from
+ * that of out, and, with factor 1, the way back. x and out have their own strides (in values; a head's values are
+ * contiguous); out may be x itself with the same strides, and must not overlap it otherwise.
+ *
+ * im_rope_kv: for rows of qkv [M, (Hq + 2 Hkv) D]: q turned to q_out [M, Hq, D]; k turned and v as it is to slot row_slot[m]
+ * of table row row_seq[m], and, with slot_pos, row_pos[m] to slot_pos[row_seq[m], every head, row_slot[m]] (if below
+ * cap). Rows whose slot is outside the table (-1, say) write no cache. No two rows of a call may name one slot.
+ *
+ * im_attention_weights: im_attention_paged's attention (seq_rows, seq_slot, row_slot, window as there; no tree masks) for
+ * IM_BF16 or IM_F16 and head_dim D a multiple of 16 up to 256, which also writes every slot's attention weights,
+ *   weights_out[s, h, j] = (j < f ? weights[s, h, j] : 0) + sum over the sequence's rows and the query heads of kv head h
+ *                          of their softmax weight on slot j,  for j < min(largest row_slot + 1, max_kv_len, cap),
+ * f being the sequence's first row's slot: slots that this call is the first to see start from zero. Other weights are
+ * left alone. weights_out may be weights. Rows that see no slot (row_slot -1, say) get zeros and add nothing. Splits:
+ * multiples of keys_per_split (a multiple of 64; 0: chosen by the sizes of the call); keep it fixed and a row's bits do
+ * not depend on the launch. seq_rows is clamped to the M rows of q; rows beyond max_rows_per_seq are not computed. No two
+ * sequences may name one table row. Workspace 256-byte aligned, nothing to initialise.
+ *
+ * im_cache_evict: of the n = lengths[s] slots of every (layer, sequence, kv head), min(n, budget) stay: those whose
+ * position (slot_pos) is below `sinks` or at least seen[s] - recent, then the heaviest (weights; NaN lightest), lower
+ * slots first among equals. The i-th kept slot behind the new end moves to the i-th dropped slot before it: K, V (a slot's
+ * row_bytes of one head; any type), weight and position. weights_out and pos_out (which may be weights and slot_pos) get
+ * the slots before the new end, lengths_out [S] (may be lengths) the new length, the same for every layer and head. weights and
+ * slot_pos are [layers][S][Hkv][cap], the caches `layers` times [pages][Hkv][16][row_bytes], layer_bytes apart; n is at
+ * most min(cap, 16 max_pages). Sequences must not share the pages of a cache that is cut. sinks + recent <= budget.
+ * Workspace 16-byte aligned, nothing to initialise.
+ *
+ * im_verify_sampled: keeps or refuses drafted tokens by the target's probabilities and given random numbers. target
+ * [B * (K + 1)] rows of V (row stride target_ld; row b (K + 1) + i is the distribution of the token after draft i - 1),
+ * draft [B * K] rows (what draft i was drawn from), or NULL for drafts without a distribution; n_drafts [B] (or NULL: K).
+ * Draft i is kept iff all before it were and u_i * draft[i][d_i] < target[i][d_i] (NULL: u_i < target[i][d_i]). At the
+ * first refusal the next token is drawn from max(target - draft, 0) (NULL: target without d_i; target itself where
+ * nothing is left), after the last draft from target: the smallest token whose cumulative weight exceeds u_K times
+ * the total, u = uniforms[b * uniforms_ld ..][K + 1], in [0, 1). Products, differences and sums are float64. Values that
+ * are not positive finite numbers count as 0; a row without any weight gives token 0; a draft outside [0, V) is refused.
+ * out_tokens [B, K + 1] (kept drafts, the drawn token, then -1), out_count [B] (kept + 1).
+ */
+enum { IM_BF16 = 0, IM_F16 = 1, IM_F32 = 2 };
+enum { IM_ROPE_HALF = 0, IM_ROPE_INTERLEAVED = 1 };
+int im_rope(const void* x, int64_t row_stride, int64_t head_stride, const void* pos, int pos_64, const void* inv_freq,
+            int freq_f64, int64_t rotary, double factor, int layout, int inverse, int64_t M, int64_t H, int64_t D,
+            int dtype, void* out, int64_t out_row_stride, int64_t out_head_stride, void* stream);
+int im_rope_kv(const void* qkv, const void* inv_freq, int freq_f64, int64_t rotary, double factor, int layout,
+               const int32_t* row_pos, const int32_t* row_slot, const int32_t* row_seq, const int32_t* page_table,
+               int64_t seqs, int64_t max_pages, int64_t pages, int64_t M, int64_t Hq, int64_t Hkv, int64_t D, int dtype,
+               void* q_out, void* k_cache, void* v_cache, int32_t* slot_pos, int64_t cap, void* stream);
+size_t im_attention_weights_workspace_bytes(int64_t B, int64_t max_rows_per_seq, int64_t Hq, int64_t Hkv, int64_t D,
+                                            int64_t max_kv_len, int64_t keys_per_split);
+int im_attention_weights(const void* q, const void* k_cache, const void* v_cache, int dtype, const int32_t* page_table,
+                         int64_t seqs, int64_t max_pages, int64_t pages, const int32_t* seq_rows,
+                         const int32_t* seq_slot, const int32_t* row_slot, int64_t M, int64_t B,
+                         int64_t max_rows_per_seq, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_kv_len, int64_t keys_per_split, int64_t window,
+                         float scale, const float* weights, float* weights_out, int64_t cap, void* out, void* workspace,
+                         size_t workspace_bytes, void* stream);
+size_t im_cache_evict_workspace_bytes(int64_t layers, int64_t S, int64_t Hkv, int64_t cap, int64_t budget);
+int im_cache_evict(void* k_cache, void* v_cache, int64_t layers, int64_t layer_bytes, int64_t pages,
+                   const int32_t* page_table, int64_t max_pages, const int32_t* lengths, const int32_t* seen,
+                   const float* weights, float* weights_out, const int32_t* slot_pos, int32_t* pos_out,
+                   int32_t* lengths_out, int64_t S, int64_t Hkv, int64_t cap, int64_t row_bytes, int64_t budget,
+                   int64_t recent, int64_t sinks, void* workspace, size_t workspace_bytes, void* stream);
+int im_verify_sampled(const void* target, int64_t target_ld, const void* draft, int64_t draft_ld, int dtype,
+                      const int32_t* drafts, int64_t drafts_ld, const int32_t* n_drafts, const float* uniforms,
+                      int64_t uniforms_ld, int64_t B, int64_t K, int64_t V, int32_t* out_tokens, int32_t* out_count,
+                      void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -16,6 +16,8 @@ IM_OK, IM_UNSUPPORTED, IM_INVALID, IM_CUDA_ERROR = 0, 1, 2, 3
 EPI_STORE, EPI_RESIDUAL, EPI_SWIGLU, EPI_GEGLU = 0, 1, 2, 3
 MOE_SOFTMAX, MOE_SIGMOID, MOE_BIAS_ON_SCORE = 0, 1, 16
 QGEMM_AUTO, QGEMM_MMA, QGEMM_FMA = 0, 1, 2
+BF16, F16, F32 = 0, 1, 2
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1
 ABI_VERSION = 1
 
 _P = ctypes.c_void_p
@@ -93,6 +95,17 @@ SIGNATURES: dict[str, tuple] = {
     "im_moe_mlp": (_INT, [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _INT, _P, _P, _SZ, _P, _SZ, _P]),
     "im_block_residual": (_INT, [_P, _P, _I64, _P, _P, _P, _I64, _I64, ctypes.c_float, _P, ctypes.c_float, _INT, _I64,
                                  _I64, _P, _P, _P, _P]),
+    "im_rope": (_INT, [_P, _I64, _I64, _P, _INT, _P, _INT, _I64, ctypes.c_double, _INT, _INT, _I64, _I64, _I64, _INT, _P,
+                       _I64, _I64, _P]),
+    "im_rope_kv": (_INT, [_P, _P, _INT, _I64, ctypes.c_double, _INT, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64,
+                          _I64, _INT, _P, _P, _P, _P, _I64, _P]),
+    "im_attention_weights_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64, _I64, _I64, _I64]),
+    "im_attention_weights": (_INT, [_P, _P, _P, _INT, _P, _I64, _I64, _I64, _P, _P, _P, _I64, _I64, _I64, _I64, _I64,
+                                    _I64, _I64, _I64, _I64, ctypes.c_float, _P, _P, _I64, _P, _P, _SZ, _P]),
+    "im_cache_evict_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64, _I64]),
+    "im_cache_evict": (_INT, [_P, _P, _I64, _I64, _I64, _P, _I64, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64,
+                              _I64, _I64, _I64, _P, _SZ, _P]),
+    "im_verify_sampled": (_INT, [_P, _I64, _P, _I64, _INT, _P, _I64, _P, _P, _I64, _I64, _I64, _I64, _P, _P, _P]),
     "im_philox4x32_10": (_INT, [ctypes.c_uint64, ctypes.c_uint64, ctypes.c_uint32, ctypes.c_uint32, _P, _P]),
 }
 

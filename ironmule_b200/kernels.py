@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import math
 import threading
 
 import torch
@@ -762,6 +763,369 @@ def block_residual(y: torch.Tensor, h: torch.Tensor, eps: float, *, weights: tor
               _ptr_or_none(gate), row, col, float(residual_scale), _ptr_or_none(next_norm), float(eps), int(gemma), m, hsz,
               out.data_ptr(), _ptr_or_none(z), _ptr_or_none(out_sq), _stream(device))
     return out, z
+
+
+# ---- decoding over a bounded cache ----------------------------------------------------------------------------
+_TYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16, torch.float32: _lib.F32}
+_FLOATS = (torch.bfloat16, torch.float16, torch.float32)
+_LAYOUTS = {"half": _lib.ROPE_HALF, "interleaved": _lib.ROPE_INTERLEAVED}
+PAGE_SLOTS = 16
+
+
+def _launch(device: torch.device, name: str, *args) -> None:
+    """_lib.call with the device current, whichever is."""
+    if torch._C._cuda_getDevice() == device.index:
+        _lib.call(name, *args)
+    else:
+        with torch.cuda.device(device):
+            _lib.call(name, *args)
+
+
+def _disjoint_or_same(a: torch.Tensor, name_a: str, b: torch.Tensor, name_b: str) -> None:
+    """Refuse tensors that overlap without being one (contiguous, or strided with positive strides)."""
+    def ends(t: torch.Tensor) -> tuple[int, int]:
+        last = sum((n - 1) * st for n, st in zip(t.shape, t.stride())) if t.numel() else -1
+        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+    (a0, a1), (b0, b1) = ends(a), ends(b)
+    if a0 < b1 and b0 < a1 and not (a0 == b0 and a.shape == b.shape and a.stride() == b.stride()):
+        raise ValueError(f"{name_a} overlaps {name_b} without being the same tensor")
+
+
+def rope_frequencies(rotary: int, base: float, *, scaling: str = "none", stretch: float = 1.0, trained: int = 0,
+                     fast: float = 32.0, slow: float = 1.0,
+                     device: torch.device | str = "cuda") -> tuple[torch.Tensor, float]:
+    """(inv_freq float64 [rotary / 2], factor) for rope and rope_kv: pair i turns by base^(-2i / rotary) per position.
+    scaling for contexts `stretch` times the `trained` length: "linear" (every frequency divided by it), "ntk" (the base
+    raised so that the slowest pair's is divided by it), "yarn" (pairs of over `fast` turns over the trained length as they
+    are, of under `slow` turns divided, a ramp between; values multiplied by factor = 0.1 ln(stretch) + 1)."""
+    if rotary < 2 or rotary % 2:
+        raise ValueError(f"rotary {rotary}: an even number of values")
+    if not (base > 1.0 and math.isfinite(base)):
+        raise ValueError(f"base {base}: a finite number above 1")
+    if scaling not in ("none", "linear", "ntk", "yarn"):
+        raise ValueError(f"scaling {scaling!r}: none, linear, ntk or yarn")
+    if scaling != "none" and not (stretch >= 1.0 and math.isfinite(stretch)):
+        raise ValueError(f"stretch {stretch}: at least 1")
+    i = torch.arange(rotary // 2, dtype=torch.float64)
+    factor = 1.0
+    if scaling == "ntk":
+        if rotary < 4:
+            raise ValueError("ntk scaling needs two pairs or more")
+        base = base * stretch ** (rotary / (rotary - 2))
+    freq = base ** (-2.0 * i / rotary)
+    if scaling == "linear":
+        freq = freq / stretch
+    elif scaling == "yarn":
+        if trained < 1 or not fast > slow > 0.0:
+            raise ValueError("yarn scaling needs the trained length, and fast > slow > 0 turns")
+        pair = [rotary * math.log(trained / (turns * 2.0 * math.pi)) / (2.0 * math.log(base)) for turns in (fast, slow)]
+        low, high = max(0, math.floor(pair[0])), min(rotary - 1, math.ceil(pair[1]))
+        ramp = ((i - low) / max(high - low, 0.001)).clamp(0.0, 1.0)
+        freq = freq / stretch * ramp + freq * (1.0 - ramp)
+        factor = 0.1 * math.log(stretch) + 1.0
+    return freq.to(device), factor
+
+
+def _rope_table(inv_freq: torch.Tensor, layout: str, d: int, device: torch.device) -> tuple[int, int]:
+    """(rotary, layout) of a table checked against the head size."""
+    _check(inv_freq, "inv_freq", (torch.float32, torch.float64), device)
+    if layout not in _LAYOUTS:
+        raise ValueError(f"layout {layout!r}: half or interleaved")
+    rotary = 2 * inv_freq.numel()
+    if inv_freq.dim() != 1 or rotary > d:
+        raise ValueError(f"inv_freq {tuple(inv_freq.shape)} turns {rotary} of a head's {d} values")
+    return rotary, _LAYOUTS[layout]
+
+
+def rope(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, layout: str = "half", factor: float = 1.0,
+         inverse: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
+    """x [M, H, D] (bf16, float16 or float32; any row and head strides) turned to positions [M] (int32 or int64): pair i
+    of a head's first 2 * len(inv_freq) values by positions * inv_freq[i], times factor; the rest is copied. Pairs are
+    (i, i + half of them) or, "interleaved", (2i, 2i + 1). inverse turns back by the transpose: rope(dy, ..., inverse=True)
+    is the gradient of x. `out` may be x; a new tensor by default."""
+    if not isinstance(x, torch.Tensor) or x.device.type != "cuda" or x.dtype not in _TYPES:
+        raise TypeError("x must be a bf16, float16 or float32 CUDA tensor")
+    if x.dim() != 3 or (x.numel() and x.stride(2) != 1 and x.shape[2] > 1):
+        raise ValueError(f"x must be [M, H, D] with contiguous heads, got {tuple(x.shape)}, strides {x.stride()}")
+    m, h, d = x.shape
+    device = x.device
+    _check(positions, "positions", (torch.int32, torch.int64), device)
+    if positions.shape != (m,):
+        raise ValueError(f"positions must be [{m}], got {tuple(positions.shape)}")
+    rotary, lay = _rope_table(inv_freq, layout, d, device)
+    if out is None:
+        out = torch.empty((m, h, d), dtype=x.dtype, device=device)
+    else:
+        if not isinstance(out, torch.Tensor) or out.dtype != x.dtype or out.device != device or out.shape != x.shape:
+            raise ValueError(f"out must be a {x.dtype} tensor {tuple(x.shape)} on {device}")
+        rs, hs = out.stride(0), out.stride(1)
+        by_row = (h < 2 or hs >= d) and (m < 2 or rs >= (h - 1) * hs + d)
+        by_head = (m < 2 or rs >= d) and (h < 2 or hs >= (m - 1) * rs + d)
+        if out.numel() and ((d > 1 and out.stride(2) != 1) or not (by_row or by_head)):
+            raise ValueError(f"out must hold every head apart and contiguous, its strides are {out.stride()}")
+        _disjoint_or_same(out, "out", x, "x")
+    if x.numel():
+        _launch(device, "im_rope", x.data_ptr(), x.stride(0), x.stride(1), positions.data_ptr(),
+                int(positions.dtype == torch.int64), inv_freq.data_ptr(), int(inv_freq.dtype == torch.float64), rotary,
+                float(factor), lay, int(inverse), m, h, d, _TYPES[x.dtype], out.data_ptr(), out.stride(0), out.stride(1),
+                _stream(device))
+    return out
+
+
+def _check_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, hkv: int, d: int, dtype,
+                 device: torch.device) -> None:
+    _check(k_cache, "k_cache", (dtype,), device)
+    _check(v_cache, "v_cache", (dtype,), device)
+    if k_cache.shape != v_cache.shape or k_cache.dim() != 4 or k_cache.shape[1:] != (hkv, PAGE_SLOTS, d):
+        raise ValueError(f"caches must be [pages, {hkv}, {PAGE_SLOTS}, {d}], got {tuple(k_cache.shape)} and "
+                         f"{tuple(v_cache.shape)}")
+    _check(page_table, "page_table", (torch.int32,), device)
+    if page_table.dim() != 2:
+        raise ValueError(f"page_table must be [sequences, pages], got {tuple(page_table.shape)}")
+
+
+def _check_ints(t: torch.Tensor, name: str, n: int, device: torch.device) -> None:
+    _check(t, name, (torch.int32,), device)
+    if t.dim() != 1 or t.numel() < n:
+        raise ValueError(f"{name} must hold {n} elements, got {tuple(t.shape)}")
+
+
+def _check_slots(t: torch.Tensor, name: str, dtype, shape: tuple, device: torch.device) -> None:
+    """A [..., sequences, Hkv, cap] tensor; shape gives all but cap."""
+    _check(t, name, (dtype,), device)
+    if t.dim() != len(shape) + 1 or t.shape[:-1] != shape:
+        raise ValueError(f"{name} must be [{', '.join(map(str, shape))}, slots], got {tuple(t.shape)}")
+
+
+def rope_kv(qkv: torch.Tensor, inv_freq: torch.Tensor, row_pos: torch.Tensor, row_slot: torch.Tensor,
+            row_seq: torch.Tensor, page_table: torch.Tensor, hq: int, hkv: int, d: int, k_cache: torch.Tensor,
+            v_cache: torch.Tensor, *, layout: str = "half", factor: float = 1.0, q_out: torch.Tensor | None = None,
+            slot_pos: torch.Tensor | None = None, rows: int | None = None) -> torch.Tensor:
+    """The first `rows` rows of qkv [M, (Hq + 2 Hkv) D] (bf16, float16 or float32): q turned to its position (returned,
+    [M, Hq, D]), k turned and v written to slot row_slot of table row row_seq of the caches [pages, Hkv, 16, D], and, with
+    slot_pos (int32 [sequences, Hkv, cap]), the position to that slot of every head. Rows whose slot is outside the table
+    (-1) write no cache; no two rows may name one slot. What rope says of inv_freq, layout and factor holds."""
+    _check(qkv, "qkv", _FLOATS)
+    device = qkv.device
+    if hq < 1 or hkv < 1 or hq % hkv or d < 1:
+        raise ValueError(f"{hq} query heads, {hkv} kv heads of {d} values")
+    if qkv.dim() != 2 or qkv.shape[1] != (hq + 2 * hkv) * d:
+        raise ValueError(f"qkv must be [M, {(hq + 2 * hkv) * d}], got {tuple(qkv.shape)}")
+    m = qkv.shape[0] if rows is None else rows
+    if not 0 <= m <= qkv.shape[0]:
+        raise ValueError(f"{m} rows of {qkv.shape[0]}")
+    rotary, lay = _rope_table(inv_freq, layout, d, device)
+    for t, name in ((row_pos, "row_pos"), (row_slot, "row_slot"), (row_seq, "row_seq")):
+        _check_ints(t, name, m, device)
+    _check_cache(k_cache, v_cache, page_table, hkv, d, qkv.dtype, device)
+    cap = 0
+    if slot_pos is not None:
+        _check_slots(slot_pos, "slot_pos", torch.int32, (page_table.shape[0], hkv), device)
+        cap = slot_pos.shape[-1]
+    if q_out is None:
+        q_out = torch.empty((m, hq, d), dtype=qkv.dtype, device=device)
+    else:
+        _check(q_out, "q_out", (qkv.dtype,), device)
+        if q_out.numel() < m * hq * d:
+            raise ValueError(f"q_out needs {m * hq * d} elements")
+    if m:
+        _launch(device, "im_rope_kv", qkv.data_ptr(), inv_freq.data_ptr(), int(inv_freq.dtype == torch.float64), rotary,
+                float(factor), lay, row_pos.data_ptr(), row_slot.data_ptr(), row_seq.data_ptr(), page_table.data_ptr(),
+                page_table.shape[0], page_table.shape[1], k_cache.shape[0], m, hq, hkv, d, _TYPES[qkv.dtype],
+                q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _ptr_or_none(slot_pos), cap, _stream(device))
+    return q_out
+
+
+@functools.lru_cache(maxsize=4096)
+def attention_weights_workspace_bytes(b: int, rows: int, hq: int, hkv: int, d: int, max_kv_len: int, kps: int) -> int:
+    return int(_lib.load().im_attention_weights_workspace_bytes(b, rows, hq, hkv, d, max_kv_len, kps))
+
+
+def attention_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+                      seq_rows: torch.Tensor, row_slot: torch.Tensor, weights: torch.Tensor, *, max_rows_per_seq: int,
+                      max_kv_len: int, scale: float, keys_per_split: int = 0, window: int = 0,
+                      weights_out: torch.Tensor | None = None, out: torch.Tensor | None = None, rows: int | None = None,
+                      seq_slot: torch.Tensor | None = None) -> torch.Tensor:
+    """Paged attention of new rows, q [M, Hq, D] -> out [M, Hq, D] (bf16 or float16, D a multiple of 16 up to 256), that
+    adds up each slot's attention weight: weights (float32 [sequences, Hkv, cap], the rows of the page table) becomes, in
+    place or in weights_out, weights + the softmax weights that the sequence's rows and the kv head's query heads put on
+    the slot, for the slots up to the last row's; from the first row's slot on it starts from zero. The other arguments
+    are `attention`'s, keys_per_split 0 meaning that the call's sizes choose it."""
+    _check(q, "q", (torch.bfloat16, torch.float16))
+    device = q.device
+    if q.dim() != 3 or k_cache.dim() != 4:
+        raise ValueError(f"q must be [M, Hq, D] and the caches [pages, Hkv, 16, D], got {tuple(q.shape)}, "
+                         f"{tuple(k_cache.shape)}")
+    hq, d, hkv = q.shape[1], q.shape[2], k_cache.shape[1]
+    m = q.shape[0] if rows is None else rows
+    if not 0 <= m <= q.shape[0]:
+        raise ValueError(f"{m} rows of {q.shape[0]}")
+    if hkv < 1 or hq < 1 or hq % hkv:
+        raise ValueError(f"{hq} query heads, {hkv} kv heads")
+    _check_cache(k_cache, v_cache, page_table, hkv, d, q.dtype, device)
+    _check_ints(seq_rows, "seq_rows", 1, device)
+    b = seq_rows.numel() - 1
+    _check_ints(row_slot, "row_slot", m, device)
+    if seq_slot is not None:
+        _check_ints(seq_slot, "seq_slot", b, device)
+    elif b > page_table.shape[0]:
+        raise ValueError(f"{b} sequences, the page table has {page_table.shape[0]}")
+    _check_slots(weights, "weights", torch.float32, (page_table.shape[0], hkv), device)
+    if weights_out is None:
+        weights_out = weights
+    else:
+        _check(weights_out, "weights_out", (torch.float32,), device)
+        if weights_out.shape != weights.shape:
+            raise ValueError(f"weights_out must be {tuple(weights.shape)}, got {tuple(weights_out.shape)}")
+        _disjoint_or_same(weights_out, "weights_out", weights, "weights")
+    if out is None:
+        out = torch.empty((m, hq, d), dtype=q.dtype, device=device)
+    else:
+        _check(out, "out", (q.dtype,), device)
+        if out.numel() < m * hq * d:
+            raise ValueError(f"out needs {m * hq * d} elements")
+    if not (0 <= max_rows_per_seq and 0 <= max_kv_len and 0 <= window and 0 <= keys_per_split):
+        raise ValueError("max_rows_per_seq, max_kv_len, window and keys_per_split are not negative")
+    if b == 0 or m == 0 or max_rows_per_seq == 0:
+        return out
+    max_rows = min(max_rows_per_seq, m)
+    need = attention_weights_workspace_bytes(b, max_rows, hq, hkv, d, max(1, max_kv_len), keys_per_split)
+    ws = torch.empty(need, dtype=torch.uint8, device=device)
+    _launch(device, "im_attention_weights", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _TYPES[q.dtype],
+            page_table.data_ptr(), page_table.shape[0], page_table.shape[1], k_cache.shape[0], seq_rows.data_ptr(),
+            _ptr_or_none(seq_slot), row_slot.data_ptr(), m, b, max_rows, hq, hkv, d, max_kv_len, keys_per_split, window,
+            float(scale), weights.data_ptr(), weights_out.data_ptr(), weights.shape[-1], out.data_ptr(), ws.data_ptr(),
+            need, _stream(device))
+    return out
+
+
+@functools.lru_cache(maxsize=4096)
+def cache_evict_workspace_bytes(layers: int, s: int, hkv: int, cap: int, budget: int) -> int:
+    return int(_lib.load().im_cache_evict_workspace_bytes(layers, s, hkv, cap, budget))
+
+
+def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
+                seen: torch.Tensor, weights: torch.Tensor, slot_pos: torch.Tensor, *, budget: int, recent: int = 0,
+                sinks: int = 0, weights_out: torch.Tensor | None = None, pos_out: torch.Tensor | None = None,
+                lengths_out: torch.Tensor | None = None) -> torch.Tensor:
+    """Cut every kv head's slots to `budget`, in place, and return the new lengths (int32 [sequences]). Of the lengths[s]
+    slots of a head, those stay that hold a token below position `sinks` or among the last `recent` of the seen[s] tokens of
+    the sequence, and the ones with the largest weights (lower slots first among equals); kept slots behind the new end
+    move into the holes before it. weights (float32) and slot_pos (int32) are [sequences, Hkv, cap] and follow, in place
+    or to weights_out and pos_out. Caches [pages, Hkv, 16, D] of any type, or [layers, pages, Hkv, 16, D] with weights
+    and slot_pos [layers, sequences, Hkv, cap]: every layer of one call makes its own choice. Page tables must not share the
+    pages that are cut."""
+    if not isinstance(k_cache, torch.Tensor) or k_cache.dim() not in (4, 5):
+        raise ValueError("caches must be [pages, Hkv, 16, D] or [layers, pages, Hkv, 16, D]")
+    device, dtype = k_cache.device, k_cache.dtype
+    _check(k_cache, "k_cache", (dtype,))
+    _check(v_cache, "v_cache", (dtype,), device)
+    if v_cache.shape != k_cache.shape or k_cache.shape[-2] != PAGE_SLOTS:
+        raise ValueError(f"caches must be of one shape with {PAGE_SLOTS} slots a page, got {tuple(k_cache.shape)} and "
+                         f"{tuple(v_cache.shape)}")
+    layers = k_cache.shape[0] if k_cache.dim() == 5 else 1
+    pages, hkv, _, d = k_cache.shape[-4:]
+    _check(page_table, "page_table", (torch.int32,), device)
+    if page_table.dim() != 2:
+        raise ValueError(f"page_table must be [sequences, pages], got {tuple(page_table.shape)}")
+    s = page_table.shape[0]
+    for t, name in ((lengths, "lengths"), (seen, "seen")):
+        _check(t, name, (torch.int32,), device)
+        if t.shape != (s,):
+            raise ValueError(f"{name} must be [{s}], got {tuple(t.shape)}")
+    lead = (layers, s, hkv) if k_cache.dim() == 5 else (s, hkv)
+    _check_slots(weights, "weights", torch.float32, lead, device)
+    _check_slots(slot_pos, "slot_pos", torch.int32, lead, device)
+    if slot_pos.shape != weights.shape:
+        raise ValueError(f"slot_pos is {tuple(slot_pos.shape)}, weights {tuple(weights.shape)}")
+    outs = []
+    for t, name, like, like_name in ((weights_out, "weights_out", weights, "weights"),
+                                     (pos_out, "pos_out", slot_pos, "slot_pos")):
+        if t is None:
+            t = like
+        else:
+            _check(t, name, (like.dtype,), device)
+            if t.shape != like.shape:
+                raise ValueError(f"{name} must be {tuple(like.shape)}, got {tuple(t.shape)}")
+            _disjoint_or_same(t, name, like, like_name)
+        outs.append(t)
+    if lengths_out is None:
+        lengths_out = torch.empty((s,), dtype=torch.int32, device=device)
+    else:
+        _check(lengths_out, "lengths_out", (torch.int32,), device)
+        if lengths_out.shape != (s,):
+            raise ValueError(f"lengths_out must be [{s}], got {tuple(lengths_out.shape)}")
+    if budget < 0 or recent < 0 or sinks < 0 or recent + sinks > budget:
+        raise ValueError(f"{recent} recent and {sinks} first slots of a budget of {budget}")
+    cap = weights.shape[-1]
+    if not (layers and s and hkv and cap and d):
+        return lengths_out.zero_()
+    need = cache_evict_workspace_bytes(layers, s, hkv, cap, budget)
+    ws = torch.empty(max(need, 16), dtype=torch.uint8, device=device)
+    size = k_cache.element_size()
+    _launch(device, "im_cache_evict", k_cache.data_ptr(), v_cache.data_ptr(), layers, pages * hkv * PAGE_SLOTS * d * size,
+            pages, page_table.data_ptr(), page_table.shape[1], lengths.data_ptr(), seen.data_ptr(), weights.data_ptr(),
+            outs[0].data_ptr(), slot_pos.data_ptr(), outs[1].data_ptr(), lengths_out.data_ptr(), s, hkv, cap, d * size,
+            budget, recent, sinks, ws.data_ptr(), need, _stream(device))
+    return lengths_out
+
+
+def _check_probs(t: torch.Tensor, name: str, rows: int, device: torch.device | None) -> int:
+    """The row stride of probabilities [B, rows, V] whose rows are evenly spaced."""
+    if not isinstance(t, torch.Tensor) or t.device.type != "cuda" or t.dtype not in _TYPES:
+        raise TypeError(f"{name} must be a bf16, float16 or float32 CUDA tensor")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    b, _, v = t.shape
+    ld = t.stride(1) if rows > 1 else t.stride(0) if b > 1 else v
+    if (v > 1 and t.stride(2) != 1) or ld < v or (b > 1 and t.stride(0) != rows * ld):
+        raise ValueError(f"{name} must have evenly spaced rows of contiguous values, its strides are {t.stride()}")
+    return ld
+
+
+def verify_sampled(target_probs: torch.Tensor, draft_probs: torch.Tensor | None, drafts: torch.Tensor,
+                   uniforms: torch.Tensor, *, n_drafts: torch.Tensor | None = None, tokens: torch.Tensor | None = None,
+                   count: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Speculative sampling from probabilities and given random numbers: target_probs [B, k+1, V] and draft_probs
+    [B, k, V] (bf16, float16 or float32), drafts int32 [B, k], uniforms float32 [B, k+1] in [0, 1) -> (tokens int32
+    [B, k+1]: the kept drafts, the drawn token, then -1; count int32 [B]). Draft i is kept iff those before it are and
+    u[i] * q(d) < p(d); the token after them is drawn with u[k] from max(p - q, 0), or from p after the last draft.
+    draft_probs None: drafts without a distribution (n-gram drafts), kept iff u[i] < p(d), else drawn from p without d.
+    n_drafts int32 [B]: sequences with fewer drafts than k."""
+    if not isinstance(drafts, torch.Tensor) or drafts.dim() != 2:
+        raise ValueError("drafts must be [B, k]")
+    b, k = drafts.shape
+    if not isinstance(target_probs, torch.Tensor) or target_probs.dim() != 3 or target_probs.shape[:2] != (b, k + 1):
+        raise ValueError(f"target_probs must be [{b}, {k + 1}, V]")
+    v = target_probs.shape[2]
+    if v < 1:
+        raise ValueError("target_probs has an empty vocabulary")
+    p_ld = _check_probs(target_probs, "target_probs", k + 1, None)
+    device = target_probs.device
+    q_ld = 0
+    if draft_probs is not None:
+        if not isinstance(draft_probs, torch.Tensor) or draft_probs.shape != (b, k, v):
+            raise ValueError(f"draft_probs must be [{b}, {k}, {v}]")
+        if draft_probs.dtype != target_probs.dtype:
+            raise TypeError(f"draft_probs is {draft_probs.dtype}, target_probs {target_probs.dtype}")
+        q_ld = _check_probs(draft_probs, "draft_probs", k, device) if k else v
+    _check(drafts, "drafts", (torch.int32,), device)
+    _check(uniforms, "uniforms", (torch.float32,), device)
+    if uniforms.shape != (b, k + 1):
+        raise ValueError(f"uniforms must be [{b}, {k + 1}], got {tuple(uniforms.shape)}")
+    for t, name, shape in ((n_drafts, "n_drafts", (b,)), (tokens, "tokens", (b, k + 1)), (count, "count", (b,))):
+        if t is not None:
+            _check(t, name, (torch.int32,), device)
+            if t.shape != shape:
+                raise ValueError(f"{name} must be {list(shape)}, got {tuple(t.shape)}")
+    tokens = torch.empty((b, k + 1), dtype=torch.int32, device=device) if tokens is None else tokens
+    count = torch.empty((b,), dtype=torch.int32, device=device) if count is None else count
+    if b:
+        _launch(device, "im_verify_sampled", target_probs.data_ptr(), p_ld, _ptr_or_none(draft_probs), q_ld,
+                _TYPES[target_probs.dtype], drafts.data_ptr(), k, _ptr_or_none(n_drafts), uniforms.data_ptr(), k + 1, b, k,
+                v, tokens.data_ptr(), count.data_ptr(), _stream(device))
+    return tokens, count
 
 
 # ---- GGUF k-quants (the ggml path) ----------------------------------------------------------------------------

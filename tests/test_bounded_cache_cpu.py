@@ -1,0 +1,148 @@
+"""Decoding over a bounded cache without a GPU: frequency tables, and what the C entry points refuse."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from ironmule_b200 import _lib, kernels
+
+
+def _status(name, *args):
+    lib = _lib.load()
+    return getattr(lib, name)(*args), lib.im_last_error().decode()
+
+
+def table(rotary, base, **kw):
+    freq, factor = kernels.rope_frequencies(rotary, base, device="cpu", **kw)
+    assert freq.dtype == torch.float64 and freq.shape == (rotary // 2,)
+    return freq.tolist(), factor
+
+
+def test_frequencies():
+    plain, factor = table(8, 10000.0)
+    assert factor == 1.0 and plain == pytest.approx([1.0, 0.1, 0.01, 0.001], rel=1e-14)
+    linear, factor = table(8, 10000.0, scaling="linear", stretch=4.0)
+    assert factor == 1.0 and linear == pytest.approx([x / 4 for x in plain], rel=1e-14)
+    ntk, factor = table(8, 10000.0, scaling="ntk", stretch=4.0)
+    assert factor == 1.0 and ntk[0] == 1.0 and ntk[-1] == pytest.approx(plain[-1] / 4, rel=1e-13)
+    yarn, factor = table(64, 10000.0, scaling="yarn", stretch=8.0, trained=4096)
+    plain, _ = table(64, 10000.0)
+    assert factor == pytest.approx(0.1 * math.log(8.0) + 1.0, rel=1e-15)
+    turns = [4096 * f / (2 * math.pi) for f in plain]
+    for f, y, t in zip(plain, yarn, turns):
+        assert f / 8 * (1 - 1e-14) <= y <= f * (1 + 1e-14)
+        if t > 40.0:
+            assert y == pytest.approx(f, rel=1e-14)
+        if t < 0.75:
+            assert y == pytest.approx(f / 8, rel=1e-14)
+    assert all(a >= b for a, b in zip(yarn, yarn[1:]))
+    assert table(64, 10000.0, scaling="yarn", stretch=1.0, trained=4096) == (pytest.approx(plain, rel=1e-14), 1.0)
+
+
+@pytest.mark.parametrize("args,kw", [((0, 1e4), {}), ((7, 1e4), {}), ((8, 1.0), {}), ((8, math.inf), {}),
+                                     ((8, 1e4), {"scaling": "other"}), ((8, 1e4), {"scaling": "linear", "stretch": 0.5}),
+                                     ((2, 1e4), {"scaling": "ntk", "stretch": 2.0}),
+                                     ((8, 1e4), {"scaling": "yarn", "stretch": 2.0}),
+                                     ((8, 1e4), {"scaling": "yarn", "stretch": 2.0, "trained": 9, "fast": 1.0, "slow": 2.0})])
+def test_frequencies_refused(args, kw):
+    with pytest.raises(ValueError):
+        kernels.rope_frequencies(*args, device="cpu", **kw)
+
+
+def rope(x=256, row=32, head=16, pos=256, freq=256, rotary=8, layout=0, m=2, h=2, d=16, dtype=0, out=256):
+    return _status("im_rope", x, row, head, pos, 0, freq, 0, rotary, 1.0, layout, 0, m, h, d, dtype, out, row, head, None)
+
+
+def test_rope_refusals():
+    assert rope(m=0)[0] == _lib.IM_OK and rope(h=0)[0] == _lib.IM_OK
+    for kw, word in (({"m": -1}, "sizes"), ({"d": 0}, "sizes"), ({"layout": 2}, "layout"), ({"dtype": 3}, "type"),
+                     ({"rotary": 7}, "turn"), ({"rotary": 18}, "turn"), ({"x": None}, "null"), ({"freq": None}, "null"),
+                     ({"out": None}, "null"), ({"x": 257}, "misaligned"), ({"pos": 258}, "misaligned")):
+        rc, msg = rope(**kw)
+        assert rc == _lib.IM_INVALID and word in msg, (kw, msg)
+    assert rope(h=1 << 17)[0] == _lib.IM_UNSUPPORTED and rope(m=1 << 31)[0] == _lib.IM_UNSUPPORTED
+
+
+def rope_kv(m=2, hq=4, hkv=2, d=16, dtype=0, rotary=16, layout=0, ptr=256, slot_pos=None, cap=0):
+    return _status("im_rope_kv", ptr, 256, 0, rotary, 1.0, layout, ptr, ptr, ptr, ptr, 1, 1, 1, m, hq, hkv, d, dtype, ptr,
+                   ptr, ptr, slot_pos, cap, None)
+
+
+def test_rope_kv_refusals():
+    assert rope_kv(m=0)[0] == _lib.IM_OK
+    for kw, word in (({"hq": 3}, "sizes"), ({"m": -2}, "sizes"), ({"cap": -1}, "sizes"), ({"layout": -1}, "layout"),
+                     ({"dtype": -1}, "type"), ({"rotary": 32}, "turn"), ({"ptr": None}, "null"),
+                     ({"slot_pos": 258}, "misaligned")):
+        rc, msg = rope_kv(**kw)
+        assert rc == _lib.IM_INVALID and word in msg, (kw, msg)
+    assert rope_kv(d=8192)[0] == _lib.IM_UNSUPPORTED
+
+
+def attend(b=2, rows=1, hq=4, hkv=2, d=64, kv=100, kps=0, window=0, dtype=0, ptr=256, ws=256, size=1 << 40, m=2, cap=100):
+    return _status("im_attention_weights", ptr, ptr, ptr, dtype, ptr, 2, 7, 14, ptr, None, ptr, m, b, rows, hq, hkv, d, kv,
+                   kps, window, 1.0, ptr, ptr, cap, ptr, ws, size, None)
+
+
+def test_attention_weights_refusals():
+    assert attend(b=0)[0] == attend(rows=0)[0] == attend(m=0)[0] == _lib.IM_OK
+    for kw, word in (({"hq": 3}, "sizes"), ({"b": -1}, "sizes"), ({"window": -1}, "sizes"), ({"cap": -1}, "sizes"),
+                     ({"kps": 65}, "multiple of 64"), ({"kps": -64}, "multiple of 64"), ({"ptr": None}, "null"),
+                     ({"ptr": 264}, "aligned"), ({"ws": None}, "workspace"), ({"ws": 128}, "workspace"),
+                     ({"size": 64}, "workspace")):
+        rc, msg = attend(**kw)
+        assert rc == _lib.IM_INVALID and word in msg, (kw, msg)
+    for kw, word in (({"dtype": 2}, "type"), ({"d": 8}, "head_dim"), ({"d": 72}, "head_dim"), ({"d": 272}, "head_dim"),
+                     ({"b": 70000}, "large"), ({"kv": 1 << 31}, "large")):
+        rc, msg = attend(**kw)
+        assert rc == _lib.IM_UNSUPPORTED and word in msg, (kw, msg)
+    lib = _lib.load()
+    need = lib.im_attention_weights_workspace_bytes(2, 1, 4, 2, 64, 100, 0)
+    assert need > 0 and attend(size=need - 1)[0] == _lib.IM_INVALID
+    assert lib.im_attention_weights_workspace_bytes(0, 1, 4, 2, 64, 100, 0) == 0
+    assert lib.im_attention_weights_workspace_bytes(1, 1, 3, 2, 64, 100, 0) == 0
+
+
+def evict(layers=1, s=2, hkv=2, cap=100, row=128, budget=50, recent=0, sinks=0, ptr=256, ws=256, size=1 << 40):
+    return _status("im_cache_evict", ptr, ptr, layers, 1 << 20, 14, ptr, 7, ptr, ptr, ptr, ptr, ptr, ptr, ptr, s, hkv, cap,
+                   row, budget, recent, sinks, ws, size, None)
+
+
+def test_evict_refusals():
+    assert evict(layers=0)[0] == evict(s=0)[0] == _lib.IM_OK
+    for kw, word in (({"hkv": 0}, "sizes"), ({"cap": 0}, "sizes"), ({"budget": -1}, "sizes"), ({"sinks": -1}, "sizes"),
+                     ({"recent": 40, "sinks": 11}, "budget"), ({"recent": 51}, "budget"), ({"ptr": None}, "null"),
+                     ({"ws": None}, "workspace"), ({"ws": 8}, "workspace"), ({"size": 16}, "workspace")):
+        rc, msg = evict(**kw)
+        assert rc == _lib.IM_INVALID and word in msg, (kw, msg)
+    assert evict(cap=1 << 30)[0] == _lib.IM_UNSUPPORTED and evict(layers=1 << 30)[0] == _lib.IM_UNSUPPORTED
+    rc, msg = evict(recent=2**62, sinks=2**62, budget=2**62 + 2**61)  # a sum past 64 bits
+    assert rc == _lib.IM_INVALID and "budget" in msg
+
+
+def verify(b=2, k=3, v=50, ld=50, dtype=2, ptr=256, q=256, n=None):
+    return _status("im_verify_sampled", ptr, ld, q, ld, dtype, ptr, k, n, ptr, k + 1, b, k, v, ptr, ptr, None)
+
+
+def test_verify_refusals():
+    assert verify(b=0)[0] == _lib.IM_OK
+    for kw, word in (({"b": -1}, "sizes"), ({"v": 0}, "sizes"), ({"ld": 49}, "sizes"), ({"k": -1}, "sizes"),
+                     ({"dtype": 5}, "type"), ({"ptr": None}, "null"), ({"q": 258}, "misaligned"), ({"n": 2}, "misaligned")):
+        rc, msg = verify(**kw)
+        assert rc == _lib.IM_INVALID and word in msg, (kw, msg)
+    assert verify(b=1 << 16)[0] == _lib.IM_UNSUPPORTED and verify(k=5000)[0] == _lib.IM_UNSUPPORTED
+
+
+def test_wrappers_need_cuda_tensors():
+    x = torch.zeros((1, 1, 4))
+    i = torch.zeros((1,), dtype=torch.int32)
+    with pytest.raises(TypeError):
+        kernels.rope(x, i, torch.ones(2))
+    with pytest.raises(ValueError):
+        kernels.rope_kv(torch.zeros((1, 12)), torch.ones(2), i, i, i, i.view(1, 1), 1, 1, 4, x, x)
+    with pytest.raises(ValueError):
+        kernels.cache_evict(torch.zeros((1, 1, 16, 4)), torch.zeros((1, 1, 16, 4)), i.view(1, 1), i, i,
+                            torch.zeros((1, 1, 16)), torch.zeros((1, 1, 16), dtype=torch.int32), budget=4)
+    with pytest.raises(TypeError):
+        kernels.verify_sampled(torch.zeros((1, 1, 4)), None, torch.zeros((1, 0), dtype=torch.int32), torch.zeros((1, 1)))
