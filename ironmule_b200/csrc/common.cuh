@@ -76,6 +76,31 @@ inline int launch(const char* what, void (*kernel)(KArgs...), dim3 grid, dim3 bl
   return IM_OK;
 }
 
+// The same as thread-block clusters of `cluster` blocks along x (above 8, the kernel must allow a size that is not portable).
+template <typename... KArgs, typename... Args>
+inline int launch_cluster(const char* what, void (*kernel)(KArgs...), dim3 grid, dim3 block, int cluster, size_t smem,
+                          cudaStream_t st, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = launch_overlap() ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+  if (e != cudaSuccess) {
+    set_error("%s: %s", what, cudaGetErrorString(e));
+    return IM_CUDA_ERROR;
+  }
+  return IM_OK;
+}
+
 // ---- bf16 as raw 16-bit patterns --------------------------------------------------------------
 // Values cross the ABI as uint16_t bit patterns; arithmetic is float32 with one rounding to bf16
 // (nearest even) wherever the reference rounds.

@@ -7,7 +7,11 @@
 // bit, and sums over a vocabulary are off by 1e-13 of themselves, where float32 sums would draw another token in a
 // percent of the draws.
 //
-// Bound: HBM, one row of p and one of q a sequence.
+// Bound: HBM, one row of p and one of q a sequence; for few sequences, the chain of dependent steps (the drafts, their
+// probabilities, a row's sum, the token). A sequence is a cluster of up to 16 blocks, each with a run of the vocabulary.
+// Every block decides on the drafts for itself (a few gathers), sums its run and tells the others its total through
+// distributed shared memory; the warp that holds the target then looks for the token in its own part.
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -15,8 +19,11 @@
 
 namespace im {
 
-constexpr int VS_THREADS = 1024;
+namespace cg = cooperative_groups;
+
+constexpr int VS_THREADS = 512;
 constexpr int VS_WARPS = VS_THREADS / 32;
+constexpr int VS_CLUSTER = 16;
 
 struct VerifyArgs {
   const void* p;
@@ -49,13 +56,17 @@ __device__ __forceinline__ double vs_warp_sum(double v) {
   return v;
 }
 
+// Cluster = sequence: rank r takes tokens [r span, (r + 1) span), a warp a part of them, read 32 at a time.
 template <typename T>
-__global__ void __launch_bounds__(VS_THREADS) verify_sampled_kernel(VerifyArgs a) {
+__global__ void __launch_bounds__(VS_THREADS, 2) verify_sampled_kernel(VerifyArgs a) {
   __shared__ int first;
   __shared__ double sums[VS_WARPS];
+  __shared__ double totals[2][VS_CLUSTER];  // of the cluster's blocks, by attempt; written by them
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ranks = cluster.num_blocks(), rank = cluster.block_rank();
   pdl_wait();
   pdl_trigger();
-  const long long b = blockIdx.x;
+  const long long b = blockIdx.x / ranks;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const T* p0 = (const T*)a.p + b * (a.K + 1) * a.p_ld;
   const T* q0 = (const T*)a.q + b * a.K * a.q_ld;
@@ -63,6 +74,7 @@ __global__ void __launch_bounds__(VS_THREADS) verify_sampled_kernel(VerifyArgs a
   const float* u = a.u + b * a.u_ld;
   int n = (int)a.K;
   if (a.n_drafts) n = min(max(a.n_drafts[b], 0), (int)a.K);
+  const double u_last = u[a.K];
   if (t == 0) first = n;
   __syncthreads();
   for (int i = t; i < n; i += VS_THREADS) {
@@ -76,69 +88,115 @@ __global__ void __launch_bounds__(VS_THREADS) verify_sampled_kernel(VerifyArgs a
   const int kept = first;
   const T* p = p0 + kept * a.p_ld;
   const T* q = a.q && kept < n ? q0 + kept * a.q_ld : nullptr;
-  const long long without = !a.q && kept < n ? drafts[kept] : -1;
-  const long long span = (a.V + VS_WARPS * 32 - 1) / (VS_WARPS * 32) * 32;
-  const long long lo = warp * span, hi = min(lo + span, a.V);
-  for (int attempt = 0;; attempt++) {  // a remainder without weight is replaced by p
-    const bool whole = attempt == 1 || kept == n;
-    auto weight = [&](long long v) {
-      double w = vs_prob(p[v]);
-      if (!whole) {
-        if (q) w = fmax(w - vs_prob(q[v]), 0.0);
-        if (v == without) w = 0.0;
-      }
-      return w;
-    };
+  const int without = !a.q && kept < n ? drafts[kept] : -1;
+  const int part = (int)((a.V + ranks * VS_WARPS * 32 - 1) / (ranks * VS_WARPS * 32)) * 32;  // tokens of a warp
+  const int V = (int)a.V;
+  const long long begin = (long long)(rank * VS_WARPS + warp) * part;
+  const int lo = (int)min(begin, a.V), hi = min(lo + part, V);
+  bool whole = kept == n;
+  auto weight = [&](int v, bool all) {
+    double w = vs_prob(p[v]);
+    if (!all) {
+      if (q) w = fmax(w - vs_prob(q[v]), 0.0);
+      if (v == without) w = 0.0;
+    }
+    return w;
+  };
+  double target = 0.0, before = 0.0;
+  int owner = -1;  // the block whose run the target falls into: the first that passes it, or the last with any weight
+  for (int attempt = 0; attempt < 2; attempt++) {
     double sum = 0.0;
-    for (long long v = lo + lane; v < hi; v += 32) sum += weight(v);
+#pragma unroll 8
+    for (int v = lo + lane; v < hi; v += 32) sum += weight(v, whole);
     sum = vs_warp_sum(sum);
     if (lane == 0) sums[warp] = sum;
     __syncthreads();
+    if (warp == 0) {
+      double s = lane < VS_WARPS ? sums[lane] : 0.0;
+      s = vs_warp_sum(s);
+      if (lane < ranks) *cluster.map_shared_rank(&totals[attempt][rank], lane) = s;
+    }
+    cluster.sync();
     double total = 0.0;
-    for (int w = 0; w < VS_WARPS; w++) total += sums[w];
-    if (!(total > 0.0) && !whole) {
-      __syncthreads();
+    for (int r = 0; r < ranks; r++) total += totals[attempt][r];
+    if (!(total > 0.0) && !whole) {  // nothing is left beside q: the token comes from p
+      whole = true;
       continue;
     }
-    // the warp whose span the target falls into: the first that passes it, or the last with any weight
-    const double target = (double)u[a.K] * total;
-    double before = 0.0, at = 0.0;
-    int mine = -1;
-    for (int w = 0; w < VS_WARPS; w++) {
-      if (sums[w] > 0.0) {
-        mine = w, before = at;
-        if (at + sums[w] > target) break;
+    target = u_last * total;
+    double at = 0.0;
+    for (int r = 0; r < ranks; r++) {
+      const double s = totals[attempt][r];
+      if (s > 0.0) {
+        owner = r, before = at;
+        if (at + s > target) break;
       }
-      at += sums[w];
+      at += s;
     }
-    int token = 0;  // of a row without any weight
-    if (mine == warp) {
-      double run = before;
-      for (long long v0 = lo; v0 < hi; v0 += 32) {
-        const double w = v0 + lane < hi ? weight(v0 + lane) : 0.0;
-        double incl = w;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const double x = __shfl_up_sync(0xffffffffu, incl, o);
-          if (lane >= o) incl += x;
-        }
-        const unsigned any = __ballot_sync(0xffffffffu, w > 0.0);
-        const unsigned pass = __ballot_sync(0xffffffffu, w > 0.0 && run + incl > target);
-        if (any) token = (int)(v0 + 31 - __clz(any));
-        if (pass) {
-          token = (int)(v0 + __ffs(pass) - 1);
-          break;
-        }
-        run += __shfl_sync(0xffffffffu, incl, 31);
-      }
-    }
-    if (mine == warp || (mine < 0 && warp == 0)) {
-      int* out = a.out_tokens + b * (a.K + 1);
-      for (int i = lane; i <= a.K; i += 32) out[i] = i < kept ? drafts[i] : i == kept ? token : -1;
-      if (lane == 0) a.out_count[b] = kept + 1;
-    }
-    return;
+    break;
   }
+  if (rank != max(owner, 0)) return;
+  // within the block, then the warp, the same
+  int mine = -1;
+  double at = before;
+  for (int w = 0; w < VS_WARPS; w++) {
+    const double s = sums[w];
+    if (s > 0.0) {
+      mine = w, before = at;
+      if (at + s > target) break;
+    }
+    at += s;
+  }
+  if (warp != max(mine, 0)) return;
+  int token = 0;  // of a row without any weight
+  if (mine >= 0) {
+    // each lane takes a run of the part in order; the lane that the target falls into walks its run
+    const int each = part / 32, v0 = min(lo + lane * each, hi), v1 = min(v0 + each, hi);
+    double sum = 0.0;
+#pragma unroll 4
+    for (int v = v0; v < v1; v++) sum += weight(v, whole);
+    double incl = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double x = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += x;
+    }
+    const unsigned any = __ballot_sync(0xffffffffu, sum > 0.0);
+    const unsigned pass = __ballot_sync(0xffffffffu, sum > 0.0 && before + incl > target);
+    const int holder = pass ? __ffs(pass) - 1 : 31 - __clz(any);
+    if (lane == holder) {
+      double run = before + incl - sum;
+      for (int v = v0; v < v1; v++) {
+        const double w = weight(v, whole);
+        run += w;
+        if (w > 0.0) {
+          token = v;
+          if (run > target) break;
+        }
+      }
+    }
+    token = __shfl_sync(0xffffffffu, token, holder);
+  }
+  int* out = a.out_tokens + b * (a.K + 1);
+  for (int i = lane; i <= a.K; i += 32) out[i] = i < kept ? drafts[i] : i == kept ? token : -1;
+  if (lane == 0) a.out_count[b] = kept + 1;
+}
+
+template <typename T>
+int launch_verify_sampled(const VerifyArgs& a, int64_t B, cudaStream_t st) {
+  // blocks a sequence: enough to fill the device's two blocks an SM, of at least 2048 tokens
+  int ranks = 1;
+  while (ranks < VS_CLUSTER && B * ranks * 2 <= 296 && a.V >= ranks * 2 * 2048) ranks *= 2;
+  if (ranks > 8) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(verify_sampled_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) {
+      set_error("verify_sampled_kernel: %s", cudaGetErrorString(e));
+      return IM_CUDA_ERROR;
+    }
+  }
+  return launch_cluster("verify_sampled_kernel", verify_sampled_kernel<T>, dim3((unsigned)(B * ranks)),
+                        dim3(VS_THREADS), ranks, 0, st, a);
 }
 
 }  // namespace im
@@ -166,11 +224,8 @@ extern "C" int im_verify_sampled(const void* target, int64_t target_ld, const vo
              IM_INVALID, "im_verify_sampled: misaligned pointer");
   VerifyArgs a = {target, K ? draft : nullptr, target_ld, draft_ld, drafts, drafts_ld, n_drafts, uniforms,
                   uniforms_ld, K, V, out_tokens, out_count};
-  const dim3 grid((unsigned)B);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (dtype == IM_BF16)
-    return launch("verify_sampled_kernel", verify_sampled_kernel<__nv_bfloat16>, grid, dim3(VS_THREADS), 0, st, a);
-  if (dtype == IM_F16)
-    return launch("verify_sampled_kernel", verify_sampled_kernel<__half>, grid, dim3(VS_THREADS), 0, st, a);
-  return launch("verify_sampled_kernel", verify_sampled_kernel<float>, grid, dim3(VS_THREADS), 0, st, a);
+  if (dtype == IM_BF16) return launch_verify_sampled<__nv_bfloat16>(a, B, st);
+  if (dtype == IM_F16) return launch_verify_sampled<__half>(a, B, st);
+  return launch_verify_sampled<float>(a, B, st);
 }
