@@ -512,7 +512,7 @@ int im_rope_kv(const void* qkv, const void* inv_freq, int freq_f64, int64_t rota
                int64_t seqs, int64_t max_pages, int64_t pages, int64_t M, int64_t Hq, int64_t Hkv, int64_t D, int dtype,
                void* q_out, void* k_cache, void* v_cache, int32_t* slot_pos, int64_t cap, void* stream);
 size_t im_attention_weights_workspace_bytes(int64_t B, int64_t max_rows_per_seq, int64_t Hq, int64_t Hkv, int64_t D,
-                                            int64_t max_kv_len, int64_t keys_per_split);
+                                            int64_t max_kv_len, int64_t keys_per_split, int64_t window);
 int im_attention_weights(const void* q, const void* k_cache, const void* v_cache, int dtype, const int32_t* page_table,
                          int64_t seqs, int64_t max_pages, int64_t pages, const int32_t* seq_rows,
                          const int32_t* seq_slot, const int32_t* row_slot, int64_t M, int64_t B,

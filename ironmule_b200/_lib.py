@@ -99,7 +99,7 @@ SIGNATURES: dict[str, tuple] = {
                        _I64, _I64, _P]),
     "im_rope_kv": (_INT, [_P, _P, _INT, _I64, ctypes.c_double, _INT, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64,
                           _I64, _INT, _P, _P, _P, _P, _I64, _P]),
-    "im_attention_weights_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64, _I64, _I64, _I64]),
+    "im_attention_weights_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64]),
     "im_attention_weights": (_INT, [_P, _P, _P, _INT, _P, _I64, _I64, _I64, _P, _P, _P, _I64, _I64, _I64, _I64, _I64,
                                     _I64, _I64, _I64, _I64, ctypes.c_float, _P, _P, _I64, _P, _P, _SZ, _P]),
     "im_cache_evict_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64, _I64]),

@@ -28,6 +28,7 @@ namespace im {
 constexpr int AW_WARPS = 4;
 constexpr int AW_THREADS = AW_WARPS * 32;
 constexpr int AW_FIN_THREADS = 256;
+constexpr int AW_FIN_SLOTS = AW_FIN_THREADS * 4;
 constexpr float AW_LOG2E = 1.4426950408889634f;
 
 struct AwArgs {
@@ -52,6 +53,7 @@ struct AwArgs {
   float* scores;           // [B][Hkv][vecs][kv_pad], in log2 units
   float2* stats;           // [B][Hkv][splits][vecs]: maximum and sum
   float* parts;            // [B][Hkv][splits][vecs][d]
+  int wide_weights;        // weights and weights_out start on 16 bytes
 };
 
 // What a block knows of its sequence.
@@ -435,61 +437,113 @@ __global__ void __launch_bounds__(AW_THREADS) aw_split_kernel(AwArgs a) {
   }
 }
 
-// Joins the splits of a (sequence, kv head) and adds up its slots' weights, AW_FIN_THREADS slots a block.
+// The final maximum and 1 / sum of one vector over its splits [s0, s1), by a warp; every lane gets them.
+__device__ __forceinline__ float2 aw_total(const AwArgs& a, long long head, int v, int s0, int s1) {
+  const int lane = threadIdx.x & 31;
+  float m = -INFINITY, l = 0.f;
+  for (int s = s0 + lane; s < s1; s += 32) {
+    const float2 x = a.stats[(head * a.splits + s) * a.vecs + v];
+    const float top = fmaxf(m, x.x);
+    if (top != -INFINITY) l = l * exp2f(m - top) + x.y * exp2f(x.x - top);
+    m = top;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), l2 = __shfl_xor_sync(0xffffffffu, l, o);
+    const float top = fmaxf(m, m2);
+    if (top != -INFINITY) l = l * exp2f(m - top) + l2 * exp2f(m2 - top);
+    m = top;
+  }
+  return make_float2(m == -INFINITY ? 0.f : m, l == 0.f ? 0.f : 1.f / l);
+}
+
+// Joins the splits of a (sequence, kv head): the first a.vecs blocks of x one vector's output each, its splits dealt to the
+// warps; the others add up the weights of AW_FIN_SLOTS slots each, four a thread.
 template <typename T>
 __global__ void __launch_bounds__(AW_FIN_THREADS) aw_finish_kernel(AwArgs a) {
-  extern __shared__ float2 s_stat[];  // a vector's maximum and 1 / sum
+  extern __shared__ __align__(16) char fin[];
   pdl_wait();
   pdl_trigger();
-  const int b = blockIdx.z, h = blockIdx.y, t = threadIdx.x;
+  const int b = blockIdx.z, h = blockIdx.y, t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  constexpr int WARPS = AW_FIN_THREADS / 32;
   const AwSeq q = aw_seq(a, b);
   const int group = a.hq / a.hkv, vecs = q.rows * group;
   const long long head = (long long)b * a.hkv + h;
-  const int j_first = blockIdx.x * AW_FIN_THREADS;
-  const bool joins = blockIdx.x * AW_FIN_THREADS < vecs * a.d;
-  if (!joins && j_first >= q.n) return;
   const int lo = q.lo / 16 * 16;  // splits [s0, s1) hold a visible slot
   const int s0 = lo / a.kps, s1 = lo < q.n ? (q.n + a.kps - 1) / a.kps : s0;
-  for (int v = t; v < vecs; v += AW_FIN_THREADS) {
-    float m = -INFINITY, l = 0.f;
-    for (int s = s0; s < s1; s++) m = fmaxf(m, a.stats[(head * a.splits + s) * a.vecs + v].x);
-    for (int s = s0; s < s1; s++) {
-      const float2 x = a.stats[(head * a.splits + s) * a.vecs + v];
-      if (x.x != -INFINITY) l += exp2f(x.x - m) * x.y;
-    }
-    s_stat[v] = make_float2(m == -INFINITY ? 0.f : m, l == 0.f ? 0.f : 1.f / l);
-  }
-  __syncthreads();
-  for (int e = j_first + t; e < vecs * a.d; e += gridDim.x * AW_FIN_THREADS) {
-    const int v = e / a.d, c = e % a.d;
-    const float2 st = s_stat[v];
-    float o = 0.f;
+  if ((int)blockIdx.x < a.vecs) {
+    const int v = blockIdx.x;
+    if (v >= vecs) return;
+    const float2 st = aw_total(a, head, v, s0, s1);
+    float* part = (float*)fin;  // [WARPS][d]
+    for (int c = lane * 4; c < a.d; c += 128) {
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int s = s0; s < s1; s++) {
-      const long long at = (head * a.splits + s) * a.vecs + v;
-      const float m = a.stats[at].x;
-      const float x = a.parts[at * a.d + c];
-      if (m != -INFINITY) o = fmaf(exp2f(m - st.x), x, o);
+      for (int s = s0 + warp; s < s1; s += WARPS) {
+        const long long at = (head * a.splits + s) * a.vecs + v;
+        const float m = a.stats[at].x;
+        const float4 x = *(const float4*)(a.parts + at * a.d + c);
+        if (m != -INFINITY) {
+          const float f = exp2f(m - st.x);
+          o.x = fmaf(f, x.x, o.x), o.y = fmaf(f, x.y, o.y), o.z = fmaf(f, x.z, o.z), o.w = fmaf(f, x.w, o.w);
+        }
+      }
+      *(float4*)(part + warp * a.d + c) = o;
     }
+    __syncthreads();
     const long long row = q.row0 + v / group;
-    ((T*)a.out)[(row * a.hq + h * group + v % group) * a.d + c] = AwType<T>::down(o * st.y);
+    for (int c = t; c < a.d; c += AW_FIN_THREADS) {
+      float o = 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; w++) o += part[w * a.d + c];
+      ((T*)a.out)[(row * a.hq + h * group + v % group) * a.d + c] = AwType<T>::down(o * st.y);
+    }
+    return;
   }
   const int n = (int)min((long long)q.n, a.cap);
-  const int j = j_first + t;
+  const int j_first = (blockIdx.x - a.vecs) * AW_FIN_SLOTS;
+  if (j_first >= n) return;
+  float2* s_stat = (float2*)fin;  // [vecs]
+  for (int v = warp; v < vecs; v += WARPS) {
+    const float2 st = aw_total(a, head, v, s0, s1);
+    if (lane == 0) s_stat[v] = st;
+  }
+  __syncthreads();
+  const int j = j_first + t * 4;
   if (j >= n) return;
   const int first = a.row_slot[q.row0];
   const long long at = (q.slot * a.hkv + h) * a.cap + j;
   const float* scores = a.scores + head * a.vecs * a.kv_pad + j;
-  float sum = 0.f;
+  const bool wide = j + 3 < n && a.cap % 4 == 0 && a.wide_weights;
+  float old[4] = {0.f, 0.f, 0.f, 0.f}, sum[4] = {0.f, 0.f, 0.f, 0.f};
+  if (wide && j + 3 < first) {
+    const float4 x = *(const float4*)(a.weights + at);
+    old[0] = x.x, old[1] = x.y, old[2] = x.z, old[3] = x.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      if (j + i < n && j + i < first) old[i] = a.weights[at + i];
+  }
   for (int r = 0; r < q.rows; r++) {
-    const int slot = a.row_slot[q.row0 + r];
-    if (j > slot || (a.window > 0 && j <= slot - a.window)) continue;
+    const int slot = a.row_slot[q.row0 + r], from = a.window > 0 ? slot - a.window + 1 : 0;
+    if (j > slot || j + 3 < from) continue;
+#pragma unroll 4
     for (int g = 0; g < group; g++) {
       const float2 st = s_stat[r * group + g];
-      sum += exp2f(scores[(long long)(r * group + g) * a.kv_pad] - st.x) * st.y;
+      const float4 x = *(const float4*)(scores + (long long)(r * group + g) * a.kv_pad);
+      const float y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        if (j + i <= slot && j + i >= from) sum[i] += exp2f(y[i] - st.x) * st.y;
     }
   }
-  a.weights_out[at] = (j < first ? a.weights[at] : 0.f) + sum;
+  if (wide) {
+    *(float4*)(a.weights_out + at) = make_float4(old[0] + sum[0], old[1] + sum[1], old[2] + sum[2], old[3] + sum[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      if (j + i < n) a.weights_out[at + i] = old[i] + sum[i];
+  }
 }
 
 struct AwPlan {
@@ -500,18 +554,20 @@ struct AwPlan {
 
 static size_t aw_round(size_t n) { return (n + 255) / 256 * 256; }
 
-// How a call is cut: keys_per_split as given, or such that the (sequence, kv head, tile) groups fill the device's resident
-// blocks (two an SM) about once for a few groups, several times for many, whose lengths differ.
-static AwPlan aw_plan(int64_t B, int64_t rows, int64_t Hq, int64_t Hkv, int64_t D, int64_t kv, int64_t kps) {
+// How a call is cut: keys_per_split as given, or such that the groups (sequence, kv head, tile) fill the device's resident
+// blocks about once, or several times where there are many groups, since their lengths differ.
+static AwPlan aw_plan(int64_t B, int64_t rows, int64_t Hq, int64_t Hkv, int64_t D, int64_t kv, int64_t window,
+                      int64_t kps) {
   AwPlan p;
   p.vecs = rows * (Hq / Hkv);
   p.tiles = (int)((p.vecs + 15) / 16);
   p.kv_pad = (kv + 63) / 64 * 64;
   if (kps == 0) {
-    const int64_t groups = B * Hkv * p.tiles;
-    int64_t want = groups >= 148 ? (296 * 6 + groups - 1) / groups : 296 / groups;
+    const int64_t groups = B * Hkv * p.tiles, resident = D > 128 ? 148 : 296;
+    const int64_t seen = window > 0 && window + rows < kv ? window + rows : kv;  // slots a sequence's rows can see
+    int64_t want = groups * 2 >= resident ? (resident * 6 + groups - 1) / groups : resident / groups;
     if (want < 1) want = 1;
-    kps = ((kv + want - 1) / want + 63) / 64 * 64;
+    kps = ((seen + want - 1) / want + 63) / 64 * 64;
   }
   if (kps > p.kv_pad) kps = p.kv_pad;
   p.kps = (int)kps;
@@ -542,9 +598,10 @@ int launch_attention_weights(const AwArgs& a, int64_t B, cudaStream_t st) {
                  : a.d <= 128 ? launch_split<T, 128>(a, grid, st)
                               : launch_split<T, 256>(a, grid, st);
   if (rc != IM_OK) return rc;
-  const int chunks = (a.max_kv + AW_FIN_THREADS - 1) / AW_FIN_THREADS;
-  return launch("aw_finish_kernel", aw_finish_kernel<T>, dim3((unsigned)(chunks < 1 ? 1 : chunks), (unsigned)a.hkv, (unsigned)B),
-                dim3(AW_FIN_THREADS), sizeof(float2) * a.vecs, st, a);
+  const int chunks = (a.max_kv + AW_FIN_SLOTS - 1) / AW_FIN_SLOTS;
+  const size_t join = (size_t)AW_FIN_THREADS / 32 * a.d * 4, sums = sizeof(float2) * a.vecs;
+  return launch("aw_finish_kernel", aw_finish_kernel<T>, dim3((unsigned)(a.vecs + chunks), (unsigned)a.hkv, (unsigned)B),
+                dim3(AW_FIN_THREADS), join > sums ? join : sums, st, a);
 }
 
 }  // namespace im
@@ -552,10 +609,11 @@ int launch_attention_weights(const AwArgs& a, int64_t B, cudaStream_t st) {
 using namespace im;
 
 extern "C" size_t im_attention_weights_workspace_bytes(int64_t B, int64_t max_rows_per_seq, int64_t Hq, int64_t Hkv,
-                                                       int64_t D, int64_t max_kv_len, int64_t keys_per_split) {
-  if (B < 1 || max_rows_per_seq < 1 || Hkv < 1 || Hq < 1 || Hq % Hkv || D < 16 || max_kv_len < 1 || keys_per_split < 0)
+                                                       int64_t D, int64_t max_kv_len, int64_t keys_per_split,
+                                                       int64_t window) {
+  if (B < 1 || max_rows_per_seq < 1 || Hkv < 1 || Hq < 1 || Hq % Hkv || D < 16 || max_kv_len < 1 || keys_per_split < 0 || window < 0)
     return 0;
-  const AwPlan p = aw_plan(B, max_rows_per_seq, Hq, Hkv, D, max_kv_len, keys_per_split);
+  const AwPlan p = aw_plan(B, max_rows_per_seq, Hq, Hkv, D, max_kv_len, window, keys_per_split);
   return p.scores + p.stats + p.parts;
 }
 
@@ -584,11 +642,11 @@ extern "C" int im_attention_weights(const void* q, const void* k_cache, const vo
                  max_rows_per_seq * (Hq / Hkv) <= 4096 && max_kv_len < (1ll << 30) && window < (1ll << 30),
              IM_UNSUPPORTED, "im_attention_weights: too large");
   const int64_t kv = max_kv_len > 0 ? max_kv_len : 1;
-  const size_t need = im_attention_weights_workspace_bytes(B, max_rows_per_seq, Hq, Hkv, D, kv, keys_per_split);
+  const size_t need = im_attention_weights_workspace_bytes(B, max_rows_per_seq, Hq, Hkv, D, kv, keys_per_split, window);
   IM_REQUIRE(workspace && aligned(workspace, 256) && workspace_bytes >= need, IM_INVALID,
              "im_attention_weights: a workspace of %zu bytes needed, %zu given", need, workspace_bytes);
   AwArgs a = {};
-  const AwPlan p = aw_plan(B, max_rows_per_seq, Hq, Hkv, D, kv, keys_per_split);
+  const AwPlan p = aw_plan(B, max_rows_per_seq, Hq, Hkv, D, kv, window, keys_per_split);
   IM_REQUIRE(Hkv * p.tiles < 65536, IM_UNSUPPORTED, "im_attention_weights: too large");
   a.q = (const char*)q, a.k = (const char*)k_cache, a.v = (const char*)v_cache;
   a.page_table = page_table, a.seqs = seqs, a.max_pages = max_pages, a.pages = pages;
@@ -597,6 +655,7 @@ extern "C" int im_attention_weights(const void* q, const void* k_cache, const vo
   a.M = (int)M, a.max_rows = (int)max_rows_per_seq, a.hq = (int)Hq, a.hkv = (int)Hkv, a.d = (int)D;
   a.max_kv = (int)max_kv_len, a.kv_pad = (int)p.kv_pad, a.window = (int)window, a.scale = scale, a.out = (char*)out;
   a.kps = p.kps, a.splits = p.splits, a.tiles = p.tiles, a.vecs = (int)p.vecs;
+  a.wide_weights = aligned(weights, 16) && aligned(weights_out, 16);
   a.scores = (float*)workspace;
   a.stats = (float2*)((char*)workspace + p.scores);
   a.parts = (float*)((char*)workspace + p.scores + p.stats);

@@ -8,12 +8,13 @@
 // which token a slot holds.
 //
 // The order is that of one 32-bit key a slot: the weight's bits made monotone, NaN lowest, protected slots highest. The
-// n'-th largest key is found digit by digit (8 bits a pass over the row's keys, which lie in shared memory), the slots that
+// n'-th largest key is found digit by digit (8 bits a pass over the row's keys, which stay in registers), the slots that
 // share it are kept from the lowest slot on; the search ends early where all of a digit's slots stay.
 //
-// Bound: HBM; weights and positions read once, n' of each written, 4 rows of head_dim values a moved slot. A short row is
-// one block's, a long one a cluster's of up to 16, each with a run of its slots, which share counts through distributed
-// shared memory.
+// Bound: HBM; weights and positions read once, n' of each written, 4 rows of head_dim values a moved slot. A row is one
+// block's up to 16384 slots, and that block moves its slots too where there are rows enough to fill the device or little to
+// move; else the pairs go through the workspace to a second kernel that spreads them. Longer rows are a cluster's of up to
+// 16 blocks, which share counts through distributed shared memory.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -23,8 +24,7 @@ namespace im {
 namespace cg = cooperative_groups;
 
 constexpr int EV_CLUSTER = 16;
-constexpr int EV_RUN = 16384;       // slots of a block before a row takes another, up to EV_CLUSTER blocks
-constexpr int EV_MOST = 49152;      // slots whose keys a block can hold
+constexpr int EV_RUN = 16384;  // slots of a block at most
 constexpr int EV_MOVE_THREADS = 256;
 
 struct EvictArgs {
@@ -45,6 +45,8 @@ struct EvictArgs {
   long long cap;
   int row_bytes;  // a slot's of one head
   long long budget, recent, sinks;
+  int moves_here;  // the first kernel moves the slots too
+  int lengths_here;  // and writes lengths_out, which is not lengths
   int* moves;  // [rows]
   int* holes;  // [rows][most]
   int* movers;
@@ -63,11 +65,10 @@ __device__ __forceinline__ uint32_t ev_key(float w, int pos, long long sinks, lo
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-// Sums x over the block's warps before this one, and over all (warps <= 32); every thread gets both.
+// Sums of x over the block's warps before this one, and over all; x is the same in a warp's lanes.
 template <int WARPS>
 __device__ __forceinline__ int2 ev_before(int x, int* scratch) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  __syncthreads();
   if (lane == 0) scratch[warp] = x;
   __syncthreads();
   int v = lane < WARPS ? scratch[lane] : 0, before = lane < warp ? v : 0;
@@ -79,15 +80,63 @@ __device__ __forceinline__ int2 ev_before(int x, int* scratch) {
   return make_int2(before, v);
 }
 
-// Which slots of a row stay, and the pairs (hole, mover). A cluster a row, a run of `run` slots a block, whose warps
-// each walk a part of it in order.
-template <int WARPS>
-__global__ void __launch_bounds__(WARPS * 32, 2) evict_select_kernel(EvictArgs a) {
-  constexpr int THREADS = WARPS * 32;
-  extern __shared__ uint32_t keys[];
+// Up to 32 moves of one row by a warp: each lane has one move's slots; the warp then copies their rows together, BYTES a
+// lane, K's and V's chunks of a move side by side, BATCH loads in flight a lane.
+template <int BYTES, int BATCH>
+__device__ __forceinline__ void ev_move(const EvictArgs& a, long long row, int moves, int to, int from) {
+  const int head = (int)(row % a.hkv), seq = (int)(row / a.hkv % a.seqs), lane = threadIdx.x & 31;
+  const int* table = a.page_table + seq * a.max_pages;
+  const long long layer = row / a.hkv / a.seqs * a.layer_bytes;
+  const int chunks = a.row_bytes / BYTES;  // of K, and of V
+  long long dst = 0, src = -1;
+  if (lane < moves) {
+    const long long to_page = table[to / 16], from_page = table[from / 16];
+    a.weights_out[row * a.cap + to] = a.weights[row * a.cap + from];
+    a.pos_out[row * a.cap + to] = a.pos[row * a.cap + from];
+    if (to_page >= 0 && to_page < a.pages && from_page >= 0 && from_page < a.pages) {
+      dst = layer + ((to_page * a.hkv + head) * 16 + to % 16) * a.row_bytes;
+      src = layer + ((from_page * a.hkv + head) * 16 + from % 16) * a.row_bytes;
+    }
+  }
+  const int work = moves * 2 * chunks;
+  for (int c0 = 0; c0 < work; c0 += 32 * BATCH) {
+    uint4 x[BATCH];
+    char* at[BATCH];
+#pragma unroll
+    for (int i = 0; i < BATCH; i++) {
+      const int c = c0 + i * 32 + lane;
+      const int move = c / (2 * chunks), part = c - move * 2 * chunks;
+      const long long here = __shfl_sync(0xffffffffu, src, move & 31);
+      const long long there = __shfl_sync(0xffffffffu, dst, move & 31);
+      at[i] = nullptr;
+      if (c < work && here >= 0) {
+        const bool is_k = part < chunks;
+        const long long off = (long long)(is_k ? part : part - chunks) * BYTES;
+        char* cache = is_k ? a.k : a.v;
+        at[i] = cache + there + off;
+        if (BYTES == 16) x[i] = *(const uint4*)(cache + here + off);
+        else x[i].x = *(const unsigned char*)(cache + here + off);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < BATCH; i++) {
+      if (at[i]) {
+        if (BYTES == 16) *(uint4*)at[i] = x[i];
+        else *(unsigned char*)at[i] = (unsigned char)x[i].x;
+      }
+    }
+  }
+}
+
+// Which slots of a row stay, the pairs (hole, mover), and the moves where they are not left to the second kernel. A cluster
+// a row; a warp has up to 32 * ITEMS slots in order, its lanes' keys in registers.
+template <int THREADS, int ITEMS, int BLOCKS, int BYTES>
+__global__ void __launch_bounds__(THREADS, BLOCKS) evict_select_kernel(EvictArgs a) {
+  constexpr int WARPS = THREADS / 32;
+  extern __shared__ int pairs[];     // holes, then movers, where the moves are made here
   __shared__ unsigned hist[2][256];  // by turns: a block may count its next digit while others still read this one
-  __shared__ unsigned s_digit, s_need, s_all;
-  __shared__ int scratch[32];
+  __shared__ unsigned s_digit[2], s_need[2], s_all[2];
+  __shared__ int scratch[2][32];
   __shared__ int3 shared_counts;  // this block's ties, holes, movers, for the others
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = cluster.num_blocks(), rank = cluster.block_rank();
@@ -98,34 +147,39 @@ __global__ void __launch_bounds__(WARPS * 32, 2) evict_select_kernel(EvictArgs a
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const int n = ev_length(a, seq);
   const int left = (int)min((long long)n, a.budget);
-  // lengths_out may be lengths: it is written here only where nothing is ever cut, else by the second kernel
-  if (a.most <= 0 && t == 0 && rank == 0 && row < (long long)a.seqs * a.hkv && row % a.hkv == 0) a.lengths_out[seq] = left;
+  if (a.lengths_here && t == 0 && rank == 0 && row < (long long)a.seqs * a.hkv && row % a.hkv == 0)
+    a.lengths_out[seq] = left;
   const float* w = a.weights + row * a.cap;
   const int* pos = a.pos + row * a.cap;
   float* wo = a.weights_out + row * a.cap;
   int* po = a.pos_out + row * a.cap;
   if (n <= left || left == 0) {  // the whole cluster
-    if (t == 0 && rank == 0) a.moves[row] = 0;
+    if (!a.moves_here && t == 0 && rank == 0) a.moves[row] = 0;
     for (int s = rank * THREADS + t; s < left; s += ranks * THREADS) wo[s] = w[s], po[s] = pos[s];
     return;
   }
   const long long recent_from = (long long)a.seen[seq] - a.recent;
-  const int run = ((n + ranks - 1) / ranks + 31) / 32 * 32;
-  const int begin = min(n, rank * run), count = min(n, begin + run) - begin;
-#pragma unroll 4
-  for (int s = t; s < count; s += THREADS) keys[s] = ev_key(w[begin + s], pos[begin + s], a.sinks, recent_from);
+  const int items = (n + ranks * THREADS - 1) / (ranks * THREADS);  // at most ITEMS
+  const int first = (rank * WARPS + warp) * 32 * items + lane;      // this lane's slots: 32 apart
+  uint32_t key[ITEMS];
+#pragma unroll
+  for (int i = 0; i < ITEMS; i++) {
+    const int s = first + 32 * i;
+    key[i] = i < items && s < n ? ev_key(w[s], pos[s], a.sinks, recent_from) : 0u;
+  }
   for (int i = t; i < 512; i += THREADS) hist[0][i] = 0;
+  const int mine = first - lane < n ? min(items, (n - first + 31) / 32) : 0;  // slots of this lane (may be 0)
   __syncthreads();
   // the left-th largest key, and how many of those that share its digits stay
   uint32_t border = 0, mask = 0;
   unsigned need = (unsigned)left;
   bool all = false;  // all of them stay
   for (int shift = 24; shift >= 0 && !all; shift -= 8) {
-    unsigned* h = hist[shift >> 3 & 1];
-    for (int s = t; s < count; s += THREADS) {
-      const uint32_t k = keys[s];
-      if ((k & mask) == border) atomicAdd(&h[k >> shift & 255], 1u);
-    }
+    const int turn = shift >> 3 & 1;
+    unsigned* h = hist[turn];
+#pragma unroll
+    for (int i = 0; i < ITEMS; i++)
+      if (i < mine && (key[i] & mask) == border) atomicAdd(&h[key[i] >> shift & 255], 1u);
     if (ranks > 1) cluster.sync();
     else __syncthreads();
     if (warp == 0) {  // eight digits a lane, from the highest down
@@ -149,28 +203,24 @@ __global__ void __launch_bounds__(WARPS * 32, 2) evict_select_kernel(EvictArgs a
       if (above < need && need <= above + sum) {  // one lane
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-          if (above < need && need <= above + c[i]) {
-            s_digit = 255 - lane * 8 - i, s_need = need - above, s_all = c[i] == need - above;
-          }
+          if (above < need && need <= above + c[i])
+            s_digit[turn] = 255 - lane * 8 - i, s_need[turn] = need - above, s_all[turn] = c[i] == need - above;
           above += c[i];
         }
       }
     }
-    // the other counts are clear before the next digit: nobody reads them since the cluster met
-    for (int i = t; i < 256; i += THREADS) hist[(shift >> 3 & 1) ^ 1][i] = 0;
+    // the other counts are clear before the next digit: nobody reads them since the blocks met
+    for (int i = t; i < 256; i += THREADS) hist[turn ^ 1][i] = 0;
     __syncthreads();
-    border |= s_digit << shift, mask |= 255u << shift, need = s_need, all = s_all != 0;
-    __syncthreads();
+    border |= s_digit[turn] << shift, mask |= 255u << shift, need = s_need[turn], all = s_all[turn] != 0;
   }
   // keys of the same digits as the border's: all stay, or the first `need` in slot order
-  const int part = ((count + WARPS - 1) / WARPS + 31) / 32 * 32;
-  const int lo = min(count, warp * part), hi = min(count, lo + part);
   const unsigned under = (1u << lane) - 1;
   int ties = 0;
   if (!all) {
-    for (int s0 = lo; s0 < hi; s0 += 32)
-      ties += __popc(__ballot_sync(0xffffffffu, s0 + lane < hi && keys[s0 + lane] == border));
-    const int2 x = ev_before<WARPS>(ties, scratch);
+#pragma unroll
+    for (int i = 0; i < ITEMS; i++) ties += __popc(__ballot_sync(0xffffffffu, i < mine && key[i] == border));
+    const int2 x = ev_before<WARPS>(ties, scratch[0]);
     ties = x.x;
     if (ranks > 1) {
       if (t == 0) shared_counts.x = x.y;
@@ -178,123 +228,108 @@ __global__ void __launch_bounds__(WARPS * 32, 2) evict_select_kernel(EvictArgs a
       for (int r = 0; r < rank; r++) ties += cluster.map_shared_rank(&shared_counts, r)->x;
     }
   }
+  unsigned kept = 0;  // of this lane's slots
   int holes = 0, movers = 0;
-  const int ties_first = ties;
-  for (int pass = 0; pass < 2; pass++) {
-    ties = ties_first;
-    for (int s0 = lo; s0 < hi; s0 += 32) {
-      const int at = s0 + lane, s = begin + at;
-      const uint32_t k = at < hi ? keys[at] : 0u;
-      bool kept;
-      if (all) {
-        kept = at < hi && (k & mask) >= border;
-      } else {
-        const unsigned tie = __ballot_sync(0xffffffffu, at < hi && k == border);
-        kept = at < hi && (k > border || (k == border && ties + __popc(tie & under) < (int)need));
-        ties += __popc(tie);
-      }
-      const unsigned hole = __ballot_sync(0xffffffffu, at < hi && s < left && !kept);
-      const unsigned mover = __ballot_sync(0xffffffffu, kept && s >= left);
-      if (pass) {
-        if (hole >> lane & 1) a.holes[row * a.most + holes + __popc(hole & under)] = s;
-        if (mover >> lane & 1) a.movers[row * a.most + movers + __popc(mover & under)] = s;
-        if (kept && s < left) wo[s] = w[s], po[s] = pos[s];
-      }
-      holes += __popc(hole), movers += __popc(mover);
+#pragma unroll
+  for (int i = 0; i < ITEMS; i++) {
+    bool k;
+    if (all) {
+      k = i < mine && (key[i] & mask) >= border;
+    } else {
+      const unsigned tie = __ballot_sync(0xffffffffu, i < mine && key[i] == border);
+      k = i < mine && (key[i] > border || (key[i] == border && ties + __popc(tie & under) < (int)need));
+      ties += __popc(tie);
     }
-    if (pass) break;
-    const int2 h = ev_before<WARPS>(holes, scratch), v = ev_before<WARPS>(movers, scratch);
-    holes = h.x, movers = v.x;
-    int total = h.y;
-    if (ranks > 1) {
-      if (t == 0) shared_counts.y = h.y, shared_counts.z = v.y;
-      cluster.sync();
-      total = 0;
-      for (int r = 0; r < ranks; r++) {
-        const int3 c = *cluster.map_shared_rank(&shared_counts, r);
-        if (r < rank) holes += c.y, movers += c.z;
-        total += c.y;
-      }
-      cluster.sync();  // nobody leaves while its counts are read
+    const int s = first + 32 * i;
+    if (k) kept |= 1u << i;
+    holes += __popc(__ballot_sync(0xffffffffu, i < mine && s < left && !k));
+    movers += __popc(__ballot_sync(0xffffffffu, k && s >= left));
+  }
+  const int2 both = ev_before<WARPS>(holes | movers << 16, scratch[1]);  // a block's are under 2^15 each
+  holes = both.x & 0xffff, movers = both.x >> 16;
+  int total = both.y & 0xffff;
+  if (ranks > 1) {
+    if (t == 0) shared_counts.y = total, shared_counts.z = both.y >> 16;
+    cluster.sync();
+    total = 0;
+    for (int r = 0; r < ranks; r++) {
+      const int3 c = *cluster.map_shared_rank(&shared_counts, r);
+      if (r < rank) holes += c.y, movers += c.z;
+      total += c.y;
     }
+    cluster.sync();  // nobody leaves while its counts are read
+  }
+  const bool copies = a.weights_out != a.weights || a.pos_out != a.pos;
+  int* hole_list = a.moves_here ? pairs : a.holes + row * a.most;
+  int* mover_list = a.moves_here ? pairs + a.most : a.movers + row * a.most;
+#pragma unroll
+  for (int i = 0; i < ITEMS; i++) {
+    const int s = first + 32 * i;
+    const bool k = kept >> i & 1;
+    const unsigned hole = __ballot_sync(0xffffffffu, i < mine && s < left && !k);
+    const unsigned mover = __ballot_sync(0xffffffffu, k && s >= left);
+    if (hole >> lane & 1) hole_list[holes + __popc(hole & under)] = s;
+    if (mover >> lane & 1) mover_list[movers + __popc(mover & under)] = s;
+    if (k && s < left && copies) wo[s] = w[s], po[s] = pos[s];
+    holes += __popc(hole), movers += __popc(mover);
+  }
+  if (!a.moves_here) {
     if (t == 0 && rank == 0) a.moves[row] = total;
+    return;
+  }
+  __syncthreads();
+  for (int i0 = warp * 32; i0 < total; i0 += THREADS) {
+    const int moves = min(32, total - i0);
+    ev_move<BYTES, 4>(a, row, moves, lane < moves ? pairs[i0 + lane] : 0, lane < moves ? pairs[a.most + i0 + lane] : 0);
   }
 }
 
-// A slot's K, V, weight and position to its new place. A warp takes 32 moves: each lane finds one move's places, then the
-// warp copies their rows, BYTES a lane, K's and V's chunks of a move side by side.
+// The moves of all rows from the workspace, and the lengths, which nobody reads any more.
 template <int BYTES>
 __global__ void __launch_bounds__(EV_MOVE_THREADS, 3) evict_move_kernel(EvictArgs a) {
   pdl_wait();
   pdl_trigger();
   const long long row = blockIdx.x;
-  const int head = (int)(row % a.hkv), seq = (int)(row / a.hkv % a.seqs);
-  const int count = a.moves[row];
-  const int lane = threadIdx.x & 31;
-  if (blockIdx.y == 0 && threadIdx.x == 0 && row < (long long)a.seqs * a.hkv && head == 0)
+  const int seq = (int)(row / a.hkv % a.seqs), lane = threadIdx.x & 31;
+  if (!a.lengths_here && blockIdx.y == 0 && threadIdx.x == 0 && row < (long long)a.seqs * a.hkv && row % a.hkv == 0)
     a.lengths_out[seq] = (int)min((long long)ev_length(a, seq), a.budget);
-  const int* table = a.page_table + seq * a.max_pages;
-  const long long layer = row / a.hkv / a.seqs * a.layer_bytes;
-  const int chunks = a.row_bytes / BYTES;  // of K, and of V
+  if (a.moves_here) return;
+  const int count = a.moves[row];
   for (int i0 = (blockIdx.y * (EV_MOVE_THREADS / 32) + threadIdx.x / 32) * 32; i0 < count;
        i0 += gridDim.y * EV_MOVE_THREADS) {
     const int moves = min(32, count - i0);
-    long long dst = 0, src = -1;
-    if (lane < moves) {
-      const int to = a.holes[row * a.most + i0 + lane], from = a.movers[row * a.most + i0 + lane];
-      const long long to_page = table[to / 16], from_page = table[from / 16];
-      a.weights_out[row * a.cap + to] = a.weights[row * a.cap + from];
-      a.pos_out[row * a.cap + to] = a.pos[row * a.cap + from];
-      if (to_page >= 0 && to_page < a.pages && from_page >= 0 && from_page < a.pages) {
-        dst = layer + ((to_page * a.hkv + head) * 16 + to % 16) * a.row_bytes;
-        src = layer + ((from_page * a.hkv + head) * 16 + from % 16) * a.row_bytes;
-      }
-    }
-    const int work = moves * 2 * chunks;
-    constexpr int BATCH = BYTES == 16 ? 8 : 4;  // loads in flight a lane
-    for (int c0 = 0; c0 < work; c0 += 32 * BATCH) {
-      uint4 x[BATCH];
-      char* to[BATCH];
-#pragma unroll
-      for (int i = 0; i < BATCH; i++) {
-        const int c = c0 + i * 32 + lane;
-        const int move = c / (2 * chunks), part = c - move * 2 * chunks;
-        const long long from = __shfl_sync(0xffffffffu, src, move & 31);
-        const long long there = __shfl_sync(0xffffffffu, dst, move & 31);
-        to[i] = nullptr;
-        if (c < work && from >= 0) {
-          const bool is_k = part < chunks;
-          const long long off = (long long)(is_k ? part : part - chunks) * BYTES;
-          char* cache = is_k ? a.k : a.v;
-          to[i] = cache + there + off;
-          if (BYTES == 16) x[i] = *(const uint4*)(cache + from + off);
-          else x[i].x = *(const unsigned char*)(cache + from + off);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < BATCH; i++) {
-        if (to[i]) {
-          if (BYTES == 16) *(uint4*)to[i] = x[i];
-          else *(unsigned char*)to[i] = (unsigned char)x[i].x;
-        }
-      }
-    }
+    ev_move<BYTES, BYTES == 16 ? 8 : 4>(a, row, moves, lane < moves ? a.holes[row * a.most + i0 + lane] : 0,
+                                        lane < moves ? a.movers[row * a.most + i0 + lane] : 0);
   }
 }
 
-template <int WARPS>
+template <int THREADS, int ITEMS, int BLOCKS, int BYTES>
 int launch_evict_select(const EvictArgs& a, long long rows, int ranks, cudaStream_t st) {
-  const long long run = ((a.cap + ranks - 1) / ranks + 31) / 32 * 32;
-  const int smem = (int)(run * 4);
-  cudaError_t e = cudaFuncSetAttribute(evict_select_kernel<WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e == cudaSuccess && ranks > 8)
-    e = cudaFuncSetAttribute(evict_select_kernel<WARPS>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  auto* kernel = evict_select_kernel<THREADS, ITEMS, BLOCKS, BYTES>;
+  const int smem = a.moves_here && a.most > 0 ? (int)(2 * a.most * 4) : 0;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess && ranks > 8) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e != cudaSuccess) {
     set_error("evict_select_kernel: %s", cudaGetErrorString(e));
     return IM_CUDA_ERROR;
   }
-  return launch_cluster("evict_select_kernel", evict_select_kernel<WARPS>, dim3((unsigned)(rows * ranks)),
-                        dim3(WARPS * 32), ranks, smem, st, a);
+  return launch_cluster("evict_select_kernel", kernel, dim3((unsigned)(rows * ranks)), dim3(THREADS), ranks, smem, st, a);
+}
+
+template <int BYTES>
+int launch_evict(EvictArgs& a, long long rows, cudaStream_t st) {
+  int ranks = 1;
+  while ((long long)ranks * EV_RUN < a.cap) ranks *= 2;
+  a.moves_here = ranks == 1 && (rows >= 148 || a.most <= 512);
+  a.lengths_here = a.lengths_out != a.lengths;
+  const int rc = a.cap <= 2048   ? launch_evict_select<256, 8, 4, BYTES>(a, rows, ranks, st)
+                 : a.cap <= 4096 ? launch_evict_select<512, 8, 2, BYTES>(a, rows, ranks, st)
+                 : a.cap <= 8192 ? launch_evict_select<512, 16, 2, BYTES>(a, rows, ranks, st)
+                                 : launch_evict_select<1024, 16, 1, BYTES>(a, rows, ranks, st);
+  if (rc != IM_OK || (a.moves_here && a.lengths_here)) return rc;
+  const long long chunks = a.moves_here || a.most <= 0 ? 1 : (a.most + EV_MOVE_THREADS - 1) / EV_MOVE_THREADS;
+  return launch("evict_move_kernel", evict_move_kernel<BYTES>,
+                dim3((unsigned)rows, (unsigned)(chunks < 1024 ? chunks : 1024)), dim3(EV_MOVE_THREADS), 0, st, a);
 }
 
 static long long evict_most(int64_t cap, int64_t budget) { return budget < cap - budget ? budget : cap - budget; }
@@ -327,25 +362,20 @@ extern "C" int im_cache_evict(void* k_cache, void* v_cache, int64_t layers, int6
                  lengths_out,
              IM_INVALID, "im_cache_evict: null pointer");
   const size_t need = im_cache_evict_workspace_bytes(layers, S, Hkv, cap, budget);
-  IM_REQUIRE(need > 0 && cap <= (int64_t)EV_CLUSTER * EV_MOST && row_bytes < (1 << 20), IM_UNSUPPORTED,
-             "im_cache_evict: rows of %lld slots (up to %d), or too many of them", (long long)cap, EV_CLUSTER * EV_MOST);
+  IM_REQUIRE(need > 0 && cap <= EV_CLUSTER * EV_RUN && row_bytes < (1 << 20), IM_UNSUPPORTED,
+             "im_cache_evict: rows of %lld slots (up to %d), or too many of them", (long long)cap, EV_CLUSTER * EV_RUN);
   IM_REQUIRE(workspace && aligned(workspace, 16) && workspace_bytes >= need, IM_INVALID,
              "im_cache_evict: a workspace of %zu bytes needed, %zu given", need, workspace_bytes);
   const long long rows = layers * S * Hkv, most = evict_most(cap, budget);
-  EvictArgs a = {(char*)k_cache, (char*)v_cache, layer_bytes, pages, page_table, max_pages, lengths, seen,
-                 weights, weights_out, slot_pos, pos_out, lengths_out, (int)S, (int)Hkv, cap, (int)row_bytes,
-                 budget, recent, sinks, (int*)workspace, nullptr, nullptr, most};
-  a.holes = a.moves + rows, a.movers = a.holes + (most > 0 ? rows * most : 0);
+  EvictArgs a = {};
+  a.k = (char*)k_cache, a.v = (char*)v_cache, a.layer_bytes = layer_bytes, a.pages = pages;
+  a.page_table = page_table, a.max_pages = max_pages, a.lengths = lengths, a.seen = seen;
+  a.weights = weights, a.weights_out = weights_out, a.pos = slot_pos, a.pos_out = pos_out, a.lengths_out = lengths_out;
+  a.seqs = (int)S, a.hkv = (int)Hkv, a.cap = cap, a.row_bytes = (int)row_bytes;
+  a.budget = budget, a.recent = recent, a.sinks = sinks;
+  a.most = most > 0 ? most : 0, a.moves = (int*)workspace, a.holes = a.moves + rows, a.movers = a.holes + rows * a.most;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  // blocks a row: one up to EV_RUN slots, more for longer rows (and so few rows that the device has room for them)
-  int ranks = 1;
-  while (ranks < EV_CLUSTER && (cap > (int64_t)ranks * EV_MOST || (cap > (int64_t)ranks * EV_RUN && rows * ranks < 296)))
-    ranks *= 2;
-  const int rc = cap <= 4096 ? launch_evict_select<8>(a, rows, ranks, st) : launch_evict_select<16>(a, rows, ranks, st);
-  if (rc != IM_OK || most <= 0) return rc;
-  const long long chunks = (most + EV_MOVE_THREADS - 1) / EV_MOVE_THREADS;
-  const dim3 grid((unsigned)rows, (unsigned)(chunks < 1024 ? chunks : 1024));
   if (row_bytes % 16 == 0 && aligned(k_cache, 16) && aligned(v_cache, 16) && layer_bytes % 16 == 0)
-    return launch("evict_move_kernel", evict_move_kernel<16>, grid, dim3(EV_MOVE_THREADS), 0, st, a);
-  return launch("evict_move_kernel", evict_move_kernel<1>, grid, dim3(EV_MOVE_THREADS), 0, st, a);
+    return launch_evict<16>(a, rows, st);
+  return launch_evict<1>(a, rows, st);
 }

@@ -6,8 +6,9 @@
 // float32 product would be off by 0.06 rad. What is left of it is within 2^-26 quarter turns, so c and s are float32
 // exact to an ulp or two wherever the position is. Rotations are float32, rounded once to the rows' type.
 //
-// Bound: HBM, every value read and written once. One block a row (several for few rows), so a row's c and s are worked
-// out once (R/2 of them) and used by every head from shared memory; values move 16 bytes a thread.
+// Bound: HBM, every value read and written once. A block takes a row (a part of one where rows are few, several where they
+// are short), works c and s out once (R/2 of them a row) and uses them for every head from shared memory; the first values
+// are on their way meanwhile. Values move 16 bytes a thread.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -16,6 +17,8 @@
 namespace im {
 
 constexpr int RP_THREADS = 256;
+constexpr int RP_ROWS = 16;   // rows a block at most
+constexpr int RP_BATCH = 2;   // units a thread has on their way
 
 struct RopeArgs {
   const char* x;            // rows
@@ -28,6 +31,8 @@ struct RopeArgs {
   int rotary, d;
   int heads;           // heads of a row that the launch walks (rope_kv: q, k and v heads)
   int heads_per_block;
+  int rows_per_block;
+  long long rows;
   char* out;
   long long o_row, o_head;
   // the serving form
@@ -86,108 +91,152 @@ __device__ __forceinline__ float2 rope_turn(double p, double f, float factor, bo
   return make_float2(factor * c, factor * s);
 }
 
-// One block: `heads_per_block` heads of one row. VEC values a load; a unit is two loads of a half-layout pair of runs, or
-// one load of neighbouring pairs, or one load of the part that is copied.
+// One block: `heads_per_block` heads of `rows_per_block` rows. VEC values a load; a unit is two loads of a half-layout pair
+// of runs, or one load of neighbouring pairs, or one load of the part that is copied (VEC 1: one pair, or one value).
 template <typename T, int VEC, bool KV>
 __global__ void __launch_bounds__(RP_THREADS) rope_kernel(RopeArgs a) {
-  extern __shared__ float2 turn[];  // [R / 2]
+  typedef RopeVec<T, VEC> V;
+  extern __shared__ float2 turn[];       // [rows][R / 2]
+  __shared__ long long s_cache[RP_ROWS];  // where a row's keys and values go: head 0's, in values; -1: nowhere
   pdl_wait();
   pdl_trigger();
-  const long long m = blockIdx.x;
+  const int t = threadIdx.x;
+  const long long m0 = (long long)blockIdx.x * a.rows_per_block;
+  const int rows = (int)min((long long)a.rows_per_block, a.rows - m0);
+  const int h0 = blockIdx.y * a.heads_per_block, heads = min(a.heads, h0 + a.heads_per_block) - h0;
   const int pairs = a.rotary / 2;
-  const double p = a.pos64 ? (double)((const long long*)a.pos)[m] : (double)((const int*)a.pos)[m];
-  for (int i = threadIdx.x; i < pairs; i += RP_THREADS) {
-    const double f = a.freq64 ? ((const double*)a.freq)[i] : (double)((const float*)a.freq)[i];
+  const int turned = a.interleaved && VEC > 1 ? a.rotary / VEC : pairs / VEC;
+  const int units = turned + (a.d - a.rotary) / VEC, row_units = heads * units;
+  const int total = rows * row_units;
+  // exact for numbers under 2^22
+  const float per_row = 1.f / row_units, per_head = 1.f / units;
+  auto place = [&](int idx, int& r, int& h, int& u) {
+    r = (int)((idx + 0.5f) * per_row);
+    const int rest = idx - r * row_units;
+    h = (int)((rest + 0.5f) * per_head);
+    u = rest - h * units;
+    h += h0;
+  };
+  V v[RP_BATCH], w[RP_BATCH];
+  auto load = [&](int idx0) {
+    if constexpr (VEC > 1) {  // single values are read where they are turned
+#pragma unroll
+      for (int i = 0; i < RP_BATCH; i++) {
+        const int idx = idx0 + i * RP_THREADS;
+        if (idx < total) {
+          int r, h, u;
+          place(idx, r, h, u);
+          const T* src = (const T*)a.x + (m0 + r) * a.x_row + h * a.x_head;
+          if (u >= turned) {
+            v[i] = *(const V*)(src + a.rotary + (u - turned) * VEC);
+          } else {
+            v[i] = *(const V*)(src + u * VEC);
+            if (!a.interleaved) w[i] = *(const V*)(src + u * VEC + pairs);
+          }
+        }
+      }
+    }
+  };
+  load(t);
+  for (int i = t; i < rows * pairs; i += RP_THREADS) {
+    const int r = i / pairs, pair = i - r * pairs;
+    const double p = a.pos64 ? (double)((const long long*)a.pos)[m0 + r] : (double)((const int*)a.pos)[m0 + r];
+    const double f = a.freq64 ? ((const double*)a.freq)[pair] : (double)((const float*)a.freq)[pair];
     turn[i] = rope_turn(p, f, (float)a.factor, a.inverse != 0);
   }
-  // where this row's keys and values go; rows without a slot of the cache are rotated, and written nowhere
-  long long cache_row = -1;  // of head 0, in values; heads are 16 D apart
-  long long seq = 0, slot = -1;
-  if (KV) {
-    slot = a.row_slot[m];
-    seq = a.row_seq[m];
+  if (KV && t < rows) {  // rows without a slot of the cache are turned, and written nowhere
+    const long long slot = a.row_slot[m0 + t], seq = a.row_seq[m0 + t];
+    long long at = -1;
     if (slot >= 0 && slot < a.max_pages * 16 && seq >= 0 && seq < a.seqs) {
       const long long page = a.page_table[seq * a.max_pages + slot / 16];
-      if (page >= 0 && page < a.pages) cache_row = (page * a.hkv * 16 + slot % 16) * a.d;
+      if (page >= 0 && page < a.pages) at = (page * a.hkv * 16 + slot % 16) * a.d;
+    }
+    s_cache[t] = at;
+    if (a.slot_pos && at >= 0 && slot < a.cap && blockIdx.y == 0) {
+      const int pos = ((const int*)a.pos)[m0 + t];
+      for (int h = 0; h < a.hkv; h++) a.slot_pos[(seq * a.hkv + h) * a.cap + slot] = pos;
     }
   }
   __syncthreads();
-  const int h0 = blockIdx.y * a.heads_per_block;
-  const int h1 = min(a.heads, h0 + a.heads_per_block);
-  const int turned = a.interleaved && VEC > 1 ? a.rotary / VEC : pairs / VEC;
-  const int units = turned + (a.d - a.rotary) / VEC;
-  for (int idx = threadIdx.x; idx < (h1 - h0) * units; idx += RP_THREADS) {
-    const int h = h0 + idx / units, u = idx % units;
-    const T* src = (const T*)a.x + m * a.x_row + h * a.x_head;
-    T* dst;
-    bool turns = true;
-    if (!KV || h < a.hq) {
-      dst = (T*)a.out + m * a.o_row + h * a.o_head;
-    } else {
-      const int kh = h < a.hq + a.hkv ? h - a.hq : h - a.hq - a.hkv;
-      turns = h < a.hq + a.hkv;
-      if (cache_row < 0) continue;
-      dst = (T*)(turns ? a.k_cache : a.v_cache) + cache_row + (long long)kh * 16 * a.d;
-    }
-    typedef RopeVec<T, VEC> V;
-    if (u >= turned) {
-      const int at = a.rotary + (u - turned) * VEC;
-      *(V*)(dst + at) = *(const V*)(src + at);
-    } else if (VEC == 1) {
-      const int at = a.interleaved ? 2 * u : u, to = a.interleaved ? at + 1 : at + pairs;
-      if (turns) {
-        const float2 t = turn[u];
-        const float x = RopeType<T>::up(src[at]), y = RopeType<T>::up(src[to]);
-        dst[at] = RopeType<T>::down(fmaf(x, t.x, -(y * t.y)));
-        dst[to] = RopeType<T>::down(fmaf(x, t.y, y * t.x));
+  for (int idx0 = t; idx0 < total; idx0 += RP_BATCH * RP_THREADS) {
+    if (idx0 != t) load(idx0);
+#pragma unroll
+    for (int i = 0; i < RP_BATCH; i++) {
+      const int idx = idx0 + i * RP_THREADS;
+      if (idx >= total) continue;
+      int r, h, u;
+      place(idx, r, h, u);
+      T* dst;
+      bool turns = true;
+      if (!KV || h < a.hq) {
+        dst = (T*)a.out + (m0 + r) * a.o_row + h * a.o_head;
       } else {
-        const T v = src[at], w = src[to];
-        dst[at] = v;
-        dst[to] = w;
+        turns = h < a.hq + a.hkv;
+        if (s_cache[r] < 0) continue;
+        dst = (T*)(turns ? a.k_cache : a.v_cache) + s_cache[r] + (long long)(turns ? h - a.hq : h - a.hq - a.hkv) * 16 * a.d;
       }
-    } else if (a.interleaved) {
-      V v = *(const V*)(src + u * VEC);
-      if (turns) {
-#pragma unroll
-        for (int e = 0; e + 1 < VEC; e += 2) {
-          const float2 t = turn[(u * VEC + e) / 2];
-          const float x = RopeType<T>::up(v.v[e]), y = RopeType<T>::up(v.v[e + 1]);
-          v.v[e] = RopeType<T>::down(fmaf(x, t.x, -(y * t.y)));
-          v.v[e + 1] = RopeType<T>::down(fmaf(x, t.y, y * t.x));
+      const float2* c = turn + r * pairs;
+      if (VEC == 1) {
+        const T* src = (const T*)a.x + (m0 + r) * a.x_row + h * a.x_head;
+        if (u >= turned) {
+          dst[a.rotary + u - turned] = src[a.rotary + u - turned];
+          continue;
         }
-      }
-      *(V*)(dst + u * VEC) = v;
-    } else {
-      const int at = u * VEC;
-      V v = *(const V*)(src + at), w = *(const V*)(src + at + pairs);
-      if (turns) {
-#pragma unroll
-        for (int e = 0; e < VEC; e++) {
-          const float2 t = turn[at + e];
-          const float x = RopeType<T>::up(v.v[e]), y = RopeType<T>::up(w.v[e]);
-          v.v[e] = RopeType<T>::down(fmaf(x, t.x, -(y * t.y)));
-          w.v[e] = RopeType<T>::down(fmaf(x, t.y, y * t.x));
+        const int at = a.interleaved ? 2 * u : u, to = a.interleaved ? at + 1 : at + pairs;
+        const T x = src[at], y = src[to];
+        if (turns) {
+          const float fx = RopeType<T>::up(x), fy = RopeType<T>::up(y);
+          dst[at] = RopeType<T>::down(fmaf(fx, c[u].x, -(fy * c[u].y)));
+          dst[to] = RopeType<T>::down(fmaf(fx, c[u].y, fy * c[u].x));
+        } else {
+          dst[at] = x;
+          dst[to] = y;
         }
+      } else if (u >= turned) {
+        *(V*)(dst + a.rotary + (u - turned) * VEC) = v[i];
+      } else if (a.interleaved) {
+        if (turns) {
+#pragma unroll
+          for (int e = 0; e + 1 < VEC; e += 2) {
+            const float2 k = c[(u * VEC + e) / 2];
+            const float x = RopeType<T>::up(v[i].v[e]), y = RopeType<T>::up(v[i].v[e + 1]);
+            v[i].v[e] = RopeType<T>::down(fmaf(x, k.x, -(y * k.y)));
+            v[i].v[e + 1] = RopeType<T>::down(fmaf(x, k.y, y * k.x));
+          }
+        }
+        *(V*)(dst + u * VEC) = v[i];
+      } else {
+        if (turns) {
+#pragma unroll
+          for (int e = 0; e < VEC; e++) {
+            const float2 k = c[u * VEC + e];
+            const float x = RopeType<T>::up(v[i].v[e]), y = RopeType<T>::up(w[i].v[e]);
+            v[i].v[e] = RopeType<T>::down(fmaf(x, k.x, -(y * k.y)));
+            w[i].v[e] = RopeType<T>::down(fmaf(x, k.y, y * k.x));
+          }
+        }
+        *(V*)(dst + u * VEC) = v[i];
+        *(V*)(dst + u * VEC + pairs) = w[i];
       }
-      *(V*)(dst + at) = v;
-      *(V*)(dst + at + pairs) = w;
     }
   }
-  if (KV && a.slot_pos && cache_row >= 0 && slot < a.cap && blockIdx.y == 0)
-    for (int h = threadIdx.x; h < a.hkv; h += RP_THREADS)
-      a.slot_pos[(seq * a.hkv + h) * a.cap + slot] = ((const int*)a.pos)[m];
 }
 
 template <typename T, bool KV>
 int launch_rope(RopeArgs& a, long long M, bool vec, cudaStream_t st) {
-  // few rows: their heads are spread over several blocks, so that one row's are not one block's latency
-  int blocks_y = 1;
+  constexpr int WIDE = 16 / sizeof(T);
+  const int n = vec ? WIDE : 1;
+  const int units = (a.interleaved && vec ? a.rotary / n : a.rotary / 2 / n) + (a.d - a.rotary) / n;
+  // few rows: their heads are spread over several blocks, so that one row's are not one block's latency; many short ones:
+  // several a block, so that its threads have a unit or two each
+  int blocks_y = 1, rows = 1;
   while (M * blocks_y < 148 && blocks_y * 4 < a.heads) blocks_y *= 2;
+  while (rows < RP_ROWS && rows * 2 * a.heads * units <= RP_BATCH * RP_THREADS && M >= rows * 2 * 592) rows *= 2;
+  a.rows = M, a.rows_per_block = rows;
   a.heads_per_block = (a.heads + blocks_y - 1) / blocks_y;
   blocks_y = (a.heads + a.heads_per_block - 1) / a.heads_per_block;
-  const dim3 grid((unsigned)M, (unsigned)blocks_y);
-  const size_t smem = sizeof(float2) * (a.rotary / 2);
-  constexpr int WIDE = 16 / sizeof(T);
+  const dim3 grid((unsigned)((M + rows - 1) / rows), (unsigned)blocks_y);
+  const size_t smem = sizeof(float2) * rows * (a.rotary / 2);
   if (vec) return launch("rope_kernel", rope_kernel<T, WIDE, KV>, grid, dim3(RP_THREADS), smem, st, a);
   return launch("rope_kernel", rope_kernel<T, 1, KV>, grid, dim3(RP_THREADS), smem, st, a);
 }

@@ -24,6 +24,7 @@ namespace cg = cooperative_groups;
 constexpr int VS_THREADS = 512;
 constexpr int VS_WARPS = VS_THREADS / 32;
 constexpr int VS_CLUSTER = 16;
+constexpr int VS_LEFT = 2048;  // weights looked through at a time for the token
 
 struct VerifyArgs {
   const void* p;
@@ -39,16 +40,19 @@ struct VerifyArgs {
   int* out_count;
 };
 
-__device__ __forceinline__ double vs_value(float v) { return v; }
-__device__ __forceinline__ double vs_value(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ double vs_value(__half v) { return __half2float(v); }
+__device__ __forceinline__ float vs_value(float v) { return v; }
+__device__ __forceinline__ float vs_value(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float vs_value(__half v) { return __half2float(v); }
 
 // A probability, or 0 where it is none.
+__device__ __forceinline__ float vs_clean(float v) { return v > 0.f && v < INFINITY ? v : 0.f; }
 template <typename T>
-__device__ __forceinline__ double vs_prob(T v) {
-  const double d = vs_value(v);
-  return d > 0.0 && d < __longlong_as_double(0x7ff0000000000000ll) ? d : 0.0;
+__device__ __forceinline__ float vs_prob(T v) {
+  return vs_clean(vs_value(v));
 }
+
+// What is left of p beside q: exact in float64 but for the last bit.
+__device__ __forceinline__ double vs_left(float p, float q) { return p > q ? (double)p - (double)q : 0.0; }
 
 __device__ __forceinline__ double vs_warp_sum(double v) {
 #pragma unroll
@@ -57,11 +61,17 @@ __device__ __forceinline__ double vs_warp_sum(double v) {
 }
 
 // Cluster = sequence: rank r takes tokens [r span, (r + 1) span), a warp a part of them, read 32 at a time.
-template <typename T>
+template <typename T, int VEC>
+struct alignas(sizeof(T) * VEC) VsVec {
+  T v[VEC];
+};
+
+template <typename T, bool WIDE>
 __global__ void __launch_bounds__(VS_THREADS, 2) verify_sampled_kernel(VerifyArgs a) {
   __shared__ int first;
   __shared__ double sums[VS_WARPS];
   __shared__ double totals[2][VS_CLUSTER];  // of the cluster's blocks, by attempt; written by them
+  extern __shared__ double left[];          // the weights of the part that holds the token
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = cluster.num_blocks(), rank = cluster.block_rank();
   pdl_wait();
@@ -80,34 +90,49 @@ __global__ void __launch_bounds__(VS_THREADS, 2) verify_sampled_kernel(VerifyArg
   for (int i = t; i < n; i += VS_THREADS) {
     const long long d = drafts[i];
     const bool inside = d >= 0 && d < a.V;
-    const double p = inside ? vs_prob(p0[i * a.p_ld + d]) : 0.0;
-    const double q = !a.q ? 1.0 : inside ? vs_prob(q0[i * a.q_ld + d]) : 0.0;
-    if (!((double)u[i] * q < p)) atomicMin(&first, i);
+    const float p = inside ? vs_prob(p0[i * a.p_ld + d]) : 0.f;
+    const float q = !a.q ? 1.f : inside ? vs_prob(q0[i * a.q_ld + d]) : 0.f;
+    if (!((double)u[i] * (double)q < (double)p)) atomicMin(&first, i);
   }
   __syncthreads();
   const int kept = first;
   const T* p = p0 + kept * a.p_ld;
   const T* q = a.q && kept < n ? q0 + kept * a.q_ld : nullptr;
   const int without = !a.q && kept < n ? drafts[kept] : -1;
-  const int part = (int)((a.V + ranks * VS_WARPS * 32 - 1) / (ranks * VS_WARPS * 32)) * 32;  // tokens of a warp
-  const int V = (int)a.V;
+  constexpr int VEC = WIDE ? 16 / (int)sizeof(T) : 1, STEP = 32 * VEC;
+  const int part = (int)((a.V + ranks * VS_WARPS * STEP - 1) / (ranks * VS_WARPS * STEP)) * STEP;  // tokens of a warp
   const long long begin = (long long)(rank * VS_WARPS + warp) * part;
-  const int lo = (int)min(begin, a.V), hi = min(lo + part, V);
+  const int lo = (int)min(begin, a.V), hi = (int)min((long long)lo + part, a.V);
   bool whole = kept == n;
-  auto weight = [&](int v, bool all) {
-    double w = vs_prob(p[v]);
-    if (!all) {
-      if (q) w = fmax(w - vs_prob(q[v]), 0.0);
-      if (v == without) w = 0.0;
-    }
-    return w;
-  };
   double target = 0.0, before = 0.0;
   int owner = -1;  // the block whose run the target falls into: the first that passes it, or the last with any weight
   for (int attempt = 0; attempt < 2; attempt++) {
+    const bool beside = !whole && q != nullptr;
     double sum = 0.0;
-#pragma unroll 8
-    for (int v = lo + lane; v < hi; v += 32) sum += weight(v, whole);
+    constexpr int BATCH = !WIDE ? 8 : sizeof(T) == 4 ? 4 : 2;  // loads in flight a lane, of p and of q each
+    for (int v0 = lo; v0 < hi; v0 += STEP * BATCH) {
+      VsVec<T, VEC> pv[BATCH], qv[BATCH];
+#pragma unroll
+      for (int i = 0; i < BATCH; i++) {
+        const int v = v0 + i * STEP + lane * VEC;
+        if (v < hi) {
+          pv[i] = *(const VsVec<T, VEC>*)(p + v);
+          if (beside) qv[i] = *(const VsVec<T, VEC>*)(q + v);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < BATCH; i++) {
+        const int v = v0 + i * STEP + lane * VEC;
+        if (v < hi) {
+#pragma unroll
+          for (int e = 0; e < VEC; e++) {
+            float x = vs_prob(pv[i].v[e]);
+            if (beside) sum += vs_left(x, vs_prob(qv[i].v[e]));
+            else sum += !whole && v + e == without ? 0.0 : (double)x;
+          }
+        }
+      }
+    }
     sum = vs_warp_sum(sum);
     if (lane == 0) sums[warp] = sum;
     __syncthreads();
@@ -150,32 +175,49 @@ __global__ void __launch_bounds__(VS_THREADS, 2) verify_sampled_kernel(VerifyArg
   if (warp != max(mine, 0)) return;
   int token = 0;  // of a row without any weight
   if (mine >= 0) {
-    // each lane takes a run of the part in order; the lane that the target falls into walks its run
-    const int each = part / 32, v0 = min(lo + lane * each, hi), v1 = min(v0 + each, hi);
-    double sum = 0.0;
-#pragma unroll 4
-    for (int v = v0; v < v1; v++) sum += weight(v, whole);
-    double incl = sum;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const double x = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += x;
-    }
-    const unsigned any = __ballot_sync(0xffffffffu, sum > 0.0);
-    const unsigned pass = __ballot_sync(0xffffffffu, sum > 0.0 && before + incl > target);
-    const int holder = pass ? __ffs(pass) - 1 : 31 - __clz(any);
-    if (lane == holder) {
-      double run = before + incl - sum;
-      for (int v = v0; v < v1; v++) {
-        const double w = weight(v, whole);
-        run += w;
-        if (w > 0.0) {
-          token = v;
-          if (run > target) break;
-        }
+    // the part's weights once more, all of them in flight; then each lane sums a run of them, and the lane whose run holds
+    // the target walks it
+    const bool beside = !whole && q != nullptr;
+    bool found = false;
+    for (int v0 = lo; v0 < hi && !found; v0 += VS_LEFT) {
+      const int size = min(VS_LEFT, hi - v0);
+      __syncwarp();
+#pragma unroll 8
+      for (int i = lane; i < size; i += 32) {
+        const int v = v0 + i;
+        const float x = vs_prob(p[v]);
+        left[i] = beside ? vs_left(x, vs_prob(q[v])) : !whole && v == without ? 0.0 : (double)x;
       }
+      __syncwarp();
+      const int each = ((size + 31) / 32) | 1;  // odd: lanes' runs start in different banks
+      const int i0 = min(size, lane * each), i1 = min(size, i0 + each);
+      double sum = 0.0;
+      for (int i = i0; i < i1; i++) sum += left[i];
+      double incl = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double x = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += x;
+      }
+      const unsigned any = __ballot_sync(0xffffffffu, sum > 0.0);
+      const unsigned pass = __ballot_sync(0xffffffffu, sum > 0.0 && before + incl > target);
+      if (any) {  // the first run that passes the target, else the last with any weight
+        const int holder = pass ? __ffs(pass) - 1 : 31 - __clz(any);
+        if (lane == holder) {
+          double run = before + incl - sum;
+          for (int i = i0; i < i1; i++) {
+            run += left[i];
+            if (left[i] > 0.0) {
+              token = v0 + i;
+              if (run > target) break;
+            }
+          }
+        }
+        token = __shfl_sync(0xffffffffu, token, holder);
+      }
+      before += __shfl_sync(0xffffffffu, incl, 31);
+      found = pass != 0;
     }
-    token = __shfl_sync(0xffffffffu, token, holder);
   }
   int* out = a.out_tokens + b * (a.K + 1);
   for (int i = lane; i <= a.K; i += 32) out[i] = i < kept ? drafts[i] : i == kept ? token : -1;
@@ -187,16 +229,19 @@ int launch_verify_sampled(const VerifyArgs& a, int64_t B, cudaStream_t st) {
   // blocks a sequence: enough to fill the device's two blocks an SM, of at least 2048 tokens
   int ranks = 1;
   while (ranks < VS_CLUSTER && B * ranks * 2 <= 296 && a.V >= ranks * 2 * 2048) ranks *= 2;
+  // 16-byte loads where every row starts on 16 bytes and is whole
+  const int n = 16 / sizeof(T);
+  const bool wide = aligned(a.p, 16) && aligned(a.q, 16) && a.p_ld % n == 0 && a.q_ld % n == 0 && a.V % n == 0;
+  auto* kernel = wide ? verify_sampled_kernel<T, true> : verify_sampled_kernel<T, false>;
   if (ranks > 8) {
-    const cudaError_t e =
-        cudaFuncSetAttribute(verify_sampled_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) {
       set_error("verify_sampled_kernel: %s", cudaGetErrorString(e));
       return IM_CUDA_ERROR;
     }
   }
-  return launch_cluster("verify_sampled_kernel", verify_sampled_kernel<T>, dim3((unsigned)(B * ranks)),
-                        dim3(VS_THREADS), ranks, 0, st, a);
+  return launch_cluster("verify_sampled_kernel", kernel, dim3((unsigned)(B * ranks)), dim3(VS_THREADS), ranks,
+                        VS_LEFT * sizeof(double), st, a);
 }
 
 }  // namespace im

@@ -938,8 +938,8 @@ def rope_kv(qkv: torch.Tensor, inv_freq: torch.Tensor, row_pos: torch.Tensor, ro
 
 
 @functools.lru_cache(maxsize=4096)
-def attention_weights_workspace_bytes(b: int, rows: int, hq: int, hkv: int, d: int, max_kv_len: int, kps: int) -> int:
-    return int(_lib.load().im_attention_weights_workspace_bytes(b, rows, hq, hkv, d, max_kv_len, kps))
+def _attention_weights_workspace(b: int, rows: int, hq: int, hkv: int, d: int, kv: int, kps: int, window: int) -> int:
+    return int(_lib.load().im_attention_weights_workspace_bytes(b, rows, hq, hkv, d, kv, kps, window))
 
 
 def attention_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
@@ -990,7 +990,7 @@ def attention_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     if b == 0 or m == 0 or max_rows_per_seq == 0:
         return out
     max_rows = min(max_rows_per_seq, m)
-    need = attention_weights_workspace_bytes(b, max_rows, hq, hkv, d, max(1, max_kv_len), keys_per_split)
+    need = _attention_weights_workspace(b, max_rows, hq, hkv, d, max(1, max_kv_len), keys_per_split, window)
     ws = torch.empty(need, dtype=torch.uint8, device=device)
     _launch(device, "im_attention_weights", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _TYPES[q.dtype],
             page_table.data_ptr(), page_table.shape[0], page_table.shape[1], k_cache.shape[0], seq_rows.data_ptr(),
@@ -1001,7 +1001,7 @@ def attention_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
 
 
 @functools.lru_cache(maxsize=4096)
-def cache_evict_workspace_bytes(layers: int, s: int, hkv: int, cap: int, budget: int) -> int:
+def _evict_workspace(layers: int, s: int, hkv: int, cap: int, budget: int) -> int:
     return int(_lib.load().im_cache_evict_workspace_bytes(layers, s, hkv, cap, budget))
 
 
@@ -1061,7 +1061,7 @@ def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.
     cap = weights.shape[-1]
     if not (layers and s and hkv and cap and d):
         return lengths_out.zero_()
-    need = cache_evict_workspace_bytes(layers, s, hkv, cap, budget)
+    need = _evict_workspace(layers, s, hkv, cap, budget)
     ws = torch.empty(max(need, 16), dtype=torch.uint8, device=device)
     size = k_cache.element_size()
     _launch(device, "im_cache_evict", k_cache.data_ptr(), v_cache.data_ptr(), layers, pages * hkv * PAGE_SLOTS * d * size,

@@ -98,10 +98,10 @@ def test_attention_weights_refusals():
         rc, msg = attend(**kw)
         assert rc == _lib.IM_UNSUPPORTED and word in msg, (kw, msg)
     lib = _lib.load()
-    need = lib.im_attention_weights_workspace_bytes(2, 1, 4, 2, 64, 100, 0)
+    need = lib.im_attention_weights_workspace_bytes(2, 1, 4, 2, 64, 100, 0, 0)
     assert need > 0 and attend(size=need - 1)[0] == _lib.IM_INVALID
-    assert lib.im_attention_weights_workspace_bytes(0, 1, 4, 2, 64, 100, 0) == 0
-    assert lib.im_attention_weights_workspace_bytes(1, 1, 3, 2, 64, 100, 0) == 0
+    assert lib.im_attention_weights_workspace_bytes(0, 1, 4, 2, 64, 100, 0, 0) == 0
+    assert lib.im_attention_weights_workspace_bytes(1, 1, 3, 2, 64, 100, 0, 0) == 0
 
 
 def evict(layers=1, s=2, hkv=2, cap=100, row=128, budget=50, recent=0, sinks=0, ptr=256, ws=256, size=1 << 40):
