@@ -6,16 +6,18 @@
 //
 // Bound: HBM, K and V of every visible slot read once (2 * 2 D bytes a slot and kv head).
 //
-// First kernel (aw_split_kernel): a block takes one split of a (sequence, kv head) and up to 16 of its (row, query head)
-// vectors, one row each of the warp MMA's m16. Its four warps take the split's pages in turn, each with a ring of pages of
-// its own in shared memory (asynchronous copies, no barrier between warps), a running maximum and sum and a 16 x D
-// accumulator in registers; they are joined once at the split's end. With one query group of 4 to 16 vectors the products
-// are under a tenth of what mma.sync gives, so tcgen05's tiles of 64 rows and more would only add work. Scores go to
-// the workspace in float32 (4 bytes a vector and slot beside 4 D of K and V): the weights need the final maximum and sum.
+// First kernel (aw_split_kernel): a block takes one split of a (sequence, kv head) and a tile of its (row, query head)
+// vectors. Its four warps (two of wide heads) take the split's pages in turn, each with a ring of pages of its own in shared memory
+// (asynchronous copies, no barrier between warps), a running maximum and sum and a D x vectors accumulator in registers;
+// they are joined once at the split's end. The products are transposed, so that the few vectors are the warp MMA's n = 8
+// (one or two of them) and slots and head values its m = 16: S^T = K Q^T, out^T = V^T P^T. With Q as the m = 16 rows, half
+// and more of the products would be of rows that are not there, and at 16 cycles each they would take half of a
+// page's time; tcgen05's tiles of 64 rows and more would add more of that. Scores go to the workspace in float32 (4 bytes
+// a vector and slot beside 4 D of K and V): the weights need the final maximum and sum.
 // Second kernel (aw_finish_kernel): joins the splits, and adds up exp2(s - max) / sum slot by slot.
 //
 // Weights that meet v are two numbers of the cache's type, high part and rest (16 bits and more of each weight are kept);
-// in float16 they are scaled by 2^14 first, so that weights down to 2^-28 of the largest are whole numbers' worth. Masked
+// in float16 they are scaled by 2^14 first, so that weights down to 2^-28 of the largest are not subnormal. Masked
 // slots never reach a row: behind the last visible slot v is zeroed on its way in; between rows of one call a page is
 // checked for values that are not finite, and if it has any its products are done one by one.
 #include <cuda_bf16.h>
@@ -25,8 +27,6 @@
 
 namespace im {
 
-constexpr int AW_WARPS = 4;
-constexpr int AW_THREADS = AW_WARPS * 32;
 constexpr int AW_FIN_THREADS = 256;
 constexpr int AW_FIN_SLOTS = AW_FIN_THREADS * 4;
 constexpr float AW_LOG2E = 1.4426950408889634f;
@@ -48,15 +48,16 @@ struct AwArgs {
   int window;
   float scale;
   char* out;
-  int kps, splits, tiles;  // keys a split, splits of max_kv, tiles of 16 vectors
+  int kps, splits, tiles;  // keys a split, splits of max_kv, tiles of 8 or 16 vectors
   int vecs;                // max_rows * Hq / Hkv
   float* scores;           // [B][Hkv][vecs][kv_pad], in log2 units
   float2* stats;           // [B][Hkv][splits][vecs]: maximum and sum
   float* parts;            // [B][Hkv][splits][vecs][d]
+  int joins, join_warps;   // blocks of the second kernel that join outputs, warps a job of theirs
   int wide_weights;        // weights and weights_out start on 16 bytes
 };
 
-// What a block knows of its sequence.
+// What a block knows of its sequence: first its rows and table row, then, from the rows' slots, what they see.
 struct AwSeq {
   int row0, rows;       // its rows that the call computes
   long long slot;       // its page-table row (-1: none)
@@ -69,21 +70,36 @@ __device__ __forceinline__ AwSeq aw_seq(const AwArgs& a, int b) {
   s.rows = max(0, min(min(a.seq_rows[b + 1], a.M) - s.row0, a.max_rows));
   s.slot = a.seq_slot ? a.seq_slot[b] : b;
   if (s.slot < 0 || s.slot >= a.seqs) s.slot = -1;
+  return s;
+}
+
+// By a whole warp.
+__device__ __forceinline__ void aw_span(const AwArgs& a, AwSeq& s) {
   int top = -1, low = 0x7fffffff;
-  for (int r = 0; r < s.rows; r++) {
+  for (int r = threadIdx.x & 31; r < s.rows; r += 32) {
     const int at = a.row_slot[s.row0 + r];
     top = max(top, at);
     if (at >= 0) low = min(low, at);
   }
+  top = __reduce_max_sync(0xffffffffu, top), low = __reduce_min_sync(0xffffffffu, low);
   const long long most = min((long long)a.max_kv, a.max_pages * 16);
   s.n = s.slot < 0 ? 0 : (int)min((long long)top + 1, most);
   s.lo = a.window > 0 && low != 0x7fffffff ? max(0, low - a.window + 1) : 0;
-  return s;
 }
 
-__device__ __forceinline__ void aw_copy16(uint32_t dst, const char* src, bool in) {
+// L2 policy of K and V: read once where one block reads them (they leave room for the scores, which the second kernel
+// reads back), kept where several tiles do.
+__device__ __forceinline__ uint64_t aw_policy(bool once) {
+  uint64_t p;
+  if (once) asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+  else asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(p));
+  return p;
+}
+__device__ __forceinline__ void aw_copy16(uint32_t dst, const char* src, bool in, uint64_t policy) {
   const int n = in ? 16 : 0;  // 0: zeros, nothing is read
-  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint.L2::128B [%0], [%1], 16, %2, %3;" ::"r"(dst), "l"(src), "r"(n),
+               "l"(policy)
+               : "memory");
 }
 __device__ __forceinline__ void aw_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -95,6 +111,12 @@ __device__ __forceinline__ void aw_ldsm(uint32_t* r, uint32_t at) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(at));
+}
+// An 8 x 8 matrix of 16-bit values, two a lane, transposed.
+__device__ __forceinline__ uint32_t aw_turn(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 __device__ __forceinline__ void aw_ldsm_t(uint32_t* r, uint32_t at) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -119,7 +141,7 @@ struct AwType<__nv_bfloat16> {
     const __nv_bfloat162 lo = __floats2bfloat162_rn(x - __low2float(hi), y - __high2float(hi));
     return make_uint2(*(const uint32_t*)&hi, *(const uint32_t*)&lo);
   }
-  static __device__ __forceinline__ float2 up(uint32_t u) { return make_float2(bf_lo(u), bf_hi(u)); }
+  static __device__ __forceinline__ float up(__nv_bfloat16 v) { return __bfloat162float(v); }
   static __device__ __forceinline__ bool finite(uint32_t u) {
     return (u & 0x7f80u) != 0x7f80u && (u & 0x7f800000u) != 0x7f800000u;
   }
@@ -139,106 +161,103 @@ struct AwType<__half> {
     const __half2 lo = __floats2half2_rn(x - __low2float(hi), y - __high2float(hi));
     return make_uint2(*(const uint32_t*)&hi, *(const uint32_t*)&lo);
   }
-  static __device__ __forceinline__ float2 up(uint32_t u) { return __half22float2(*(const __half2*)&u); }
+  static __device__ __forceinline__ float up(__half v) { return __half2float(v); }
   static __device__ __forceinline__ bool finite(uint32_t u) {
     return (u & 0x7c00u) != 0x7c00u && (u & 0x7c000000u) != 0x7c000000u;
   }
   static __device__ __forceinline__ __half down(float f) { return __float2half_rn(f); }
 };
 
-// DP: head_dim rounded up to what is built; columns from d on are zeros in shared memory.
-template <int DP>
+// DP: head_dim rounded up to what is built; columns from d on are zeros in shared memory. NT: tiles of 8 vectors a block.
+template <int DP, int NT>
 struct AwShape {
+  static constexpr int WARPS = DP > 128 ? 2 : 4;
   static constexpr int PITCH = DP * 2 + 16;   // an odd number of 16-byte steps: ldmatrix without bank conflicts
   static constexpr int PAGE = 16 * PITCH;     // one page's K or V
-  static constexpr int STAGES = 3;
+  static constexpr int STAGES = DP > 64 ? 2 : 3;
   static constexpr int RING = STAGES * 2 * PAGE;
-  static constexpr int JOIN = 16 * DP * 4;    // a warp's accumulator
-  static constexpr bool Q_REGS = DP <= 128;
-  static constexpr int Q_BYTES = Q_REGS ? 0 : PAGE;
-  static constexpr int SMEM = AW_WARPS * (RING > JOIN ? RING : JOIN) + Q_BYTES;
+  static constexpr int JOIN = DP + 4;         // floats of a vector where the warps' accumulators are joined
+  static constexpr bool Q_REGS = NT * DP <= 256;
+  static constexpr int Q_BYTES = Q_REGS ? 0 : NT * 8 * PITCH;
+  static constexpr int SMEM = WARPS * RING + Q_BYTES;
+  static_assert(NT * 8 * JOIN * 4 <= RING, "a warp's ring takes its accumulator at the end");
 };
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(AW_THREADS) aw_split_kernel(AwArgs a) {
-  using S = AwShape<DP>;
+template <typename T, int DP, int NT>
+__global__ void __launch_bounds__(AwShape<DP, NT>::WARPS * 32) aw_split_kernel(AwArgs a) {
+  using S = AwShape<DP, NT>;
   using Ty = AwType<T>;
+  constexpr int TILE = NT * 8, WARPS = S::WARPS;
   extern __shared__ __align__(128) char smem[];
-  __shared__ float s_m[AW_WARPS][16], s_l[AW_WARPS][16];
+  __shared__ float s_m[WARPS][TILE], s_l[WARPS][TILE];
   pdl_wait();
   pdl_trigger();
   const int split = blockIdx.x, h = blockIdx.y / a.tiles, tile = blockIdx.y % a.tiles, b = blockIdx.z;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  const AwSeq q = aw_seq(a, b);
-  const int k0 = max(split * a.kps, q.lo / 16 * 16), k1 = min(split * a.kps + a.kps, q.n);
+  constexpr int STEPS = DP / 16, CP = DP / 8;
+  AwSeq q = aw_seq(a, b);
   const int group = a.hq / a.hkv;
   const int vecs = q.rows * group;  // live ones
-  if (tile * 16 >= vecs || k0 >= k1) return;
-
-  // this lane's two rows of the tile: vectors tile * 16 + lane / 4 (+ 8)
-  int last[2], from[2];
-  const char* qp[2];
+  if (tile * TILE >= vecs || q.slot < 0) return;
+  const int* table = a.page_table + q.slot * a.max_pages;
+  // pages of this warp: those whose number is warp mod WARPS, so that a slot's place does not depend on the call. The page
+  // numbers are fetched a round ahead of the copies that need them, the first before it is known how many there are
+  int next = split * a.kps / 16;
+  next += (warp - next) & (WARPS - 1);
+  int entry = next < a.max_pages ? table[next] : 0;
+  // this lane's vectors of each tile of 8: 2 (lane mod 4) and the next (accumulators), lane / 4 (Q as an operand)
+  int last[NT][2], from[NT][2];
+  bool live[NT][2];
 #pragma unroll
-  for (int i = 0; i < 2; i++) {
-    const int vec = tile * 16 + lane / 4 + 8 * i;
-    last[i] = -1, from[i] = 0, qp[i] = nullptr;
-    if (vec < vecs) {
-      const int r = q.row0 + vec / group;
-      last[i] = a.row_slot[r];
-      from[i] = a.window > 0 ? last[i] - a.window + 1 : 0;
-      qp[i] = a.q + ((long long)r * a.hq + h * group + vec % group) * a.d * 2;
+  for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      const int vec = tile * TILE + nt * 8 + lane % 4 * 2 + e;
+      live[nt][e] = vec < vecs;
+      last[nt][e] = live[nt][e] ? a.row_slot[q.row0 + vec / group] : -1;
+    }
+  uint32_t qf[S::Q_REGS ? STEPS : 1][NT][2];
+  const char* q_smem = smem + WARPS * S::RING;
+  if (S::Q_REGS) {
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+      const int vec = tile * TILE + nt * 8 + lane / 4;
+      const char* p = a.q + (((long long)q.row0 + vec / group) * a.hq + h * group + vec % group) * a.d * 2;
+#pragma unroll
+      for (int st = 0; st < STEPS; st++)
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          const int c = st * 16 + i * 8 + lane % 4 * 2;
+          qf[S::Q_REGS ? st : 0][nt][i] = vec < vecs && c < a.d ? *(const uint32_t*)(p + c * 2) : 0u;
+        }
+    }
+  } else {
+    for (int c = t; c < TILE * CP; c += WARPS * 32) {
+      const int vec = tile * TILE + c / CP, col = c % CP * 8;
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (vec < vecs && col < a.d)
+        x = *(const uint4*)(a.q + (((long long)(q.row0 + vec / group) * a.hq + h * group + vec % group) * a.d + col) * 2);
+      *(uint4*)(smem + WARPS * S::RING + c / CP * S::PITCH + col * 2) = x;
     }
   }
-  // slots that every row of the tile sees: pages inside need no mask
-  int all_last = vecs > tile * 16 ? 0x7fffffff : -1, all_from = 0;
-#pragma unroll
-  for (int i = 0; i < 2; i++)
-    if (qp[i]) all_last = min(all_last, last[i]), all_from = max(all_from, from[i]);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    all_last = min(all_last, __shfl_xor_sync(0xffffffffu, all_last, o));
-    all_from = max(all_from, __shfl_xor_sync(0xffffffffu, all_from, o));
+  aw_span(a, q);
+  const int k0 = max(split * a.kps, q.lo / 16 * 16), k1 = min(split * a.kps + a.kps, q.n);
+  if (k0 >= k1) return;  // the whole block
+  if (!S::Q_REGS) __syncthreads();
+  const int p0 = k0 / 16, p1 = (k1 + 15) / 16;
+  if (next < p0) {  // behind a window's begin
+    next = p0 + ((warp - p0) & (WARPS - 1));
+    entry = next < p1 ? table[next] : 0;
   }
-
-  char* ring = smem + warp * (S::SMEM - S::Q_BYTES) / AW_WARPS;
+  int page = next;
+  uint32_t pages_ok = 0;  // of the pages in flight, the newest in bit 0: the table names one of the cache
+  char* ring = smem + warp * S::RING;
   const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
-  constexpr int STEPS = DP / 16, CP = DP / 8;
   if (a.d < DP) {  // columns behind the head: zeros, once
     for (int c = lane; c < S::STAGES * 2 * 16 * CP; c += 32)
       if (c % CP * 8 >= a.d) *(uint4*)(ring + c / CP * S::PITCH + c % CP * 16) = make_uint4(0, 0, 0, 0);
   }
-  uint32_t qf[S::Q_REGS ? STEPS : 1][4];
-  const char* q_smem = smem + S::SMEM - S::Q_BYTES;
-  if (S::Q_REGS) {
-#pragma unroll
-    for (int st = 0; st < STEPS; st++) {
-      const int col = st * 16 + lane % 4 * 2;
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const int c = col + (i & 2) * 4;
-        const char* p = qp[i & 1];
-        qf[S::Q_REGS ? st : 0][i] = p && c < a.d ? *(const uint32_t*)(p + c * 2) : 0u;
-      }
-    }
-  } else {
-    for (int c = t; c < 16 * CP; c += AW_THREADS) {
-      const int vec = tile * 16 + c / CP, col = c % CP * 8;
-      uint4 x = make_uint4(0, 0, 0, 0);
-      if (vec < vecs && col < a.d)
-        x = *(const uint4*)(a.q + (((long long)(q.row0 + vec / group) * a.hq + h * group + vec % group) * a.d + col) * 2);
-      *(uint4*)(smem + S::SMEM - S::Q_BYTES + c / CP * S::PITCH + col * 2) = x;
-    }
-    __syncthreads();
-  }
-
-  const int* table = a.page_table + q.slot * a.max_pages;
-  const int p0 = k0 / 16, p1 = (k1 + 15) / 16;
-  // pages of this warp: those whose number is warp mod 4, so that a slot's place does not depend on the call
-  int next = p0 + ((warp - p0) & (AW_WARPS - 1));
-  int page = next;
-  // the page numbers are fetched a round ahead of the copies that need them
-  int entry = next < p1 ? table[next] : 0;
-  uint32_t pages_ok = 0;  // of the pages in flight, the newest in bit 0: the table names one of the cache
+  const uint64_t policy = aw_policy(a.tiles == 1);
   auto fetch = [&](int stage) {
     const bool ok = entry >= 0 && entry < a.pages;
     pages_ok = pages_ok << 1 | (ok ? 1u : 0u);
@@ -246,151 +265,188 @@ __global__ void __launch_bounds__(AW_THREADS) aw_split_kernel(AwArgs a) {
       const long long at = ok ? ((long long)entry * a.hkv + h) * 16 * a.d * 2 : 0;
       const int rows = ok ? min(16, q.n - next * 16) : 0;
       const uint32_t dst = ring_at + stage * 2 * S::PAGE;
+      if (rows == 16 && a.d == DP) {  // a page lies in one piece
+        const char* k = a.k + at + lane * 16;
+        const char* v = a.v + at + lane * 16;
 #pragma unroll
-      for (int i = 0; i < 16 * CP / 32; i++) {
-        const int c = lane + 32 * i, row = c / CP, col = c % CP;
-        if (col * 8 < a.d) {
-          const bool in = row < rows;
-          const long long off = at + (in ? (row * a.d + col * 8) * 2 : 0);
-          aw_copy16(dst + row * S::PITCH + col * 16, a.k + off, in);
-          aw_copy16(dst + S::PAGE + row * S::PITCH + col * 16, a.v + off, in);
+        for (int i = 0; i < 16 * CP / 32; i++) {
+          const int c = lane + 32 * i;
+          aw_copy16(dst + c / CP * S::PITCH + c % CP * 16, k + i * 512, true, policy);
+          aw_copy16(dst + S::PAGE + c / CP * S::PITCH + c % CP * 16, v + i * 512, true, policy);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16 * CP / 32; i++) {
+          const int c = lane + 32 * i, row = c / CP, col = c % CP;
+          if (col * 8 < a.d) {
+            const bool in = row < rows;
+            const long long off = at + (in ? (row * a.d + col * 8) * 2 : 0);
+            aw_copy16(dst + row * S::PITCH + col * 16, a.k + off, in, policy);
+            aw_copy16(dst + S::PAGE + row * S::PITCH + col * 16, a.v + off, in, policy);
+          }
         }
       }
     }
     aw_commit();
-    next += AW_WARPS;
+    next += WARPS;
     entry = next < p1 ? table[next] : 0;
   };
   __syncwarp();
 #pragma unroll
   for (int i = 0; i < S::STAGES - 1; i++) fetch(i);
 
-  float o[DP / 8][4];
+  int all_last = 0x7fffffff, all_from = 0;  // slots that every row of the tile sees: pages inside need no mask
 #pragma unroll
-  for (int i = 0; i < DP / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      from[nt][e] = a.window > 0 ? last[nt][e] - a.window + 1 : 0;
+      if (live[nt][e]) all_last = min(all_last, last[nt][e]), all_from = max(all_from, from[nt][e]);
+    }
+  all_last = __reduce_min_sync(0xffffffffu, all_last), all_from = __reduce_max_sync(0xffffffffu, all_from);
+
+  float o[STEPS][NT][4];  // head values 16 i + lane / 4 (+ 8) of vectors 2 (lane mod 4) (+ 1)
+#pragma unroll
+  for (int i = 0; i < STEPS; i++)
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.f;
+  float m[NT][2], l[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; nt++) m[nt][0] = m[nt][1] = -INFINITY, l[nt][0] = l[nt][1] = 0.f;
   const float scale2 = a.scale * AW_LOG2E;
-  float* scores = a.scores + (((long long)b * a.hkv + h) * a.vecs + tile * 16 + lane / 4) * a.kv_pad;
+  float* scores = a.scores + (((long long)b * a.hkv + h) * a.vecs + tile * TILE + lane % 4 * 2) * a.kv_pad + lane / 4;
   // ldmatrix: lane i gives row i % 8 of matrix i / 8
   const int lr = lane & 7, lm = lane >> 3;
-  const uint32_t k_off = (lr + (lm >> 1) * 8) * S::PITCH + (lm & 1) * 16;
-  const uint32_t v_off = (lr + (lm & 1) * 8) * S::PITCH + (lm >> 1) * 16;
-  const uint32_t q_off = (uint32_t)__cvta_generic_to_shared(q_smem) + (lr + (lm & 1) * 8) * S::PITCH + (lm >> 1) * 16;
+  const uint32_t k_off = (lr + (lm & 1) * 8) * S::PITCH + (lm >> 1) * 16;  // slots 0-7, 8-15, then the next 8 values
+  const uint32_t v_off = (lr + (lm >> 1) * 8) * S::PITCH + (lm & 1) * 16;  // turned: values 0-7, 8-15, then slots 8-15
+  const uint32_t q_off = (uint32_t)__cvta_generic_to_shared(q_smem) + (lr + (lm >> 1) * 8) * S::PITCH + (lm & 1) * 16;
 
-  for (int stage = 0; page < p1; page += AW_WARPS) {
+  for (int stage = 0; page < p1; page += WARPS) {
     aw_wait<S::STAGES - 2>();
     __syncwarp();
     const bool ok = pages_ok >> (S::STAGES - 2) & 1;
     const int ahead = stage + S::STAGES - 1;
     fetch(ahead >= S::STAGES ? ahead - S::STAGES : ahead);
     const uint32_t kp = ring_at + stage * 2 * S::PAGE, vp = kp + S::PAGE;
-    float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    const char* v_page = ring + stage * 2 * S::PAGE + S::PAGE;
+    // slots lane / 4 (c0, c1) and + 8 (c2, c3) of vectors 2 (lane mod 4) and the next; even and odd steps apart, two
+    // shorter chains of products
+    float s[NT][4], s_odd[NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) s[nt][e] = s_odd[nt][e] = 0.f;
 #pragma unroll
     for (int st = 0; st < STEPS; st++) {
-      uint32_t kb[4];
-      aw_ldsm(kb, kp + k_off + st * 32);
-      if (S::Q_REGS) {
-        Ty::mma(s[0], qf[S::Q_REGS ? st : 0], kb[0], kb[1]);
-        Ty::mma(s[1], qf[S::Q_REGS ? st : 0], kb[2], kb[3]);
-      } else {
-        uint32_t qa[4];
-        aw_ldsm(qa, q_off + st * 32);
-        Ty::mma(s[0], qa, kb[0], kb[1]);
-        Ty::mma(s[1], qa, kb[2], kb[3]);
+      uint32_t ka[4];
+      aw_ldsm(ka, kp + k_off + st * 32);
+      uint32_t qb[4];
+      if (!S::Q_REGS) aw_ldsm(qb, q_off + st * 32);
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++) {
+        float* to = st & 1 ? s_odd[nt] : s[nt];
+        if (S::Q_REGS) Ty::mma(to, ka, qf[S::Q_REGS ? st : 0][nt][0], qf[S::Q_REGS ? st : 0][nt][1]);
+        else Ty::mma(to, ka, qb[2 * nt], qb[2 * nt + 1]);
       }
     }
-    const int j0 = page * 16 + lane % 4 * 2;  // this lane's slots: j0, j0 + 1, j0 + 8, j0 + 9
+    const int j0 = page * 16 + lane / 4;  // this lane's slots: j0, j0 + 8
 #pragma unroll
-    for (int nt = 0; nt < 2; nt++)
+    for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-      for (int e = 0; e < 4; e++) s[nt][e] *= scale2;
+      for (int e = 0; e < 4; e++) s[nt][e] = (s[nt][e] + s_odd[nt][e]) * scale2;
     const bool whole = page * 16 + 15 <= all_last && page * 16 >= all_from && page * 16 + 16 <= q.n && ok;
     if (!whole) {
 #pragma unroll
-      for (int nt = 0; nt < 2; nt++)
+      for (int nt = 0; nt < NT; nt++)
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          const int j = j0 + nt * 8 + (e & 1);
-          if (!ok || j > last[e >> 1] || j < from[e >> 1] || j >= q.n) s[nt][e] = -INFINITY;
+          const int j = j0 + (e >> 1) * 8;
+          if (!ok || j > last[nt][e & 1] || j < from[nt][e & 1] || j >= q.n) s[nt][e] = -INFINITY;
+        }
+    }
+    bool more = false;
+    float top[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        if (live[nt][e]) {
+          float* to = scores + (long long)(nt * 8 + e) * a.kv_pad + page * 16;
+          to[0] = s[nt][e];
+          to[8] = s[nt][e + 2];
+        }
+        float x = fmaxf(s[nt][e], s[nt][e + 2]);
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+        top[nt][e] = fmaxf(m[nt][e], x - Ty::SHIFT);
+        more = more || top[nt][e] > m[nt][e];
+      }
+    if (__any_sync(0xffffffffu, more)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          const float f = top[nt][e] > m[nt][e] ? exp2f(m[nt][e] - top[nt][e]) : 1.f;
+          m[nt][e] = top[nt][e];
+          l[nt][e] *= f;
+#pragma unroll
+          for (int i = 0; i < STEPS; i++) o[i][nt][e] *= f, o[i][nt][e + 2] *= f;
         }
     }
 #pragma unroll
-    for (int i = 0; i < 2; i++)
-      if (qp[i]) {
-        float* to = scores + (long long)i * 8 * a.kv_pad + j0;
-        *(float2*)to = make_float2(s[0][2 * i], s[0][2 * i + 1]);
-        *(float2*)(to + 8) = make_float2(s[1][2 * i], s[1][2 * i + 1]);
-      }
-    float top[2];
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-      float x = fmaxf(fmaxf(s[0][2 * i], s[0][2 * i + 1]), fmaxf(s[1][2 * i], s[1][2 * i + 1]));
-      x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-      x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-      top[i] = fmaxf(m[i], x - Ty::SHIFT);
-    }
-    if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
-#pragma unroll
-      for (int i = 0; i < 2; i++) {
-        const float f = top[i] > m[i] ? exp2f(m[i] - top[i]) : 1.f;
-        m[i] = top[i];
-        l[i] *= f;
-#pragma unroll
-        for (int c = 0; c < DP / 8; c++) o[c][2 * i] *= f, o[c][2 * i + 1] *= f;
-      }
-    }
-    const float base[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
-#pragma unroll
-    for (int nt = 0; nt < 2; nt++)
+    for (int nt = 0; nt < NT; nt++)
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        s[nt][e] = exp2f(s[nt][e] - base[e >> 1]);
-        l[e >> 1] += s[nt][e];
+        const float base = m[nt][e & 1] == -INFINITY ? 0.f : m[nt][e & 1];
+        s[nt][e] = exp2f(s[nt][e] - base);
+        l[nt][e & 1] += s[nt][e];
       }
     bool by_mma = true;
     if (!whole && (a.max_rows > 1 || a.window > 0)) {  // a row may be blind to a slot of this page that holds anything
       bool fine = true;
-      for (int c = lane; c < 16 * (a.d / 2); c += 32)
-        fine = fine && Ty::finite(*(const uint32_t*)(ring + stage * 2 * S::PAGE + S::PAGE + c / (a.d / 2) * S::PITCH +
-                                                     c % (a.d / 2) * 4));
+#pragma unroll 4
+      for (int c = lane; c < 16 * CP; c += 32) {
+        const uint4 x = *(const uint4*)(v_page + c / CP * S::PITCH + c % CP * 16);
+        fine = fine && Ty::finite(x.x) && Ty::finite(x.y) && Ty::finite(x.z) && Ty::finite(x.w);
+      }
       by_mma = __all_sync(0xffffffffu, fine);
     }
     if (by_mma) {
-      uint32_t hi[4], rest[4];
+      uint32_t hi[NT][2], rest[NT][2];
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const uint2 x = Ty::parts(s[i >> 1][(i & 1) * 2], s[i >> 1][(i & 1) * 2 + 1]);
-        hi[i] = x.x, rest[i] = x.y;
-      }
+      for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          const uint2 x = Ty::parts(s[nt][2 * i], s[nt][2 * i + 1]);
+          hi[nt][i] = aw_turn(x.x), rest[nt][i] = aw_turn(x.y);
+        }
 #pragma unroll
       for (int st = 0; st < STEPS; st++) {
-        uint32_t vb[4];
-        aw_ldsm_t(vb, vp + v_off + st * 32);
-        Ty::mma(o[2 * st], hi, vb[0], vb[1]);
-        Ty::mma(o[2 * st + 1], hi, vb[2], vb[3]);
-        Ty::mma(o[2 * st], rest, vb[0], vb[1]);
-        Ty::mma(o[2 * st + 1], rest, vb[2], vb[3]);
+        uint32_t va[4];
+        aw_ldsm_t(va, vp + v_off + st * 32);
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) Ty::mma(o[st][nt], va, hi[nt][0], hi[nt][1]);
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) Ty::mma(o[st][nt], va, rest[nt][0], rest[nt][1]);
       }
     } else {
 #pragma unroll 1
       for (int kk = 0; kk < 16; kk++) {
-        const int src = (lane & ~3) | ((kk & 7) >> 1);
-        float p[2];
-        bool see[2];
+        const int src = (kk & 7) * 4 + lane % 4, j = page * 16 + kk;
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-          const float x = kk < 8 ? (kk & 1 ? s[0][2 * i + 1] : s[0][2 * i]) : (kk & 1 ? s[1][2 * i + 1] : s[1][2 * i]);
-          p[i] = __shfl_sync(0xffffffffu, x, src);
-          const int j = page * 16 + kk;
-          see[i] = j <= last[i] && j >= from[i] && j < q.n;
-        }
+        for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-        for (int c = 0; c < DP / 8; c++) {
-          const float2 x = Ty::up(*(const uint32_t*)(ring + stage * 2 * S::PAGE + S::PAGE + kk * S::PITCH + c * 16 +
-                                                     lane % 4 * 4));
-          if (see[0]) o[c][0] = fmaf(p[0], x.x, o[c][0]), o[c][1] = fmaf(p[0], x.y, o[c][1]);
-          if (see[1]) o[c][2] = fmaf(p[1], x.x, o[c][2]), o[c][3] = fmaf(p[1], x.y, o[c][3]);
-        }
+          for (int e = 0; e < 2; e++) {
+            const float p = __shfl_sync(0xffffffffu, kk < 8 ? s[nt][e] : s[nt][e + 2], src);
+            if (j > last[nt][e] || j < from[nt][e] || j >= q.n) continue;
+#pragma unroll
+            for (int i = 0; i < STEPS; i++) {
+              const T* v = (const T*)(v_page + kk * S::PITCH) + i * 16 + lane / 4;
+              o[i][nt][e] = fmaf(p, Ty::up(v[0]), o[i][nt][e]);
+              o[i][nt][e + 2] = fmaf(p, Ty::up(v[8]), o[i][nt][e + 2]);
+            }
+          }
       }
     }
     __syncwarp();
@@ -398,41 +454,49 @@ __global__ void __launch_bounds__(AW_THREADS) aw_split_kernel(AwArgs a) {
   }
   aw_wait<0>();
 #pragma unroll
-  for (int i = 0; i < 2; i++) {
-    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-    if (lane % 4 == 0) s_m[warp][lane / 4 + 8 * i] = m[i], s_l[warp][lane / 4 + 8 * i] = l[i];
-  }
-  __syncthreads();  // every warp is done with its ring, which now takes its accumulator
-  float top[2];
+  for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-  for (int i = 0; i < 2; i++) {
-    const int row = lane / 4 + 8 * i;
-    top[i] = fmaxf(fmaxf(s_m[0][row], s_m[1][row]), fmaxf(s_m[2][row], s_m[3][row]));
-    const float f = m[i] == -INFINITY ? 0.f : exp2f(m[i] - top[i]);
-    float* to = (float*)ring + row * DP + lane % 4 * 2;
+    for (int e = 0; e < 2; e++) {
 #pragma unroll
-    for (int c = 0; c < DP / 8; c++) *(float2*)(to + c * 8) = make_float2(o[c][2 * i] * f, o[c][2 * i + 1] * f);
-  }
-  __syncthreads();
-  const long long at = (((long long)b * a.hkv + h) * a.splits + split) * a.vecs + tile * 16;
-  const int live = min(16, vecs - tile * 16);
-  constexpr int WARP_BYTES = (S::SMEM - S::Q_BYTES) / AW_WARPS;
-  for (int c = t; c < live * (a.d / 4); c += AW_THREADS) {
-    const int row = c / (a.d / 4), col = c % (a.d / 4) * 4;
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int w = 0; w < AW_WARPS; w++) {
-      const float4 y = *(const float4*)(smem + w * WARP_BYTES + (row * DP + col) * 4);
-      x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+      for (int x = 4; x < 32; x <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], x);
+      if (lane < 4) s_m[warp][nt * 8 + lane * 2 + e] = m[nt][e], s_l[warp][nt * 8 + lane * 2 + e] = l[nt][e];
     }
-    *(float4*)(a.parts + (at + row) * a.d + col) = x;
-  }
-  if (t < live) {
-    const float mm = fmaxf(fmaxf(s_m[0][t], s_m[1][t]), fmaxf(s_m[2][t], s_m[3][t]));
+  __syncthreads();  // every warp is done with its ring, which now takes its accumulator
+#pragma unroll
+  for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      const int row = nt * 8 + lane % 4 * 2 + e;
+      float top = s_m[0][row];
+#pragma unroll
+      for (int w = 1; w < WARPS; w++) top = fmaxf(top, s_m[w][row]);
+      const float f = m[nt][e] == -INFINITY ? 0.f : exp2f(m[nt][e] - top);
+      float* to = (float*)ring + row * S::JOIN + lane / 4;
+      if (live[nt][e]) {
+#pragma unroll
+        for (int i = 0; i < STEPS; i++) to[i * 16] = o[i][nt][e] * f, to[i * 16 + 8] = o[i][nt][e + 2] * f;
+      }
+    }
+  __syncthreads();
+  const long long at = (((long long)b * a.hkv + h) * a.splits + split) * a.vecs + tile * TILE;
+  const int count = min(TILE, vecs - tile * TILE);
+  for (int row = warp; row < count; row += WARPS)
+    for (int c = lane * 4; c < a.d; c += 128) {
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < WARPS; w++) {
+        const float4 y = *(const float4*)(smem + w * S::RING + (row * S::JOIN + c) * 4);
+        x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+      }
+      *(float4*)(a.parts + (at + row) * a.d + c) = x;
+    }
+  if (t < count) {
+    float mm = s_m[0][t];
+#pragma unroll
+    for (int w = 1; w < WARPS; w++) mm = fmaxf(mm, s_m[w][t]);
     float sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < AW_WARPS; w++) sum += s_m[w][t] == -INFINITY ? 0.f : exp2f(s_m[w][t] - mm) * s_l[w][t];
+    for (int w = 0; w < WARPS; w++) sum += s_m[w][t] == -INFINITY ? 0.f : exp2f(s_m[w][t] - mm) * s_l[w][t];
     a.stats[at + t] = make_float2(mm, sum);
   }
 }
@@ -457,102 +521,145 @@ __device__ __forceinline__ float2 aw_total(const AwArgs& a, long long head, int 
   return make_float2(m == -INFINITY ? 0.f : m, l == 0.f ? 0.f : 1.f / l);
 }
 
-// Joins the splits of a (sequence, kv head): the first a.vecs blocks of x one vector's output each, its splits dealt to the
-// warps; the others add up the weights of AW_FIN_SLOTS slots each, four a thread.
+// Joins the splits of a (sequence, kv head): the first a.joins blocks of x the output, 128 values of one vector a job of
+// a.join_warps warps, which share its splits; the others add up the slots' weights, AW_FIN_SLOTS at a time, four a thread.
 template <typename T>
 __global__ void __launch_bounds__(AW_FIN_THREADS) aw_finish_kernel(AwArgs a) {
   extern __shared__ __align__(16) char fin[];
-  pdl_wait();
-  pdl_trigger();
+  // Before the wait only what the first kernel does not write: its blocks let this one start after their own wait, so
+  // everything before the first kernel is done. weights_out is written behind the wait (weights may be it).
   const int b = blockIdx.z, h = blockIdx.y, t = threadIdx.x, lane = t & 31, warp = t >> 5;
   constexpr int WARPS = AW_FIN_THREADS / 32;
-  const AwSeq q = aw_seq(a, b);
+  AwSeq q = aw_seq(a, b);
+  aw_span(a, q);
   const int group = a.hq / a.hkv, vecs = q.rows * group;
   const long long head = (long long)b * a.hkv + h;
   const int lo = q.lo / 16 * 16;  // splits [s0, s1) hold a visible slot
   const int s0 = lo / a.kps, s1 = lo < q.n ? (q.n + a.kps - 1) / a.kps : s0;
-  if ((int)blockIdx.x < a.vecs) {
-    const int v = blockIdx.x;
-    if (v >= vecs) return;
-    const float2 st = aw_total(a, head, v, s0, s1);
-    float* part = (float*)fin;  // [WARPS][d]
-    for (int c = lane * 4; c < a.d; c += 128) {
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  if ((int)blockIdx.x < a.joins) {
+    pdl_wait();
+    pdl_trigger();
+    const int segments = (a.d + 127) / 128;  // of 128 values
+    const int job = blockIdx.x * (WARPS / a.join_warps) + warp / a.join_warps;
+    const int v = job / segments, c = job % segments * 128 + lane * 4;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    float2 st = make_float2(0.f, 0.f);
+    if (v < vecs) {
+      st = aw_total(a, head, v, s0, s1);
+      if (c < a.d) {
 #pragma unroll 4
-      for (int s = s0 + warp; s < s1; s += WARPS) {
-        const long long at = (head * a.splits + s) * a.vecs + v;
-        const float m = a.stats[at].x;
-        const float4 x = *(const float4*)(a.parts + at * a.d + c);
-        if (m != -INFINITY) {
-          const float f = exp2f(m - st.x);
-          o.x = fmaf(f, x.x, o.x), o.y = fmaf(f, x.y, o.y), o.z = fmaf(f, x.z, o.z), o.w = fmaf(f, x.w, o.w);
+        for (int s = s0 + warp % a.join_warps; s < s1; s += a.join_warps) {
+          const long long at = (head * a.splits + s) * a.vecs + v;
+          const float m = a.stats[at].x;
+          const float4 x = *(const float4*)(a.parts + at * a.d + c);
+          if (m != -INFINITY) {
+            const float f = exp2f(m - st.x);
+            o.x = fmaf(f, x.x, o.x), o.y = fmaf(f, x.y, o.y), o.z = fmaf(f, x.z, o.z), o.w = fmaf(f, x.w, o.w);
+          }
         }
       }
-      *(float4*)(part + warp * a.d + c) = o;
     }
-    __syncthreads();
-    const long long row = q.row0 + v / group;
-    for (int c = t; c < a.d; c += AW_FIN_THREADS) {
-      float o = 0.f;
-#pragma unroll
-      for (int w = 0; w < WARPS; w++) o += part[w * a.d + c];
-      ((T*)a.out)[(row * a.hq + h * group + v % group) * a.d + c] = AwType<T>::down(o * st.y);
+    if (a.join_warps > 1) {  // in the warps' order
+      float4* part = (float4*)fin;
+      part[t] = o;
+      __syncthreads();
+      if (warp % a.join_warps) return;
+      for (int w = 1; w < a.join_warps; w++) {
+        const float4 x = part[t + w * 32];
+        o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
+      }
+    }
+    if (v < vecs && c < a.d) {
+      const long long row = q.row0 + v / group;
+      alignas(8) T r[4] = {AwType<T>::down(o.x * st.y), AwType<T>::down(o.y * st.y), AwType<T>::down(o.z * st.y),
+                           AwType<T>::down(o.w * st.y)};
+      *(uint2*)((T*)a.out + (row * a.hq + h * group + v % group) * a.d + c) = *(const uint2*)r;
     }
     return;
   }
   const int n = (int)min((long long)q.n, a.cap);
-  const int j_first = (blockIdx.x - a.vecs) * AW_FIN_SLOTS;
-  if (j_first >= n) return;
-  float2* s_stat = (float2*)fin;  // [vecs]
-  for (int v = warp; v < vecs; v += WARPS) {
-    const float2 st = aw_total(a, head, v, s0, s1);
-    if (lane == 0) s_stat[v] = st;
-  }
-  __syncthreads();
-  const int j = j_first + t * 4;
-  if (j >= n) return;
+  int j = (blockIdx.x - a.joins) * AW_FIN_SLOTS + t * 4;
+  if (j - t * 4 >= n) return;  // no wait: nothing is read or written
+  const int step = (gridDim.x - a.joins) * AW_FIN_SLOTS;
   const int first = a.row_slot[q.row0];
-  const long long at = (q.slot * a.hkv + h) * a.cap + j;
-  const float* scores = a.scores + head * a.vecs * a.kv_pad + j;
-  const bool wide = j + 3 < n && a.cap % 4 == 0 && a.wide_weights;
-  float old[4] = {0.f, 0.f, 0.f, 0.f}, sum[4] = {0.f, 0.f, 0.f, 0.f};
-  if (wide && j + 3 < first) {
-    const float4 x = *(const float4*)(a.weights + at);
-    old[0] = x.x, old[1] = x.y, old[2] = x.z, old[3] = x.w;
-  } else {
+  const bool aligned4 = a.cap % 4 == 0 && a.wide_weights;
+  const float* scores = a.scores + head * a.vecs * a.kv_pad;
+  const long long base = (q.slot * a.hkv + h) * a.cap;
+  constexpr int AHEAD = 4;  // vectors whose scores are on their way while the sums are found
+  float4 ahead[AHEAD];
+  float old[4];
+  auto load_old = [&]() {
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-      if (j + i < n && j + i < first) old[i] = a.weights[at + i];
-  }
-  for (int r = 0; r < q.rows; r++) {
-    const int slot = a.row_slot[q.row0 + r], from = a.window > 0 ? slot - a.window + 1 : 0;
-    if (j > slot || j + 3 < from) continue;
-#pragma unroll 4
-    for (int g = 0; g < group; g++) {
-      const float2 st = s_stat[r * group + g];
-      const float4 x = *(const float4*)(scores + (long long)(r * group + g) * a.kv_pad);
-      const float y[4] = {x.x, x.y, x.z, x.w};
+    for (int i = 0; i < 4; i++) old[i] = 0.f;
+    if (aligned4 && j + 3 < n && j + 3 < first) {
+      const float4 x = *(const float4*)(a.weights + base + j);
+      old[0] = x.x, old[1] = x.y, old[2] = x.z, old[3] = x.w;
+    } else {
 #pragma unroll
       for (int i = 0; i < 4; i++)
-        if (j + i <= slot && j + i >= from) sum[i] += exp2f(y[i] - st.x) * st.y;
+        if (j + i < n && j + i < first) old[i] = a.weights[base + j + i];
+    }
+  };
+  auto load_scores = [&]() {
+#pragma unroll
+    for (int v = 0; v < AHEAD; v++)  // what lies behind n was never written, and is not used
+      if (v < vecs && j < n && j + 3 >= q.lo) ahead[v] = *(const float4*)(scores + (long long)v * a.kv_pad + j);
+  };
+  load_old();
+  pdl_wait();
+  pdl_trigger();
+  load_scores();
+  // of each vector: maximum, 1 / sum, and the slots that it sees, [from, last]
+  float4* s_vec = (float4*)fin;
+  for (int v = warp; v < vecs; v += WARPS) {
+    const float2 st = aw_total(a, head, v, s0, s1);
+    if (lane == 0) {
+      const int slot = a.row_slot[q.row0 + v / group];
+      s_vec[v] = make_float4(st.x, st.y, __int_as_float(a.window > 0 ? slot - a.window + 1 : 0), __int_as_float(slot));
     }
   }
-  if (wide) {
-    *(float4*)(a.weights_out + at) = make_float4(old[0] + sum[0], old[1] + sum[1], old[2] + sum[2], old[3] + sum[3]);
-  } else {
+  __syncthreads();
+  while (j < n) {
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    auto add = [&](const float4& x, const float4& vec) {
+      const float y[4] = {x.x, x.y, x.z, x.w};
+      const int from = __float_as_int(vec.z), to = __float_as_int(vec.w);
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-      if (j + i < n) a.weights_out[at + i] = old[i] + sum[i];
+      for (int i = 0; i < 4; i++)
+        if (j + i >= from && j + i <= to) sum[i] = fmaf(exp2f(y[i] - vec.x), vec.y, sum[i]);
+    };
+    if (j + 3 >= q.lo) {  // else no row sees them
+#pragma unroll
+      for (int v = 0; v < AHEAD; v++)
+        if (v < vecs) add(ahead[v], s_vec[v]);
+#pragma unroll 4
+      for (int v = AHEAD; v < vecs; v++) add(*(const float4*)(scores + (long long)v * a.kv_pad + j), s_vec[v]);
+    }
+    float* to = a.weights_out + base + j;
+    if (aligned4 && j + 3 < n) {
+      *(float4*)to = make_float4(old[0] + sum[0], old[1] + sum[1], old[2] + sum[2], old[3] + sum[3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        if (j + i < n) to[i] = old[i] + sum[i];
+    }
+    j += step;
+    load_old();
+    load_scores();
   }
 }
 
 struct AwPlan {
-  int kps, splits, tiles;
+  int kps, splits, tile, tiles;
   long long vecs, kv_pad;
   size_t scores, stats, parts;  // bytes
 };
 
 static size_t aw_round(size_t n) { return (n + 255) / 256 * 256; }
+
+// Blocks of the first kernel on an SM, by their shared memory. For head_dim 128 three with rings of two pages read 5.7 TB/s
+// where two with rings of three read 5.5 (131071 slots 99.9 against 102.7 us, 32 sequences 156.8 against 162.1 us).
+static int aw_resident(int64_t D) { return D > 64 ? 3 : 4; }
 
 // How a call is cut: keys_per_split as given, or such that the groups (sequence, kv head, tile) fill the device's resident
 // blocks about once, or several times where there are many groups, since their lengths differ.
@@ -560,10 +667,11 @@ static AwPlan aw_plan(int64_t B, int64_t rows, int64_t Hq, int64_t Hkv, int64_t 
                       int64_t kps) {
   AwPlan p;
   p.vecs = rows * (Hq / Hkv);
-  p.tiles = (int)((p.vecs + 15) / 16);
+  p.tile = p.vecs <= 8 ? 8 : 16;
+  p.tiles = (int)((p.vecs + p.tile - 1) / p.tile);
   p.kv_pad = (kv + 63) / 64 * 64;
   if (kps == 0) {
-    const int64_t groups = B * Hkv * p.tiles, resident = D > 128 ? 148 : 296;
+    const int64_t groups = B * Hkv * p.tiles, resident = 148 * aw_resident(D);
     const int64_t seen = window > 0 && window + rows < kv ? window + rows : kv;  // slots a sequence's rows can see
     int64_t want = groups * 2 >= resident ? (resident * 6 + groups - 1) / groups : resident / groups;
     if (want < 1) want = 1;
@@ -579,28 +687,40 @@ static AwPlan aw_plan(int64_t B, int64_t rows, int64_t Hq, int64_t Hkv, int64_t 
   return p;
 }
 
-template <typename T, int DP>
+template <typename T, int DP, int NT>
 int launch_split(const AwArgs& a, dim3 grid, cudaStream_t st) {
-  const cudaError_t e = cudaFuncSetAttribute(aw_split_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             AwShape<DP>::SMEM);
+  auto* kernel = aw_split_kernel<T, DP, NT>;
+  constexpr int smem = AwShape<DP, NT>::SMEM;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) {
     set_error("aw_split_kernel: %s", cudaGetErrorString(e));
     return IM_CUDA_ERROR;
   }
-  return launch("aw_split_kernel", aw_split_kernel<T, DP>, grid, dim3(AW_THREADS), AwShape<DP>::SMEM, st, a);
+  return launch("aw_split_kernel", kernel, grid, dim3(AwShape<DP, NT>::WARPS * 32), smem, st, a);
+}
+
+template <typename T, int NT>
+int launch_split_d(const AwArgs& a, dim3 grid, cudaStream_t st) {
+  return a.d <= 64    ? launch_split<T, 64, NT>(a, grid, st)
+         : a.d <= 96  ? launch_split<T, 96, NT>(a, grid, st)
+         : a.d <= 128 ? launch_split<T, 128, NT>(a, grid, st)
+                      : launch_split<T, 256, NT>(a, grid, st);
 }
 
 template <typename T>
-int launch_attention_weights(const AwArgs& a, int64_t B, cudaStream_t st) {
+int launch_attention_weights(AwArgs& a, int64_t B, cudaStream_t st) {
   const dim3 grid((unsigned)a.splits, (unsigned)(a.hkv * a.tiles), (unsigned)B);
-  const int rc = a.d <= 64    ? launch_split<T, 64>(a, grid, st)
-                 : a.d <= 96  ? launch_split<T, 96>(a, grid, st)
-                 : a.d <= 128 ? launch_split<T, 128>(a, grid, st)
-                              : launch_split<T, 256>(a, grid, st);
+  const int rc = a.vecs <= 8 ? launch_split_d<T, 1>(a, grid, st) : launch_split_d<T, 2>(a, grid, st);
   if (rc != IM_OK) return rc;
-  const int chunks = (a.max_kv + AW_FIN_SLOTS - 1) / AW_FIN_SLOTS;
-  const size_t join = (size_t)AW_FIN_THREADS / 32 * a.d * 4, sums = sizeof(float2) * a.vecs;
-  return launch("aw_finish_kernel", aw_finish_kernel<T>, dim3((unsigned)(a.vecs + chunks), (unsigned)a.hkv, (unsigned)B),
+  // many splits that a row can see: a block's eight warps share a job's, else each has a job
+  const int64_t seen = a.window > 0 ? ((int64_t)a.window + a.max_rows) / a.kps + 2 : a.splits;
+  a.join_warps = seen >= 16 && a.splits >= 16 ? AW_FIN_THREADS / 32 : 1;
+  a.joins = (int)(((int64_t)a.vecs * ((a.d + 127) / 128) * a.join_warps * 32 + AW_FIN_THREADS - 1) / AW_FIN_THREADS);
+  // blocks of slots a (sequence, kv head): the device's worth in all, so that a block's sums serve many slots
+  const int64_t most = (a.max_kv + AW_FIN_SLOTS - 1) / AW_FIN_SLOTS, share = (369 + B * a.hkv) / (B * a.hkv);
+  const int chunks = (int)(most < share ? most : share);
+  const size_t join = sizeof(float4) * AW_FIN_THREADS, sums = sizeof(float4) * a.vecs;
+  return launch("aw_finish_kernel", aw_finish_kernel<T>, dim3((unsigned)(a.joins + chunks), (unsigned)a.hkv, (unsigned)B),
                 dim3(AW_FIN_THREADS), join > sums ? join : sums, st, a);
 }
 
@@ -639,7 +759,7 @@ extern "C" int im_attention_weights(const void* q, const void* k_cache, const vo
   IM_REQUIRE(aligned(q, 16) && aligned(k_cache, 16) && aligned(v_cache, 16) && aligned(out, 16), IM_INVALID,
              "im_attention_weights: q, the caches and out must be 16-byte aligned");
   IM_REQUIRE(M < (1ll << 31) && B < 65536 && Hkv <= 4096 && max_rows_per_seq <= 4096 && Hq / Hkv <= 256 &&
-                 max_rows_per_seq * (Hq / Hkv) <= 4096 && max_kv_len < (1ll << 30) && window < (1ll << 30),
+                 max_rows_per_seq * (Hq / Hkv) <= 2048 && max_kv_len < (1ll << 30) && window < (1ll << 30),
              IM_UNSUPPORTED, "im_attention_weights: too large");
   const int64_t kv = max_kv_len > 0 ? max_kv_len : 1;
   const size_t need = im_attention_weights_workspace_bytes(B, max_rows_per_seq, Hq, Hkv, D, kv, keys_per_split, window);

@@ -227,11 +227,11 @@ int launch_rope(RopeArgs& a, long long M, bool vec, cudaStream_t st) {
   constexpr int WIDE = 16 / sizeof(T);
   const int n = vec ? WIDE : 1;
   const int units = (a.interleaved && vec ? a.rotary / n : a.rotary / 2 / n) + (a.d - a.rotary) / n;
-  // few rows: their heads are spread over several blocks, so that one row's are not one block's latency; many short ones:
-  // several a block, so that its threads have a unit or two each
+  // few rows: their heads are spread over several blocks, so that one row's are not one block's latency; many:
+  // several a block, so that every thread works out a pair's c and s
   int blocks_y = 1, rows = 1;
   while (M * blocks_y < 148 && blocks_y * 4 < a.heads) blocks_y *= 2;
-  while (rows < RP_ROWS && rows * 2 * a.heads * units <= RP_BATCH * RP_THREADS && M >= rows * 2 * 592) rows *= 2;
+  while (rows < RP_ROWS && rows * 2 * (a.rotary / 2) <= RP_THREADS && M >= rows * 2 * 592) rows *= 2;
   a.rows = M, a.rows_per_block = rows;
   a.heads_per_block = (a.heads + blocks_y - 1) / blocks_y;
   blocks_y = (a.heads + a.heads_per_block - 1) / a.heads_per_block;
