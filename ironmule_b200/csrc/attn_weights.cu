@@ -53,6 +53,7 @@ struct AwArgs {
   float* scores;           // [B][Hkv][vecs][kv_pad], in log2 units
   float2* stats;           // [B][Hkv][splits][vecs]: maximum and sum
   float* parts;            // [B][Hkv][splits][vecs][d]
+  int seen;                // splits that a sequence's rows see, if they follow one another: the first kernel's blocks
   int joins, join_warps;   // blocks of the second kernel that join outputs, warps a job of theirs
   int wide_weights;        // weights and weights_out start on 16 bytes
 };
@@ -184,7 +185,8 @@ struct AwShape {
 };
 
 template <typename T, int DP, int NT>
-__global__ void __launch_bounds__(AwShape<DP, NT>::WARPS * 32) aw_split_kernel(AwArgs a) {
+__global__ void __launch_bounds__(AwShape<DP, NT>::WARPS * 32, DP > 64 ? 3 : 4)
+    aw_split_kernel(AwArgs a) {
   using S = AwShape<DP, NT>;
   using Ty = AwType<T>;
   constexpr int TILE = NT * 8, WARPS = S::WARPS;
@@ -192,7 +194,8 @@ __global__ void __launch_bounds__(AwShape<DP, NT>::WARPS * 32) aw_split_kernel(A
   __shared__ float s_m[WARPS][TILE], s_l[WARPS][TILE];
   pdl_wait();
   pdl_trigger();
-  const int split = blockIdx.x, h = blockIdx.y / a.tiles, tile = blockIdx.y % a.tiles, b = blockIdx.z;
+  int split = blockIdx.x;  // with a window: counted from the first that a row sees
+  const int h = blockIdx.y / a.tiles, tile = blockIdx.y % a.tiles, b = blockIdx.z;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   constexpr int STEPS = DP / 16, CP = DP / 8;
   AwSeq q = aw_seq(a, b);
@@ -204,7 +207,7 @@ __global__ void __launch_bounds__(AwShape<DP, NT>::WARPS * 32) aw_split_kernel(A
   // numbers are fetched a round ahead of the copies that need them, the first before it is known how many there are
   int next = split * a.kps / 16;
   next += (warp - next) & (WARPS - 1);
-  int entry = next < a.max_pages ? table[next] : 0;
+  int entry = a.window == 0 && next < a.max_pages ? table[next] : 0;
   // this lane's vectors of each tile of 8: 2 (lane mod 4) and the next (accumulators), lane / 4 (Q as an operand)
   int last[NT][2], from[NT][2];
   bool live[NT][2];
@@ -241,16 +244,8 @@ __global__ void __launch_bounds__(AwShape<DP, NT>::WARPS * 32) aw_split_kernel(A
     }
   }
   aw_span(a, q);
-  const int k0 = max(split * a.kps, q.lo / 16 * 16), k1 = min(split * a.kps + a.kps, q.n);
-  if (k0 >= k1) return;  // the whole block
+  if (a.window > 0) split += q.lo / 16 * 16 / a.kps;
   if (!S::Q_REGS) __syncthreads();
-  const int p0 = k0 / 16, p1 = (k1 + 15) / 16;
-  if (next < p0) {  // behind a window's begin
-    next = p0 + ((warp - p0) & (WARPS - 1));
-    entry = next < p1 ? table[next] : 0;
-  }
-  int page = next;
-  uint32_t pages_ok = 0;  // of the pages in flight, the newest in bit 0: the table names one of the cache
   char* ring = smem + warp * S::RING;
   const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
   if (a.d < DP) {  // columns behind the head: zeros, once
@@ -258,43 +253,6 @@ __global__ void __launch_bounds__(AwShape<DP, NT>::WARPS * 32) aw_split_kernel(A
       if (c % CP * 8 >= a.d) *(uint4*)(ring + c / CP * S::PITCH + c % CP * 16) = make_uint4(0, 0, 0, 0);
   }
   const uint64_t policy = aw_policy(a.tiles == 1);
-  auto fetch = [&](int stage) {
-    const bool ok = entry >= 0 && entry < a.pages;
-    pages_ok = pages_ok << 1 | (ok ? 1u : 0u);
-    if (next < p1) {
-      const long long at = ok ? ((long long)entry * a.hkv + h) * 16 * a.d * 2 : 0;
-      const int rows = ok ? min(16, q.n - next * 16) : 0;
-      const uint32_t dst = ring_at + stage * 2 * S::PAGE;
-      if (rows == 16 && a.d == DP) {  // a page lies in one piece
-        const char* k = a.k + at + lane * 16;
-        const char* v = a.v + at + lane * 16;
-#pragma unroll
-        for (int i = 0; i < 16 * CP / 32; i++) {
-          const int c = lane + 32 * i;
-          aw_copy16(dst + c / CP * S::PITCH + c % CP * 16, k + i * 512, true, policy);
-          aw_copy16(dst + S::PAGE + c / CP * S::PITCH + c % CP * 16, v + i * 512, true, policy);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 16 * CP / 32; i++) {
-          const int c = lane + 32 * i, row = c / CP, col = c % CP;
-          if (col * 8 < a.d) {
-            const bool in = row < rows;
-            const long long off = at + (in ? (row * a.d + col * 8) * 2 : 0);
-            aw_copy16(dst + row * S::PITCH + col * 16, a.k + off, in, policy);
-            aw_copy16(dst + S::PAGE + row * S::PITCH + col * 16, a.v + off, in, policy);
-          }
-        }
-      }
-    }
-    aw_commit();
-    next += WARPS;
-    entry = next < p1 ? table[next] : 0;
-  };
-  __syncwarp();
-#pragma unroll
-  for (int i = 0; i < S::STAGES - 1; i++) fetch(i);
-
   int all_last = 0x7fffffff, all_from = 0;  // slots that every row of the tile sees: pages inside need no mask
 #pragma unroll
   for (int nt = 0; nt < NT; nt++)
@@ -304,15 +262,6 @@ __global__ void __launch_bounds__(AwShape<DP, NT>::WARPS * 32) aw_split_kernel(A
       if (live[nt][e]) all_last = min(all_last, last[nt][e]), all_from = max(all_from, from[nt][e]);
     }
   all_last = __reduce_min_sync(0xffffffffu, all_last), all_from = __reduce_max_sync(0xffffffffu, all_from);
-
-  float o[STEPS][NT][4];  // head values 16 i + lane / 4 (+ 8) of vectors 2 (lane mod 4) (+ 1)
-#pragma unroll
-  for (int i = 0; i < STEPS; i++)
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.f;
-  float m[NT][2], l[NT][2];
-#pragma unroll
-  for (int nt = 0; nt < NT; nt++) m[nt][0] = m[nt][1] = -INFINITY, l[nt][0] = l[nt][1] = 0.f;
   const float scale2 = a.scale * AW_LOG2E;
   float* scores = a.scores + (((long long)b * a.hkv + h) * a.vecs + tile * TILE + lane % 4 * 2) * a.kv_pad + lane / 4;
   // ldmatrix: lane i gives row i % 8 of matrix i / 8
@@ -321,183 +270,241 @@ __global__ void __launch_bounds__(AwShape<DP, NT>::WARPS * 32) aw_split_kernel(A
   const uint32_t v_off = (lr + (lm >> 1) * 8) * S::PITCH + (lm & 1) * 16;  // turned: values 0-7, 8-15, then slots 8-15
   const uint32_t q_off = (uint32_t)__cvta_generic_to_shared(q_smem) + (lr + (lm >> 1) * 8) * S::PITCH + (lm & 1) * 16;
 
-  for (int stage = 0; page < p1; page += WARPS) {
-    aw_wait<S::STAGES - 2>();
-    __syncwarp();
-    const bool ok = pages_ok >> (S::STAGES - 2) & 1;
-    const int ahead = stage + S::STAGES - 1;
-    fetch(ahead >= S::STAGES ? ahead - S::STAGES : ahead);
-    const uint32_t kp = ring_at + stage * 2 * S::PAGE, vp = kp + S::PAGE;
-    const char* v_page = ring + stage * 2 * S::PAGE + S::PAGE;
-    // slots lane / 4 (c0, c1) and + 8 (c2, c3) of vectors 2 (lane mod 4) and the next; even and odd steps apart, two
-    // shorter chains of products
-    float s[NT][4], s_odd[NT][4];
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-      for (int e = 0; e < 4; e++) s[nt][e] = s_odd[nt][e] = 0.f;
-#pragma unroll
-    for (int st = 0; st < STEPS; st++) {
-      uint32_t ka[4];
-      aw_ldsm(ka, kp + k_off + st * 32);
-      uint32_t qb[4];
-      if (!S::Q_REGS) aw_ldsm(qb, q_off + st * 32);
-#pragma unroll
-      for (int nt = 0; nt < NT; nt++) {
-        float* to = st & 1 ? s_odd[nt] : s[nt];
-        if (S::Q_REGS) Ty::mma(to, ka, qf[S::Q_REGS ? st : 0][nt][0], qf[S::Q_REGS ? st : 0][nt][1]);
-        else Ty::mma(to, ka, qb[2 * nt], qb[2 * nt + 1]);
-      }
+  // one split, unless rows with a window lie so far apart that there are more than blocks
+  for (;; split += gridDim.x) {
+    const int k0 = max(split * a.kps, q.lo / 16 * 16), k1 = min(split * a.kps + a.kps, q.n);
+    if (k0 >= k1) return;  // the whole block
+    const int p0 = k0 / 16, p1 = (k1 + 15) / 16;
+    if (a.window > 0 || split != (int)blockIdx.x) {
+      next = p0 + ((warp - p0) & (WARPS - 1));
+      entry = next < p1 ? table[next] : 0;
     }
-    const int j0 = page * 16 + lane / 4;  // this lane's slots: j0, j0 + 8
+    int page = next;
+    uint32_t pages_ok = 0;  // of the pages in flight, the newest in bit 0: the table names one of the cache
+    auto fetch = [&](int stage) {
+      const bool ok = entry >= 0 && entry < a.pages;
+      pages_ok = pages_ok << 1 | (ok ? 1u : 0u);
+      if (next < p1) {
+        const long long at = ok ? ((long long)entry * a.hkv + h) * 16 * a.d * 2 : 0;
+        const int rows = ok ? min(16, q.n - next * 16) : 0;
+        const uint32_t dst = ring_at + stage * 2 * S::PAGE;
+        if (rows == 16 && a.d == DP) {  // a page lies in one piece
+          const char* k = a.k + at + lane * 16;
+          const char* v = a.v + at + lane * 16;
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++)
+          for (int i = 0; i < 16 * CP / 32; i++) {
+            const int c = lane + 32 * i;
+            aw_copy16(dst + c / CP * S::PITCH + c % CP * 16, k + i * 512, true, policy);
+            aw_copy16(dst + S::PAGE + c / CP * S::PITCH + c % CP * 16, v + i * 512, true, policy);
+          }
+        } else {
 #pragma unroll
-      for (int e = 0; e < 4; e++) s[nt][e] = (s[nt][e] + s_odd[nt][e]) * scale2;
-    const bool whole = page * 16 + 15 <= all_last && page * 16 >= all_from && page * 16 + 16 <= q.n && ok;
-    if (!whole) {
+          for (int i = 0; i < 16 * CP / 32; i++) {
+            const int c = lane + 32 * i, row = c / CP, col = c % CP;
+            if (col * 8 < a.d) {
+              const bool in = row < rows;
+              const long long off = at + (in ? (row * a.d + col * 8) * 2 : 0);
+              aw_copy16(dst + row * S::PITCH + col * 16, a.k + off, in, policy);
+              aw_copy16(dst + S::PAGE + row * S::PITCH + col * 16, a.v + off, in, policy);
+            }
+          }
+        }
+      }
+      aw_commit();
+      next += WARPS;
+      entry = next < p1 ? table[next] : 0;
+    };
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < S::STAGES - 1; i++) fetch(i);
+
+    float o[STEPS][NT][4];  // head values 16 i + lane / 4 (+ 8) of vectors 2 (lane mod 4) (+ 1)
+#pragma unroll
+    for (int i = 0; i < STEPS; i++)
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.f;
+    float m[NT][2], l[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) m[nt][0] = m[nt][1] = -INFINITY, l[nt][0] = l[nt][1] = 0.f;
+    for (int stage = 0; page < p1; page += WARPS) {
+      aw_wait<S::STAGES - 2>();
+      __syncwarp();
+      const bool ok = pages_ok >> (S::STAGES - 2) & 1;
+      const int ahead = stage + S::STAGES - 1;
+      fetch(ahead >= S::STAGES ? ahead - S::STAGES : ahead);
+      const uint32_t kp = ring_at + stage * 2 * S::PAGE, vp = kp + S::PAGE;
+      const char* v_page = ring + stage * 2 * S::PAGE + S::PAGE;
+      // slots lane / 4 (c0, c1) and + 8 (c2, c3) of vectors 2 (lane mod 4) and the next; even and odd steps apart, two
+      // shorter chains of products
+      float s[NT][4], s_odd[NT][4];
 #pragma unroll
       for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const int j = j0 + (e >> 1) * 8;
-          if (!ok || j > last[nt][e & 1] || j < from[nt][e & 1] || j >= q.n) s[nt][e] = -INFINITY;
-        }
-    }
-    bool more = false;
-    float top[NT][2];
+        for (int e = 0; e < 4; e++) s[nt][e] = s_odd[nt][e] = 0.f;
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++)
+      for (int st = 0; st < STEPS; st++) {
+        uint32_t ka[4];
+        aw_ldsm(ka, kp + k_off + st * 32);
+        uint32_t qb[4];
+        if (!S::Q_REGS) aw_ldsm(qb, q_off + st * 32);
 #pragma unroll
-      for (int e = 0; e < 2; e++) {
-        if (live[nt][e]) {
-          float* to = scores + (long long)(nt * 8 + e) * a.kv_pad + page * 16;
-          to[0] = s[nt][e];
-          to[8] = s[nt][e + 2];
+        for (int nt = 0; nt < NT; nt++) {
+          float* to = st & 1 ? s_odd[nt] : s[nt];
+          if (S::Q_REGS) Ty::mma(to, ka, qf[S::Q_REGS ? st : 0][nt][0], qf[S::Q_REGS ? st : 0][nt][1]);
+          else Ty::mma(to, ka, qb[2 * nt], qb[2 * nt + 1]);
         }
-        float x = fmaxf(s[nt][e], s[nt][e + 2]);
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-        top[nt][e] = fmaxf(m[nt][e], x - Ty::SHIFT);
-        more = more || top[nt][e] > m[nt][e];
       }
-    if (__any_sync(0xffffffffu, more)) {
+      const int j0 = page * 16 + lane / 4;  // this lane's slots: j0, j0 + 8
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) s[nt][e] = (s[nt][e] + s_odd[nt][e]) * scale2;
+      const bool whole = page * 16 + 15 <= all_last && page * 16 >= all_from && page * 16 + 16 <= q.n && ok;
+      if (!whole) {
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const int j = j0 + (e >> 1) * 8;
+            if (!ok || j > last[nt][e & 1] || j < from[nt][e & 1] || j >= q.n) s[nt][e] = -INFINITY;
+          }
+      }
+      bool more = false;
+      float top[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; nt++)
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-          const float f = top[nt][e] > m[nt][e] ? exp2f(m[nt][e] - top[nt][e]) : 1.f;
-          m[nt][e] = top[nt][e];
-          l[nt][e] *= f;
-#pragma unroll
-          for (int i = 0; i < STEPS; i++) o[i][nt][e] *= f, o[i][nt][e + 2] *= f;
+          if (live[nt][e]) {
+            float* to = scores + (long long)(nt * 8 + e) * a.kv_pad + page * 16;
+            to[0] = s[nt][e];
+            to[8] = s[nt][e + 2];
+          }
+          float x = fmaxf(s[nt][e], s[nt][e + 2]);
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+          top[nt][e] = fmaxf(m[nt][e], x - Ty::SHIFT);
+          more = more || top[nt][e] > m[nt][e];
         }
-    }
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const float base = m[nt][e & 1] == -INFINITY ? 0.f : m[nt][e & 1];
-        s[nt][e] = exp2f(s[nt][e] - base);
-        l[nt][e & 1] += s[nt][e];
-      }
-    bool by_mma = true;
-    if (!whole && (a.max_rows > 1 || a.window > 0)) {  // a row may be blind to a slot of this page that holds anything
-      bool fine = true;
-#pragma unroll 4
-      for (int c = lane; c < 16 * CP; c += 32) {
-        const uint4 x = *(const uint4*)(v_page + c / CP * S::PITCH + c % CP * 16);
-        fine = fine && Ty::finite(x.x) && Ty::finite(x.y) && Ty::finite(x.z) && Ty::finite(x.w);
-      }
-      by_mma = __all_sync(0xffffffffu, fine);
-    }
-    if (by_mma) {
-      uint32_t hi[NT][2], rest[NT][2];
-#pragma unroll
-      for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-          const uint2 x = Ty::parts(s[nt][2 * i], s[nt][2 * i + 1]);
-          hi[nt][i] = aw_turn(x.x), rest[nt][i] = aw_turn(x.y);
-        }
-#pragma unroll
-      for (int st = 0; st < STEPS; st++) {
-        uint32_t va[4];
-        aw_ldsm_t(va, vp + v_off + st * 32);
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++) Ty::mma(o[st][nt], va, hi[nt][0], hi[nt][1]);
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++) Ty::mma(o[st][nt], va, rest[nt][0], rest[nt][1]);
-      }
-    } else {
-#pragma unroll 1
-      for (int kk = 0; kk < 16; kk++) {
-        const int src = (kk & 7) * 4 + lane % 4, j = page * 16 + kk;
+      if (__any_sync(0xffffffffu, more)) {
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
           for (int e = 0; e < 2; e++) {
-            const float p = __shfl_sync(0xffffffffu, kk < 8 ? s[nt][e] : s[nt][e + 2], src);
-            if (j > last[nt][e] || j < from[nt][e] || j >= q.n) continue;
+            const float f = top[nt][e] > m[nt][e] ? exp2f(m[nt][e] - top[nt][e]) : 1.f;
+            m[nt][e] = top[nt][e];
+            l[nt][e] *= f;
 #pragma unroll
-            for (int i = 0; i < STEPS; i++) {
-              const T* v = (const T*)(v_page + kk * S::PITCH) + i * 16 + lane / 4;
-              o[i][nt][e] = fmaf(p, Ty::up(v[0]), o[i][nt][e]);
-              o[i][nt][e + 2] = fmaf(p, Ty::up(v[8]), o[i][nt][e + 2]);
-            }
+            for (int i = 0; i < STEPS; i++) o[i][nt][e] *= f, o[i][nt][e + 2] *= f;
           }
       }
-    }
-    __syncwarp();
-    stage = stage + 1 == S::STAGES ? 0 : stage + 1;
-  }
-  aw_wait<0>();
 #pragma unroll
-  for (int nt = 0; nt < NT; nt++)
+      for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-    for (int e = 0; e < 2; e++) {
-#pragma unroll
-      for (int x = 4; x < 32; x <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], x);
-      if (lane < 4) s_m[warp][nt * 8 + lane * 2 + e] = m[nt][e], s_l[warp][nt * 8 + lane * 2 + e] = l[nt][e];
-    }
-  __syncthreads();  // every warp is done with its ring, which now takes its accumulator
-#pragma unroll
-  for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-    for (int e = 0; e < 2; e++) {
-      const int row = nt * 8 + lane % 4 * 2 + e;
-      float top = s_m[0][row];
-#pragma unroll
-      for (int w = 1; w < WARPS; w++) top = fmaxf(top, s_m[w][row]);
-      const float f = m[nt][e] == -INFINITY ? 0.f : exp2f(m[nt][e] - top);
-      float* to = (float*)ring + row * S::JOIN + lane / 4;
-      if (live[nt][e]) {
-#pragma unroll
-        for (int i = 0; i < STEPS; i++) to[i * 16] = o[i][nt][e] * f, to[i * 16 + 8] = o[i][nt][e + 2] * f;
+        for (int e = 0; e < 4; e++) {
+          const float base = m[nt][e & 1] == -INFINITY ? 0.f : m[nt][e & 1];
+          s[nt][e] = exp2f(s[nt][e] - base);
+          l[nt][e & 1] += s[nt][e];
+        }
+      bool by_mma = true;
+      if (!whole && (a.max_rows > 1 || a.window > 0)) {  // a row may be blind to a slot of this page that holds anything
+        bool fine = true;
+#pragma unroll 4
+        for (int c = lane; c < 16 * CP; c += 32) {
+          const uint4 x = *(const uint4*)(v_page + c / CP * S::PITCH + c % CP * 16);
+          fine = fine && Ty::finite(x.x) && Ty::finite(x.y) && Ty::finite(x.z) && Ty::finite(x.w);
+        }
+        by_mma = __all_sync(0xffffffffu, fine);
       }
-    }
-  __syncthreads();
-  const long long at = (((long long)b * a.hkv + h) * a.splits + split) * a.vecs + tile * TILE;
-  const int count = min(TILE, vecs - tile * TILE);
-  for (int row = warp; row < count; row += WARPS)
-    for (int c = lane * 4; c < a.d; c += 128) {
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (by_mma) {
+        uint32_t hi[NT][2], rest[NT][2];
 #pragma unroll
-      for (int w = 0; w < WARPS; w++) {
-        const float4 y = *(const float4*)(smem + w * S::RING + (row * S::JOIN + c) * 4);
-        x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+          for (int i = 0; i < 2; i++) {
+            const uint2 x = Ty::parts(s[nt][2 * i], s[nt][2 * i + 1]);
+            hi[nt][i] = aw_turn(x.x), rest[nt][i] = aw_turn(x.y);
+          }
+#pragma unroll
+        for (int st = 0; st < STEPS; st++) {
+          uint32_t va[4];
+          aw_ldsm_t(va, vp + v_off + st * 32);
+#pragma unroll
+          for (int nt = 0; nt < NT; nt++) Ty::mma(o[st][nt], va, hi[nt][0], hi[nt][1]);
+#pragma unroll
+          for (int nt = 0; nt < NT; nt++) Ty::mma(o[st][nt], va, rest[nt][0], rest[nt][1]);
+        }
+      } else {
+#pragma unroll 1
+        for (int kk = 0; kk < 16; kk++) {
+          const int src = (kk & 7) * 4 + lane % 4, j = page * 16 + kk;
+#pragma unroll
+          for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+              const float p = __shfl_sync(0xffffffffu, kk < 8 ? s[nt][e] : s[nt][e + 2], src);
+              if (j > last[nt][e] || j < from[nt][e] || j >= q.n) continue;
+#pragma unroll
+              for (int i = 0; i < STEPS; i++) {
+                const T* v = (const T*)(v_page + kk * S::PITCH) + i * 16 + lane / 4;
+                o[i][nt][e] = fmaf(p, Ty::up(v[0]), o[i][nt][e]);
+                o[i][nt][e + 2] = fmaf(p, Ty::up(v[8]), o[i][nt][e + 2]);
+              }
+            }
+        }
       }
-      *(float4*)(a.parts + (at + row) * a.d + c) = x;
+      __syncwarp();
+      stage = stage + 1 == S::STAGES ? 0 : stage + 1;
     }
-  if (t < count) {
-    float mm = s_m[0][t];
+    aw_wait<0>();
 #pragma unroll
-    for (int w = 1; w < WARPS; w++) mm = fmaxf(mm, s_m[w][t]);
-    float sum = 0.f;
+    for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-    for (int w = 0; w < WARPS; w++) sum += s_m[w][t] == -INFINITY ? 0.f : exp2f(s_m[w][t] - mm) * s_l[w][t];
-    a.stats[at + t] = make_float2(mm, sum);
+      for (int e = 0; e < 2; e++) {
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], x);
+        if (lane < 4) s_m[warp][nt * 8 + lane * 2 + e] = m[nt][e], s_l[warp][nt * 8 + lane * 2 + e] = l[nt][e];
+      }
+    __syncthreads();  // every warp is done with its ring, which now takes its accumulator
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        const int row = nt * 8 + lane % 4 * 2 + e;
+        float top = s_m[0][row];
+#pragma unroll
+        for (int w = 1; w < WARPS; w++) top = fmaxf(top, s_m[w][row]);
+        const float f = m[nt][e] == -INFINITY ? 0.f : exp2f(m[nt][e] - top);
+        float* to = (float*)ring + row * S::JOIN + lane / 4;
+        if (live[nt][e]) {
+#pragma unroll
+          for (int i = 0; i < STEPS; i++) to[i * 16] = o[i][nt][e] * f, to[i * 16 + 8] = o[i][nt][e + 2] * f;
+        }
+      }
+    __syncthreads();
+    const long long at = (((long long)b * a.hkv + h) * a.splits + split) * a.vecs + tile * TILE;
+    const int count = min(TILE, vecs - tile * TILE);
+    for (int row = warp; row < count; row += WARPS)
+      for (int c = lane * 4; c < a.d; c += 128) {
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < WARPS; w++) {
+          const float4 y = *(const float4*)(smem + w * S::RING + (row * S::JOIN + c) * 4);
+          x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+        }
+        *(float4*)(a.parts + (at + row) * a.d + c) = x;
+      }
+    if (t < count) {
+      float mm = s_m[0][t];
+#pragma unroll
+      for (int w = 1; w < WARPS; w++) mm = fmaxf(mm, s_m[w][t]);
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; w++) sum += s_m[w][t] == -INFINITY ? 0.f : exp2f(s_m[w][t] - mm) * s_l[w][t];
+      a.stats[at + t] = make_float2(mm, sum);
+    }
+    __syncthreads();  // the ring is the copies' again
   }
 }
 
@@ -650,7 +657,7 @@ __global__ void __launch_bounds__(AW_FIN_THREADS) aw_finish_kernel(AwArgs a) {
 }
 
 struct AwPlan {
-  int kps, splits, tile, tiles;
+  int kps, splits, tile, tiles, seen;
   long long vecs, kv_pad;
   size_t scores, stats, parts;  // bytes
 };
@@ -680,6 +687,7 @@ static AwPlan aw_plan(int64_t B, int64_t rows, int64_t Hq, int64_t Hkv, int64_t 
   if (kps > p.kv_pad) kps = p.kv_pad;
   p.kps = (int)kps;
   p.splits = (int)((kv + kps - 1) / kps);
+  p.seen = window > 0 && (window + rows) / kps + 2 < p.splits ? (int)((window + rows) / kps + 2) : p.splits;
   const size_t heads = (size_t)B * Hkv;
   p.scores = aw_round(heads * p.vecs * p.kv_pad * 4);
   p.stats = aw_round(heads * p.splits * p.vecs * 8);
@@ -709,12 +717,11 @@ int launch_split_d(const AwArgs& a, dim3 grid, cudaStream_t st) {
 
 template <typename T>
 int launch_attention_weights(AwArgs& a, int64_t B, cudaStream_t st) {
-  const dim3 grid((unsigned)a.splits, (unsigned)(a.hkv * a.tiles), (unsigned)B);
+  const dim3 grid((unsigned)a.seen, (unsigned)(a.hkv * a.tiles), (unsigned)B);
   const int rc = a.vecs <= 8 ? launch_split_d<T, 1>(a, grid, st) : launch_split_d<T, 2>(a, grid, st);
   if (rc != IM_OK) return rc;
   // many splits that a row can see: a block's eight warps share a job's, else each has a job
-  const int64_t seen = a.window > 0 ? ((int64_t)a.window + a.max_rows) / a.kps + 2 : a.splits;
-  a.join_warps = seen >= 16 && a.splits >= 16 ? AW_FIN_THREADS / 32 : 1;
+  a.join_warps = a.seen >= 16 ? AW_FIN_THREADS / 32 : 1;
   a.joins = (int)(((int64_t)a.vecs * ((a.d + 127) / 128) * a.join_warps * 32 + AW_FIN_THREADS - 1) / AW_FIN_THREADS);
   // blocks of slots a (sequence, kv head): the device's worth in all, so that a block's sums serve many slots
   const int64_t most = (a.max_kv + AW_FIN_SLOTS - 1) / AW_FIN_SLOTS, share = (369 + B * a.hkv) / (B * a.hkv);
@@ -774,7 +781,7 @@ extern "C" int im_attention_weights(const void* q, const void* k_cache, const vo
   a.weights = weights, a.weights_out = weights_out, a.cap = cap;
   a.M = (int)M, a.max_rows = (int)max_rows_per_seq, a.hq = (int)Hq, a.hkv = (int)Hkv, a.d = (int)D;
   a.max_kv = (int)max_kv_len, a.kv_pad = (int)p.kv_pad, a.window = (int)window, a.scale = scale, a.out = (char*)out;
-  a.kps = p.kps, a.splits = p.splits, a.tiles = p.tiles, a.vecs = (int)p.vecs;
+  a.kps = p.kps, a.splits = p.splits, a.tiles = p.tiles, a.seen = p.seen, a.vecs = (int)p.vecs;
   a.wide_weights = aligned(weights, 16) && aligned(weights_out, 16);
   a.scores = (float*)workspace;
   a.stats = (float2*)((char*)workspace + p.scores);

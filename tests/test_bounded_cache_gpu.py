@@ -294,6 +294,17 @@ def test_attention_weights_splits(cuda, kps):
     attend_check(case, keys_per_split=kps, window=130)
 
 
+@pytest.mark.parametrize("window", [1, 20, 100])
+@pytest.mark.parametrize("kps", [0, 64])
+def test_attention_weights_of_rows_far_apart(cuda, window, kps):
+    """Rows of one sequence need not follow one another: with a window, slots between them are seen by none."""
+    q, k, v, table, bounds, slot, weights = attend_case(cuda, 8, [2000, 900], [6, 3], 8, 2, 128, torch.bfloat16)
+    slot[:] = ints([3, 1999, 700, 64, 1500, 90, 899, 0, 333], cuda)
+    attend_check((q, k, v, table, bounds, slot, weights), window=window, keys_per_split=kps)
+    attend_check((q, k, v, table, bounds, slot, weights), window=window, keys_per_split=kps, in_place=True)
+    attend_check((q, k, v, table, bounds, slot, weights), keys_per_split=kps)
+
+
 def test_attention_weights_bits_do_not_depend_on_the_launch(cuda):
     """With keys_per_split given, a row alone equals the same row in a batch, among other rows."""
     q, k, v, table, bounds, slot, weights = attend_case(cuda, 11, [700, 333, 64], [5, 3, 1], 8, 2, 128, torch.bfloat16)
