@@ -46,6 +46,7 @@ struct EvictArgs {
   int row_bytes;  // a slot's of one head
   long long budget, recent, sinks;
   int moves_here;  // the first kernel moves the slots too
+  int chunk_shift;  // log2 of a move's chunks (K's and V's), -1: no power of two
   int lengths_here;  // and writes lengths_out, which is not lengths
   int* moves;  // [rows]
   int* holes;  // [rows][most]
@@ -59,11 +60,13 @@ __device__ __forceinline__ int ev_length(const EvictArgs& a, int s) {
 }
 
 __device__ __forceinline__ uint32_t ev_key(float w, int pos, long long sinks, long long recent_from) {
-  if (pos < sinks || pos >= recent_from) return 0xffffffffu;
-  if (w != w) return 0u;
   const uint32_t b = __float_as_uint(w + 0.0f);  // -0 as +0
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
+  const uint32_t k = w != w ? 0u : b ^ ((uint32_t)((int)b >> 31) | 0x80000000u);
+  return pos < sinks || pos >= recent_from ? 0xffffffffu : k;
 }
+
+// Where a digit is counted: the eight that a lane reads lie 32 apart.
+__device__ __forceinline__ int ev_bin(int digit) { return (digit & 7) * 32 + (digit >> 3); }
 
 // Sums of x over the block's warps before this one, and over all; x is the same in a warp's lanes.
 template <int WARPS>
@@ -81,8 +84,9 @@ __device__ __forceinline__ int2 ev_before(int x, int* scratch) {
 }
 
 // Up to 32 moves of one row by a warp: each lane has one move's slots; the warp then copies their rows together, BYTES a
-// lane, K's and V's chunks of a move side by side, BATCH loads in flight a lane.
-template <int BYTES, int BATCH>
+// lane, K's and V's chunks of a move side by side, four loads in flight a lane (with eight, at half the
+// warps an SM, a prompt's cut took 111 us in the place of 106).
+template <int BYTES>
 __device__ __forceinline__ void ev_move(const EvictArgs& a, long long row, int moves, int to, int from) {
   const int head = (int)(row % a.hkv), seq = (int)(row / a.hkv % a.seqs), lane = threadIdx.x & 31;
   const int* table = a.page_table + seq * a.max_pages;
@@ -98,6 +102,7 @@ __device__ __forceinline__ void ev_move(const EvictArgs& a, long long row, int m
       src = layer + ((from_page * a.hkv + head) * 16 + from % 16) * a.row_bytes;
     }
   }
+  constexpr int BATCH = 4;
   const int work = moves * 2 * chunks;
   for (int c0 = 0; c0 < work; c0 += 32 * BATCH) {
     uint4 x[BATCH];
@@ -105,7 +110,7 @@ __device__ __forceinline__ void ev_move(const EvictArgs& a, long long row, int m
 #pragma unroll
     for (int i = 0; i < BATCH; i++) {
       const int c = c0 + i * 32 + lane;
-      const int move = c / (2 * chunks), part = c - move * 2 * chunks;
+      const int move = a.chunk_shift >= 0 ? c >> a.chunk_shift : c / (2 * chunks), part = c - move * 2 * chunks;
       const long long here = __shfl_sync(0xffffffffu, src, move & 31);
       const long long there = __shfl_sync(0xffffffffu, dst, move & 31);
       at[i] = nullptr;
@@ -162,10 +167,17 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) evict_select_kernel(EvictArgs
   const int items = (n + ranks * THREADS - 1) / (ranks * THREADS);  // at most ITEMS
   const int first = (rank * WARPS + warp) * 32 * items + lane;      // this lane's slots: 32 apart
   uint32_t key[ITEMS];
+  {
+    float wv[ITEMS];  // all on their way before the first is used
+    int pv[ITEMS];
 #pragma unroll
-  for (int i = 0; i < ITEMS; i++) {
-    const int s = first + 32 * i;
-    key[i] = i < items && s < n ? ev_key(w[s], pos[s], a.sinks, recent_from) : 0u;
+    for (int i = 0; i < ITEMS; i++) {
+      const int s = min(first + 32 * i, n - 1);
+      wv[i] = 0.f, pv[i] = 0;
+      if (i < items) wv[i] = w[s], pv[i] = pos[s];
+    }
+#pragma unroll
+    for (int i = 0; i < ITEMS; i++) key[i] = ev_key(wv[i], pv[i], a.sinks, recent_from);
   }
   for (int i = t; i < 512; i += THREADS) hist[0][i] = 0;
   const int mine = first - lane < n ? min(items, (n - first + 31) / 32) : 0;  // slots of this lane (may be 0)
@@ -179,7 +191,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) evict_select_kernel(EvictArgs
     unsigned* h = hist[turn];
 #pragma unroll
     for (int i = 0; i < ITEMS; i++)
-      if (i < mine && (key[i] & mask) == border) atomicAdd(&h[key[i] >> shift & 255], 1u);
+      if (i < mine && (key[i] & mask) == border) atomicAdd(&h[ev_bin(key[i] >> shift & 255)], 1u);
     if (ranks > 1) cluster.sync();
     else __syncthreads();
     if (warp == 0) {  // eight digits a lane, from the highest down
@@ -188,9 +200,9 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) evict_select_kernel(EvictArgs
       for (int i = 0; i < 8; i++) {
         const int d = 255 - lane * 8 - i;
         c[i] = 0;
-        if (ranks == 1) c[i] = h[d];
+        if (ranks == 1) c[i] = h[ev_bin(d)];
         else
-          for (int r = 0; r < ranks; r++) c[i] += *cluster.map_shared_rank(&h[d], r);
+          for (int r = 0; r < ranks; r++) c[i] += *cluster.map_shared_rank(&h[ev_bin(d)], r);
         sum += c[i];
       }
       unsigned above = sum;
@@ -278,15 +290,16 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) evict_select_kernel(EvictArgs
     return;
   }
   __syncthreads();
-  for (int i0 = warp * 32; i0 < total; i0 += THREADS) {
-    const int moves = min(32, total - i0);
-    ev_move<BYTES, 4>(a, row, moves, lane < moves ? pairs[i0 + lane] : 0, lane < moves ? pairs[a.most + i0 + lane] : 0);
+  const int share = min(32, (total + WARPS - 1) / WARPS);  // moves of a warp at a time
+  for (int i0 = warp * share; i0 < total; i0 += WARPS * share) {
+    const int moves = min(share, total - i0);
+    ev_move<BYTES>(a, row, moves, lane < moves ? pairs[i0 + lane] : 0, lane < moves ? pairs[a.most + i0 + lane] : 0);
   }
 }
 
 // The moves of all rows from the workspace, and the lengths, which nobody reads any more.
 template <int BYTES>
-__global__ void __launch_bounds__(EV_MOVE_THREADS, 3) evict_move_kernel(EvictArgs a) {
+__global__ void __launch_bounds__(EV_MOVE_THREADS, 6) evict_move_kernel(EvictArgs a) {
   pdl_wait();
   pdl_trigger();
   const long long row = blockIdx.x;
@@ -298,7 +311,7 @@ __global__ void __launch_bounds__(EV_MOVE_THREADS, 3) evict_move_kernel(EvictArg
   for (int i0 = (blockIdx.y * (EV_MOVE_THREADS / 32) + threadIdx.x / 32) * 32; i0 < count;
        i0 += gridDim.y * EV_MOVE_THREADS) {
     const int moves = min(32, count - i0);
-    ev_move<BYTES, BYTES == 16 ? 8 : 4>(a, row, moves, lane < moves ? a.holes[row * a.most + i0 + lane] : 0,
+    ev_move<BYTES>(a, row, moves, lane < moves ? a.holes[row * a.most + i0 + lane] : 0,
                                         lane < moves ? a.movers[row * a.most + i0 + lane] : 0);
   }
 }
@@ -320,16 +333,18 @@ template <int BYTES>
 int launch_evict(EvictArgs& a, long long rows, cudaStream_t st) {
   int ranks = 1;
   while ((long long)ranks * EV_RUN < a.cap) ranks *= 2;
-  a.moves_here = ranks == 1 && (rows >= 148 || a.most <= 512);
+  a.moves_here = ranks == 1 && a.most <= 1024;
   a.lengths_here = a.lengths_out != a.lengths;
+  const int chunks = 2 * (a.row_bytes / BYTES);
+  a.chunk_shift = (chunks & (chunks - 1)) == 0 ? __builtin_ctz(chunks) : -1;
   const int rc = a.cap <= 2048   ? launch_evict_select<256, 8, 4, BYTES>(a, rows, ranks, st)
                  : a.cap <= 4096 ? launch_evict_select<512, 8, 2, BYTES>(a, rows, ranks, st)
                  : a.cap <= 8192 ? launch_evict_select<512, 16, 2, BYTES>(a, rows, ranks, st)
                                  : launch_evict_select<1024, 16, 1, BYTES>(a, rows, ranks, st);
   if (rc != IM_OK || (a.moves_here && a.lengths_here)) return rc;
-  const long long chunks = a.moves_here || a.most <= 0 ? 1 : (a.most + EV_MOVE_THREADS - 1) / EV_MOVE_THREADS;
+  const long long blocks = a.moves_here || a.most <= 0 ? 1 : (a.most + EV_MOVE_THREADS - 1) / EV_MOVE_THREADS;
   return launch("evict_move_kernel", evict_move_kernel<BYTES>,
-                dim3((unsigned)rows, (unsigned)(chunks < 1024 ? chunks : 1024)), dim3(EV_MOVE_THREADS), 0, st, a);
+                dim3((unsigned)rows, (unsigned)(blocks < 1024 ? blocks : 1024)), dim3(EV_MOVE_THREADS), 0, st, a);
 }
 
 static long long evict_most(int64_t cap, int64_t budget) { return budget < cap - budget ? budget : cap - budget; }

@@ -6,9 +6,10 @@
 // float32 product would be off by 0.06 rad. What is left of it is within 2^-26 quarter turns, so c and s are float32
 // exact to an ulp or two wherever the position is. Rotations are float32, rounded once to the rows' type.
 //
-// Bound: HBM, every value read and written once. A block takes a row (a part of one where rows are few, several where they
-// are short), works c and s out once (R/2 of them a row) and uses them for every head from shared memory; the first values
-// are on their way meanwhile. Values move 16 bytes a thread.
+// Bound: HBM, every value read and written once. A warp takes a part of a row's heads, for itself: it works the row's c and
+// s out (R/2 of them, two or so a lane), hands them over in shared memory of its own, and walks the heads; a lane keeps to
+// one run of pairs, whose c and s it holds in registers. Nothing waits for another warp, so some load while others work:
+// 8192 rows of 48 heads of 128 took 50 us with a block a row and a barrier behind c and s.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -16,9 +17,8 @@
 
 namespace im {
 
-constexpr int RP_THREADS = 256;
-constexpr int RP_ROWS = 16;   // rows a block at most
-constexpr int RP_BATCH = 2;   // units a thread has on their way
+constexpr int RP_WARPS = 8;  // of a block, where their c and s fit 48 KB
+constexpr int RP_HEADS = 3;  // heads that a lane has on their way
 
 struct RopeArgs {
   const char* x;            // rows
@@ -30,8 +30,8 @@ struct RopeArgs {
   int inverse, interleaved;
   int rotary, d;
   int heads;           // heads of a row that the launch walks (rope_kv: q, k and v heads)
-  int heads_per_block;
-  int rows_per_block;
+  int parts, heads_per_part;  // of a row's heads, a warp each
+  int lanes;                  // units of a row that lie side by side in a warp
   long long rows;
   char* out;
   long long o_row, o_head;
@@ -47,22 +47,33 @@ struct RopeArgs {
   long long cap;
 };
 
+// Values as float32 and back, singly and two at a time (one conversion instruction for two 16-bit values).
 template <typename T>
 struct RopeType;
 template <>
 struct RopeType<__nv_bfloat16> {
   static __device__ __forceinline__ float up(__nv_bfloat16 v) { return __bfloat162float(v); }
   static __device__ __forceinline__ __nv_bfloat16 down(float v) { return __float2bfloat16_rn(v); }
+  static __device__ __forceinline__ float2 up2(const __nv_bfloat16* v) {
+    return __bfloat1622float2(*(const __nv_bfloat162*)v);
+  }
+  static __device__ __forceinline__ void down2(__nv_bfloat16* v, float x, float y) {
+    *(__nv_bfloat162*)v = __floats2bfloat162_rn(x, y);
+  }
 };
 template <>
 struct RopeType<__half> {
   static __device__ __forceinline__ float up(__half v) { return __half2float(v); }
   static __device__ __forceinline__ __half down(float v) { return __float2half_rn(v); }
+  static __device__ __forceinline__ float2 up2(const __half* v) { return __half22float2(*(const __half2*)v); }
+  static __device__ __forceinline__ void down2(__half* v, float x, float y) { *(__half2*)v = __floats2half2_rn(x, y); }
 };
 template <>
 struct RopeType<float> {
   static __device__ __forceinline__ float up(float v) { return v; }
   static __device__ __forceinline__ float down(float v) { return v; }
+  static __device__ __forceinline__ float2 up2(const float* v) { return make_float2(v[0], v[1]); }
+  static __device__ __forceinline__ void down2(float* v, float x, float y) { v[0] = x, v[1] = y; }
 };
 
 template <typename T, int VEC>
@@ -91,133 +102,134 @@ __device__ __forceinline__ float2 rope_turn(double p, double f, float factor, bo
   return make_float2(factor * c, factor * s);
 }
 
-// One block: `heads_per_block` heads of `rows_per_block` rows. VEC values a load; a unit is two loads of a half-layout pair
-// of runs, or one load of neighbouring pairs, or one load of the part that is copied (VEC 1: one pair, or one value).
+// A unit is VEC values: neighbouring pairs (interleaved), or the first halves of VEC pairs with the second halves `pairs`
+// further on; VEC 1 is one pair, wherever its values lie.
 template <typename T, int VEC, bool KV>
-__global__ void __launch_bounds__(RP_THREADS) rope_kernel(RopeArgs a) {
+__global__ void __launch_bounds__(RP_WARPS * 32) rope_kernel(RopeArgs a) {
   typedef RopeVec<T, VEC> V;
-  extern __shared__ float2 turn[];       // [rows][R / 2]
-  __shared__ long long s_cache[RP_ROWS];  // where a row's keys and values go: head 0's, in values; -1: nowhere
+  extern __shared__ float2 turns_of[];  // [warps][R / 2]
   pdl_wait();
   pdl_trigger();
-  const int t = threadIdx.x;
-  const long long m0 = (long long)blockIdx.x * a.rows_per_block;
-  const int rows = (int)min((long long)a.rows_per_block, a.rows - m0);
-  const int h0 = blockIdx.y * a.heads_per_block, heads = min(a.heads, h0 + a.heads_per_block) - h0;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long id = (long long)blockIdx.x * (blockDim.x / 32) + warp, m = id / a.parts;
+  if (m >= a.rows) return;
+  const int h0 = (int)(id - m * a.parts) * a.heads_per_part, h1 = min(a.heads, h0 + a.heads_per_part);
   const int pairs = a.rotary / 2;
-  const int turned = a.interleaved && VEC > 1 ? a.rotary / VEC : pairs / VEC;
-  const int units = turned + (a.d - a.rotary) / VEC, row_units = heads * units;
-  const int total = rows * row_units;
-  // exact for numbers under 2^22
-  const float per_row = 1.f / row_units, per_head = 1.f / units;
-  auto place = [&](int idx, int& r, int& h, int& u) {
-    r = (int)((idx + 0.5f) * per_row);
-    const int rest = idx - r * row_units;
-    h = (int)((rest + 0.5f) * per_head);
-    u = rest - h * units;
-    h += h0;
-  };
-  V v[RP_BATCH], w[RP_BATCH];
-  auto load = [&](int idx0) {
-    if constexpr (VEC > 1) {  // single values are read where they are turned
+  float2* turn = turns_of + warp * pairs;
+  const bool near = a.interleaved;
+  const int units = near && VEC > 1 ? a.rotary / VEC : pairs / VEC;
+  // this lane's first unit and head: a.lanes units side by side, as many heads as fit
+  const int groups = 32 / a.lanes, g = lane / a.lanes;
+  int u = lane - g * a.lanes;
+  const int h_first = h0 + g;
+  const bool works = g < groups && units > 0;
+  const T* src = (const T*)a.x + m * a.x_row;
+  V v[RP_HEADS], w[RP_HEADS];
+  auto load = [&](int h) {
 #pragma unroll
-      for (int i = 0; i < RP_BATCH; i++) {
-        const int idx = idx0 + i * RP_THREADS;
-        if (idx < total) {
-          int r, h, u;
-          place(idx, r, h, u);
-          const T* src = (const T*)a.x + (m0 + r) * a.x_row + h * a.x_head;
-          if (u >= turned) {
-            v[i] = *(const V*)(src + a.rotary + (u - turned) * VEC);
-          } else {
-            v[i] = *(const V*)(src + u * VEC);
-            if (!a.interleaved) w[i] = *(const V*)(src + u * VEC + pairs);
-          }
+    for (int i = 0; i < RP_HEADS; i++) {
+      if (h + i * groups < h1) {
+        const T* p = src + (h + i * groups) * a.x_head;
+        if constexpr (VEC > 1) {
+          v[i] = *(const V*)(p + u * VEC);
+          if (!near) w[i] = *(const V*)(p + u * VEC + pairs);
+        } else {
+          v[i].v[0] = p[near ? 2 * u : u];
+          w[i].v[0] = p[near ? 2 * u + 1 : u + pairs];
         }
       }
     }
   };
-  load(t);
-  for (int i = t; i < rows * pairs; i += RP_THREADS) {
-    const int r = i / pairs, pair = i - r * pairs;
-    const double p = a.pos64 ? (double)((const long long*)a.pos)[m0 + r] : (double)((const int*)a.pos)[m0 + r];
-    const double f = a.freq64 ? ((const double*)a.freq)[pair] : (double)((const float*)a.freq)[pair];
-    turn[i] = rope_turn(p, f, (float)a.factor, a.inverse != 0);
-  }
-  if (KV && t < rows) {  // rows without a slot of the cache are turned, and written nowhere
-    const long long slot = a.row_slot[m0 + t], seq = a.row_seq[m0 + t];
-    long long at = -1;
+  if (works) load(h_first);
+  const double p = a.pos64 ? (double)((const long long*)a.pos)[m] : (double)((const int*)a.pos)[m];
+  // where the row's key and value of head 0 go; a row without a slot of the cache is turned, and written nowhere
+  long long cache = -1;
+  if (KV) {
+    const long long slot = a.row_slot[m], seq = a.row_seq[m];
     if (slot >= 0 && slot < a.max_pages * 16 && seq >= 0 && seq < a.seqs) {
       const long long page = a.page_table[seq * a.max_pages + slot / 16];
-      if (page >= 0 && page < a.pages) at = (page * a.hkv * 16 + slot % 16) * a.d;
+      if (page >= 0 && page < a.pages) cache = (page * a.hkv * 16 + slot % 16) * a.d;
     }
-    s_cache[t] = at;
-    if (a.slot_pos && at >= 0 && slot < a.cap && blockIdx.y == 0) {
-      const int pos = ((const int*)a.pos)[m0 + t];
-      for (int h = 0; h < a.hkv; h++) a.slot_pos[(seq * a.hkv + h) * a.cap + slot] = pos;
-    }
+    if (a.slot_pos && cache >= 0 && slot < a.cap && h0 == 0)
+      for (int h = lane; h < a.hkv; h += 32) a.slot_pos[(seq * a.hkv + h) * a.cap + slot] = ((const int*)a.pos)[m];
   }
-  __syncthreads();
-  for (int idx0 = t; idx0 < total; idx0 += RP_BATCH * RP_THREADS) {
-    if (idx0 != t) load(idx0);
+  // where head h goes (nullptr: nowhere), and whether it is turned
+  auto place = [&](int h, bool& turns) -> T* {
+    turns = true;
+    if (!KV || h < a.hq) return (T*)a.out + m * a.o_row + h * a.o_head;
+    turns = h < a.hq + a.hkv;
+    if (cache < 0) return nullptr;
+    return (T*)(turns ? a.k_cache : a.v_cache) + cache + (long long)(h - a.hq - (turns ? 0 : a.hkv)) * 16 * a.d;
+  };
+  // what is copied as it is, while the first heads are on their way
+  const int rest = (a.d - a.rotary) / VEC;
+#pragma unroll 4
+  for (int idx = lane; idx < (h1 - h0) * rest; idx += 32) {
+    const int head = idx / rest, at = a.rotary + (idx - head * rest) * VEC;
+    bool turns;
+    T* dst = place(h0 + head, turns);
+    if (dst) *(V*)(dst + at) = *(const V*)(src + (h0 + head) * a.x_head + at);
+  }
+  for (int i = lane; i < pairs; i += 32) {
+    const double f = a.freq64 ? ((const double*)a.freq)[i] : (double)((const float*)a.freq)[i];
+    turn[i] = rope_turn(p, f, (float)a.factor, a.inverse != 0);
+  }
+  __syncwarp();
+  if (works) {
+    for (bool loaded = true; u < units; u += a.lanes) {
+      float c[VEC], s[VEC];  // of VEC pairs; of half as many where they lie side by side
+      const float2* from = turn + (near && VEC > 1 ? u * VEC / 2 : u * VEC);
 #pragma unroll
-    for (int i = 0; i < RP_BATCH; i++) {
-      const int idx = idx0 + i * RP_THREADS;
-      if (idx >= total) continue;
-      int r, h, u;
-      place(idx, r, h, u);
-      T* dst;
-      bool turns = true;
-      if (!KV || h < a.hq) {
-        dst = (T*)a.out + (m0 + r) * a.o_row + h * a.o_head;
-      } else {
-        turns = h < a.hq + a.hkv;
-        if (s_cache[r] < 0) continue;
-        dst = (T*)(turns ? a.k_cache : a.v_cache) + s_cache[r] + (long long)(turns ? h - a.hq : h - a.hq - a.hkv) * 16 * a.d;
+      for (int e = 0; e < VEC; e++) {
+        if (e < (VEC + 1) / 2 || !near) {
+          const float2 x = from[e];
+          c[e] = x.x, s[e] = x.y;
+        }
       }
-      const float2* c = turn + r * pairs;
-      if (VEC == 1) {
-        const T* src = (const T*)a.x + (m0 + r) * a.x_row + h * a.x_head;
-        if (u >= turned) {
-          dst[a.rotary + u - turned] = src[a.rotary + u - turned];
-          continue;
-        }
-        const int at = a.interleaved ? 2 * u : u, to = a.interleaved ? at + 1 : at + pairs;
-        const T x = src[at], y = src[to];
-        if (turns) {
-          const float fx = RopeType<T>::up(x), fy = RopeType<T>::up(y);
-          dst[at] = RopeType<T>::down(fmaf(fx, c[u].x, -(fy * c[u].y)));
-          dst[to] = RopeType<T>::down(fmaf(fx, c[u].y, fy * c[u].x));
-        } else {
-          dst[at] = x;
-          dst[to] = y;
-        }
-      } else if (u >= turned) {
-        *(V*)(dst + a.rotary + (u - turned) * VEC) = v[i];
-      } else if (a.interleaved) {
-        if (turns) {
+      for (int h = h_first; h < h1; h += RP_HEADS * groups, loaded = false) {
+        if (!loaded) load(h);
 #pragma unroll
-          for (int e = 0; e + 1 < VEC; e += 2) {
-            const float2 k = c[(u * VEC + e) / 2];
-            const float x = RopeType<T>::up(v[i].v[e]), y = RopeType<T>::up(v[i].v[e + 1]);
-            v[i].v[e] = RopeType<T>::down(fmaf(x, k.x, -(y * k.y)));
-            v[i].v[e + 1] = RopeType<T>::down(fmaf(x, k.y, y * k.x));
+        for (int i = 0; i < RP_HEADS; i++) {
+          if (h + i * groups >= h1) continue;
+          bool turns;
+          T* dst = place(h + i * groups, turns);
+          if (!dst) continue;
+          if constexpr (VEC > 1) {
+            if (near) {
+              if (turns) {
+#pragma unroll
+                for (int e = 0; e < VEC; e += 2) {
+                  const float2 x = RopeType<T>::up2(v[i].v + e);
+                  RopeType<T>::down2(v[i].v + e, fmaf(x.x, c[e / 2], -(x.y * s[e / 2])),
+                                     fmaf(x.x, s[e / 2], x.y * c[e / 2]));
+                }
+              }
+              *(V*)(dst + u * VEC) = v[i];
+              continue;
+            }
+            if (turns) {
+#pragma unroll
+              for (int e = 0; e < VEC; e += 2) {
+                const float2 x = RopeType<T>::up2(v[i].v + e), y = RopeType<T>::up2(w[i].v + e);
+                RopeType<T>::down2(v[i].v + e, fmaf(x.x, c[e], -(y.x * s[e])), fmaf(x.y, c[e + 1], -(y.y * s[e + 1])));
+                RopeType<T>::down2(w[i].v + e, fmaf(x.x, s[e], y.x * c[e]), fmaf(x.y, s[e + 1], y.y * c[e + 1]));
+              }
+            }
+          } else if (turns) {
+            const float x = RopeType<T>::up(v[i].v[0]), y = RopeType<T>::up(w[i].v[0]);
+            v[i].v[0] = RopeType<T>::down(fmaf(x, c[0], -(y * s[0])));
+            w[i].v[0] = RopeType<T>::down(fmaf(x, s[0], y * c[0]));
+          }
+          if constexpr (VEC > 1) {
+            *(V*)(dst + u * VEC) = v[i];
+            *(V*)(dst + u * VEC + pairs) = w[i];
+          } else {
+            dst[near ? 2 * u : u] = v[i].v[0];
+            dst[near ? 2 * u + 1 : u + pairs] = w[i].v[0];
           }
         }
-        *(V*)(dst + u * VEC) = v[i];
-      } else {
-        if (turns) {
-#pragma unroll
-          for (int e = 0; e < VEC; e++) {
-            const float2 k = c[u * VEC + e];
-            const float x = RopeType<T>::up(v[i].v[e]), y = RopeType<T>::up(w[i].v[e]);
-            v[i].v[e] = RopeType<T>::down(fmaf(x, k.x, -(y * k.y)));
-            w[i].v[e] = RopeType<T>::down(fmaf(x, k.y, y * k.x));
-          }
-        }
-        *(V*)(dst + u * VEC) = v[i];
-        *(V*)(dst + u * VEC + pairs) = w[i];
       }
+      loaded = false;
     }
   }
 }
@@ -225,20 +237,23 @@ __global__ void __launch_bounds__(RP_THREADS) rope_kernel(RopeArgs a) {
 template <typename T, bool KV>
 int launch_rope(RopeArgs& a, long long M, bool vec, cudaStream_t st) {
   constexpr int WIDE = 16 / sizeof(T);
-  const int n = vec ? WIDE : 1;
-  const int units = (a.interleaved && vec ? a.rotary / n : a.rotary / 2 / n) + (a.d - a.rotary) / n;
-  // few rows: their heads are spread over several blocks, so that one row's are not one block's latency; many:
-  // several a block, so that every thread works out a pair's c and s
-  int blocks_y = 1, rows = 1;
-  while (M * blocks_y < 148 && blocks_y * 4 < a.heads) blocks_y *= 2;
-  while (rows < RP_ROWS && rows * 2 * (a.rotary / 2) <= RP_THREADS && M >= rows * 2 * 592) rows *= 2;
-  a.rows = M, a.rows_per_block = rows;
-  a.heads_per_block = (a.heads + blocks_y - 1) / blocks_y;
-  blocks_y = (a.heads + a.heads_per_block - 1) / a.heads_per_block;
-  const dim3 grid((unsigned)((M + rows - 1) / rows), (unsigned)blocks_y);
-  const size_t smem = sizeof(float2) * rows * (a.rotary / 2);
-  if (vec) return launch("rope_kernel", rope_kernel<T, WIDE, KV>, grid, dim3(RP_THREADS), smem, st, a);
-  return launch("rope_kernel", rope_kernel<T, 1, KV>, grid, dim3(RP_THREADS), smem, st, a);
+  const int pairs = a.rotary / 2;
+  const int units = !vec ? pairs : a.interleaved ? a.rotary / WIDE : pairs / WIDE;
+  a.lanes = units < 1 ? 1 : units < 32 ? units : 32;
+  // parts of a row: so many that the device has three rounds of warps, as long as a part is a load of every lane
+  const int least = RP_HEADS * (32 / a.lanes);
+  int parts = 1;
+  while (M * parts < 148 * 32 * 3 && a.heads >= parts * 2 * least) parts *= 2;
+  a.rows = M, a.heads_per_part = (a.heads + parts - 1) / parts;
+  a.parts = (a.heads + a.heads_per_part - 1) / a.heads_per_part;
+  int warps = RP_WARPS;
+  while (warps * pairs * sizeof(float2) > 48 * 1024) warps /= 2;
+  const long long blocks = (M * a.parts + warps - 1) / warps;
+  IM_REQUIRE(blocks < (1ll << 31), IM_UNSUPPORTED, "rope_kernel: too many rows");
+  const size_t smem = warps * pairs * sizeof(float2);
+  const dim3 grid((unsigned)blocks), block(warps * 32);
+  if (vec) return launch("rope_kernel", rope_kernel<T, WIDE, KV>, grid, block, smem, st, a);
+  return launch("rope_kernel", rope_kernel<T, 1, KV>, grid, block, smem, st, a);
 }
 
 template <bool KV>
