@@ -772,23 +772,34 @@ _LAYOUTS = {"half": _lib.ROPE_HALF, "interleaved": _lib.ROPE_INTERLEAVED}
 PAGE_SLOTS = 16
 
 
-def _launch(device: torch.device, name: str, *args) -> None:
-    """_lib.call with the device current, whichever is."""
-    if torch._C._cuda_getDevice() == device.index:
-        _lib.call(name, *args)
+def _launch(index: int, name: str, *args) -> None:
+    """_lib.call on a device's current stream (the entry point's last argument), with the device current."""
+    if torch._C._cuda_getDevice() == index:
+        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(device):
-            _lib.call(name, *args)
+        with torch.cuda.device(index):
+            _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+
+
+def _need(t: torch.Tensor, name: str, dtype: torch.dtype, device: torch.device, index: int) -> None:
+    """_check for one type; what fits costs a third of it."""
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == index and t.is_contiguous()):
+        _check(t, name, (dtype,), device)
 
 
 def _disjoint_or_same(a: torch.Tensor, name_a: str, b: torch.Tensor, name_b: str) -> None:
-    """Refuse tensors that overlap without being one (contiguous, or strided with positive strides)."""
-    def ends(t: torch.Tensor) -> tuple[int, int]:
-        last = sum((n - 1) * st for n, st in zip(t.shape, t.stride())) if t.numel() else -1
-        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+    """Refuse tensors that overlap without being one (strides are not negative)."""
+    if a is b:
+        return
 
-    (a0, a1), (b0, b1) = ends(a), ends(b)
-    if a0 < b1 and b0 < a1 and not (a0 == b0 and a.shape == b.shape and a.stride() == b.stride()):
+    def end(t: torch.Tensor) -> int:
+        if t.is_contiguous():
+            return t.data_ptr() + t.numel() * t.element_size()
+        last = sum((n - 1) * st for n, st in zip(t.shape, t.stride())) if t.numel() else -1
+        return t.data_ptr() + (last + 1) * t.element_size()
+
+    a0, b0 = a.data_ptr(), b.data_ptr()
+    if a0 < end(b) and b0 < end(a) and not (a0 == b0 and a.shape == b.shape and a.stride() == b.stride()):
         raise ValueError(f"{name_a} overlaps {name_b} without being the same tensor")
 
 
@@ -827,15 +838,17 @@ def rope_frequencies(rotary: int, base: float, *, scaling: str = "none", stretch
     return freq.to(device), factor
 
 
-def _rope_table(inv_freq: torch.Tensor, layout: str, d: int, device: torch.device) -> tuple[int, int]:
-    """(rotary, layout) of a table checked against the head size."""
-    _check(inv_freq, "inv_freq", (torch.float32, torch.float64), device)
-    if layout not in _LAYOUTS:
+def _rope_table(inv_freq: torch.Tensor, layout: str, d: int, device: torch.device, index: int) -> tuple[int, int, int]:
+    """(rotary, layout, whether in float64) of a table checked against the head size."""
+    wide = isinstance(inv_freq, torch.Tensor) and inv_freq.dtype is torch.float64
+    _need(inv_freq, "inv_freq", torch.float64 if wide else torch.float32, device, index)
+    lay = _LAYOUTS.get(layout)
+    if lay is None:
         raise ValueError(f"layout {layout!r}: half or interleaved")
     rotary = 2 * inv_freq.numel()
     if inv_freq.dim() != 1 or rotary > d:
         raise ValueError(f"inv_freq {tuple(inv_freq.shape)} turns {rotary} of a head's {d} values")
-    return rotary, _LAYOUTS[layout]
+    return rotary, lay, int(wide)
 
 
 def rope(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, layout: str = "half", factor: float = 1.0,
@@ -850,10 +863,12 @@ def rope(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, la
         raise ValueError(f"x must be [M, H, D] with contiguous heads, got {tuple(x.shape)}, strides {x.stride()}")
     m, h, d = x.shape
     device = x.device
-    _check(positions, "positions", (torch.int32, torch.int64), device)
+    index = device.index
+    wide = isinstance(positions, torch.Tensor) and positions.dtype is torch.int64
+    _need(positions, "positions", torch.int64 if wide else torch.int32, device, index)
     if positions.shape != (m,):
         raise ValueError(f"positions must be [{m}], got {tuple(positions.shape)}")
-    rotary, lay = _rope_table(inv_freq, layout, d, device)
+    rotary, lay, freq64 = _rope_table(inv_freq, layout, d, device, index)
     if out is None:
         out = torch.empty((m, h, d), dtype=x.dtype, device=device)
     else:
@@ -866,36 +881,41 @@ def rope(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, la
             raise ValueError(f"out must hold every head apart and contiguous, its strides are {out.stride()}")
         _disjoint_or_same(out, "out", x, "x")
     if x.numel():
-        _launch(device, "im_rope", x.data_ptr(), x.stride(0), x.stride(1), positions.data_ptr(),
-                int(positions.dtype == torch.int64), inv_freq.data_ptr(), int(inv_freq.dtype == torch.float64), rotary,
-                float(factor), lay, int(inverse), m, h, d, _TYPES[x.dtype], out.data_ptr(), out.stride(0), out.stride(1),
-                _stream(device))
+        _launch(index, "im_rope", x.data_ptr(), x.stride(0), x.stride(1), positions.data_ptr(),
+                int(wide), inv_freq.data_ptr(), freq64, rotary, float(factor), lay, int(inverse), m, h, d,
+                _TYPES[x.dtype], out.data_ptr(), out.stride(0), out.stride(1))
     return out
 
 
 def _check_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, hkv: int, d: int, dtype,
-                 device: torch.device) -> None:
-    _check(k_cache, "k_cache", (dtype,), device)
-    _check(v_cache, "v_cache", (dtype,), device)
-    if k_cache.shape != v_cache.shape or k_cache.dim() != 4 or k_cache.shape[1:] != (hkv, PAGE_SLOTS, d):
+                 device: torch.device, index: int) -> tuple[int, int, int]:
+    """(sequences, pages a sequence, pages) of caches [pages, Hkv, 16, D] and their page table."""
+    _need(k_cache, "k_cache", dtype, device, index)
+    _need(v_cache, "v_cache", dtype, device, index)
+    shape = k_cache.shape
+    if v_cache.shape != shape or len(shape) != 4 or shape[1:] != (hkv, PAGE_SLOTS, d):
         raise ValueError(f"caches must be [pages, {hkv}, {PAGE_SLOTS}, {d}], got {tuple(k_cache.shape)} and "
                          f"{tuple(v_cache.shape)}")
-    _check(page_table, "page_table", (torch.int32,), device)
-    if page_table.dim() != 2:
+    _need(page_table, "page_table", torch.int32, device, index)
+    table = page_table.shape
+    if len(table) != 2:
         raise ValueError(f"page_table must be [sequences, pages], got {tuple(page_table.shape)}")
+    return table[0], table[1], shape[0]
 
 
-def _check_ints(t: torch.Tensor, name: str, n: int, device: torch.device) -> None:
-    _check(t, name, (torch.int32,), device)
+def _check_ints(t: torch.Tensor, name: str, n: int, device: torch.device, index: int) -> None:
+    _need(t, name, torch.int32, device, index)
     if t.dim() != 1 or t.numel() < n:
         raise ValueError(f"{name} must hold {n} elements, got {tuple(t.shape)}")
 
 
-def _check_slots(t: torch.Tensor, name: str, dtype, shape: tuple, device: torch.device) -> None:
-    """A [..., sequences, Hkv, cap] tensor; shape gives all but cap."""
-    _check(t, name, (dtype,), device)
-    if t.dim() != len(shape) + 1 or t.shape[:-1] != shape:
-        raise ValueError(f"{name} must be [{', '.join(map(str, shape))}, slots], got {tuple(t.shape)}")
+def _check_slots(t: torch.Tensor, name: str, dtype, lead: tuple, device: torch.device, index: int) -> int:
+    """cap of a [..., sequences, Hkv, cap] tensor; lead: all but cap."""
+    _need(t, name, dtype, device, index)
+    shape = t.shape
+    if len(shape) != len(lead) + 1 or shape[:-1] != lead:
+        raise ValueError(f"{name} must be [{', '.join(map(str, lead))}, slots], got {tuple(t.shape)}")
+    return shape[-1]
 
 
 def rope_kv(qkv: torch.Tensor, inv_freq: torch.Tensor, row_pos: torch.Tensor, row_slot: torch.Tensor,
@@ -906,8 +926,10 @@ def rope_kv(qkv: torch.Tensor, inv_freq: torch.Tensor, row_pos: torch.Tensor, ro
     [M, Hq, D]), k turned and v written to slot row_slot of table row row_seq of the caches [pages, Hkv, 16, D], and, with
     slot_pos (int32 [sequences, Hkv, cap]), the position to that slot of every head. Rows whose slot is outside the table
     (-1) write no cache; no two rows may name one slot. What rope says of inv_freq, layout and factor holds."""
-    _check(qkv, "qkv", _FLOATS)
-    device = qkv.device
+    if not (isinstance(qkv, torch.Tensor) and qkv.is_cuda and qkv.dtype in _TYPES and qkv.is_contiguous()):
+        _check(qkv, "qkv", _FLOATS)
+    device, dtype = qkv.device, qkv.dtype
+    index = device.index
     if hq < 1 or hkv < 1 or hq % hkv or d < 1:
         raise ValueError(f"{hq} query heads, {hkv} kv heads of {d} values")
     if qkv.dim() != 2 or qkv.shape[1] != (hq + 2 * hkv) * d:
@@ -915,25 +937,26 @@ def rope_kv(qkv: torch.Tensor, inv_freq: torch.Tensor, row_pos: torch.Tensor, ro
     m = qkv.shape[0] if rows is None else rows
     if not 0 <= m <= qkv.shape[0]:
         raise ValueError(f"{m} rows of {qkv.shape[0]}")
-    rotary, lay = _rope_table(inv_freq, layout, d, device)
-    for t, name in ((row_pos, "row_pos"), (row_slot, "row_slot"), (row_seq, "row_seq")):
-        _check_ints(t, name, m, device)
-    _check_cache(k_cache, v_cache, page_table, hkv, d, qkv.dtype, device)
-    cap = 0
-    if slot_pos is not None:
-        _check_slots(slot_pos, "slot_pos", torch.int32, (page_table.shape[0], hkv), device)
-        cap = slot_pos.shape[-1]
+    rotary, lay, freq64 = _rope_table(inv_freq, layout, d, device, index)
+    _check_ints(row_pos, "row_pos", m, device, index)
+    _check_ints(row_slot, "row_slot", m, device, index)
+    _check_ints(row_seq, "row_seq", m, device, index)
+    seqs, max_pages, pages = _check_cache(k_cache, v_cache, page_table, hkv, d, dtype, device, index)
+    cap = 0 if slot_pos is None else _check_slots(slot_pos, "slot_pos", torch.int32, (seqs, hkv), device, index)
     if q_out is None:
-        q_out = torch.empty((m, hq, d), dtype=qkv.dtype, device=device)
+        q_out = qkv.new_empty((m, hq, d))
     else:
-        _check(q_out, "q_out", (qkv.dtype,), device)
+        _need(q_out, "q_out", dtype, device, index)
         if q_out.numel() < m * hq * d:
             raise ValueError(f"q_out needs {m * hq * d} elements")
+        _disjoint_or_same(q_out, "q_out", qkv, "qkv")
+        if q_out.data_ptr() == qkv.data_ptr():
+            raise ValueError("q_out must not be qkv")
     if m:
-        _launch(device, "im_rope_kv", qkv.data_ptr(), inv_freq.data_ptr(), int(inv_freq.dtype == torch.float64), rotary,
-                float(factor), lay, row_pos.data_ptr(), row_slot.data_ptr(), row_seq.data_ptr(), page_table.data_ptr(),
-                page_table.shape[0], page_table.shape[1], k_cache.shape[0], m, hq, hkv, d, _TYPES[qkv.dtype],
-                q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _ptr_or_none(slot_pos), cap, _stream(device))
+        _launch(index, "im_rope_kv", qkv.data_ptr(), inv_freq.data_ptr(), freq64, rotary, float(factor), lay,
+                row_pos.data_ptr(), row_slot.data_ptr(), row_seq.data_ptr(), page_table.data_ptr(), seqs, max_pages, pages,
+                m, hq, hkv, d, _TYPES[dtype],
+                q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _ptr_or_none(slot_pos), cap)
     return q_out
 
 
@@ -952,37 +975,40 @@ def attention_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     place or in weights_out, weights + the softmax weights that the sequence's rows and the kv head's query heads put on
     the slot, for the slots up to the last row's; from the first row's slot on it starts from zero. The other arguments
     are `attention`'s, keys_per_split 0 meaning that the call's sizes choose it."""
-    _check(q, "q", (torch.bfloat16, torch.float16))
+    dtype = torch.float16 if isinstance(q, torch.Tensor) and q.dtype is torch.float16 else torch.bfloat16
+    if not (isinstance(q, torch.Tensor) and q.is_cuda and q.dtype is dtype and q.is_contiguous()):
+        _check(q, "q", (torch.bfloat16, torch.float16))
     device = q.device
-    if q.dim() != 3 or k_cache.dim() != 4:
-        raise ValueError(f"q must be [M, Hq, D] and the caches [pages, Hkv, 16, D], got {tuple(q.shape)}, "
-                         f"{tuple(k_cache.shape)}")
-    hq, d, hkv = q.shape[1], q.shape[2], k_cache.shape[1]
-    m = q.shape[0] if rows is None else rows
-    if not 0 <= m <= q.shape[0]:
-        raise ValueError(f"{m} rows of {q.shape[0]}")
+    index = device.index
+    if q.dim() != 3 or not isinstance(k_cache, torch.Tensor) or k_cache.dim() != 4:
+        raise ValueError(f"q must be [M, Hq, D] and the caches [pages, Hkv, 16, D], got q {tuple(q.shape)}")
+    held, hq, d = q.shape
+    hkv = k_cache.shape[1]
+    m = held if rows is None else rows
+    if not 0 <= m <= held:
+        raise ValueError(f"{m} rows of {held}")
     if hkv < 1 or hq < 1 or hq % hkv:
         raise ValueError(f"{hq} query heads, {hkv} kv heads")
-    _check_cache(k_cache, v_cache, page_table, hkv, d, q.dtype, device)
-    _check_ints(seq_rows, "seq_rows", 1, device)
+    seqs, max_pages, pages = _check_cache(k_cache, v_cache, page_table, hkv, d, dtype, device, index)
+    _check_ints(seq_rows, "seq_rows", 1, device, index)
     b = seq_rows.numel() - 1
-    _check_ints(row_slot, "row_slot", m, device)
+    _check_ints(row_slot, "row_slot", m, device, index)
     if seq_slot is not None:
-        _check_ints(seq_slot, "seq_slot", b, device)
-    elif b > page_table.shape[0]:
-        raise ValueError(f"{b} sequences, the page table has {page_table.shape[0]}")
-    _check_slots(weights, "weights", torch.float32, (page_table.shape[0], hkv), device)
+        _check_ints(seq_slot, "seq_slot", b, device, index)
+    elif b > seqs:
+        raise ValueError(f"{b} sequences, the page table has {seqs}")
+    cap = _check_slots(weights, "weights", torch.float32, (seqs, hkv), device, index)
     if weights_out is None:
         weights_out = weights
     else:
-        _check(weights_out, "weights_out", (torch.float32,), device)
+        _need(weights_out, "weights_out", torch.float32, device, index)
         if weights_out.shape != weights.shape:
             raise ValueError(f"weights_out must be {tuple(weights.shape)}, got {tuple(weights_out.shape)}")
         _disjoint_or_same(weights_out, "weights_out", weights, "weights")
     if out is None:
-        out = torch.empty((m, hq, d), dtype=q.dtype, device=device)
+        out = q.new_empty((m, hq, d))
     else:
-        _check(out, "out", (q.dtype,), device)
+        _need(out, "out", dtype, device, index)
         if out.numel() < m * hq * d:
             raise ValueError(f"out needs {m * hq * d} elements")
     if not (0 <= max_rows_per_seq and 0 <= max_kv_len and 0 <= window and 0 <= keys_per_split):
@@ -992,11 +1018,11 @@ def attention_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     max_rows = min(max_rows_per_seq, m)
     need = _attention_weights_workspace(b, max_rows, hq, hkv, d, max(1, max_kv_len), keys_per_split, window)
     ws = torch.empty(need, dtype=torch.uint8, device=device)
-    _launch(device, "im_attention_weights", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _TYPES[q.dtype],
-            page_table.data_ptr(), page_table.shape[0], page_table.shape[1], k_cache.shape[0], seq_rows.data_ptr(),
+    _launch(index, "im_attention_weights", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _TYPES[dtype],
+            page_table.data_ptr(), seqs, max_pages, pages, seq_rows.data_ptr(),
             _ptr_or_none(seq_slot), row_slot.data_ptr(), m, b, max_rows, hq, hkv, d, max_kv_len, keys_per_split, window,
-            float(scale), weights.data_ptr(), weights_out.data_ptr(), weights.shape[-1], out.data_ptr(), ws.data_ptr(),
-            need, _stream(device))
+            float(scale), weights.data_ptr(), weights_out.data_ptr(), cap, out.data_ptr(), ws.data_ptr(),
+            need)
     return out
 
 
@@ -1019,55 +1045,50 @@ def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.
     if not isinstance(k_cache, torch.Tensor) or k_cache.dim() not in (4, 5):
         raise ValueError("caches must be [pages, Hkv, 16, D] or [layers, pages, Hkv, 16, D]")
     device, dtype = k_cache.device, k_cache.dtype
-    _check(k_cache, "k_cache", (dtype,))
-    _check(v_cache, "v_cache", (dtype,), device)
+    index = device.index
+    if not (k_cache.is_cuda and k_cache.is_contiguous()):
+        _check(k_cache, "k_cache", (dtype,))
+    _need(v_cache, "v_cache", dtype, device, index)
     if v_cache.shape != k_cache.shape or k_cache.shape[-2] != PAGE_SLOTS:
         raise ValueError(f"caches must be of one shape with {PAGE_SLOTS} slots a page, got {tuple(k_cache.shape)} and "
                          f"{tuple(v_cache.shape)}")
-    layers = k_cache.shape[0] if k_cache.dim() == 5 else 1
-    pages, hkv, _, d = k_cache.shape[-4:]
-    _check(page_table, "page_table", (torch.int32,), device)
+    shape = k_cache.shape
+    layers = shape[0] if len(shape) == 5 else 1
+    pages, hkv, _, d = shape[-4:]
+    _need(page_table, "page_table", torch.int32, device, index)
     if page_table.dim() != 2:
         raise ValueError(f"page_table must be [sequences, pages], got {tuple(page_table.shape)}")
-    s = page_table.shape[0]
-    for t, name in ((lengths, "lengths"), (seen, "seen")):
-        _check(t, name, (torch.int32,), device)
-        if t.shape != (s,):
-            raise ValueError(f"{name} must be [{s}], got {tuple(t.shape)}")
-    lead = (layers, s, hkv) if k_cache.dim() == 5 else (s, hkv)
-    _check_slots(weights, "weights", torch.float32, lead, device)
-    _check_slots(slot_pos, "slot_pos", torch.int32, lead, device)
-    if slot_pos.shape != weights.shape:
+    s, max_pages = page_table.shape
+    for t, name in ((lengths, "lengths"), (seen, "seen"), (lengths_out, "lengths_out")):
+        if t is not None or name != "lengths_out":
+            _need(t, name, torch.int32, device, index)
+            if t.shape != (s,):
+                raise ValueError(f"{name} must be [{s}], got {tuple(t.shape)}")
+    lead = (layers, s, hkv) if len(shape) == 5 else (s, hkv)
+    cap = _check_slots(weights, "weights", torch.float32, lead, device, index)
+    if _check_slots(slot_pos, "slot_pos", torch.int32, lead, device, index) != cap:
         raise ValueError(f"slot_pos is {tuple(slot_pos.shape)}, weights {tuple(weights.shape)}")
-    outs = []
     for t, name, like, like_name in ((weights_out, "weights_out", weights, "weights"),
                                      (pos_out, "pos_out", slot_pos, "slot_pos")):
-        if t is None:
-            t = like
-        else:
-            _check(t, name, (like.dtype,), device)
+        if t is not None:
+            _need(t, name, like.dtype, device, index)
             if t.shape != like.shape:
                 raise ValueError(f"{name} must be {tuple(like.shape)}, got {tuple(t.shape)}")
             _disjoint_or_same(t, name, like, like_name)
-        outs.append(t)
     if lengths_out is None:
         lengths_out = torch.empty((s,), dtype=torch.int32, device=device)
-    else:
-        _check(lengths_out, "lengths_out", (torch.int32,), device)
-        if lengths_out.shape != (s,):
-            raise ValueError(f"lengths_out must be [{s}], got {tuple(lengths_out.shape)}")
     if budget < 0 or recent < 0 or sinks < 0 or recent + sinks > budget:
         raise ValueError(f"{recent} recent and {sinks} first slots of a budget of {budget}")
-    cap = weights.shape[-1]
     if not (layers and s and hkv and cap and d):
         return lengths_out.zero_()
     need = _evict_workspace(layers, s, hkv, cap, budget)
     ws = torch.empty(max(need, 16), dtype=torch.uint8, device=device)
     size = k_cache.element_size()
-    _launch(device, "im_cache_evict", k_cache.data_ptr(), v_cache.data_ptr(), layers, pages * hkv * PAGE_SLOTS * d * size,
-            pages, page_table.data_ptr(), page_table.shape[1], lengths.data_ptr(), seen.data_ptr(), weights.data_ptr(),
-            outs[0].data_ptr(), slot_pos.data_ptr(), outs[1].data_ptr(), lengths_out.data_ptr(), s, hkv, cap, d * size,
-            budget, recent, sinks, ws.data_ptr(), need, _stream(device))
+    _launch(index, "im_cache_evict", k_cache.data_ptr(), v_cache.data_ptr(), layers, pages * hkv * PAGE_SLOTS * d * size,
+            pages, page_table.data_ptr(), max_pages, lengths.data_ptr(), seen.data_ptr(), weights.data_ptr(),
+            (weights if weights_out is None else weights_out).data_ptr(), slot_pos.data_ptr(),
+            (slot_pos if pos_out is None else pos_out).data_ptr(), lengths_out.data_ptr(), s, hkv, cap, d * size,
+            budget, recent, sinks, ws.data_ptr(), need)
     return lengths_out
 
 
@@ -1110,21 +1131,22 @@ def verify_sampled(target_probs: torch.Tensor, draft_probs: torch.Tensor | None,
         if draft_probs.dtype != target_probs.dtype:
             raise TypeError(f"draft_probs is {draft_probs.dtype}, target_probs {target_probs.dtype}")
         q_ld = _check_probs(draft_probs, "draft_probs", k, device) if k else v
-    _check(drafts, "drafts", (torch.int32,), device)
-    _check(uniforms, "uniforms", (torch.float32,), device)
+    index = device.index
+    _need(drafts, "drafts", torch.int32, device, index)
+    _need(uniforms, "uniforms", torch.float32, device, index)
     if uniforms.shape != (b, k + 1):
         raise ValueError(f"uniforms must be [{b}, {k + 1}], got {tuple(uniforms.shape)}")
     for t, name, shape in ((n_drafts, "n_drafts", (b,)), (tokens, "tokens", (b, k + 1)), (count, "count", (b,))):
         if t is not None:
-            _check(t, name, (torch.int32,), device)
+            _need(t, name, torch.int32, device, index)
             if t.shape != shape:
                 raise ValueError(f"{name} must be {list(shape)}, got {tuple(t.shape)}")
-    tokens = torch.empty((b, k + 1), dtype=torch.int32, device=device) if tokens is None else tokens
-    count = torch.empty((b,), dtype=torch.int32, device=device) if count is None else count
+    tokens = drafts.new_empty((b, k + 1)) if tokens is None else tokens
+    count = drafts.new_empty((b,)) if count is None else count
     if b:
-        _launch(device, "im_verify_sampled", target_probs.data_ptr(), p_ld, _ptr_or_none(draft_probs), q_ld,
+        _launch(index, "im_verify_sampled", target_probs.data_ptr(), p_ld, _ptr_or_none(draft_probs), q_ld,
                 _TYPES[target_probs.dtype], drafts.data_ptr(), k, _ptr_or_none(n_drafts), uniforms.data_ptr(), k + 1, b, k,
-                v, tokens.data_ptr(), count.data_ptr(), _stream(device))
+                v, tokens.data_ptr(), count.data_ptr())
     return tokens, count
 
 
