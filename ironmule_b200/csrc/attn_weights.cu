@@ -697,14 +697,10 @@ static AwPlan aw_plan(int64_t B, int64_t rows, int64_t Hq, int64_t Hkv, int64_t 
 
 template <typename T, int DP, int NT>
 int launch_split(const AwArgs& a, dim3 grid, cudaStream_t st) {
-  auto* kernel = aw_split_kernel<T, DP, NT>;
   constexpr int smem = AwShape<DP, NT>::SMEM;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) {
-    set_error("aw_split_kernel: %s", cudaGetErrorString(e));
-    return IM_CUDA_ERROR;
-  }
-  return launch("aw_split_kernel", kernel, grid, dim3(AwShape<DP, NT>::WARPS * 32), smem, st, a);
+  const int rc = configure<aw_split_kernel<T, DP, NT>>("aw_split_kernel", smem, false);
+  if (rc != IM_OK) return rc;
+  return launch("aw_split_kernel", aw_split_kernel<T, DP, NT>, grid, dim3(AwShape<DP, NT>::WARPS * 32), smem, st, a);
 }
 
 template <typename T, int NT>

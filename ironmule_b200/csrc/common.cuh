@@ -4,6 +4,8 @@
 #include <stdint.h>
 #include <stdio.h>
 
+#include <atomic>
+
 #include "../../include/imspec.h"
 
 namespace im {
@@ -76,7 +78,27 @@ inline int launch(const char* what, void (*kernel)(KArgs...), dim3 grid, dim3 bl
   return IM_OK;
 }
 
-// The same as thread-block clusters of `cluster` blocks along x (above 8, the kernel must allow a size that is not portable).
+// A kernel's attributes, set once on each device: dynamic shared memory beyond 48 KB, clusters of more than 8 blocks.
+template <auto Kernel>
+inline int configure(const char* what, int smem, bool wide_cluster) {
+  static std::atomic<unsigned long long> done{0};  // a bit a device, of the first 64
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
+  if (e == cudaSuccess && (bit == 0 || !(done.load(std::memory_order_acquire) & bit))) {
+    if (smem > 48 * 1024) e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess && wide_cluster)
+      e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  }
+  if (e != cudaSuccess) {
+    set_error("%s: %s", what, cudaGetErrorString(e));
+    return IM_CUDA_ERROR;
+  }
+  return IM_OK;
+}
+
+// launch() as thread-block clusters of `cluster` blocks along x (above 8, the kernel must allow a size that is not portable).
 template <typename... KArgs, typename... Args>
 inline int launch_cluster(const char* what, void (*kernel)(KArgs...), dim3 grid, dim3 block, int cluster, size_t smem,
                           cudaStream_t st, Args... args) {

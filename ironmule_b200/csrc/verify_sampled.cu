@@ -224,6 +224,14 @@ __global__ void __launch_bounds__(VS_THREADS, 2) verify_sampled_kernel(VerifyArg
   if (lane == 0) a.out_count[b] = kept + 1;
 }
 
+template <typename T, bool WIDE>
+int launch_verify_ranks(const VerifyArgs& a, int64_t B, int ranks, cudaStream_t st) {
+  const int rc = configure<verify_sampled_kernel<T, WIDE>>("verify_sampled_kernel", 0, true);
+  if (rc != IM_OK) return rc;
+  return launch_cluster("verify_sampled_kernel", verify_sampled_kernel<T, WIDE>, dim3((unsigned)(B * ranks)),
+                        dim3(VS_THREADS), ranks, VS_LEFT * sizeof(double), st, a);
+}
+
 template <typename T>
 int launch_verify_sampled(const VerifyArgs& a, int64_t B, cudaStream_t st) {
   // blocks a sequence: enough to fill the device's two blocks an SM, of at least 2048 tokens
@@ -232,16 +240,7 @@ int launch_verify_sampled(const VerifyArgs& a, int64_t B, cudaStream_t st) {
   // 16-byte loads where every row starts on 16 bytes and is whole
   const int n = 16 / sizeof(T);
   const bool wide = aligned(a.p, 16) && aligned(a.q, 16) && a.p_ld % n == 0 && a.q_ld % n == 0 && a.V % n == 0;
-  auto* kernel = wide ? verify_sampled_kernel<T, true> : verify_sampled_kernel<T, false>;
-  if (ranks > 8) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) {
-      set_error("verify_sampled_kernel: %s", cudaGetErrorString(e));
-      return IM_CUDA_ERROR;
-    }
-  }
-  return launch_cluster("verify_sampled_kernel", kernel, dim3((unsigned)(B * ranks)), dim3(VS_THREADS), ranks,
-                        VS_LEFT * sizeof(double), st, a);
+  return wide ? launch_verify_ranks<T, true>(a, B, ranks, st) : launch_verify_ranks<T, false>(a, B, ranks, st);
 }
 
 }  // namespace im

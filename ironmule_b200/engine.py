@@ -184,6 +184,7 @@ class RowMeta:
     slot: torch.Tensor | None = None      # KV slot per row when it differs from the position (draft trees)
     tree_mask: torch.Tensor | None = None  # int64 per row: ancestor bits over the tree slots
     tree_base: torch.Tensor | None = None  # int32 per sequence group: the first tree slot
+    weights: torch.Tensor | None = None    # float32 [layers, slots, Hkv, max_ctx]: attention weights added up per KV slot
 
 
 class QuantModel:
@@ -377,9 +378,13 @@ class QuantModel:
         kernels.embed(meta.tokens, self.embed.w, self.embed.s, self.embed.b, mult=mult, out=h, rows=m,
                       stride=meta.token_stride, out_sq=self.sq_embed)
         sq, parts = self.sq_embed, 1
-        row_page = None  # page-table row of every row, for the two-kernel attention of wide prefill chunks
-        if meta.max_rows_per_seq > MAX_SEQ_ROWS:
-            if self.q_wide is None or m > self.q_wide.shape[0]:
+        row_page = None  # page-table row of every row, for the two-kernel attention of wide prefill chunks or with weights
+        weighed = meta.weights is not None
+        if weighed and meta.tree_mask is not None:
+            raise ValueError("slot weights are not added up for draft trees")
+        two_kernels = weighed or meta.max_rows_per_seq > MAX_SEQ_ROWS
+        if two_kernels:
+            if meta.max_rows_per_seq > MAX_SEQ_ROWS and (self.q_wide is None or m > self.q_wide.shape[0]):
                 raise ValueError(f"{meta.max_rows_per_seq} rows of one sequence exceed this model's rows")
             row_page = meta.seq if meta.seq_slot is None else meta.seq_slot[meta.seq.long()]
         def tr(key: str, t: torch.Tensor) -> None:
@@ -396,18 +401,25 @@ class QuantModel:
             row_slot = meta.pos if meta.slot is None else meta.slot
             # few rows: the attention leaves its split partials for the o-projection's prologue to merge (same
             # bits; the per-op trace keeps the attention output, so it takes the unmerged route)
-            merge_in_o = m <= self.o_merge_rows and trace is None
+            merge_in_o = m <= self.o_merge_rows and trace is None and not weighed
             inv_freq = self.inv_freq if glob else self.inv_freq_local
             window = 0 if glob else c.sliding_window
-            if meta.max_rows_per_seq > MAX_SEQ_ROWS:  # prefill chunks beyond the fused attention's rows
+            if two_kernels:  # prefill chunks beyond the fused attention's rows, and forwards that add up slot weights
                 q = kernels.qk_norm_rope_kv(self.qkv, layer.q_norm, layer.k_norm, inv_freq, meta.pos, row_slot, row_page,
                                             self.page_table, c.heads, c.kv_heads, c.head_dim, c.eps, self.k_cache[li],
                                             self.v_cache[li], gemma=gemma, q_out=self.q_wide, rows=m)
-                kernels.attention(q.view(-1, c.heads, c.head_dim), self.k_cache[li], self.v_cache[li], self.page_table,
-                                  meta.seq_rows, row_slot, max_rows_per_seq=meta.max_rows_per_seq,
-                                  max_kv_len=max_kv_len, scale=c.scale, keys_per_split=self.keys_per_split,
-                                  window=window, tree_mask=meta.tree_mask, tree_base=meta.tree_base, out=self.attn,
-                                  rows=m, ws=self.ws_attn, seq_slot=meta.seq_slot)
+                if weighed:
+                    kernels.attention_weights(q.view(-1, c.heads, c.head_dim), self.k_cache[li], self.v_cache[li],
+                                              self.page_table, meta.seq_rows, row_slot, meta.weights[li],
+                                              max_rows_per_seq=meta.max_rows_per_seq, max_kv_len=max_kv_len,
+                                              scale=c.scale, keys_per_split=self.keys_per_split, window=window,
+                                              out=self.attn, rows=m, seq_slot=meta.seq_slot)
+                else:
+                    kernels.attention(q.view(-1, c.heads, c.head_dim), self.k_cache[li], self.v_cache[li],
+                                      self.page_table, meta.seq_rows, row_slot, max_rows_per_seq=meta.max_rows_per_seq,
+                                      max_kv_len=max_kv_len, scale=c.scale, keys_per_split=self.keys_per_split,
+                                      window=window, tree_mask=meta.tree_mask, tree_base=meta.tree_base, out=self.attn,
+                                      rows=m, ws=self.ws_attn, seq_slot=meta.seq_slot)
             else:
                 kernels.attention_qkv(self.qkv, layer.q_norm, layer.k_norm, inv_freq, meta.pos, self.k_cache[li],
                                       self.v_cache[li], self.page_table, meta.seq_rows, row_slot,
@@ -1099,6 +1111,84 @@ def greedy_decode(model: QuantModel, prompt: torch.Tensor, max_new: int, seq: in
         model.check_waits()
         pos += 1
     return out
+
+
+class BoundedDecoder:
+    """Greedy decoding over a cache that does not grow: every kv head of every layer keeps at most `budget` slots when the
+    cache is cut, which happens whenever the next tokens would pass model.max_ctx slots. Kept are the first `sinks` tokens, the
+    last `recent`, and the tokens with the most attention so far (kernels.attention_weights adds it up, prompt included;
+    kernels.cache_evict cuts). A text may so be longer than the cache; a token's position is not its slot. Until the first
+    cut this is plain decoding; behind it the answers are the cut cache's. Not for models with a sliding window, whose
+    layers go by slots, nor over pages that sequences share."""
+
+    def __init__(self, model: QuantModel, budget: int, *, recent: int | None = None, sinks: int = 4):
+        recent = budget // 4 if recent is None else recent
+        if model.cfg.sliding_window:
+            raise ValueError(f"{model.cfg.name}: a sliding window goes by slots, which a cut cache reorders")
+        if not 0 < budget < model.max_ctx:
+            raise ValueError(f"a budget of {budget} slots of {model.max_ctx}")
+        if recent < 0 or sinks < 0 or recent + sinks > budget:
+            raise ValueError(f"{recent} recent and {sinks} first slots of a budget of {budget}")
+        self.model, self.budget, self.recent, self.sinks = model, budget, recent, sinks
+        c, s, dev = model.lc, model.max_seqs, model.device
+        self.weights = torch.zeros((c.layers, s, c.kv_heads, model.max_ctx), dtype=torch.float32, device=dev)
+        self.slot_pos = torch.full((c.layers, s, c.kv_heads, model.max_ctx), -1, dtype=torch.int32, device=dev)
+        self.lengths = torch.zeros((s,), dtype=torch.int32, device=dev)  # slots held and tokens seen, per sequence slot
+        self.seen = torch.zeros((s,), dtype=torch.int32, device=dev)
+        self._held, self._seen = [0] * s, [0] * s                        # the same on the host
+        self.cuts = 0
+
+    def start(self, seq: int = 0) -> None:
+        """Forget the sequence of a slot."""
+        self._set(seq, 0, 0)
+
+    def _set(self, seq: int, held: int, seen: int) -> None:
+        self._held[seq], self._seen[seq] = held, seen
+        self.lengths[seq], self.seen[seq] = held, seen
+
+    def cut(self) -> None:
+        """Cut every sequence slot's cache to the budget, in one call for all layers."""
+        m = self.model
+        kernels.cache_evict(m.k_cache, m.v_cache, m.page_table, self.lengths, self.seen, self.weights, self.slot_pos,
+                            budget=self.budget, recent=self.recent, sinks=self.sinks, lengths_out=self.lengths)
+        self._held = [min(n, self.budget) for n in self._held]
+        self.cuts += 1
+
+    def feed(self, tokens: torch.Tensor, seq: int = 0, logits: bool = False) -> torch.Tensor | None:
+        """Run the next tokens (int32 on the device) of sequence slot `seq`; with `logits`, the last one's [1, V]."""
+        m = self.model
+        step = min(m.max_rows, PREFILL_SEQ_ROWS, MAX_QGEMM_ROWS, m.max_ctx - self.budget)
+        last = tokens.numel() - 1 if logits else tokens.numel()  # a token whose logits are wanted goes by itself
+        ends = [*range(step, last, step), last] if last else []
+        out, at = None, 0
+        for end in [*ends, tokens.numel()] if logits else ends:
+            part = tokens[at:end].to(torch.int32).contiguous()
+            n = end - at
+            if self._held[seq] + n > m.max_ctx:
+                self.cut()
+            held, seen = self._held[seq], self._seen[seq]
+            meta = m._meta(part, list(range(seen, seen + n)), seq)
+            meta.slot = torch.arange(held, held + n, dtype=torch.int32, device=m.device)
+            meta.weights = self.weights
+            self.slot_pos[:, seq, :, held:held + n] = meta.pos
+            kv = min(m.max_ctx, -(-(held + n) // 64) * 64)
+            out = m.forward(meta, max_kv_len=kv, logit_rows=1 if logits and end == tokens.numel() else 0)
+            self._set(seq, held + n, seen + n)
+            at = end
+        return out
+
+    def generate(self, prompt: torch.Tensor, max_new: int, seq: int = 0) -> list[int]:
+        """The greedy answer to a prompt, in a fresh sequence."""
+        m = self.model
+        self.start(seq)
+        out: list[int] = []
+        last = prompt.to(torch.int32)
+        for _ in range(max_new):
+            idx, _ = kernels.argmax_rows(self.feed(last, seq, logits=True), ws=m.ws_argmax)
+            last = idx.clone()
+            out.append(int(idx.item()))
+            m.check_waits()
+        return out
 
 
 # ---- the draft-model protocol of the reference's host speculation, on the device ------------------------------

@@ -1092,15 +1092,18 @@ def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.
     return lengths_out
 
 
-def _check_probs(t: torch.Tensor, name: str, rows: int, device: torch.device | None) -> int:
+def _check_probs(t: torch.Tensor, name: str, rows: int, index: int | None) -> int:
     """The row stride of probabilities [B, rows, V] whose rows are evenly spaced."""
-    if not isinstance(t, torch.Tensor) or t.device.type != "cuda" or t.dtype not in _TYPES:
+    if not t.is_cuda or t.dtype not in _TYPES:
         raise TypeError(f"{name} must be a bf16, float16 or float32 CUDA tensor")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    if index is not None and t.get_device() != index:
+        raise ValueError(f"{name} is on {t.device}, expected cuda:{index}")
     b, _, v = t.shape
-    ld = t.stride(1) if rows > 1 else t.stride(0) if b > 1 else v
-    if (v > 1 and t.stride(2) != 1) or ld < v or (b > 1 and t.stride(0) != rows * ld):
+    if t.is_contiguous():
+        return v
+    by_b, by_row, by_v = t.stride()
+    ld = by_row if rows > 1 else by_b if b > 1 else v
+    if (v > 1 and by_v != 1) or ld < v or (b > 1 and by_b != rows * ld):
         raise ValueError(f"{name} must have evenly spaced rows of contiguous values, its strides are {t.stride()}")
     return ld
 
@@ -1124,14 +1127,14 @@ def verify_sampled(target_probs: torch.Tensor, draft_probs: torch.Tensor | None,
         raise ValueError("target_probs has an empty vocabulary")
     p_ld = _check_probs(target_probs, "target_probs", k + 1, None)
     device = target_probs.device
+    index = device.index
     q_ld = 0
     if draft_probs is not None:
         if not isinstance(draft_probs, torch.Tensor) or draft_probs.shape != (b, k, v):
             raise ValueError(f"draft_probs must be [{b}, {k}, {v}]")
         if draft_probs.dtype != target_probs.dtype:
             raise TypeError(f"draft_probs is {draft_probs.dtype}, target_probs {target_probs.dtype}")
-        q_ld = _check_probs(draft_probs, "draft_probs", k, device) if k else v
-    index = device.index
+        q_ld = _check_probs(draft_probs, "draft_probs", k, index) if k else v
     _need(drafts, "drafts", torch.int32, device, index)
     _need(uniforms, "uniforms", torch.float32, device, index)
     if uniforms.shape != (b, k + 1):
