@@ -480,7 +480,7 @@ size_t im_kq_workspace_bytes(int64_t K, int64_t B);
  * f being the sequence's first row's slot: slots that this call is the first to see start from zero. Other weights are
  * left alone. weights_out may be weights. Rows that see no slot (row_slot -1, say) get zeros and add nothing. Splits:
  * multiples of keys_per_split (a multiple of 64; 0: chosen by the sizes of the call); keep it fixed and a row's bits do
- * not depend on the launch. seq_rows is clamped to the M rows of q; rows beyond max_rows_per_seq are not computed. No two
+ * not depend on the launch. The workspace holds 4 bytes a (row, query head, slot). seq_rows is clamped to the M rows of q; rows beyond max_rows_per_seq are not computed. No two
  * sequences may name one table row. Workspace 256-byte aligned, nothing to initialise.
  *
  * im_cache_evict: of the n = lengths[s] slots of every (layer, sequence, kv head), min(n, budget) stay: those whose
@@ -489,7 +489,7 @@ size_t im_kq_workspace_bytes(int64_t K, int64_t B);
  * row_bytes of one head; any type), weight and position. weights_out and pos_out (which may be weights and slot_pos) get
  * the slots before the new end, lengths_out [S] (may be lengths) the new length, the same for every layer and head. weights and
  * slot_pos are [layers][S][Hkv][cap], the caches `layers` times [pages][Hkv][16][row_bytes], layer_bytes apart; n is at
- * most min(cap, 16 max_pages). Sequences must not share the pages of a cache that is cut. sinks + recent <= budget.
+ * most min(cap, 16 max_pages), cap at most 262144. Sequences must not share the pages of a cache that is cut. sinks + recent <= budget.
  * Workspace 16-byte aligned, nothing to initialise.
  *
  * im_verify_sampled: keeps or refuses drafted tokens by the target's probabilities and given random numbers. target

@@ -757,7 +757,8 @@ extern "C" int im_attention_weights(const void* q, const void* k_cache, const vo
   IM_REQUIRE(D >= 16 && D <= 256 && D % 16 == 0, IM_UNSUPPORTED,
              "im_attention_weights: head_dim %lld (multiples of 16 up to 256)", (long long)D);
   if (M == 0 || B == 0 || max_rows_per_seq == 0) return IM_OK;
-  IM_REQUIRE(q && k_cache && v_cache && page_table && seq_rows && row_slot && weights && weights_out && out, IM_INVALID,
+  IM_REQUIRE(q && k_cache && v_cache && page_table && seq_rows && row_slot && out && ((weights && weights_out) || cap == 0),
+             IM_INVALID,
              "im_attention_weights: null pointer");
   IM_REQUIRE(aligned(q, 16) && aligned(k_cache, 16) && aligned(v_cache, 16) && aligned(out, 16), IM_INVALID,
              "im_attention_weights: q, the caches and out must be 16-byte aligned");

@@ -353,7 +353,7 @@ static long long evict_most(int64_t cap, int64_t budget) { return budget < cap -
 using namespace im;
 
 extern "C" size_t im_cache_evict_workspace_bytes(int64_t layers, int64_t S, int64_t Hkv, int64_t cap, int64_t budget) {
-  if (layers < 1 || S < 1 || Hkv < 1 || cap < 1 || budget < 0 || layers * S * Hkv >= (1ll << 31)) return 0;
+  if (layers < 1 || S < 1 || Hkv < 1 || cap < 1 || budget < 0 || layers * S * Hkv >= (1ll << 27)) return 0;
   const long long rows = layers * S * Hkv, most = evict_most(cap, budget);
   return (size_t)(rows * 4 + (most > 0 ? 2 * rows * most * 4 : 0));
 }

@@ -1157,6 +1157,8 @@ class BoundedDecoder:
     def feed(self, tokens: torch.Tensor, seq: int = 0, logits: bool = False) -> torch.Tensor | None:
         """Run the next tokens (int32 on the device) of sequence slot `seq`; with `logits`, the last one's [1, V]."""
         m = self.model
+        if logits and not tokens.numel():
+            raise ValueError("logits of no token")
         step = min(m.max_rows, PREFILL_SEQ_ROWS, MAX_QGEMM_ROWS, m.max_ctx - self.budget)
         last = tokens.numel() - 1 if logits else tokens.numel()  # a token whose logits are wanted goes by itself
         ends = [*range(step, last, step), last] if last else []

@@ -116,7 +116,7 @@ def test_evict_refusals():
                      ({"ws": None}, "workspace"), ({"ws": 8}, "workspace"), ({"size": 16}, "workspace")):
         rc, msg = evict(**kw)
         assert rc == _lib.IM_INVALID and word in msg, (kw, msg)
-    assert evict(cap=1 << 30)[0] == _lib.IM_UNSUPPORTED and evict(layers=1 << 30)[0] == _lib.IM_UNSUPPORTED
+    assert evict(cap=262145)[0] == _lib.IM_UNSUPPORTED and evict(layers=1 << 30)[0] == _lib.IM_UNSUPPORTED
     rc, msg = evict(recent=2**62, sinks=2**62, budget=2**62 + 2**61)  # a sum past 64 bits
     assert rc == _lib.IM_INVALID and "budget" in msg
 

@@ -769,8 +769,97 @@ def test_calls_on_two_streams_at_once(cuda):
             assert torch.equal(a, b)
 
 
+def test_caches_whose_offsets_pass_32_bits(cuda):
+    """Pages far behind 2^31 values of a cache: the bits of the same pages in a small one."""
+    far, hq, hkv, d = 140000, 8, 8, 128
+    g = gen(cuda, 50)
+    small = [torch.randn((40, hkv, 16, d), generator=g, device=cuda).to(torch.bfloat16) for _ in range(2)]
+    large = [torch.empty((far, hkv, 16, d), dtype=torch.bfloat16, device=cuda) for _ in range(2)]
+    for a, b in zip(small, large):
+        b[far - 40:] = a
+    table = torch.randperm(40, generator=g, device=cuda).to(torch.int32).view(2, 20).contiguous()
+    qkv = torch.randn((2, (hq + 2 * hkv) * d), generator=g, device=cuda).to(torch.bfloat16)
+    freq, _ = kernels.rope_frequencies(d, 10000.0, device=cuda)
+    outs = []
+    for (k, v), pages in ((small, table), (large, table + (far - 40))):
+        n, w = ints([311, 250], cuda), torch.rand((2, hkv, 320), generator=gen(cuda, 51), device=cuda)
+        pos = torch.arange(320, device=cuda, dtype=torch.int32).expand(2, hkv, 320).contiguous()
+        q = kernels.rope_kv(qkv, freq, n, n, ints([0, 1], cuda), pages, hq, hkv, d, k, v, slot_pos=pos)
+        out = kernels.attention_weights(q, k, v, pages, ints([0, 1, 2], cuda), n, w, max_rows_per_seq=1, max_kv_len=320,
+                                        scale=0.1)
+        left = kernels.cache_evict(k, v, pages, n, n, w, pos, budget=100, recent=10)
+        outs.append((q, out, left, w, pos, k[-40:], v[-40:]))
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+
+
+def test_layers_whose_offsets_pass_32_bits(cuda):
+    k = torch.empty((3, 50000, 8, 16, 128), dtype=torch.bfloat16, device=cuda)  # 2.4 * 10^9 values
+    v = torch.empty_like(k)
+    g = gen(cuda, 52)
+    table = ints([[49990, 3, 49999, 17]], cuda)
+    for t in (k, v):
+        t[:, table[0].long()] = torch.randn((3, 4, 8, 16, 128), generator=g, device=cuda).to(torch.bfloat16)
+    w = torch.rand((3, 1, 8, 64), generator=g, device=cuda)
+    pos = torch.arange(64, device=cuda, dtype=torch.int32).expand(3, 1, 8, 64).contiguous()
+    near = [t[:, table[0].long()].clone() for t in (k, v)]
+    args = (ints([[0, 1, 2, 3]], cuda), ints([60], cuda), ints([60], cuda), w.clone(), pos.clone())
+    kernels.cache_evict(*near, *args, budget=20, recent=3)
+    kernels.cache_evict(k, v, table, *args[1:3], w, pos, budget=20, recent=3)
+    assert torch.equal(k[:, table[0].long()], near[0]) and torch.equal(v[:, table[0].long()], near[1])
+    assert torch.equal(w, args[3]) and torch.equal(pos, args[4])
+
+
+FIRST_CALL_CAPTURED = """
+import sys
+import torch
+sys.path.insert(0, sys.argv[1])
+from ironmule_b200 import kernels
+dev = torch.device("cuda:0")
+g = torch.Generator(device=dev).manual_seed(1)
+k = torch.randn((4, 2, 16, 64), generator=g, device=dev).to(torch.bfloat16)
+v = k.flip(0).contiguous()
+n = torch.tensor([40], dtype=torch.int32, device=dev)
+i01 = torch.tensor([0, 1], dtype=torch.int32, device=dev)
+table = torch.arange(4, dtype=torch.int32, device=dev).view(1, 4)
+w = torch.rand((1, 2, 64), generator=g, device=dev)
+pos = torch.arange(64, dtype=torch.int32, device=dev).expand(1, 2, 64).contiguous()
+p = torch.softmax(torch.randn((1, 2, 9999), generator=g, device=dev), -1)
+u = torch.tensor([[0.9, 0.3]], device=dev)
+qkv = torch.randn((1, 8 * 64), generator=g, device=dev).to(torch.bfloat16)
+freq, _ = kernels.rope_frequencies(64, 10000.0, device=dev)
+kept = [t.clone() for t in (k, v, w, pos)]
+def step(k, v, w, pos):
+    q = kernels.rope_kv(qkv, freq, n, n, i01[:1], table, 4, 2, 64, k, v, slot_pos=pos)
+    out = kernels.attention_weights(q, k, v, table, i01, n, w, max_rows_per_seq=1, max_kv_len=64, scale=0.1)
+    left = kernels.cache_evict(k, v, table, n, n, w, pos, budget=20)
+    return out, left, *kernels.verify_sampled(p, p[:, :1].contiguous(), i01[:1].view(1, 1), u)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    outs = step(k, v, w, pos)
+graph.replay()
+for a, b in zip(outs, step(*kept)):
+    assert torch.equal(a, b)
+for a, b in zip((k, v, w, pos), kept):
+    assert torch.equal(a, b)
+print("ok")
+"""
+
+
+def test_the_first_calls_of_a_process_may_be_captured(cuda):
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    root = Path(__file__).resolve().parents[1]
+    run = subprocess.run([sys.executable, "-c", FIRST_CALL_CAPTURED, str(root)], capture_output=True, text=True,
+                         timeout=300, cwd=root)
+    assert run.returncode == 0 and run.stdout.strip().endswith("ok"), run.stdout + run.stderr
+
+
 # ---- refusals ---------------------------------------------------------------------------------------------------
-def refuses(fn, *args, error=ValueError, match="", **kw):
+def refuses(fn, *args, error=ValueError, match=None, **kw):
     with pytest.raises(error, match=match):
         fn(*args, **kw)
 
@@ -800,6 +889,9 @@ def test_refusals_of_the_wrappers(cuda):
     refuses(kernels.attention_weights, q, k, v, table, bounds, slot, weights[:, :1].contiguous(), match="weights", **kw)
     refuses(kernels.attention_weights, q, k, v, table, bounds, slot, weights, weights_out=weights[:1], match="weights_out",
             **kw)
+    none = torch.zeros((2, 2, 0), device=cuda)  # no slot's weight is kept
+    out = kernels.attention_weights(q, k, v, table, bounds, slot, none, **kw)
+    assert torch.equal(out, kernels.attention_weights(q, k, v, table, bounds, slot, weights.clone(), **kw))
     from ironmule_b200 import _lib
 
     refuses(kernels.attention_weights, q, k, v, table, bounds, slot, weights, keys_per_split=65, error=_lib.KernelError,

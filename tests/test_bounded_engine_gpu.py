@@ -80,5 +80,9 @@ def test_refusals(cuda):
     for budget, kw in ((0, {}), (96, {}), (200, {}), (32, {"recent": 30, "sinks": 3}), (32, {"recent": -1})):
         with pytest.raises(ValueError):
             engine.BoundedDecoder(m, budget, **kw)
+    dec = engine.BoundedDecoder(m, 32)
+    assert dec.feed(tokens(cuda, 0)) is None
+    with pytest.raises(ValueError, match="no token"):
+        dec.generate(tokens(cuda, 0), 3)
     with pytest.raises(ValueError, match="sliding window"):
         engine.BoundedDecoder(model(cuda, 96, "tiny-gemma"), 32)
