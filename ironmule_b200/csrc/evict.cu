@@ -88,9 +88,9 @@ __device__ __forceinline__ int2 ev_before(int x, int* scratch) {
 // lane, K's and V's chunks of a move side by side, four loads in flight a lane (with eight, at half the
 // warps an SM, a prompt's cut took 111 us in the place of 106).
 template <int BYTES>
-__device__ __forceinline__ void ev_move(const EvictArgs& a, long long row, int moves, int to, int from) {
-  const int head = (int)(row % a.hkv), seq = (int)(row / a.hkv % a.seqs), lane = threadIdx.x & 31;
-  const int* table = a.page_table + seq * a.max_pages;
+__device__ __forceinline__ void ev_move(const EvictArgs& a, long long row, const int* table, int moves, int to,
+                                        int from) {
+  const int head = (int)(row % a.hkv), lane = threadIdx.x & 31;
   const long long layer = row / a.hkv / a.seqs * a.layer_bytes;
   const int chunks = a.row_bytes / BYTES;  // of K, and of V
   long long dst = 0, src = -1;
@@ -139,11 +139,13 @@ __device__ __forceinline__ void ev_move(const EvictArgs& a, long long row, int m
 template <int THREADS, int ITEMS, int BLOCKS, int BYTES>
 __global__ void __launch_bounds__(THREADS, BLOCKS) evict_select_kernel(EvictArgs a) {
   constexpr int WARPS = THREADS / 32;
-  extern __shared__ int pairs[];     // holes, then movers, where the moves are made here
+  extern __shared__ int pairs[];     // where the moves are made here: holes, movers, the sequence's pages
   __shared__ unsigned hist[2][256];  // by turns: a block may count its next digit while others still read this one
   __shared__ unsigned s_digit[2], s_need[2], s_all[2];
   __shared__ int scratch[2][32];
-  __shared__ int3 shared_counts;  // this block's ties, holes, movers, for the others
+  __shared__ unsigned merged[256];           // a cluster's counts of the digit
+  __shared__ int3 shared_counts;             // this block's ties, holes, movers, for the others
+  __shared__ int3 all_counts[EV_CLUSTER];    // theirs
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = cluster.num_blocks(), rank = cluster.block_rank();
   pdl_wait();
@@ -181,6 +183,9 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) evict_select_kernel(EvictArgs
     for (int i = 0; i < ITEMS; i++) key[i] = ev_key(wv[i], pv[i], a.sinks, recent_from);
   }
   for (int i = t; i < 512; i += THREADS) hist[0][i] = 0;
+  int* pages = pairs + 2 * a.most;
+  if (a.moves_here)
+    for (int i = t; i < (n + 15) / 16; i += THREADS) pages[i] = a.page_table[seq * a.max_pages + i];
   const int mine = first - lane < n ? min(items, (n - first + 31) / 32) : 0;  // slots of this lane (may be 0)
   __syncthreads();
   // the left-th largest key, and how many of those that share its digits stay
@@ -193,17 +198,22 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) evict_select_kernel(EvictArgs
 #pragma unroll
     for (int i = 0; i < ITEMS; i++)
       if (i < mine && (key[i] & mask) == border) atomicAdd(&h[ev_bin(key[i] >> shift & 255)], 1u);
-    if (ranks > 1) cluster.sync();
-    else __syncthreads();
+    if (ranks > 1) {
+      cluster.sync();
+      for (int i = t; i < 256; i += THREADS) {
+        unsigned sum = 0;
+#pragma unroll 4
+        for (int r = 0; r < ranks; r++) sum += *cluster.map_shared_rank(&h[i], r);
+        merged[i] = sum;
+      }
+      h = merged;
+    }
+    __syncthreads();
     if (warp == 0) {  // eight digits a lane, from the highest down
       unsigned c[8], sum = 0;
 #pragma unroll
       for (int i = 0; i < 8; i++) {
-        const int d = 255 - lane * 8 - i;
-        c[i] = 0;
-        if (ranks == 1) c[i] = h[ev_bin(d)];
-        else
-          for (int r = 0; r < ranks; r++) c[i] += *cluster.map_shared_rank(&h[ev_bin(d)], r);
+        c[i] = h[ev_bin(255 - lane * 8 - i)];
         sum += c[i];
       }
       unsigned above = sum;
@@ -238,7 +248,9 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) evict_select_kernel(EvictArgs
     if (ranks > 1) {
       if (t == 0) shared_counts.x = x.y;
       cluster.sync();
-      for (int r = 0; r < rank; r++) ties += cluster.map_shared_rank(&shared_counts, r)->x;
+      if (t < ranks) all_counts[t].x = cluster.map_shared_rank(&shared_counts, t)->x;
+      __syncthreads();
+      for (int r = 0; r < rank; r++) ties += all_counts[r].x;
     }
   }
   unsigned kept = 0;  // of this lane's slots
@@ -264,13 +276,14 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) evict_select_kernel(EvictArgs
   if (ranks > 1) {
     if (t == 0) shared_counts.y = total, shared_counts.z = both.y >> 16;
     cluster.sync();
+    if (t < ranks) all_counts[t] = *cluster.map_shared_rank(&shared_counts, t);
+    cluster.sync();  // nobody leaves while its counts are read
     total = 0;
     for (int r = 0; r < ranks; r++) {
-      const int3 c = *cluster.map_shared_rank(&shared_counts, r);
+      const int3 c = all_counts[r];
       if (r < rank) holes += c.y, movers += c.z;
       total += c.y;
     }
-    cluster.sync();  // nobody leaves while its counts are read
   }
   const bool copies = a.weights_out != a.weights || a.pos_out != a.pos;
   int* hole_list = a.moves_here ? pairs : a.holes + row * a.most;
@@ -294,7 +307,8 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) evict_select_kernel(EvictArgs
   const int share = min(32, (total + WARPS - 1) / WARPS);  // moves of a warp at a time
   for (int i0 = warp * share; i0 < total; i0 += WARPS * share) {
     const int moves = min(share, total - i0);
-    ev_move<BYTES>(a, row, moves, lane < moves ? pairs[i0 + lane] : 0, lane < moves ? pairs[a.most + i0 + lane] : 0);
+    ev_move<BYTES>(a, row, pages, moves, lane < moves ? pairs[i0 + lane] : 0,
+                   lane < moves ? pairs[a.most + i0 + lane] : 0);
   }
 }
 
@@ -312,14 +326,15 @@ __global__ void __launch_bounds__(EV_MOVE_THREADS, 6) evict_move_kernel(EvictArg
   for (int i0 = (blockIdx.y * (EV_MOVE_THREADS / 32) + threadIdx.x / 32) * 32; i0 < count;
        i0 += gridDim.y * EV_MOVE_THREADS) {
     const int moves = min(32, count - i0);
-    ev_move<BYTES>(a, row, moves, lane < moves ? a.holes[row * a.most + i0 + lane] : 0,
+    ev_move<BYTES>(a, row, a.page_table + seq * a.max_pages, moves, lane < moves ? a.holes[row * a.most + i0 + lane] : 0,
                                         lane < moves ? a.movers[row * a.most + i0 + lane] : 0);
   }
 }
 
 template <int THREADS, int ITEMS, int BLOCKS, int BYTES>
 int launch_evict_select(const EvictArgs& a, long long rows, int ranks, cudaStream_t st) {
-  const int smem = a.moves_here && a.most > 0 ? (int)(2 * a.most * 4) : 0;  // at most EV_HERE moves: 8 KB
+  // at most EV_HERE moves and EV_RUN / 16 pages: 12 KB
+  const int smem = a.moves_here ? (int)(2 * a.most + (a.cap + 15) / 16) * 4 : 0;
   const int rc = configure<evict_select_kernel<THREADS, ITEMS, BLOCKS, BYTES>>("evict_select_kernel", 0, true);
   if (rc != IM_OK) return rc;
   return launch_cluster("evict_select_kernel", evict_select_kernel<THREADS, ITEMS, BLOCKS, BYTES>,
