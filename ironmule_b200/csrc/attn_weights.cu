@@ -17,7 +17,7 @@
 // Second kernel (aw_finish_kernel): joins the splits, and adds up exp2(s - max) / sum slot by slot.
 //
 // Weights that meet v are two numbers of the cache's type, high part and rest (16 bits and more of each weight are kept);
-// in float16 they are scaled by 2^14 first, so that weights down to 2^-28 of the largest are not subnormal. Masked
+// in float16 they are scaled by 2^6 to 2^14 first, so that weights down to 2^-20 of the largest are not subnormal. Masked
 // slots never reach a row: behind the last visible slot v is zeroed on its way in; between rows of one call a page is
 // checked for values that are not finite, and if it has any its products are done one by one.
 #include <cuda_bf16.h>
@@ -28,8 +28,8 @@
 namespace im {
 
 constexpr int AW_FIN_THREADS = 256;
-constexpr int AW_FIN_SLOTS = AW_FIN_THREADS * 4;
 constexpr float AW_LOG2E = 1.4426950408889634f;
+constexpr float AW_SLACK = 8.f;
 
 struct AwArgs {
   const char* q;
@@ -48,12 +48,13 @@ struct AwArgs {
   int window;
   float scale;
   char* out;
-  int kps, splits, tiles;  // keys a split, splits of max_kv, tiles of 8 or 16 vectors
+  int kps, splits, tile, tiles;  // keys a split, splits of max_kv, vectors a tile, tiles
   int vecs;                // max_rows * Hq / Hkv
   float* scores;           // [B][Hkv][vecs][kv_pad], in log2 units
   float2* stats;           // [B][Hkv][splits][vecs]: maximum and sum
   float* parts;            // [B][Hkv][splits][vecs][d]
   int seen;                // splits that a sequence's rows see, if they follow one another: the first kernel's blocks
+  int groups;              // threads of the second kernel that share four slots
   int joins, join_warps;   // blocks of the second kernel that join outputs, warps a job of theirs
   int wide_weights;        // weights and weights_out start on 16 bytes
 };
@@ -86,6 +87,13 @@ __device__ __forceinline__ void aw_span(const AwArgs& a, AwSeq& s) {
   const long long most = min((long long)a.max_kv, a.max_pages * 16);
   s.n = s.slot < 0 ? 0 : (int)min((long long)top + 1, most);
   s.lo = a.window > 0 && low != 0x7fffffff ? max(0, low - a.window + 1) : 0;
+}
+
+// 2^x to two ulps; what would be subnormal is 0.
+__device__ __forceinline__ float aw_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 // L2 policy of K and V: read once where one block reads them (they leave room for the scores, which the second kernel
@@ -150,7 +158,7 @@ struct AwType<__nv_bfloat16> {
 };
 template <>
 struct AwType<__half> {
-  static constexpr float SHIFT = 14.f;
+  static constexpr float SHIFT = 6.f;  // with AW_SLACK, weights stay below 2^14
   static __device__ __forceinline__ void mma(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
                  "{%0, %1, %2, %3};"
@@ -178,14 +186,15 @@ struct AwShape {
   static constexpr int STAGES = DP > 64 ? 2 : 3;
   static constexpr int RING = STAGES * 2 * PAGE;
   static constexpr int JOIN = DP + 4;         // floats of a vector where the warps' accumulators are joined
-  static constexpr bool Q_REGS = NT * DP <= 256;
+  static constexpr bool Q_REGS = NT * DP <= 384;
+  static_assert(Q_REGS || NT == 2, "Q in shared memory is read two tiles at a time");
   static constexpr int Q_BYTES = Q_REGS ? 0 : NT * 8 * PITCH;
   static constexpr int SMEM = WARPS * RING + Q_BYTES;
   static_assert(NT * 8 * JOIN * 4 <= RING, "a warp's ring takes its accumulator at the end");
 };
 
 template <typename T, int DP, int NT>
-__global__ void __launch_bounds__(AwShape<DP, NT>::WARPS * 32, DP > 64 ? 3 : 4)
+__global__ void __launch_bounds__(AwShape<DP, NT>::WARPS * 32, NT > 2 ? 2 : DP > 64 ? 3 : 4)
     aw_split_kernel(AwArgs a) {
   using S = AwShape<DP, NT>;
   using Ty = AwType<T>;
@@ -346,7 +355,7 @@ __global__ void __launch_bounds__(AwShape<DP, NT>::WARPS * 32, DP > 64 ? 3 : 4)
         uint32_t ka[4];
         aw_ldsm(ka, kp + k_off + st * 32);
         uint32_t qb[4];
-        if (!S::Q_REGS) aw_ldsm(qb, q_off + st * 32);
+        if (!S::Q_REGS) aw_ldsm(qb, q_off + st * 32);  // of two tiles
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
           float* to = st & 1 ? s_odd[nt] : s[nt];
@@ -369,42 +378,60 @@ __global__ void __launch_bounds__(AwShape<DP, NT>::WARPS * 32, DP > 64 ? 3 : 4)
             if (!ok || j > last[nt][e & 1] || j < from[nt][e & 1] || j >= q.n) s[nt][e] = -INFINITY;
           }
       }
-      bool more = false;
+      // the largest of each vector's scores: every step for all vectors, so that their shuffles overlap
       float top[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; nt++)
 #pragma unroll
+        for (int e = 0; e < 2; e++) top[nt][e] = fmaxf(s[nt][e], s[nt][e + 2]);
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1)
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+          for (int e = 0; e < 2; e++)
+            top[nt][e] = fmaxf(top[nt][e], __shfl_xor_sync(0xffffffffu, top[nt][e], x));
+      // a vector's base follows its maximum when that is AW_SLACK and more above it: weights of up to 2^AW_SLACK lose
+      // nothing, and most pages leave the accumulators alone. Each vector decides for itself, whatever its neighbours
+      bool more = false;
+      float f[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++)
+#pragma unroll
         for (int e = 0; e < 2; e++) {
-          if (live[nt][e]) {
-            float* to = scores + (long long)(nt * 8 + e) * a.kv_pad + page * 16;
-            to[0] = s[nt][e];
-            to[8] = s[nt][e + 2];
+          const float base = top[nt][e] - Ty::SHIFT;
+          f[nt][e] = 1.f;
+          if (base > m[nt][e] + AW_SLACK) {
+            f[nt][e] = aw_exp2(m[nt][e] - base);
+            m[nt][e] = base;
+            more = true;
           }
-          float x = fmaxf(s[nt][e], s[nt][e + 2]);
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-          top[nt][e] = fmaxf(m[nt][e], x - Ty::SHIFT);
-          more = more || top[nt][e] > m[nt][e];
         }
       if (__any_sync(0xffffffffu, more)) {
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
           for (int e = 0; e < 2; e++) {
-            const float f = top[nt][e] > m[nt][e] ? exp2f(m[nt][e] - top[nt][e]) : 1.f;
-            m[nt][e] = top[nt][e];
-            l[nt][e] *= f;
+            l[nt][e] *= f[nt][e];
 #pragma unroll
-            for (int i = 0; i < STEPS; i++) o[i][nt][e] *= f, o[i][nt][e + 2] *= f;
+            for (int i = 0; i < STEPS; i++) o[i][nt][e] *= f[nt][e], o[i][nt][e + 2] *= f[nt][e];
           }
       }
 #pragma unroll
       for (int nt = 0; nt < NT; nt++)
 #pragma unroll
+        for (int e = 0; e < 2; e++)
+          if (live[nt][e]) {
+            float* to = scores + (long long)(nt * 8 + e) * a.kv_pad + page * 16;
+            to[0] = s[nt][e];
+            to[8] = s[nt][e + 2];
+          }
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++)
+#pragma unroll
         for (int e = 0; e < 4; e++) {
           const float base = m[nt][e & 1] == -INFINITY ? 0.f : m[nt][e & 1];
-          s[nt][e] = exp2f(s[nt][e] - base);
+          s[nt][e] = aw_exp2(s[nt][e] - base);
           l[nt][e & 1] += s[nt][e];
         }
       bool by_mma = true;
@@ -475,7 +502,7 @@ __global__ void __launch_bounds__(AwShape<DP, NT>::WARPS * 32, DP > 64 ? 3 : 4)
         float top = s_m[0][row];
 #pragma unroll
         for (int w = 1; w < WARPS; w++) top = fmaxf(top, s_m[w][row]);
-        const float f = m[nt][e] == -INFINITY ? 0.f : exp2f(m[nt][e] - top);
+        const float f = m[nt][e] == -INFINITY ? 0.f : aw_exp2(m[nt][e] - top);
         float* to = (float*)ring + row * S::JOIN + lane / 4;
         if (live[nt][e]) {
 #pragma unroll
@@ -501,7 +528,7 @@ __global__ void __launch_bounds__(AwShape<DP, NT>::WARPS * 32, DP > 64 ? 3 : 4)
       for (int w = 1; w < WARPS; w++) mm = fmaxf(mm, s_m[w][t]);
       float sum = 0.f;
 #pragma unroll
-      for (int w = 0; w < WARPS; w++) sum += s_m[w][t] == -INFINITY ? 0.f : exp2f(s_m[w][t] - mm) * s_l[w][t];
+      for (int w = 0; w < WARPS; w++) sum += s_m[w][t] == -INFINITY ? 0.f : aw_exp2(s_m[w][t] - mm) * s_l[w][t];
       a.stats[at + t] = make_float2(mm, sum);
     }
     __syncthreads();  // the ring is the copies' again
@@ -515,23 +542,23 @@ __device__ __forceinline__ float2 aw_total(const AwArgs& a, long long head, int 
   for (int s = s0 + lane; s < s1; s += 32) {
     const float2 x = a.stats[(head * a.splits + s) * a.vecs + v];
     const float top = fmaxf(m, x.x);
-    if (top != -INFINITY) l = l * exp2f(m - top) + x.y * exp2f(x.x - top);
+    if (top != -INFINITY) l = l * aw_exp2(m - top) + x.y * aw_exp2(x.x - top);
     m = top;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const float m2 = __shfl_xor_sync(0xffffffffu, m, o), l2 = __shfl_xor_sync(0xffffffffu, l, o);
     const float top = fmaxf(m, m2);
-    if (top != -INFINITY) l = l * exp2f(m - top) + l2 * exp2f(m2 - top);
+    if (top != -INFINITY) l = l * aw_exp2(m - top) + l2 * aw_exp2(m2 - top);
     m = top;
   }
   return make_float2(m == -INFINITY ? 0.f : m, l == 0.f ? 0.f : 1.f / l);
 }
 
 // Joins the splits of a (sequence, kv head): the first a.joins blocks of x the output, 128 values of one vector a job of
-// a.join_warps warps, which share its splits; the others add up the slots' weights, AW_FIN_SLOTS at a time, four a thread.
+// a.join_warps warps, which share its splits; the others add up the slots' weights, four a thread or a few threads.
 template <typename T>
-__global__ void __launch_bounds__(AW_FIN_THREADS) aw_finish_kernel(AwArgs a) {
+__global__ void __launch_bounds__(AW_FIN_THREADS, 4) aw_finish_kernel(AwArgs a) {
   extern __shared__ __align__(16) char fin[];
   // Before the wait only what the first kernel does not write: its blocks let this one start after their own wait, so
   // everything before the first kernel is done. weights_out is written behind the wait (weights may be it).
@@ -560,7 +587,7 @@ __global__ void __launch_bounds__(AW_FIN_THREADS) aw_finish_kernel(AwArgs a) {
           const float m = a.stats[at].x;
           const float4 x = *(const float4*)(a.parts + at * a.d + c);
           if (m != -INFINITY) {
-            const float f = exp2f(m - st.x);
+            const float f = aw_exp2(m - st.x);
             o.x = fmaf(f, x.x, o.x), o.y = fmaf(f, x.y, o.y), o.z = fmaf(f, x.z, o.z), o.w = fmaf(f, x.w, o.w);
           }
         }
@@ -584,20 +611,24 @@ __global__ void __launch_bounds__(AW_FIN_THREADS) aw_finish_kernel(AwArgs a) {
     }
     return;
   }
+  // a.groups threads share four slots, each with its part of the vectors
   const int n = (int)min((long long)q.n, a.cap);
-  int j = (blockIdx.x - a.joins) * AW_FIN_SLOTS + t * 4;
-  if (j - t * 4 >= n) return;  // no wait: nothing is read or written
-  const int step = (gridDim.x - a.joins) * AW_FIN_SLOTS;
+  const int quads = AW_FIN_THREADS / a.groups, part = t / quads;
+  int j0 = (blockIdx.x - a.joins) * quads * 4;
+  if (j0 >= n) return;  // no wait: nothing is read or written
+  const int step = (gridDim.x - a.joins) * quads * 4;
   const int first = a.row_slot[q.row0];
   const bool aligned4 = a.cap % 4 == 0 && a.wide_weights;
   const float* scores = a.scores + head * a.vecs * a.kv_pad;
   const long long base = (q.slot * a.hkv + h) * a.cap;
-  constexpr int AHEAD = 4;  // vectors whose scores are on their way while the sums are found
+  constexpr int AHEAD = 4;  // vectors whose scores are on their way at a time, the first while the sums are found
   float4 ahead[AHEAD];
   float old[4];
+  int j = j0 + t % quads * 4;
   auto load_old = [&]() {
 #pragma unroll
     for (int i = 0; i < 4; i++) old[i] = 0.f;
+    if (part) return;
     if (aligned4 && j + 3 < n && j + 3 < first) {
       const float4 x = *(const float4*)(a.weights + base + j);
       old[0] = x.x, old[1] = x.y, old[2] = x.z, old[3] = x.w;
@@ -607,52 +638,84 @@ __global__ void __launch_bounds__(AW_FIN_THREADS) aw_finish_kernel(AwArgs a) {
         if (j + i < n && j + i < first) old[i] = a.weights[base + j + i];
     }
   };
-  auto load_scores = [&]() {
+  auto load_scores = [&](int v0) {
 #pragma unroll
-    for (int v = 0; v < AHEAD; v++)  // what lies behind n was never written, and is not used
-      if (v < vecs && j < n && j + 3 >= q.lo) ahead[v] = *(const float4*)(scores + (long long)v * a.kv_pad + j);
+    for (int i = 0; i < AHEAD; i++) {  // what lies behind n was never written, and is not used
+      const int v = v0 + i * a.groups;
+      if (v < vecs && j < n && j + 3 >= q.lo) ahead[i] = *(const float4*)(scores + (long long)v * a.kv_pad + j);
+    }
   };
   load_old();
   pdl_wait();
   pdl_trigger();
-  load_scores();
+  load_scores(part);
   // of each vector: maximum, 1 / sum, and the slots that it sees, [from, last]
   float4* s_vec = (float4*)fin;
-  for (int v = warp; v < vecs; v += WARPS) {
-    const float2 st = aw_total(a, head, v, s0, s1);
-    if (lane == 0) {
-      const int slot = a.row_slot[q.row0 + v / group];
-      s_vec[v] = make_float4(st.x, st.y, __int_as_float(a.window > 0 ? slot - a.window + 1 : 0), __int_as_float(slot));
+  float4* s_sum = s_vec + a.vecs;  // [AW_FIN_THREADS]
+  auto keep = [&](int v, float2 st) {
+    const int slot = a.row_slot[q.row0 + v / group];
+    s_vec[v] = make_float4(st.x, st.y, __int_as_float(a.window > 0 ? slot - a.window + 1 : 0), __int_as_float(slot));
+  };
+  if (vecs > 2 * WARPS && s1 - s0 <= 16) {  // many vectors of few splits: a thread each
+    for (int v = t; v < vecs; v += AW_FIN_THREADS) {
+      float m = -INFINITY, l = 0.f;
+#pragma unroll 4
+      for (int s = s0; s < s1; s++) {
+        const float2 x = a.stats[(head * a.splits + s) * a.vecs + v];
+        const float top = fmaxf(m, x.x);
+        if (top != -INFINITY) l = l * aw_exp2(m - top) + x.y * aw_exp2(x.x - top);
+        m = top;
+      }
+      keep(v, make_float2(m == -INFINITY ? 0.f : m, l == 0.f ? 0.f : 1.f / l));
+    }
+  } else {
+    for (int v = warp; v < vecs; v += WARPS) {
+      const float2 st = aw_total(a, head, v, s0, s1);
+      if (lane == 0) keep(v, st);
     }
   }
   __syncthreads();
-  while (j < n) {
+  for (; j0 < n; j0 += step) {
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
-    auto add = [&](const float4& x, const float4& vec) {
-      const float y[4] = {x.x, x.y, x.z, x.w};
-      const int from = __float_as_int(vec.z), to = __float_as_int(vec.w);
+    if (j < n && j + 3 >= q.lo) {  // else no row sees them
+      for (int v0 = part; v0 < vecs; v0 += AHEAD * a.groups) {
 #pragma unroll
-      for (int i = 0; i < 4; i++)
-        if (j + i >= from && j + i <= to) sum[i] = fmaf(exp2f(y[i] - vec.x), vec.y, sum[i]);
-    };
-    if (j + 3 >= q.lo) {  // else no row sees them
+        for (int i = 0; i < AHEAD; i++) {
+          const int v = v0 + i * a.groups;
+          if (v >= vecs) continue;
+          const float4 vec = s_vec[v];
+          const float y[4] = {ahead[i].x, ahead[i].y, ahead[i].z, ahead[i].w};
+          const int from = __float_as_int(vec.z), to = __float_as_int(vec.w);
 #pragma unroll
-      for (int v = 0; v < AHEAD; v++)
-        if (v < vecs) add(ahead[v], s_vec[v]);
-#pragma unroll 4
-      for (int v = AHEAD; v < vecs; v++) add(*(const float4*)(scores + (long long)v * a.kv_pad + j), s_vec[v]);
+          for (int e = 0; e < 4; e++)
+            if (j + e >= from && j + e <= to) sum[e] = fmaf(aw_exp2(y[e] - vec.x), vec.y, sum[e]);
+        }
+        load_scores(v0 + AHEAD * a.groups);
+      }
     }
-    float* to = a.weights_out + base + j;
-    if (aligned4 && j + 3 < n) {
-      *(float4*)to = make_float4(old[0] + sum[0], old[1] + sum[1], old[2] + sum[2], old[3] + sum[3]);
-    } else {
+    if (a.groups > 1) {  // the parts, in their order
+      s_sum[t] = make_float4(sum[0], sum[1], sum[2], sum[3]);
+      __syncthreads();
+      if (part == 0)
+        for (int g = 1; g < a.groups; g++) {
+          const float4 x = s_sum[t + g * quads];
+          sum[0] += x.x, sum[1] += x.y, sum[2] += x.z, sum[3] += x.w;
+        }
+      __syncthreads();
+    }
+    if (part == 0 && j < n) {
+      float* to = a.weights_out + base + j;
+      if (aligned4 && j + 3 < n) {
+        *(float4*)to = make_float4(old[0] + sum[0], old[1] + sum[1], old[2] + sum[2], old[3] + sum[3]);
+      } else {
 #pragma unroll
-      for (int i = 0; i < 4; i++)
-        if (j + i < n) to[i] = old[i] + sum[i];
+        for (int i = 0; i < 4; i++)
+          if (j + i < n) to[i] = old[i] + sum[i];
+      }
     }
     j += step;
     load_old();
-    load_scores();
+    load_scores(part);
   }
 }
 
@@ -664,24 +727,27 @@ struct AwPlan {
 
 static size_t aw_round(size_t n) { return (n + 255) / 256 * 256; }
 
-// Blocks of the first kernel on an SM, by their shared memory. For head_dim 128 three with rings of two pages read 5.7 TB/s
+// Blocks of the first kernel on an SM, by their shared memory (tiles of 24: registers). For head_dim 128 three with rings of two pages read 5.7 TB/s
 // where two with rings of three read 5.5 (131071 slots 99.9 against 102.7 us, 32 sequences 156.8 against 162.1 us).
-static int aw_resident(int64_t D) { return D > 64 ? 3 : 4; }
+static int aw_resident(int64_t D, int tile) { return tile == 24 ? 2 : D > 64 ? 3 : 4; }
 
 // How a call is cut: keys_per_split as given, or such that the groups (sequence, kv head, tile) fill the device's resident
-// blocks about once, or several times where there are many groups, since their lengths differ.
+// blocks once; where there are groups enough for that, splits of up to 768 keys, since the groups' lengths differ (shorter
+// ones cost more in the blocks' starts than they even out: 12 sequences of 9 rows over a window of 512 took 56 us with 64
+// keys a split).
 static AwPlan aw_plan(int64_t B, int64_t rows, int64_t Hq, int64_t Hkv, int64_t D, int64_t kv, int64_t window,
                       int64_t kps) {
   AwPlan p;
   p.vecs = rows * (Hq / Hkv);
+  // of 8, 16 or (heads up to 128) 24 vectors; a page costs about 10, 16 and 23
   p.tile = p.vecs <= 8 ? 8 : 16;
+  if (D <= 128 && p.vecs > 16 && (p.vecs + 23) / 24 * 23 < (p.vecs + 15) / 16 * 16) p.tile = 24;
   p.tiles = (int)((p.vecs + p.tile - 1) / p.tile);
   p.kv_pad = (kv + 63) / 64 * 64;
   if (kps == 0) {
-    const int64_t groups = B * Hkv * p.tiles, resident = 148 * aw_resident(D);
+    const int64_t groups = B * Hkv * p.tiles, resident = 148 * aw_resident(D, p.tile);
     const int64_t seen = window > 0 && window + rows < kv ? window + rows : kv;  // slots a sequence's rows can see
-    int64_t want = groups * 2 >= resident ? (resident * 6 + groups - 1) / groups : resident / groups;
-    if (want < 1) want = 1;
+    const int64_t want = groups * 2 >= resident ? (seen + 767) / 768 : resident / groups;
     kps = ((seen + want - 1) / want + 63) / 64 * 64;
   }
   if (kps > p.kv_pad) kps = p.kv_pad;
@@ -708,21 +774,27 @@ int launch_split_d(const AwArgs& a, dim3 grid, cudaStream_t st) {
   return a.d <= 64    ? launch_split<T, 64, NT>(a, grid, st)
          : a.d <= 96  ? launch_split<T, 96, NT>(a, grid, st)
          : a.d <= 128 ? launch_split<T, 128, NT>(a, grid, st)
-                      : launch_split<T, 256, NT>(a, grid, st);
+                      : launch_split<T, 256, NT < 3 ? NT : 2>(a, grid, st);  // NT 3 is not chosen for them
 }
 
 template <typename T>
 int launch_attention_weights(AwArgs& a, int64_t B, cudaStream_t st) {
   const dim3 grid((unsigned)a.seen, (unsigned)(a.hkv * a.tiles), (unsigned)B);
-  const int rc = a.vecs <= 8 ? launch_split_d<T, 1>(a, grid, st) : launch_split_d<T, 2>(a, grid, st);
+  const int rc = a.tile == 8    ? launch_split_d<T, 1>(a, grid, st)
+                 : a.tile == 16 ? launch_split_d<T, 2>(a, grid, st)
+                                : launch_split_d<T, 3>(a, grid, st);
   if (rc != IM_OK) return rc;
   // many splits that a row can see: a block's eight warps share a job's, else each has a job
   a.join_warps = a.seen >= 16 ? AW_FIN_THREADS / 32 : 1;
   a.joins = (int)(((int64_t)a.vecs * ((a.d + 127) / 128) * a.join_warps * 32 + AW_FIN_THREADS - 1) / AW_FIN_THREADS);
-  // blocks of slots a (sequence, kv head): the device's worth in all, so that a block's sums serve many slots
-  const int64_t most = (a.max_kv + AW_FIN_SLOTS - 1) / AW_FIN_SLOTS, share = (369 + B * a.hkv) / (B * a.hkv);
-  const int chunks = (int)(most < share ? most : share);
-  const size_t join = sizeof(float4) * AW_FIN_THREADS, sums = sizeof(float4) * a.vecs;
+  // blocks of slots a (sequence, kv head): the device's worth in all, so that a block's sums serve many slots; where the
+  // slots are too few for them, threads share slots by vectors
+  const int64_t share = (369 + B * a.hkv) / (B * a.hkv);
+  auto blocks = [&](int groups) { return ((int64_t)a.max_kv * groups + AW_FIN_THREADS * 4 - 1) / (AW_FIN_THREADS * 4); };
+  a.groups = 1;
+  while (a.groups < 8 && a.vecs >= a.groups * 16 && blocks(a.groups * 2) <= (share > 2 ? share : 2)) a.groups *= 2;
+  const int chunks = (int)(blocks(a.groups) < share ? blocks(a.groups) : share);
+  const size_t join = sizeof(float4) * AW_FIN_THREADS, sums = sizeof(float4) * (a.vecs + AW_FIN_THREADS);
   return launch("aw_finish_kernel", aw_finish_kernel<T>, dim3((unsigned)(a.joins + chunks), (unsigned)a.hkv, (unsigned)B),
                 dim3(AW_FIN_THREADS), join > sums ? join : sums, st, a);
 }
@@ -778,7 +850,7 @@ extern "C" int im_attention_weights(const void* q, const void* k_cache, const vo
   a.weights = weights, a.weights_out = weights_out, a.cap = cap;
   a.M = (int)M, a.max_rows = (int)max_rows_per_seq, a.hq = (int)Hq, a.hkv = (int)Hkv, a.d = (int)D;
   a.max_kv = (int)max_kv_len, a.kv_pad = (int)p.kv_pad, a.window = (int)window, a.scale = scale, a.out = (char*)out;
-  a.kps = p.kps, a.splits = p.splits, a.tiles = p.tiles, a.seen = p.seen, a.vecs = (int)p.vecs;
+  a.kps = p.kps, a.splits = p.splits, a.tile = p.tile, a.tiles = p.tiles, a.seen = p.seen, a.vecs = (int)p.vecs;
   a.wide_weights = aligned(weights, 16) && aligned(weights_out, 16);
   a.scores = (float*)workspace;
   a.stats = (float2*)((char*)workspace + p.scores);
