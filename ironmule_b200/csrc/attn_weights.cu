@@ -535,11 +535,12 @@ __global__ void __launch_bounds__(AwShape<DP, NT>::WARPS * 32, NT > 2 ? 2 : DP >
   }
 }
 
-// The final maximum and 1 / sum of one vector over its splits [s0, s1), by a warp; every lane gets them.
+// The final maximum and 1 / sum of one vector over its splits [s0, s1), by a warp; every lane gets them. Split s is lane
+// s mod 32's, whatever s0 and s1 are: splits that a row does not see change no bit of its sum.
 __device__ __forceinline__ float2 aw_total(const AwArgs& a, long long head, int v, int s0, int s1) {
   const int lane = threadIdx.x & 31;
   float m = -INFINITY, l = 0.f;
-  for (int s = s0 + lane; s < s1; s += 32) {
+  for (int s = s0 + ((lane - s0) & 31); s < s1; s += 32) {
     const float2 x = a.stats[(head * a.splits + s) * a.vecs + v];
     const float top = fmaxf(m, x.x);
     if (top != -INFINITY) l = l * aw_exp2(m - top) + x.y * aw_exp2(x.x - top);
@@ -576,30 +577,40 @@ __global__ void __launch_bounds__(AW_FIN_THREADS, 4) aw_finish_kernel(AwArgs a) 
     const int segments = (a.d + 127) / 128;  // of 128 values
     const int job = blockIdx.x * (WARPS / a.join_warps) + warp / a.join_warps;
     const int v = job / segments, c = job % segments * 128 + lane * 4;
+    // the splits are added in eight runs, split s to run s mod 8, and the runs in their order, however many warps do it
+    constexpr int RUNS = AW_FIN_THREADS / 32;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     float2 st = make_float2(0.f, 0.f);
-    if (v < vecs) {
-      st = aw_total(a, head, v, s0, s1);
-      if (c < a.d) {
+    auto add = [&](int run) {
+      float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-        for (int s = s0 + warp % a.join_warps; s < s1; s += a.join_warps) {
-          const long long at = (head * a.splits + s) * a.vecs + v;
-          const float m = a.stats[at].x;
-          const float4 x = *(const float4*)(a.parts + at * a.d + c);
-          if (m != -INFINITY) {
-            const float f = aw_exp2(m - st.x);
-            o.x = fmaf(f, x.x, o.x), o.y = fmaf(f, x.y, o.y), o.z = fmaf(f, x.z, o.z), o.w = fmaf(f, x.w, o.w);
-          }
+      for (int s = s0 + ((run - s0) & (RUNS - 1)); s < s1; s += RUNS) {
+        const long long at = (head * a.splits + s) * a.vecs + v;
+        const float m = a.stats[at].x;
+        const float4 x = *(const float4*)(a.parts + at * a.d + c);
+        if (m != -INFINITY) {
+          const float f = aw_exp2(m - st.x);
+          y.x = fmaf(f, x.x, y.x), y.y = fmaf(f, x.y, y.y), y.z = fmaf(f, x.z, y.z), y.w = fmaf(f, x.w, y.w);
         }
       }
-    }
-    if (a.join_warps > 1) {  // in the warps' order
-      float4* part = (float4*)fin;
-      part[t] = o;
+      return y;
+    };
+    if (v < vecs) st = aw_total(a, head, v, s0, s1);
+    if (a.join_warps > 1) {
+      float4* sums = (float4*)fin;
+      if (v < vecs && c < a.d) o = add(warp);
+      sums[t] = o;
       __syncthreads();
-      if (warp % a.join_warps) return;
-      for (int w = 1; w < a.join_warps; w++) {
-        const float4 x = part[t + w * 32];
+      if (warp) return;
+      for (int w = 1; w < RUNS; w++) {
+        const float4 x = sums[t + w * 32];
+        o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
+      }
+    } else if (v < vecs && c < a.d) {
+      o = add(0);
+#pragma unroll
+      for (int run = 1; run < RUNS; run++) {
+        const float4 x = add(run);
         o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
       }
     }

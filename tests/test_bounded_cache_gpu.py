@@ -322,6 +322,24 @@ def test_attention_weights_bits_do_not_depend_on_the_launch(cuda):
     assert torch.equal(again, many)
 
 
+@pytest.mark.parametrize("window", [0, 700])
+def test_attention_weights_bits_over_many_splits(cuda, window):
+    """The same with more splits than one warp joins, and rows whose windows begin at different splits: neither the launch's
+    max_kv_len nor the other rows' windows change a row's bits."""
+    lengths, rows = [2500, 1300, 1999], [5, 1, 3]
+    q, k, v, table, bounds, slot, weights = attend_case(cuda, 12, lengths, rows, 8, 2, 64, torch.float16)
+    slot[0], slot[6] = 900, 1500  # rows of other splits beside rows at the end
+    kw = {"scale": 0.125, "keys_per_split": 64, "window": window}
+    many = kernels.attention_weights(q, k, v, table, bounds, slot, weights.clone(), max_rows_per_seq=5, max_kv_len=2520, **kw)
+    for b in range(3):
+        for r in range(int(bounds[b]), int(bounds[b + 1])):
+            for most in (int(slot[r]) + 1, 2520):
+                one = kernels.attention_weights(q[r:r + 1].contiguous(), k, v, table, ints([0, 1], cuda),
+                                                slot[r:r + 1].contiguous(), weights.clone(), max_rows_per_seq=1,
+                                                max_kv_len=most, seq_slot=ints([b], cuda), **kw)
+                assert torch.equal(one[0], many[r])
+
+
 def test_attention_weights_masks(cuda):
     # masked rows, a sequence without rows, table rows in another order, weights shorter than the cache, a short max_kv
     q, k, v, table, bounds, slot, weights = attend_case(cuda, 4, [90, 40, 77], [3, 0, 2], 4, 2, 64, torch.float16)
