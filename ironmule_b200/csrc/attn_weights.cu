@@ -606,6 +606,24 @@ __global__ void __launch_bounds__(AW_FIN_THREADS, 4) aw_finish_kernel(AwArgs a) 
         const float4 x = sums[t + w * 32];
         o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
       }
+    } else if (v < vecs && c < a.d && s1 - s0 <= RUNS) {  // a split a run at most: all loads on their way at once
+      float4 x[RUNS];
+      float m[RUNS];
+#pragma unroll
+      for (int run = 0; run < RUNS; run++) {
+        const int s = s0 + ((run - s0) & (RUNS - 1));
+        const long long at = (head * a.splits + s) * a.vecs + v;
+        m[run] = s < s1 ? a.stats[at].x : -INFINITY;
+        if (s < s1) x[run] = *(const float4*)(a.parts + at * a.d + c);
+      }
+#pragma unroll
+      for (int run = 0; run < RUNS; run++)
+        if (m[run] != -INFINITY) {
+          const float f = aw_exp2(m[run] - st.x);
+          // not contracted: a run's sum is rounded before it joins
+          o.x = __fadd_rn(o.x, __fmul_rn(f, x[run].x)), o.y = __fadd_rn(o.y, __fmul_rn(f, x[run].y));
+          o.z = __fadd_rn(o.z, __fmul_rn(f, x[run].z)), o.w = __fadd_rn(o.w, __fmul_rn(f, x[run].w));
+        }
     } else if (v < vecs && c < a.d) {
       o = add(0);
 #pragma unroll
