@@ -481,7 +481,8 @@ size_t im_kq_workspace_bytes(int64_t K, int64_t B);
  * left alone. weights_out may be weights. Rows that see no slot (row_slot -1, say) get zeros and add nothing. Splits:
  * multiples of keys_per_split (a multiple of 64; 0: chosen by the sizes of the call); keep it fixed and a row's bits do
  * not depend on the launch. The workspace holds 4 bytes a (row, query head, slot). seq_rows is clamped to the M rows of q; rows beyond max_rows_per_seq are not computed. No two
- * sequences may name one table row. Workspace 256-byte aligned, nothing to initialise.
+ * sequences may name one table row. Workspace 256-byte aligned, nothing to initialise;
+ * calls of few, short splits need none (0 bytes).
  *
  * im_cache_evict: of the n = lengths[s] slots of every (layer, sequence, kv head), min(n, budget) stay: those whose
  * position (slot_pos) is below `sinks` or at least seen[s] - recent, then the heaviest (weights; NaN lightest), lower

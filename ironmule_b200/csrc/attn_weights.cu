@@ -15,11 +15,15 @@
 // page's time; tcgen05's tiles of 64 rows and more would add more of that. Scores go to the workspace in float32 (4 bytes
 // a vector and slot beside 4 D of K and V): the weights need the final maximum and sum.
 // Second kernel (aw_finish_kernel): joins the splits, and adds up exp2(s - max) / sum slot by slot.
+// Calls of few and short splits are one kernel's (aw_split_kernel with ONE): the splits of a (sequence, kv head) are a
+// cluster, scores stay in shared memory, and the blocks tell each other their maxima, sums and accumulators through
+// distributed shared memory. One token over 2048 slots takes one launch and no workspace then.
 //
 // Weights that meet v are two numbers of the cache's type, high part and rest (16 bits and more of each weight are kept);
 // in float16 they are scaled by 2^6 to 2^14 first, so that weights down to 2^-20 of the largest are not subnormal. Masked
 // slots never reach a row: behind the last visible slot v is zeroed on its way in; between rows of one call a page is
 // checked for values that are not finite, and if it has any its products are done one by one.
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -27,9 +31,13 @@
 
 namespace im {
 
+namespace cg = cooperative_groups;
+
 constexpr int AW_FIN_THREADS = 256;
 constexpr float AW_LOG2E = 1.4426950408889634f;
 constexpr float AW_SLACK = 8.f;
+constexpr int AW_CLUSTER = 16;             // splits of a call that one kernel does
+constexpr int AW_HELD = 24 * 1024;         // and bytes of scores that its blocks hold
 
 struct AwArgs {
   const char* q;
@@ -177,6 +185,29 @@ struct AwType<__half> {
   static __device__ __forceinline__ __half down(float f) { return __float2half_rn(f); }
 };
 
+// The total of a vector whose splits' maxima and sums lie in a warp's lanes (-inf and 0 where there is none): maximum and
+// 1 / sum, in every lane.
+__device__ __forceinline__ float2 aw_join(float m, float l) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), l2 = __shfl_xor_sync(0xffffffffu, l, o);
+    const float top = fmaxf(m, m2);
+    if (top != -INFINITY) l = l * aw_exp2(m - top) + l2 * aw_exp2(m2 - top);
+    m = top;
+  }
+  return make_float2(m == -INFINITY ? 0.f : m, l == 0.f ? 0.f : 1.f / l);
+}
+
+// Four values of vector v's output.
+template <typename T>
+__device__ __forceinline__ void aw_store(const AwArgs& a, const AwSeq& q, int h, int group, int v, int c, const float4& o,
+                                         float inv) {
+  const long long row = q.row0 + v / group;
+  alignas(8) T r[4] = {AwType<T>::down(o.x * inv), AwType<T>::down(o.y * inv), AwType<T>::down(o.z * inv),
+                       AwType<T>::down(o.w * inv)};
+  *(uint2*)((T*)a.out + (row * a.hq + h * group + v % group) * a.d + c) = *(const uint2*)r;
+}
+
 // DP: head_dim rounded up to what is built; columns from d on are zeros in shared memory. NT: tiles of 8 vectors a block.
 template <int DP, int NT>
 struct AwShape {
@@ -190,10 +221,11 @@ struct AwShape {
   static_assert(Q_REGS || NT == 2, "Q in shared memory is read two tiles at a time");
   static constexpr int Q_BYTES = Q_REGS ? 0 : NT * 8 * PITCH;
   static constexpr int SMEM = WARPS * RING + Q_BYTES;
+  static constexpr int SMEM_ONE = SMEM + NT * 8 * JOIN * 4 + AW_HELD + NT * 8 * 16;  // with accumulators and scores, padded
   static_assert(NT * 8 * JOIN * 4 <= RING, "a warp's ring takes its accumulator at the end");
 };
 
-template <typename T, int DP, int NT>
+template <typename T, int DP, int NT, bool ONE>
 __global__ void __launch_bounds__(AwShape<DP, NT>::WARPS * 32, NT > 2 ? 2 : DP > 64 ? 3 : 4)
     aw_split_kernel(AwArgs a) {
   using S = AwShape<DP, NT>;
@@ -201,6 +233,11 @@ __global__ void __launch_bounds__(AwShape<DP, NT>::WARPS * 32, NT > 2 ? 2 : DP >
   constexpr int TILE = NT * 8, WARPS = S::WARPS;
   extern __shared__ __align__(128) char smem[];
   __shared__ float s_m[WARPS][TILE], s_l[WARPS][TILE];
+  // ONE: this block's maxima and sums, the whole cluster's, the final ones
+  __shared__ float2 s_stat[ONE ? TILE : 1], s_all[ONE ? AW_CLUSTER : 1][ONE ? TILE : 1], s_total[ONE ? TILE : 1];
+  float* s_out = (float*)(smem + S::SMEM);  // ONE: [TILE][JOIN]
+  float* s_scores = s_out + TILE * S::JOIN;  // ONE: [TILE][kps + 4]
+  const int held = a.kps + 4;
   pdl_wait();
   pdl_trigger();
   int split = blockIdx.x;  // with a window: counted from the first that a row sees
@@ -210,13 +247,13 @@ __global__ void __launch_bounds__(AwShape<DP, NT>::WARPS * 32, NT > 2 ? 2 : DP >
   AwSeq q = aw_seq(a, b);
   const int group = a.hq / a.hkv;
   const int vecs = q.rows * group;  // live ones
-  if (tile * TILE >= vecs || q.slot < 0) return;
-  const int* table = a.page_table + q.slot * a.max_pages;
+  if (tile * TILE >= vecs || (!ONE && q.slot < 0)) return;  // the whole cluster
+  const int* table = a.page_table + max(q.slot, 0ll) * a.max_pages;
   // pages of this warp: those whose number is warp mod WARPS, so that a slot's place does not depend on the call. The page
   // numbers are fetched a round ahead of the copies that need them, the first before it is known how many there are
   int next = split * a.kps / 16;
   next += (warp - next) & (WARPS - 1);
-  int entry = a.window == 0 && next < a.max_pages ? table[next] : 0;
+  int entry = a.window == 0 && q.slot >= 0 && next < a.max_pages ? table[next] : 0;
   // this lane's vectors of each tile of 8: 2 (lane mod 4) and the next (accumulators), lane / 4 (Q as an operand)
   int last[NT][2], from[NT][2];
   bool live[NT][2];
@@ -282,8 +319,8 @@ __global__ void __launch_bounds__(AwShape<DP, NT>::WARPS * 32, NT > 2 ? 2 : DP >
   // one split, unless rows with a window lie so far apart that there are more than blocks
   for (;; split += gridDim.x) {
     const int k0 = max(split * a.kps, q.lo / 16 * 16), k1 = min(split * a.kps + a.kps, q.n);
-    if (k0 >= k1) return;  // the whole block
-    const int p0 = k0 / 16, p1 = (k1 + 15) / 16;
+    if (!ONE && k0 >= k1) return;  // the whole block
+    const int p0 = k0 / 16, p1 = k0 < k1 ? (k1 + 15) / 16 : p0;
     if (a.window > 0 || split != (int)blockIdx.x) {
       next = p0 + ((warp - p0) & (WARPS - 1));
       entry = next < p1 ? table[next] : 0;
@@ -422,7 +459,8 @@ __global__ void __launch_bounds__(AwShape<DP, NT>::WARPS * 32, NT > 2 ? 2 : DP >
 #pragma unroll
         for (int e = 0; e < 2; e++)
           if (live[nt][e]) {
-            float* to = scores + (long long)(nt * 8 + e) * a.kv_pad + page * 16;
+            float* to = ONE ? s_scores + (nt * 8 + lane % 4 * 2 + e) * held + page * 16 - split * a.kps + lane / 4
+                            : scores + (long long)(nt * 8 + e) * a.kv_pad + page * 16;
             to[0] = s[nt][e];
             to[8] = s[nt][e + 2];
           }
@@ -520,7 +558,8 @@ __global__ void __launch_bounds__(AwShape<DP, NT>::WARPS * 32, NT > 2 ? 2 : DP >
           const float4 y = *(const float4*)(smem + w * S::RING + (row * S::JOIN + c) * 4);
           x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
         }
-        *(float4*)(a.parts + (at + row) * a.d + c) = x;
+        if (ONE) *(float4*)(s_out + row * S::JOIN + c) = x;
+        else *(float4*)(a.parts + (at + row) * a.d + c) = x;
       }
     if (t < count) {
       float mm = s_m[0][t];
@@ -529,7 +568,74 @@ __global__ void __launch_bounds__(AwShape<DP, NT>::WARPS * 32, NT > 2 ? 2 : DP >
       float sum = 0.f;
 #pragma unroll
       for (int w = 0; w < WARPS; w++) sum += s_m[w][t] == -INFINITY ? 0.f : aw_exp2(s_m[w][t] - mm) * s_l[w][t];
-      a.stats[at + t] = make_float2(mm, sum);
+      if (ONE) s_stat[t] = make_float2(mm, sum);
+      else a.stats[at + t] = make_float2(mm, sum);
+    }
+    if constexpr (ONE) {
+      cg::cluster_group cluster = cg::this_cluster();
+      const int ranks = gridDim.x;
+      // this block's slots and their weights so far, on their way while the blocks meet
+      const int n = (int)min((long long)min(split * a.kps + a.kps, q.n), a.cap), first = a.row_slot[q.row0];
+      const long long base = (q.slot * a.hkv + h) * a.cap;
+      constexpr int MOST = 768 / (WARPS * 32);  // slots of a thread: AW_HELD / 4 / 8 of a block
+      float old[MOST];
+#pragma unroll
+      for (int i = 0; i < MOST; i++) {
+        const int j = split * a.kps + t + i * WARPS * 32;
+        old[i] = j < n && j < first ? a.weights[base + j] : 0.f;
+      }
+      cluster.sync();
+      for (int i = t; i < ranks * count; i += WARPS * 32) {
+        const int r = i / count, v = i - r * count;
+        s_all[r][v] = *cluster.map_shared_rank(&s_stat[v], r);
+      }
+      __syncthreads();
+      for (int v = warp; v < count; v += WARPS) {  // as aw_total does
+        float mm = lane < ranks ? s_all[lane % AW_CLUSTER][v].x : -INFINITY;
+        float ll = lane < ranks ? s_all[lane % AW_CLUSTER][v].y : 0.f;
+        const float2 st = aw_join(mm, ll);
+        if (lane == 0) s_total[v] = st;
+      }
+      __syncthreads();
+      // the output: splits in eight runs, as aw_finish_kernel joins them; four values a thread, dealt to the blocks
+      for (int u = split + ranks * t; u < count * (a.d / 4); u += ranks * WARPS * 32) {
+        const int v = u / (a.d / 4), c = (u - v * (a.d / 4)) * 4;
+        const float2 st = s_total[v];
+        float4 x[AW_CLUSTER];
+#pragma unroll
+        for (int r = 0; r < AW_CLUSTER; r++)
+          if (r < ranks) x[r] = *(const float4*)cluster.map_shared_rank(s_out + v * S::JOIN + c, r);
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int run = 0; run < 8; run++) {
+          float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int r = run; r < AW_CLUSTER; r += 8) {
+            const float at_r = r < ranks ? s_all[r][v].x : -INFINITY;
+            if (at_r != -INFINITY) {
+              const float f = aw_exp2(at_r - st.x);
+              y.x = fmaf(f, x[r].x, y.x), y.y = fmaf(f, x[r].y, y.y);
+              y.z = fmaf(f, x[r].z, y.z), y.w = fmaf(f, x[r].w, y.w);
+            }
+          }
+          sum.x += y.x, sum.y += y.y, sum.z += y.z, sum.w += y.w;
+        }
+        aw_store<T>(a, q, h, group, v, c, sum, st.y);
+      }
+      // the weights of this block's slots
+#pragma unroll
+      for (int i = 0; i < MOST; i++) {
+        const int j = split * a.kps + t + i * WARPS * 32;
+        if (j >= n) continue;
+        float sum = 0.f;
+        for (int v = 0; v < count; v++) {
+          const float2 st = s_total[v];
+          sum = fmaf(aw_exp2(s_scores[v * held + j - split * a.kps] - st.x), st.y, sum);
+        }
+        a.weights_out[base + j] = old[i] + sum;
+      }
+      cluster.sync();  // nobody leaves while its accumulators are read
+      return;
     }
     __syncthreads();  // the ring is the copies' again
   }
@@ -546,14 +652,7 @@ __device__ __forceinline__ float2 aw_total(const AwArgs& a, long long head, int 
     if (top != -INFINITY) l = l * aw_exp2(m - top) + x.y * aw_exp2(x.x - top);
     m = top;
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), l2 = __shfl_xor_sync(0xffffffffu, l, o);
-    const float top = fmaxf(m, m2);
-    if (top != -INFINITY) l = l * aw_exp2(m - top) + l2 * aw_exp2(m2 - top);
-    m = top;
-  }
-  return make_float2(m == -INFINITY ? 0.f : m, l == 0.f ? 0.f : 1.f / l);
+  return aw_join(m, l);
 }
 
 // Joins the splits of a (sequence, kv head): the first a.joins blocks of x the output, 128 values of one vector a job of
@@ -632,12 +731,7 @@ __global__ void __launch_bounds__(AW_FIN_THREADS, 4) aw_finish_kernel(AwArgs a) 
         o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
       }
     }
-    if (v < vecs && c < a.d) {
-      const long long row = q.row0 + v / group;
-      alignas(8) T r[4] = {AwType<T>::down(o.x * st.y), AwType<T>::down(o.y * st.y), AwType<T>::down(o.z * st.y),
-                           AwType<T>::down(o.w * st.y)};
-      *(uint2*)((T*)a.out + (row * a.hq + h * group + v % group) * a.d + c) = *(const uint2*)r;
-    }
+    if (v < vecs && c < a.d) aw_store<T>(a, q, h, group, v, c, o, st.y);
     return;
   }
   // a.groups threads share four slots, each with its part of the vectors
@@ -751,6 +845,7 @@ __global__ void __launch_bounds__(AW_FIN_THREADS, 4) aw_finish_kernel(AwArgs a) 
 struct AwPlan {
   int kps, splits, tile, tiles, seen;
   long long vecs, kv_pad;
+  bool one;                     // one kernel does it
   size_t scores, stats, parts;  // bytes
 };
 
@@ -773,17 +868,28 @@ static AwPlan aw_plan(int64_t B, int64_t rows, int64_t Hq, int64_t Hkv, int64_t 
   if (D <= 128 && p.vecs > 16 && (p.vecs + 23) / 24 * 23 < (p.vecs + 15) / 16 * 16) p.tile = 24;
   p.tiles = (int)((p.vecs + p.tile - 1) / p.tile);
   p.kv_pad = (kv + 63) / 64 * 64;
+  // one kernel: no window (its splits begin where the rows' slots say), one tile, blocks that are on the device at once
+  const int64_t groups = B * Hkv * p.tiles;
+  auto one = [&](int64_t k) {
+    const int64_t n = (kv + k - 1) / k;
+    return window == 0 && p.tiles == 1 && n <= AW_CLUSTER && groups * n <= 296 && p.tile * k * 4 <= AW_HELD;
+  };
   if (kps == 0) {
-    const int64_t groups = B * Hkv * p.tiles, resident = 148 * aw_resident(D, p.tile);
+    const int64_t resident = 148 * aw_resident(D, p.tile);
     const int64_t seen = window > 0 && window + rows < kv ? window + rows : kv;  // slots a sequence's rows can see
-    const int64_t want = groups * 2 >= resident ? (seen + 767) / 768 : resident / groups;
-    kps = ((seen + want - 1) / want + 63) / 64 * 64;
+    const int64_t most = groups <= 296 ? 296 / groups : 1, few = most < AW_CLUSTER ? most : AW_CLUSTER;
+    kps = ((kv + few - 1) / few + 63) / 64 * 64;
+    if (!one(kps) || kps > 256) {
+      const int64_t want = groups * 2 >= resident ? (seen + 767) / 768 : resident / groups;
+      kps = ((seen + want - 1) / want + 63) / 64 * 64;
+    }
   }
   if (kps > p.kv_pad) kps = p.kv_pad;
   p.kps = (int)kps;
   p.splits = (int)((kv + kps - 1) / kps);
+  p.one = one(kps);
   p.seen = window > 0 && (window + rows) / kps + 2 < p.splits ? (int)((window + rows) / kps + 2) : p.splits;
-  const size_t heads = (size_t)B * Hkv;
+  const size_t heads = p.one ? 0 : (size_t)B * Hkv;
   p.scores = aw_round(heads * p.vecs * p.kv_pad * 4);
   p.stats = aw_round(heads * p.splits * p.vecs * 8);
   p.parts = aw_round(heads * p.splits * p.vecs * D * 4);
@@ -791,28 +897,35 @@ static AwPlan aw_plan(int64_t B, int64_t rows, int64_t Hq, int64_t Hkv, int64_t 
 }
 
 template <typename T, int DP, int NT>
-int launch_split(const AwArgs& a, dim3 grid, cudaStream_t st) {
+int launch_split(const AwArgs& a, bool one, dim3 grid, cudaStream_t st) {
+  constexpr int threads = AwShape<DP, NT>::WARPS * 32;
+  if (one) {
+    const int rc = configure<aw_split_kernel<T, DP, NT, true>>("aw_split_kernel", AwShape<DP, NT>::SMEM_ONE, true);
+    if (rc != IM_OK) return rc;
+    return launch_cluster("aw_split_kernel", aw_split_kernel<T, DP, NT, true>, grid, dim3(threads), (int)grid.x,
+                          AwShape<DP, NT>::SMEM + NT * 8 * (AwShape<DP, NT>::JOIN + a.kps + 4) * 4, st, a);
+  }
   constexpr int smem = AwShape<DP, NT>::SMEM;
-  const int rc = configure<aw_split_kernel<T, DP, NT>>("aw_split_kernel", smem, false);
+  const int rc = configure<aw_split_kernel<T, DP, NT, false>>("aw_split_kernel", smem, false);
   if (rc != IM_OK) return rc;
-  return launch("aw_split_kernel", aw_split_kernel<T, DP, NT>, grid, dim3(AwShape<DP, NT>::WARPS * 32), smem, st, a);
+  return launch("aw_split_kernel", aw_split_kernel<T, DP, NT, false>, grid, dim3(threads), smem, st, a);
 }
 
 template <typename T, int NT>
-int launch_split_d(const AwArgs& a, dim3 grid, cudaStream_t st) {
-  return a.d <= 64    ? launch_split<T, 64, NT>(a, grid, st)
-         : a.d <= 96  ? launch_split<T, 96, NT>(a, grid, st)
-         : a.d <= 128 ? launch_split<T, 128, NT>(a, grid, st)
-                      : launch_split<T, 256, NT < 3 ? NT : 2>(a, grid, st);  // NT 3 is not chosen for them
+int launch_split_d(const AwArgs& a, bool one, dim3 grid, cudaStream_t st) {
+  return a.d <= 64    ? launch_split<T, 64, NT>(a, one, grid, st)
+         : a.d <= 96  ? launch_split<T, 96, NT>(a, one, grid, st)
+         : a.d <= 128 ? launch_split<T, 128, NT>(a, one, grid, st)
+                      : launch_split<T, 256, NT < 3 ? NT : 2>(a, one, grid, st);  // NT 3 is not chosen for them
 }
 
 template <typename T>
-int launch_attention_weights(AwArgs& a, int64_t B, cudaStream_t st) {
+int launch_attention_weights(AwArgs& a, bool one, int64_t B, cudaStream_t st) {
   const dim3 grid((unsigned)a.seen, (unsigned)(a.hkv * a.tiles), (unsigned)B);
-  const int rc = a.tile == 8    ? launch_split_d<T, 1>(a, grid, st)
-                 : a.tile == 16 ? launch_split_d<T, 2>(a, grid, st)
-                                : launch_split_d<T, 3>(a, grid, st);
-  if (rc != IM_OK) return rc;
+  const int rc = a.tile == 8    ? launch_split_d<T, 1>(a, one, grid, st)
+                 : a.tile == 16 ? launch_split_d<T, 2>(a, one, grid, st)
+                                : launch_split_d<T, 3>(a, one, grid, st);
+  if (rc != IM_OK || one) return rc;
   // many splits that a row can see: a block's eight warps share a job's, else each has a job
   a.join_warps = a.seen >= 16 ? AW_FIN_THREADS / 32 : 1;
   a.joins = (int)(((int64_t)a.vecs * ((a.d + 127) / 128) * a.join_warps * 32 + AW_FIN_THREADS - 1) / AW_FIN_THREADS);
@@ -868,7 +981,7 @@ extern "C" int im_attention_weights(const void* q, const void* k_cache, const vo
              IM_UNSUPPORTED, "im_attention_weights: too large");
   const int64_t kv = max_kv_len > 0 ? max_kv_len : 1;
   const size_t need = im_attention_weights_workspace_bytes(B, max_rows_per_seq, Hq, Hkv, D, kv, keys_per_split, window);
-  IM_REQUIRE(workspace && aligned(workspace, 256) && workspace_bytes >= need, IM_INVALID,
+  IM_REQUIRE(need == 0 || (workspace && aligned(workspace, 256) && workspace_bytes >= need), IM_INVALID,
              "im_attention_weights: a workspace of %zu bytes needed, %zu given", need, workspace_bytes);
   AwArgs a = {};
   const AwPlan p = aw_plan(B, max_rows_per_seq, Hq, Hkv, D, kv, window, keys_per_split);
@@ -885,5 +998,6 @@ extern "C" int im_attention_weights(const void* q, const void* k_cache, const vo
   a.stats = (float2*)((char*)workspace + p.scores);
   a.parts = (float*)((char*)workspace + p.scores + p.stats);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  return dtype == IM_BF16 ? launch_attention_weights<__nv_bfloat16>(a, B, st) : launch_attention_weights<__half>(a, B, st);
+  return dtype == IM_BF16 ? launch_attention_weights<__nv_bfloat16>(a, p.one, B, st)
+                          : launch_attention_weights<__half>(a, p.one, B, st);
 }

@@ -1017,11 +1017,11 @@ def attention_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
         return out
     max_rows = min(max_rows_per_seq, m)
     need = _attention_weights_workspace(b, max_rows, hq, hkv, d, max(1, max_kv_len), keys_per_split, window)
-    ws = torch.empty(need, dtype=torch.uint8, device=device)
+    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None  # few, short splits need none
     _launch(index, "im_attention_weights", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _TYPES[dtype],
             page_table.data_ptr(), seqs, max_pages, pages, seq_rows.data_ptr(),
             _ptr_or_none(seq_slot), row_slot.data_ptr(), m, b, max_rows, hq, hkv, d, max_kv_len, keys_per_split, window,
-            float(scale), weights.data_ptr(), weights_out.data_ptr(), cap, out.data_ptr(), ws.data_ptr(),
+            float(scale), weights.data_ptr(), weights_out.data_ptr(), cap, out.data_ptr(), _ptr_or_none(ws),
             need)
     return out
 

@@ -89,8 +89,8 @@ def test_attention_weights_refusals():
     assert attend(b=0)[0] == attend(rows=0)[0] == attend(m=0)[0] == _lib.IM_OK
     for kw, word in (({"hq": 3}, "sizes"), ({"b": -1}, "sizes"), ({"window": -1}, "sizes"), ({"cap": -1}, "sizes"),
                      ({"kps": 65}, "multiple of 64"), ({"kps": -64}, "multiple of 64"), ({"ptr": None}, "null"),
-                     ({"ptr": 264}, "aligned"), ({"ws": None}, "workspace"), ({"ws": 128}, "workspace"),
-                     ({"size": 64}, "workspace")):
+                     ({"ptr": 264}, "aligned"), ({"ws": None, "window": 9}, "workspace"),
+                     ({"ws": 128, "window": 9}, "workspace"), ({"size": 64, "window": 9}, "workspace")):
         rc, msg = attend(**kw)
         assert rc == _lib.IM_INVALID and word in msg, (kw, msg)
     for kw, word in (({"dtype": 2}, "type"), ({"d": 8}, "head_dim"), ({"d": 72}, "head_dim"), ({"d": 272}, "head_dim"),
@@ -98,8 +98,10 @@ def test_attention_weights_refusals():
         rc, msg = attend(**kw)
         assert rc == _lib.IM_UNSUPPORTED and word in msg, (kw, msg)
     lib = _lib.load()
-    need = lib.im_attention_weights_workspace_bytes(2, 1, 4, 2, 64, 100, 0, 0)
-    assert need > 0 and attend(size=need - 1)[0] == _lib.IM_INVALID
+    need = lib.im_attention_weights_workspace_bytes(2, 1, 4, 2, 64, 100, 0, 9)
+    assert need > 0 and attend(size=need - 1, window=9)[0] == _lib.IM_INVALID
+    assert lib.im_attention_weights_workspace_bytes(2, 1, 4, 2, 64, 100, 0, 0) == 0  # one kernel, nothing to hold
+    assert lib.im_attention_weights_workspace_bytes(2, 1, 4, 2, 64, 10000, 0, 0) > 0
     assert lib.im_attention_weights_workspace_bytes(0, 1, 4, 2, 64, 100, 0, 0) == 0
     assert lib.im_attention_weights_workspace_bytes(1, 1, 3, 2, 64, 100, 0, 0) == 0
 
