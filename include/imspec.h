@@ -491,7 +491,7 @@ size_t im_kq_workspace_bytes(int64_t K, int64_t B);
  * the slots before the new end, lengths_out [S] (may be lengths) the new length, the same for every layer and head. weights and
  * slot_pos are [layers][S][Hkv][cap], the caches `layers` times [pages][Hkv][16][row_bytes], layer_bytes apart; n is at
  * most min(cap, 16 max_pages), cap at most 262144. Sequences must not share the pages of a cache that is cut. sinks + recent <= budget.
- * Workspace 16-byte aligned, nothing to initialise.
+ * Workspace 16-byte aligned, nothing to initialise; none (0 bytes) where few slots of a row can move.
  *
  * im_verify_sampled: keeps or refuses drafted tokens by the target's probabilities and given random numbers. target
  * [B * (K + 1)] rows of V (row stride target_ld; row b (K + 1) + i is the distribution of the token after draft i - 1),

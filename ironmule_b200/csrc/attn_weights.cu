@@ -879,7 +879,10 @@ static AwPlan aw_plan(int64_t B, int64_t rows, int64_t Hq, int64_t Hkv, int64_t 
     const int64_t seen = window > 0 && window + rows < kv ? window + rows : kv;  // slots a sequence's rows can see
     const int64_t most = groups <= 296 ? 296 / groups : 1, few = most < AW_CLUSTER ? most : AW_CLUSTER;
     kps = ((kv + few - 1) / few + 63) / 64 * 64;
-    if (!one(kps) || kps > 256) {
+    // up to 384 keys a block (128 for wide heads or more vectors): one row over 6144 slots takes 15.8 us a call with one
+    // kernel and 20.0 with two (as a graph 14.7 and 12.6), over 8192 slots 17.2 and 19.6 (17.1 and 14.1); 5 rows over 4096
+    // slots 22.6 and 19.2
+    if (!one(kps) || kps > (D <= 128 && p.tile == 8 ? 384 : 128)) {
       const int64_t want = groups * 2 >= resident ? (seen + 767) / 768 : resident / groups;
       kps = ((seen + want - 1) / want + 63) / 64 * 64;
     }

@@ -341,13 +341,24 @@ int launch_evict_select(const EvictArgs& a, long long rows, int ranks, cudaStrea
                         dim3((unsigned)(rows * ranks)), dim3(THREADS), ranks, smem, st, a);
 }
 
+static long long evict_most(int64_t cap, int64_t budget) { return budget < cap - budget ? budget : cap - budget; }
+
+// Whether a row's moves are made by its own block. Up to 777 moves a row of 624 rows: 20.0 us so, 22.6 by a second kernel; up
+// to 2048 of 288 rows: 112 and 106 us. With fewer rows than SMs a row's moves are spread sooner.
+static bool evict_here(long long rows, long long cap, long long most) {
+  return cap <= EV_RUN && most <= (rows >= 148 ? EV_HERE : 128);
+}
+
+static bool evict_fits(int64_t layers, int64_t S, int64_t Hkv, int64_t cap) {
+  return layers >= 1 && S >= 1 && Hkv >= 1 && cap >= 1 && cap <= EV_CLUSTER * EV_RUN && layers < (1 << 27) &&
+         S < (1 << 27) && Hkv < (1 << 27) && layers * S < (1 << 27) && layers * S * Hkv < (1 << 27);
+}
+
 template <int BYTES>
 int launch_evict(EvictArgs& a, long long rows, cudaStream_t st) {
   int ranks = 1;
   while ((long long)ranks * EV_RUN < a.cap) ranks *= 2;
-  // up to 777 moves a row of 624 rows: 20.0 us moved by the rows' blocks, 22.6 by a second kernel; up to 2048 of 288 rows:
-  // 112 and 106 us. With fewer rows than SMs a row's moves are spread sooner
-  a.moves_here = ranks == 1 && a.most <= (rows >= 148 ? EV_HERE : 128);
+  a.moves_here = evict_here(rows, a.cap, a.most);
   a.lengths_here = a.lengths_out != a.lengths;
   const int chunks = 2 * (a.row_bytes / BYTES);
   a.chunk_shift = (chunks & (chunks - 1)) == 0 ? __builtin_ctz(chunks) : -1;
@@ -361,16 +372,14 @@ int launch_evict(EvictArgs& a, long long rows, cudaStream_t st) {
                 dim3((unsigned)rows, (unsigned)(blocks < 1024 ? blocks : 1024)), dim3(EV_MOVE_THREADS), 0, st, a);
 }
 
-static long long evict_most(int64_t cap, int64_t budget) { return budget < cap - budget ? budget : cap - budget; }
-
 }  // namespace im
 
 using namespace im;
 
 extern "C" size_t im_cache_evict_workspace_bytes(int64_t layers, int64_t S, int64_t Hkv, int64_t cap, int64_t budget) {
-  if (layers < 1 || S < 1 || Hkv < 1 || cap < 1 || budget < 0 || layers * S * Hkv >= (1ll << 27)) return 0;
-  const long long rows = layers * S * Hkv, most = evict_most(cap, budget);
-  return (size_t)(rows * 4 + (most > 0 ? 2 * rows * most * 4 : 0));
+  if (!evict_fits(layers, S, Hkv, cap) || budget < 0) return 0;
+  const long long rows = layers * S * Hkv, most = evict_most(cap, budget) > 0 ? evict_most(cap, budget) : 0;
+  return evict_here(rows, cap, most) ? 0 : (size_t)(rows * 4 + 2 * rows * most * 4);
 }
 
 extern "C" int im_cache_evict(void* k_cache, void* v_cache, int64_t layers, int64_t layer_bytes, int64_t pages,
@@ -390,10 +399,10 @@ extern "C" int im_cache_evict(void* k_cache, void* v_cache, int64_t layers, int6
   IM_REQUIRE(k_cache && v_cache && page_table && lengths && seen && weights && weights_out && slot_pos && pos_out &&
                  lengths_out,
              IM_INVALID, "im_cache_evict: null pointer");
-  const size_t need = im_cache_evict_workspace_bytes(layers, S, Hkv, cap, budget);
-  IM_REQUIRE(need > 0 && cap <= EV_CLUSTER * EV_RUN && row_bytes < (1 << 20), IM_UNSUPPORTED,
+  IM_REQUIRE(evict_fits(layers, S, Hkv, cap) && row_bytes < (1 << 20), IM_UNSUPPORTED,
              "im_cache_evict: rows of %lld slots (up to %d), or too many of them", (long long)cap, EV_CLUSTER * EV_RUN);
-  IM_REQUIRE(workspace && aligned(workspace, 16) && workspace_bytes >= need, IM_INVALID,
+  const size_t need = im_cache_evict_workspace_bytes(layers, S, Hkv, cap, budget);
+  IM_REQUIRE(need == 0 || (workspace && aligned(workspace, 16) && workspace_bytes >= need), IM_INVALID,
              "im_cache_evict: a workspace of %zu bytes needed, %zu given", need, workspace_bytes);
   const long long rows = layers * S * Hkv, most = evict_most(cap, budget);
   EvictArgs a = {};

@@ -857,11 +857,13 @@ def rope(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, la
     of a head's first 2 * len(inv_freq) values by positions * inv_freq[i], times factor; the rest is copied. Pairs are
     (i, i + half of them) or, "interleaved", (2i, 2i + 1). inverse turns back by the transpose: rope(dy, ..., inverse=True)
     is the gradient of x. `out` may be x; a new tensor by default."""
-    if not isinstance(x, torch.Tensor) or x.device.type != "cuda" or x.dtype not in _TYPES:
+    kind = _TYPES.get(x.dtype) if isinstance(x, torch.Tensor) and x.is_cuda else None
+    if kind is None:
         raise TypeError("x must be a bf16, float16 or float32 CUDA tensor")
-    if x.dim() != 3 or (x.numel() and x.stride(2) != 1 and x.shape[2] > 1):
-        raise ValueError(f"x must be [M, H, D] with contiguous heads, got {tuple(x.shape)}, strides {x.stride()}")
-    m, h, d = x.shape
+    shape, strides = x.shape, x.stride()
+    if len(shape) != 3 or (strides[2] != 1 and shape[2] > 1 and x.numel()):
+        raise ValueError(f"x must be [M, H, D] with contiguous heads, got {tuple(shape)}, strides {strides}")
+    m, h, d = shape
     device = x.device
     index = device.index
     wide = isinstance(positions, torch.Tensor) and positions.dtype is torch.int64
@@ -870,20 +872,20 @@ def rope(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, la
         raise ValueError(f"positions must be [{m}], got {tuple(positions.shape)}")
     rotary, lay, freq64 = _rope_table(inv_freq, layout, d, device, index)
     if out is None:
-        out = torch.empty((m, h, d), dtype=x.dtype, device=device)
+        out = x.new_empty((m, h, d))
+        rs, hs = h * d, d
     else:
-        if not isinstance(out, torch.Tensor) or out.dtype != x.dtype or out.device != device or out.shape != x.shape:
-            raise ValueError(f"out must be a {x.dtype} tensor {tuple(x.shape)} on {device}")
-        rs, hs = out.stride(0), out.stride(1)
+        if not isinstance(out, torch.Tensor) or out.dtype != x.dtype or out.device != device or out.shape != shape:
+            raise ValueError(f"out must be a {x.dtype} tensor {tuple(shape)} on {device}")
+        rs, hs, by_value = out.stride()
         by_row = (h < 2 or hs >= d) and (m < 2 or rs >= (h - 1) * hs + d)
         by_head = (m < 2 or rs >= d) and (h < 2 or hs >= (m - 1) * rs + d)
-        if out.numel() and ((d > 1 and out.stride(2) != 1) or not (by_row or by_head)):
+        if out.numel() and ((d > 1 and by_value != 1) or not (by_row or by_head)):
             raise ValueError(f"out must hold every head apart and contiguous, its strides are {out.stride()}")
         _disjoint_or_same(out, "out", x, "x")
-    if x.numel():
-        _launch(index, "im_rope", x.data_ptr(), x.stride(0), x.stride(1), positions.data_ptr(),
-                int(wide), inv_freq.data_ptr(), freq64, rotary, float(factor), lay, int(inverse), m, h, d,
-                _TYPES[x.dtype], out.data_ptr(), out.stride(0), out.stride(1))
+    if m and h and d:
+        _launch(index, "im_rope", x.data_ptr(), strides[0], strides[1], positions.data_ptr(), int(wide),
+                inv_freq.data_ptr(), freq64, rotary, float(factor), lay, int(inverse), m, h, d, kind, out.data_ptr(), rs, hs)
     return out
 
 
@@ -938,9 +940,10 @@ def rope_kv(qkv: torch.Tensor, inv_freq: torch.Tensor, row_pos: torch.Tensor, ro
     if not 0 <= m <= qkv.shape[0]:
         raise ValueError(f"{m} rows of {qkv.shape[0]}")
     rotary, lay, freq64 = _rope_table(inv_freq, layout, d, device, index)
-    _check_ints(row_pos, "row_pos", m, device, index)
-    _check_ints(row_slot, "row_slot", m, device, index)
-    _check_ints(row_seq, "row_seq", m, device, index)
+    for t, name in ((row_pos, "row_pos"), (row_slot, "row_slot"), (row_seq, "row_seq")):
+        if not (isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.get_device() == index and t.is_contiguous()
+                and t.dim() == 1 and t.numel() >= m):
+            _check_ints(t, name, m, device, index)
     seqs, max_pages, pages = _check_cache(k_cache, v_cache, page_table, hkv, d, dtype, device, index)
     cap = 0 if slot_pos is None else _check_slots(slot_pos, "slot_pos", torch.int32, (seqs, hkv), device, index)
     if q_out is None:
@@ -1076,19 +1079,19 @@ def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.
                 raise ValueError(f"{name} must be {tuple(like.shape)}, got {tuple(t.shape)}")
             _disjoint_or_same(t, name, like, like_name)
     if lengths_out is None:
-        lengths_out = torch.empty((s,), dtype=torch.int32, device=device)
+        lengths_out = lengths.new_empty((s,))
     if budget < 0 or recent < 0 or sinks < 0 or recent + sinks > budget:
         raise ValueError(f"{recent} recent and {sinks} first slots of a budget of {budget}")
     if not (layers and s and hkv and cap and d):
         return lengths_out.zero_()
     need = _evict_workspace(layers, s, hkv, cap, budget)
-    ws = torch.empty(max(need, 16), dtype=torch.uint8, device=device)
+    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None  # few moves a row need none
     size = k_cache.element_size()
     _launch(index, "im_cache_evict", k_cache.data_ptr(), v_cache.data_ptr(), layers, pages * hkv * PAGE_SLOTS * d * size,
             pages, page_table.data_ptr(), max_pages, lengths.data_ptr(), seen.data_ptr(), weights.data_ptr(),
             (weights if weights_out is None else weights_out).data_ptr(), slot_pos.data_ptr(),
             (slot_pos if pos_out is None else pos_out).data_ptr(), lengths_out.data_ptr(), s, hkv, cap, d * size,
-            budget, recent, sinks, ws.data_ptr(), need)
+            budget, recent, sinks, _ptr_or_none(ws), need)
     return lengths_out
 
 

@@ -115,10 +115,14 @@ def test_evict_refusals():
     assert evict(layers=0)[0] == evict(s=0)[0] == _lib.IM_OK
     for kw, word in (({"hkv": 0}, "sizes"), ({"cap": 0}, "sizes"), ({"budget": -1}, "sizes"), ({"sinks": -1}, "sizes"),
                      ({"recent": 40, "sinks": 11}, "budget"), ({"recent": 51}, "budget"), ({"ptr": None}, "null"),
-                     ({"ws": None}, "workspace"), ({"ws": 8}, "workspace"), ({"size": 16}, "workspace")):
+                     ({"ws": None, "cap": 900, "budget": 400}, "workspace"),
+                     ({"ws": 8, "cap": 20000}, "workspace"), ({"size": 16, "cap": 20000}, "workspace")):
         rc, msg = evict(**kw)
         assert rc == _lib.IM_INVALID and word in msg, (kw, msg)
     assert evict(cap=262145)[0] == _lib.IM_UNSUPPORTED and evict(layers=1 << 30)[0] == _lib.IM_UNSUPPORTED
+    lib = _lib.load()
+    assert lib.im_cache_evict_workspace_bytes(1, 2, 2, 100, 50) == 0  # a row's own block moves its slots
+    assert lib.im_cache_evict_workspace_bytes(1, 2, 2, 900, 400) > 0
     rc, msg = evict(recent=2**62, sinks=2**62, budget=2**62 + 2**61)  # a sum past 64 bits
     assert rc == _lib.IM_INVALID and "budget" in msg
 
