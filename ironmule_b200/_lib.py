@@ -158,9 +158,12 @@ def load(path: Path | None = None) -> ctypes.CDLL:
 
 def call(name: str, *args) -> None:
     """Call an int-returning entry point and raise on a non-zero status."""
-    lib = load()
-    status = getattr(lib, name)(*args)
+    check(name, getattr(load(), name)(*args))
+
+
+def check(name: str, status: int) -> None:
+    """Raise on an entry point's non-zero status, with its message."""
     if status != IM_OK:
-        message = (lib.im_last_error() or b"").decode(errors="replace")
+        message = (load().im_last_error() or b"").decode(errors="replace")
         cls = KernelUnsupported if status == IM_UNSUPPORTED else KernelError
         raise cls(name, status, message)

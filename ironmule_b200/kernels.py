@@ -775,10 +775,12 @@ PAGE_SLOTS = 16
 def _launch(index: int, name: str, *args) -> None:
     """_lib.call on a device's current stream (the entry point's last argument), with the device current."""
     if torch._C._cuda_getDevice() == index:
-        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+        status = getattr(_lib.load(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
-            _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+            status = getattr(_lib.load(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        _lib.check(name, status)
 
 
 def _need(t: torch.Tensor, name: str, dtype: torch.dtype, device: torch.device, index: int) -> None:
