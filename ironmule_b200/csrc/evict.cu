@@ -86,7 +86,7 @@ __device__ __forceinline__ int2 ev_before(int x, int* scratch) {
 
 // Up to 32 moves of one row by a warp: each lane has one move's slots; the warp then copies their rows together, BYTES a
 // lane, K's and V's chunks of a move side by side, four loads in flight a lane (with eight, at half the
-// warps an SM, a prompt's cut took 111 us in the place of 106).
+// warps an SM, a prompt's cut took 111 us in the place of 102).
 template <int BYTES>
 __device__ __forceinline__ void ev_move(const EvictArgs& a, long long row, const int* table, int moves, int to,
                                         int from) {
@@ -312,9 +312,10 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) evict_select_kernel(EvictArgs
   }
 }
 
-// The moves of all rows from the workspace, and the lengths, which nobody reads any more.
+// The moves of all rows from the workspace, and the lengths, which nobody reads any more. Five blocks an SM: with the
+// registers of six, a prompt's cut (288 rows, 2048 moves each) takes 106 us in the place of 102, with eight 114.
 template <int BYTES>
-__global__ void __launch_bounds__(EV_MOVE_THREADS, 6) evict_move_kernel(EvictArgs a) {
+__global__ void __launch_bounds__(EV_MOVE_THREADS, 5) evict_move_kernel(EvictArgs a) {
   pdl_wait();
   pdl_trigger();
   const long long row = blockIdx.x;
@@ -344,7 +345,7 @@ int launch_evict_select(const EvictArgs& a, long long rows, int ranks, cudaStrea
 static long long evict_most(int64_t cap, int64_t budget) { return budget < cap - budget ? budget : cap - budget; }
 
 // Whether a row's moves are made by its own block. Up to 777 moves a row of 624 rows: 20.0 us so, 22.6 by a second kernel; up
-// to 2048 of 288 rows: 112 and 106 us. With fewer rows than SMs a row's moves are spread sooner.
+// to 2048 of 288 rows: 112 and 102 us. With fewer rows than SMs a row's moves are spread sooner.
 static bool evict_here(long long rows, long long cap, long long most) {
   return cap <= EV_RUN && most <= (rows >= 148 ? EV_HERE : 128);
 }
@@ -356,16 +357,20 @@ static bool evict_fits(int64_t layers, int64_t S, int64_t Hkv, int64_t cap) {
 
 template <int BYTES>
 int launch_evict(EvictArgs& a, long long rows, cudaStream_t st) {
-  int ranks = 1;
-  while ((long long)ranks * EV_RUN < a.cap) ranks *= 2;
   a.moves_here = evict_here(rows, a.cap, a.most);
   a.lengths_here = a.lengths_out != a.lengths;
   const int chunks = 2 * (a.row_bytes / BYTES);
   a.chunk_shift = (chunks & (chunks - 1)) == 0 ? __builtin_ctz(chunks) : -1;
-  const int rc = a.cap <= 2048   ? launch_evict_select<256, 8, 4, BYTES>(a, rows, ranks, st)
-                 : a.cap <= 4096 ? launch_evict_select<512, 8, 2, BYTES>(a, rows, ranks, st)
-                 : a.cap <= 8192 ? launch_evict_select<512, 16, 2, BYTES>(a, rows, ranks, st)
-                                 : launch_evict_select<1024, 16, 1, BYTES>(a, rows, ranks, st);
+  // blocks a row: as many as its slots need, and more where that leaves SMs idle, down to 2048 slots each (16 rows of 10409
+  // slots: 21.5 us with one, 17.5 with four; 24 rows of 17203: 27.7 with two, 21.6 with four)
+  int ranks = 1;
+  while ((long long)ranks * EV_RUN < a.cap) ranks *= 2;
+  while (!a.moves_here && ranks < EV_CLUSTER && rows * ranks * 2 <= 148 && a.cap >= ranks * 2 * 2048) ranks *= 2;
+  const long long run = (a.cap + ranks - 1) / ranks;
+  const int rc = run <= 2048   ? launch_evict_select<256, 8, 4, BYTES>(a, rows, ranks, st)
+                 : run <= 4096 ? launch_evict_select<512, 8, 2, BYTES>(a, rows, ranks, st)
+                 : run <= 8192 ? launch_evict_select<512, 16, 2, BYTES>(a, rows, ranks, st)
+                               : launch_evict_select<1024, 16, 1, BYTES>(a, rows, ranks, st);
   if (rc != IM_OK || (a.moves_here && a.lengths_here)) return rc;
   const long long blocks = a.moves_here || a.most <= 0 ? 1 : (a.most + EV_MOVE_THREADS - 1) / EV_MOVE_THREADS;
   return launch("evict_move_kernel", evict_move_kernel<BYTES>,
@@ -399,8 +404,9 @@ extern "C" int im_cache_evict(void* k_cache, void* v_cache, int64_t layers, int6
   IM_REQUIRE(k_cache && v_cache && page_table && lengths && seen && weights && weights_out && slot_pos && pos_out &&
                  lengths_out,
              IM_INVALID, "im_cache_evict: null pointer");
-  IM_REQUIRE(evict_fits(layers, S, Hkv, cap) && row_bytes < (1 << 20), IM_UNSUPPORTED,
-             "im_cache_evict: rows of %lld slots (up to %d), or too many of them", (long long)cap, EV_CLUSTER * EV_RUN);
+  IM_REQUIRE(evict_fits(layers, S, Hkv, cap) && row_bytes <= (1 << 16), IM_UNSUPPORTED,
+             "im_cache_evict: rows of %lld slots (up to %d) of %lld bytes (up to 65536), or too many of them", (long long)cap,
+             EV_CLUSTER * EV_RUN, (long long)row_bytes);
   const size_t need = im_cache_evict_workspace_bytes(layers, S, Hkv, cap, budget);
   IM_REQUIRE(need == 0 || (workspace && aligned(workspace, 16) && workspace_bytes >= need), IM_INVALID,
              "im_cache_evict: a workspace of %zu bytes needed, %zu given", need, workspace_bytes);

@@ -56,7 +56,8 @@ def assert_turned(got, want, size, factor):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("layout", ["half", "interleaved"])
 @pytest.mark.parametrize("m,h,d,rotary", [(1, 1, 2, 2), (1, 32, 128, 128), (7, 3, 80, 32), (33, 5, 96, 96), (5, 2, 20, 6),
-                                          (3, 9, 17, 16), (200, 8, 256, 64), (2, 4, 64, 0)])
+                                          (3, 9, 17, 16), (200, 8, 256, 64), (2, 4, 64, 0),
+                                          (70, 6, 144, 72), (9, 4, 20, 8)])
 def test_rope_turns_rows(cuda, dtype, layout, m, h, d, rotary):
     g = gen(cuda, m * d + rotary)
     x = torch.randn((m, h, d), generator=g, device=cuda).to(dtype)
@@ -137,7 +138,7 @@ def kv_case(cuda, seed, m, hq, hkv, d, dtype, seqs=3, slots=70):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
-@pytest.mark.parametrize("m,hq,hkv,d,rotary,layout", [(1, 32, 8, 128, 128, "half"), (5, 4, 4, 64, 32, "interleaved"),
+@pytest.mark.parametrize("m,hq,hkv,d,rotary,layout", [(1, 32, 8, 128, 128, "half"), (5, 4, 4, 64, 32, "interleaved"), (60, 4, 2, 144, 72, "half"),
                                                       (40, 6, 2, 80, 80, "half"), (3, 2, 1, 18, 10, "half"),
                                                       (150, 8, 1, 256, 64, "interleaved")])
 def test_rope_kv_turns_and_writes_the_cache(cuda, dtype, m, hq, hkv, d, rotary, layout):
@@ -495,7 +496,8 @@ def test_evict_moves_any_type_and_head_size(cuda, dtype, d):
     evict_check(evict_case(cuda, d, [90, 33], 1, 2, d, dtype), 40, 10, 2)
 
 
-@pytest.mark.parametrize("length,budget", [(5000, 1250), (20000, 19990), (40000, 7), (70001, 30000)])
+@pytest.mark.parametrize("length,budget", [(5000, 1250), (20000, 19990), (40000, 7), (70001, 30000), (9000, 4500),
+                                           (262144, 100000)])
 def test_evict_long_rows(cuda, length, budget):
     evict_check(evict_case(cuda, budget, [length, 100], 1, 1, 8, torch.bfloat16), budget, min(7, budget), 0)
     evict_check(evict_case(cuda, budget, [length], 1, 1, 8, torch.bfloat16, kind="ties"), budget, min(7, budget), 0, False)
