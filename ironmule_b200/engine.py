@@ -1130,6 +1130,9 @@ class BoundedDecoder:
         if recent < 0 or sinks < 0 or recent + sinks > budget:
             raise ValueError(f"{recent} recent and {sinks} first slots of a budget of {budget}")
         self.model, self.budget, self.recent, self.sinks = model, budget, recent, sinks
+        # tokens of one forward: attention_weights takes 2048 query heads' rows of a kv head
+        self.step = min(model.max_rows, PREFILL_SEQ_ROWS, MAX_QGEMM_ROWS, model.max_ctx - budget,
+                        2048 // (model.lc.heads // model.lc.kv_heads))
         c, s, dev = model.lc, model.max_seqs, model.device
         self.weights = torch.zeros((c.layers, s, c.kv_heads, model.max_ctx), dtype=torch.float32, device=dev)
         self.slot_pos = torch.full((c.layers, s, c.kv_heads, model.max_ctx), -1, dtype=torch.int32, device=dev)
@@ -1140,6 +1143,8 @@ class BoundedDecoder:
 
     def start(self, seq: int = 0) -> None:
         """Forget the sequence of a slot."""
+        if not 0 <= seq < self.model.max_seqs:
+            raise ValueError(f"sequence {seq} of {self.model.max_seqs}")
         self._set(seq, 0, 0)
 
     def _set(self, seq: int, held: int, seen: int) -> None:
@@ -1159,7 +1164,9 @@ class BoundedDecoder:
         m = self.model
         if logits and not tokens.numel():
             raise ValueError("logits of no token")
-        step = min(m.max_rows, PREFILL_SEQ_ROWS, MAX_QGEMM_ROWS, m.max_ctx - self.budget)
+        if not 0 <= seq < m.max_seqs:
+            raise ValueError(f"sequence {seq} of {m.max_seqs}")
+        step = self.step
         last = tokens.numel() - 1 if logits else tokens.numel()  # a token whose logits are wanted goes by itself
         ends = [*range(step, last, step), last] if last else []
         out, at = None, 0

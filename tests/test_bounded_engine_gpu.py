@@ -84,5 +84,10 @@ def test_refusals(cuda):
     assert dec.feed(tokens(cuda, 0)) is None
     with pytest.raises(ValueError, match="no token"):
         dec.generate(tokens(cuda, 0), 3)
+    for seq in (-1, 1):
+        with pytest.raises(ValueError, match="sequence"):
+            dec.generate(tokens(cuda, 5), 3, seq=seq)
+        with pytest.raises(ValueError, match="sequence"):
+            dec.feed(tokens(cuda, 5), seq=seq)
     with pytest.raises(ValueError, match="sliding window"):
         engine.BoundedDecoder(model(cuda, 96, "tiny-gemma"), 32)
