@@ -477,8 +477,8 @@ size_t im_kq_workspace_bytes(int64_t K, int64_t B);
  * IM_BF16 or IM_F16 and head_dim D a multiple of 16 up to 256, which also writes every slot's attention weights,
  *   weights_out[s, h, j] = (j < f ? weights[s, h, j] : 0) + sum over the sequence's rows and the query heads of kv head h
  *                          of their softmax weight on slot j,  for j < min(largest row_slot + 1, max_kv_len, cap),
- * f being the sequence's first row's slot: slots that this call is the first to see start from zero. Other weights are
- * left alone. weights_out may be weights. Rows that see no slot (row_slot -1, say) get zeros and add nothing. Splits:
+ * f being the slot of the sequence's first row that has one (row_slot >= 0): slots that this call is the first to see start
+ * from zero. Other weights are left alone. weights_out may be weights, out may be q. Rows that see no slot (row_slot -1, say) get zeros and add nothing. Splits:
  * multiples of keys_per_split (a multiple of 64; 0: chosen by the sizes of the call); keep it fixed and a row's bits do
  * not depend on the launch. The workspace holds 4 bytes a (row, query head, slot). seq_rows is clamped to the M rows of q; rows beyond max_rows_per_seq are not computed. No two
  * sequences may name one table row. Workspace 256-byte aligned, nothing to initialise;
@@ -488,9 +488,9 @@ size_t im_kq_workspace_bytes(int64_t K, int64_t B);
  * position (slot_pos) is below `sinks` or at least seen[s] - recent, then the heaviest (weights; NaN lightest), lower
  * slots first among equals. The i-th kept slot behind the new end moves to the i-th dropped slot before it: K, V (a slot's
  * row_bytes of one head; any type), weight and position. weights_out and pos_out (which may be weights and slot_pos) get
- * the slots before the new end, lengths_out [S] (may be lengths) the new length, the same for every layer and head. weights and
+ * the slots before the new end, lengths_out [S] (may be lengths, not seen) the new length, the same for every layer and head. weights and
  * slot_pos are [layers][S][Hkv][cap], the caches `layers` times [pages][Hkv][16][row_bytes], layer_bytes apart; n is at
- * most min(cap, 16 max_pages), cap at most 262144. Sequences must not share the pages of a cache that is cut. sinks + recent <= budget.
+ * most min(cap, 16 max_pages), cap at most 262144 and row_bytes 65536. Sequences must not share the pages of a cache that is cut. sinks + recent <= budget.
  * Workspace 16-byte aligned, nothing to initialise; none (0 bytes) where few slots of a row can move.
  *
  * im_verify_sampled: keeps or refuses drafted tokens by the target's probabilities and given random numbers. target

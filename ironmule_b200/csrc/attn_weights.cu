@@ -97,6 +97,13 @@ __device__ __forceinline__ void aw_span(const AwArgs& a, AwSeq& s) {
   s.lo = a.window > 0 && low != 0x7fffffff ? max(0, low - a.window + 1) : 0;
 }
 
+// The slot of the first row that has one: weights from it on start from zero.
+__device__ __forceinline__ int aw_first(const AwArgs& a, const AwSeq& s) {
+  int first = a.row_slot[s.row0];
+  for (int r = 1; first < 0 && r < s.rows; r++) first = a.row_slot[s.row0 + r];  // padding before a sequence's rows
+  return first;
+}
+
 // 2^x to two ulps; what would be subnormal is 0.
 __device__ __forceinline__ float aw_exp2(float x) {
   float y;
@@ -575,7 +582,7 @@ __global__ void __launch_bounds__(AwShape<DP, NT>::WARPS * 32, NT > 2 ? 2 : DP >
       cg::cluster_group cluster = cg::this_cluster();
       const int ranks = gridDim.x;
       // this block's slots and their weights so far, on their way while the blocks meet
-      const int n = (int)min((long long)min(split * a.kps + a.kps, q.n), a.cap), first = a.row_slot[q.row0];
+      const int n = (int)min((long long)min(split * a.kps + a.kps, q.n), a.cap), first = aw_first(a, q);
       const long long base = (q.slot * a.hkv + h) * a.cap;
       constexpr int MOST = 768 / (WARPS * 32);  // slots of a thread: AW_HELD / 4 / 8 of a block
       float old[MOST];
@@ -740,7 +747,7 @@ __global__ void __launch_bounds__(AW_FIN_THREADS, 4) aw_finish_kernel(AwArgs a) 
   int j0 = (blockIdx.x - a.joins) * quads * 4;
   if (j0 >= n) return;  // no wait: nothing is read or written
   const int step = (gridDim.x - a.joins) * quads * 4;
-  const int first = a.row_slot[q.row0];
+  const int first = aw_first(a, q);
   const bool aligned4 = a.cap % 4 == 0 && a.wide_weights;
   const float* scores = a.scores + head * a.vecs * a.kv_pad;
   const long long base = (q.slot * a.hkv + h) * a.cap;
@@ -979,6 +986,9 @@ extern "C" int im_attention_weights(const void* q, const void* k_cache, const vo
              "im_attention_weights: null pointer");
   IM_REQUIRE(aligned(q, 16) && aligned(k_cache, 16) && aligned(v_cache, 16) && aligned(out, 16), IM_INVALID,
              "im_attention_weights: q, the caches and out must be 16-byte aligned");
+  IM_REQUIRE(aligned(weights, 4) && aligned(weights_out, 4) && aligned(page_table, 4) && aligned(seq_rows, 4) &&
+                 aligned(seq_slot, 4) && aligned(row_slot, 4),
+             IM_INVALID, "im_attention_weights: misaligned pointer");
   IM_REQUIRE(M < (1ll << 31) && B < 65536 && Hkv <= 4096 && max_rows_per_seq <= 4096 && Hq / Hkv <= 256 &&
                  max_rows_per_seq * (Hq / Hkv) <= 2048 && max_kv_len < (1ll << 30) && window < (1ll << 30),
              IM_UNSUPPORTED, "im_attention_weights: too large");

@@ -404,12 +404,16 @@ extern "C" int im_cache_evict(void* k_cache, void* v_cache, int64_t layers, int6
   IM_REQUIRE(k_cache && v_cache && page_table && lengths && seen && weights && weights_out && slot_pos && pos_out &&
                  lengths_out,
              IM_INVALID, "im_cache_evict: null pointer");
+  IM_REQUIRE(aligned(page_table, 4) && aligned(lengths, 4) && aligned(seen, 4) && aligned(weights, 4) &&
+                 aligned(weights_out, 4) && aligned(slot_pos, 4) && aligned(pos_out, 4) && aligned(lengths_out, 4),
+             IM_INVALID, "im_cache_evict: misaligned pointer");
   IM_REQUIRE(evict_fits(layers, S, Hkv, cap) && row_bytes <= (1 << 16), IM_UNSUPPORTED,
              "im_cache_evict: rows of %lld slots (up to %d) of %lld bytes (up to 65536), or too many of them", (long long)cap,
              EV_CLUSTER * EV_RUN, (long long)row_bytes);
   const size_t need = im_cache_evict_workspace_bytes(layers, S, Hkv, cap, budget);
   IM_REQUIRE(need == 0 || (workspace && aligned(workspace, 16) && workspace_bytes >= need), IM_INVALID,
              "im_cache_evict: a workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+  IM_REQUIRE(lengths_out != seen, IM_INVALID, "im_cache_evict: lengths_out is seen");
   const long long rows = layers * S * Hkv, most = evict_most(cap, budget);
   EvictArgs a = {};
   a.k = (char*)k_cache, a.v = (char*)v_cache, a.layer_bytes = layer_bytes, a.pages = pages;

@@ -978,7 +978,8 @@ def attention_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     """Paged attention of new rows, q [M, Hq, D] -> out [M, Hq, D] (bf16 or float16, D a multiple of 16 up to 256), that
     adds up each slot's attention weight: weights (float32 [sequences, Hkv, cap], the rows of the page table) becomes, in
     place or in weights_out, weights + the softmax weights that the sequence's rows and the kv head's query heads put on
-    the slot, for the slots up to the last row's; from the first row's slot on it starts from zero. The other arguments
+    the slot, for the slots up to the last row's; from the slot of the first row that has one on it starts from zero. Rows
+    without a slot (-1) get zeros and add nothing. `out` may be q. The other arguments
     are `attention`'s, keys_per_split 0 meaning that the call's sizes choose it."""
     dtype = torch.float16 if isinstance(q, torch.Tensor) and q.dtype is torch.float16 else torch.bfloat16
     if not (isinstance(q, torch.Tensor) and q.is_cuda and q.dtype is dtype and q.is_contiguous()):
@@ -1016,6 +1017,7 @@ def attention_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
         _need(out, "out", dtype, device, index)
         if out.numel() < m * hq * d:
             raise ValueError(f"out needs {m * hq * d} elements")
+        _disjoint_or_same(out, "out", q, "q")
     if not (0 <= max_rows_per_seq and 0 <= max_kv_len and 0 <= window and 0 <= keys_per_split):
         raise ValueError("max_rows_per_seq, max_kv_len, window and keys_per_split are not negative")
     if b == 0 or m == 0 or max_rows_per_seq == 0:
@@ -1082,6 +1084,10 @@ def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.
             _disjoint_or_same(t, name, like, like_name)
     if lengths_out is None:
         lengths_out = lengths.new_empty((s,))
+    else:
+        _disjoint_or_same(lengths_out, "lengths_out", lengths, "lengths")
+        if s and lengths_out.data_ptr() < seen.data_ptr() + 4 * s and seen.data_ptr() < lengths_out.data_ptr() + 4 * s:
+            raise ValueError("lengths_out overlaps seen")
     if budget < 0 or recent < 0 or sinks < 0 or recent + sinks > budget:
         raise ValueError(f"{recent} recent and {sinks} first slots of a budget of {budget}")
     if not (layers and s and hkv and cap and d):

@@ -195,7 +195,7 @@ def attend_plain(q, k, v, table, seq_rows, row_slot, weights, scale, window=0, m
         n = min(max(slots[r] for r in rows) + 1, max_kv, table.shape[1] * 16)
         if n <= 0:
             continue
-        first, cap = slots[rows[0]], after.shape[-1]
+        first, cap = next(slots[r] for r in rows if slots[r] >= 0), after.shape[-1]
         kept = min(n, cap)
         after[s, :, max(0, min(first, kept)):kept] = 0
         pages = table[s, :-(-n // 16)].long()
@@ -354,6 +354,31 @@ def test_attention_weights_masks(cuda):
     slot[2] = 10**6  # a slot behind the table sees what the table has
     attend_check((q, k.nan_to_num(0.5), v.nan_to_num(0.5, 0.5, 0.5), table, bounds, slot, weights), in_place=True,
                  max_kv=2 * 10**6)
+
+
+@pytest.mark.parametrize("lengths,rows", [([90, 40], [4, 3]), ([5000, 900], [4, 3]), ([300], [9])])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_attention_weights_of_rows_padded_in_front(cuda, lengths, rows, in_place):
+    """Rows without a slot before a sequence's own: what the earlier slots have gathered stays."""
+    q, k, v, table, bounds, slot, weights = attend_case(cuda, 6, lengths, rows, 4, 2, 64, torch.bfloat16)
+    for b in range(len(rows)):
+        slot[int(bounds[b]):int(bounds[b]) + rows[b] // 2] = -1
+    out, after = attend_check((q, k, v, table, bounds, slot, weights), in_place=in_place)
+    lone = [int(bounds[b]) + i for b in range(len(rows)) for i in range(rows[b] // 2)]
+    assert not bool(out[lone].any())
+    for b, n in enumerate(lengths):
+        assert bool((after[b, :, :n - rows[b]] >= weights[b, :, :n - rows[b]]).all())
+
+
+def test_attention_weights_over_its_own_queries(cuda):
+    for length in (100, 5000):
+        case = attend_case(cuda, 7, [length, 33], [3, 2], 8, 2, 128, torch.bfloat16)
+        q, k, v, table, bounds, slot, weights = case
+        kw = {"max_rows_per_seq": 3, "max_kv_len": length, "scale": 0.1}
+        want = kernels.attention_weights(q, k, v, table, bounds, slot, weights.clone(), **kw)
+        own = q.clone()
+        assert kernels.attention_weights(own, k, v, table, bounds, slot, weights.clone(), out=own, **kw) is own
+        assert torch.equal(own, want)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
@@ -909,6 +934,9 @@ def test_refusals_of_the_wrappers(cuda):
     refuses(kernels.attention_weights, q, k, v, table, bounds, slot, weights[:, :1].contiguous(), match="weights", **kw)
     refuses(kernels.attention_weights, q, k, v, table, bounds, slot, weights, weights_out=weights[:1], match="weights_out",
             **kw)
+    twice = torch.zeros(3 * 4 * 64, dtype=torch.bfloat16, device=cuda)
+    refuses(kernels.attention_weights, twice[:512].view(2, 4, 64), k, v, table, bounds, slot, weights, match="overlaps",
+            out=twice[256:].view(2, 4, 64), **kw)
     none = torch.zeros((2, 2, 0), device=cuda)  # no slot's weight is kept
     out = kernels.attention_weights(q, k, v, table, bounds, slot, none, **kw)
     assert torch.equal(out, kernels.attention_weights(q, k, v, table, bounds, slot, weights.clone(), **kw))
@@ -924,6 +952,10 @@ def test_refusals_of_the_wrappers(cuda):
     refuses(kernels.cache_evict, k5, v5, table, lengths[:1], seen, weights, spos, budget=10, match="lengths")
     refuses(kernels.cache_evict, k5, v5, table, lengths, seen, weights, spos[..., :50].contiguous(), budget=10,
             match="slot_pos")
+    both = torch.zeros(4, dtype=torch.int32, device=cuda)
+    for out, what in ((seen, "seen"), (both[1:3], "seen"), (both[:2], "lengths")):
+        refuses(kernels.cache_evict, k5, v5, table, lengths if what == "seen" else both[1:3],
+                seen if out is seen else both[2:], weights, spos, budget=10, lengths_out=out, match=what)
     refuses(kernels.cache_evict, k5, v5.half(), table, lengths, seen, weights, spos, budget=10, error=TypeError)
     p, q, drafts, u = verify_case(cuda, 9, 2, 3, 50, torch.float32)
     refuses(kernels.verify_sampled, p[:, :3], q, drafts, u, match="target_probs")
