@@ -7,9 +7,9 @@
 // Bound: HBM, K and V of every visible slot read once (2 * 2 D bytes a slot and kv head).
 //
 // First kernel (aw_split_kernel): a block takes one split of a (sequence, kv head) and a tile of its (row, query head)
-// vectors. Its four warps (two of wide heads) take the split's pages in turn, each with a ring of pages of its own in shared memory
-// (asynchronous copies, no barrier between warps), a running maximum and sum and a D x vectors accumulator in registers;
-// they are joined once at the split's end. The products are transposed, so that the few vectors are the warp MMA's n = 8
+// vectors. Its four warps (two, or two pairs, of wide heads) take the split's pages in turn, each with a ring of pages of its own in
+// shared memory (asynchronous copies, no barrier between warps), a running maximum and sum and a D x vectors accumulator in
+// registers; they are joined once at the split's end. The products are transposed, so that the few vectors are the warp MMA's n = 8
 // (one or two of them) and slots and head values its m = 16: S^T = K Q^T, out^T = V^T P^T. With Q as the m = 16 rows, half
 // and more of the products would be of rows that are not there, and at 16 cycles each they would take half of a
 // page's time; tcgen05's tiles of 64 rows and more would add more of that. Scores go to the workspace in float32 (4 bytes
@@ -215,31 +215,33 @@ __device__ __forceinline__ void aw_store(const AwArgs& a, const AwSeq& q, int h,
   *(uint2*)((T*)a.out + (row * a.hq + h * group + v % group) * a.d + c) = *(const uint2*)r;
 }
 
-// DP: head_dim rounded up to what is built; columns from d on are zeros in shared memory. NT: tiles of 8 vectors a block.
-template <int DP, int NT>
+// DP: head_dim rounded up to what is built; columns from d on are zeros in shared memory. NT: tiles of 8 vectors a warp.
+// WPP: warps that work on a page, each with its own vectors.
+template <int DP, int NT, int WPP>
 struct AwShape {
-  static constexpr int WARPS = DP > 128 ? 2 : 4;
+  static constexpr int TILE = NT * WPP * 8;   // vectors of a block
+  static constexpr int RINGS = DP > 128 ? 2 : 4;
+  static constexpr int WARPS = RINGS * WPP;
   static constexpr int PITCH = DP * 2 + 16;   // an odd number of 16-byte steps: ldmatrix without bank conflicts
   static constexpr int PAGE = 16 * PITCH;     // one page's K or V
   static constexpr int STAGES = DP > 64 ? 2 : 3;
   static constexpr int RING = STAGES * 2 * PAGE;
   static constexpr int JOIN = DP + 4;         // floats of a vector where the warps' accumulators are joined
-  static constexpr bool Q_REGS = NT * DP <= 384;
-  static_assert(Q_REGS || NT == 2, "Q in shared memory is read two tiles at a time");
-  static constexpr int Q_BYTES = Q_REGS ? 0 : NT * 8 * PITCH;
-  static constexpr int SMEM = WARPS * RING + Q_BYTES;
-  static constexpr int SMEM_ONE = SMEM + NT * 8 * JOIN * 4 + AW_HELD + NT * 8 * 16;  // with accumulators and scores, padded
-  static_assert(NT * 8 * JOIN * 4 <= RING, "a warp's ring takes its accumulator at the end");
+  static_assert(NT * DP <= 384, "Q stays in registers");
+  static constexpr int SMEM = RINGS * RING;
+  static constexpr int SMEM_ONE = SMEM + TILE * JOIN * 4 + AW_HELD + TILE * 16;  // with accumulators and scores, padded
+  static_assert(TILE * JOIN * 4 <= RING, "a ring takes its accumulator at the end");
+  static constexpr int BLOCKS = WPP > 1 ? (DP > 128 ? 3 : 2) : NT > 2 ? 2 : DP > 64 ? 3 : 4;  // on an SM
 };
 
-template <typename T, int DP, int NT, bool ONE>
-__global__ void __launch_bounds__(AwShape<DP, NT>::WARPS * 32, NT > 2 ? 2 : DP > 64 ? 3 : 4)
+template <typename T, int DP, int NT, int WPP, bool ONE>
+__global__ void __launch_bounds__(AwShape<DP, NT, WPP>::WARPS * 32, AwShape<DP, NT, WPP>::BLOCKS)
     aw_split_kernel(AwArgs a) {
-  using S = AwShape<DP, NT>;
+  using S = AwShape<DP, NT, WPP>;
   using Ty = AwType<T>;
-  constexpr int TILE = NT * 8, WARPS = S::WARPS;
+  constexpr int TILE = S::TILE, WARPS = S::WARPS, RINGS = S::RINGS;
   extern __shared__ __align__(128) char smem[];
-  __shared__ float s_m[WARPS][TILE], s_l[WARPS][TILE];
+  __shared__ float s_m[RINGS][TILE], s_l[RINGS][TILE];
   // ONE: this block's maxima and sums, the whole cluster's, the final ones
   __shared__ float2 s_stat[ONE ? TILE : 1], s_all[ONE ? AW_CLUSTER : 1][ONE ? TILE : 1], s_total[ONE ? TILE : 1];
   float* s_out = (float*)(smem + S::SMEM);  // ONE: [TILE][JOIN]
@@ -250,16 +252,17 @@ __global__ void __launch_bounds__(AwShape<DP, NT>::WARPS * 32, NT > 2 ? 2 : DP >
   int split = blockIdx.x;  // with a window: counted from the first that a row sees
   const int h = blockIdx.y / a.tiles, tile = blockIdx.y % a.tiles, b = blockIdx.z;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  const int worker = warp / WPP, part = warp % WPP;  // which pages, which vectors
   constexpr int STEPS = DP / 16, CP = DP / 8;
   AwSeq q = aw_seq(a, b);
   const int group = a.hq / a.hkv;
   const int vecs = q.rows * group;  // live ones
   if (tile * TILE >= vecs || (!ONE && q.slot < 0)) return;  // the whole cluster
   const int* table = a.page_table + max(q.slot, 0ll) * a.max_pages;
-  // pages of this warp: those whose number is warp mod WARPS, so that a slot's place does not depend on the call. The page
+  // pages of this warp: those whose number is its worker's mod RINGS, so that a slot's place does not depend on the call. The page
   // numbers are fetched a round ahead of the copies that need them, the first before it is known how many there are
   int next = split * a.kps / 16;
-  next += (warp - next) & (WARPS - 1);
+  next += (worker - next) & (RINGS - 1);
   int entry = a.window == 0 && q.slot >= 0 && next < a.max_pages ? table[next] : 0;
   // this lane's vectors of each tile of 8: 2 (lane mod 4) and the next (accumulators), lane / 4 (Q as an operand)
   int last[NT][2], from[NT][2];
@@ -268,41 +271,29 @@ __global__ void __launch_bounds__(AwShape<DP, NT>::WARPS * 32, NT > 2 ? 2 : DP >
   for (int nt = 0; nt < NT; nt++)
 #pragma unroll
     for (int e = 0; e < 2; e++) {
-      const int vec = tile * TILE + nt * 8 + lane % 4 * 2 + e;
+      const int vec = tile * TILE + (part * NT + nt) * 8 + lane % 4 * 2 + e;
       live[nt][e] = vec < vecs;
       last[nt][e] = live[nt][e] ? a.row_slot[q.row0 + vec / group] : -1;
     }
-  uint32_t qf[S::Q_REGS ? STEPS : 1][NT][2];
-  const char* q_smem = smem + WARPS * S::RING;
-  if (S::Q_REGS) {
+  uint32_t qf[STEPS][NT][2];
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-      const int vec = tile * TILE + nt * 8 + lane / 4;
-      const char* p = a.q + (((long long)q.row0 + vec / group) * a.hq + h * group + vec % group) * a.d * 2;
+  for (int nt = 0; nt < NT; nt++) {
+    const int vec = tile * TILE + (part * NT + nt) * 8 + lane / 4;
+    const char* p = a.q + (((long long)q.row0 + vec / group) * a.hq + h * group + vec % group) * a.d * 2;
 #pragma unroll
-      for (int st = 0; st < STEPS; st++)
+    for (int st = 0; st < STEPS; st++)
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-          const int c = st * 16 + i * 8 + lane % 4 * 2;
-          qf[S::Q_REGS ? st : 0][nt][i] = vec < vecs && c < a.d ? *(const uint32_t*)(p + c * 2) : 0u;
-        }
-    }
-  } else {
-    for (int c = t; c < TILE * CP; c += WARPS * 32) {
-      const int vec = tile * TILE + c / CP, col = c % CP * 8;
-      uint4 x = make_uint4(0, 0, 0, 0);
-      if (vec < vecs && col < a.d)
-        x = *(const uint4*)(a.q + (((long long)(q.row0 + vec / group) * a.hq + h * group + vec % group) * a.d + col) * 2);
-      *(uint4*)(smem + WARPS * S::RING + c / CP * S::PITCH + col * 2) = x;
-    }
+      for (int i = 0; i < 2; i++) {
+        const int c = st * 16 + i * 8 + lane % 4 * 2;
+        qf[st][nt][i] = vec < vecs && c < a.d ? *(const uint32_t*)(p + c * 2) : 0u;
+      }
   }
   aw_span(a, q);
   if (a.window > 0) split += q.lo / 16 * 16 / a.kps;
-  if (!S::Q_REGS) __syncthreads();
-  char* ring = smem + warp * S::RING;
+  char* ring = smem + worker * S::RING;
   const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
   if (a.d < DP) {  // columns behind the head: zeros, once
-    for (int c = lane; c < S::STAGES * 2 * 16 * CP; c += 32)
+    for (int c = lane + 32 * part; c < S::STAGES * 2 * 16 * CP; c += 32 * WPP)
       if (c % CP * 8 >= a.d) *(uint4*)(ring + c / CP * S::PITCH + c % CP * 16) = make_uint4(0, 0, 0, 0);
   }
   const uint64_t policy = aw_policy(a.tiles == 1);
@@ -316,12 +307,17 @@ __global__ void __launch_bounds__(AwShape<DP, NT>::WARPS * 32, NT > 2 ? 2 : DP >
     }
   all_last = __reduce_min_sync(0xffffffffu, all_last), all_from = __reduce_max_sync(0xffffffffu, all_from);
   const float scale2 = a.scale * AW_LOG2E;
-  float* scores = a.scores + (((long long)b * a.hkv + h) * a.vecs + tile * TILE + lane % 4 * 2) * a.kv_pad + lane / 4;
+  float* scores = a.scores + (((long long)b * a.hkv + h) * a.vecs + tile * TILE + part * NT * 8 + lane % 4 * 2) * a.kv_pad + lane / 4;
   // ldmatrix: lane i gives row i % 8 of matrix i / 8
   const int lr = lane & 7, lm = lane >> 3;
   const uint32_t k_off = (lr + (lm & 1) * 8) * S::PITCH + (lm >> 1) * 16;  // slots 0-7, 8-15, then the next 8 values
   const uint32_t v_off = (lr + (lm >> 1) * 8) * S::PITCH + (lm & 1) * 16;  // turned: values 0-7, 8-15, then slots 8-15
-  const uint32_t q_off = (uint32_t)__cvta_generic_to_shared(q_smem) + (lr + (lm >> 1) * 8) * S::PITCH + (lm & 1) * 16;
+
+  // the warps of a page: what they copied is there for all, and what they read may be overwritten
+  auto meet = [&]() {
+    if (WPP == 1) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(worker + 1), "n"(WPP * 32) : "memory");
+  };
 
   // one split, unless rows with a window lie so far apart that there are more than blocks
   for (;; split += gridDim.x) {
@@ -329,7 +325,7 @@ __global__ void __launch_bounds__(AwShape<DP, NT>::WARPS * 32, NT > 2 ? 2 : DP >
     if (!ONE && k0 >= k1) return;  // the whole block
     const int p0 = k0 / 16, p1 = k0 < k1 ? (k1 + 15) / 16 : p0;
     if (a.window > 0 || split != (int)blockIdx.x) {
-      next = p0 + ((warp - p0) & (WARPS - 1));
+      next = p0 + ((worker - p0) & (RINGS - 1));
       entry = next < p1 ? table[next] : 0;
     }
     int page = next;
@@ -345,14 +341,14 @@ __global__ void __launch_bounds__(AwShape<DP, NT>::WARPS * 32, NT > 2 ? 2 : DP >
           const char* k = a.k + at + lane * 16;
           const char* v = a.v + at + lane * 16;
 #pragma unroll
-          for (int i = 0; i < 16 * CP / 32; i++) {
+          for (int i = part; i < 16 * CP / 32; i += WPP) {
             const int c = lane + 32 * i;
             aw_copy16(dst + c / CP * S::PITCH + c % CP * 16, k + i * 512, true, policy);
             aw_copy16(dst + S::PAGE + c / CP * S::PITCH + c % CP * 16, v + i * 512, true, policy);
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < 16 * CP / 32; i++) {
+          for (int i = part; i < 16 * CP / 32; i += WPP) {
             const int c = lane + 32 * i, row = c / CP, col = c % CP;
             if (col * 8 < a.d) {
               const bool in = row < rows;
@@ -364,10 +360,10 @@ __global__ void __launch_bounds__(AwShape<DP, NT>::WARPS * 32, NT > 2 ? 2 : DP >
         }
       }
       aw_commit();
-      next += WARPS;
+      next += RINGS;
       entry = next < p1 ? table[next] : 0;
     };
-    __syncwarp();
+    meet();
 #pragma unroll
     for (int i = 0; i < S::STAGES - 1; i++) fetch(i);
 
@@ -379,9 +375,9 @@ __global__ void __launch_bounds__(AwShape<DP, NT>::WARPS * 32, NT > 2 ? 2 : DP >
     float m[NT][2], l[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) m[nt][0] = m[nt][1] = -INFINITY, l[nt][0] = l[nt][1] = 0.f;
-    for (int stage = 0; page < p1; page += WARPS) {
+    for (int stage = 0; page < p1; page += RINGS) {
       aw_wait<S::STAGES - 2>();
-      __syncwarp();
+      meet();
       const bool ok = pages_ok >> (S::STAGES - 2) & 1;
       const int ahead = stage + S::STAGES - 1;
       fetch(ahead >= S::STAGES ? ahead - S::STAGES : ahead);
@@ -398,13 +394,9 @@ __global__ void __launch_bounds__(AwShape<DP, NT>::WARPS * 32, NT > 2 ? 2 : DP >
       for (int st = 0; st < STEPS; st++) {
         uint32_t ka[4];
         aw_ldsm(ka, kp + k_off + st * 32);
-        uint32_t qb[4];
-        if (!S::Q_REGS) aw_ldsm(qb, q_off + st * 32);  // of two tiles
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-          float* to = st & 1 ? s_odd[nt] : s[nt];
-          if (S::Q_REGS) Ty::mma(to, ka, qf[S::Q_REGS ? st : 0][nt][0], qf[S::Q_REGS ? st : 0][nt][1]);
-          else Ty::mma(to, ka, qb[2 * nt], qb[2 * nt + 1]);
+          Ty::mma(st & 1 ? s_odd[nt] : s[nt], ka, qf[st][nt][0], qf[st][nt][1]);
         }
       }
       const int j0 = page * 16 + lane / 4;  // this lane's slots: j0, j0 + 8
@@ -466,7 +458,7 @@ __global__ void __launch_bounds__(AwShape<DP, NT>::WARPS * 32, NT > 2 ? 2 : DP >
 #pragma unroll
         for (int e = 0; e < 2; e++)
           if (live[nt][e]) {
-            float* to = ONE ? s_scores + (nt * 8 + lane % 4 * 2 + e) * held + page * 16 - split * a.kps + lane / 4
+            float* to = ONE ? s_scores + ((part * NT + nt) * 8 + lane % 4 * 2 + e) * held + page * 16 - split * a.kps + lane / 4
                             : scores + (long long)(nt * 8 + e) * a.kv_pad + page * 16;
             to[0] = s[nt][e];
             to[8] = s[nt][e + 2];
@@ -536,17 +528,18 @@ __global__ void __launch_bounds__(AwShape<DP, NT>::WARPS * 32, NT > 2 ? 2 : DP >
       for (int e = 0; e < 2; e++) {
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], x);
-        if (lane < 4) s_m[warp][nt * 8 + lane * 2 + e] = m[nt][e], s_l[warp][nt * 8 + lane * 2 + e] = l[nt][e];
+        const int row = (part * NT + nt) * 8 + lane * 2 + e;
+        if (lane < 4) s_m[worker][row] = m[nt][e], s_l[worker][row] = l[nt][e];
       }
     __syncthreads();  // every warp is done with its ring, which now takes its accumulator
 #pragma unroll
     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
       for (int e = 0; e < 2; e++) {
-        const int row = nt * 8 + lane % 4 * 2 + e;
+        const int row = (part * NT + nt) * 8 + lane % 4 * 2 + e;
         float top = s_m[0][row];
 #pragma unroll
-        for (int w = 1; w < WARPS; w++) top = fmaxf(top, s_m[w][row]);
+        for (int w = 1; w < RINGS; w++) top = fmaxf(top, s_m[w][row]);
         const float f = m[nt][e] == -INFINITY ? 0.f : aw_exp2(m[nt][e] - top);
         float* to = (float*)ring + row * S::JOIN + lane / 4;
         if (live[nt][e]) {
@@ -561,7 +554,7 @@ __global__ void __launch_bounds__(AwShape<DP, NT>::WARPS * 32, NT > 2 ? 2 : DP >
       for (int c = lane * 4; c < a.d; c += 128) {
         float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int w = 0; w < WARPS; w++) {
+        for (int w = 0; w < RINGS; w++) {
           const float4 y = *(const float4*)(smem + w * S::RING + (row * S::JOIN + c) * 4);
           x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
         }
@@ -571,10 +564,10 @@ __global__ void __launch_bounds__(AwShape<DP, NT>::WARPS * 32, NT > 2 ? 2 : DP >
     if (t < count) {
       float mm = s_m[0][t];
 #pragma unroll
-      for (int w = 1; w < WARPS; w++) mm = fmaxf(mm, s_m[w][t]);
+      for (int w = 1; w < RINGS; w++) mm = fmaxf(mm, s_m[w][t]);
       float sum = 0.f;
 #pragma unroll
-      for (int w = 0; w < WARPS; w++) sum += s_m[w][t] == -INFINITY ? 0.f : aw_exp2(s_m[w][t] - mm) * s_l[w][t];
+      for (int w = 0; w < RINGS; w++) sum += s_m[w][t] == -INFINITY ? 0.f : aw_exp2(s_m[w][t] - mm) * s_l[w][t];
       if (ONE) s_stat[t] = make_float2(mm, sum);
       else a.stats[at + t] = make_float2(mm, sum);
     }
@@ -906,27 +899,31 @@ static AwPlan aw_plan(int64_t B, int64_t rows, int64_t Hq, int64_t Hkv, int64_t 
   return p;
 }
 
-template <typename T, int DP, int NT>
+template <typename T, int DP, int NT, int WPP>
 int launch_split(const AwArgs& a, bool one, dim3 grid, cudaStream_t st) {
-  constexpr int threads = AwShape<DP, NT>::WARPS * 32;
+  constexpr int threads = AwShape<DP, NT, WPP>::WARPS * 32;
   if (one) {
-    const int rc = configure<aw_split_kernel<T, DP, NT, true>>("aw_split_kernel", AwShape<DP, NT>::SMEM_ONE, true);
+    const int rc = configure<aw_split_kernel<T, DP, NT, WPP, true>>("aw_split_kernel", AwShape<DP, NT, WPP>::SMEM_ONE, true);
     if (rc != IM_OK) return rc;
-    return launch_cluster("aw_split_kernel", aw_split_kernel<T, DP, NT, true>, grid, dim3(threads), (int)grid.x,
-                          AwShape<DP, NT>::SMEM + NT * 8 * (AwShape<DP, NT>::JOIN + a.kps + 4) * 4, st, a);
+    return launch_cluster("aw_split_kernel", aw_split_kernel<T, DP, NT, WPP, true>, grid, dim3(threads), (int)grid.x,
+                          AwShape<DP, NT, WPP>::SMEM + AwShape<DP, NT, WPP>::TILE * (AwShape<DP, NT, WPP>::JOIN + a.kps + 4) * 4, st, a);
   }
-  constexpr int smem = AwShape<DP, NT>::SMEM;
-  const int rc = configure<aw_split_kernel<T, DP, NT, false>>("aw_split_kernel", smem, false);
+  constexpr int smem = AwShape<DP, NT, WPP>::SMEM;
+  const int rc = configure<aw_split_kernel<T, DP, NT, WPP, false>>("aw_split_kernel", smem, false);
   if (rc != IM_OK) return rc;
-  return launch("aw_split_kernel", aw_split_kernel<T, DP, NT, false>, grid, dim3(threads), smem, st, a);
+  return launch("aw_split_kernel", aw_split_kernel<T, DP, NT, WPP, false>, grid, dim3(threads), smem, st, a);
 }
 
+// Wide heads leave an SM room for six rings; a warp a tile of 8 vectors there: 9 rows of 32/8 heads of 256 over 6762 slots
+// take 44.5 us, with one warp for both tiles 48.6; 2 rows of 16/2 over 3000 slots 14.4 and 17.1. Up to 128 the products bound it
+// with either, and a second warp that reads the same page costs more than it hides: 8 x 5 rows of 32/8 heads of 128 over
+// 8192 slots 77 us with one, 89 with three.
 template <typename T, int NT>
 int launch_split_d(const AwArgs& a, bool one, dim3 grid, cudaStream_t st) {
-  return a.d <= 64    ? launch_split<T, 64, NT>(a, one, grid, st)
-         : a.d <= 96  ? launch_split<T, 96, NT>(a, one, grid, st)
-         : a.d <= 128 ? launch_split<T, 128, NT>(a, one, grid, st)
-                      : launch_split<T, 256, NT < 3 ? NT : 2>(a, one, grid, st);  // NT 3 is not chosen for them
+  return a.d <= 64    ? launch_split<T, 64, NT, 1>(a, one, grid, st)
+         : a.d <= 96  ? launch_split<T, 96, NT, 1>(a, one, grid, st)
+         : a.d <= 128 ? launch_split<T, 128, NT, 1>(a, one, grid, st)
+                      : launch_split<T, 256, 1, NT < 3 ? NT : 2>(a, one, grid, st);  // NT 3 is not chosen for them
 }
 
 template <typename T>
