@@ -530,6 +530,11 @@ int im_verify_sampled(const void* target, int64_t target_ld, const void* draft, 
                       const int32_t* drafts, int64_t drafts_ld, const int32_t* n_drafts, const float* uniforms,
                       int64_t uniforms_ld, int64_t B, int64_t K, int64_t V, int32_t* out_tokens, int32_t* out_count,
                       void* stream);
+/* One of these calls with its arguments in an array: 64-bit words, the first the entry's number, then every argument in its
+ * order, the stream last (pointers and integers as they are, scale and factor as a double). For bindings whose calls cost by the
+ * argument. Returns what the entry returns. */
+enum { IM_CALL_ROPE = 0, IM_CALL_ROPE_KV = 1, IM_CALL_ATTENTION_WEIGHTS = 2, IM_CALL_CACHE_EVICT = 3, IM_CALL_VERIFY_SAMPLED = 4 };
+int im_bounded_call(const void* words, size_t bytes);
 
 #ifdef __cplusplus
 }

@@ -106,6 +106,7 @@ SIGNATURES: dict[str, tuple] = {
     "im_cache_evict": (_INT, [_P, _P, _I64, _I64, _I64, _P, _I64, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64,
                               _I64, _I64, _I64, _P, _SZ, _P]),
     "im_verify_sampled": (_INT, [_P, _I64, _P, _I64, _INT, _P, _I64, _P, _P, _I64, _I64, _I64, _I64, _P, _P, _P]),
+    "im_bounded_call": (_INT, [ctypes.c_char_p, _SZ]),
     "im_philox4x32_10": (_INT, [ctypes.c_uint64, ctypes.c_uint64, ctypes.c_uint32, ctypes.c_uint32, _P, _P]),
 }
 

@@ -13,6 +13,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+import struct
 import threading
 
 import torch
@@ -772,15 +773,28 @@ _LAYOUTS = {"half": _lib.ROPE_HALF, "interleaved": _lib.ROPE_INTERLEAVED}
 PAGE_SLOTS = 16
 
 
+# entry point -> its number in im_bounded_call and its arguments' words: integers and pointers, or one double
+_WORDS = {"im_rope": (0, struct.Struct("=9qd10q").pack), "im_rope_kv": (1, struct.Struct("=5qd19q").pack),
+          "im_attention_weights": (2, struct.Struct("=21qd7q").pack), "im_cache_evict": (3, struct.Struct("=25q").pack),
+          "im_verify_sampled": (4, struct.Struct("=17q").pack)}
+
+
 def _launch(index: int, name: str, *args) -> None:
-    """_lib.call on a device's current stream (the entry point's last argument), with the device current."""
+    """Call an entry point on a device's current stream (its last argument), with the device current; no tensor is 0."""
+    entry, pack = _WORDS[name]
     if torch._C._cuda_getDevice() == index:
-        status = getattr(_lib.load(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
+        words = pack(entry, *args, torch._C._cuda_getCurrentRawStream(index))
+        status = _lib.load().im_bounded_call(words, len(words))
     else:
         with torch.cuda.device(index):
-            status = getattr(_lib.load(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
+            words = pack(entry, *args, torch._C._cuda_getCurrentRawStream(index))
+            status = _lib.load().im_bounded_call(words, len(words))
     if status:
         _lib.check(name, status)
+
+
+def _ptr_or_zero(t: torch.Tensor | None) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def _need(t: torch.Tensor, name: str, dtype: torch.dtype, device: torch.device, index: int) -> None:
@@ -961,7 +975,7 @@ def rope_kv(qkv: torch.Tensor, inv_freq: torch.Tensor, row_pos: torch.Tensor, ro
         _launch(index, "im_rope_kv", qkv.data_ptr(), inv_freq.data_ptr(), freq64, rotary, float(factor), lay,
                 row_pos.data_ptr(), row_slot.data_ptr(), row_seq.data_ptr(), page_table.data_ptr(), seqs, max_pages, pages,
                 m, hq, hkv, d, _TYPES[dtype],
-                q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _ptr_or_none(slot_pos), cap)
+                q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _ptr_or_zero(slot_pos), cap)
     return q_out
 
 
@@ -1027,8 +1041,8 @@ def attention_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None  # few, short splits need none
     _launch(index, "im_attention_weights", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _TYPES[dtype],
             page_table.data_ptr(), seqs, max_pages, pages, seq_rows.data_ptr(),
-            _ptr_or_none(seq_slot), row_slot.data_ptr(), m, b, max_rows, hq, hkv, d, max_kv_len, keys_per_split, window,
-            float(scale), weights.data_ptr(), weights_out.data_ptr(), cap, out.data_ptr(), _ptr_or_none(ws),
+            _ptr_or_zero(seq_slot), row_slot.data_ptr(), m, b, max_rows, hq, hkv, d, max_kv_len, keys_per_split, window,
+            float(scale), weights.data_ptr(), weights_out.data_ptr(), cap, out.data_ptr(), _ptr_or_zero(ws),
             need)
     return out
 
@@ -1099,7 +1113,7 @@ def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.
             pages, page_table.data_ptr(), max_pages, lengths.data_ptr(), seen.data_ptr(), weights.data_ptr(),
             (weights if weights_out is None else weights_out).data_ptr(), slot_pos.data_ptr(),
             (slot_pos if pos_out is None else pos_out).data_ptr(), lengths_out.data_ptr(), s, hkv, cap, d * size,
-            budget, recent, sinks, _ptr_or_none(ws), need)
+            budget, recent, sinks, _ptr_or_zero(ws), need)
     return lengths_out
 
 
@@ -1158,8 +1172,8 @@ def verify_sampled(target_probs: torch.Tensor, draft_probs: torch.Tensor | None,
     tokens = drafts.new_empty((b, k + 1)) if tokens is None else tokens
     count = drafts.new_empty((b,)) if count is None else count
     if b:
-        _launch(index, "im_verify_sampled", target_probs.data_ptr(), p_ld, _ptr_or_none(draft_probs), q_ld,
-                _TYPES[target_probs.dtype], drafts.data_ptr(), k, _ptr_or_none(n_drafts), uniforms.data_ptr(), k + 1, b, k,
+        _launch(index, "im_verify_sampled", target_probs.data_ptr(), p_ld, _ptr_or_zero(draft_probs), q_ld,
+                _TYPES[target_probs.dtype], drafts.data_ptr(), k, _ptr_or_zero(n_drafts), uniforms.data_ptr(), k + 1, b, k,
                 v, tokens.data_ptr(), count.data_ptr())
     return tokens, count
 

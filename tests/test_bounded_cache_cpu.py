@@ -152,3 +152,46 @@ def test_wrappers_need_cuda_tensors():
                             torch.zeros((1, 1, 16)), torch.zeros((1, 1, 16), dtype=torch.int32), budget=4)
     with pytest.raises(TypeError):
         kernels.verify_sampled(torch.zeros((1, 1, 4)), None, torch.zeros((1, 0), dtype=torch.int32), torch.zeros((1, 1)))
+
+
+@pytest.mark.parametrize("name", sorted(kernels._WORDS))
+def test_calls_in_one_array_answer_as_the_entries_do(name):
+    """Every argument arrives at its place: small pointers and sizes, one of them wrong at a time, are refused alike."""
+    lib = _lib.load()
+    entry, pack = kernels._WORDS[name]
+    kinds = [t.__name__ for t in _lib.SIGNATURES[name][1]]
+    good = {"im_rope": (256, 16, 16, 256, 0, 256, 0, 4, 1.0, 0, 0, 1, 1, 16, 0, 256, 16, 16, 0),
+            "im_rope_kv": (256, 256, 0, 4, 1.0, 0, 256, 256, 256, 256, 1, 1, 1, 1, 4, 2, 16, 0, 256, 256, 256, 256, 16, 0),
+            "im_attention_weights": (256, 256, 256, 0, 256, 1, 1, 1, 256, 256, 256, 1, 1, 1, 4, 2, 16, 16, 0, 0, 1.0, 256,
+                                     256, 16, 256, 256, 1 << 30, 0),
+            "im_cache_evict": (256, 256, 1, 512, 1, 256, 1, 256, 512, 256, 256, 256, 256, 256, 1, 2, 16, 32, 8, 2, 2, 256,
+                               1 << 30, 0),
+            "im_verify_sampled": (256, 64, 256, 64, 0, 256, 2, 256, 256, 3, 1, 2, 64, 256, 256, 0)}[name]
+    assert len(good) == len(kinds)
+    refused = 0
+    for at, kind in enumerate(kinds[:-1]):
+        for bad in (257, 0, -1, 1 << 20, 1 << 40) if kind not in ("c_double", "c_float") else (0.5,):
+            args = [*good]
+            args[at] = bad
+            # a second fault, so that nothing is ever launched: a type that is none, more recent slots than any budget
+            if name == "im_cache_evict":
+                args[19] = 1 << 41
+            else:
+                args[[i for i, k in enumerate(kinds) if k == "c_int"][-1]] = 9
+            if kind == "c_int" and bad == 1 << 40:
+                continue  # not an int
+            want = getattr(lib, name)(*args), lib.im_last_error()
+            words = pack(entry, *args)
+            assert (lib.im_bounded_call(words, len(words)), lib.im_last_error()) == want, (at, bad)
+            refused += want[0] != _lib.IM_OK
+    assert refused > len(kinds)
+
+
+def test_calls_in_one_array_refusals():
+    lib = _lib.load()
+    words = kernels._WORDS["im_verify_sampled"][1](*[0] * 17)
+    for given, size in ((None, 136), (words, 0), (words, 7), (words, 136), (words, 128), (words, 1 << 20)):
+        assert lib.im_bounded_call(given, size) == _lib.IM_INVALID and b"im_bounded_call" in lib.im_last_error()
+    for entry in (-1, 5, 1 << 40):
+        words = kernels._WORDS["im_verify_sampled"][1](entry, *[0] * 16)
+        assert lib.im_bounded_call(words, 136) == _lib.IM_INVALID
