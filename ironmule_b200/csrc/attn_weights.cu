@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(AwShape<DP, NT, WPP>::WARPS * 32, AwShape<DP, 
   const int held = a.kps + 4;
   pdl_wait();
   pdl_trigger();
-  int split = blockIdx.x;  // with a window: counted from the first that a row sees
+  int split = blockIdx.x;  // of two kernels' with a window: counted from the first that a row sees
   const int h = blockIdx.y / a.tiles, tile = blockIdx.y % a.tiles, b = blockIdx.z;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const int worker = warp / WPP, part = warp % WPP;  // which pages, which vectors
@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(AwShape<DP, NT, WPP>::WARPS * 32, AwShape<DP, 
       }
   }
   aw_span(a, q);
-  if (a.window > 0) split += q.lo / 16 * 16 / a.kps;
+  if (!ONE && a.window > 0) split += q.lo / 16 * 16 / a.kps;
   char* ring = smem + worker * S::RING;
   const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
   if (a.d < DP) {  // columns behind the head: zeros, once
@@ -628,7 +628,7 @@ __global__ void __launch_bounds__(AwShape<DP, NT, WPP>::WARPS * 32, AwShape<DP, 
         const int j = split * a.kps + t + i * WARPS * 32;
         if (j >= n) continue;
         float sum = 0.f;
-        for (int v = 0; v < count; v++) {
+        for (int v = 0; v < count && j >= k0; v++) {  // no row sees the slots before
           const float2 st = s_total[v];
           sum = fmaf(aw_exp2(s_scores[v * held + j - split * a.kps] - st.x), st.y, sum);
         }
@@ -868,11 +868,13 @@ static AwPlan aw_plan(int64_t B, int64_t rows, int64_t Hq, int64_t Hkv, int64_t 
   if (D <= 128 && p.vecs > 16 && (p.vecs + 23) / 24 * 23 < (p.vecs + 15) / 16 * 16) p.tile = 24;
   p.tiles = (int)((p.vecs + p.tile - 1) / p.tile);
   p.kv_pad = (kv + 63) / 64 * 64;
-  // one kernel: no window (its splits begin where the rows' slots say), one tile, blocks that are on the device at once
+  // one kernel: no window, or one of half the slots and more (the blocks are those of all slots), one tile, blocks that are
+  // on the device at once. One row with a window of 512 over 1000 slots 10.9 us a call, with two kernels 14.7 (as a graph 9.4 and
+  // 11.0); of 1024 over 2048 11.0 and 14.8 (10.2 and 8.2)
   const int64_t groups = B * Hkv * p.tiles;
   auto one = [&](int64_t k) {
     const int64_t n = (kv + k - 1) / k;
-    return window == 0 && p.tiles == 1 && n <= AW_CLUSTER && groups * n <= 296 && p.tile * k * 4 <= AW_HELD;
+    return (window == 0 || 2 * (window + rows) >= kv) && p.tiles == 1 && n <= AW_CLUSTER && groups * n <= 296 && p.tile * k * 4 <= AW_HELD;
   };
   if (kps == 0) {
     const int64_t resident = 148 * aw_resident(D, p.tile);
@@ -891,7 +893,7 @@ static AwPlan aw_plan(int64_t B, int64_t rows, int64_t Hq, int64_t Hkv, int64_t 
   p.kps = (int)kps;
   p.splits = (int)((kv + kps - 1) / kps);
   p.one = one(kps);
-  p.seen = window > 0 && (window + rows) / kps + 2 < p.splits ? (int)((window + rows) / kps + 2) : p.splits;
+  p.seen = !p.one && window > 0 && (window + rows) / kps + 2 < p.splits ? (int)((window + rows) / kps + 2) : p.splits;
   const size_t heads = p.one ? 0 : (size_t)B * Hkv;
   p.scores = aw_round(heads * p.vecs * p.kv_pad * 4);
   p.stats = aw_round(heads * p.splits * p.vecs * 8);

@@ -356,6 +356,26 @@ def test_attention_weights_masks(cuda):
                  max_kv=2 * 10**6)
 
 
+@pytest.mark.parametrize("rows", [[1, 1, 1], [5, 3, 5]])
+@pytest.mark.parametrize("window", [110, 150, 215])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_attention_weights_of_half_a_window(cuda, rows, window, in_place):
+    """Windows of half the slots and more, whose splits a call may take in one kernel: some splits are seen by no row, in
+    some the first pages are not. A row's bits are those of a call over a longer table."""
+    case = attend_case(cuda, window, [200, 64, 190], rows, 8, 4, 128, torch.bfloat16)
+    out, after = attend_check(case, window=window, in_place=in_place, keys_per_split=64)
+    attend_check(case, window=window, in_place=in_place)
+    q, k, v, table, bounds, slot, weights = case
+    wider = torch.cat([table, table.new_full((3, 60), -1)], dim=1)
+    given = torch.full((3, 4, wider.shape[1] * 16), -7.0, device=cuda)
+    given[:, :, :weights.shape[2]] = weights
+    far = kernels.attention_weights(q, k, v, wider, bounds, slot, given, max_rows_per_seq=max(rows), max_kv_len=1100,
+                                    scale=128 ** -0.5, window=window, keys_per_split=64)
+    assert torch.equal(far, out)
+    for b, n in enumerate((200, 64, 190)):
+        torch.testing.assert_close(given[b, :, :n], after[b, :, :n], rtol=1e-5, atol=1e-7)
+
+
 @pytest.mark.parametrize("lengths,rows", [([90, 40], [4, 3]), ([5000, 900], [4, 3]), ([300], [9])])
 @pytest.mark.parametrize("in_place", [False, True])
 def test_attention_weights_of_rows_padded_in_front(cuda, lengths, rows, in_place):
