@@ -881,10 +881,10 @@ static AwPlan aw_plan(int64_t B, int64_t rows, int64_t Hq, int64_t Hkv, int64_t 
     const int64_t seen = window > 0 && window + rows < kv ? window + rows : kv;  // slots a sequence's rows can see
     const int64_t most = groups <= 296 ? 296 / groups : 1, few = most < AW_CLUSTER ? most : AW_CLUSTER;
     kps = ((kv + few - 1) / few + 63) / 64 * 64;
-    // up to 384 keys a block (128 for wide heads or more vectors): one row over 6144 slots takes 15.8 us a call with one
-    // kernel and 20.0 with two (as a graph 14.7 and 12.6), over 8192 slots 17.2 and 19.6 (17.1 and 14.1); 5 rows over 4096
-    // slots 22.6 and 19.2
-    if (!one(kps) || kps > (D <= 128 && p.tile == 8 ? 384 : 128)) {
+    // up to 320 keys a block (128 for wide heads or 16 vectors, 64 for 24): one row over 5000 slots takes 13.9 us a call with
+    // one kernel and 14.7 with two (as a graph 13.7 and 11.6), over 6144 slots 14.8 and 15.0 (14.6 and 12.5); 5 rows of 32/8
+    // heads over 2048 slots 18.2 with blocks of 128 keys and 16.8 with two kernels
+    if (!one(kps) || kps > (p.tile == 24 ? 64 : D <= 128 && p.tile == 8 ? 320 : 128)) {
       const int64_t want = groups * 2 >= resident ? (seen + 767) / 768 : resident / groups;
       kps = ((seen + want - 1) / want + 63) / 64 * 64;
     }

@@ -1046,7 +1046,7 @@ def attention_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
         return out
     max_rows = min(max_rows_per_seq, m)
     need = _attention_weights_workspace(b, max_rows, hq, hkv, d, max(1, max_kv_len), keys_per_split, window)
-    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None  # few, short splits need none
+    ws = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=device) if need else None  # few, short splits need none
     _launch(index, "im_attention_weights", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _TYPES[dtype],
             page_table.data_ptr(), seqs, max_pages, pages, seq_rows.data_ptr(),
             _ptr_or_zero(seq_slot), row_slot.data_ptr(), m, b, max_rows, hq, hkv, d, max_kv_len, keys_per_split, window,
@@ -1115,7 +1115,7 @@ def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.
     if not (layers and s and hkv and cap and d):
         return lengths_out.zero_()
     need = _evict_workspace(layers, s, hkv, cap, budget)
-    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None  # few moves a row need none
+    ws = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=device) if need else None  # few moves a row need none
     size = k_cache.element_size()
     _launch(index, "im_cache_evict", k_cache.data_ptr(), v_cache.data_ptr(), layers, pages * hkv * PAGE_SLOTS * d * size,
             pages, page_table.data_ptr(), max_pages, lengths.data_ptr(), seen.data_ptr(), weights.data_ptr(),
