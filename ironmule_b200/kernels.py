@@ -1034,7 +1034,7 @@ def attention_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
             raise ValueError(f"weights_out must be {tuple(weights.shape)}, got {tuple(weights_out.shape)}")
         _apart(weights_out, "weights_out", weights, "weights")
     if out is None:
-        out = q.new_empty(m, hq, d)  # a list of sizes costs 0.4 us less than a tuple of them
+        out = q.new_empty(m, hq, d)  # sizes one by one: 0.4 us less than a tuple of them
     else:
         _need(out, "out", dtype, device, index)
         if out.numel() < m * hq * d:
