@@ -783,14 +783,16 @@ def _launch(index: int, name: str, *args) -> None:
     """Call an entry point on a device's current stream (its last argument), with the device current; no tensor is 0."""
     entry, pack = _WORDS[name]
     if torch._C._cuda_getDevice() == index:
-        words = pack(entry, *args, torch._C._cuda_getCurrentRawStream(index))
+        try:
+            words = pack(entry, *args, torch._C._cuda_getCurrentRawStream(index))
+        except struct.error as exc:
+            raise ValueError(f"{name}: an argument is no 64-bit integer ({exc})") from exc
         status = _lib.load().im_bounded_call(words, len(words))
+        if status:
+            _lib.check(name, status)
     else:
         with torch.cuda.device(index):
-            words = pack(entry, *args, torch._C._cuda_getCurrentRawStream(index))
-            status = _lib.load().im_bounded_call(words, len(words))
-    if status:
-        _lib.check(name, status)
+            _launch(index, name, *args)
 
 
 def _ptr_or_zero(t: torch.Tensor | None) -> int:

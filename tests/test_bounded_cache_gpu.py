@@ -976,6 +976,7 @@ def test_refusals_of_the_wrappers(cuda):
     for out, what in ((seen, "seen"), (both[1:3], "seen"), (both[:2], "lengths")):
         refuses(kernels.cache_evict, k5, v5, table, lengths if what == "seen" else both[1:3],
                 seen if out is seen else both[2:], weights, spos, budget=10, lengths_out=out, match=what)
+    refuses(kernels.cache_evict, k5, v5, table, lengths, seen, weights, spos, budget=2**70, match="64-bit")
     refuses(kernels.cache_evict, k5, v5.half(), table, lengths, seen, weights, spos, budget=10, error=TypeError)
     p, q, drafts, u = verify_case(cuda, 9, 2, 3, 50, torch.float32)
     refuses(kernels.verify_sampled, p[:, :3], q, drafts, u, match="target_probs")
