@@ -16,6 +16,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <utility>
+
 #include "common.cuh"
 
 namespace im {
@@ -75,6 +77,9 @@ __global__ void __launch_bounds__(VS_THREADS, 2) verify_sampled_kernel(VerifyArg
   extern __shared__ double left[];          // the weights of the part that holds the token
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = cluster.num_blocks(), rank = cluster.block_rank();
+  // a block may be written to once it is known to run: all arrive here, and wait for the others before the first remote
+  // store, with the gathers and sums between
+  auto started = cluster.barrier_arrive();
   pdl_wait();
   pdl_trigger();
   const long long b = blockIdx.x / ranks;
@@ -137,6 +142,7 @@ __global__ void __launch_bounds__(VS_THREADS, 2) verify_sampled_kernel(VerifyArg
     sum = vs_warp_sum(sum);
     if (lane == 0) sums[warp] = sum;
     __syncthreads();
+    if (attempt == 0) cluster.barrier_wait(std::move(started));
     if (warp == 0) {
       double s = lane < VS_WARPS ? sums[lane] : 0.0;
       s = vs_warp_sum(s);

@@ -2,6 +2,8 @@
 from __future__ import annotations
 
 import math
+import re
+from pathlib import Path
 
 import pytest
 import torch
@@ -195,3 +197,19 @@ def test_calls_in_one_array_refusals():
     for entry in (-1, 5, 1 << 40):
         words = kernels._WORDS["im_verify_sampled"][1](entry, *[0] * 16)
         assert lib.im_bounded_call(words, 136) == _lib.IM_INVALID
+
+
+def test_blocks_of_a_cluster_meet_before_they_reach_into_each_other():
+    """A block's shared memory may be read or written by others once it is known to run: in every kernel's text a meeting
+    of the cluster stands before the first remote address."""
+    seen = 0
+    for path in sorted((Path(kernels.__file__).parent / "csrc").glob("*.cu*")):
+        text = re.sub(r"//[^\n]*", "", path.read_text())
+        for body in text.split("__global__")[1:]:
+            remote = body.find("map_shared_rank")
+            if remote < 0:
+                continue
+            seen += 1
+            met = re.search(r"\.(sync|barrier_wait)\(", body)
+            assert met and met.start() < remote, f"{path.name}: remote shared memory before a meeting"
+    assert seen >= 3

@@ -655,6 +655,18 @@ def test_verify_sampled_many_drafts(cuda):
     assert all(c >= 1 for c in counts)
 
 
+@pytest.mark.parametrize("b", [1, 2, 9, 150])
+@pytest.mark.parametrize("v", [2, 4096, 32768])
+def test_verify_sampled_with_little_between_start_and_meeting(cuda, b, v):
+    """No drafts and few tokens a block: blocks of a cluster tell each other their sums right after their start."""
+    p, _, drafts, u = verify_case(cuda, b + v, b, 0, v, torch.float32)
+    verify_check(p, None, drafts, u)
+    tokens, count = kernels.verify_sampled(p, None, drafts, u)
+    for _ in range(200):
+        got = kernels.verify_sampled(p, None, drafts, u)
+        assert torch.equal(got[0], tokens) and torch.equal(got[1], count)
+
+
 def test_verify_sampled_borders(cuda):
     p = torch.tensor([[0.25, 0.0, 0.25, 0.5], [0.5, 0.25, 0.0, 0.25]], device=cuda)[None]
     q = torch.tensor([[0.5, 0.0, 0.25, 0.25]], device=cuda)[None]
