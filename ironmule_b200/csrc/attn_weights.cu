@@ -293,10 +293,11 @@ __global__ void __launch_bounds__(AwShape<DP, NT, WPP>::WARPS * 32, AwShape<DP, 
   if (!ONE && a.window > 0) split += q.lo / 16 * 16 / a.kps;
   char* ring = smem + worker * S::RING;
   const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
-  if (a.d < DP) {  // columns behind the head: zeros, once
+  auto clear = [&]() {  // columns behind the head: zeros; the accumulators of a split lie over them at its end
     for (int c = lane + 32 * part; c < S::STAGES * 2 * 16 * CP; c += 32 * WPP)
       if (c % CP * 8 >= a.d) *(uint4*)(ring + c / CP * S::PITCH + c % CP * 16) = make_uint4(0, 0, 0, 0);
-  }
+  };
+  if (a.d < DP) clear();
   const uint64_t policy = aw_policy(a.tiles == 1);
   int all_last = 0x7fffffff, all_from = 0;  // slots that every row of the tile sees: pages inside need no mask
 #pragma unroll
@@ -639,6 +640,7 @@ __global__ void __launch_bounds__(AwShape<DP, NT, WPP>::WARPS * 32, AwShape<DP, 
       return;
     }
     __syncthreads();  // the ring is the copies' again
+    if (a.d < DP) clear();
   }
 }
 

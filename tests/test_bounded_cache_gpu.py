@@ -306,6 +306,18 @@ def test_attention_weights_of_rows_far_apart(cuda, window, kps):
     attend_check((q, k, v, table, bounds, slot, weights), keys_per_split=kps)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [16, 48, 64, 80, 96, 112, 128, 144, 192, 256])
+@pytest.mark.parametrize("kps", [0, 64])
+def test_attention_weights_of_blocks_with_several_splits(cuda, dtype, d, kps):
+    """Rows of two windows side by side: a block takes a split of one and then a split of the other, and what the first leaves
+    in shared memory reaches nothing, in heads that are narrower than the columns kept for them either."""
+    for seed in range(3):
+        q, k, v, table, bounds, slot, weights = attend_case(cuda, d + seed, [420, 420], [6, 3], 8, 2, d, dtype)
+        slot[:] = ints([200, 201, 202, 392, 393, 394, 150, 342, 343], cuda)
+        attend_check((q, k, v, table, bounds, slot, weights), window=100, keys_per_split=kps)
+
+
 def test_attention_weights_bits_do_not_depend_on_the_launch(cuda):
     """With keys_per_split given, a row alone equals the same row in a batch, among other rows."""
     q, k, v, table, bounds, slot, weights = attend_case(cuda, 11, [700, 333, 64], [5, 3, 1], 8, 2, 128, torch.bfloat16)
