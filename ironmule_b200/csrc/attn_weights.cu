@@ -193,15 +193,21 @@ struct AwType<__half> {
   static __device__ __forceinline__ __half down(float f) { return __float2half_rn(f); }
 };
 
+// Adds a split's maximum and sum to (m, l). -inf and 0 are those of no visible slot; a sum of NaN (scores of NaN have no
+// maximum: it may be -inf) stays one.
+__device__ __forceinline__ void aw_add(float& m, float& l, float m2, float l2) {
+  const float top = fmaxf(m, m2);
+  l = top != -INFINITY ? l * aw_exp2(m - top) + l2 * aw_exp2(m2 - top) : l + l2;
+  m = top;
+}
+
 // The total of a vector whose splits' maxima and sums lie in a warp's lanes (-inf and 0 where there is none): maximum and
 // 1 / sum, in every lane.
 __device__ __forceinline__ float2 aw_join(float m, float l) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const float m2 = __shfl_xor_sync(0xffffffffu, m, o), l2 = __shfl_xor_sync(0xffffffffu, l, o);
-    const float top = fmaxf(m, m2);
-    if (top != -INFINITY) l = l * aw_exp2(m - top) + l2 * aw_exp2(m2 - top);
-    m = top;
+    aw_add(m, l, m2, l2);
   }
   return make_float2(m == -INFINITY ? 0.f : m, l == 0.f ? 0.f : 1.f / l);
 }
@@ -245,6 +251,7 @@ __global__ void __launch_bounds__(AwShape<DP, NT, WPP>::WARPS * 32, AwShape<DP, 
   __shared__ float s_m[RINGS][TILE], s_l[RINGS][TILE];
   // ONE: this block's maxima and sums, the whole cluster's, the final ones
   __shared__ float2 s_stat[ONE ? TILE : 1], s_all[ONE ? AW_CLUSTER : 1][ONE ? TILE : 1], s_total[ONE ? TILE : 1];
+  __shared__ int2 s_sees[ONE ? TILE : 1];  // ONE: the slots that a vector sees, [x, y]
   float* s_out = (float*)(smem + S::SMEM);  // ONE: [TILE][JOIN]
   float* s_scores = s_out + TILE * S::JOIN;  // ONE: [TILE][kps + 4]
   const int held = a.kps + 4;
@@ -532,6 +539,7 @@ __global__ void __launch_bounds__(AwShape<DP, NT, WPP>::WARPS * 32, AwShape<DP, 
         for (int x = 4; x < 32; x <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], x);
         const int row = (part * NT + nt) * 8 + lane * 2 + e;
         if (lane < 4) s_m[worker][row] = m[nt][e], s_l[worker][row] = l[nt][e];
+        if (ONE && worker == 0 && lane < 4) s_sees[row] = make_int2(from[nt][e], last[nt][e]);
       }
     __syncthreads();  // every warp is done with its ring, which now takes its accumulator
 #pragma unroll
@@ -569,7 +577,7 @@ __global__ void __launch_bounds__(AwShape<DP, NT, WPP>::WARPS * 32, AwShape<DP, 
       for (int w = 1; w < RINGS; w++) mm = fmaxf(mm, s_m[w][t]);
       float sum = 0.f;
 #pragma unroll
-      for (int w = 0; w < RINGS; w++) sum += s_m[w][t] == -INFINITY ? 0.f : aw_exp2(s_m[w][t] - mm) * s_l[w][t];
+      for (int w = 0; w < RINGS; w++) sum += s_l[w][t] == 0.f ? 0.f : aw_exp2(s_m[w][t] - mm) * s_l[w][t];  // 0: no slot
       if (ONE) s_stat[t] = make_float2(mm, sum);
       else a.stats[at + t] = make_float2(mm, sum);
     }
@@ -632,7 +640,8 @@ __global__ void __launch_bounds__(AwShape<DP, NT, WPP>::WARPS * 32, AwShape<DP, 
         float sum = 0.f;
         for (int v = 0; v < count && j >= k0; v++) {  // no row sees the slots before
           const float2 st = s_total[v];
-          sum = fmaf(aw_exp2(s_scores[v * held + j - split * a.kps] - st.x), st.y, sum);
+          const int2 sees = s_sees[v];
+          if (j >= sees.x && j <= sees.y) sum = fmaf(aw_exp2(s_scores[v * held + j - split * a.kps] - st.x), st.y, sum);
         }
         a.weights_out[base + j] = old[i] + sum;
       }
@@ -651,9 +660,7 @@ __device__ __forceinline__ float2 aw_total(const AwArgs& a, long long head, int 
   float m = -INFINITY, l = 0.f;
   for (int s = s0 + ((lane - s0) & 31); s < s1; s += 32) {
     const float2 x = a.stats[(head * a.splits + s) * a.vecs + v];
-    const float top = fmaxf(m, x.x);
-    if (top != -INFINITY) l = l * aw_exp2(m - top) + x.y * aw_exp2(x.x - top);
-    m = top;
+    aw_add(m, l, x.x, x.y);
   }
   return aw_join(m, l);
 }
@@ -788,9 +795,7 @@ __global__ void __launch_bounds__(AW_FIN_THREADS, 4) aw_finish_kernel(AwArgs a) 
 #pragma unroll 4
       for (int s = s0; s < s1; s++) {
         const float2 x = a.stats[(head * a.splits + s) * a.vecs + v];
-        const float top = fmaxf(m, x.x);
-        if (top != -INFINITY) l = l * aw_exp2(m - top) + x.y * aw_exp2(x.x - top);
-        m = top;
+        aw_add(m, l, x.x, x.y);
       }
       keep(v, make_float2(m == -INFINITY ? 0.f : m, l == 0.f ? 0.f : 1.f / l));
     }

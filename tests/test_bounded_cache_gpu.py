@@ -438,6 +438,51 @@ def test_attention_weights_of_values_that_are_not_finite(cuda, dtype):
     assert bool((out == 0).all())
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lengths,rows,d,window,kps", [([37], [1], 64, 0, 0), ([37, 20], [5, 3], 64, 0, 0), ([700], [1], 128, 0, 64),
+                                                       ([700, 300], [5, 2], 80, 0, 0), ([5000], [1], 128, 0, 0),
+                                                       ([3000, 200], [5, 2], 256, 0, 0), ([900], [33], 64, 0, 64),
+                                                       ([3000], [5], 128, 300, 0), ([300], [3], 128, 200, 0)])
+def test_attention_weights_of_a_query_that_is_nan(cuda, dtype, lengths, rows, d, window, kps):
+    """Its row is NaN, and so are the weights of the slots that it sees; nothing else changes by a bit."""
+    q, k, v, table, bounds, slot, weights = attend_case(cuda, 31, lengths, rows, 8, 2, d, dtype)
+    kw = {"max_rows_per_seq": max(rows), "max_kv_len": table.shape[1] * 16, "scale": d ** -0.5, "window": window,
+          "keys_per_split": kps}
+    want, after = kernels.attention_weights(q, k, v, table, bounds, slot, was := weights.clone(), **kw), was
+    for at, head in ((0, 1), (rows[0] // 2, 6), (int(bounds[-1]) - 1, 3)):
+        bad = q.clone()
+        bad[at, head, 5] = NAN
+        got = weights.clone()
+        out = kernels.attention_weights(bad, k, v, table, bounds, slot, got, **kw)
+        assert bool(out[at, head].isnan().all())
+        others = torch.ones_like(out, dtype=torch.bool)
+        others[at, head] = False
+        assert torch.equal(out[others], want[others])
+        s = 0 if at < rows[0] else 1
+        sees = torch.zeros_like(weights, dtype=torch.bool)
+        last = int(slot[at])
+        sees[s, head // 4, max(0, last - window + 1) if window else 0:last + 1] = True
+        assert bool(got[sees].isnan().all())
+        assert torch.equal(got[~sees], after[~sees])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lengths,rows,kps,bad", [([300], [1], 64, (64, 128)), ([300], [5], 64, (0, 64)), ([3000], [1], 64, (128, 192)),
+                                                  ([3000, 500], [5, 1], 64, (0, 64)), ([300, 100], [4, 2], 0, (10, 11))])
+def test_attention_weights_of_keys_that_are_nan(cuda, dtype, lengths, rows, kps, bad):
+    """A split that has NaN scores alone is no split without a slot: every row that sees it is NaN."""
+    q, k, v, table, bounds, slot, weights = attend_case(cuda, 32, lengths, rows, 8, 2, 128, dtype)
+    for j in range(*bad):
+        k[int(table[0, j // 16]), 1, j % 16] = NAN
+    kw = {"max_rows_per_seq": max(rows), "max_kv_len": table.shape[1] * 16, "scale": 0.1, "keys_per_split": kps}
+    out = kernels.attention_weights(q, k, v, table, bounds, slot, got := weights.clone(), **kw)
+    want, after, tol, w_tol = attend_plain(q, k, v, table, bounds, slot, weights, 0.1)
+    assert torch.equal(out.isnan(), want.isnan()) and bool(out[:rows[0], 4:].isnan().all())
+    assert torch.equal(got.isnan(), after.isnan())
+    fine = ~want.isnan()
+    assert bool(((out.double() - want).abs() <= tol)[fine].all())
+
+
 def test_attention_weights_of_large_scores_and_equal_ones(cuda):
     case = attend_case(cuda, 21, [500, 64], [1, 4], 8, 2, 128, torch.bfloat16, spread=8.0)
     attend_check(case, scale=1.0)  # scores in the hundreds: one slot has nearly all the weight
