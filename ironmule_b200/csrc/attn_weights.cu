@@ -28,6 +28,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace im {
@@ -329,259 +331,276 @@ __global__ void __launch_bounds__(AwShape<DP, NT, WPP>::WARPS * 32, AwShape<DP, 
   };
 
   // one split, unless rows with a window lie so far apart that there are more than blocks
-  for (;; split += gridDim.x) {
+  bool redo = false;  // the same split once more
+  for (;; split += redo ? 0 : (int)gridDim.x) {
     const int k0 = max(split * a.kps, q.lo / 16 * 16), k1 = min(split * a.kps + a.kps, q.n);
     if (!ONE && k0 >= k1) return;  // the whole block
     const int p0 = k0 / 16, p1 = k0 < k1 ? (k1 + 15) / 16 : p0;
-    if (a.window > 0 || split != (int)blockIdx.x) {
-      next = p0 + ((worker - p0) & (RINGS - 1));
-      entry = next < p1 ? table[next] : 0;
-    }
-    int page = next;
-    uint32_t pages_ok = 0;  // of the pages in flight, the newest in bit 0: the table names one of the cache
-    auto fetch = [&](int stage) {
-      const bool ok = entry >= 0 && entry < a.pages;
-      pages_ok = pages_ok << 1 | (ok ? 1u : 0u);
-      if (next < p1) {
-        const long long at = ok ? ((long long)entry * a.hkv + h) * 16 * a.d * 2 : 0;
-        const int rows = ok ? min(16, q.n - next * 16) : 0;
-        const uint32_t dst = ring_at + stage * 2 * S::PAGE;
-        if (rows == 16 && a.d == DP) {  // a page lies in one piece
-          const char* k = a.k + at + lane * 16;
-          const char* v = a.v + at + lane * 16;
+    const int count = min(TILE, vecs - tile * TILE);
+    // A weight's high part and rest times an infinite value are not its product (the rest may be 0 or negative): where an
+    // output comes out NaN and its sum of weights did not, the split is done again, with every page looked through
+    auto run = [&](auto again) __attribute__((always_inline)) -> bool {
+      if (a.window > 0 || split != (int)blockIdx.x || again) {
+        next = p0 + ((worker - p0) & (RINGS - 1));
+        entry = next < p1 ? table[next] : 0;
+      }
+      int page = next;
+      uint32_t pages_ok = 0;  // of the pages in flight, the newest in bit 0: the table names one of the cache
+      auto fetch = [&](int stage) {
+        const bool ok = entry >= 0 && entry < a.pages;
+        pages_ok = pages_ok << 1 | (ok ? 1u : 0u);
+        if (next < p1) {
+          const long long at = ok ? ((long long)entry * a.hkv + h) * 16 * a.d * 2 : 0;
+          const int rows = ok ? min(16, q.n - next * 16) : 0;
+          const uint32_t dst = ring_at + stage * 2 * S::PAGE;
+          if (rows == 16 && a.d == DP) {  // a page lies in one piece
+            const char* k = a.k + at + lane * 16;
+            const char* v = a.v + at + lane * 16;
 #pragma unroll
-          for (int i = part; i < 16 * CP / 32; i += WPP) {
-            const int c = lane + 32 * i;
-            aw_copy16(dst + c / CP * S::PITCH + c % CP * 16, k + i * 512, true, policy);
-            aw_copy16(dst + S::PAGE + c / CP * S::PITCH + c % CP * 16, v + i * 512, true, policy);
-          }
-        } else {
+            for (int i = part; i < 16 * CP / 32; i += WPP) {
+              const int c = lane + 32 * i;
+              aw_copy16(dst + c / CP * S::PITCH + c % CP * 16, k + i * 512, true, policy);
+              aw_copy16(dst + S::PAGE + c / CP * S::PITCH + c % CP * 16, v + i * 512, true, policy);
+            }
+          } else {
 #pragma unroll
-          for (int i = part; i < 16 * CP / 32; i += WPP) {
-            const int c = lane + 32 * i, row = c / CP, col = c % CP;
-            if (col * 8 < a.d) {
-              const bool in = row < rows;
-              const long long off = at + (in ? (row * a.d + col * 8) * 2 : 0);
-              aw_copy16(dst + row * S::PITCH + col * 16, a.k + off, in, policy);
-              aw_copy16(dst + S::PAGE + row * S::PITCH + col * 16, a.v + off, in, policy);
+            for (int i = part; i < 16 * CP / 32; i += WPP) {
+              const int c = lane + 32 * i, row = c / CP, col = c % CP;
+              if (col * 8 < a.d) {
+                const bool in = row < rows;
+                const long long off = at + (in ? (row * a.d + col * 8) * 2 : 0);
+                aw_copy16(dst + row * S::PITCH + col * 16, a.k + off, in, policy);
+                aw_copy16(dst + S::PAGE + row * S::PITCH + col * 16, a.v + off, in, policy);
+              }
             }
           }
         }
-      }
-      aw_commit();
-      next += RINGS;
-      entry = next < p1 ? table[next] : 0;
-    };
-    meet();
-#pragma unroll
-    for (int i = 0; i < S::STAGES - 1; i++) fetch(i);
-
-    float o[STEPS][NT][4];  // head values 16 i + lane / 4 (+ 8) of vectors 2 (lane mod 4) (+ 1)
-#pragma unroll
-    for (int i = 0; i < STEPS; i++)
-#pragma unroll
-      for (int nt = 0; nt < NT; nt++) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.f;
-    float m[NT][2], l[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) m[nt][0] = m[nt][1] = -INFINITY, l[nt][0] = l[nt][1] = 0.f;
-    for (int stage = 0; page < p1; page += RINGS) {
-      aw_wait<S::STAGES - 2>();
+        aw_commit();
+        next += RINGS;
+        entry = next < p1 ? table[next] : 0;
+      };
       meet();
-      const bool ok = pages_ok >> (S::STAGES - 2) & 1;
-      const int ahead = stage + S::STAGES - 1;
-      fetch(ahead >= S::STAGES ? ahead - S::STAGES : ahead);
-      const uint32_t kp = ring_at + stage * 2 * S::PAGE, vp = kp + S::PAGE;
-      const char* v_page = ring + stage * 2 * S::PAGE + S::PAGE;
-      // slots lane / 4 (c0, c1) and + 8 (c2, c3) of vectors 2 (lane mod 4) and the next; even and odd steps apart, two
-      // shorter chains of products
-      float s[NT][4], s_odd[NT][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; nt++)
+      for (int i = 0; i < S::STAGES - 1; i++) fetch(i);
+
+      float o[STEPS][NT][4];  // head values 16 i + lane / 4 (+ 8) of vectors 2 (lane mod 4) (+ 1)
 #pragma unroll
-        for (int e = 0; e < 4; e++) s[nt][e] = s_odd[nt][e] = 0.f;
+      for (int i = 0; i < STEPS; i++)
 #pragma unroll
-      for (int st = 0; st < STEPS; st++) {
-        uint32_t ka[4];
-        aw_ldsm(ka, kp + k_off + st * 32);
+        for (int nt = 0; nt < NT; nt++) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.f;
+      float m[NT][2], l[NT][2];
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-          Ty::mma(st & 1 ? s_odd[nt] : s[nt], ka, qf[st][nt][0], qf[st][nt][1]);
-        }
-      }
-      const int j0 = page * 16 + lane / 4;  // this lane's slots: j0, j0 + 8
-#pragma unroll
-      for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) s[nt][e] = (s[nt][e] + s_odd[nt][e]) * scale2;
-      const bool whole = page * 16 + 15 <= all_last && page * 16 >= all_from && page * 16 + 16 <= q.n && ok;
-      if (!whole) {
+      for (int nt = 0; nt < NT; nt++) m[nt][0] = m[nt][1] = -INFINITY, l[nt][0] = l[nt][1] = 0.f;
+      for (int stage = 0; page < p1; page += RINGS) {
+        aw_wait<S::STAGES - 2>();
+        meet();
+        const bool ok = pages_ok >> (S::STAGES - 2) & 1;
+        const int ahead = stage + S::STAGES - 1;
+        fetch(ahead >= S::STAGES ? ahead - S::STAGES : ahead);
+        const uint32_t kp = ring_at + stage * 2 * S::PAGE, vp = kp + S::PAGE;
+        const char* v_page = ring + stage * 2 * S::PAGE + S::PAGE;
+        // slots lane / 4 (c0, c1) and + 8 (c2, c3) of vectors 2 (lane mod 4) and the next; even and odd steps apart, two
+        // shorter chains of products
+        float s[NT][4], s_odd[NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const int j = j0 + (e >> 1) * 8;
-            if (!ok || j > last[nt][e & 1] || j < from[nt][e & 1] || j >= q.n) s[nt][e] = -INFINITY;
+          for (int e = 0; e < 4; e++) s[nt][e] = s_odd[nt][e] = 0.f;
+#pragma unroll
+        for (int st = 0; st < STEPS; st++) {
+          uint32_t ka[4];
+          aw_ldsm(ka, kp + k_off + st * 32);
+#pragma unroll
+          for (int nt = 0; nt < NT; nt++) {
+            Ty::mma(st & 1 ? s_odd[nt] : s[nt], ka, qf[st][nt][0], qf[st][nt][1]);
           }
-      }
-      // the largest of each vector's scores: every step for all vectors, so that their shuffles overlap
-      float top[NT][2];
-#pragma unroll
-      for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-        for (int e = 0; e < 2; e++) top[nt][e] = fmaxf(s[nt][e], s[nt][e + 2]);
-#pragma unroll
-      for (int x = 4; x < 32; x <<= 1)
+        }
+        const int j0 = page * 16 + lane / 4;  // this lane's slots: j0, j0 + 8
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-          for (int e = 0; e < 2; e++)
-            top[nt][e] = fmaxf(top[nt][e], __shfl_xor_sync(0xffffffffu, top[nt][e], x));
-      // a vector's base follows its maximum when that is AW_SLACK and more above it: weights of up to 2^AW_SLACK lose
-      // nothing, and most pages leave the accumulators alone. Each vector decides for itself, whatever its neighbours
-      bool more = false;
-      float f[NT][2];
+          for (int e = 0; e < 4; e++) s[nt][e] = (s[nt][e] + s_odd[nt][e]) * scale2;
+        const bool whole = page * 16 + 15 <= all_last && page * 16 >= all_from && page * 16 + 16 <= q.n && ok;
+        if (!whole) {
 #pragma unroll
-      for (int nt = 0; nt < NT; nt++)
+          for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
-          const float base = top[nt][e] - Ty::SHIFT;
-          f[nt][e] = 1.f;
-          if (base > m[nt][e] + AW_SLACK) {
-            f[nt][e] = aw_exp2(m[nt][e] - base);
-            m[nt][e] = base;
-            more = true;
-          }
+            for (int e = 0; e < 4; e++) {
+              const int j = j0 + (e >> 1) * 8;
+              if (!ok || j > last[nt][e & 1] || j < from[nt][e & 1] || j >= q.n) s[nt][e] = -INFINITY;
+            }
         }
-      if (__any_sync(0xffffffffu, more)) {
+        // the largest of each vector's scores: every step for all vectors, so that their shuffles overlap
+        float top[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+          for (int e = 0; e < 2; e++) top[nt][e] = fmaxf(s[nt][e], s[nt][e + 2]);
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1)
+#pragma unroll
+          for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+              top[nt][e] = fmaxf(top[nt][e], __shfl_xor_sync(0xffffffffu, top[nt][e], x));
+        // a vector's base follows its maximum when that is AW_SLACK and more above it: weights of up to 2^AW_SLACK lose
+        // nothing, and most pages leave the accumulators alone. Each vector decides for itself, whatever its neighbours
+        bool more = false;
+        float f[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
           for (int e = 0; e < 2; e++) {
-            l[nt][e] *= f[nt][e];
-#pragma unroll
-            for (int i = 0; i < STEPS; i++) o[i][nt][e] *= f[nt][e], o[i][nt][e + 2] *= f[nt][e];
+            const float base = top[nt][e] - Ty::SHIFT;
+            f[nt][e] = 1.f;
+            if (base > m[nt][e] + AW_SLACK) {
+              f[nt][e] = aw_exp2(m[nt][e] - base);
+              m[nt][e] = base;
+              more = true;
+            }
           }
-      }
-#pragma unroll
-      for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-        for (int e = 0; e < 2; e++)
-          if (live[nt][e]) {
-            float* to = ONE ? s_scores + ((part * NT + nt) * 8 + lane % 4 * 2 + e) * held + page * 16 - split * a.kps + lane / 4
-                            : scores + (long long)(nt * 8 + e) * a.kv_pad + page * 16;
-            to[0] = s[nt][e];
-            to[8] = s[nt][e + 2];
-          }
-#pragma unroll
-      for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const float base = m[nt][e & 1] == -INFINITY ? 0.f : m[nt][e & 1];
-          s[nt][e] = aw_exp2(s[nt][e] - base);
-          l[nt][e & 1] += s[nt][e];
-        }
-      bool by_mma = true;
-      if (!whole && (a.max_rows > 1 || a.window > 0)) {  // a row may be blind to a slot of this page that holds anything
-        bool fine = true;
-#pragma unroll 4
-        for (int c = lane; c < 16 * CP; c += 32) {
-          const uint4 x = *(const uint4*)(v_page + c / CP * S::PITCH + c % CP * 16);
-          fine = fine && Ty::finite(x.x) && Ty::finite(x.y) && Ty::finite(x.z) && Ty::finite(x.w);
-        }
-        by_mma = __all_sync(0xffffffffu, fine);
-      }
-      if (by_mma) {
-        uint32_t hi[NT][2], rest[NT][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-          for (int i = 0; i < 2; i++) {
-            const uint2 x = Ty::parts(s[nt][2 * i], s[nt][2 * i + 1]);
-            hi[nt][i] = aw_turn(x.x), rest[nt][i] = aw_turn(x.y);
-          }
-#pragma unroll
-        for (int st = 0; st < STEPS; st++) {
-          uint32_t va[4];
-          aw_ldsm_t(va, vp + v_off + st * 32);
-#pragma unroll
-          for (int nt = 0; nt < NT; nt++) Ty::mma(o[st][nt], va, hi[nt][0], hi[nt][1]);
-#pragma unroll
-          for (int nt = 0; nt < NT; nt++) Ty::mma(o[st][nt], va, rest[nt][0], rest[nt][1]);
-        }
-      } else {
-#pragma unroll 1
-        for (int kk = 0; kk < 16; kk++) {
-          const int src = (kk & 7) * 4 + lane % 4, j = page * 16 + kk;
+        if (__any_sync(0xffffffffu, more)) {
 #pragma unroll
           for (int nt = 0; nt < NT; nt++)
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-              const float p = __shfl_sync(0xffffffffu, kk < 8 ? s[nt][e] : s[nt][e + 2], src);
-              if (j > last[nt][e] || j < from[nt][e] || j >= q.n) continue;
+              l[nt][e] *= f[nt][e];
 #pragma unroll
-              for (int i = 0; i < STEPS; i++) {
-                const T* v = (const T*)(v_page + kk * S::PITCH) + i * 16 + lane / 4;
-                o[i][nt][e] = fmaf(p, Ty::up(v[0]), o[i][nt][e]);
-                o[i][nt][e + 2] = fmaf(p, Ty::up(v[8]), o[i][nt][e + 2]);
-              }
+              for (int i = 0; i < STEPS; i++) o[i][nt][e] *= f[nt][e], o[i][nt][e + 2] *= f[nt][e];
             }
         }
-      }
-      __syncwarp();
-      stage = stage + 1 == S::STAGES ? 0 : stage + 1;
-    }
-    aw_wait<0>();
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++)
+        for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-      for (int e = 0; e < 2; e++) {
+          for (int e = 0; e < 2; e++)
+            if (live[nt][e]) {
+              float* to = ONE ? s_scores + ((part * NT + nt) * 8 + lane % 4 * 2 + e) * held + page * 16 - split * a.kps + lane / 4
+                              : scores + (long long)(nt * 8 + e) * a.kv_pad + page * 16;
+              to[0] = s[nt][e];
+              to[8] = s[nt][e + 2];
+            }
 #pragma unroll
-        for (int x = 4; x < 32; x <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], x);
-        const int row = (part * NT + nt) * 8 + lane * 2 + e;
-        if (lane < 4) s_m[worker][row] = m[nt][e], s_l[worker][row] = l[nt][e];
-        if (ONE && worker == 0 && lane < 4) s_sees[row] = make_int2(from[nt][e], last[nt][e]);
-      }
-    __syncthreads();  // every warp is done with its ring, which now takes its accumulator
+        for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-      for (int e = 0; e < 2; e++) {
-        const int row = (part * NT + nt) * 8 + lane % 4 * 2 + e;
-        float top = s_m[0][row];
-#pragma unroll
-        for (int w = 1; w < RINGS; w++) top = fmaxf(top, s_m[w][row]);
-        const float f = m[nt][e] == -INFINITY ? 0.f : aw_exp2(m[nt][e] - top);
-        float* to = (float*)ring + row * S::JOIN + lane / 4;
-        if (live[nt][e]) {
-#pragma unroll
-          for (int i = 0; i < STEPS; i++) to[i * 16] = o[i][nt][e] * f, to[i * 16 + 8] = o[i][nt][e + 2] * f;
+          for (int e = 0; e < 4; e++) {
+            const float base = m[nt][e & 1] == -INFINITY ? 0.f : m[nt][e & 1];
+            s[nt][e] = aw_exp2(s[nt][e] - base);
+            l[nt][e & 1] += s[nt][e];
+          }
+        bool by_mma = true;
+        if (again || (!whole && (a.max_rows > 1 || a.window > 0))) {  // a row may be blind to a slot that holds anything
+          bool fine = true;
+#pragma unroll 4
+          for (int c = lane; c < 16 * CP; c += 32) {
+            const uint4 x = *(const uint4*)(v_page + c / CP * S::PITCH + c % CP * 16);
+            fine = fine && Ty::finite(x.x) && Ty::finite(x.y) && Ty::finite(x.z) && Ty::finite(x.w);
+          }
+          by_mma = __all_sync(0xffffffffu, fine);
         }
-      }
-    __syncthreads();
-    const long long at = (((long long)b * a.hkv + h) * a.splits + split) * a.vecs + tile * TILE;
-    const int count = min(TILE, vecs - tile * TILE);
-    for (int row = warp; row < count; row += WARPS)
-      for (int c = lane * 4; c < a.d; c += 128) {
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (by_mma) {
+          uint32_t hi[NT][2], rest[NT][2];
 #pragma unroll
-        for (int w = 0; w < RINGS; w++) {
-          const float4 y = *(const float4*)(smem + w * S::RING + (row * S::JOIN + c) * 4);
-          x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+          for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+              const uint2 x = Ty::parts(s[nt][2 * i], s[nt][2 * i + 1]);
+              hi[nt][i] = aw_turn(x.x), rest[nt][i] = aw_turn(x.y);
+            }
+#pragma unroll
+          for (int st = 0; st < STEPS; st++) {
+            uint32_t va[4];
+            aw_ldsm_t(va, vp + v_off + st * 32);
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) Ty::mma(o[st][nt], va, hi[nt][0], hi[nt][1]);
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) Ty::mma(o[st][nt], va, rest[nt][0], rest[nt][1]);
+          }
+        } else {
+#pragma unroll 1
+          for (int kk = 0; kk < 16; kk++) {
+            const int src = (kk & 7) * 4 + lane % 4, j = page * 16 + kk;
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+              for (int e = 0; e < 2; e++) {
+                const float p = __shfl_sync(0xffffffffu, kk < 8 ? s[nt][e] : s[nt][e + 2], src);
+                if (j > last[nt][e] || j < from[nt][e] || j >= q.n) continue;
+#pragma unroll
+                for (int i = 0; i < STEPS; i++) {
+                  const T* v = (const T*)(v_page + kk * S::PITCH) + i * 16 + lane / 4;
+                  o[i][nt][e] = fmaf(p, Ty::up(v[0]), o[i][nt][e]);
+                  o[i][nt][e + 2] = fmaf(p, Ty::up(v[8]), o[i][nt][e + 2]);
+                }
+              }
+          }
         }
-        if (ONE) *(float4*)(s_out + row * S::JOIN + c) = x;
-        else *(float4*)(a.parts + (at + row) * a.d + c) = x;
+        __syncwarp();
+        stage = stage + 1 == S::STAGES ? 0 : stage + 1;
       }
-    if (t < count) {
-      float mm = s_m[0][t];
+      aw_wait<0>();
 #pragma unroll
-      for (int w = 1; w < RINGS; w++) mm = fmaxf(mm, s_m[w][t]);
-      float sum = 0.f;
+      for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-      for (int w = 0; w < RINGS; w++) sum += s_l[w][t] == 0.f ? 0.f : aw_exp2(s_m[w][t] - mm) * s_l[w][t];  // 0: no slot
-      if (ONE) s_stat[t] = make_float2(mm, sum);
-      else a.stats[at + t] = make_float2(mm, sum);
-    }
-    if constexpr (ONE) {
+        for (int e = 0; e < 2; e++) {
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], x);
+          const int row = (part * NT + nt) * 8 + lane * 2 + e;
+          if (lane < 4) s_m[worker][row] = m[nt][e], s_l[worker][row] = l[nt][e];
+          if (ONE && worker == 0 && lane < 4) s_sees[row] = make_int2(from[nt][e], last[nt][e]);
+        }
+      __syncthreads();  // every warp is done with its ring, which now takes its accumulator
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          const int row = (part * NT + nt) * 8 + lane % 4 * 2 + e;
+          float top = s_m[0][row];
+#pragma unroll
+          for (int w = 1; w < RINGS; w++) top = fmaxf(top, s_m[w][row]);
+          const float f = m[nt][e] == -INFINITY ? 0.f : aw_exp2(m[nt][e] - top);
+          float* to = (float*)ring + row * S::JOIN + lane / 4;
+          if (live[nt][e]) {
+#pragma unroll
+            for (int i = 0; i < STEPS; i++) to[i * 16] = o[i][nt][e] * f, to[i * 16 + 8] = o[i][nt][e + 2] * f;
+          }
+        }
+      __syncthreads();
+      const long long at = (((long long)b * a.hkv + h) * a.splits + split) * a.vecs + tile * TILE;
+      bool odd = false;
+      for (int row = warp; row < count; row += WARPS)
+        for (int c = lane * 4; c < a.d; c += 128) {
+          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int w = 0; w < RINGS; w++) {
+            const float4 y = *(const float4*)(smem + w * S::RING + (row * S::JOIN + c) * 4);
+            x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+          }
+          if (x.x != x.x || x.y != x.y || x.z != x.z || x.w != x.w) {
+            float sums = 0.f;
+#pragma unroll
+            for (int w = 0; w < RINGS; w++) sums += s_l[w][row];
+            odd = odd || sums == sums;
+          }
+          if (ONE) *(float4*)(s_out + row * S::JOIN + c) = x;
+          else *(float4*)(a.parts + (at + row) * a.d + c) = x;
+        }
+      if (t < count) {
+        float mm = s_m[0][t];
+#pragma unroll
+        for (int w = 1; w < RINGS; w++) mm = fmaxf(mm, s_m[w][t]);
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < RINGS; w++) sum += s_l[w][t] == 0.f ? 0.f : aw_exp2(s_m[w][t] - mm) * s_l[w][t];  // 0: no slot
+        if (ONE) s_stat[t] = make_float2(mm, sum);
+        else a.stats[at + t] = make_float2(mm, sum);
+      }
+      return __syncthreads_or(odd);  // the ring is the copies' again
+    };
+    if constexpr (ONE) {  // two copies: with a loop the only split's pages take 0.7 us longer (3500 slots and more)
+      if (run(std::false_type())) {
+        if (a.d < DP) clear();
+        run(std::true_type());
+      }
       cg::cluster_group cluster = cg::this_cluster();
       const int ranks = gridDim.x;
       // this block's slots and their weights so far, on their way while the blocks meet
@@ -648,7 +667,7 @@ __global__ void __launch_bounds__(AwShape<DP, NT, WPP>::WARPS * 32, AwShape<DP, 
       cluster.sync();  // nobody leaves while its accumulators are read
       return;
     }
-    __syncthreads();  // the ring is the copies' again
+    redo = run(redo) && !redo;
     if (a.d < DP) clear();
   }
 }

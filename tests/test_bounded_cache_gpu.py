@@ -483,6 +483,27 @@ def test_attention_weights_of_keys_that_are_nan(cuda, dtype, lengths, rows, kps,
     assert bool(((out.double() - want).abs() <= tol)[fine].all())
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lengths,rows,hq,d,window,kps", [([100], [1], 8, 64, 0, 0), ([100], [5], 8, 80, 0, 0), ([3000], [1], 8, 128, 0, 64),
+                                                          ([3000, 200], [5, 1], 8, 256, 0, 0), ([700], [9], 14, 96, 0, 0),
+                                                          ([2000], [3], 8, 128, 1990, 0), ([400], [2], 16, 192, 0, 0)])
+def test_attention_weights_of_values_that_are_infinite(cuda, dtype, lengths, rows, hq, d, window, kps):
+    """Under a positive weight they are infinite, with their sign; of both signs they are NaN; nothing else is."""
+    q, k, v, table, bounds, slot, weights = attend_case(cuda, 35, lengths, rows, hq, 2, d, dtype)
+    for j, at, bad in ((5 + 30, 3, INF), (20 + 30, 4, -INF), (21 + 30, 5, INF), (40 + 30, 5, -INF), (41 + 30, d - 1, NAN)):
+        v[int(table[0, j // 16]), :, j % 16, at] = bad
+    want, after, tol, w_tol = attend_plain(q, k, v, table, bounds, slot, weights, d ** -0.5, window)
+    kw = {"max_rows_per_seq": max(rows), "max_kv_len": table.shape[1] * 16, "scale": d ** -0.5, "window": window,
+          "keys_per_split": kps}
+    out = kernels.attention_weights(q, k, v, table, bounds, slot, got := weights.clone(), **kw).double()
+    fine = want.isfinite()
+    assert torch.equal(out.isnan(), want.isnan()) and torch.equal(out[want.isinf()], want[want.isinf()])
+    assert not bool(fine.all()) and bool(((out - want).abs() <= tol)[fine].all())
+    plain = torch.where(v.isfinite(), v, 0.0)
+    kernels.attention_weights(q, k, plain, table, bounds, slot, same := weights.clone(), **kw)
+    assert torch.equal(got, same)
+
+
 def test_attention_weights_of_large_scores_and_equal_ones(cuda):
     case = attend_case(cuda, 21, [500, 64], [1, 4], 8, 2, 128, torch.bfloat16, spread=8.0)
     attend_check(case, scale=1.0)  # scores in the hundreds: one slot has nearly all the weight
