@@ -487,7 +487,8 @@ size_t im_kq_workspace_bytes(int64_t K, int64_t B);
  * im_cache_evict: of the n = lengths[s] slots of every (layer, sequence, kv head), min(n, budget) stay: those whose
  * position (slot_pos) is below `sinks` or at least seen[s] - recent, then the heaviest (weights; NaN lightest), lower
  * slots first among equals. The i-th kept slot behind the new end moves to the i-th dropped slot before it: K, V (a slot's
- * row_bytes of one head; any type), weight and position. weights_out and pos_out (which may be weights and slot_pos) get
+ * row_bytes of one head; any type), weight and position; where either's page is outside the cache nothing moves, and the
+ * hole keeps its token. weights_out and pos_out (which may be weights and slot_pos) get
  * the slots before the new end, lengths_out [S] (may be lengths, not seen) the new length, the same for every layer and head. weights and
  * slot_pos are [layers][S][Hkv][cap], the caches `layers` times [pages][Hkv][16][row_bytes], layer_bytes apart; n is at
  * most min(cap, 16 max_pages), cap at most 262144 and row_bytes 65536. Sequences must not share the pages of a cache that is cut. sinks + recent <= budget.

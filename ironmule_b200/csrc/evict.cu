@@ -97,9 +97,13 @@ __device__ __forceinline__ void ev_move(const EvictArgs& a, long long row, const
   long long dst = 0, src = -1;
   if (lane < moves) {
     const long long to_page = table[to / 16], from_page = table[from / 16];
-    a.weights_out[row * a.cap + to] = a.weights[row * a.cap + from];
-    a.pos_out[row * a.cap + to] = a.pos[row * a.cap + from];
-    if (to_page >= 0 && to_page < a.pages && from_page >= 0 && from_page < a.pages) {
+    const bool on = to_page >= 0 && to_page < a.pages && from_page >= 0 && from_page < a.pages;
+    // a slot whose page is none of the cache's neither moves nor is moved to: the hole keeps its token, so that position and
+    // weight stay those of what the slot holds
+    const int at = on ? from : to;
+    a.weights_out[row * a.cap + to] = a.weights[row * a.cap + at];
+    a.pos_out[row * a.cap + to] = a.pos[row * a.cap + at];
+    if (on) {
       dst = layer + ((to_page * a.hkv + head) * 16 + to % 16) * a.row_bytes;
       src = layer + ((from_page * a.hkv + head) * 16 + from % 16) * a.row_bytes;
     }

@@ -638,6 +638,43 @@ def test_evict_lengths_beyond_the_tables(cuda):
     assert got.tolist() == [20, 0, 20]
 
 
+@pytest.mark.parametrize("in_place", [True, False])
+@pytest.mark.parametrize("length,budget", [(100, 40), (3000, 1000), (3000, 2990)])
+def test_evict_over_pages_that_are_none(cuda, in_place, length, budget):
+    """A slot whose page lies outside the cache neither moves nor is moved to: every slot of the cache holds the token that
+    slot_pos names, with its weight."""
+    g = gen(cuda, 3)
+    table, pages = page_table(g, 2, length)
+    cap = table.shape[1] * 16
+    pos = torch.stack([torch.randperm(cap, generator=g, device=cuda) for _ in range(4)]).to(torch.int32).view(2, 2, cap)
+    k = torch.zeros((pages, 2, 16, 8), device=cuda)
+    for s in range(2):
+        rows = pos[s].view(2, -1, 16).transpose(0, 1).float()
+        k[table[s].long()] = rows[..., None].expand(-1, -1, -1, 8)
+    v = k + 0.5
+    heavy = torch.rand((2, 2, cap), generator=g, device=cuda)  # a token's weight, by head
+    weights = torch.gather(heavy, 2, pos.long())
+    bad = table.clone()
+    for s, page in ((0, 1), (0, table.shape[1] - 1), (1, 0), (1, table.shape[1] - 2)):
+        bad[s, page] = -1 if page else 10**6
+    wo = weights if in_place else torch.full_like(weights, -3.0)
+    po = pos if in_place else torch.full_like(pos, -3)
+    was = pos.clone()
+    left = kernels.cache_evict(k, v, bad, ints([length, length], cuda), ints([cap, cap], cuda), weights, pos, budget=budget,
+                               weights_out=None if in_place else wo, pos_out=None if in_place else po)
+    assert left.tolist() == [budget] * 2
+    now = po[:, :, :budget]
+    assert torch.equal(wo[:, :, :budget], torch.gather(heavy, 2, now.long()))
+    moved = 0
+    for s in range(2):
+        held = k[table[s].long()].transpose(0, 1).flatten(1, 2)[:, :budget]
+        on = ((bad[s] >= 0) & (bad[s] < pages)).repeat_interleave(16)[:budget]
+        assert torch.equal(held[:, on], now[s][:, on, None].float().expand(-1, -1, 8))
+        assert torch.equal(now[s][:, ~on], was[s][:, :budget][:, ~on])
+        moved += int((now[s] != was[s][:, :budget]).sum())
+    assert moved > 0 and torch.equal(v, k + 0.5)
+
+
 def test_evict_protects_more_than_the_budget_has_room_for(cuda):
     """Positions that repeat (no program's) protect more slots than stay: the lower slots win."""
     k, v, table, lengths, seen, weights, pos = evict_case(cuda, 6, [60], 1, 1, 32, torch.bfloat16)
