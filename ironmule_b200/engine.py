@@ -1114,12 +1114,12 @@ def greedy_decode(model: QuantModel, prompt: torch.Tensor, max_new: int, seq: in
 
 
 class BoundedDecoder:
-    """Greedy decoding over a cache that does not grow: every kv head of every layer keeps at most `budget` slots when the
-    cache is cut, which happens whenever the next tokens would pass model.max_ctx slots. Kept are the first `sinks` tokens, the
-    last `recent`, and the tokens with the most attention so far (kernels.attention_weights adds it up, prompt included;
-    kernels.cache_evict cuts). A text may so be longer than the cache; a token's position is not its slot. Until the first
-    cut this is plain decoding; behind it the answers are the cut cache's. Not for models with a sliding window, whose
-    layers go by slots, nor over pages that sequences share."""
+    """Greedy decoding over a cache that does not grow: every kv head of every layer keeps at most `budget` slots when a
+    sequence's cache is cut, which happens whenever its next tokens would pass model.max_ctx slots. Kept are the first `sinks`
+    tokens, the last `recent`, and the tokens with the most attention so far (kernels.attention_weights adds it up, prompt
+    included; kernels.cache_evict cuts). A text may so be longer than the cache; a token's position is not its slot. Until
+    its first cut a sequence is decoded plainly; behind it the answers are the cut cache's, whatever the other slots hold. Not
+    for models with a sliding window, whose layers go by slots, nor over pages that sequences share."""
 
     def __init__(self, model: QuantModel, budget: int, *, recent: int | None = None, sinks: int = 4):
         recent = budget // 4 if recent is None else recent
@@ -1143,20 +1143,32 @@ class BoundedDecoder:
 
     def start(self, seq: int = 0) -> None:
         """Forget the sequence of a slot."""
+        self._check(seq)
+        self._set(seq, 0, 0)
+
+    def _check(self, seq: int) -> None:
         if not 0 <= seq < self.model.max_seqs:
             raise ValueError(f"sequence {seq} of {self.model.max_seqs}")
-        self._set(seq, 0, 0)
 
     def _set(self, seq: int, held: int, seen: int) -> None:
         self._held[seq], self._seen[seq] = held, seen
         self.lengths[seq], self.seen[seq] = held, seen
 
-    def cut(self) -> None:
-        """Cut every sequence slot's cache to the budget, in one call for all layers."""
+    def cut(self, seq: int | None = None) -> None:
+        """Cut a sequence slot's cache to the budget (every slot's by default), in one call for all layers."""
         m = self.model
-        kernels.cache_evict(m.k_cache, m.v_cache, m.page_table, self.lengths, self.seen, self.weights, self.slot_pos,
-                            budget=self.budget, recent=self.recent, sinks=self.sinks, lengths_out=self.lengths)
-        self._held = [min(n, self.budget) for n in self._held]
+        lengths = self.lengths
+        if seq is not None:
+            self._check(seq)
+            if any(n > self.budget for b, n in enumerate(self._held) if b != seq):  # others that a cut would change
+                lengths = torch.zeros_like(self.lengths)
+                lengths[seq] = self._held[seq]
+        left = kernels.cache_evict(m.k_cache, m.v_cache, m.page_table, lengths, self.seen, self.weights, self.slot_pos,
+                                   budget=self.budget, recent=self.recent, sinks=self.sinks, lengths_out=lengths)
+        for b in range(len(self._held)) if seq is None else (seq,):
+            self._held[b] = min(self._held[b], self.budget)
+        if left is not self.lengths:
+            self.lengths[seq] = self._held[seq]
         self.cuts += 1
 
     def feed(self, tokens: torch.Tensor, seq: int = 0, logits: bool = False) -> torch.Tensor | None:
@@ -1164,8 +1176,7 @@ class BoundedDecoder:
         m = self.model
         if logits and not tokens.numel():
             raise ValueError("logits of no token")
-        if not 0 <= seq < m.max_seqs:
-            raise ValueError(f"sequence {seq} of {m.max_seqs}")
+        self._check(seq)
         step = self.step
         last = tokens.numel() - 1 if logits else tokens.numel()  # a token whose logits are wanted goes by itself
         ends = [*range(step, last, step), last] if last else []
@@ -1174,7 +1185,7 @@ class BoundedDecoder:
             part = tokens[at:end].to(torch.int32).contiguous()
             n = end - at
             if self._held[seq] + n > m.max_ctx:
-                self.cut()
+                self.cut(seq)
             held, seen = self._held[seq], self._seen[seq]
             meta = m._meta(part, list(range(seen, seen + n)), seq)
             meta.slot = torch.arange(held, held + n, dtype=torch.int32, device=m.device)

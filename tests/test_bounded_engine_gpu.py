@@ -58,6 +58,30 @@ def test_a_cut_cache_holds_the_keys_of_the_tokens_it_names(cuda):
     assert dec.cuts >= 4
 
 
+def test_a_cut_is_its_sequences(cuda):
+    """A sequence's tokens stay when another's cache is cut, over the budget or not, and its logits keep their bits."""
+    text, other = tokens(cuda, 130, seed=5), tokens(cuda, 300, seed=6)
+    kw = {"recent": 16, "sinks": 4}
+    both, alone = (engine.BoundedDecoder(model(cuda, 128, max_seqs=3), 64, **kw) for _ in range(2))
+    for dec in (both, alone):
+        dec.feed(text[:100], seq=1)
+        dec.feed(text[:20], seq=2)
+    both.feed(other, seq=0)
+    assert both.cuts >= 3 and both.lengths.tolist() == [both._held[0], 100, 20] and both._held[1:] == [100, 20]
+    for seq, done in ((1, 100), (2, 20)):
+        for dec in (both, alone):
+            assert dec._held[seq] == done
+        for t in ("weights", "slot_pos"):
+            assert torch.equal(getattr(both, t)[:, seq, :, :done], getattr(alone, t)[:, seq, :, :done])
+        assert torch.equal(both.feed(text[done:done + 9], seq, logits=True), alone.feed(text[done:done + 9], seq, logits=True))
+    both.feed(text[109:], seq=1)  # and its own cut does come
+    alone.feed(text[109:], seq=1)
+    assert both._held[1] == alone._held[1] < 128 and torch.equal(both.slot_pos[:, 1], alone.slot_pos[:, 1])
+    assert alone.cuts == 1 and both.seen.tolist() == [300, 130, 29]
+    both.cut()
+    assert both._held == both.lengths.tolist() == [64, 64, 29]
+
+
 def test_generate_runs_past_the_cache_and_starts_afresh(cuda):
     m = model(cuda, 96)
     dec = engine.BoundedDecoder(m, 48, recent=12, sinks=2)
