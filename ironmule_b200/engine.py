@@ -1119,7 +1119,8 @@ class BoundedDecoder:
     tokens, the last `recent`, and the tokens with the most attention so far (kernels.attention_weights adds it up, prompt
     included; kernels.cache_evict cuts). A text may so be longer than the cache; a token's position is not its slot. Until
     its first cut a sequence is decoded plainly; behind it the answers are the cut cache's, whatever the other slots hold. Not
-    for models with a sliding window, whose layers go by slots, nor over pages that sequences share."""
+    for models with a sliding window, whose layers go by slots, nor over pages that sequences share (a sequence's first
+    tokens are refused then)."""
 
     def __init__(self, model: QuantModel, budget: int, *, recent: int | None = None, sinks: int = 4):
         recent = budget // 4 if recent is None else recent
@@ -1150,6 +1151,13 @@ class BoundedDecoder:
         if not 0 <= seq < self.model.max_seqs:
             raise ValueError(f"sequence {seq} of {self.model.max_seqs}")
 
+    def _own_pages(self, seq: int) -> None:
+        """Refuse a slot whose pages are another's too: a cut moves slots within them."""
+        table = self.model.page_table
+        mine, others = table[seq], torch.cat([table[:seq], table[seq + 1:]]).flatten()
+        if mine.unique().numel() < mine.numel() or bool(torch.isin(mine, others).any()):
+            raise ValueError(f"sequence {seq} does not have its pages to itself")
+
     def _set(self, seq: int, held: int, seen: int) -> None:
         self._held[seq], self._seen[seq] = held, seen
         self.lengths[seq], self.seen[seq] = held, seen
@@ -1177,6 +1185,8 @@ class BoundedDecoder:
         if logits and not tokens.numel():
             raise ValueError("logits of no token")
         self._check(seq)
+        if tokens.numel() and not self._held[seq]:
+            self._own_pages(seq)
         step = self.step
         last = tokens.numel() - 1 if logits else tokens.numel()  # a token whose logits are wanted goes by itself
         ends = [*range(step, last, step), last] if last else []

@@ -82,6 +82,21 @@ def test_a_cut_is_its_sequences(cuda):
     assert both._held == both.lengths.tolist() == [64, 64, 29]
 
 
+def test_a_sequence_has_its_pages_to_itself(cuda):
+    m = model(cuda, 96, max_seqs=2)
+    dec = engine.BoundedDecoder(m, 32)
+    dec.feed(tokens(cuda, 5))
+    m.page_table[1, 2] = m.page_table[0, 1]
+    for seq in (0, 1):
+        dec.start(seq)
+        with pytest.raises(ValueError, match="pages to itself"):
+            dec.feed(tokens(cuda, 5), seq=seq)
+    m.page_table[1, 2] = m.page_table[1, 3]
+    dec.feed(tokens(cuda, 5))
+    with pytest.raises(ValueError, match="pages to itself"):
+        dec.generate(tokens(cuda, 5), 2, seq=1)
+
+
 def test_generate_runs_past_the_cache_and_starts_afresh(cuda):
     m = model(cuda, 96)
     dec = engine.BoundedDecoder(m, 48, recent=12, sinks=2)
