@@ -502,7 +502,8 @@ size_t im_kq_workspace_bytes(int64_t K, int64_t B);
  * nothing is left), after the last draft from target: the smallest token whose cumulative weight exceeds u_K times
  * the total, u = uniforms[b * uniforms_ld ..][K + 1], in [0, 1). Products, differences and sums are float64. Values that
  * are not positive finite numbers count as 0; a row without any weight gives token 0; a draft outside [0, V) is refused.
- * out_tokens [B, K + 1] (kept drafts, the drawn token, then -1), out_count [B] (kept + 1).
+ * out_tokens [B, K + 1] (kept drafts, the drawn token, then -1), out_count [B] (kept + 1). They may lie over what only the
+ * same sequence reads (out_count over n_drafts, say), but not over drafts that begin before out_tokens.
  */
 enum { IM_BF16 = 0, IM_F16 = 1, IM_F32 = 2 };
 enum { IM_ROPE_HALF = 0, IM_ROPE_INTERLEAVED = 1 };

@@ -1143,6 +1143,20 @@ def _check_probs(t: torch.Tensor, name: str, rows: int, index: int | None) -> in
     return ld
 
 
+def _check_verified(tokens: torch.Tensor | None, count: torch.Tensor | None, drafts: torch.Tensor, uniforms: torch.Tensor,
+                    n_drafts: torch.Tensor | None) -> None:
+    """Refuse outputs that lie over inputs of another sequence, which may still be read. A sequence's own are read by then,
+    but for drafts, which are copied upwards."""
+    if tokens is not None and count is not None:
+        _disjoint_or_same(tokens, "tokens", count, "count")
+    for out, name in ((tokens, "tokens"), (count, "count")):
+        if out is None:
+            continue
+        for t, what in ((drafts, "drafts"), (uniforms, "uniforms"), (n_drafts, "n_drafts")):
+            if t is not None and (drafts.shape[0] > 1 or (t is drafts and out.data_ptr() > t.data_ptr())):
+                _disjoint_or_same(out, name, t, what)
+
+
 def verify_sampled(target_probs: torch.Tensor, draft_probs: torch.Tensor | None, drafts: torch.Tensor,
                    uniforms: torch.Tensor, *, n_drafts: torch.Tensor | None = None, tokens: torch.Tensor | None = None,
                    count: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
@@ -1179,6 +1193,8 @@ def verify_sampled(target_probs: torch.Tensor, draft_probs: torch.Tensor | None,
             _need(t, name, torch.int32, device, index)
             if t.shape != shape:
                 raise ValueError(f"{name} must be {list(shape)}, got {tuple(t.shape)}")
+    if tokens is not None or count is not None:
+        _check_verified(tokens, count, drafts, uniforms, n_drafts)
     tokens = drafts.new_empty(b, k + 1) if tokens is None else tokens
     count = drafts.new_empty(b) if count is None else count
     if b:

@@ -806,6 +806,31 @@ def test_verify_sampled_of_what_is_no_distribution(cuda):
     verify_check(one((NAN, 0.5, 0.5), (INF, 0.1, 0.3)), one((0.1, INF, 0.2)), d, u)
 
 
+def test_verify_sampled_outputs_over_inputs(cuda):
+    """A sequence's count may take the place of its n_drafts, and its tokens that of its random numbers; one sequence's
+    drafts may lie in the buffer that takes its tokens. What another sequence still reads is refused."""
+    p, q, drafts, u = verify_case(cuda, 15, 40, 3, 5000, torch.float32)
+    n = torch.randint(0, 4, (40,), generator=gen(cuda, 2), device=cuda, dtype=torch.int32)
+    tokens, count = kernels.verify_sampled(p, q, drafts, u, n_drafts=n)
+    own, over = n.clone(), u.clone()
+    got = kernels.verify_sampled(p, q, drafts, over, n_drafts=own, tokens=over.view(torch.int32), count=own)
+    assert torch.equal(got[0], tokens) and torch.equal(got[1], count) and got[1] is own
+    for b in range(3):
+        buffer = torch.cat([drafts[b, :1], drafts[b]]).view(1, 4)
+        got = kernels.verify_sampled(p[b:b + 1], q[b:b + 1], buffer[:, 1:], u[b:b + 1], n_drafts=n[b:b + 1], tokens=buffer)
+        assert torch.equal(got[0], tokens[b:b + 1]) and torch.equal(got[1], count[b:b + 1])
+    flat = torch.zeros(400, dtype=torch.int32, device=cuda)
+    held = flat[:120].view(40, 3).copy_(drafts)
+    for kw, word in (({"tokens": flat[:160].view(40, 4)}, "drafts"), ({"count": flat[100:140]}, "drafts"),
+                     ({"tokens": flat[200:360].view(40, 4), "count": flat[350:390]}, "count"),
+                     ({"tokens": flat[200:360].view(40, 4), "n_drafts": flat[359:399].copy_(n)}, "n_drafts")):
+        with pytest.raises(ValueError, match=word):
+            kernels.verify_sampled(p, q, held, u, **{"n_drafts": n, **kw})
+    with pytest.raises(ValueError, match="drafts"):  # upwards within one sequence
+        kernels.verify_sampled(p[:1], q[:1], flat[:3].view(1, 3), u[:1], tokens=flat[1:5].view(1, 4))
+    assert torch.equal(held, drafts)
+
+
 def test_verify_sampled_takes_wider_rows(cuda):
     p, q, drafts, u = verify_case(cuda, 5, 3, 2, 100, torch.float32)
     wide = torch.full((9, 133), NAN, device=cuda)
