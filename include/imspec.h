@@ -465,7 +465,7 @@ size_t im_kq_workspace_bytes(int64_t K, int64_t B);
  * im_rope: out[m, h] = x[m, h] turned to position pos[m] (int32, or int64 with pos_64; of any size, also negative). Pair i
  * of the first `rotary` values turns by pos * inv_freq[i] (float32, or float64 with freq_f64; rotary / 2 of them) and is
  * multiplied by `factor`; pairs are (i, i + rotary / 2) (IM_ROPE_HALF) or (2 i, 2 i + 1) (IM_ROPE_INTERLEAVED), the other
- * values are copied. The angle is a float64 product. inverse turns back, by the transpose: the gradient of x from
+ * values are copied. The angle is a float64 product, within 2^-51 of itself: far positions lose that much. inverse turns back, by the transpose: the gradient of x from
  * that of out, and, with factor 1, the way back. x and out have their own strides (in values; a head's values are
  * contiguous); out may be x itself with the same strides, and must not overlap it otherwise.
  *
@@ -479,7 +479,8 @@ size_t im_kq_workspace_bytes(int64_t K, int64_t B);
  *                          of their softmax weight on slot j,  for j < min(largest row_slot + 1, max_kv_len, cap),
  * f being the slot of the sequence's first row that has one (row_slot >= 0): slots that this call is the first to see start
  * from zero. Other weights are left alone. weights_out may be weights, out may be q. Rows that see no slot (row_slot -1, say) get zeros and add nothing. Splits:
- * multiples of keys_per_split (a multiple of 64; 0: chosen by the sizes of the call); keep it fixed and a row's bits do
+ * multiples of keys_per_split (a multiple of 64; 0: chosen by the sizes of the call for the least time of a call from Python;
+ * more than 16 splits always take two kernels, which can be faster in a captured graph); keep it fixed and a row's bits do
  * not depend on the launch. The workspace holds 4 bytes a (row, query head, slot). seq_rows is clamped to the M rows of q; rows beyond max_rows_per_seq are not computed. No two
  * sequences may name one table row. Workspace 256-byte aligned, nothing to initialise;
  * calls of few, short splits need none (0 bytes).

@@ -3,8 +3,9 @@
 // A pair (a, b) of frequency f at position p turns by t = p f: a' = c a - s b, b' = s a + c b with c = factor cos t,
 // s = factor sin t. Pairs are (i, i + R/2) (half) or (2i, 2i + 1) (interleaved) of a head's first R values; the rest is
 // copied. The angle is a float64 product reduced to a quarter turn before it is rounded to float32: at position 10^6 a
-// float32 product would be off by 0.06 rad. What is left of it is within 2^-26 quarter turns, so c and s are float32
-// exact to an ulp or two wherever the position is. Rotations are float32, rounded once to the rows' type.
+// float32 product would be off by 0.06 rad. The product and 2 / pi are rounded, within 2^-51 of the angle together, and what is
+// left of a turn within 2^-26 quarter turns: up to angles of 2^25 rad c and s are float32 exact to an ulp or two, beyond
+// that they lose what the float64 angle has lost (2^-11 rad at 2^40). Rotations are float32, rounded once to the rows' type.
 //
 // Bound: HBM, every value read and written once. A warp takes a part of a row's heads, for itself: it works the row's c and
 // s out (R/2 of them, two or so a lane), hands them over in shared memory of its own, and walks the heads; a lane keeps to

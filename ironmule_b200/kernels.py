@@ -884,7 +884,8 @@ def rope(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, la
     """x [M, H, D] (bf16, float16 or float32; any row and head strides) turned to positions [M] (int32 or int64): pair i
     of a head's first 2 * len(inv_freq) values by positions * inv_freq[i], times factor; the rest is copied. Pairs are
     (i, i + half of them) or, "interleaved", (2i, 2i + 1). inverse turns back by the transpose: rope(dy, ..., inverse=True)
-    is the gradient of x. `out` may be x; a new tensor by default."""
+    is the gradient of x, which autograd does not take by itself. An angle is a float64 product, within 2^-51 of itself.
+    `out` may be x; a new tensor by default."""
     kind = _TYPES.get(x.dtype) if isinstance(x, torch.Tensor) and x.is_cuda else None
     if kind is None:
         raise TypeError("x must be a bf16, float16 or float32 CUDA tensor")
@@ -1003,8 +1004,10 @@ def attention_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     adds up each slot's attention weight: weights (float32 [sequences, Hkv, cap], the rows of the page table) becomes, in
     place or in weights_out, weights + the softmax weights that the sequence's rows and the kv head's query heads put on
     the slot, for the slots up to the last row's; from the slot of the first row that has one on it starts from zero. Rows
-    without a slot (-1) get zeros and add nothing. `out` may be q. The other arguments
-    are `attention`'s, keys_per_split 0 meaning that the call's sizes choose it."""
+    without a slot (-1) get zeros and add nothing. `out` may be q. No two sequences may name one table row. The other arguments
+    are `attention`'s, keys_per_split 0 meaning that the call's sizes choose it, for the least time of a call from Python: in a
+    captured graph a length that makes more than 16 splits can be faster (one row of 32/8 heads over 5000 slots 11.6 us
+    with two kernels, 13.7 with the one that is chosen)."""
     dtype = torch.float16 if isinstance(q, torch.Tensor) and q.dtype is torch.float16 else torch.bfloat16
     if not (isinstance(q, torch.Tensor) and q.is_cuda and q.dtype is dtype and q.is_contiguous()):
         _check(q, "q", (torch.bfloat16, torch.float16))

@@ -402,6 +402,14 @@ def test_attention_weights_of_rows_padded_in_front(cuda, lengths, rows, in_place
         assert bool((after[b, :, :n - rows[b]] >= weights[b, :, :n - rows[b]]).all())
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lengths,rows,hq,hkv,d,window", [([300], [256], 8, 1, 64, 0), ([2100, 5], [2048, 5], 1, 1, 80, 0),
+                                                          ([700, 300], [256, 100], 16, 2, 128, 0), ([600], [512], 4, 1, 256, 100)])
+def test_attention_weights_of_prompt_pieces(cuda, dtype, lengths, rows, hq, hkv, d, window):
+    """Up to 2048 vectors a kv head."""
+    attend_check(attend_case(cuda, 36, lengths, rows, hq, hkv, d, dtype), window=window)
+
+
 def test_attention_weights_over_its_own_queries(cuda):
     for length in (100, 5000):
         case = attend_case(cuda, 7, [length, 33], [3, 2], 8, 2, 128, torch.bfloat16)
