@@ -15,7 +15,7 @@
 // block's up to 16384 slots, and that block moves its slots too where they are few; else the pairs go through the workspace
 // to a second kernel that spreads them over the device. Longer rows are a cluster's of up to 16 blocks, which share counts
 // through distributed shared memory. 288 rows of 8192 slots of 2 x 256 bytes cut to 2048 take 102 us: 20 of selection, bound by
-// instructions, and 80 of moves at 5.7 TB/s; 288 rows of 2064 cut by 16 slots 13.8 us.
+// instructions, and 80 of moves at 5.8 TB/s; 288 rows of 2064 cut by 16 slots 13.8 us.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
